@@ -15,6 +15,7 @@
 #include "attn/sla.h"
 #include "comm/comm.h"
 #include "moe/moe.h"
+#include "kvcache/kvcache.h"
 #include "vae/conv3d.h"
 #include "vae/groupnorm.h"
 
@@ -1397,6 +1398,135 @@ void ep_copy_rows(c10::optional<torch::Tensor> src_table, int64_t src_ptr,
   ddb::ep_copy_rows(a, stream());
 }
 
+// ---------------------------------------------------------------- 8-bit paged key/value cache
+// Codes [L, P, heads, 64, 64] of one byte and fp32 scales [L, P, heads] of a cache; the
+// pointers of one layer of it.
+ddb::KvPool kv_pool(const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& ks,
+                    const torch::Tensor& vs, int64_t layer) {
+  for (const auto* t : {&k, &v}) {
+    check_cuda_tensor(*t, "cache codes");
+    TORCH_CHECK(t->scalar_type() == torch::kFloat8_e4m3fn && t->is_contiguous() && t->dim() == 5 &&
+                    t->size(3) == ddb::kKvPage && t->size(4) == 64 && t->sizes() == k.sizes(),
+                "cache codes must be contiguous float8_e4m3fn [layers, pages, heads, 64, 64]");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "cache codes must be 16-byte aligned");
+    TORCH_CHECK(t->device() == k.device(), "the cache's tensors must be on one device");
+  }
+  for (const auto* t : {&ks, &vs})
+    TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->is_contiguous() && t->dim() == 3 &&
+                    t->size(0) == k.size(0) && t->size(1) == k.size(1) && t->size(2) == k.size(2) &&
+                    t->device() == k.device(),
+                "cache scales must be contiguous float32 [layers, pages, heads]");
+  TORCH_CHECK(layer >= 0 && layer < k.size(0), "layer ", layer, " of a cache of ", k.size(0));
+  TORCH_CHECK(k.size(1) <= 0x7fffffff && k.size(2) <= 65535, "cache too large");
+  ddb::KvPool p;
+  const int64_t blocks = layer * k.size(1) * k.size(2);
+  p.k = reinterpret_cast<uint8_t*>(k.data_ptr()) + blocks * 4096;
+  p.v = reinterpret_cast<uint8_t*>(v.data_ptr()) + blocks * 4096;
+  p.k_scale = ks.data_ptr<float>() + blocks;
+  p.v_scale = vs.data_ptr<float>() + blocks;
+  p.pages = k.size(1);
+  p.heads = k.size(2);
+  return p;
+}
+
+ddb::KvStep kv_step(const torch::Tensor& rows, const torch::Tensor& k) {
+  TORCH_CHECK(rows.scalar_type() == torch::kInt32 && rows.is_contiguous() && rows.dim() == 2 &&
+                  rows.size(1) > ddb::kKvInfo && rows.device() == k.device(),
+              "a step's table must be contiguous int32 [sequences, 4 + pages] on the cache's device");
+  TORCH_CHECK(rows.size(0) <= 65535, "at most 65535 sequences in a step");
+  ddb::KvStep s;
+  s.rows = rows.data_ptr<int>();
+  s.ld = rows.size(1);
+  s.width = rows.size(1) - ddb::kKvInfo;
+  s.B = rows.size(0);
+  return s;
+}
+
+// [B, T, H, 64] bf16 whose channels are contiguous and whose rows are 16-byte aligned
+void check_tokens(const torch::Tensor& t, const char* name, const torch::Tensor& k, int64_t B) {
+  check_bf16(t, name);
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == B && t.size(3) == 64, name, " must be [", B, ", T, heads, 64]");
+  TORCH_CHECK(t.device() == k.device(), name, " must be on the cache's device");
+  TORCH_CHECK(t.numel() == 0 || (t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+                                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
+              name, " must have contiguous channels and 16-byte aligned rows");
+}
+
+void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs, int64_t layer,
+                    torch::Tensor rows, torch::Tensor new_k, torch::Tensor new_v) {
+  ddb::KvWriteArgs a;
+  a.pool = kv_pool(k, v, ks, vs, layer);
+  a.step = kv_step(rows, k);
+  check_tokens(new_k, "keys", k, a.step.B);
+  check_tokens(new_v, "values", k, a.step.B);
+  TORCH_CHECK(new_k.sizes() == new_v.sizes() && new_k.size(2) == a.pool.heads, "keys and values must be [B, T, ",
+              a.pool.heads, ", 64]");
+  const c10::cuda::CUDAGuard guard(k.device());
+  a.k = new_k.data_ptr();
+  a.k_sb = new_k.stride(0); a.k_st = new_k.stride(1); a.k_sh = new_k.stride(2);
+  a.v = new_v.data_ptr();
+  a.v_sb = new_v.stride(0); a.v_st = new_v.stride(1); a.v_sh = new_v.stride(2);
+  a.T = new_k.size(1);
+  ddb::kv_cache_write(a, stream());
+}
+
+void kv_cache_attend(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs, int64_t layer,
+                     torch::Tensor rows, torch::Tensor q, torch::Tensor o, c10::optional<torch::Tensor> lse,
+                     bool causal, int64_t unit, int64_t window, int64_t sinks, double scale,
+                     int64_t max_tokens) {
+  ddb::KvAttendArgs a;
+  a.pool = kv_pool(k, v, ks, vs, layer);
+  a.step = kv_step(rows, k);
+  check_tokens(q, "queries", k, a.step.B);
+  TORCH_CHECK(a.pool.heads > 0 && q.size(2) % a.pool.heads == 0, "query heads must be a multiple of the cache's ", a.pool.heads);
+  check_bf16(o, "o");
+  TORCH_CHECK(o.is_contiguous() && o.sizes() == q.sizes() && o.device() == k.device() &&
+                  reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0, "o must be contiguous and like q");
+  TORCH_CHECK(unit >= 1 && unit <= (1 << 24) && window >= 0 && window <= (1 << 24) && sinks >= 0 && sinks <= (1 << 30) &&
+                  unit * window <= (1 << 30),
+              "kv_cache_attend: unit, window or sinks out of range");
+  TORCH_CHECK(q.size(1) * (q.size(2) / a.pool.heads) <= (1 << 30), "kv_cache_attend: too many query rows");
+  const c10::cuda::CUDAGuard guard(k.device());
+  a.q = q.data_ptr();
+  a.q_sb = q.stride(0); a.q_st = q.stride(1); a.q_sh = q.stride(2);
+  a.o = o.data_ptr();
+  if (lse) {
+    TORCH_CHECK(lse->scalar_type() == torch::kFloat32 && lse->is_contiguous() && lse->device() == k.device() &&
+                    lse->numel() == q.size(0) * q.size(1) * q.size(2), "lse must be contiguous fp32 [B, H, T]");
+    a.lse = lse->data_ptr<float>();
+  }
+  a.T = q.size(1);
+  a.H = q.size(2);
+  a.causal = causal;
+  a.unit = unit;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = static_cast<float>(scale);
+  a.max_tokens = max_tokens;
+  ddb::kv_cache_attend(a, stream());
+}
+
+void kv_cache_copy_pages(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
+                         std::vector<int64_t> src, std::vector<int64_t> dst) {
+  TORCH_CHECK(k.dim() == 5, "cache codes must be [layers, pages, heads, 64, 64]");
+  if (k.size(0) == 0) return;
+  const auto p = kv_pool(k, v, ks, vs, 0);
+  TORCH_CHECK(k.size(0) <= 65535, "cache too large");
+  TORCH_CHECK(src.size() == dst.size(), "as many pages to copy from as to");
+  std::vector<int> s(src.size()), d(dst.size());
+  std::vector<char> is_dst(p.pages, 0);
+  for (size_t i = 0; i < src.size(); ++i) {
+    TORCH_CHECK(src[i] >= 0 && src[i] < p.pages && dst[i] >= 0 && dst[i] < p.pages, "page id out of range");
+    TORCH_CHECK(!is_dst[dst[i]], "page ", dst[i], " is written twice");
+    is_dst[dst[i]] = 1;
+    s[i] = src[i];
+    d[i] = dst[i];
+  }
+  for (const int x : s) TORCH_CHECK(!is_dst[x], "page ", x, " is read and written by one copy");
+  const c10::cuda::CUDAGuard guard(k.device());
+  ddb::kv_cache_copy_pages(p.k, p.v, p.k_scale, p.v_scale, k.size(0), p.pages, p.heads, s.data(), d.data(), s.size(), stream());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1452,6 +1582,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q_pos_offset"), py::arg("kv_pos_offset"), py::arg("scale"), py::arg("kv_qtiles"),
         py::arg("kv_qmask"), py::arg("kv_count"), py::arg("debug_flags") = 0,
         py::arg("trace") = py::none(), py::arg("trace_cta") = 0);
+  m.def("kv_cache_write", &kv_cache_write, "tokens into the pages of an 8-bit key/value cache");
+  m.def("kv_cache_attend", &kv_cache_attend, "attention over an 8-bit paged key/value cache");
+  m.def("kv_cache_copy_pages", &kv_cache_copy_pages, "copy cache pages in every layer");
   m.def("attn_delta", &attn_delta, "rowsum(dO * O) per head");
   m.def("ipc_alloc", &ipc_alloc, "cudaMalloc + IPC handle -> (ptr, handle)");
   m.def("ipc_open", &ipc_open, "open a peer's IPC handle -> ptr");

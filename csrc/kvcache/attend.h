@@ -1,0 +1,15 @@
+// Shared by the cache attention's kernels.
+#pragma once
+#include "kvcache.h"
+
+namespace ddb {
+
+// e of the power of two 2^e that brings a query row's largest magnitude into [2^14, 2^15), in
+// [-120, 113]; 0 for a row of zeros, or one that holds an infinity or a NaN (its output
+// is not finite in any case)
+__device__ __forceinline__ int row_exponent(float amax) {
+  const int k = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+  return amax > 0.f && k < 128 ? max(k - 14, -120) : 0;
+}
+
+}  // namespace ddb

@@ -1,0 +1,538 @@
+"""Paged key/value cache in 8 bits for streaming generation.
+
+A page holds 64 consecutive tokens of one sequence, for every layer and head, as e4m3
+codes with one power-of-two scale for each (layer, page, head), keys and values apart:
+half a bf16 cache's memory and reads. Sequences are lists of pages of one pool, so the
+oldest tokens are dropped by giving pages back (:meth:`PagedKVCache.trim`), one sequence
+becomes several by sharing pages (:meth:`PagedKVCache.fork`), and the pool is packed
+without touching any sequence's contents (:meth:`PagedKVCache.compact`).
+
+Use::
+
+    cache = PagedKVCache(n_layers, n_heads, n_pages, device="cuda")
+    seqs = cache.add(batch)
+    step = cache.begin(seqs, n_new)            # room for n_new tokens of each sequence
+    for layer in range(n_layers):
+        step.write(layer, k, v)                # [B, n_new, n_heads, 64]
+        o = step.attend(layer, q, causal="frame", tokens_per_frame=512, window=36, sinks=4)
+    step.commit()                              # the tokens stay; without it they are redone
+
+What a cached block stands for: ``code * scale``, ``scale = 2^e`` with the smallest ``e``
+for which the block's largest finite magnitude is at most ``448 * 2^e`` (``e`` in
+[-100, 119]), codes rounded to nearest even, infinities saturated, NaN kept. Writing into an
+unfinished page re-codes the tokens it already holds when its scale changes.
+
+CUDA caches run the sm_100a kernels (``csrc/kvcache``); CPU caches the PyTorch statements
+below, which are also the kernels' oracle. Calls run on the current stream. A step may
+be used on another stream than the one it was begun on (its table is waited for); the
+order of writes and reads of the cache itself between streams is the caller's, as for
+any tensor. Bookkeeping is on the host: calls on one cache come from one thread.
+"""
+from __future__ import annotations
+
+import heapq
+import math
+from typing import List, Optional, Sequence, Union
+
+import torch
+
+from ._ext import ext
+
+PAGE = 64       # tokens of a page
+_INFO = 4       # words of a step's row before its page ids
+_MAX_TOKENS = 1 << 30
+
+
+class _Seq:
+    __slots__ = ("pages", "length", "first", "sinks", "version")
+
+    def __init__(self):
+        self.pages: List[int] = []  # ids by page of the sequence; -1: given back
+        self.length = 0             # committed tokens
+        self.first = 0              # tokens in [sinks, first) are gone
+        self.sinks = 0
+        self.version = 0            # a step begun at another version is stale
+
+
+def _two_to(e: torch.Tensor) -> torch.Tensor:
+    """``2^e`` of whole ``e`` in [-126, 127], exactly."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def quantize_block(x: torch.Tensor):
+    """Codes and scales of blocks ``x [..., tokens, channels]`` (fp32): ``(e4m3, fp32 [...])``."""
+    amax = torch.where(x.isfinite(), x, 0.0).abs().amax((-1, -2))
+    mant, exp = torch.frexp(amax)
+    e = torch.where(mant <= 0.875, exp - 9, exp - 8)
+    e = torch.where(amax > 0, e, -100).clamp(-100, 119)
+    y = x * _two_to(-e)[..., None, None]
+    return y.clamp(-448.0, 448.0).to(torch.float8_e4m3fn), _two_to(e)
+
+
+class CacheStep:
+    """Room for new tokens of some sequences (:meth:`PagedKVCache.begin`).
+
+    ``write`` / ``attend`` may run any number of times, for any layers, before ``commit``.
+    Once a sequence of the step has changed otherwise (commit, trim, fork, free, a later
+    ``begin``, compaction) the step is stale and its calls raise."""
+
+    def __init__(self, cache: "PagedKVCache", seqs, n_new, rows, max_tokens):
+        self.cache = cache
+        self.seqs, self.n_new = seqs, n_new
+        self.max_tokens = max_tokens  # launches are shaped for sequences up to this length
+        self.rows = rows              # int32 [B, 4 + max_pages_per_seq]
+        self._states = [cache._seqs[i] for i in seqs]
+        self._versions = [s.version for s in self._states]
+        self._ready = None            # (event, stream) of the rows' upload
+
+    @property
+    def table(self) -> torch.Tensor:
+        """Page ids by sequence, int32 ``[B, max_pages_per_seq]`` (-1: none)."""
+        return self.rows[:, _INFO:]
+
+    def _check(self):
+        if any(s.version != v for s, v in zip(self._states, self._versions)):
+            raise RuntimeError("stale step: a sequence has changed since it was begun; begin a new one")
+        if self._ready is not None and not torch.cuda.is_current_stream_capturing():
+            event, stream = self._ready
+            now = torch.cuda.current_stream(self.rows.device)
+            if now != stream:
+                now.wait_event(event)
+                self.rows.record_stream(now)
+
+    def _tokens(self, x: torch.Tensor, name: str, heads: Optional[int]):
+        c = self.cache
+        if x.dim() != 4 or x.shape[0] != len(self.seqs) or x.shape[3] != 64:
+            raise ValueError(f"{name} must be [{len(self.seqs)}, T, heads, 64], got {tuple(x.shape)}")
+        if heads is not None and x.shape[2] != heads:
+            raise ValueError(f"{name} has {x.shape[2]} heads, the cache {heads}")
+        if x.shape[2] == 0 or x.shape[2] % c.n_heads:
+            raise ValueError(f"{name}'s {x.shape[2]} heads are no multiple of the cache's {c.n_heads}")
+        if x.shape[1] < max(self.n_new, default=0):
+            raise ValueError(f"{name} holds {x.shape[1]} tokens, the step {max(self.n_new)}")
+        if x.device != c.device:
+            raise ValueError(f"{name} is on {x.device}, the cache on {c.device}")
+        if c.device.type == "cuda":
+            if x.dtype != torch.bfloat16:
+                raise ValueError(f"{name} must be bfloat16 on CUDA, got {x.dtype}")
+            # the kernels read 16 bytes at a time from rows of contiguous channels
+            if x.numel() and (x.stride(3) != 1 or any(s % 8 for s in x.stride()[:3]) or x.data_ptr() % 16):
+                x = x.contiguous()
+                if x.data_ptr() % 16:
+                    x = x.clone()
+        return x
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Cache the new tokens' ``k``, ``v`` ``[B, T, n_heads, 64]`` (any strides; sequence
+        ``i`` has the first ``n_new[i]`` rows, the others are not read)."""
+        c = self.cache
+        self._check()
+        c._layer(layer)
+        k, v = self._tokens(k, "k", c.n_heads), self._tokens(v, "v", c.n_heads)
+        if k.shape != v.shape:
+            raise ValueError("k and v differ in shape")
+        if c.device.type == "cuda":
+            ext().kv_cache_write(c.k, c.v, c.k_scale, c.v_scale, layer, self.rows, k, v)
+        else:
+            self._write_torch(layer, k, v)
+
+    def attend(self, layer: int, q: torch.Tensor, causal: str = "frame", tokens_per_frame: int = 1,
+               window: int = 0, sinks: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+        """Attention of the new tokens ``q [B, T, heads, 64]`` over their sequences, the new
+        tokens (written before) among them; ``heads`` is a multiple of the cache's, head
+        ``h`` reading cached head ``h // (heads / n_heads)``.
+
+        ``causal``: "frame" (a query sees its whole frame and earlier ones), "token" or
+        "none". ``window`` (frames, for "token" tokens; 0: no limit) keeps the newest ones
+        visible, the query's own counted, and ``sinks`` the sequence's first ones beside
+        them. Of a trimmed sequence what :meth:`PagedKVCache.trim` kept is visible at most.
+        Returns ``o [B, T, heads, 64]`` (and ``lse [B, heads, T]``, log2 domain); rows
+        behind a sequence's ``n_new`` and rows that see no key are zero (-inf)."""
+        c = self.cache
+        self._check()
+        c._layer(layer)
+        q = self._tokens(q, "q", None)
+        if causal not in ("frame", "token", "none"):
+            raise ValueError(f"causal must be frame, token or none, got {causal!r}")
+        unit = tokens_per_frame if causal == "frame" else 1
+        if unit < 1 or window < 0 or sinks < 0:
+            raise ValueError("tokens_per_frame must be positive, window and sinks not negative")
+        if causal == "none" and (window or sinks):
+            raise ValueError("a window needs causal frame or token")
+        # a window or sinks past every token mean all of them
+        unit = min(unit, 1 << 24)
+        window = window if window * unit < _MAX_TOKENS and window <= 1 << 24 else 0
+        n_sink = min(sinks * unit, _MAX_TOKENS)
+        scale = 1.0 / math.sqrt(64) if scale is None else float(scale)
+        if not (scale > 0 and math.isfinite(scale)):
+            raise ValueError("scale must be positive and finite")
+        for s in self._states:
+            if s.first > s.sinks and s.sinks != n_sink and (window or sinks):
+                raise ValueError(f"a sequence was trimmed to its first {s.sinks} tokens, the call names {n_sink} sinks")
+        if c.device.type != "cuda":
+            return self._attend_torch(layer, q, causal, unit, window, n_sink, scale, return_lse)
+        o = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
+        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device) if return_lse else None
+        ext().kv_cache_attend(c.k, c.v, c.k_scale, c.v_scale, layer, self.rows, q, o, lse, causal != "none",
+                              unit, window, n_sink, scale, self.max_tokens)
+        return (o, lse) if return_lse else o
+
+    def commit(self) -> None:
+        """Keep the step's tokens: its sequences grow by ``n_new``."""
+        self._check()
+        for s, n in zip(self._states, self.n_new):
+            s.length += n
+            s.version += 1
+
+    # ------------------------------------------------------------------ PyTorch form
+    def _write_torch(self, layer, k, v):
+        c = self.cache
+        for i, (s, n) in enumerate(zip(self._states, self.n_new)):
+            for j in range(s.length // PAGE, -(-(s.length + n) // PAGE)) if n else ():
+                lo, hi = max(s.length, j * PAGE), min(s.length + n, (j + 1) * PAGE)
+                kept = max(0, s.length - j * PAGE)
+                for codes, scales, new, last in ((c.k, c.k_scale, k, False), (c.v, c.v_scale, v, True)):
+                    held = codes[layer, s.pages[j]].float() * scales[layer, s.pages[j]][:, None, None]
+                    x = torch.zeros(c.n_heads, PAGE, 64, device=c.device)
+                    x[:, :kept] = (held.mT if last else held)[:, :kept]
+                    x[:, lo - j * PAGE:hi - j * PAGE] = new[i, lo - s.length:hi - s.length].transpose(0, 1).float()
+                    y, sc = quantize_block(x)
+                    codes[layer, s.pages[j]] = y.mT if last else y
+                    scales[layer, s.pages[j]] = sc
+
+    def _attend_torch(self, layer, q, causal, unit, window, n_sink, scale, return_lse):
+        c = self.cache
+        o = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.full((q.shape[0], q.shape[2], q.shape[1]), -math.inf, device=q.device)
+        G = q.shape[2] // c.n_heads
+        for i, (s, n) in enumerate(zip(self._states, self.n_new)):
+            if not n:
+                continue
+            total = s.length + n
+            k, v = c._values(layer, s, total)                                  # [total, heads, 64]
+            k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+            sc = torch.einsum("thd,shd->hts", q[i, :n].float(), k) * scale
+            qf = (torch.arange(s.length, total, device=q.device) // unit)[:, None]
+            pos = torch.arange(total, device=q.device)
+            kf = (pos // unit)[None]
+            seen = kf <= qf if causal != "none" else torch.ones(n, total, dtype=torch.bool, device=q.device)
+            if window:
+                seen = seen & ((kf > qf - window) | (pos < n_sink))
+            if s.first > s.sinks:
+                seen = seen & ((pos >= s.first) | (pos < s.sinks))
+            sc = sc.masked_fill(~seen, -math.inf)
+            ls = torch.logsumexp(sc, -1)
+            p = torch.where(seen, torch.exp(sc - ls[..., None]), 0.0)
+            o[i, :n] = torch.einsum("hts,shd->thd", p, torch.where(seen.any(0)[:, None, None], v, 0.0)).to(q.dtype)
+            lse[i, :, :n] = ls / math.log(2)
+        return (o, lse) if return_lse else o
+
+
+class PagedKVCache:
+    """A pool of ``n_pages`` pages of 64 tokens for ``n_layers`` x ``n_heads`` (cached heads,
+    64 channels each) and the sequences that own them.
+
+    ``k`` / ``v``: float8_e4m3fn ``[layers, pages, heads, 64, 64]``, keys by (token, channel),
+    values by (channel, token); ``k_scale`` / ``v_scale``: float32 ``[layers, pages, heads]``.
+    ``max_pages_per_seq`` bounds a sequence (default: the pool). Free pages are taken in
+    the order of their ids. Every call that does not fit raises before it changes anything."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_pages: int, device=None,
+                 max_pages_per_seq: Optional[int] = None):
+        if n_layers < 1 or n_heads < 1 or n_pages < 1:
+            raise ValueError("layers, heads and pages must be positive")
+        device = torch.device(device if device is not None else ("cuda" if torch.cuda.is_available() else "cpu"))
+        if device.type == "cuda":
+            if device.index is None:
+                device = torch.device("cuda", torch.cuda.current_device())
+            with torch.cuda.device(device):
+                ext().read_status()  # the status word exists before any capture
+        self.device = device
+        self.n_layers, self.n_heads, self.n_pages = n_layers, n_heads, n_pages
+        self.max_pages_per_seq = n_pages if max_pages_per_seq is None else max_pages_per_seq
+        if not 1 <= self.max_pages_per_seq <= _MAX_TOKENS // PAGE:
+            raise ValueError("max_pages_per_seq out of range")
+        self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
+        self._free: List[int] = list(range(n_pages))
+        self._refs = [0] * n_pages
+        self._seqs: dict = {}
+        self._next = 0
+
+    def _pool(self, n):
+        shape = (self.n_layers, n, self.n_heads)
+        codes = [torch.zeros(*shape, PAGE, 64, dtype=torch.uint8, device=self.device).view(torch.float8_e4m3fn) for _ in "kv"]
+        return (*codes, *(torch.ones(*shape, device=self.device) for _ in "kv"))
+
+    # ------------------------------------------------------------------ bookkeeping
+    def _layer(self, layer):
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"layer {layer} of a cache of {self.n_layers}")
+
+    def _get(self, seqs) -> List[_Seq]:
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
+        missing = [i for i in seqs if i not in self._seqs]
+        if missing:
+            raise ValueError(f"no sequence {missing[0]} in this cache")
+        return [self._seqs[i] for i in seqs]
+
+    def _need(self, n):
+        if n > len(self._free):
+            raise RuntimeError(f"out of cache pages: {n} needed, {len(self._free)} of {self.n_pages} free")
+
+    def _take(self) -> int:
+        page = heapq.heappop(self._free)
+        self._refs[page] = 1
+        return page
+
+    def _give(self, page: int):
+        if page < 0:
+            return
+        self._refs[page] -= 1
+        if not self._refs[page]:
+            heapq.heappush(self._free, page)
+
+    def _copy(self, src: Sequence[int], dst: Sequence[int]):
+        if not src:
+            return
+        if self.device.type == "cuda":
+            ext().kv_cache_copy_pages(self.k, self.v, self.k_scale, self.v_scale, list(src), list(dst))
+        else:
+            for t in (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale):
+                t[:, list(dst)] = t[:, list(src)]
+
+    def _not_capturing(self, what):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} changes the cache's tables on the host and cannot be captured")
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    @property
+    def sequences(self) -> List[int]:
+        return list(self._seqs)
+
+    def length(self, seq: int) -> int:
+        """Committed tokens of a sequence (its next position), dropped ones counted."""
+        return self._get([seq])[0].length
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
+
+    def table(self, seqs: Sequence[int]) -> torch.Tensor:
+        """Page ids of the sequences, int32 ``[n, max_pages_per_seq]`` (-1: none)."""
+        return self._upload([s.pages for s in self._get(seqs)], self.max_pages_per_seq)
+
+    def _upload(self, rows, width, out=None):
+        # pinned memory from the caching host allocator: kept until the copy has run
+        t = torch.empty(len(rows), width, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        a = t.numpy()
+        a.fill(-1)
+        for i, r in enumerate(rows):
+            a[i, :len(r)] = r
+        if out is not None:
+            return out.copy_(t, non_blocking=True)
+        return t.to(self.device, non_blocking=True) if self.device.type == "cuda" else t
+
+    # ------------------------------------------------------------------ sequences
+    def add(self, n: int = 1) -> List[int]:
+        """``n`` new empty sequences; returns their ids."""
+        if n < 0:
+            raise ValueError("n must not be negative")
+        ids = list(range(self._next, self._next + n))
+        self._next += n
+        for i in ids:
+            self._seqs[i] = _Seq()
+        return ids
+
+    def begin(self, seqs: Sequence[int], n_new: Union[int, Sequence[int]], max_tokens: Optional[int] = None,
+              out: Optional[CacheStep] = None) -> CacheStep:
+        """Make room for ``n_new`` tokens (one number, or one for each sequence) behind each
+        sequence's committed ones. A shared unfinished page that they go into is copied first.
+
+        ``max_tokens``: the longest sequence (its new tokens counted) that the step's launches
+        are shaped for, for steps whose calls are captured into a graph; default: the
+        longest of now. ``out``: a step of as many sequences to refill in place, so that
+        a graph captured with it runs on the new tables; its ``max_tokens`` must suffice."""
+        self._not_capturing("begin")
+        states = self._get(seqs)
+        n_new = [int(n_new)] * len(states) if not isinstance(n_new, (list, tuple)) else [int(n) for n in n_new]
+        if len(n_new) != len(states) or any(n < 0 for n in n_new):
+            raise ValueError("n_new must be one number, or one for each sequence, none negative")
+        longest = max((s.length + n for s, n in zip(states, n_new)), default=0)
+        if longest > self.max_pages_per_seq * PAGE:
+            raise ValueError(f"{longest} tokens do not fit a sequence's {self.max_pages_per_seq} pages")
+        if out is not None:
+            if out.cache is not self or len(out.seqs) != len(states):
+                raise ValueError("out is a step of another cache or number of sequences")
+            max_tokens = out.max_tokens if max_tokens is None else max_tokens
+            if max_tokens != out.max_tokens:
+                raise ValueError("out keeps its max_tokens")
+        max_tokens = longest if max_tokens is None else int(max_tokens)
+        if max_tokens < longest:
+            raise ValueError(f"sequences of {longest} tokens in a step for {max_tokens}")
+        # pages to take: behind the present ones, and for a shared page that gets new tokens.
+        # Of pages shared within this call the last one to write keeps the page.
+        need, left = 0, {}
+        for s, n in zip(states, n_new):
+            have = -(-s.length // PAGE)
+            need += max(0, -(-(s.length + n) // PAGE) - len(s.pages))
+            for j in range(s.length // PAGE, min(-(-(s.length + n) // PAGE), len(s.pages))) if n else ():
+                p = s.pages[j]
+                left[p] = left.get(p, self._refs[p]) - 1
+                need += left[p] > 0
+            need -= max(0, len(s.pages) - max(have, -(-(s.length + n) // PAGE)))
+        self._need(need)
+        moves = []
+        for s, n in zip(states, n_new):
+            upto = -(-(s.length + n) // PAGE)
+            while len(s.pages) > upto:  # room of an abandoned step
+                self._give(s.pages.pop())
+        for s, n in zip(states, n_new):
+            upto = -(-(s.length + n) // PAGE)
+            for j in range(s.length // PAGE, upto) if n else ():
+                if j < len(s.pages):
+                    p = s.pages[j]
+                    if self._refs[p] > 1:
+                        s.pages[j] = self._take()
+                        if j * PAGE < s.length:
+                            moves.append((p, s.pages[j]))
+                        self._give(p)
+                else:
+                    s.pages.append(self._take())
+            s.version += 1
+        self._copy([a for a, _ in moves], [b for _, b in moves])
+        W = self.max_pages_per_seq
+        rows = [[s.length + n, n, *((s.first, s.sinks) if s.first > s.sinks else (0, -1))] + s.pages
+                for s, n in zip(states, n_new)]
+        rows = self._upload(rows, _INFO + W, None if out is None else out.rows)
+        if out is None:
+            step = CacheStep(self, list(seqs), n_new, rows, max_tokens)
+        else:
+            step = out
+            out.__init__(self, list(seqs), n_new, rows, max_tokens)
+        if self.device.type == "cuda":
+            stream = torch.cuda.current_stream(self.device)
+            event = torch.cuda.Event()
+            event.record(stream)
+            step._ready = (event, stream)
+        return step
+
+    def fork(self, seqs: Sequence[int], copies: int = 1) -> List[int]:
+        """``copies`` new sequences from each of ``seqs`` (all copies of the first, then of the
+        next), sharing its pages; an unfinished page is copied when one of them is written."""
+        states = self._get(seqs)
+        if copies < 0:
+            raise ValueError("copies must not be negative")
+        out = []
+        for s in states:
+            s.version += 1
+            n = -(-s.length // PAGE)
+            for i in self.add(copies):
+                t = self._seqs[i]
+                t.pages, t.length, t.first, t.sinks = s.pages[:n], s.length, s.first, s.sinks
+                for p in t.pages:
+                    if p >= 0:
+                        self._refs[p] += 1
+                out.append(i)
+        return out
+
+    def copy(self, seqs: Sequence[int]) -> List[int]:
+        """New sequences with the committed tokens of ``seqs`` in pages of their own."""
+        self._not_capturing("copy")
+        states = self._get(seqs)
+        kept = [s.pages[:-(-s.length // PAGE)] for s in states]
+        self._need(sum(p >= 0 for ps in kept for p in ps))
+        out, moves = self.add(len(states)), []
+        for i, s, ps in zip(out, states, kept):
+            t = self._seqs[i]
+            t.length, t.first, t.sinks = s.length, s.first, s.sinks
+            t.pages = [self._take() if p >= 0 else -1 for p in ps]
+            moves += [(a, b) for a, b in zip(ps, t.pages) if a >= 0]
+        self._copy([a for a, _ in moves], [b for _, b in moves])
+        return out
+
+    def free(self, seqs: Sequence[int]) -> None:
+        """Drop sequences; pages that no other sequence shares become free."""
+        for i, s in zip(list(seqs), self._get(seqs)):
+            for p in s.pages:
+                self._give(p)
+            s.version += 1
+            del self._seqs[i]
+
+    def trim(self, seqs: Sequence[int], keep: int, sinks: int = 0) -> None:
+        """Drop each sequence's tokens but its first ``sinks`` and its newest ``keep`` ones:
+        no query sees them any more, and pages that held nothing else become free."""
+        states = self._get(seqs)
+        if keep < 0 or sinks < 0:
+            raise ValueError("keep and sinks must not be negative")
+        if any(s.first > s.sinks and s.sinks != sinks for s in states):
+            raise ValueError("a sequence that was trimmed keeps its number of sinks")
+        for s in states:
+            first = max(s.first, s.length - keep)
+            if first <= sinks:
+                continue
+            s.first, s.sinks = first, sinks
+            for j in range(-(-sinks // PAGE), min(first // PAGE, len(s.pages))):
+                self._give(s.pages[j])
+                s.pages[j] = -1
+            s.version += 1
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool; returns how many there are."""
+        self._not_capturing("compact")
+        used = [p for p in range(self.n_pages) if self._refs[p]]
+        n = len(used)
+        src = [p for p in used if p >= n]
+        dst = [p for p in range(n) if not self._refs[p]]
+        if src:
+            self._copy(src, dst)
+            to = dict(zip(src, dst))
+            for s in self._seqs.values():
+                if any(p in to for p in s.pages):
+                    s.pages = [to.get(p, p) for p in s.pages]
+                    s.version += 1
+            for a, b in to.items():
+                self._refs[b], self._refs[a] = self._refs[a], 0
+            self._free = list(range(n, self.n_pages))
+        return n
+
+    def resize(self, n_pages: int) -> None:
+        """Change the pool to ``n_pages`` pages (compacted first when it shrinks below a page
+        in use); the pages in use keep their contents."""
+        self._not_capturing("resize")
+        used = sum(r > 0 for r in self._refs)
+        if n_pages < max(used, 1):
+            raise ValueError(f"{used} pages are in use, {n_pages} asked for")
+        if any(self._refs[n_pages:]):
+            self.compact()
+        old, n = (self.k, self.v, self.k_scale, self.v_scale), min(n_pages, self.n_pages)
+        self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
+        for a, b in zip((self.k, self.v, self.k_scale, self.v_scale), old):
+            a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
+            a[:, :n].copy_(b[:, :n])
+        self._refs = self._refs[:n] + [0] * (n_pages - n)
+        self._free = [p for p in range(n_pages) if not self._refs[p]]
+        self.n_pages = n_pages
+        for s in self._seqs.values():
+            s.version += 1
+
+    def _values(self, layer, s: _Seq, n: int):
+        ids = torch.tensor([max(p, 0) for p in s.pages[:-(-n // PAGE)]], dtype=torch.long, device=self.device)
+        out = []
+        for codes, scales, last in ((self.k, self.k_scale, False), (self.v, self.v_scale, True)):
+            x = codes[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float() * scales[layer, ids][..., None, None]
+            x = (x.mT if last else x).transpose(1, 2).reshape(-1, self.n_heads, 64)[:n]
+            if s.first > s.sinks:
+                x = x.clone()
+                x[s.sinks:s.first] = 0
+            out.append(x)
+        return out
+
+    def read(self, layer: int, seq: int):
+        """The committed keys and values of a sequence as they are held, fp32
+        ``[length, n_heads, 64]`` each (dropped tokens zero)."""
+        self._layer(layer)
+        s = self._get([seq])[0]
+        return tuple(self._values(layer, s, s.length))
