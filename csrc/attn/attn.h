@@ -48,7 +48,21 @@ struct AttnArgs {
   int kv_splits = 1;
   float* o_part = nullptr;
   float* lse_part = nullptr;
+  // windowed mode (attn_window_fwd / attn_window_bwd): a query of frame f sees the keys of
+  // frames f - window + 1 .. f (window 0: every frame up to f) and the first sink_tokens
+  // positions. q, k, v (and dout) are [B, rows, H, 64] with the element strides below, any
+  // row count; keys past S and queries past Tq are never read. o, dk, dv and dq_acc are
+  // contiguous; lse and delta rows have a stride of lse_ld >= Tq (backward: whole tiles of 128).
+  int window = 0;
+  int sink_tokens = 0;
+  long lse_ld = 0;
+  long q_sb = 0, q_st = 0, q_sh = 0;
+  long k_sb = 0, k_st = 0, k_sh = 0;
+  long v_sb = 0, v_st = 0, v_sh = 0;
 };
+
+void attn_window_fwd(const AttnArgs& a, cudaStream_t s);
+int attn_window_kv_splits(const AttnArgs& a);  // as attn_fwd_kv_splits, for attn_window_fwd
 
 void attn_fwd(const AttnArgs& a, cudaStream_t s);
 // key-range splits attn_fwd would use for `a` on this device (1: no scratch needed) and
@@ -80,17 +94,19 @@ struct AttnBwdArgs {
   const int* kv_count = nullptr;
   int max_q = 0;
   int debug_flags = 0;        // bit 0: skip the dQ reductions (timing experiments only)
+  long do_sb = 0, do_st = 0, do_sh = 0;  // windowed mode: strides of dout
   long long* trace = nullptr; // optional per-role clock64 trace of CTA `trace_cta`
   int trace_cta = 0;
 };
 
 void attn_bwd(const AttnBwdArgs& a, cudaStream_t s);
+void attn_window_bwd(const AttnBwdArgs& a, cudaStream_t s);
 void attn_bwd_with_status(const AttnBwdArgs& a, int* status, cudaStream_t s);
 
 // delta[b,h,t] = sum_d dO * O over each head's 64 columns
 void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long lddo,
                     int do_col, float* delta, int B, int H, int Tq, long rows_per_b,
-                    cudaStream_t s);
+                    cudaStream_t s, long delta_ld = 0);  // 0: Tq floats between delta rows
 // dq (bf16, optionally rotated back by a rotary table) from the fp32 accumulator
 void attn_dq_finalize(const float* dq_acc, long ld_acc, void* dq, long lddq, int dq_col,
                       int rows, int H, const float2* rope_tab, int rows_per_seq,

@@ -35,6 +35,7 @@
 #include "../common/ptx.cuh"
 #include "../common/tma.h"
 #include "attn.h"
+#include "window.cuh"
 
 namespace ddb {
 namespace {
@@ -77,6 +78,9 @@ __device__ __forceinline__ int first_query_seeing(const AttnArgs& a, int k) {
       g.trace[((role) * 8 + (ev)) * 64 + (j)] = clock64();                          \
   } while (0)
 
+// WIN: the windowed mode (any number of queries and keys, strided heads), instantiated
+// apart so that the other masks' code is unchanged.
+template <bool WIN>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
@@ -118,7 +122,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool sparse = g.kv_count != nullptr;
   const long list_idx = static_cast<long>(bh) * n_kvtiles + kt;
   int nq, qt_first = 0;
-  if (sparse) {
+  if constexpr (WIN) {
+    // the tile's keys are seen from its first key's first query on, up to the last query
+    // of its last key, or to the end if it holds a sink (the first key is one then)
+    const WindowQueries first = window_queries(a, k0), last = window_queries(a, min(k0 + 127, a.S - 1));
+    const int q_end = max(first.hi, last.hi);
+    qt_first = first.lo / 128;
+    nq = first.lo < q_end ? (q_end + 127) / 128 - qt_first : 0;
+  } else if (sparse) {
     nq = min(g.kv_count[list_idx], g.max_q);
   } else {
     const int fq = max(0, first_query_seeing(a, k0));
@@ -184,10 +195,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tmDO);
       const int krow = static_cast<int>(b * a.kv_rows_per_b) + k0;
       mbar_arrive_expect_tx(kv_full, 2 * TILE);
-      tma_load_2d(smem + OFF_K, &tmK, kv_full, a.k_col + h * 64, krow);
-      tma_load_2d(smem + OFF_K + 8192, &tmK, kv_full, a.k_col + h * 64, krow + 64);
-      tma_load_2d(smem + OFF_V, &tmV, kv_full, a.v_col + h * 64, krow);
-      tma_load_2d(smem + OFF_V + 8192, &tmV, kv_full, a.v_col + h * 64, krow + 64);
+      if constexpr (WIN) {
+        tma_load_4d(smem + OFF_K, &tmK, kv_full, 0, h, k0, b);
+        tma_load_4d(smem + OFF_K + 8192, &tmK, kv_full, 0, h, k0 + 64, b);
+        tma_load_4d(smem + OFF_V, &tmV, kv_full, 0, h, k0, b);
+        tma_load_4d(smem + OFF_V + 8192, &tmV, kv_full, 0, h, k0 + 64, b);
+      } else {
+        tma_load_2d(smem + OFF_K, &tmK, kv_full, a.k_col + h * 64, krow);
+        tma_load_2d(smem + OFF_K + 8192, &tmK, kv_full, a.k_col + h * 64, krow + 64);
+        tma_load_2d(smem + OFF_V, &tmV, kv_full, a.v_col + h * 64, krow);
+        tma_load_2d(smem + OFF_V + 8192, &tmV, kv_full, a.v_col + h * 64, krow + 64);
+      }
       bool ok = true;
       int issued = 0;
       for (int j = 0; j < nq; ++j) {
@@ -204,13 +222,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* sd = smem + OFF_DO + s * TILE;
         uint8_t* sv = smem + OFF_VEC + s * 1024;
         // lse / delta of the two blocks: 64 floats (256 bytes, 16-byte aligned) each
-        const long va = static_cast<long>(bh) * a.Tq + qa * 64;
-        const long vb = static_cast<long>(bh) * a.Tq + qb * 64;
+        const long va = static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + qa * 64;
+        const long vb = static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + qb * 64;
         mbar_arrive_expect_tx(&qd_full[s], 2 * TILE + 1024);
-        tma_load_2d(sq, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qa * 64);
-        tma_load_2d(sq + 8192, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qb * 64);
-        tma_load_2d(sd, &tmDO, &qd_full[s], g.do_col + h * 64, rowb + qa * 64);
-        tma_load_2d(sd + 8192, &tmDO, &qd_full[s], g.do_col + h * 64, rowb + qb * 64);
+        if constexpr (WIN) {
+          tma_load_4d(sq, &tmQ, &qd_full[s], 0, h, qa * 64, b);
+          tma_load_4d(sq + 8192, &tmQ, &qd_full[s], 0, h, qb * 64, b);
+          tma_load_4d(sd, &tmDO, &qd_full[s], 0, h, qa * 64, b);
+          tma_load_4d(sd + 8192, &tmDO, &qd_full[s], 0, h, qb * 64, b);
+        } else {
+          tma_load_2d(sq, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qa * 64);
+          tma_load_2d(sq + 8192, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qb * 64);
+          tma_load_2d(sd, &tmDO, &qd_full[s], g.do_col + h * 64, rowb + qa * 64);
+          tma_load_2d(sd + 8192, &tmDO, &qd_full[s], g.do_col + h * 64, rowb + qb * 64);
+        }
         bulk_load(sv, a.lse + va, 256, &qd_full[s]);
         bulk_load(sv + 256, a.lse + vb, 256, &qd_full[s]);
         bulk_load(sv + 512, g.delta + va, 256, &qd_full[s]);
@@ -329,9 +354,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t swz = r & 7;
     // this key is visible to every query q >= qmin (masks are monotone in the query);
     // keys past the sequence end are visible to none
-    const int qmin = (key < a.S) ? (sparse ? 0 : first_query_seeing(a, key)) : (1 << 30);
+    int qmin = (key < a.S) ? (sparse ? 0 : first_query_seeing(a, key)) : (1 << 30);
+    int qmax = 0;  // windowed mode: and by every query below qmax
     bool ok = true;
-    for (int j = 0; j < nq; ++j) {
+    if constexpr (WIN) {
+      const WindowQueries w = key < a.S ? window_queries(a, key) : WindowQueries{0, 0};
+      qmin = w.lo, qmax = w.hi;
+      // a key that no query sees stays out of dQ = dS K whatever it holds (0 * NaN)
+      if (half == 0 && qmin >= qmax && nq > 0) {
+        ok = mbar_wait(kv_full, 0, abort_flag);
+        const uint32_t krow = smem_u32(smem + OFF_K) + r * 128;
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) st_shared_v4(krow + c * 16, 0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    for (int j = 0; j < nq && ok; ++j) {
       const int s = j % NS;
       const int pb = j & 1;
       // first query of the unit; only the dense (adjacent-block) masks read it
@@ -371,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             p[c] = __uint_as_float(rs[c]);
             ds[c] = __uint_as_float(rp[c]);
           }
-        } else if (__all_sync(0xffffffffu, half_on && q0 + c0 >= qmin)) {
+        } else if (__all_sync(0xffffffffu, half_on && q0 + c0 >= qmin && (!WIN || q0 + c0 + 32 <= qmax))) {
           // every query of the chunk sees every key of the warp: no per-element mask;
           // dS = P * (scale * dP - scale * delta) as one FFMA and one FMUL
 #pragma unroll
@@ -398,10 +439,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int c = c4 + e;
-              const bool vis = half_on && (q0 + c0 + c >= qmin);
+              const bool vis = half_on && (q0 + c0 + c >= qmin) && (!WIN || q0 + c0 + c < qmax);
               const float pv = vis ? exp2f(__uint_as_float(rs[c]) * sl2 - lv[e]) : 0.f;
               p[c] = pv;
               ds[c] = pv * (__uint_as_float(rp[c]) - dv[e]) * a.scale;
+              if (WIN && !vis) ds[c] = 0.f;  // a masked key's dP may be anything
             }
           }
         }
@@ -528,6 +570,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int qh = 0; qh < 2; ++qh) {
             if (!((bits >> (2 * qh)) & 3)) continue;
+            if constexpr (WIN) {
+              const int q = ((qp >> (16 * qh)) & 0xffff) * 64;
+              if (q < a.Tq) {  // rows of the box past Tq are left out by the map
+                tma_reduce_add_4d(&tmDQ, stage + qh * 8192, 0, h, q, b);
+                tma_reduce_add_4d(&tmDQ, stage + TILE + qh * 8192, 32, h, q, b);
+              }
+              continue;
+            }
             const int row0 = rowb + ((qp >> (16 * qh)) & 0xffff) * 64;
             tma_reduce_add_2d(&tmDQ, stage + qh * 8192, h * 64, row0);
             tma_reduce_add_2d(&tmDQ, stage + TILE + qh * 8192, h * 64 + 32, row0);
@@ -561,7 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // delta[b,h,t] = sum over the head's 64 columns of dO * O (one warp per row)
 __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int o_col,
                              const __nv_bfloat16* __restrict__ dout, long lddo, int do_col,
-                             float* __restrict__ delta, int B, int H, int Tq, long rows_per_b) {
+                             float* __restrict__ delta, int B, int H, int Tq, long rows_per_b,
+                             long delta_ld) {
   const int lane = threadIdx.x & 31;
   const long row = blockIdx.x * 8L + (threadIdx.x >> 5);
   if (row >= static_cast<long>(B) * Tq) return;
@@ -589,7 +640,7 @@ __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int 
     s += __shfl_xor_sync(0xffffffffu, s, 4);
     if ((lane & 7) == 0 && c < chunks) {
       const int hh = c / 8;
-      delta[(static_cast<long>(b) * H + hh) * Tq + t] = s;
+      delta[(static_cast<long>(b) * H + hh) * delta_ld + t] = s;
     }
   }
 }
@@ -645,7 +696,7 @@ void launch_bwd(const AttnBwdArgs& g, int* status, cudaStream_t stream) {
                                  g.ld_dqacc * 4, 32, 64, CU_TENSOR_MAP_SWIZZLE_128B);
   const int n_kvtiles = (a.S + 127) / 128;
   const int n_qtiles = (a.Tq + 127) / 128;
-  attn_bwd_kernel<<<a.B * a.H * n_kvtiles, kThreads, SMEM_BYTES, stream>>>(
+  attn_bwd_kernel<false><<<a.B * a.H * n_kvtiles, kThreads, SMEM_BYTES, stream>>>(
       tQ, tK, tV, tDO, tDQ, g, n_kvtiles, n_qtiles, status);
   count_launch();
   check_cuda(cudaGetLastError(), "attn_bwd_kernel launch");
@@ -658,7 +709,7 @@ void attn_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
   if (a.Tq % 128 != 0) throw std::runtime_error("attn_bwd: queries per sample must be a multiple of 128");
   static bool attr = false;
   if (!attr) {
-    check_cuda(cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    check_cuda(cudaFuncSetAttribute(attn_bwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     SMEM_BYTES),
                "cudaFuncSetAttribute(attn_bwd)");
     attr = true;
@@ -668,12 +719,43 @@ void attn_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
   launch_bwd(g, device_status(dev), stream);
 }
 
+void attn_window_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
+  const AttnArgs& a = g.f;
+  if (a.B <= 0 || a.H <= 0 || a.S <= 0 || a.Tq <= 0) return;
+  const int n_kvtiles = (a.S + 127) / 128;
+  const int n_qtiles = (a.Tq + 127) / 128;
+  // query blocks are 16-bit numbers of 64 queries; lse / delta are read in whole tiles
+  if (a.Tq > 65536L * 64) throw std::runtime_error("attn_window_bwd: more than 4,194,304 queries per sample");
+  if (a.lse_ld < n_qtiles * 128L || a.lse_ld % 4 != 0)
+    throw std::runtime_error("attn_window_bwd: lse and delta rows must hold whole tiles of 128 queries");
+  const long grid = static_cast<long>(a.B) * a.H * n_kvtiles;
+  if (grid > 0x7fffffffL) throw std::runtime_error("attn_window_bwd: too many key tiles for one launch");
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  raise_smem_limit<attn_bwd_kernel<true>>(SMEM_BYTES, dev);
+  const CUtensorMap tQ = window_tmap(a.q, a.B, a.Tq, a.H, a.q_sb, a.q_st, a.q_sh);
+  const CUtensorMap tK = window_tmap(a.k, a.B, a.S, a.H, a.k_sb, a.k_st, a.k_sh);
+  const CUtensorMap tV = window_tmap(a.v, a.B, a.S, a.H, a.v_sb, a.v_st, a.v_sh);
+  const CUtensorMap tDO = window_tmap(g.dout, a.B, a.Tq, a.H, g.do_sb, g.do_st, g.do_sh);
+  // dQ accumulator [B, Tq, H, 64] fp32, boxes of 32 columns x 64 queries of one head
+  const uint64_t dims[4] = {64, static_cast<uint64_t>(a.H), static_cast<uint64_t>(a.Tq), static_cast<uint64_t>(a.B)};
+  const uint64_t strides[3] = {256, 256ull * a.H, 256ull * a.H * a.Tq};
+  const uint32_t box[4] = {32, 1, 64, 1};
+  const CUtensorMap tDQ = make_tmap_nd(g.dq_acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 4, dims, strides, box,
+                                       CU_TENSOR_MAP_SWIZZLE_128B);
+  attn_bwd_kernel<true><<<static_cast<int>(grid), kThreads, SMEM_BYTES, stream>>>(
+      tQ, tK, tV, tDO, tDQ, g, n_kvtiles, n_qtiles, device_status(dev));
+  count_launch();
+  check_cuda(cudaGetLastError(), "attn_bwd_kernel (windowed) launch");
+}
+
 void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long lddo, int do_col,
-                    float* delta, int B, int H, int Tq, long rows_per_b, cudaStream_t s) {
+                    float* delta, int B, int H, int Tq, long rows_per_b, cudaStream_t s, long delta_ld) {
   const long rows = static_cast<long>(B) * Tq;
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(o), ldo, o_col,
-      reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b);
+      reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b,
+      delta_ld ? delta_ld : Tq);
   count_launch();
 }
 
@@ -697,7 +779,7 @@ void attn_bwd_with_status(const AttnBwdArgs& g, int* status, cudaStream_t stream
   const AttnArgs& a = g.f;
   if (a.B <= 0 || a.H <= 0 || a.S <= 0) return;
   if (a.Tq % 128 != 0) throw std::runtime_error("attn_bwd: queries per sample must be a multiple of 128");
-  check_cuda(cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  check_cuda(cudaFuncSetAttribute(attn_bwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   SMEM_BYTES),
              "cudaFuncSetAttribute(attn_bwd)");
   launch_bwd(g, status, stream);

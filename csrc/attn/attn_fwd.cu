@@ -22,6 +22,10 @@
 // 12 heads x 16 tiles of a 4-frame chunk against a 36-frame window), `kv_splits` CTAs
 // share each query tile's key tiles; each writes its normalised fp32 O and its lse, and
 // attn_split_merge_kernel combines them (O = sum 2^(lse_i - lse) O_i).
+//
+// Windowed mode (attn_window_fwd): the keys of the newest frames and the first ones; a
+// query tile walks only tiles with a visible key. Any number of queries and keys, any
+// strides of the heads' rows.
 // Semantics oracle: layers/attention.py attention_reference (reference layers/mha.py:88-116
 // with fp32 softmax), layers/sla.py sla_sparse_reference.
 #include <cuda.h>
@@ -33,6 +37,7 @@
 #include "../common/ptx.cuh"
 #include "../common/tma.h"
 #include "attn.h"
+#include "window.cuh"
 
 namespace ddb {
 namespace {
@@ -79,7 +84,10 @@ __device__ __forceinline__ int row_limit(const AttnArgs& a, int q_local) {
   return max(lim, 0);
 }
 
-
+// WIN: the windowed mode, instantiated apart so that the other masks' code is unchanged.
+// Its tiles are those of the sinks, then those of the window; q, k and v come through 4-D
+// maps (channels, heads, tokens, samples), so rows past a sample read as zeros.
+template <bool WIN>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ,
                     const __grid_constant__ CUtensorMap tmK,
@@ -121,7 +129,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   const long list_idx = static_cast<long>(bh) * n_qtiles + qt;
   int ntiles;
   int j0 = 0;  // first key tile of this CTA (split-KV: its share of the tile's key range)
-  if (sparse) {
+  WindowTiles wt{};
+  if constexpr (WIN) {
+    wt = window_tiles(a, q0, min(q0 + 127, a.Tq - 1));
+    ntiles = wt.n;
+    if (splits > 1) {
+      const int per = (ntiles + splits - 1) / splits;
+      j0 = min(ntiles, split * per);
+      ntiles = min(ntiles, j0 + per) - j0;
+    }
+  } else if (sparse) {
     ntiles = min(a.pair_count[list_idx], a.max_pairs);
   } else {
     const int lim = row_limit(a, min(q0 + 127, a.Tq - 1));
@@ -167,8 +184,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int qrow = static_cast<int>(b * a.q_rows_per_b) + q0;
       const int qcol = a.q_col + h * 64;
       mbar_arrive_expect_tx(q_full, TILE_BYTES);
-      tma_load_2d(sQ, &tmQ, q_full, qcol, qrow);
-      tma_load_2d(sQ + 8192, &tmQ, q_full, qcol, qrow + 64);
+      if constexpr (WIN) {
+        tma_load_4d(sQ, &tmQ, q_full, 0, h, q0, b);
+        tma_load_4d(sQ + 8192, &tmQ, q_full, 0, h, q0 + 64, b);
+      } else {
+        tma_load_2d(sQ, &tmQ, q_full, qcol, qrow);
+        tma_load_2d(sQ + 8192, &tmQ, q_full, qcol, qrow + 64);
+      }
       const int krow0 = static_cast<int>(b * a.kv_rows_per_b);
       int issued_k = 0, issued_v = 0;
       // one 128-key tile of K (is_v false) or V into its stage, once the stage is free
@@ -194,8 +216,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         const CUtensorMap* tm = is_v ? &tmV : &tmK;
         const int col = (is_v ? a.v_col : a.k_col) + h * 64;
         mbar_arrive_expect_tx(full, TILE_BYTES);
-        tma_load_2d(dst, tm, full, col, krow0 + b0 * 64);
-        tma_load_2d(dst + 8192, tm, full, col, krow0 + b1 * 64);
+        if constexpr (WIN) {
+          const int key = wt.at(j0 + j) * 128;
+          tma_load_4d(dst, tm, full, 0, h, key, b);
+          tma_load_4d(dst + 8192, tm, full, 0, h, key + 64, b);
+        } else {
+          tma_load_2d(dst, tm, full, col, krow0 + b0 * 64);
+          tma_load_2d(dst + 8192, tm, full, col, krow0 + b1 * 64);
+        }
         if (is_v) ++issued_v; else ++issued_k;
         return true;
       };
@@ -285,6 +313,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int q_local = q0 + r;
     const bool row_ok = q_local < a.Tq;
     const int lim = row_ok ? row_limit(a, q_local) : 0;
+    WindowSpan span{};
+    if constexpr (WIN) span = row_ok ? window_span(a, q_local) : WindowSpan{0, 0, 0};
     const int qhalf = r >> 6;
     const float sl2 = a.scale * 1.4426950408889634f;
     const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -318,7 +348,28 @@ __global__ void __launch_bounds__(kThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
       if (tw) fwd_trace(tr, 2, 1, j);
-      if (sparse) {
+      if constexpr (WIN) {
+        const int base = wt.at(j0 + j) * 128;
+        if (!span.whole(base, 128)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (!span.sees(base + c)) sf[c] = -INFINITY;
+        }
+        // keys that no query of the tile sees stay out of P V whatever their values are
+        // (0 * NaN): their value rows become zeros
+        if (!wt.span.whole(base, 128)) {
+          if (!mbar_wait(&v_full[j % NS], (j / NS) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (!wt.span.sees(base + r)) {
+            const uint32_t vrow = smem_u32(smem + OFF_V + (j % NS) * TILE_BYTES) + r * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) st_shared_v4(vrow + c * 16, 0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+        }
+      } else if (sparse) {
         const int bits = a.pair_mask[list_idx * a.max_pairs + j];
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh) {
@@ -444,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      pack_bf16(ov[c + 2] * inv, ov[c + 3] * inv),
                      pack_bf16(ov[c + 4] * inv, ov[c + 5] * inv),
                      pack_bf16(ov[c + 6] * inv, ov[c + 7] * inv));
-      if (a.lse) a.lse[static_cast<long>(bh) * a.Tq + q_local] = l > 0.f ? m + __log2f(l) : -INFINITY;
+      if (a.lse) a.lse[static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + q_local] = l > 0.f ? m + __log2f(l) : -INFINITY;
     }
   }
 
@@ -489,7 +540,7 @@ __global__ void __launch_bounds__(256) attn_split_merge_kernel(const AttnArgs a)
   __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) +
                         (b * a.q_rows_per_b + q) * a.ldo + a.o_col + h * 64;
   *reinterpret_cast<uint32_t*>(orow + 2 * lane) = pack_bf16(o0 * inv, o1 * inv);
-  if (a.lse && lane == 0) a.lse[bh * a.Tq + q] = wsum > 0.f ? mx + __log2f(wsum) : -INFINITY;
+  if (a.lse && lane == 0) a.lse[bh * (a.lse_ld ? a.lse_ld : a.Tq) + q] = wsum > 0.f ? mx + __log2f(wsum) : -INFINITY;
 }
 
 }  // namespace
@@ -531,7 +582,7 @@ void attn_fwd(const AttnArgs& a, cudaStream_t stream) {
   if (a.B <= 0 || a.H <= 0 || a.Tq <= 0) return;
   static bool attr = false;
   if (!attr) {
-    check_cuda(cudaFuncSetAttribute(attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    check_cuda(cudaFuncSetAttribute(attn_fwd_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     SMEM_BYTES),
                "cudaFuncSetAttribute(attn_fwd)");
     attr = true;
@@ -551,10 +602,64 @@ void attn_fwd(const AttnArgs& a, cudaStream_t stream) {
   const int grid = a.B * a.H * n_qtiles * splits;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  attn_fwd_kernel<<<grid, kThreads, SMEM_BYTES, stream>>>(tQ, tK, tV, a, n_qtiles,
+  attn_fwd_kernel<false><<<grid, kThreads, SMEM_BYTES, stream>>>(tQ, tK, tV, a, n_qtiles,
                                                           device_status(dev), g_fwd_trace);
   count_launch();
   check_cuda(cudaGetLastError(), "attn_fwd_kernel launch");
+  if (splits > 1) {
+    const long items = static_cast<long>(a.B) * a.Tq * a.H;
+    attn_split_merge_kernel<<<static_cast<int>((items + 7) / 8), 256, 0, stream>>>(a);
+    count_launch();
+    check_cuda(cudaGetLastError(), "attn_split_merge_kernel launch");
+  }
+}
+
+namespace {
+// visible key tiles of the query tile at q0 .. q0 + 127
+int window_tile_count(const AttnArgs& a, long q0) {
+  return window_tiles(a, static_cast<int>(q0), static_cast<int>(std::min<long>(q0 + 127, a.Tq - 1))).n;
+}
+}  // namespace
+
+int attn_window_kv_splits(const AttnArgs& a) {
+  if (a.B <= 0 || a.H <= 0 || a.Tq <= 0) return 1;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  const long slots = 2L * num_sms(dev);  // two CTAs per SM
+  const long ctas = static_cast<long>(a.B) * a.H * ((a.Tq + 127) / 128);
+  if (ctas >= slots) return 1;
+  const int tiles = window_tile_count(a, (a.Tq - 1) / 128 * 128);
+  // time ~ waves x key tiles of a split: the fewest splits with the smallest estimate
+  int best = 1;
+  double best_t = 1.0;
+  for (int s = 2; s <= 8 && tiles / s >= 4; ++s) {
+    const double t = static_cast<double>((ctas * s + slots - 1) / slots) / s;
+    if (t < best_t - 1e-9) {
+      best_t = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+void attn_window_fwd(const AttnArgs& a, cudaStream_t stream) {
+  if (a.B <= 0 || a.H <= 0 || a.Tq <= 0) return;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  raise_smem_limit<attn_fwd_kernel<true>>(SMEM_BYTES, dev);
+  const CUtensorMap tQ = window_tmap(a.q, a.B, a.Tq, a.H, a.q_sb, a.q_st, a.q_sh);
+  const CUtensorMap tK = window_tmap(a.k, a.B, a.S, a.H, a.k_sb, a.k_st, a.k_sh);
+  const CUtensorMap tV = window_tmap(a.v, a.B, a.S, a.H, a.v_sb, a.v_st, a.v_sh);
+  const int n_qtiles = (a.Tq + 127) / 128;
+  const int splits = a.kv_splits > 1 ? a.kv_splits : 1;
+  if (splits > 1 && (a.o_part == nullptr || a.lse_part == nullptr))
+    throw std::runtime_error("attn_window_fwd: split-KV needs both scratch buffers");
+  const long grid = static_cast<long>(a.B) * a.H * n_qtiles * splits;
+  if (grid > 0x7fffffffL) throw std::runtime_error("attn_window_fwd: too many query tiles for one launch");
+  attn_fwd_kernel<true><<<static_cast<int>(grid), kThreads, SMEM_BYTES, stream>>>(
+      tQ, tK, tV, a, n_qtiles, device_status(dev), FwdTrace{nullptr, 0});
+  count_launch();
+  check_cuda(cudaGetLastError(), "attn_fwd_kernel (windowed) launch");
   if (splits > 1) {
     const long items = static_cast<long>(a.B) * a.Tq * a.H;
     attn_split_merge_kernel<<<static_cast<int>((items + 7) / 8), 256, 0, stream>>>(a);

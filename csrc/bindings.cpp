@@ -1398,6 +1398,120 @@ void ep_copy_rows(c10::optional<torch::Tensor> src_table, int64_t src_ptr,
   ddb::ep_copy_rows(a, stream());
 }
 
+// ---------------------------------------------------------------- windowed attention
+// [B, rows, H, 64] bf16 with contiguous channels; the element strides a TMA map takes (16-byte
+// multiples; a stride of a dimension of one is free)
+void window_strides(const torch::Tensor& t, const char* name, const torch::Tensor& like, int64_t B, int64_t H,
+                    long& sb, long& st, long& sh) {
+  check_bf16(t, name);
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == B && t.size(2) == H && t.size(3) == 64, name, " must be [", B, ", rows, ", H, ", 64]");
+  TORCH_CHECK(t.device() == like.device(), name, " must be on q's device");
+  TORCH_CHECK(t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
+              " must have contiguous, 16-byte aligned channels");
+  sh = t.size(2) > 1 ? t.stride(2) : 64;
+  st = t.size(1) > 1 ? t.stride(1) : sh * H;
+  sb = t.size(0) > 1 ? t.stride(0) : st * t.size(1);
+  for (long s : {sb, st, sh})
+    TORCH_CHECK(s > 0 && s % 8 == 0 && s < (1L << 38), name, " has strides that are no multiples of 16 bytes");
+}
+
+ddb::AttnArgs window_args(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, int64_t causal,
+                          int64_t unit, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos, double scale) {
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.numel() > 0 && k.numel() > 0, "windowed attention: empty input");
+  ddb::AttnArgs a;
+  const int64_t B = q.size(0), H = q.size(2), limit = 1 << 30;
+  window_strides(q, "q", q, B, H, a.q_sb, a.q_st, a.q_sh);
+  window_strides(k, "k", q, B, H, a.k_sb, a.k_st, a.k_sh);
+  window_strides(v, "v", q, B, H, a.v_sb, a.v_st, a.v_sh);
+  TORCH_CHECK(k.size(1) == v.size(1), "windowed attention: k and v differ in length");
+  TORCH_CHECK(q_pos >= 0 && kv_pos >= 0 && q_pos + q.size(1) <= limit && kv_pos + k.size(1) <= limit &&
+                  unit >= 1 && unit <= (1 << 24) && window >= 0 && window * unit <= limit && sinks >= 0 && sinks <= limit,
+              "windowed attention: positions, unit, window or sinks out of range");
+  TORCH_CHECK(causal == ddb::kCausalNone || causal == ddb::kCausalFrame, "windowed attention: causal is 0 or 1");
+  a.B = B; a.H = H; a.Tq = q.size(1); a.S = k.size(1);
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+  a.q_rows_per_b = a.Tq; a.kv_rows_per_b = a.S;
+  a.causal = causal; a.tpf = unit; a.window = window; a.sink_tokens = sinks;
+  a.q_pos_offset = q_pos; a.kv_pos_offset = kv_pos; a.scale = static_cast<float>(scale);
+  return a;
+}
+
+void check_window_lse(const torch::Tensor& t, const char* name, const ddb::AttnArgs& a) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.dim() == 3 && t.size(0) == a.B &&
+                  t.size(1) == a.H && t.size(2) >= a.Tq && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be contiguous fp32 [B, H, >= T]");
+}
+
+void attn_window_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor lse,
+                     int64_t causal, int64_t unit, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
+                     double scale) {
+  auto a = window_args(q, k, v, causal, unit, window, sinks, q_pos, kv_pos, scale);
+  check_bf16(o, "o");
+  TORCH_CHECK(o.is_contiguous() && o.sizes() == q.sizes() && o.device() == q.device() &&
+                  reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0, "o must be contiguous and like q");
+  check_window_lse(lse, "lse", a);
+  const c10::cuda::CUDAGuard guard(q.device());
+  a.o = o.data_ptr(); a.ldo = a.H * 64;
+  a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
+  const int splits = g_attn_kv_splits > 0 ? static_cast<int>(g_attn_kv_splits) : ddb::attn_window_kv_splits(a);
+  torch::Tensor scratch;  // of this call: streams and captured graphs share none
+  if (splits > 1) {
+    long oe = 0, le = 0;
+    ddb::attn_fwd_split_scratch(a, splits, &oe, &le);
+    oe = (oe + 63) / 64 * 64;
+    scratch = torch::empty({oe + le}, q.options().dtype(torch::kFloat32));
+    a.kv_splits = splits;
+    a.o_part = scratch.data_ptr<float>();
+    a.lse_part = a.o_part + oe;
+  }
+  ddb::attn_window_fwd(a, stream());
+}
+
+// dk, dv: [B, S, H, 64] views whose rows lie at one stride over the samples, heads 64 apart
+void window_grad_rows(const torch::Tensor& t, const char* name, const ddb::AttnArgs& a, const torch::Tensor& q, long& ld) {
+  check_bf16(t, name);
+  TORCH_CHECK(t.dim() == 4 && t.size(0) == a.B && t.size(1) == a.S && t.size(2) == a.H && t.size(3) == 64 &&
+                  t.device() == q.device(), name, " must be like k");
+  ld = t.size(1) > 1 ? t.stride(1) : t.size(0) > 1 ? t.stride(0) : a.H * 64L;
+  TORCH_CHECK(t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == 64) && ld >= a.H * 64L && ld % 8 == 0 &&
+                  (t.size(0) == 1 || t.stride(0) == ld * a.S) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be rows of contiguous heads at one 16-byte aligned stride");
+}
+
+void attn_window_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
+                     torch::Tensor lse, torch::Tensor delta, torch::Tensor dq_acc, torch::Tensor dk, torch::Tensor dv,
+                     int64_t causal, int64_t unit, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
+                     double scale) {
+  ddb::AttnBwdArgs g;
+  g.f = window_args(q, k, v, causal, unit, window, sinks, q_pos, kv_pos, scale);
+  auto& a = g.f;
+  check_window_lse(lse, "lse", a);
+  check_window_lse(delta, "delta", a);
+  TORCH_CHECK(lse.size(2) == delta.size(2) && lse.size(2) >= (a.Tq + 127) / 128 * 128 && lse.size(2) % 4 == 0 &&
+                  lse.device() == q.device() && delta.device() == q.device(),
+              "lse and delta rows must hold whole tiles of 128 queries");
+  for (const auto* t : {&o, &dout})
+    TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->is_contiguous() && t->sizes() == q.sizes() &&
+                    t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "o and dout must be contiguous bf16 and like q");
+  TORCH_CHECK(dq_acc.is_cuda() && dq_acc.scalar_type() == torch::kFloat32 && dq_acc.is_contiguous() &&
+                  dq_acc.numel() == q.numel() && dq_acc.device() == q.device(), "dq_acc must be contiguous fp32 and like q");
+  const c10::cuda::CUDAGuard guard(q.device());
+  a.o = o.data_ptr(); a.ldo = a.H * 64;
+  a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
+  g.dout = dout.data_ptr();
+  g.do_sh = 64; g.do_st = a.H * 64L; g.do_sb = g.do_st * a.Tq;
+  g.delta = delta.data_ptr<float>();
+  g.dq_acc = dq_acc.data_ptr<float>(); g.ld_dqacc = a.H * 64;
+  window_grad_rows(dk, "dk", a, q, g.lddk);
+  window_grad_rows(dv, "dv", a, q, g.lddv);
+  g.dk = dk.data_ptr();
+  g.dv = dv.data_ptr();
+  ddb::attn_bwd_delta(o.data_ptr(), a.ldo, 0, dout.data_ptr(), a.ldo, 0, delta.data_ptr<float>(), a.B, a.H, a.Tq, a.Tq,
+                      stream(), lse.size(2));
+  ddb::attn_window_bwd(g, stream());
+}
+
 // ---------------------------------------------------------------- 8-bit paged key/value cache
 // Codes [L, P, heads, 64, 64] of one byte and fp32 scales [L, P, heads] of a cache; the
 // pointers of one layer of it.
@@ -1582,6 +1696,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q_pos_offset"), py::arg("kv_pos_offset"), py::arg("scale"), py::arg("kv_qtiles"),
         py::arg("kv_qmask"), py::arg("kv_count"), py::arg("debug_flags") = 0,
         py::arg("trace") = py::none(), py::arg("trace_cta") = 0);
+  m.def("attn_window_fwd", &attn_window_fwd, "tcgen05 attention over a window and the first tokens, forward");
+  m.def("attn_window_bwd", &attn_window_bwd, "tcgen05 attention over a window and the first tokens, backward");
   m.def("kv_cache_write", &kv_cache_write, "tokens into the pages of an 8-bit key/value cache");
   m.def("kv_cache_attend", &kv_cache_attend, "attention over an 8-bit paged key/value cache");
   m.def("kv_cache_copy_pages", &kv_cache_copy_pages, "copy cache pages in every layer");

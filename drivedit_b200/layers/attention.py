@@ -58,6 +58,20 @@ def frame_causal_mask(T: int, tokens_per_frame: int, S: Optional[int] = None,
     return (kf <= qf)[None, None]
 
 
+def window_mask(T: int, S: int, causal: str = "frame", tokens_per_frame: int = 1, window: int = 0,
+                sinks: int = 0, q_pos_offset: int = 0, kv_pos_offset: int = 0, device=None) -> torch.Tensor:
+    """``[T, S]`` bool, True = attend: a query of frame f sees the frames f - window + 1 .. f
+    (``window`` 0: every frame up to f) and the first ``sinks`` frames. ``causal`` "token"
+    counts in tokens, "none" sees everything; positions are the offsets plus the indexes."""
+    unit = tokens_per_frame if causal == "frame" else 1
+    qf = ((torch.arange(T, device=device) + q_pos_offset) // unit)[:, None]
+    kf = ((torch.arange(S, device=device) + kv_pos_offset) // unit)[None, :]
+    if causal == "none":
+        return torch.ones(T, S, dtype=torch.bool, device=device)
+    seen = kf <= qf
+    return seen & ((kf > qf - window) | (kf < sinks)) if window else seen
+
+
 def attention_reference(q, k, v, mask: Optional[torch.Tensor] = None,
                         scale: Optional[float] = None, return_lse: bool = False):
     """fp32 softmax attention on ``[B, T, H, D]``; ``mask`` is bool (True = attend),

@@ -159,9 +159,10 @@ class CacheStep:
             raise ValueError("tokens_per_frame must be positive, window and sinks not negative")
         if causal == "none" and (window or sinks):
             raise ValueError("a window needs causal frame or token")
+        if unit > 1 << 24:
+            raise ValueError("at most 2^24 tokens per frame")
         # a window or sinks past every token mean all of them
-        unit = min(unit, 1 << 24)
-        window = window if window * unit < _MAX_TOKENS and window <= 1 << 24 else 0
+        window = window if window * unit <= _MAX_TOKENS and window <= 1 << 24 else 0
         n_sink = min(sinks * unit, _MAX_TOKENS)
         scale = 1.0 / math.sqrt(64) if scale is None else float(scale)
         if not (scale > 0 and math.isfinite(scale)):
