@@ -77,6 +77,10 @@ class ModelConfig:
     action_dim: int = 2
     attention: str = "dense"        # "dense" | "sla"
     causal: str = "frame"           # "frame" | "token" | "none"
+    # dense causal attention over a sliding window: a frame's tokens see its newest
+    # window_frames frames (its own counted; 0: all earlier ones) and the first sink_frames
+    window_frames: int = 0
+    sink_frames: int = 0
     sla: SLAParams = field(default_factory=SLAParams)
     moe: Optional[MoEParams] = None
     rope_base: float = 10000.0
@@ -145,6 +149,10 @@ class RolloutConfig:
     context_frames: int = 4
     batch: int = 1
     tp: int = 1
+    # "bf16": contiguous rolling buffers; "fp8": 8-bit pages (drivedit_b200.ops.kv_cache),
+    # half the memory and reads, which also keep the first sink_frames frames visible
+    kv_cache: str = "bf16"
+    sink_frames: int = 0
 
 
 @dataclass

@@ -7,7 +7,8 @@ Workload (``rollout_dit_b`` preset): the causal DiT-B student (12 layers, d=768,
 frame-causal attention, 3-D RoPE), 4 context frames ~N(0,1), then 116 more latent frames of
 16 ch x 32x64 (512 tokens) generated in chunks of 4 frames with 4 Euler flow steps per chunk
 and a 32-frame rolling KV window; 3-D actions ~U[-1,1]; random-init weights; bf16.
-Per-chunk latency is device time (CUDA events) around the 4 denoising forwards plus the
+The overrides ``rollout.kv_cache=fp8 rollout.sink_frames=4`` hold the window in 8-bit pages
+and keep the context frames visible. Per-chunk latency is device time (CUDA events) around the 4 denoising forwards plus the
 cache-fill forward; frames/s = batch * generated frames / sum of chunk times. One JSON
 line per batch size. Under torchrun the model runs tensor-parallel over the N ranks
 (:mod:`drivedit_b200.parallel.tensor`); chunk times are the max over ranks.
@@ -70,6 +71,8 @@ def run(batch: int, frames: int, warm_chunks: int = 2, overrides=None, tp_transp
         "chunk_frames": cfg.rollout.chunk_frames,
         "flow_steps": cfg.rollout.flow_steps,
         "window_frames": cfg.rollout.window_frames,
+        "kv_cache": cfg.rollout.kv_cache,
+        "sink_frames": cfg.rollout.sink_frames,
         "chunks": len(res.chunk_ms),
         "p50_chunk_ms": round(res.percentile_ms(50), 3),
         "p99_chunk_ms": round(res.percentile_ms(99), 3),

@@ -24,7 +24,7 @@ import torch
 import torch.nn.functional as F
 
 from ..config import RolloutConfig
-from ..models.world_dit import KVCacheSet, WorldDiT
+from ..models.world_dit import KVCacheSet, PagedKVCacheSet, WorldDiT
 from ..models.world_dit import forward_cached as _forward_cached
 
 
@@ -187,15 +187,45 @@ class StreamingRollout:
         (a callable ``(f0, n) -> chunk or None``) may supply the chunk of frames
         ``[f0, f0 + n)`` instead of generating it (e.g. the ground-truth frames in
         self-forcing training for chunks that are not self-generated)."""
+        return self._run(context, actions, total_frames, generator, extra_cond, replace, 1)
+
+    @torch.no_grad()
+    def run_branches(self, context: torch.Tensor, actions: torch.Tensor, total_frames: Optional[int] = None,
+                     generator: Optional[torch.Generator] = None) -> RolloutResult:
+        """``K`` futures of each context, one for each action sequence ``actions
+        [B, K, F_total, A]`` (equal over the context's frames; those of the first sequence
+        are used there). The context is encoded once and its cached pages are shared
+        (``kv_cache="fp8"``). Returns frames ``[B * K, F_total, C, H, W]``, stream by stream."""
+        if self.cfg.kv_cache != "fp8":
+            raise ValueError('branches share pages of the 8-bit cache: set kv_cache="fp8"')
+        if actions.dim() != 4 or actions.shape[0] != context.shape[0]:
+            raise ValueError(f"actions must be [B, K, F, A], got {tuple(actions.shape)}")
+        return self._run(context, actions.flatten(0, 1), total_frames, generator, None, None, actions.shape[1])
+
+    def _make_cache(self, B: int, total: int, branches: int):
+        cfg, m = self.cfg, self.model
+        make_cache = getattr(m, "make_kv_cache", None)     # e.g. a tensor-parallel model
+        if cfg.kv_cache not in ("bf16", "fp8"):
+            raise ValueError(f'kv_cache must be "bf16" or "fp8", got {cfg.kv_cache!r}')
+        if cfg.kv_cache == "fp8":
+            if make_cache is not None:
+                raise ValueError("tensor-parallel rollouts hold their window in bf16")
+            return PagedKVCacheSet(m, B, cfg.window_frames, cfg.chunk_frames, self.device,
+                                   cfg.sink_frames or m.cfg.sink_frames, total, branches)
+        if cfg.sink_frames:
+            raise ValueError('sink_frames needs kv_cache="fp8"')
+        if make_cache is not None:
+            return make_cache(B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype)
+        return KVCacheSet(m, B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype)
+
+    def _run(self, context, actions, total_frames, generator, extra_cond, replace, branches) -> RolloutResult:
         cfg = self.cfg
         m = self.model
         B, Fc = context.shape[:2]
         total = total_frames or cfg.total_frames
         chunk = cfg.chunk_frames
-        make_cache = getattr(m, "make_kv_cache", None)     # e.g. a tensor-parallel model
         fwd_chunk = getattr(m, "forward_cached_chunk", None)
-        cache = (make_cache(B, cfg.window_frames, chunk, self.device, self.dtype) if make_cache is not None
-                 else KVCacheSet(m, B, cfg.window_frames, chunk, self.device, self.dtype))
+        cache = self._make_cache(B, total, branches)
 
         def forward_cached(m_, x_, t_, a_, cache_, commit=False, extra_cond=None):
             if fwd_chunk is not None:
@@ -207,8 +237,13 @@ class StreamingRollout:
         # context frames -> cache (clean, t = 1)
         for f0 in range(0, Fc, chunk):
             f1 = min(Fc, f0 + chunk)
-            forward_cached(m, context[:, f0:f1].to(self.dtype), ones, actions[:, f0:f1], cache,
+            forward_cached(m, context[:, f0:f1].to(self.dtype), ones, actions[::branches, f0:f1], cache,
                            commit=True, extra_cond=None if extra_cond is None else extra_cond[:, f0:f1])
+        if branches != 1:
+            cache.branch(branches)
+            B *= branches
+            out = [out[0].repeat_interleave(branches, 0)]
+            ones = torch.ones(B, device=self.device)
         ts = torch.linspace(0.0, 1.0, cfg.flow_steps + 1, device=self.device)
         chunk_ms: List[float] = []
         t_all0 = time.perf_counter()

@@ -34,11 +34,18 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..config import ModelConfig
-from ..layers.attention import attention_reference, frame_causal_mask
+from ..layers.attention import attention_reference, frame_causal_mask, window_mask
 from ..layers.mlp import split_gu
 from ..layers.moe import MoEFFN
 from ..layers.rope import RoPE3D, apply_rope
 from ..layers.sla import SLAConfig, sla_topk_reference
+
+
+def attention_span(cfg: ModelConfig, tpf: int) -> Dict:
+    """The model's causal mask as the windowed operators' arguments (``causal``,
+    ``tokens_per_frame``, ``window``, ``sinks``; frames for "frame", tokens for "token")."""
+    per = 1 if cfg.causal == "frame" else tpf
+    return dict(causal=cfg.causal, tokens_per_frame=tpf, window=cfg.window_frames * per, sinks=cfg.sink_frames * per)
 
 
 def patchify(x: torch.Tensor, p: int) -> torch.Tensor:
@@ -162,7 +169,9 @@ class WorldDiTBlock(nn.Module):
             a = o_s.to(dt).reshape(B, T, d) @ self.attn.proj.weight.to(dt).t() + \
                 o_l.to(dt).reshape(B, T, d) @ self.attn.proj_lin.weight.to(dt).t()
         else:
-            if cfg.causal == "frame":
+            if cfg.window_frames:
+                mask = window_mask(T, T, device=x.device, **attention_span(cfg, tpf))[None, None]
+            elif cfg.causal == "frame":
                 mask = frame_causal_mask(T, tpf, device=x.device)
             elif cfg.causal == "token":
                 mask = torch.tril(torch.ones(T, T, dtype=torch.bool, device=x.device))[None, None]
@@ -196,6 +205,10 @@ class WorldDiT(nn.Module):
 
     def __init__(self, cfg: ModelConfig):
         super().__init__()
+        if cfg.window_frames < 0 or cfg.sink_frames < 0 or (cfg.sink_frames and not cfg.window_frames):
+            raise ValueError("window_frames and sink_frames must not be negative, and sinks need a window")
+        if cfg.window_frames and (cfg.attention != "dense" or cfg.causal == "none"):
+            raise ValueError("window_frames needs dense causal attention")
         self.cfg = cfg
         d = cfg.d_model
         self.patch_embed = nn.Linear(cfg.patch_dim, d)
@@ -349,6 +362,9 @@ class KVCacheSet:
     def __init__(self, model: "WorldDiT", B: int, window_frames: int, chunk_frames: int,
                  device, dtype):
         cfg = model.cfg
+        if cfg.sink_frames:
+            raise ValueError("the rolling buffers drop the first frames; a model with sink_frames streams "
+                             "through the 8-bit paged cache (kv_cache=\"fp8\")")
         tpf = cfg.tokens_per_frame
         cap = (2 * window_frames + chunk_frames) * tpf
         self.layers = [LayerKVCache(B, cap, cfg.d_model, window_frames * tpf, device, dtype)
@@ -366,9 +382,61 @@ class KVCacheSet:
         self.frames += n_frames
 
 
-def _block_cached_torch(blk: WorldDiTBlock, x, mod, tab_q, cache: LayerKVCache, row, frames):
+class PagedKVCacheSet:
+    """The rolling window of a streaming rollout in an 8-bit paged cache
+    (:class:`~drivedit_b200.ops.kv_cache.PagedKVCache`): of ``B`` streams the newest
+    ``window_frames`` committed frames and the first ``sink_frames`` stay, older ones give
+    their pages back. ``max_frames`` bounds a stream's length. :meth:`branch` turns the
+    streams into several that share their past."""
+
+    def __init__(self, model: "WorldDiT", B: int, window_frames: int, chunk_frames: int, device,
+                 sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1):
+        from ..ops.kv_cache import PAGE, PagedKVCache
+
+        cfg = model.cfg
+        if cfg.d_head != 64:
+            raise ValueError("the 8-bit cache holds heads of 64 channels")
+        if cfg.causal == "none":
+            raise ValueError("the paged cache streams causal models")
+        if cfg.window_frames and sink_frames != cfg.sink_frames:
+            raise ValueError(f"the model attends to {cfg.sink_frames} sink frames, the cache would keep {sink_frames}")
+        self.tpf = cfg.tokens_per_frame
+        self.window, self.sinks = window_frames * self.tpf, sink_frames * self.tpf
+        pages = lambda frames: -(-frames * self.tpf // PAGE)  # noqa: E731
+        # a chunk joins the window before the oldest frames leave it; two unfinished pages
+        own = pages(window_frames + 2 * chunk_frames) + 2
+        total = pages(max_frames or cfg.max_frames) + 1
+        n = B * (pages(sink_frames) + own) + (B * branches * own if branches > 1 else 0)
+        self.cache = PagedKVCache(len(model.blocks), cfg.n_heads, n, device, max_pages_per_seq=max(total, own))
+        self.layers = [None] * len(model.blocks)
+        self.seqs = self.cache.add(B)
+        self.frames = 0
+        self._step = None
+
+    def step(self, n_tokens: int):
+        """The open step for ``n_tokens`` more of each stream (kept until committed)."""
+        if self._step is None or self._step.n_new[:1] != [n_tokens]:
+            self._step = self.cache.begin(self.seqs, n_tokens)
+        return self._step
+
+    def commit(self, n_frames: int):
+        self.step(n_frames * self.tpf).commit()
+        self._step = None
+        self.cache.trim(self.seqs, self.window, self.sinks)
+        self.frames += n_frames
+
+    def branch(self, copies: int) -> None:
+        """Every stream becomes ``copies`` streams (those of the first stream first)."""
+        old = self.seqs
+        self.seqs = self.cache.fork(old, copies)
+        self.cache.free(old)
+        self._step = None
+
+
+def _block_cached_torch(blk: WorldDiTBlock, x, mod, tab_q, cache: LayerKVCache, row, frames, step=None,
+                        layer=0):
     """One block over a chunk ``x [B, T, d]`` attending to the cache window + itself;
-    writes the chunk's K/V into the cache rows ``[row, row + T)``."""
+    writes the chunk's K/V into the cache rows ``[row, row + T)`` (or the paged ``step``)."""
     cfg = blk.cfg
     B, T, d = x.shape
     H, Dh = cfg.n_heads, cfg.d_head
@@ -385,13 +453,21 @@ def _block_cached_torch(blk: WorldDiTBlock, x, mod, tab_q, cache: LayerKVCache, 
     qkv = (h @ blk.attn.qkv.weight.to(dt).t()).view(B, T, 3, H, Dh)
     q, k, v = qkv.unbind(2)
     q, k = apply_rope(q, tab_q), apply_rope(k, tab_q)
-    cache.k[:, row:row + T] = k.reshape(B, T, d)
-    cache.v[:, row:row + T] = v.reshape(B, T, d)
-    kk = cache.k[:, cache.start:row + T].view(B, -1, H, Dh)
-    vv = cache.v[:, cache.start:row + T].view(B, -1, H, Dh)
-    S = kk.shape[1]
-    mask = frame_causal_mask(T, tpf, S, x.device)
-    o = attention_reference(q, kk, vv, mask).to(dt)
+    if step is not None:
+        step.write(layer, k, v)
+        o = step.attend(layer, q, **attention_span(cfg, tpf))
+    else:
+        cache.k[:, row:row + T] = k.reshape(B, T, d)
+        cache.v[:, row:row + T] = v.reshape(B, T, d)
+        kk = cache.k[:, cache.start:row + T].view(B, -1, H, Dh)
+        vv = cache.v[:, cache.start:row + T].view(B, -1, H, Dh)
+        S = kk.shape[1]
+        if cfg.window_frames:
+            mask = window_mask(T, S, q_pos_offset=cache.pos0 + row, kv_pos_offset=cache.pos0 + cache.start,
+                               device=x.device, **attention_span(cfg, tpf))
+        else:
+            mask = frame_causal_mask(T, tpf, S, x.device)
+        o = attention_reference(q, kk, vv, mask).to(dt)
     x = x + o.reshape(B, T, d) @ blk.attn.proj.weight.to(dt).t()
     h2 = norm(x, blk.norm2.weight) * (1 + s2) + b2
     gu = h2 @ blk.mlp.w13.weight.to(dt).t()
@@ -416,10 +492,11 @@ def forward_cached(model: "WorldDiT", x_t: torch.Tensor, t: torch.Tensor, action
     c = model.condition(t, actions, extra_cond)
     T = x.shape[1]
     tab = model.rope.table(Fc, cache.frames).to(x.device)
-    row = cache.reserve(T)
-    for blk, lc in zip(model.blocks, cache.layers):
+    step = cache.step(T) if isinstance(cache, PagedKVCacheSet) else None
+    row = cache.reserve(T) if step is None else 0
+    for i, (blk, lc) in enumerate(zip(model.blocks, cache.layers)):
         mod = blk.ada(c).to(dt)
-        x = _block_cached_torch(blk, x, mod, tab, lc, row, Fc)
+        x = _block_cached_torch(blk, x, mod, tab, lc, row, Fc, step, i)
     if commit:
         cache.commit(Fc)
     fm = model.final_ada(c).to(dt).repeat_interleave(T // Fc, 1)

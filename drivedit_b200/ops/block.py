@@ -38,7 +38,7 @@ class BlockCtx:
     """Static per-call data shared by all blocks of one forward."""
 
     def __init__(self, B, T, frames, tpf, d, H, Dh, rope_tab, attn_mode, sla_cfg, causal,
-                 rope_pos_offset=0):
+                 rope_pos_offset=0, window_frames=0, sink_frames=0):
         self.B, self.T, self.frames, self.tpf = B, T, frames, tpf
         self.d, self.H, self.Dh = d, H, Dh
         self.rope_tab = rope_tab
@@ -46,6 +46,7 @@ class BlockCtx:
         self.sla_cfg = sla_cfg
         self.causal = causal
         self.rope_pos_offset = rope_pos_offset
+        self.window_frames, self.sink_frames = window_frames, sink_frames
         self.recompute = False  # activation checkpointing: blocks rerun their forward in backward
         self.grad_ready = None  # callback(block index) once a block's backward is enqueued
 
@@ -304,7 +305,8 @@ class FusedWorldDiT:
         c2 = c.reshape(B * Fr, d)
         tab = model.rope.table(Fr, frame_offset).to(x.device)
         bc = BlockCtx(B, T, Fr, T // Fr, d, cfg.n_heads, cfg.d_head, tab, cfg.attention,
-                      cfg.sla, cfg.causal)
+                      cfg.sla, cfg.causal, window_frames=cfg.window_frames,
+                      sink_frames=cfg.sink_frames)
         bc.recompute = self.recompute and torch.is_grad_enabled()
         bc.grad_ready = self.grad_ready
         feats = None
@@ -384,7 +386,7 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
     every block is AdaLN-RMSNorm -> QKV GEMM (rotary by absolute frame) -> K/V into the
     cache window -> flash attention with absolute query/key offsets -> output GEMM with
     residual -> AdaLN-RMSNorm -> SwiGLU GEMM -> down GEMM with residual."""
-    from ..models.world_dit import patchify, unpatchify
+    from ..models.world_dit import PagedKVCacheSet, attention_span, patchify, unpatchify
     from ._ext import ext
 
     cfg = model.cfg
@@ -398,7 +400,9 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
     x = gemm(tok, W(model.patch_embed.weight), bias=model.patch_embed.bias)
     c2 = model.condition(t, actions, extra_cond).reshape(B * Fc, d)
     tab = model.rope.table(Fc, cache.frames).to(x.device)
-    row = cache.reserve(T)
+    paged = isinstance(cache, PagedKVCacheSet)
+    step = cache.step(T) if paged else None
+    row = 0 if paged else cache.reserve(T)
     if self._runs is False:
         self._runs = _mod_runs(model, g)
     mods = None
@@ -407,7 +411,7 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
         mods = gemm(c2.to(torch.bfloat16).contiguous(), g.compute[w0:w0 + wn].view(-1, d),
                     epi="f32", bias=g.master[b0:b0 + bn])
     col = 0
-    for blk, lc in zip(model.blocks, cache.layers):
+    for i, (blk, lc) in enumerate(zip(model.blocks, cache.layers)):
         if mods is not None:
             n = blk.ada.weight.shape[0]
             mod = mods[:, col:col + n]
@@ -418,16 +422,28 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
         qkv = gemm(h1, W(blk.attn.qkv.weight), epi="rope", rope_tab=tab, rope_cols=2 * d,
                    rope_rows_per_seq=T, rope_head_dim=cfg.d_head)
         q3 = qkv.view(B, T, 3 * d)
-        lc.k[:, row:row + T].copy_(q3[:, :, d:2 * d])
-        lc.v[:, row:row + T].copy_(q3[:, :, 2 * d:])
-        cap = lc.k.shape[1]
-        k2 = lc.k.view(B * cap, d)[lc.start:]
-        v2 = lc.v.view(B * cap, d)[lc.start:]
-        S = row + T - lc.start
-        o = torch.empty(B * T, d, device=x.device, dtype=torch.bfloat16)
-        ext().attn_fwd(qkv, k2, v2, o, None, 0, 0, 0, 0, B, Hh, T, S, T, cap, 1, tpf,
-                       lc.pos0 + row, lc.pos0 + lc.start, 1.0 / math.sqrt(cfg.d_head),
-                       None, None, None)
+        if paged:
+            qh, kh, vh = qkv.view(B, T, 3, Hh, cfg.d_head).unbind(2)
+            step.write(i, kh, vh)
+            o = step.attend(i, qh, **attention_span(cfg, tpf)).view(B * T, d)
+        else:
+            lc.k[:, row:row + T].copy_(q3[:, :, d:2 * d])
+            lc.v[:, row:row + T].copy_(q3[:, :, 2 * d:])
+            cap = lc.k.shape[1]
+            S = row + T - lc.start
+        if not paged and cfg.window_frames:
+            from .window_attention import window_attention
+
+            kh, vh = (c.view(B, cap, Hh, cfg.d_head)[:, lc.start:row + T] for c in (lc.k, lc.v))
+            o = window_attention(qkv.view(B, T, 3, Hh, cfg.d_head)[:, :, 0], kh, vh, q_pos_offset=lc.pos0 + row,
+                                 kv_pos_offset=lc.pos0 + lc.start, **attention_span(cfg, tpf)).view(B * T, d)
+        elif not paged:
+            k2 = lc.k.view(B * cap, d)[lc.start:]
+            v2 = lc.v.view(B * cap, d)[lc.start:]
+            o = torch.empty(B * T, d, device=x.device, dtype=torch.bfloat16)
+            ext().attn_fwd(qkv, k2, v2, o, None, 0, 0, 0, 0, B, Hh, T, S, T, cap, 1, tpf,
+                           lc.pos0 + row, lc.pos0 + lc.start, 1.0 / math.sqrt(cfg.d_head),
+                           None, None, None)
         x1 = gemm(o, W(blk.attn.proj.weight), residual=x)
         h2, _ = adaln_rmsnorm(x1, blk.norm2.weight, mod, 2 * d, 3 * d, tpf)
         w13 = W(blk.mlp.w13.weight)

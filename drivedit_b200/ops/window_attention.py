@@ -56,6 +56,32 @@ def window_backward(q, k, v, o, lse, do, mask, dq, dk, dv):
     ext().attn_dq_finalize(acc, rows, 0, H, None, T, 0)
 
 
+_STREAM = "drivedit_b200.stream"
+
+
+def _leaf_nodes(*tensors):
+    """The accumulation nodes of the leaves among ``tensors``."""
+    return [x.view_as(x).grad_fn.next_functions[0][0] for x in tensors if x.requires_grad and x.is_leaf]
+
+
+def _apply(q, k, v, mask):
+    """A backward pass that is captured while an eager graph of the same leaf is alive ends
+    the process inside autograd: the leaf's accumulation node belongs to the default
+    stream. So the nodes that a graph made here keeps alive are marked with their stream,
+    and a capture that meets a node of the default stream is refused."""
+    leaves = torch.is_grad_enabled() and any(x.requires_grad and x.is_leaf for x in (q, k, v))
+    if leaves and torch.cuda.is_current_stream_capturing():
+        if any(n.metadata.get(_STREAM) == 0 for n in _leaf_nodes(q, k, v)):
+            raise RuntimeError("an autograd graph made on the default stream still uses this leaf: drop it before "
+                               "capturing a backward pass, or warm up on another stream")
+    out = _WindowAttention.apply(q, k, v, mask)
+    if leaves:
+        stream = torch.cuda.current_stream(q.device).cuda_stream
+        for n in _leaf_nodes(q, k, v):
+            n.metadata.setdefault(_STREAM, stream)
+    return out
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask):
@@ -128,7 +154,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
         o = q.masked_fill(yes, 0) + (k.sum() + v.sum()).masked_fill(yes, 0)
         lse = torch.full((B, H, T), -math.inf, device=q.device)
     elif q.is_cuda:
-        o, lse = _WindowAttention.apply(q, k, v, mask)
+        o, lse = _apply(q, k, v, mask)
     else:
         seen = window_mask(T, S, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, q.device)
         f = torch.promote_types(q.dtype, torch.float32)

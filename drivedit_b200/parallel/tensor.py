@@ -121,6 +121,8 @@ class TensorParallelWorldDiT:
         GEMM as peer TMA loads; wider ones pull the rows once and overlap.
         ``replicate_rows_max``: chunks of at most this many token rows run with the
         residual stream replicated on every rank and all-reduces (see the module notes)."""
+        if model.cfg.window_frames:
+            raise ValueError("windowed models (window_frames) have no tensor-parallel rollout")
         self.model = model
         self.cfg = model.cfg
         self.group = group if group is not None else dist.group.WORLD

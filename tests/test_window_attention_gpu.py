@@ -216,6 +216,25 @@ def test_captured_forward_and_backward():
         assert (out[1].float() - want[1].float()).abs().max() <= 2.0 ** -7 * want[1].float().abs().max()
 
 
+def test_capture_beside_an_eager_graph_is_refused():
+    from drivedit_b200.ops.window_attention import window_attention
+    x = _bits(1, 64, 1, 64).requires_grad_(True)
+    alive = window_attention(x, x, x, "token")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="default stream"):
+            window_attention(x, x, x, "token")
+        window_attention(x.detach(), x.detach(), x.detach(), "token")
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (g,) = torch.autograd.grad(window_attention(x, x, x, "token"), x, torch.ones_like(x))
+    graph.replay()
+    torch.cuda.synchronize()
+    (w,) = torch.autograd.grad(window_attention(x, x, x, "token"), x, torch.ones_like(x))
+    assert (g.float() - w.float()).abs().max() <= 2.0 ** -7 * w.float().abs().max()
+
+
 def test_empty_inputs():
     from drivedit_b200.ops.window_attention import window_attention
     q, k = _bits(2, 5, 1, 64).requires_grad_(True), _bits(2, 0, 1, 64).requires_grad_(True)
@@ -231,3 +250,79 @@ def test_status_clean():
     from drivedit_b200.ops._ext import device_status
     torch.cuda.synchronize()
     assert device_status() == 0
+
+
+def _world(*over, frames=4):
+    from drivedit_b200.config import get_config
+    from drivedit_b200.models.world_dit import WorldDiT
+    torch.manual_seed(0)
+    cfg = get_config("tiny", ["model.n_layers=2", f"train.frames={frames}", *over])
+    m = WorldDiT(cfg.model)
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.abs().sum() == 0:
+                p.normal_(0, 0.02)
+    return cfg, m
+
+
+@pytest.mark.parametrize("over", [("model.window_frames=2", "model.sink_frames=1"),
+                                  ("model.window_frames=2", "model.causal=token")])
+def test_windowed_model_trains_on_the_kernels(over):
+    """The flagship's fused forward and backward with a window against its PyTorch path."""
+    cfg, m = _world(*over, frames=6)
+    m = m.cuda()
+    x, t, a = torch.randn(2, 6, 16, 16, 16, device="cuda"), torch.rand(2, device="cuda"), torch.rand(2, 6, 2, device="cuda")
+    w = torch.randn(2, 6, 16, 16, 16, device="cuda")
+    ref = m(x, t, a)
+    (ref * w).sum().backward()
+    names = ["blocks.0.attn.qkv.weight", "blocks.1.attn.qkv.weight", "blocks.0.attn.proj.weight"]
+    want = {n: p.grad.clone() for n, p in m.named_parameters() if n in names}
+    m.zero_grad(set_to_none=True)
+    m.enable_fused()
+    m.fused.group.grad.zero_()
+    got = m(x, t, a)
+    # bf16 activations (2^-8 a rounding, about 20 in a row in two blocks) against fp32
+    assert (got.float() - ref).norm() / ref.norm() < 20 * 2.0 ** -9
+    (got.float() * w).sum().backward()
+    for n, p in m.named_parameters():
+        if n in names:
+            assert (p.grad - want[n]).norm() / want[n].norm() < 40 * 2.0 ** -9, n
+
+
+def test_streams_on_the_kernels_match_the_pytorch_form():
+    """A chunked stream on the GPU, bf16 buffers and 8-bit pages, with a window and sinks."""
+    from drivedit_b200.models.world_dit import KVCacheSet, PagedKVCacheSet, forward_cached
+    x, t, a = torch.randn(2, 6, 16, 16, 16), torch.rand(2), torch.rand(2, 6, 2)
+    for over, sinks in ((("model.window_frames=2",), 0), (("model.window_frames=2", "model.sink_frames=1"), 1), ((), 1)):
+        outs = []
+        for dev, dt in (("cpu", torch.float32), ("cuda", torch.bfloat16)):
+            cfg, m = _world(*over)
+            m = m.to(dev)
+            if dev == "cuda":
+                m.enable_fused()
+            caches = [PagedKVCacheSet(m, 2, 2, 2, torch.device(dev), sinks, 6)]
+            if not m.cfg.sink_frames:
+                caches.append(KVCacheSet(m, 2, 4, 2, dev, dt))
+            outs.append([torch.cat([forward_cached(m, x[:, f:f + 2].to(dev, dt), t.to(dev), a[:, f:f + 2].to(dev), c, commit=True)
+                                    .float().cpu() for f in (0, 2, 4)], 1) for c in caches])
+        for got, want in zip(outs[1], outs[0]):
+            # bf16 activations, and codes that fall to the other side of an e4m3 step for it
+            assert (got - want).norm() / want.norm() < 20 * 2.0 ** -9 + 2.0 ** -5
+
+
+def test_rollout_branches_on_the_kernels():
+    from drivedit_b200.inference.rollout import StreamingRollout
+    cfg, m = _world()
+    m = m.cuda().eval()
+    m.enable_fused()
+    r = cfg.rollout
+    r.chunk_frames, r.flow_steps, r.window_frames, r.kv_cache, r.sink_frames = 2, 2, 2, "fp8", 1
+    ctx, act = torch.randn(2, 2, 16, 16, 16, device="cuda"), torch.rand(2, 3, 10, 2, device="cuda")
+    act[:, :, :2] = act[:, :1, :2]
+    roll = StreamingRollout(m, r)
+    g = lambda: torch.Generator(device="cuda").manual_seed(4)  # noqa: E731
+    res = roll.run_branches(ctx, act, total_frames=10, generator=g())
+    one = roll.run(ctx.repeat_interleave(3, 0), act.flatten(0, 1), total_frames=10, generator=g())
+    assert res.frames.shape == (6, 10, 16, 16, 16) and torch.isfinite(res.frames).all()
+    # the same pages' contents and the same kernels: equal but for the context's batch shape
+    assert (res.frames - one.frames).norm() / one.frames.norm() < 2.0 ** -6
