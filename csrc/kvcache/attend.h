@@ -12,4 +12,7 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return amax > 0.f && k < 128 ? max(k - 14, -120) : 0;
 }
 
+// attend_tiles.cu: blocks of 256 rows on the tensor cores' 128-row products
+void kv_attend_tiles_launch(KvAttendArgs a, int dev, cudaStream_t stream);
+
 }  // namespace ddb

@@ -425,7 +425,10 @@ void kv_cache_attend(const KvAttendArgs& a, cudaStream_t stream) {
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  launch<1>(a, dev, stream);
+  if (a.T * static_cast<long>(a.H / a.pool.heads) > 64)
+    kv_attend_tiles_launch(a, dev, stream);
+  else
+    launch<1>(a, dev, stream);
 }
 
 }  // namespace ddb

@@ -1,0 +1,654 @@
+// Attention over the 8-bit paged cache for many query rows (chunks of frames, prompts).
+//
+// One CTA = 256 rows (token, query head of the group) of one (sequence, cached head), as
+// two tiles of 128, and a share of its pages; tiles of 128 keys are two pages. Both row
+// tiles use each key tile, so a code is converted once for 256 rows. Roles (512 threads,
+// one CTA per SM):
+//   warp 0       bulk copies of the pages' codes (keys 4 KB, values 4 KB each), 3 stages
+//   warp 1       TMEM owner and MMA issuer: S = Q K^T (M 128, N 128, K 64) and
+//                O += P V (M 128, N 64, K 128; P from TMEM), per row tile
+//   warps 4-7    e4m3 -> fp16 into the swizzled operand tiles (3 stages of 16 KB each):
+//                exact but for the page's scale relative to the largest of the CTA's
+//                pages, a power of two (below 2^-14 of it fp16 is subnormal: an error of
+//                2^-33 of the largest); tokens that no row sees become zeros
+//   warps 8-15   softmax: one thread per row and tile, as in the bf16 kernel; it also
+//                brings Q to fp16, scaled by a power of two per row
+// P is rounded to fp16 (2^-11), finer than the bf16 kernel's P.
+// The CTAs that share a row block form a cluster and meet through distributed shared
+// memory: no scratch memory, no second launch.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../common/ptx.cuh"
+#include "../common/tma.h"
+#include "attend.h"
+#include "masks.cuh"
+
+namespace ddb {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRows = 256;
+constexpr int NR = 3;  // stages of codes
+constexpr int NS = 3;  // stages of fp16 tiles
+constexpr int TILE = 16384;
+constexpr int OFF_Q = 0;
+constexpr int OFF_K = OFF_Q + 2 * TILE;
+constexpr int OFF_V = OFF_K + NS * TILE;
+constexpr int OFF_RAW = OFF_V + NS * TILE;   // per stage: keys of both pages, values of both
+constexpr int OFF_BAR = OFF_RAW + NR * TILE;
+constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 8 + 1;
+constexpr int OFF_META = OFF_BAR + N_BARS * 8;
+constexpr int OFF_MISC = OFF_META + NR * 16;
+constexpr int SMEM_BYTES = OFF_MISC + 32;
+static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+constexpr int OFF_RES = OFF_K;                    // results, once K and V are no longer read
+constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
+static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
+constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
+constexpr float kRescaleLog2 = 8.f;
+
+// kind::f16 with fp16 A and B, fp32 D, both K-major
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
+  return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+constexpr uint32_t IDESC_S = idesc_f16(128, 128);
+constexpr uint32_t IDESC_PV = idesc_f16(128, 64);
+
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// two codes times a power of two
+__device__ __forceinline__ uint32_t half2_scaled(uint32_t two, __half2 mul) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h), mul);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float inverse_power(float p) {  // 1 / 2^e, e in [-126, 126]
+  return __int_as_float((254 << 23) - __float_as_int(p));
+}
+// every warp has its role's registers
+__device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    kv_attend_tiles(const KvAttendArgs a, int row_tiles, int* status) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023) != 0) {  // uniform over the grid
+    if (threadIdx.x == 0 && status) atomicCAS(status, 0, kStatusBadArgument);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* raw_full = bars + 1;
+  uint64_t* raw_empty = raw_full + NR;
+  uint64_t* k_full = raw_empty + NR;
+  uint64_t* k_empty = k_full + NS;
+  uint64_t* v_full = k_empty + NS;
+  uint64_t* v_empty = v_full + NS;
+  uint64_t* s_full = v_empty + NS;  // [2], and so on
+  uint64_t* s_free = s_full + 2;
+  uint64_t* p_full = s_full + 4;
+  uint64_t* o_done = s_full + 6;
+  uint64_t* drain = s_full + 8;
+  float4* meta = reinterpret_cast<float4*>(smem + OFF_META);  // per stage: key, value factors of both pages
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+  int* ref_bits = reinterpret_cast<int*>(smem + OFF_MISC + 8);  // largest key, value scale
+
+  const int warp = warp_id(), lane = lane_id();
+  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  int item = blockIdx.x / ranks;
+  const int tile = row_tiles - 1 - item % row_tiles;  // long (late) tiles first
+  item /= row_tiles;
+  const int kh = item % a.pool.heads, b = item / a.pool.heads;
+  const int G = a.H / a.pool.heads;
+  const int* row = a.step.rows + static_cast<long>(b) * a.step.ld;
+  const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
+  const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
+  const int r0 = tile * kRows, rows = own * G;       // rows behind `rows` are padding
+  const int n_t = rows - r0 > 128 ? 2 : 1;
+
+  // the block's pages, and this CTA's run of key tiles (page pairs)
+  KvPages pages{0, 0, 0};
+  KvSpan all{0, 0};
+  if (r0 < rows) {
+    const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
+    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + kRows) - 1) / G, len, first);
+    all = KvSpan{s0.lo, s1.hi};
+    pages = kv_pages(s0.lo, s1.hi, sinks, a.step.width);
+  }
+  const int pairs = (pages.n + 1) / 2, per = (pairs + ranks - 1) / ranks;
+  const int j0 = min(pairs, rank * per), n = min(pairs, j0 + per) - j0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 8);
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 4);
+    }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&k_full[s], 4);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 4);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    ref_bits[0] = ref_bits[1] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the largest scales of this CTA's pages (positive floats order like their bits)
+  {
+    int mk = 0, mv = 0;
+    for (int i = 2 * j0 + threadIdx.x; i < min(pages.n, 2 * (j0 + n)); i += kThreads) {
+      const int id = row[kKvInfo + pages.at(i)];
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages)) {
+        const long block = static_cast<long>(id) * a.pool.heads + kh;
+        mk = max(mk, __float_as_int(a.pool.k_scale[block]));
+        mv = max(mv, __float_as_int(a.pool.v_scale[block]));
+      }
+    }
+    mk = __reduce_max_sync(0xffffffffu, mk);
+    mv = __reduce_max_sync(0xffffffffu, mv);
+    if (lane == 0 && mk) {
+      atomicMax(&ref_bits[0], mk);
+      atomicMax(&ref_bits[1], mv);
+    }
+  }
+  __syncthreads();
+  const float k_ref = ref_bits[0] ? __int_as_float(ref_bits[0]) : 1.f;
+  const float v_ref = ref_bits[1] ? __int_as_float(ref_bits[1]) : 1.f;
+
+  // Registers by role: 56 + 72 + 2 * 192 = 512 = 4 * 128, the launch's own. All go back to 128
+  // before the common end; none may before every role has its share (registers_split),
+  // or a role with nothing to do would take back what the softmax warps still wait for.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    registers_split();
+    if (warp == 0) {
+      // ---------------------------------------------------------- copies of the codes
+      bool ok = true;
+      int ids = -1, issued = 0;
+      float ks = 0.f, vs = 0.f;
+      for (int j = 0; j < n; ++j) {
+        if ((j & 15) == 0) {  // the next 16 pairs, one page a lane
+          const int i = 2 * (j0 + j) + lane;
+          ids = i < min(pages.n, 2 * (j0 + n)) ? row[kKvInfo + pages.at(i)] : -2;
+          if (ids != -2 && static_cast<unsigned>(ids) >= static_cast<unsigned>(a.pool.pages)) {
+            record_bad_index(status, ids);  // recorded, read as zeros
+            ids = -2;
+          }
+          ks = vs = 0.f;
+          if (ids >= 0) {
+            const long block = static_cast<long>(ids) * a.pool.heads + kh;
+            // zero stands for an absent page; below 2^-30 the product is zero in fp16 anyway
+            ks = fmaxf(a.pool.k_scale[block] * inverse_power(k_ref), 9.3132257e-10f);
+            vs = fmaxf(a.pool.v_scale[block] * inverse_power(v_ref), 9.3132257e-10f);
+          }
+        }
+        const int l0 = 2 * (j & 15), s = j % NR;
+        const int id0 = __shfl_sync(0xffffffffu, ids, l0), id1 = __shfl_sync(0xffffffffu, ids, l0 + 1);
+        const float4 f = make_float4(__shfl_sync(0xffffffffu, ks, l0), __shfl_sync(0xffffffffu, ks, l0 + 1),
+                                     __shfl_sync(0xffffffffu, vs, l0), __shfl_sync(0xffffffffu, vs, l0 + 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[s], ((j / NR) & 1) ^ 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* dst = smem + OFF_RAW + s * TILE;
+          meta[s] = f;
+          mbar_arrive_expect_tx(&raw_full[s], (id0 >= 0 ? 8192 : 0) + (id1 >= 0 ? 8192 : 0));
+          const int id[2] = {id0, id1};
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            if (id[p] >= 0) {
+              const long at = (static_cast<long>(id[p]) * a.pool.heads + kh) * 4096;
+              bulk_load(dst + p * 4096, a.pool.k + at, 4096, &raw_full[s]);
+              bulk_load(dst + 8192 + p * 4096, a.pool.v + at, 4096, &raw_full[s]);
+            }
+        }
+        ++issued;
+        __syncwarp();
+      }
+      if (lane == 0) {
+        if (!ok) {
+          if (status) atomicCAS(status, 0, kStatusTimeoutProducer);
+          *abort_flag = 1;
+        }
+        for (int j = max(0, issued - NR); j < issued; ++j) {  // copies in flight land
+          const long long t0 = clock64();
+          while (!mbar_try_wait(&raw_full[j % NR], (j / NR) & 1) && clock64() - t0 < kSpinLimitCycles / 8) {
+          }
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag);
+      const uint32_t sq = smem_u32(smem + OFF_Q);
+      auto issue_pv = [&](int i) -> bool {
+        if (!mbar_wait(&v_full[i % NS], (i / NS) & 1, abort_flag)) return false;
+        const uint32_t sv = smem_u32(smem + OFF_V + (i % NS) * TILE);
+        for (int t = 0; t < n_t; ++t) {
+          if (!mbar_wait(&p_full[t], i & 1, abort_flag)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)  // 16 tokens a step: page kk / 4
+            mma_bf16_ts(tmem + C_O + t * 64, tmem + C_P + t * 64 + kk * 8,
+                        make_sw128_desc(sv + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024), IDESC_PV,
+                        (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&o_done[t]);
+        }
+        mma_commit(&v_empty[i % NS]);
+        return true;
+      };
+      for (int j = 0; j < n && ok; ++j) {
+        ok = mbar_wait(&k_full[j % NS], (j / NS) & 1, abort_flag);
+        const uint32_t sk = smem_u32(smem + OFF_K + (j % NS) * TILE);
+        for (int t = 0; t < n_t && ok; ++t) {
+          if (j > 0) ok = mbar_wait(&s_free[t], (j - 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_bf16_ss(tmem + C_S + t * 128, make_sw128_desc(sq + t * TILE + kk * 32, 16, 1024),
+                        make_sw128_desc(sk + kk * 32, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
+          mma_commit(&s_full[t]);
+        }
+        if (ok) mma_commit(&k_empty[j % NS]);
+        if (ok && j > 0) ok = issue_pv(j - 1);
+      }
+      if (ok && n > 0) ok = issue_pv(n - 1);
+      if (!ok) {
+        if (status) atomicCAS(status, 0, kStatusTimeoutMma);
+        *abort_flag = 1;
+      }
+      mma_commit(drain);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(drain, 0) && clock64() - t0 < kSpinLimitCycles / 8) {
+      }
+    }
+    __syncwarp();
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ conversion
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    registers_split();
+    const int t = threadIdx.x - 128;
+    const int r = t >> 2, c = t & 3;  // row of 32, 16-byte piece of it; then rows r + 32 i
+    bool ok = true;
+    auto convert = [&](const uint8_t* raw, uint32_t dst, float f0, float f1, const uint32_t (&keep)[2][4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 mul = __float2half2_rn(i < 2 ? f0 : f1);
+        uint4 w = *reinterpret_cast<const uint4*>(raw + t * 16 + i * 2048);
+        const uint32_t ws[4] = {w.x & keep[i >> 1][0], w.y & keep[i >> 1][1], w.z & keep[i >> 1][2], w.w & keep[i >> 1][3]};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o[2 * k] = half2_scaled(ws[k] & 0xffff, mul);
+          o[2 * k + 1] = half2_scaled(ws[k] >> 16, mul);
+        }
+        const int R = r + 32 * i;
+        const uint32_t d = dst + R * 128;
+        st_shared_v4(d + (((2 * c) ^ (R & 7)) << 4), o[0], o[1], o[2], o[3]);
+        st_shared_v4(d + (((2 * c + 1) ^ (R & 7)) << 4), o[4], o[5], o[6], o[7]);
+      }
+    };
+    for (int j = 0; j < n; ++j) {
+      const int sr = j % NR, s = j % NS;
+      ok = mbar_wait(&raw_full[sr], (j / NR) & 1, abort_flag) &&
+           mbar_wait(&k_empty[s], ((j / NS) & 1) ^ 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      const float4 f = meta[sr];
+      const uint8_t* raw = smem + OFF_RAW + sr * TILE;
+      uint32_t keep[2][4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p)  // an absent page (factor 0) holds whatever the stage held
+#pragma unroll
+        for (int k = 0; k < 4; ++k) keep[p][k] = (p ? f.y : f.x) != 0.f ? ~0u : 0u;
+      convert(raw, smem_u32(smem + OFF_K + s * TILE), f.x, f.y, keep);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_full[s]);
+      // tokens that no row of the block sees stay out of P V whatever they hold
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int i = 2 * (j0 + j) + p;
+        const int key = pages.at(i) * kKvPage;
+        if (keep[p][0] && !(key + kKvPage <= all.hi && (key >= all.lo || key + kKvPage <= sinks))) {
+          for (int k = 0; k < 16; ++k)
+            if (!kv_visible(all, sinks, key + 16 * c + k)) keep[p][k >> 2] &= ~(0xffu << (8 * (k & 3)));
+        }
+      }
+      ok = mbar_wait(&v_empty[s], ((j / NS) & 1) ^ 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), f.z, f.w, keep);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&v_full[s]);
+        mbar_arrive(&raw_empty[sr]);
+      }
+    }
+    if (!ok) {
+      if (lane == 0 && status) atomicCAS(status, 0, kStatusTimeoutProducer);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+  } else {
+    // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    registers_split();
+    const int t = (warp - 8) >> 2, quad = warp & 3;
+    const int lr = quad * 32 + lane;
+    const int r = r0 + t * 128 + lr;
+    const bool active = t < n_t;  // of a second tile that is all padding nothing is computed
+    const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    // a padding row keeps zeros and the span of the last row: its result is not used
+    const KvSpan span = kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
+    float sl2;
+    {
+      uint4 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + (r / G) * a.q_st +
+                                 (kh * G + r % G) * a.q_sh;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = ld_global_v4(q + i * 8);
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = unpack_bf16(ws[k]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      const int e = row_exponent(amax);
+      const float down = __int_as_float((127 - e) << 23);
+      const uint32_t dst = smem_u32(smem + OFF_Q + t * TILE) + lr * 128;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = unpack_bf16(ws[k]);
+          h[k] = pack_half(f.x * down, f.y * down);
+        }
+        st_shared_v4(dst + ((i ^ (lr & 7)) << 4), h[0], h[1], h[2], h[3]);
+      }
+      // not zero: a masked score is -inf times it
+      sl2 = fmaxf(a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23) * k_ref, 1e-37f);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    if (active) {
+      for (int j = 0; j < n; ++j) {
+        if (!mbar_wait(&s_full[t], j & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float sf[128];
+        {
+          uint32_t x0[32], x1[32], x2[32], x3[32];
+          tmem_ld32(trow + C_S + t * 128, x0);
+          tmem_ld32(trow + C_S + t * 128 + 32, x1);
+          tmem_ld32(trow + C_S + t * 128 + 64, x2);
+          tmem_ld32(trow + C_S + t * 128 + 96, x3);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            sf[c] = __uint_as_float(x0[c]);
+            sf[32 + c] = __uint_as_float(x1[c]);
+            sf[64 + c] = __uint_as_float(x2[c]);
+            sf[96 + c] = __uint_as_float(x3[c]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int i = 2 * (j0 + j) + p;
+          const int key = i < pages.n ? pages.at(i) * kKvPage : 0x40000000;  // no page: no key
+          if (!(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= sinks))) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (!kv_visible(span, sinks, key + c)) sf[p * 64 + c] = -INFINITY;
+          }
+        }
+        float mp[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mp[i] = sf[i];
+#pragma unroll
+        for (int c = 8; c < 128; ++c) mp[c & 7] = fmaxf(mp[c & 7], sf[c]);
+        const float mx2 = sl2 * fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
+                                      fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
+        // the maximum moves only when a score passes it by 2^8: P <= 256, few rescales of O
+        float alpha = 1.f;
+        if (mx2 > m + kRescaleLog2) {
+          alpha = exp2f(m - mx2);
+          m = mx2;
+        }
+        const float use = m == -INFINITY ? 0.f : m;
+        float sp[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[64];
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const float p0 = exp2f(sf[c] * sl2 - use);
+          const float p1 = exp2f(sf[c + 1] * sl2 - use);
+          sp[c & 7] += p0;
+          sp[(c + 1) & 7] += p1;
+          pk[c >> 1] = pack_half(p0, p1);
+        }
+        l = l * alpha + (((sp[0] + sp[1]) + (sp[2] + sp[3])) + ((sp[4] + sp[5]) + (sp[6] + sp[7])));
+        if (j > 0) {
+          if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) {
+              uint32_t ov[16];
+              tmem_ld16(trow + C_O + t * 64 + c, ov);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+              tmem_st16(trow + C_O + t * 64 + c, ov);
+            }
+            tmem_wait_st();
+          }
+        }
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = pk[ch * 16 + i];
+          tmem_st16(trow + C_P + t * 64 + ch * 16, x);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+    }
+    if (!ok) {
+      if (lane == 0 && status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
+      *abort_flag = 1;
+    }
+    // every MMA is done: O may be read, and the operand tiles overwritten
+    float ov[64];
+    const bool done = __all_sync(0xffffffffu, mbar_wait(drain, 0, abort_flag) && ok);
+    if (done && active && n > 0) {
+      tc_fence_after();
+      uint32_t x0[32], x1[32];
+      tmem_ld32(trow + C_O + t * 64, x0);
+      tmem_ld32(trow + C_O + t * 64 + 32, x1);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        ov[c] = __uint_as_float(x0[c]) * v_ref;
+        ov[32 + c] = __uint_as_float(x1[c]) * v_ref;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 64; ++c) ov[c] = 0.f;
+    }
+    if (r >= rows) {
+      l = 0.f;
+#pragma unroll
+      for (int c = 0; c < 64; ++c) ov[c] = 0.f;
+    }
+    if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores
+    if (ranks > 1) {
+      if (done) {  // not while something may still read the operand tiles
+        const uint32_t dst = smem_u32(smem + OFF_RES) + (t * 128 + lr) * 256;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          st_shared_v4(dst + ((c ^ (lr & 15)) << 4), __float_as_uint(ov[4 * c]), __float_as_uint(ov[4 * c + 1]),
+                       __float_as_uint(ov[4 * c + 2]), __float_as_uint(ov[4 * c + 3]));
+        *reinterpret_cast<float2*>(smem + OFF_RES_ML + (t * 128 + lr) * 8) = make_float2(r < rows ? m : -INFINITY, l);
+      }
+    } else if (r < a.T * G) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int tok = r / G, h = kh * G + r % G;
+      const long at = (static_cast<long>(b) * a.T + tok) * a.H + h;
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64;
+#pragma unroll
+      for (int c = 0; c < 64; c += 8)
+        st_global_v4(o + c, pack_bf16(ov[c] * inv, ov[c + 1] * inv), pack_bf16(ov[c + 2] * inv, ov[c + 3] * inv),
+                     pack_bf16(ov[c + 4] * inv, ov[c + 5] * inv), pack_bf16(ov[c + 6] * inv, ov[c + 7] * inv));
+      if (a.lse) a.lse[(static_cast<long>(b) * a.H + h) * a.T + tok] = l == 0.f ? -INFINITY : m + __log2f(l);
+    }
+    __syncwarp();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (ranks > 1) {
+    // ---- each CTA of the cluster adds up its share of the rows, in rank order; 16 threads a
+    // row, 4 channels each
+    cluster_sync_all();
+    const uint32_t res = smem_u32(smem + OFF_RES), ml = smem_u32(smem + OFF_RES_ML);
+    for (int i = threadIdx.x + rank * kThreads; i < kRows * 16; i += ranks * kThreads) {
+      const int lr = i >> 4, c = i & 15, r = r0 + lr;
+      if (r >= a.T * G) break;
+      float top = -INFINITY, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < ranks; ++k) top = fmaxf(top, ld_cluster_v2(mapa_shared(ml + lr * 8, k)).x);
+      if (top != -INFINITY)
+        for (int k = 0; k < ranks; ++k) {
+          const float2 x = ld_cluster_v2(mapa_shared(ml + lr * 8, k));
+          const float4 y = ld_cluster_v4(mapa_shared(res + lr * 256 + ((c ^ (lr & 15)) << 4), k));
+          const float w = exp2f(x.x - top);
+          sum += w * x.y;
+          v.x += w * y.x;
+          v.y += w * y.y;
+          v.z += w * y.z;
+          v.w += w * y.w;
+        }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int tok = r / G, h = kh * G + r % G;
+      const long at = (static_cast<long>(b) * a.T + tok) * a.H + h;
+      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64 + c * 4) =
+          make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+      if (a.lse && c == 0)
+        a.lse[(static_cast<long>(b) * a.H + h) * a.T + tok] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its results
+  }
+}
+
+}  // namespace
+
+void kv_attend_tiles_launch(KvAttendArgs a, int dev, cudaStream_t stream) {
+  static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+  if (!(set.load() >> (dev & 63) & 1)) {
+    check_cuda(cudaFuncSetAttribute(kv_attend_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+               "cudaFuncSetAttribute(kv_attend_tiles)");
+    set.fetch_or(1ull << (dev & 63));
+  }
+  const int G = a.H / a.pool.heads;
+  const int tiles = (a.T * G + kRows - 1) / kRows;
+  const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
+  // Share an item's key tiles over the CTAs of a cluster: time ~ waves of CTAs x key tiles
+  // of one, the fewest CTAs with the smallest estimate; a CTA keeps 8 key tiles or more,
+  // some times the cost of its start and of the merge.
+  const int pairs = (a.max_tokens + 2 * kKvPage - 1) / (2 * kKvPage);
+  const long slots = num_sms(dev);
+  int ranks = 1;
+  double best = static_cast<double>((items + slots - 1) / slots);
+  for (int s = 2; s <= 8 && pairs / s >= 8; ++s) {
+    const double t = static_cast<double>((items * s + slots - 1) / slots) / s;
+    if (t < best - 1e-9) {
+      best = t;
+      ranks = s;
+    }
+  }
+  if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  a.cluster = ranks;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, tiles, device_status(dev)), "kv_attend_tiles launch");
+  count_launch();
+}
+
+}  // namespace ddb

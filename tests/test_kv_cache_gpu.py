@@ -133,7 +133,35 @@ CASES = [
     ([4000, 10], [1, 1], 1, 16, "token", 1, 0, 0),
     ([100], [1], 2, 1, "frame", 1000, 5, 5),
     ([900, 77], [300, 128], 1, 3, "frame", 64, 4, 2),
+    ([0, 3, 100], [257, 129, 65], 2, 1, "token", 1, 0, 0),
+    ([5000], [130], 1, 2, "token", 1, 0, 0),
+    ([6000, 40], [200, 3], 1, 1, "token", 1, 4500, 130),
+    ([4100], [700], 2, 4, "frame", 100, 7, 1),
+    ([8000], [65], 1, 1, "token", 1, 64, 1),
 ]
+
+
+def test_blocks_of_zeros_and_far_scales():
+    """Pages of zero keys, and pages whose scales lie far apart: zero keys still weigh."""
+    for T in (1, 100):
+        c = _cache(1, 1, 16)
+        seqs = c.add(1)
+        step = c.begin(seqs, 256)
+        k, v = _randn(1, 256, 1, 64), _randn(1, 256, 1, 64)
+        k[:, 64:128] = 0
+        v[:, 128:192] *= 2.0 ** -40
+        k[:, 192:] *= 2.0 ** 20
+        k[:, 192:, :, 1:] = 0
+        step.write(0, k, v)
+        step.commit()
+        step = c.begin(seqs, T)
+        step.write(0, _randn(1, T, 1, 64), _randn(1, T, 1, 64))
+        q = _randn(1, T, 1, 64)
+        q[..., 0] = 0
+        o, lse = step.attend(0, q, causal="token", return_lse=True)
+        kk, vv = c._values(0, c._seqs[seqs[0]], 256 + T)
+        ref, mean, rlse, mag = _oracle(kk, vv, q[0], T, "token", 1, 0, 0)
+        _check(o[0], lse[0], ref, mean, rlse, mag)
 
 
 @pytest.mark.parametrize("case", CASES)
@@ -204,8 +232,9 @@ def test_trimmed_sequence(T):
         step.attend(0, q, causal="token", window=150, sinks=3)
 
 
+@pytest.mark.parametrize("T", [4, 100])
 @pytest.mark.parametrize("magnitude", [2.0 ** -60, 2.0 ** 40])
-def test_attend_scales_exactly(magnitude):
+def test_attend_scales_exactly(magnitude, T):
     """Queries, keys and values of very small and very large magnitude: powers of two change
     nothing but the result's own."""
     lens, outs = [200], []
@@ -213,9 +242,9 @@ def test_attend_scales_exactly(magnitude):
         torch.manual_seed(3)
         c = _cache(1, 1, 8)
         seqs = _fill(c, lens, scale=f)
-        step = c.begin(seqs, 4)
-        step.write(0, _randn(1, 4, 1, 64, scale=f), _randn(1, 4, 1, 64, scale=f))
-        outs.append(step.attend(0, _randn(1, 4, 2, 64, scale=1 / f), causal="token"))
+        step = c.begin(seqs, T)
+        step.write(0, _randn(1, T, 1, 64, scale=f), _randn(1, T, 1, 64, scale=f))
+        outs.append(step.attend(0, _randn(1, T, 2, 64, scale=1 / f), causal="token"))
     assert torch.equal(outs[0].float() * magnitude, outs[1].float())
 
 
