@@ -41,7 +41,7 @@ constexpr int OFF_K = OFF_Q + 2 * TILE;
 constexpr int OFF_V = OFF_K + NS * TILE;
 constexpr int OFF_RAW = OFF_V + NS * TILE;   // per stage: keys of both pages, values of both
 constexpr int OFF_BAR = OFF_RAW + NR * TILE;
-constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 8 + 1;
+constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 10 + 1;
 constexpr int OFF_META = OFF_BAR + N_BARS * 8;
 constexpr int OFF_MISC = OFF_META + NR * 16;
 constexpr int SMEM_BYTES = OFF_MISC + 32;
@@ -51,6 +51,7 @@ constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
 static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
 constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kHandOver = 3;  // quarters of a row's exponentials after which the other tile may begin
 
 // kind::f16 with fp16 A and B, fp32 D, both K-major
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
@@ -105,7 +106,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_free = s_full + 2;
   uint64_t* p_full = s_full + 4;
   uint64_t* o_done = s_full + 6;
-  uint64_t* drain = s_full + 8;
+  uint64_t* turn = s_full + 8;
+  uint64_t* drain = s_full + 10;
   float4* meta = reinterpret_cast<float4*>(smem + OFF_META);  // per stage: key, value factors of both pages
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
@@ -153,6 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s_free[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
+      mbar_init(&turn[t], 4);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -249,48 +252,64 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
-      bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag);
-      const uint32_t sq = smem_u32(smem + OFF_Q);
+      // The whole warp walks the loop, so that addresses and descriptors stay in uniform
+      // registers, where the instruction takes them; one elected lane issues.
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+      };
+      bool ok = n == 0 || wait(q_full, 0);
+      const uint64_t dq = make_sw128_desc(smem_u32(smem + OFF_Q), 16, 1024);
+      const uint64_t dk = make_sw128_desc(smem_u32(smem + OFF_K), 16, 1024);
+      const uint64_t dv = make_sw128_desc(smem_u32(smem + OFF_V), 16, 1024);
       auto issue_pv = [&](int i) -> bool {
-        if (!mbar_wait(&v_full[i % NS], (i / NS) & 1, abort_flag)) return false;
-        const uint32_t sv = smem_u32(smem + OFF_V + (i % NS) * TILE);
+        if (!wait(&v_full[i % NS], (i / NS) & 1)) return false;
+        const uint64_t d = dv + (i % NS) * (TILE >> 4);
         for (int t = 0; t < n_t; ++t) {
-          if (!mbar_wait(&p_full[t], i & 1, abort_flag)) return false;
+          if (!wait(&p_full[t], i & 1)) return false;
           tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // 16 tokens a step: page kk / 4
-            mma_bf16_ts(tmem + C_O + t * 64, tmem + C_P + t * 64 + kk * 8,
-                        make_sw128_desc(sv + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024), IDESC_PV,
-                        (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&o_done[t]);
+            for (int kk = 0; kk < 8; ++kk)  // 16 tokens a step: page kk / 4
+              mma_bf16_ts(tmem + C_O + t * 64, tmem + C_P + t * 64 + kk * 8, d + (kk >> 2) * 512 + (kk & 3) * 2, IDESC_PV,
+                          (i > 0 || kk > 0) ? 1u : 0u);
+            mma_commit(&o_done[t]);
+          }
+          __syncwarp();
         }
-        mma_commit(&v_empty[i % NS]);
+        if (elect_one()) mma_commit(&v_empty[i % NS]);
         return true;
       };
       for (int j = 0; j < n && ok; ++j) {
-        ok = mbar_wait(&k_full[j % NS], (j / NS) & 1, abort_flag);
-        const uint32_t sk = smem_u32(smem + OFF_K + (j % NS) * TILE);
+        ok = wait(&k_full[j % NS], (j / NS) & 1);
+        const uint64_t d = dk + (j % NS) * (TILE >> 4);
         for (int t = 0; t < n_t && ok; ++t) {
-          if (j > 0) ok = mbar_wait(&s_free[t], (j - 1) & 1, abort_flag);
+          if (j > 0) ok = wait(&s_free[t], (j - 1) & 1);
           if (!ok) break;
           tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_bf16_ss(tmem + C_S + t * 128, make_sw128_desc(sq + t * TILE + kk * 32, 16, 1024),
-                        make_sw128_desc(sk + kk * 32, 16, 1024), IDESC_S, kk > 0 ? 1u : 0u);
-          mma_commit(&s_full[t]);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_bf16_ss(tmem + C_S + t * 128, dq + t * (TILE >> 4) + kk * 2, d + kk * 2, IDESC_S, kk > 0 ? 1u : 0u);
+            mma_commit(&s_full[t]);
+          }
+          __syncwarp();
         }
-        if (ok) mma_commit(&k_empty[j % NS]);
+        if (ok && elect_one()) mma_commit(&k_empty[j % NS]);
+        __syncwarp();
         if (ok && j > 0) ok = issue_pv(j - 1);
       }
       if (ok && n > 0) ok = issue_pv(n - 1);
-      if (!ok) {
-        if (status) atomicCAS(status, 0, kStatusTimeoutMma);
-        *abort_flag = 1;
+      if (lane == 0) {
+        if (!ok) {
+          if (status) atomicCAS(status, 0, kStatusTimeoutMma);
+          *abort_flag = 1;
+        }
       }
-      mma_commit(drain);
+      __syncwarp();
+      if (elect_one()) mma_commit(drain);
+      __syncwarp();
       const long long t0 = clock64();
       while (!mbar_try_wait(drain, 0) && clock64() - t0 < kSpinLimitCycles / 8) {
       }
@@ -474,17 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mx2;
         }
         const float use = m == -INFINITY ? 0.f : m;
-        float sp[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t pk[64];
-#pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float p0 = exp2f(sf[c] * sl2 - use);
-          const float p1 = exp2f(sf[c + 1] * sl2 - use);
-          sp[c & 7] += p0;
-          sp[(c + 1) & 7] += p1;
-          pk[c >> 1] = pack_half(p0, p1);
-        }
-        l = l * alpha + (((sp[0] + sp[1]) + (sp[2] + sp[3])) + ((sp[4] + sp[5]) + (sp[6] + sp[7])));
+        // P V of the last key tile is done: O may be rescaled and P overwritten
         if (j > 0) {
           if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) {
             ok = false;
@@ -501,16 +510,33 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
               tmem_st16(trow + C_O + t * 64 + c, ov);
             }
-            tmem_wait_st();
           }
         }
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint32_t x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = pk[ch * 16 + i];
-          tmem_st16(trow + C_P + t * 64 + ch * 16, x);
+        // The tiles take turns at their exponentials, which one tile alone issues near the
+        // unit's full rate: in step, both would leave it idle during their loads and maxima.
+        if (n_t == 2 && (t == 1 || j > 0) && !mbar_wait(&turn[1 - t], (j - 1 + t) & 1, abort_flag)) {
+          ok = false;
+          break;
         }
+        float sp[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {  // stored 32 columns at a time, to hold few registers
+          if (ch == kHandOver) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&turn[t]);
+          }
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float p0 = exp2f(sf[ch * 32 + c] * sl2 - use);
+            const float p1 = exp2f(sf[ch * 32 + c + 1] * sl2 - use);
+            sp[c & 7] += p0;
+            sp[(c + 1) & 7] += p1;
+            pk[c >> 1] = pack_half(p0, p1);
+          }
+          tmem_st16(trow + C_P + t * 64 + ch * 16, pk);
+        }
+        l = l * alpha + (((sp[0] + sp[1]) + (sp[2] + sp[3])) + ((sp[4] + sp[5]) + (sp[6] + sp[7])));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -620,32 +646,43 @@ void kv_attend_tiles_launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   const int G = a.H / a.pool.heads;
   const int tiles = (a.T * G + kRows - 1) / kRows;
   const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
-  // Share an item's key tiles over the CTAs of a cluster: time ~ waves of CTAs x key tiles
-  // of one, the fewest CTAs with the smallest estimate; a CTA keeps 8 key tiles or more,
-  // some times the cost of its start and of the merge.
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  // Share an item's key tiles over the CTAs of a cluster: time ~ waves of clusters x key
+  // tiles of one CTA, the fewest CTAs with the smallest estimate; a CTA keeps 8 key tiles
+  // or more, some times the cost of its start and of the merge. How many clusters of a
+  // size run at once is the device's to say: of 3 CTAs only 45 do on 148 SMs (the GPCs'
+  // SMs are no multiple), so 96 of them take three waves, not two.
   const int pairs = (a.max_tokens + 2 * kKvPage - 1) / (2 * kKvPage);
-  const long slots = num_sms(dev);
+  static std::atomic<int> fits[64][9];
   int ranks = 1;
-  double best = static_cast<double>((items + slots - 1) / slots);
-  for (int s = 2; s <= 8 && pairs / s >= 8; ++s) {
-    const double t = static_cast<double>((items * s + slots - 1) / slots) / s;
-    if (t < best - 1e-9) {
+  double best = 0.;
+  for (int s = 1; s <= 8 && (s == 1 || pairs / s >= 8); ++s) {
+    int slots = s == 1 ? num_sms(dev) : fits[dev & 63][s].load();
+    if (slots == 0) {
+      cfg.gridDim = dim3(s);
+      attr[0].val.clusterDim.x = s;
+      cfg.numAttrs = 1;
+      check_cuda(cudaOccupancyMaxActiveClusters(&slots, kv_attend_tiles, &cfg), "cudaOccupancyMaxActiveClusters");
+      slots = std::max(slots, 1);
+      fits[dev & 63][s].store(slots);
+    }
+    const double t = static_cast<double>((items + slots - 1) / slots) / s;
+    if (s == 1 || t < best - 1e-9) {
       best = t;
       ranks = s;
     }
   }
   if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
   a.cluster = ranks;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = SMEM_BYTES;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
   check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, tiles, device_status(dev)), "kv_attend_tiles launch");
   count_launch();
