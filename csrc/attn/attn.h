@@ -106,7 +106,11 @@ void attn_bwd_with_status(const AttnBwdArgs& a, int* status, cudaStream_t s);
 // delta[b,h,t] = sum_d dO * O over each head's 64 columns
 void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long lddo,
                     int do_col, float* delta, int B, int H, int Tq, long rows_per_b,
-                    cudaStream_t s, long delta_ld = 0);  // 0: Tq floats between delta rows
+                    cudaStream_t s);
+// the same with delta rows delta_ld floats apart, clearing the contiguous dQ accumulator
+// [B * Tq][H * 64] on the way
+void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
+                         int B, int H, int Tq, cudaStream_t s);
 // dq (bf16, optionally rotated back by a rotary table) from the fp32 accumulator
 void attn_dq_finalize(const float* dq_acc, long ld_acc, void* dq, long lddq, int dq_col,
                       int rows, int H, const float2* rope_tab, int rows_per_seq,

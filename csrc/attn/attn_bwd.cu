@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int o_col,
                              const __nv_bfloat16* __restrict__ dout, long lddo, int do_col,
                              float* __restrict__ delta, int B, int H, int Tq, long rows_per_b,
-                             long delta_ld) {
+                             long delta_ld, float* __restrict__ clear) {
   const int lane = threadIdx.x & 31;
   const long row = blockIdx.x * 8L + (threadIdx.x >> 5);
   if (row >= static_cast<long>(B) * Tq) return;
@@ -624,6 +624,11 @@ __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int 
     const int c = base + lane;
     float s = 0.f;
     if (c < chunks) {
+      if (clear) {  // 8 columns of the row's dQ accumulator
+        float* z = clear + (row * H * 64 + c * 8);
+        st_global_v4(z, 0, 0, 0, 0);
+        st_global_v4(z + 4, 0, 0, 0, 0);
+      }
       uint4 ov = ld_global_v4(o + grow * ldo + o_col + c * 8);
       uint4 dv = ld_global_v4(dout + grow * lddo + do_col + c * 8);
       uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w};
@@ -750,13 +755,23 @@ void attn_window_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
 }
 
 void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long lddo, int do_col,
-                    float* delta, int B, int H, int Tq, long rows_per_b, cudaStream_t s, long delta_ld) {
+                    float* delta, int B, int H, int Tq, long rows_per_b, cudaStream_t s) {
   const long rows = static_cast<long>(B) * Tq;
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(o), ldo, o_col,
-      reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b,
-      delta_ld ? delta_ld : Tq);
+      reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b, Tq,
+      nullptr);
   count_launch();
+}
+
+void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
+                         int B, int H, int Tq, cudaStream_t s) {
+  const long rows = static_cast<long>(B) * Tq;
+  delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
+      reinterpret_cast<const __nv_bfloat16*>(o), H * 64L, 0, reinterpret_cast<const __nv_bfloat16*>(dout),
+      H * 64L, 0, delta, B, H, Tq, Tq, delta_ld, dq_acc);
+  count_launch();
+  check_cuda(cudaGetLastError(), "delta_kernel launch");
 }
 
 void attn_dq_finalize(const float* dq_acc, long ld_acc, void* dq, long lddq, int dq_col, int rows,

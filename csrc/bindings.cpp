@@ -3,6 +3,7 @@
 // kernel never receives arguments it was not written for.
 #include <torch/extension.h>
 
+#include <cmath>
 #include <map>
 #include <utility>
 #include <ATen/cuda/CUDAContext.h>
@@ -1436,21 +1437,44 @@ ddb::AttnArgs window_args(const torch::Tensor& q, const torch::Tensor& k, const 
   return a;
 }
 
-void check_window_lse(const torch::Tensor& t, const char* name, const ddb::AttnArgs& a) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.dim() == 3 && t.size(0) == a.B &&
-                  t.size(1) == a.H && t.size(2) >= a.Tq && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must be contiguous fp32 [B, H, >= T]");
+// The mask and positions of a call, checked: the kernels' codes and units.
+struct WindowMask {
+  int64_t causal, unit, window, sinks, q_pos, kv_pos;
+  double scale;
+};
+
+WindowMask window_mask(const std::string& causal, int64_t tokens_per_frame, int64_t window, int64_t sinks, int64_t q_pos,
+                       int64_t kv_pos, double scale, int64_t T, int64_t S) {
+  const int64_t limit = 1 << 30;  // positions stay below
+  TORCH_CHECK_VALUE(causal == "frame" || causal == "token" || causal == "none", "causal must be frame, token or none, got '", causal, "'");
+  TORCH_CHECK_VALUE(tokens_per_frame >= 1 && window >= 0 && sinks >= 0 && q_pos >= 0 && kv_pos >= 0,
+                    "tokens_per_frame must be positive; window, sinks and offsets not negative");
+  TORCH_CHECK_VALUE(causal != "none" || (window == 0 && sinks == 0), "a window needs causal frame or token");
+  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+  TORCH_CHECK_VALUE(q_pos <= limit - T && kv_pos <= limit - S, "positions must stay below ", limit);
+  const int64_t unit = causal == "frame" ? tokens_per_frame : 1;
+  TORCH_CHECK_VALUE(unit <= (1 << 24), "at most 2^24 tokens per frame");
+  // a window or run of sinks past every position is the same as all of them
+  return {causal == "none" ? ddb::kCausalNone : ddb::kCausalFrame, unit, window <= limit / unit ? window : 0,
+          std::min(sinks, limit / unit) * unit, q_pos, kv_pos, scale};
 }
 
-void attn_window_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor lse,
-                     int64_t causal, int64_t unit, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
-                     double scale) {
-  auto a = window_args(q, k, v, causal, unit, window, sinks, q_pos, kv_pos, scale);
-  check_bf16(o, "o");
-  TORCH_CHECK(o.is_contiguous() && o.sizes() == q.sizes() && o.device() == q.device() &&
-                  reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0, "o must be contiguous and like q");
-  check_window_lse(lse, "lse", a);
+bool tma_rows(const torch::Tensor& t) {
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) != 1 && (t.stride(i) <= 0 || t.stride(i) % 8 != 0)) return false;
+  return true;
+}
+// `t` as the kernels read it (a copy if its strides or alignment do not fit)
+torch::Tensor tma_ready(const torch::Tensor& t) { return tma_rows(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+// o [B, T, H, 64], and lse [B, H, T rounded up to 128] (log2 domain)
+std::vector<torch::Tensor> attn_window_fwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                           const WindowMask& m) {
+  auto a = window_args(q, k, v, m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos, m.scale);
   const c10::cuda::CUDAGuard guard(q.device());
+  auto o = torch::empty({a.B, a.Tq, a.H, 64}, q.options());
+  auto lse = torch::empty({a.B, a.H, (a.Tq + 127) / 128 * 128}, q.options().dtype(torch::kFloat32));
   a.o = o.data_ptr(); a.ldo = a.H * 64;
   a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
   const int splits = g_attn_kv_splits > 0 ? static_cast<int>(g_attn_kv_splits) : ddb::attn_window_kv_splits(a);
@@ -1465,51 +1489,121 @@ void attn_window_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
     a.lse_part = a.o_part + oe;
   }
   ddb::attn_window_fwd(a, stream());
+  return {o, lse};
 }
 
-// dk, dv: [B, S, H, 64] views whose rows lie at one stride over the samples, heads 64 apart
-void window_grad_rows(const torch::Tensor& t, const char* name, const ddb::AttnArgs& a, const torch::Tensor& q, long& ld) {
+// [B, rows, H, 64] views of a gradient whose rows lie at one stride over the samples, heads 64 apart
+void window_grad_rows(const torch::Tensor& t, const char* name, const torch::Tensor& like, long& ld) {
   check_bf16(t, name);
-  TORCH_CHECK(t.dim() == 4 && t.size(0) == a.B && t.size(1) == a.S && t.size(2) == a.H && t.size(3) == 64 &&
-                  t.device() == q.device(), name, " must be like k");
-  ld = t.size(1) > 1 ? t.stride(1) : t.size(0) > 1 ? t.stride(0) : a.H * 64L;
-  TORCH_CHECK(t.stride(3) == 1 && (t.size(2) == 1 || t.stride(2) == 64) && ld >= a.H * 64L && ld % 8 == 0 &&
-                  (t.size(0) == 1 || t.stride(0) == ld * a.S) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+  const int64_t H = like.size(2);
+  TORCH_CHECK(t.dim() == 4 && t.sizes() == like.sizes() && t.device() == like.device(), name, " has another shape or device");
+  ld = t.size(1) > 1 ? t.stride(1) : t.size(0) > 1 ? t.stride(0) : H * 64;
+  TORCH_CHECK(t.stride(3) == 1 && (H == 1 || t.stride(2) == 64) && ld >= H * 64 && ld % 8 == 0 &&
+                  (t.size(0) == 1 || t.stride(0) == ld * t.size(1)) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               name, " must be rows of contiguous heads at one 16-byte aligned stride");
 }
 
-void attn_window_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
-                     torch::Tensor lse, torch::Tensor delta, torch::Tensor dq_acc, torch::Tensor dk, torch::Tensor dv,
-                     int64_t causal, int64_t unit, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
-                     double scale) {
+// Gradients into dq, dk, dv. dQ is summed over the key tiles in fp32 in no fixed order: equal
+// calls may differ in its last fp32 bits before the rounding to bf16.
+void attn_window_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
+                     const torch::Tensor& lse, const torch::Tensor& grad, const WindowMask& m, const torch::Tensor& dq,
+                     const torch::Tensor& dk, const torch::Tensor& dv) {
   ddb::AttnBwdArgs g;
-  g.f = window_args(q, k, v, causal, unit, window, sinks, q_pos, kv_pos, scale);
+  g.f = window_args(q, k, v, m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos, m.scale);
   auto& a = g.f;
-  check_window_lse(lse, "lse", a);
-  check_window_lse(delta, "delta", a);
-  TORCH_CHECK(lse.size(2) == delta.size(2) && lse.size(2) >= (a.Tq + 127) / 128 * 128 && lse.size(2) % 4 == 0 &&
-                  lse.device() == q.device() && delta.device() == q.device(),
-              "lse and delta rows must hold whole tiles of 128 queries");
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == torch::kFloat32 && lse.is_contiguous() && lse.dim() == 3 &&
+                  lse.size(0) == a.B && lse.size(1) == a.H && lse.size(2) == (a.Tq + 127) / 128 * 128 && lse.device() == q.device(),
+              "lse must be the forward's [B, H, T rounded up to 128]");
+  const auto dout = grad.is_contiguous() && reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0 ? grad : grad.clone(at::MemoryFormat::Contiguous);
   for (const auto* t : {&o, &dout})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->is_contiguous() && t->sizes() == q.sizes() &&
                     t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "o and dout must be contiguous bf16 and like q");
-  TORCH_CHECK(dq_acc.is_cuda() && dq_acc.scalar_type() == torch::kFloat32 && dq_acc.is_contiguous() &&
-                  dq_acc.numel() == q.numel() && dq_acc.device() == q.device(), "dq_acc must be contiguous fp32 and like q");
+                "o and its gradient must be contiguous bf16 and like q");
   const c10::cuda::CUDAGuard guard(q.device());
+  long ld_dq = 0;
+  window_grad_rows(dq, "dq", q, ld_dq);
+  window_grad_rows(dk, "dk", k, g.lddk);
+  window_grad_rows(dv, "dv", v, g.lddv);
+  auto delta = torch::empty_like(lse);
+  auto acc = torch::empty({static_cast<int64_t>(a.B) * a.Tq, a.H * 64L}, lse.options());
   a.o = o.data_ptr(); a.ldo = a.H * 64;
   a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
   g.dout = dout.data_ptr();
   g.do_sh = 64; g.do_st = a.H * 64L; g.do_sb = g.do_st * a.Tq;
   g.delta = delta.data_ptr<float>();
-  g.dq_acc = dq_acc.data_ptr<float>(); g.ld_dqacc = a.H * 64;
-  window_grad_rows(dk, "dk", a, q, g.lddk);
-  window_grad_rows(dv, "dv", a, q, g.lddv);
+  g.dq_acc = acc.data_ptr<float>(); g.ld_dqacc = a.H * 64;
   g.dk = dk.data_ptr();
   g.dv = dv.data_ptr();
-  ddb::attn_bwd_delta(o.data_ptr(), a.ldo, 0, dout.data_ptr(), a.ldo, 0, delta.data_ptr<float>(), a.B, a.H, a.Tq, a.Tq,
-                      stream(), lse.size(2));
+  ddb::attn_window_prepare(o.data_ptr(), dout.data_ptr(), delta.data_ptr<float>(), lse.size(2), acc.data_ptr<float>(), a.B,
+                           a.H, a.Tq, stream());
   ddb::attn_window_bwd(g, stream());
+  ddb::attn_dq_finalize(acc.data_ptr<float>(), a.H * 64L, dq.data_ptr(), ld_dq, 0, a.B * a.Tq, a.H, nullptr, a.Tq, 0, stream());
+}
+
+class WindowAttention : public torch::autograd::Function<WindowAttention> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& q0,
+                                                const torch::Tensor& k0, const torch::Tensor& v0, const WindowMask& m) {
+    const auto q = tma_ready(q0), k = tma_ready(k0), v = tma_ready(v0);
+    auto out = attn_window_fwd(q, k, v, m);
+    ctx->save_for_backward({q, k, v, out[0], out[1]});
+    ctx->saved_data["mask"] = std::vector<int64_t>{m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos};
+    ctx->saved_data["scale"] = m.scale;
+    ctx->set_materialize_grads(false);
+    auto lse = out[1].narrow(2, 0, q.size(1));
+    ctx->mark_non_differentiable({lse});
+    return {out[0], lse};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    const auto s = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["mask"].toIntVector();
+    const WindowMask m{n[0], n[1], n[2], n[3], n[4], n[5], ctx->saved_data["scale"].toDouble()};
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    auto dq = torch::empty(s[0].sizes(), s[0].options()), dk = torch::empty(s[1].sizes(), s[1].options()),
+         dv = torch::empty(s[2].sizes(), s[2].options());
+    attn_window_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(torch::kBFloat16), m, dq, dk, dv);
+    return {dq, dk, dv, torch::Tensor()};
+  }
+};
+
+// A backward pass that is captured while an eager graph of the same leaf is alive ends the
+// process inside autograd: the leaf's accumulation node belongs to the default stream.
+void refuse_eager_leaf(const torch::Tensor& t) {
+  if (!t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto s = node->stream();
+  TORCH_CHECK(!s || c10::cuda::CUDAStream(*s).stream() != nullptr,
+              "an autograd graph made on the default stream still uses this leaf: drop it before capturing a backward "
+              "pass, or warm up on another stream");
+}
+
+std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                            const std::string& causal, int64_t tokens_per_frame, int64_t window,
+                                            int64_t sinks, int64_t q_pos, int64_t kv_pos, c10::optional<double> scale) {
+  TORCH_CHECK_VALUE(q.scalar_type() == torch::kBFloat16, "window_attention takes bfloat16 on CUDA, got ", q.scalar_type());
+  const auto m = window_mask(causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale ? *scale : 0.125, q.size(1), k.size(1));
+  TORCH_CHECK_VALUE(q.size(1) <= 65536 * 64, "at most ", 65536 * 64, " queries per sample");
+  if (at::GradMode::is_enabled()) {
+    const c10::cuda::CUDAGuard guard(q.device());
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
+      for (const auto* t : {&q, &k, &v}) refuse_eager_leaf(*t);
+  }
+  return WindowAttention::apply(q, k, v, m);
+}
+
+std::vector<torch::Tensor> attn_window_fwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                              const std::string& causal, int64_t tokens_per_frame, int64_t window,
+                                              int64_t sinks, double scale) {
+  return attn_window_fwd(q, k, v, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)));
+}
+void attn_window_bwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
+                        const torch::Tensor& lse, const torch::Tensor& grad, const std::string& causal,
+                        int64_t tokens_per_frame, int64_t window, int64_t sinks, double scale, const torch::Tensor& dq,
+                        const torch::Tensor& dk, const torch::Tensor& dv) {
+  attn_window_bwd(q, k, v, o, lse, grad, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)),
+                  dq, dk, dv);
 }
 
 // ---------------------------------------------------------------- 8-bit paged key/value cache
@@ -1696,8 +1790,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("q_pos_offset"), py::arg("kv_pos_offset"), py::arg("scale"), py::arg("kv_qtiles"),
         py::arg("kv_qmask"), py::arg("kv_count"), py::arg("debug_flags") = 0,
         py::arg("trace") = py::none(), py::arg("trace_cta") = 0);
-  m.def("attn_window_fwd", &attn_window_fwd, "tcgen05 attention over a window and the first tokens, forward");
-  m.def("attn_window_bwd", &attn_window_bwd, "tcgen05 attention over a window and the first tokens, backward");
+  m.def("window_attention", &window_attention, "differentiable attention over a window and the first tokens");
+  m.def("attn_window_fwd", &attn_window_fwd_py, "its forward, for callers with a backward of their own");
+  m.def("attn_window_bwd", &attn_window_bwd_py, "its backward, into given gradients");
   m.def("kv_cache_write", &kv_cache_write, "tokens into the pages of an 8-bit key/value cache");
   m.def("kv_cache_attend", &kv_cache_attend, "attention over an 8-bit paged key/value cache");
   m.def("kv_cache_copy_pages", &kv_cache_copy_pages, "copy cache pages in every layer");

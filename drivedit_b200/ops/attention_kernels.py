@@ -23,7 +23,6 @@ import torch
 
 from ..layers.sla import SLAConfig, block_valid_mask, n_selected, sla_linear_reference
 from ._ext import ext
-from .window_attention import mask_args, window_backward, window_forward
 
 CAUSAL = {"none": 0, "frame": 1, "token": 2}
 
@@ -180,11 +179,9 @@ def _heads(qkv, bc):
     return v[:, :, 0], v[:, :, 1], v[:, :, 2]
 
 
-def _window_mask(bc):
-    unit = bc.tpf if bc.causal == "frame" else 1
+def _window_args(bc):
     per = 1 if bc.causal == "frame" else bc.tpf
-    return mask_args(bc.causal, unit, bc.window_frames * per, bc.sink_frames * per, 0, 0, 1.0 / math.sqrt(bc.Dh),
-                     bc.T, bc.T)
+    return bc.causal, bc.tpf, bc.window_frames * per, bc.sink_frames * per, 1.0 / math.sqrt(bc.Dh)
 
 
 def attention_fwd_kernel(qkv: torch.Tensor, bc):
@@ -199,7 +196,7 @@ def attention_fwd_kernel(qkv: torch.Tensor, bc):
     o_lin = None
     lists = (None, None, None)
     if bc.window_frames and bc.attn_mode == "dense":
-        o4, lse = window_forward(*_heads(qkv, bc), _window_mask(bc))
+        o4, lse = ext().attn_window_fwd(*_heads(qkv, bc), *_window_args(bc))
         return o4.view(M, d), None, lse, None
     if bc.attn_mode == "sla":
         plan = sla_plan_kernel(qkv, B, T, H, bc.sla_cfg, bc.tpf, bc.causal)
@@ -217,8 +214,8 @@ def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc):
     dev = qkv.device
     if bc.window_frames and bc.attn_mode == "dense":
         dqkv = torch.empty(M, 3 * d, device=dev, dtype=torch.bfloat16)
-        window_backward(*_heads(qkv, bc), o.view(B, T, H, 64), lse, do.view(B, T, H, 64), _window_mask(bc),
-                        *_heads(dqkv, bc))
+        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), lse, do.view(B, T, H, 64), *_window_args(bc),
+                              *_heads(dqkv, bc))
         return dqkv
     delta = torch.empty(B * H * T, device=dev, dtype=torch.float32)
     ext().attn_delta(o, do, delta, 0, 0, B, H, T, T)
