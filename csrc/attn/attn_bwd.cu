@@ -256,6 +256,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
+  } else if (WIN && warp == 1) {
+    // ------------------------------------------------------------ MMA issuer, windowed mode
+    // The whole warp walks the loop, so that addresses and descriptors stay in uniform
+    // registers, where the instruction takes them; one elected lane issues.
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+    };
+    bool ok = wait(kv_full, 0);
+    // operands read K-major (rows of 64 channels) and MN-major (as the transposed factor)
+    const uint64_t dk = make_sw128_desc(smem_u32(smem + OFF_K), 16, 1024);
+    const uint64_t dv = make_sw128_desc(smem_u32(smem + OFF_V), 16, 1024);
+    const uint64_t dq = make_sw128_desc(smem_u32(smem + OFF_Q), 16, 1024);
+    const uint64_t ddo = make_sw128_desc(smem_u32(smem + OFF_DO), 16, 1024);
+    const uint64_t dkt = make_sw128_desc(smem_u32(smem + OFF_K), 8192, 1024);
+    const uint64_t dqt = make_sw128_desc(smem_u32(smem + OFF_Q), 8192, 1024);
+    const uint64_t ddot = make_sw128_desc(smem_u32(smem + OFF_DO), 8192, 1024);
+    const uint64_t dst = make_sw128_desc(smem_u32(smem + OFF_DST), 16, 1024);
+    const uint64_t dstt = make_sw128_desc(smem_u32(smem + OFF_DST), TILE, 1024);
+    auto issue_grads = [&](int i) -> bool {
+      const int pb = i & 1, s = i % NS;
+      if (!wait(&ds_full[pb], (i >> 1) & 1) || (i > 0 && !wait(dq_free, (i - 1) & 1))) return false;
+      tc_fence_after();
+      const uint64_t so = s * (TILE >> 4), po = pb * 2 * (TILE >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO
+          mma_bf16_ts(tmem + C_DV, tmem + C_PT + kk * 8, ddot + so + kk * 128, IDESC_GRAD, (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(pt_tfree);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dK += dS^T Q
+          mma_bf16_ss(tmem + C_DK, dst + po + (kk >> 2) * (TILE >> 4) + (kk & 3) * 2, dqt + so + kk * 128, IDESC_GRAD,
+                      (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&qd_empty[s]);  // Q and dO of this stage are no longer read
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // dQ = dS K over the tile's 128 keys
+          mma_bf16_ss(tmem + C_DQ, dstt + po + kk * 128, dkt + kk * 128, IDESC_DQ, kk > 0 ? 1u : 0u);
+        mma_commit(&ds_empty[pb]);
+        mma_commit(dq_full);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int j = 0; j < nq && ok; ++j) {
+      const int s = j % NS;
+      ok = wait(&qd_full[s], (j / NS) & 1) && (j == 0 || wait(s_free, (j - 1) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t so = s * (TILE >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          mma_bf16_ss(tmem + C_S, dk + kk * 2, dq + so + kk * 2, IDESC_SS, kk > 0 ? 1u : 0u);
+          mma_bf16_ss(tmem + C_DP, dv + kk * 2, ddo + so + kk * 2, IDESC_SS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(s_full);
+      }
+      __syncwarp();
+      if (j > 0) ok = issue_grads(j - 1);
+    }
+    if (ok && nq > 0) ok = issue_grads(nq - 1);
+    if (!ok && lane == 0) {
+      if (status) atomicCAS(status, 0, kStatusTimeoutMma);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+    if (elect_one()) mma_commit(drain);
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!mbar_try_wait(drain, 0) && clock64() - t0 < kSpinLimitCycles / 8) {
+    }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {

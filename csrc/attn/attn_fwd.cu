@@ -254,6 +254,57 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
+  } else if (WIN && warp == 1) {
+    // The whole warp walks the loop, so that addresses and descriptors stay in uniform
+    // registers, where the instruction takes them; one elected lane issues.
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+    };
+    bool ok = wait(q_full, 0);
+    const uint64_t dq = make_sw128_desc(smem_u32(sQ), 16, 1024);
+    const uint64_t dk = make_sw128_desc(smem_u32(smem + OFF_K), 16, 1024);
+    const uint64_t dv = make_sw128_desc(smem_u32(smem + OFF_V), 8192, 1024);
+    auto issue_pv = [&](int i) -> bool {
+      if (!wait(p_full, i & 1) || !wait(&v_full[i % NS], (i / NS) & 1)) return false;
+      tc_fence_after();
+      const uint64_t d = dv + (i % NS) * (TILE_BYTES >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)  // A = P from TMEM: 16 keys per 8 columns
+          mma_bf16_ts(tmem + O_COL, tmem + P_COL + kk * 8, d + kk * 128, IDESC_PV, (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&v_empty[i % NS]);
+        mma_commit(o_done);
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int j = 0; j < ntiles && ok; ++j) {
+      const int s = j % NS;
+      ok = wait(&k_full[s], (j / NS) & 1) && (j == 0 || wait(s_free, (j - 1) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t d = dk + s * (TILE_BYTES >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_bf16_ss(tmem + S_COL, dq + kk * 2, d + kk * 2, IDESC_S, kk > 0 ? 1u : 0u);
+        mma_commit(&k_empty[s]);
+        mma_commit(s_full);
+      }
+      __syncwarp();
+      if (j > 0) ok = issue_pv(j - 1);
+    }
+    if (ok && ntiles > 0) ok = issue_pv(ntiles - 1);
+    if (!ok && lane == 0) {
+      if (status) atomicCAS(status, 0, kStatusTimeoutMma);
+      *abort_flag = 1;
+    }
+    __syncwarp();
+    if (elect_one()) mma_commit(drain);
+    __syncwarp();
+    const long long t0 = clock64();
+    while (!mbar_try_wait(drain, 0) && clock64() - t0 < kSpinLimitCycles / 8) {
+    }
   } else if (warp == 1) {
     if (lane == 0) {
       bool ok = mbar_wait(q_full, 0, abort_flag);
