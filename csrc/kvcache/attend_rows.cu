@@ -1,21 +1,22 @@
 // Attention over the 8-bit paged cache for few query rows (generated tokens).
 //
 // Rows are (token, query head of the group): all query heads that share a cached head read
-// its pages once. One CTA = 16 * MT rows of one (sequence, cached head) and a share of its
+// its pages once. One CTA = 8 * NT rows of one (sequence, cached head) and a share of its
 // pages; each of its 4 warps walks pages of its own, a ring of bulk copies (keys 4 KB,
 // values 4 KB) ahead of it, and keeps a running maximum, sum and output.
-//   S = Q K^T and O = P V run on the warp-level 16x8x16 matrix instruction in fp16 with fp32
-//   sums: these kernels wait for memory, not for matrix rate, and the register operands
-//   take the codes without a pass through shared memory. e4m3 -> fp16 is exact, one
-//   instruction for two codes. Q is scaled by a power of two per row (largest element near
-//   2^14), exact but for elements 2^-28 of the row's largest. P <= 1 in fp16 is rounded by
-//   at most 2^-11 of itself. A page's key scale multiplies its scores, its value scale
-//   its P V product, both in fp32.
+//   S^T = K Q^T and O^T = V^T P^T run on the warp-level 16x8x16 matrix instruction in fp16
+//   with fp32 sums: these kernels wait for memory, not for matrix rate, and the register
+//   operands take the codes without a pass through shared memory. The codes are the
+//   16-row operand, the 8-column one holds 8 query rows, so one generated token wastes
+//   little. e4m3 -> fp16 is exact, one instruction for two codes. Q is scaled by a power of
+//   two per row (largest element near 2^14), exact but for elements 2^-28 of the row's
+//   largest. P <= 1 in fp16 is rounded by at most 2^-11 of itself. A page's key scale
+//   multiplies its scores, its value scale its P V product, both in fp32.
 //   Reduced indexes are permuted so that a lane's operand bytes are contiguous: of a key
 //   row, lane c of a quad holds channels 16c..16c+15 (a word of 4 codes is one k-step of
-//   16), of a value channel tokens 16c..16c+15; the score columns are the tokens in the
-//   order that makes the score registers the P operand (column 2c+i of tile j is token
-//   16c + 4(j/2) + 2(j%2) + i).
+//   16), of a value channel tokens 16c..16c+15. Row r < 8 of key tile i is token
+//   16 (r / 2) + 4 i + r % 2, row 8 + r the token 2 behind it; an 8x8 transpose of the packed
+//   weights then gives the P operand of k-step i.
 // The warps' results meet in shared memory; the CTAs that share a (sequence, cached head)
 // form a cluster and meet through distributed shared memory. No scratch memory, no second
 // launch, and a fixed order of sums.
@@ -35,16 +36,19 @@ namespace ddb {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kPageBytes = 8192;  // keys, then values
+constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
-__host__ __device__ constexpr int out_floats(int MT) { return 16 * MT * 64; }
-// ring | barriers | page scales | results: [warp] O, m, l, then the CTA's O, m, l
-__host__ __device__ constexpr int off_bar() { return kWarps * kStages * kPageBytes; }
-__host__ __device__ constexpr int off_scale() { return off_bar() + kWarps * kStages * 8; }
-__host__ __device__ constexpr int off_flag() { return off_scale() + kWarps * kStages * 16; }
-__host__ __device__ constexpr int off_cta(int) { return off_flag() + 32; }
-__host__ __device__ constexpr int smem_bytes(int MT) { return off_cta(MT) + (out_floats(MT) + 32 * MT) * 4; }
+__host__ __device__ constexpr int out_floats(int NT) { return 8 * NT * kPitch; }
+// rings, later the warps' results | barriers | page scales | the CTA's result
+__host__ __device__ constexpr int off_bar(int NT) {
+  return kWarps * (kStages * kPageBytes > out_floats(NT) * 4 + 64 * NT ? kStages * kPageBytes : out_floats(NT) * 4 + 64 * NT);
+}
+__host__ __device__ constexpr int off_scale(int NT) { return off_bar(NT) + kWarps * kStages * 8; }
+__host__ __device__ constexpr int off_flag(int NT) { return off_scale(NT) + kWarps * kStages * 16; }
+__host__ __device__ constexpr int off_cta(int NT) { return off_flag(NT) + 64; }
+__host__ __device__ constexpr int smem_bytes(int NT) { return off_cta(NT) + out_floats(NT) * 4 + 64 * NT; }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -65,15 +69,28 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// transposes an 8x8 matrix of 16-bit values held two to a lane (row lane / 4)
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-template <int MT>
+template <int NT>
 __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs a, int row_tiles, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int R = 8 * NT;
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, c = lane & 3;
   const int ranks = a.cluster, rank = blockIdx.x % ranks;
@@ -85,11 +102,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
   const int* row = a.step.rows + static_cast<long>(b) * a.step.ld;
   const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
   const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
-  const int r0 = tile * 16 * MT, rows = own * G;  // rows behind `rows` are padding
+  const int r0 = tile * R, rows = own * G;           // rows behind `rows` are padding
 
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_bar()) + warp * kStages;
-  float* scales = reinterpret_cast<float*>(smem + off_scale()) + warp * kStages * 4;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + off_flag());
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_bar(NT)) + warp * kStages;
+  float4* scales = reinterpret_cast<float4*>(smem + off_scale(NT)) + warp * kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + off_flag(NT));
   uint8_t* ring = smem + warp * kStages * kPageBytes;
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&bars[s], 1);
@@ -103,95 +120,102 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
   int lo_max = 0, hi_min = 0, lo_min = 0, hi_max = 0;
   if (r0 < rows) {
     const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
-    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + 16 * MT) - 1) / G, len, first);
+    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + R) - 1) / G, len, first);
     lo_min = s0.lo, hi_min = s0.hi, lo_max = s1.lo, hi_max = s1.hi;
     pages = kv_pages(lo_min, hi_max, sinks, a.step.width);
   }
   const int part = rank * kWarps + warp, parts = ranks * kWarps;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
 
-  // page ids of the warp's next 32 pages, one a lane
-  int ids = -1;
+  // the warp's next 32 pages, one a lane: block of codes (-1: not in the pool) and scales
+  long block = -1;
+  float ks = 0.f, vs = 0.f;
   auto issue = [&](int i) {  // i-th page of this warp; whole warp
     if ((i & 31) == 0) {
       const int n = part + (i + lane) * parts;
-      ids = n < pages.n ? row[kKvInfo + pages.at(n)] : -1;
+      block = -1;
+      if (n < pages.n) {
+        const int id = row[kKvInfo + pages.at(n)];
+        if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages)) {
+          block = static_cast<long>(id) * a.pool.heads + kh;
+          ks = a.pool.k_scale[block];
+          vs = a.pool.v_scale[block];
+        } else {  // no call's mask reaches a page that the table lacks: recorded, hidden
+          record_bad_index(status, id);
+        }
+      }
     }
-    int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    const long at = __shfl_sync(0xffffffffu, block, i & 31);
+    const float kf = __shfl_sync(0xffffffffu, ks, i & 31), vf = __shfl_sync(0xffffffffu, vs, i & 31);
     if (lane == 0) {
       const int s = i % kStages;
-      const bool there = static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages);
-      if (!there) {  // no call's mask reaches a page that the table lacks: recorded, hidden
-        record_bad_index(status, id);
-        id = 0;
-      }
-      const long block = static_cast<long>(id) * a.pool.heads + kh;
+      const long from = max(at, 0L) * 4096;
+      scales[s] = make_float4(kf, vf, at >= 0 ? 1.f : 0.f, 0.f);
       mbar_arrive_expect_tx(&bars[s], kPageBytes);
-      bulk_load(ring + s * kPageBytes, a.pool.k + block * 4096, 4096, &bars[s]);
-      bulk_load(ring + s * kPageBytes + 4096, a.pool.v + block * 4096, 4096, &bars[s]);
-      scales[s * 4] = a.pool.k_scale[block];
-      scales[s * 4 + 1] = a.pool.v_scale[block];
-      scales[s * 4 + 2] = there ? 1.f : 0.f;
+      bulk_load(ring + s * kPageBytes, a.pool.k + from, 4096, &bars[s]);
+      bulk_load(ring + s * kPageBytes + 4096, a.pool.v + from, 4096, &bars[s]);
     }
   };
   for (int i = 0; i < min(mine, kStages); ++i) issue(i);
 
-  // Q: rows g and g + 8 of each 16, channels 16c..16c+15
-  uint32_t qf[MT][4][4];
-  float sl2[MT][2];
-  KvSpan span[MT][2];
+  // Q: row g of each 8, channels 16c..16c+15
+  uint32_t qf[NT][4][2];
+  float sl2[NT][2];   // score factors of rows 2c and 2c + 1, which this lane's scores belong to
+  KvSpan span[NT][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = r0 + nt * 8 + g;
+    float x[16];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = r0 + mt * 16 + u * 8 + g;
-      float x[16];
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    if (r < rows) {
+      const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + (r / G) * a.q_st +
+                               (kh * G + r % G) * a.q_sh + 16 * c;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = 0.f;
-      // a padding row keeps zeros and the span of the last row: its result is not used
-      span[mt][u] = kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
-      if (r < rows) {
-        const int t = r / G, h = kh * G + r % G;
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + t * a.q_st + h * a.q_sh + 16 * c;
+      for (int i = 0; i < 2; ++i) {
+        const uint4 w = ld_global_v4(q + i * 8);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 w = ld_global_v4(q + i * 8);
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = unpack_bf16(ws[k]);
-            x[i * 8 + 2 * k] = f.x;
-            x[i * 8 + 2 * k + 1] = f.y;
-          }
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = unpack_bf16(ws[k]);
+          x[i * 8 + 2 * k] = f.x;
+          x[i * 8 + 2 * k + 1] = f.y;
         }
       }
-      float amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const int e = row_exponent(amax);
-      const float down = __int_as_float((127 - e) << 23);
-      sl2[mt][u] = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        qf[mt][s][u] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
-        qf[mt][s][2 + u] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
-      }
     }
-
-  float m[MT][2], l[MT][2], o[MT][8][4];
+    float amax = 0.f;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int e = row_exponent(amax);
+    const float down = __int_as_float((127 - e) << 23);
+    const float up = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      qf[nt][s][0] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
+      qf[nt][s][1] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      m[mt][u] = -INFINITY;
-      l[mt][u] = 0.f;
+      sl2[nt][u] = __shfl_sync(0xffffffffu, up, (2 * c + u) * 4);
+      // a padding row keeps zeros and the span of the last row: its result is not used
+      span[nt][u] = kv_span(a, old + (min(max(rows, 1), r0 + nt * 8 + 2 * c + u + 1) - 1) / G, len, first);
+    }
+  }
+
+  float m[NT][2], l[NT][2], o[NT][4][4];  // o: channels 16 i + g, + 8 of rows 2c, 2c + 1
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[nt][u] = -INFINITY;
+      l[nt][u] = 0.f;
     }
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.f;
+      for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
   }
 
   bool ok = true;
@@ -201,68 +225,69 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
     ok = __all_sync(0xffffffffu, mbar_wait(&bars[st], (i / kStages) & 1, abort_flag));
     if (!ok) break;
     const uint32_t sk = smem_u32(ring + st * kPageBytes), sv = sk + 4096;
-    const float ks = scales[st * 4], vs = scales[st * 4 + 1];
-    const bool there = scales[st * 4 + 2] != 0.f;
+    const float4 f = scales[st];
+    const bool there = f.z != 0.f;
     const int key0 = pages.at(part + i * parts) * kKvPage;
 
-    float s[MT][8][4];
+    float s[NT][4][4];  // keys krow + 4 t (and 2 behind it) of rows 2c, 2c + 1
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint4 w = lds128(sk + (krow + 4 * (j >> 1) + 2 * (j & 1)) * 64 + c * 16);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    for (int t = 0; t < 4; ++t) {
+      const uint4 w0 = lds128(sk + (krow + 4 * t) * 64 + c * 16), w1 = lds128(sk + (krow + 4 * t + 2) * 64 + c * 16);
+      const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[mt][j][k] = 0.f;
+        for (int k = 0; k < 4; ++k) s[nt][t][k] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t b0 = half2_of(ws[k] & 0xffff), b1 = half2_of(ws[k] >> 16);
+        const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][j], qf[mt][k], b0, b1);
+        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][t], av, qf[nt][k][0], qf[nt][k][1]);
       }
     }
     // a page that every row of the tile sees whole needs no mask
     const bool whole = there && key0 + kKvPage <= hi_min && (key0 >= lo_max || key0 + kKvPage <= sinks);
-    uint32_t pf[MT][4][4];
-    float alpha[MT][2];
+    uint32_t pf[NT][4][2];
+    float alpha[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int nt = 0; nt < NT; ++nt) {
+      float p[4][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const float f = sl2[mt][u] * ks;
-        float mx = -INFINITY;
+        const float fu = sl2[nt][u] * f.x;
         if (!whole) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int key = key0 + 16 * c + 4 * (j >> 1) + 2 * (j & 1) + k;
-              if (!there || !kv_visible(span[mt][u], sinks, key)) s[mt][j][2 * u + k] = -INFINITY;
-            }
+            for (int k = 0; k < 2; ++k)
+              if (!there || !kv_visible(span[nt][u], sinks, key0 + krow + 4 * t + 2 * k)) s[nt][t][2 * k + u] = -INFINITY;
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * u], s[mt][j][2 * u + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float top = mx == -INFINITY ? m[mt][u] : fmaxf(m[mt][u], mx * f);
+        float mx = fmaxf(fmaxf(s[nt][0][u], s[nt][0][2 + u]), fmaxf(s[nt][1][u], s[nt][1][2 + u]));
+        mx = fmaxf(mx, fmaxf(fmaxf(s[nt][2][u], s[nt][2][2 + u]), fmaxf(s[nt][3][u], s[nt][3][2 + u])));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float top = mx == -INFINITY ? m[nt][u] : fmaxf(m[nt][u], mx * fu);
         const float use = top == -INFINITY ? 0.f : top;
-        alpha[mt][u] = exp2f(m[mt][u] - use);
-        m[mt][u] = top;
+        alpha[nt][u] = exp2f(m[nt][u] - use);
+        m[nt][u] = top;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float p0, p1;
-          if (!whole) {  // a masked score stays -inf whatever the factor is
-            p0 = s[mt][j][2 * u] == -INFINITY ? 0.f : exp2f(s[mt][j][2 * u] * f - use);
-            p1 = s[mt][j][2 * u + 1] == -INFINITY ? 0.f : exp2f(s[mt][j][2 * u + 1] * f - use);
-          } else {
-            p0 = exp2f(s[mt][j][2 * u] * f - use);
-            p1 = exp2f(s[mt][j][2 * u + 1] * f - use);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x = s[nt][t][2 * k + u];
+            float w = exp2f(x * fu - use);
+            if (!whole && x == -INFINITY) w = 0.f;  // a masked score, whatever the factor is
+            p[t][2 * k + u] = w;
+            sum += w;
           }
-          sum += p0 + p1;
-          pf[mt][j >> 1][(j & 1) * 2 + u] = pack_half(p0, p1);
-        }
-        l[mt][u] = l[mt][u] * alpha[mt][u] + sum;
+        l[nt][u] = l[nt][u] * alpha[nt][u] + sum;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        pf[nt][t][0] = transpose8x8(pack_half(p[t][0], p[t][1]));
+        pf[nt][t][1] = transpose8x8(pack_half(p[t][2], p[t][3]));
       }
     }
     // tokens that no row of the tile sees are left out of P V whatever they hold
@@ -274,140 +299,151 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
         if (!there || !kv_visible(all, sinks, key0 + 16 * c + k)) keep[k >> 2] &= ~(0xffu << (8 * (k & 3)));
     }
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const uint4 w = lds128(sv + (n * 8 + g) * 64 + c * 16);
-      const uint32_t ws[4] = {w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]};
-      float d[MT][4];
+    for (int t = 0; t < 4; ++t) {
+      const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
+      const uint32_t x0[4] = {w0.x & keep[0], w0.y & keep[1], w0.z & keep[2], w0.w & keep[3]};
+      const uint32_t x1[4] = {w1.x & keep[0], w1.y & keep[1], w1.z & keep[2], w1.w & keep[3]};
+      float d[NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[mt][k] = 0.f;
+        for (int k = 0; k < 4; ++k) d[nt][k] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t b0 = half2_of(ws[k] & 0xffff), b1 = half2_of(ws[k] >> 16);
+        const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) mma_f16(d[mt], pf[mt][k], b0, b1);
+        for (int nt = 0; nt < NT; ++nt) mma_f16(d[nt], av, pf[nt][k][0], pf[nt][k][1]);
       }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[mt][n][k] = o[mt][n][k] * alpha[mt][k >> 1] + d[mt][k] * vs;
+        for (int k = 0; k < 4; ++k) o[nt][t][k] = o[nt][t][k] * alpha[nt][k & 1] + d[nt][k] * f.y;
     }
     __syncwarp();  // every lane has read the stage
     if (i + kStages < mine) issue(i + kStages);
   }
   if (!ok) {
-    if (lane == 0 && status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
-    *abort_flag = 1;
-    if (lane == 0) {  // copies in flight land before the ring is reused or the CTA retires
-      const long long t0 = clock64();
+    if (lane == 0) {
+      if (status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
+      *abort_flag = 1;
+      const long long t0 = clock64();  // copies in flight land before the ring is reused
       for (int s = 0; s < kStages; ++s)
         for (int ph = 0; ph < 2; ++ph)
           while (!mbar_try_wait(&bars[s], ph) && clock64() - t0 < kSpinLimitCycles / 8) {
           }
     }
+    __syncwarp();
   }
-  // ---- the warps' results: unnormalised O, m, l (quad sums), over the rings
+  // ---- the warps' results: unnormalised O, m and l (whole sums), over the rings
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 1);
-      l[mt][u] += __shfl_xor_sync(0xffffffffu, l[mt][u], 2);
-      if (m[mt][u] == -INFINITY && l[mt][u] != 0.f) m[mt][u] = 0.f;  // only NaN scores so far
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], x);
+      if (m[nt][u] == -INFINITY && l[nt][u] != 0.f) m[nt][u] = 0.f;  // only NaN scores so far
     }
   __syncthreads();
-  float* wo = reinterpret_cast<float*>(smem);                // [warp][row][64]
-  float* wml = wo + kWarps * out_floats(MT);                 // [warp][row][2]
+  float* wo = reinterpret_cast<float*>(smem);  // [warp][row][kPitch], then [warp][row] (m, l)
+  float2* wml = reinterpret_cast<float2*>(wo + kWarps * out_floats(NT));
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int r = mt * 16 + u * 8 + g;
+      const int r = nt * 8 + 2 * c + u;
+      float* w = wo + warp * out_floats(NT) + r * kPitch + g;
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
-        *reinterpret_cast<float2*>(wo + warp * out_floats(MT) + r * 64 + n * 8 + 2 * c) =
-            make_float2(o[mt][n][2 * u], o[mt][n][2 * u + 1]);
-      if (c == 0) {
-        wml[(warp * 16 * MT + r) * 2] = m[mt][u];
-        wml[(warp * 16 * MT + r) * 2 + 1] = l[mt][u];
+      for (int t = 0; t < 4; ++t) {
+        w[t * 16] = o[nt][t][u];
+        w[t * 16 + 8] = o[nt][t][2 + u];
       }
+      if (g == 0) wml[warp * R + r] = make_float2(m[nt][u], l[nt][u]);
     }
   __syncthreads();
-  float* co = reinterpret_cast<float*>(smem + off_cta(MT));  // the CTA's [row][64], then [row][2]
-  float* cml = co + out_floats(MT);
-  for (int i = threadIdx.x; i < out_floats(MT); i += kWarps * 32) {
-    const int r = i >> 6;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
+  float* co = reinterpret_cast<float*>(smem + off_cta(NT));  // the CTA's [row][kPitch], then [row] (m, l)
+  float2* cml = reinterpret_cast<float2*>(co + out_floats(NT));
+  for (int i = threadIdx.x; i < R * 16; i += kWarps * 32) {
+    const int r = i >> 4, d = (i & 15) * 4;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[(w * 16 * MT + r) * 2]);
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[w * R + r].x);
     if (top != -INFINITY) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float k = exp2f(wml[(w * 16 * MT + r) * 2] - top);
-        v += k * wo[w * out_floats(MT) + i];
-        sum += k * wml[(w * 16 * MT + r) * 2 + 1];
+        const float2 ml = wml[w * R + r];
+        const float k = exp2f(ml.x - top);
+        const float4 x = *reinterpret_cast<const float4*>(wo + w * out_floats(NT) + r * kPitch + d);
+        v.x += k * x.x;
+        v.y += k * x.y;
+        v.z += k * x.z;
+        v.w += k * x.w;
+        sum += k * ml.y;
       }
     }
-    co[i] = v;
-    if ((i & 63) == 0) {
-      cml[r * 2] = top;
-      cml[r * 2 + 1] = sum;
-    }
+    *reinterpret_cast<float4*>(co + r * kPitch + d) = v;
+    if (d == 0) cml[r] = make_float2(top, sum);
   }
   if (ranks > 1) cluster_sync_all(); else __syncthreads();
   // ---- the cluster's CTAs share the rows; each adds the others' parts in rank order
   const uint32_t so = smem_u32(co), sml = smem_u32(cml);
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.o);
-  for (int i = threadIdx.x + rank * kWarps * 32; i < out_floats(MT) / 2; i += ranks * kWarps * 32) {
-    const int r = i >> 5, d = (i & 31) * 2, R = r0 + r;
-    if (R >= a.T * G) break;
-    float top = -INFINITY, sum = 0.f, v0 = 0.f, v1 = 0.f;
-    for (int k = 0; k < ranks; ++k) top = fmaxf(top, ld_cluster(ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8));
-    if (top != -INFINITY) {
+  for (int i = threadIdx.x + rank * kWarps * 32; i < R * 16; i += ranks * kWarps * 32) {
+    const int r = i >> 4, d = (i & 15) * 4, row_id = r0 + r;
+    if (row_id >= a.T * G) break;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < ranks; ++k) top = fmaxf(top, ld_cluster_v2(ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8).x);
+    if (top != -INFINITY)
       for (int k = 0; k < ranks; ++k) {
         const uint32_t ml = ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8;
-        const uint32_t ov = ranks > 1 ? mapa_shared(so + (r * 64 + d) * 4, k) : so + (r * 64 + d) * 4;
-        const float w = exp2f(ld_cluster(ml) - top);
-        sum += w * ld_cluster(ml + 4);
-        v0 += w * ld_cluster(ov);
-        v1 += w * ld_cluster(ov + 4);
+        const uint32_t ov = ranks > 1 ? mapa_shared(so + (r * kPitch + d) * 4, k) : so + (r * kPitch + d) * 4;
+        const float2 x = ld_cluster_v2(ml);
+        const float4 y = ld_cluster_v4(ov);
+        const float w = exp2f(x.x - top);
+        sum += w * x.y;
+        v.x += w * y.x;
+        v.y += w * y.y;
+        v.z += w * y.z;
+        v.w += w * y.w;
       }
+    const int t = row_id / G, h = kh * G + row_id % G;
+    if (t >= own) {  // behind the sequence's own tokens
+      sum = 0.f;
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const int t = R / G, h = kh * G + R % G;
-    if (t >= own) sum = v0 = v1 = 0.f;  // behind the sequence's own tokens
     // a NaN among the scores makes the row NaN, as the formula has it
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const long at = (static_cast<long>(b) * a.T + t) * a.H + h;
-    *reinterpret_cast<uint32_t*>(out + at * 64 + d) = pack_bf16(v0 * inv, v1 * inv);
+    *reinterpret_cast<uint2*>(out + at * 64 + d) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
     if (a.lse && d == 0)
       a.lse[(static_cast<long>(b) * a.H + h) * a.T + t] = sum == 0.f ? -INFINITY : top + __log2f(sum);
   }
   if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its results
 }
 
-template <int MT>
+template <int NT>
 void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_rows<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(MT)),
+    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT)),
                "cudaFuncSetAttribute(kv_attend_rows)");
     set.fetch_or(1ull << (dev & 63));
   }
   const int G = a.H / a.pool.heads;
-  const int tiles = (a.T * G + 16 * MT - 1) / (16 * MT);
+  const int tiles = (a.T * G + 8 * NT - 1) / (8 * NT);
   const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
-  // Share the pages of an item over more CTAs while the SMs' two slots are not filled and
+  // Share the pages of an item over more CTAs while the SMs' three slots are not filled and
   // every warp keeps two pages or more.
   const int pages = (a.max_tokens + kKvPage - 1) / kKvPage;
   int ranks = 1;
-  while (ranks < 8 && items * ranks < 2L * num_sms(dev) && pages >= ranks * 2 * kWarps * 2) ranks *= 2;
+  while (ranks < 8 && items * ranks < 3L * num_sms(dev) && pages >= ranks * 2 * kWarps * 2) ranks *= 2;
   if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
   a.cluster = ranks;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
   cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem_bytes(MT);
+  cfg.dynamicSmemBytes = smem_bytes(NT);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -415,7 +451,7 @@ void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<MT>, a, tiles, device_status(dev)), "kv_attend_rows launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, device_status(dev)), "kv_attend_rows launch");
   count_launch();
 }
 
@@ -425,10 +461,17 @@ void kv_cache_attend(const KvAttendArgs& a, cudaStream_t stream) {
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  if (a.T * static_cast<long>(a.H / a.pool.heads) > 64)
+  const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
+  if (rows > 64)
     kv_attend_tiles_launch(a, dev, stream);
-  else
+  else if (rows <= 8)
     launch<1>(a, dev, stream);
+  else if (rows <= 16)
+    launch<2>(a, dev, stream);
+  else if (rows <= 24)
+    launch<3>(a, dev, stream);
+  else
+    launch<4>(a, dev, stream);
 }
 
 }  // namespace ddb
