@@ -2,8 +2,9 @@
 //
 // Rows are (token, query head of the group): all query heads that share a cached head read
 // its pages once. One CTA = 8 * NT rows of one (sequence, cached head) and a share of its
-// pages; each of its 4 warps walks pages of its own, a ring of bulk copies (keys 4 KB,
-// values 4 KB) ahead of it, and keeps a running maximum, sum and output.
+// pages, as 4 groups of NT warps: a group walks pages of its own, a ring of bulk copies
+// (keys 4 KB, values 4 KB) ahead of it, and each of its warps keeps a running maximum,
+// sum and output for 8 rows.
 //   S^T = K Q^T and O^T = V^T P^T run on the warp-level 16x8x16 matrix instruction in fp16
 //   with fp32 sums: these kernels wait for memory, not for matrix rate, and the register
 //   operands take the codes without a pass through shared memory. The codes are the
@@ -35,20 +36,22 @@
 namespace ddb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kStages = 2;
+constexpr int kGroups = 4;
+constexpr int kMaxStages = 6;
 constexpr int kPageBytes = 8192;  // keys, then values
 constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
-__host__ __device__ constexpr int out_floats(int NT) { return 8 * NT * kPitch; }
-// rings, later the warps' results | barriers | page scales | the CTA's result
-__host__ __device__ constexpr int off_bar(int NT) {
-  return kWarps * (kStages * kPageBytes > out_floats(NT) * 4 + 64 * NT ? kStages * kPageBytes : out_floats(NT) * 4 + 64 * NT);
-}
-__host__ __device__ constexpr int off_scale(int NT) { return off_bar(NT) + kWarps * kStages * 8; }
-__host__ __device__ constexpr int off_flag(int NT) { return off_scale(NT) + kWarps * kStages * 16; }
-__host__ __device__ constexpr int off_cta(int NT) { return off_flag(NT) + 64; }
-__host__ __device__ constexpr int smem_bytes(int NT) { return off_cta(NT) + out_floats(NT) * 4 + 64 * NT; }
+// the CTA's result and its rows' (m, l) | barriers | page scales | flag | rings, later the
+// groups' results
+constexpr int out_floats(int NT) { return 8 * NT * kPitch; }
+constexpr int off_ml(int NT) { return out_floats(NT) * 4; }
+constexpr int off_bar(int NT) { return off_ml(NT) + 64 * NT; }
+constexpr int off_scale(int NT) { return off_bar(NT) + kGroups * kMaxStages * 16; }
+constexpr int off_flag(int NT) { return off_scale(NT) + kGroups * kMaxStages * 16; }
+constexpr int off_ring(int NT) { return (off_flag(NT) + 16 + 127) / 128 * 128; }
+constexpr int smem_bytes(int NT, int stages) { return off_ring(NT) + kGroups * stages * kPageBytes; }
+static_assert(kGroups * (out_floats(4) * 4 + 64 * 4) <= kGroups * 2 * kPageBytes, "results fit the rings");
+static_assert(smem_bytes(4, kMaxStages) <= 232448, "shared memory per CTA");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -88,10 +91,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 template <int NT>
-__global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs a, int row_tiles, int* status) {
+__global__ void __launch_bounds__(kGroups * NT * 32)
+    kv_attend_rows(const KvAttendArgs a, int row_tiles, int stages, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int R = 8 * NT;
+  constexpr int R = 8 * NT, kThreads = kGroups * NT * 32;
   const int warp = warp_id(), lane = lane_id();
+  const int rg = warp % NT, pg = warp / NT;  // the warp's 8 rows, and its group
   const int g = lane >> 2, c = lane & 3;
   const int ranks = a.cluster, rank = blockIdx.x % ranks;
   int item = blockIdx.x / ranks;
@@ -104,13 +109,17 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
   const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
   const int r0 = tile * R, rows = own * G;           // rows behind `rows` are padding
 
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_bar(NT)) + warp * kStages;
-  float4* scales = reinterpret_cast<float4*>(smem + off_scale(NT)) + warp * kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + off_bar(NT)) + pg * 2 * kMaxStages;
+  uint64_t* empty = full + kMaxStages;
+  float4* scales = reinterpret_cast<float4*>(smem + off_scale(NT)) + pg * kMaxStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + off_flag(NT));
-  uint8_t* ring = smem + warp * kStages * kPageBytes;
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bars[s], 1);
-    if (warp == 0) *abort_flag = 0;
+  uint8_t* ring = smem + off_ring(NT) + pg * stages * kPageBytes;
+  if (rg == 0 && lane == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], NT);
+    }
+    if (pg == 0) *abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
@@ -124,15 +133,16 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
     lo_min = s0.lo, hi_min = s0.hi, lo_max = s1.lo, hi_max = s1.hi;
     pages = kv_pages(lo_min, hi_max, sinks, a.step.width);
   }
-  const int part = rank * kWarps + warp, parts = ranks * kWarps;
+  const int part = rank * kGroups + pg, parts = ranks * kGroups;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
 
-  // the warp's next 32 pages, one a lane: block of codes (-1: not in the pool) and scales
+  // the group's next 32 pages, one a lane: block of codes (-1: not in the pool) and scales
   long block = -1;
   float ks = 0.f, vs = 0.f;
-  auto issue = [&](int i) {  // i-th page of this warp; whole warp
-    if ((i & 31) == 0) {
-      const int n = part + (i + lane) * parts;
+  int put = 0, put_stage = 0, put_phase = 1;
+  auto issue = [&]() -> bool {  // the group's next page; its first warp, whole
+    if ((put & 31) == 0) {
+      const int n = part + (put + lane) * parts;
       block = -1;
       if (n < pages.n) {
         const int id = row[kKvInfo + pages.at(n)];
@@ -145,26 +155,35 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
         }
       }
     }
-    const long at = __shfl_sync(0xffffffffu, block, i & 31);
-    const float kf = __shfl_sync(0xffffffffu, ks, i & 31), vf = __shfl_sync(0xffffffffu, vs, i & 31);
+    if (NT > 1 && !__all_sync(0xffffffffu, mbar_wait(&empty[put_stage], put_phase, abort_flag))) return false;
+    const long at = __shfl_sync(0xffffffffu, block, put & 31);
+    const float kf = __shfl_sync(0xffffffffu, ks, put & 31), vf = __shfl_sync(0xffffffffu, vs, put & 31);
     if (lane == 0) {
-      const int s = i % kStages;
       const long from = max(at, 0L) * 4096;
-      scales[s] = make_float4(kf, vf, at >= 0 ? 1.f : 0.f, 0.f);
-      mbar_arrive_expect_tx(&bars[s], kPageBytes);
-      bulk_load(ring + s * kPageBytes, a.pool.k + from, 4096, &bars[s]);
-      bulk_load(ring + s * kPageBytes + 4096, a.pool.v + from, 4096, &bars[s]);
+      uint64_t* bar = &full[put_stage];
+      uint8_t* dst = ring + put_stage * kPageBytes;
+      scales[put_stage] = make_float4(kf, vf, at >= 0 ? 1.f : 0.f, 0.f);
+      mbar_arrive_expect_tx(bar, kPageBytes);
+      bulk_load(dst, a.pool.k + from, 4096, bar);
+      bulk_load(dst + 4096, a.pool.v + from, 4096, bar);
     }
+    ++put;
+    if (++put_stage == stages) {
+      put_stage = 0;
+      put_phase ^= 1;
+    }
+    return true;
   };
-  for (int i = 0; i < min(mine, kStages); ++i) issue(i);
+  bool ok = true;
+  if (rg == 0)
+    for (int i = 0; i < min(mine, stages); ++i) issue();  // no wait: the stages are empty
 
-  // Q: row g of each 8, channels 16c..16c+15
-  uint32_t qf[NT][4][2];
-  float sl2[NT][2];   // score factors of rows 2c and 2c + 1, which this lane's scores belong to
-  KvSpan span[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = r0 + nt * 8 + g;
+  // Q: row g of the warp's 8, channels 16c..16c+15
+  uint32_t qf[4][2];
+  float sl2[2];   // score factors of rows 2c and 2c + 1, which this lane's scores belong to
+  KvSpan span[2];
+  {
+    const int r = r0 + rg * 8 + g;
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -193,102 +212,87 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
     const float up = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      qf[nt][s][0] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
-      qf[nt][s][1] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
+      qf[s][0] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
+      qf[s][1] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      sl2[nt][u] = __shfl_sync(0xffffffffu, up, (2 * c + u) * 4);
+      sl2[u] = __shfl_sync(0xffffffffu, up, (2 * c + u) * 4);
       // a padding row keeps zeros and the span of the last row: its result is not used
-      span[nt][u] = kv_span(a, old + (min(max(rows, 1), r0 + nt * 8 + 2 * c + u + 1) - 1) / G, len, first);
+      span[u] = kv_span(a, old + (min(max(rows, 1), r0 + rg * 8 + 2 * c + u + 1) - 1) / G, len, first);
     }
   }
 
-  float m[NT][2], l[NT][2], o[NT][4][4];  // o: channels 16 i + g, + 8 of rows 2c, 2c + 1
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float o[4][4];  // channels 16 i + g, + 8 of rows 2c, 2c + 1
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      m[nt][u] = -INFINITY;
-      l[nt][u] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[nt][i][k] = 0.f;
-  }
+    for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
 
-  bool ok = true;
   const int krow = 16 * (g >> 1) + (g & 1);
+  int st = 0, phase = 0;
   for (int i = 0; i < mine; ++i) {
-    const int st = i % kStages;
-    ok = __all_sync(0xffffffffu, mbar_wait(&bars[st], (i / kStages) & 1, abort_flag));
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[st], phase, abort_flag));
     if (!ok) break;
     const uint32_t sk = smem_u32(ring + st * kPageBytes), sv = sk + 4096;
     const float4 f = scales[st];
     const bool there = f.z != 0.f;
     const int key0 = pages.at(part + i * parts) * kKvPage;
 
-    float s[NT][4][4];  // keys krow + 4 t (and 2 behind it) of rows 2c, 2c + 1
+    float s[4][4];  // keys krow + 4 t (and 2 behind it) of rows 2c, 2c + 1
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint4 w0 = lds128(sk + (krow + 4 * t) * 64 + c * 16), w1 = lds128(sk + (krow + 4 * t + 2) * 64 + c * 16);
       const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[nt][t][k] = 0.f;
+      for (int k = 0; k < 4; ++k) s[t][k] = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt][t], av, qf[nt][k][0], qf[nt][k][1]);
+        mma_f16(s[t], av, qf[k][0], qf[k][1]);
       }
     }
     // a page that every row of the tile sees whole needs no mask
     const bool whole = there && key0 + kKvPage <= hi_min && (key0 >= lo_max || key0 + kKvPage <= sinks);
-    uint32_t pf[NT][4][2];
-    float alpha[NT][2];
+    float p[4][4], alpha[2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4][4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float fu = sl2[nt][u] * f.x;
-        if (!whole) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (!there || !kv_visible(span[nt][u], sinks, key0 + krow + 4 * t + 2 * k)) s[nt][t][2 * k + u] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(s[nt][0][u], s[nt][0][2 + u]), fmaxf(s[nt][1][u], s[nt][1][2 + u]));
-        mx = fmaxf(mx, fmaxf(fmaxf(s[nt][2][u], s[nt][2][2 + u]), fmaxf(s[nt][3][u], s[nt][3][2 + u])));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float top = mx == -INFINITY ? m[nt][u] : fmaxf(m[nt][u], mx * fu);
-        const float use = top == -INFINITY ? 0.f : top;
-        alpha[nt][u] = exp2f(m[nt][u] - use);
-        m[nt][u] = top;
-        float sum = 0.f;
+    for (int u = 0; u < 2; ++u) {
+      const float fu = sl2[u] * f.x;
+      if (!whole) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float x = s[nt][t][2 * k + u];
-            float w = exp2f(x * fu - use);
-            if (!whole && x == -INFINITY) w = 0.f;  // a masked score, whatever the factor is
-            p[t][2 * k + u] = w;
-            sum += w;
-          }
-        l[nt][u] = l[nt][u] * alpha[nt][u] + sum;
+          for (int k = 0; k < 2; ++k)
+            if (!there || !kv_visible(span[u], sinks, key0 + krow + 4 * t + 2 * k)) s[t][2 * k + u] = -INFINITY;
       }
+      float mx = fmaxf(fmaxf(s[0][u], s[0][2 + u]), fmaxf(s[1][u], s[1][2 + u]));
+      mx = fmaxf(mx, fmaxf(fmaxf(s[2][u], s[2][2 + u]), fmaxf(s[3][u], s[3][2 + u])));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float top = mx == -INFINITY ? m[u] : fmaxf(m[u], mx * fu);
+      const float use = top == -INFINITY ? 0.f : top;
+      alpha[u] = exp2f(m[u] - use);
+      m[u] = top;
+      float sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        pf[nt][t][0] = transpose8x8(pack_half(p[t][0], p[t][1]));
-        pf[nt][t][1] = transpose8x8(pack_half(p[t][2], p[t][3]));
-      }
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float x = s[t][2 * k + u];
+          float w = exp2f(x * fu - use);
+          if (!whole && x == -INFINITY) w = 0.f;  // a masked score, whatever the factor is
+          p[t][2 * k + u] = w;
+          sum += w;
+        }
+      l[u] = l[u] * alpha[u] + sum;
+    }
+    uint32_t pf[4][2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      pf[t][0] = transpose8x8(pack_half(p[t][0], p[t][1]));
+      pf[t][1] = transpose8x8(pack_half(p[t][2], p[t][3]));
     }
     // tokens that no row of the tile sees are left out of P V whatever they hold
     uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
@@ -303,74 +307,71 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
       const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
       const uint32_t x0[4] = {w0.x & keep[0], w0.y & keep[1], w0.z & keep[2], w0.w & keep[3]};
       const uint32_t x1[4] = {w1.x & keep[0], w1.y & keep[1], w1.z & keep[2], w1.w & keep[3]};
-      float d[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) d[nt][k] = 0.f;
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(d[nt], av, pf[nt][k][0], pf[nt][k][1]);
+        mma_f16(d, av, pf[k][0], pf[k][1]);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[nt][t][k] = o[nt][t][k] * alpha[nt][k & 1] + d[nt][k] * f.y;
+      for (int k = 0; k < 4; ++k) o[t][k] = o[t][k] * alpha[k & 1] + d[k] * f.y;
     }
     __syncwarp();  // every lane has read the stage
-    if (i + kStages < mine) issue(i + kStages);
+    if (NT > 1 && lane == 0) mbar_arrive(&empty[st]);
+    // The next page goes into the stage that the group has just left; with several warps
+    // into the one before, which the others have left too.
+    if (rg == 0 && put < mine && (NT == 1 || i > 0)) ok = issue();
+    if (!ok) break;
+    if (++st == stages) {
+      st = 0;
+      phase ^= 1;
+    }
   }
   if (!ok) {
     if (lane == 0) {
       if (status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
       *abort_flag = 1;
       const long long t0 = clock64();  // copies in flight land before the ring is reused
-      for (int s = 0; s < kStages; ++s)
+      for (int s = 0; s < stages; ++s)
         for (int ph = 0; ph < 2; ++ph)
-          while (!mbar_try_wait(&bars[s], ph) && clock64() - t0 < kSpinLimitCycles / 8) {
+          while (!mbar_try_wait(&full[s], ph) && clock64() - t0 < kSpinLimitCycles / 8) {
           }
     }
     __syncwarp();
   }
-  // ---- the warps' results: unnormalised O, m and l (whole sums), over the rings
+  // ---- the groups' results: unnormalised O, m and l (whole sums), over the rings
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int u = 0; u < 2; ++u) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int x = 4; x < 32; x *= 2) l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], x);
-      if (m[nt][u] == -INFINITY && l[nt][u] != 0.f) m[nt][u] = 0.f;  // only NaN scores so far
-    }
+    for (int x = 4; x < 32; x *= 2) l[u] += __shfl_xor_sync(0xffffffffu, l[u], x);
+    if (m[u] == -INFINITY && l[u] != 0.f) m[u] = 0.f;  // only NaN scores so far
+  }
   __syncthreads();
-  float* wo = reinterpret_cast<float*>(smem);  // [warp][row][kPitch], then [warp][row] (m, l)
-  float2* wml = reinterpret_cast<float2*>(wo + kWarps * out_floats(NT));
+  float* wo = reinterpret_cast<float*>(smem + off_ring(NT));  // [group][row][kPitch], then [group][row] (m, l)
+  float2* wml = reinterpret_cast<float2*>(wo + kGroups * out_floats(NT));
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int u = 0; u < 2; ++u) {
+    const int r = rg * 8 + 2 * c + u;
+    float* w = wo + pg * out_floats(NT) + r * kPitch + g;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = nt * 8 + 2 * c + u;
-      float* w = wo + warp * out_floats(NT) + r * kPitch + g;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        w[t * 16] = o[nt][t][u];
-        w[t * 16 + 8] = o[nt][t][2 + u];
-      }
-      if (g == 0) wml[warp * R + r] = make_float2(m[nt][u], l[nt][u]);
+    for (int t = 0; t < 4; ++t) {
+      w[t * 16] = o[t][u];
+      w[t * 16 + 8] = o[t][2 + u];
     }
+    if (g == 0) wml[pg * R + r] = make_float2(m[u], l[u]);
+  }
   __syncthreads();
-  float* co = reinterpret_cast<float*>(smem + off_cta(NT));  // the CTA's [row][kPitch], then [row] (m, l)
-  float2* cml = reinterpret_cast<float2*>(co + out_floats(NT));
-  for (int i = threadIdx.x; i < R * 16; i += kWarps * 32) {
+  float* co = reinterpret_cast<float*>(smem);  // the CTA's [row][kPitch], then [row] (m, l)
+  float2* cml = reinterpret_cast<float2*>(smem + off_ml(NT));
+  for (int i = threadIdx.x; i < R * 16; i += kThreads) {
     const int r = i >> 4, d = (i & 15) * 4;
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[w * R + r].x);
+    for (int w = 0; w < kGroups; ++w) top = fmaxf(top, wml[w * R + r].x);
     if (top != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < kGroups; ++w) {
         const float2 ml = wml[w * R + r];
         const float k = exp2f(ml.x - top);
         const float4 x = *reinterpret_cast<const float4*>(wo + w * out_floats(NT) + r * kPitch + d);
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv_attend_rows(const KvAttendArgs
   // ---- the cluster's CTAs share the rows; each adds the others' parts in rank order
   const uint32_t so = smem_u32(co), sml = smem_u32(cml);
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.o);
-  for (int i = threadIdx.x + rank * kWarps * 32; i < R * 16; i += ranks * kWarps * 32) {
+  for (int i = threadIdx.x + rank * kThreads; i < R * 16; i += ranks * kThreads) {
     const int r = i >> 4, d = (i & 15) * 4, row_id = r0 + r;
     if (row_id >= a.T * G) break;
     float top = -INFINITY, sum = 0.f;
@@ -426,24 +427,30 @@ template <int NT>
 void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT)),
+    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
                "cudaFuncSetAttribute(kv_attend_rows)");
     set.fetch_or(1ull << (dev & 63));
   }
-  const int G = a.H / a.pool.heads;
+  const int G = a.H / a.pool.heads, sms = num_sms(dev);
   const int tiles = (a.T * G + 8 * NT - 1) / (8 * NT);
   const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
-  // Share the pages of an item over more CTAs while the SMs' three slots are not filled and
-  // every warp keeps two pages or more.
-  const int pages = (a.max_tokens + kKvPage - 1) / kKvPage;
+  // The pages that a tile sees at most: all, or the sinks', the window's and its own rows'.
+  const long seen = std::min<long>(a.max_tokens, a.window > 0 ? a.sinks + (a.window + 1L) * a.unit + a.T + 2 * kKvPage : a.max_tokens);
+  const int pages = static_cast<int>((seen + kKvPage - 1) / kKvPage);
+  // Share the pages of an item over the CTAs of a cluster while SMs stand idle (with few
+  // rows, three CTAs fit one) and every group keeps a page or more.
+  const long slots = static_cast<long>(sms) * (NT == 1 ? 3 : NT == 2 ? 2 : 1);
   int ranks = 1;
-  while (ranks < 8 && items * ranks < 3L * num_sms(dev) && pages >= ranks * 2 * kWarps * 2) ranks *= 2;
+  while (ranks < 8 && items * ranks * 2 <= slots && pages >= ranks * 2 * kGroups) ranks *= 2;
   if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
   a.cluster = ranks;
+  // Stages: all that fit where an SM holds one CTA anyway (few rows of few sequences wait for
+  // the copies' latency), fewer where more CTAs share it.
+  const int stages = NT > 2 || items * ranks <= sms ? kMaxStages : NT == 2 ? 3 : 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem_bytes(NT);
+  cfg.blockDim = dim3(kGroups * NT * 32);
+  cfg.dynamicSmemBytes = smem_bytes(NT, stages);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -451,7 +458,7 @@ void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, device_status(dev)), "kv_attend_rows launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, stages, device_status(dev)), "kv_attend_rows launch");
   count_launch();
 }
 

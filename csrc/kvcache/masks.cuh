@@ -12,7 +12,7 @@ struct KvSpan {
 
 __device__ __forceinline__ KvSpan kv_span(const KvAttendArgs& a, int pos, int len, int first) {
   KvSpan s;
-  const int frame = pos / a.unit;
+  const int frame = a.unit == 1 ? pos : pos / a.unit;
   s.hi = a.causal ? min(len, (frame + 1) * a.unit) : len;
   s.lo = a.window > 0 ? max(first, (frame - a.window + 1) * a.unit) : first;
   return s;
