@@ -7,6 +7,8 @@
 #include <map>
 #include <utility>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "common/tma.h"
@@ -1650,89 +1652,138 @@ ddb::KvStep kv_step(const torch::Tensor& rows, const torch::Tensor& k) {
   return s;
 }
 
-// [B, T, H, 64] bf16 whose channels are contiguous and whose rows are 16-byte aligned
-void check_tokens(const torch::Tensor& t, const char* name, const torch::Tensor& k, int64_t B) {
-  check_bf16(t, name);
-  TORCH_CHECK(t.dim() == 4 && t.size(0) == B && t.size(3) == 64, name, " must be [", B, ", T, heads, 64]");
-  TORCH_CHECK(t.device() == k.device(), name, " must be on the cache's device");
-  TORCH_CHECK(t.numel() == 0 || (t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
-                                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
-              name, " must have contiguous channels and 16-byte aligned rows");
+// A step of the cache: the pool's tensors, the table on the device, and the stream that its
+// upload ran on. Calls on another stream wait for the upload.
+struct KvStepHandle {
+  torch::Tensor k, v, ks, vs, rows;
+  int64_t max_tokens = 0, most_new = 0;
+  int64_t trim_sinks = -1;  // sinks of the trimmed sequences; -1: none is, -2: they differ
+  c10::optional<c10::cuda::CUDAStream> begun;
+  at::cuda::CUDAEvent ready;
+};
+
+// rows: int32 [B, 4 + pages] in host memory; `out`: a step to refill in place
+std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
+                                            torch::Tensor rows, int64_t max_tokens, int64_t most_new, int64_t trim_sinks,
+                                            std::shared_ptr<KvStepHandle> out) {
+  kv_pool(k, v, ks, vs, 0);
+  TORCH_CHECK(rows.device().is_cpu() && rows.scalar_type() == torch::kInt32 && rows.is_contiguous() && rows.dim() == 2 &&
+                  rows.size(1) > ddb::kKvInfo && rows.size(0) <= 65535, "a step's table must be int32 [<= 65535, 4 + pages]");
+  const c10::cuda::CUDAGuard guard(k.device());
+  auto h = out ? out : std::make_shared<KvStepHandle>();
+  // pinned memory of the caching host allocator: kept until the copy has run
+  const auto staged = rows.pin_memory();
+  if (out) {
+    TORCH_CHECK(h->rows.sizes() == rows.sizes() && h->rows.device() == k.device(), "the refilled step has another shape");
+    h->rows.copy_(staged, true);
+  } else {
+    h->rows = staged.to(k.device(), torch::kInt32, true);
+  }
+  h->k = k; h->v = v; h->ks = ks; h->vs = vs;
+  h->max_tokens = max_tokens;
+  h->most_new = most_new;
+  h->trim_sinks = trim_sinks;
+  h->begun = at::cuda::getCurrentCUDAStream();
+  h->ready.record(*h->begun);
+  return h;
 }
 
-void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs, int64_t layer,
-                    torch::Tensor rows, torch::Tensor new_k, torch::Tensor new_v) {
+void kv_step_wait(KvStepHandle& h) {
+  const auto now = at::cuda::getCurrentCUDAStream();
+  if (now == *h.begun || at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
+  h.ready.block(now);
+  h.rows.record_stream(now);
+}
+
+// tokens [B, T, H, 64] bf16 as the kernels read them: contiguous channels, rows on 16 bytes
+torch::Tensor kv_tokens(const torch::Tensor& t, const char* name, const KvStepHandle& h, int64_t heads) {
+  TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == h.rows.size(0) && t.size(3) == 64, name, " must be [", h.rows.size(0),
+                    ", T, heads, 64], got ", t.sizes());
+  TORCH_CHECK_VALUE(heads ? t.size(2) == heads : t.size(2) > 0 && t.size(2) % h.k.size(2) == 0, name, " has ", t.size(2),
+                    " heads, the cache ", h.k.size(2));
+  TORCH_CHECK_VALUE(t.size(1) >= h.most_new, name, " holds ", t.size(1), " tokens, the step ", h.most_new);
+  TORCH_CHECK_VALUE(t.device() == h.k.device(), name, " is on ", t.device(), ", the cache on ", h.k.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16 on CUDA, got ", t.scalar_type());
+  if (t.numel() == 0 || (t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 &&
+                         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0))
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
+void kv_step_write(std::shared_ptr<KvStepHandle> hp, int64_t layer, const torch::Tensor& k, const torch::Tensor& v) {
+  KvStepHandle& h = *hp;
+  TORCH_CHECK_VALUE(layer >= 0 && layer < h.k.size(0), "layer ", layer, " of a cache of ", h.k.size(0));
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "k and v differ in shape");
+  const c10::cuda::CUDAGuard guard(h.k.device());
+  const auto kk = kv_tokens(k, "k", h, h.k.size(2)), vv = kv_tokens(v, "v", h, h.k.size(2));
   ddb::KvWriteArgs a;
-  a.pool = kv_pool(k, v, ks, vs, layer);
-  a.step = kv_step(rows, k);
-  check_tokens(new_k, "keys", k, a.step.B);
-  check_tokens(new_v, "values", k, a.step.B);
-  TORCH_CHECK(new_k.sizes() == new_v.sizes() && new_k.size(2) == a.pool.heads, "keys and values must be [B, T, ",
-              a.pool.heads, ", 64]");
-  const c10::cuda::CUDAGuard guard(k.device());
-  a.k = new_k.data_ptr();
-  a.k_sb = new_k.stride(0); a.k_st = new_k.stride(1); a.k_sh = new_k.stride(2);
-  a.v = new_v.data_ptr();
-  a.v_sb = new_v.stride(0); a.v_st = new_v.stride(1); a.v_sh = new_v.stride(2);
-  a.T = new_k.size(1);
+  a.pool = kv_pool(h.k, h.v, h.ks, h.vs, layer);
+  a.step = kv_step(h.rows, h.k);
+  a.k = kk.data_ptr();
+  a.k_sb = kk.stride(0); a.k_st = kk.stride(1); a.k_sh = kk.stride(2);
+  a.v = vv.data_ptr();
+  a.v_sb = vv.stride(0); a.v_st = vv.stride(1); a.v_sh = vv.stride(2);
+  a.T = kk.size(1);
+  kv_step_wait(h);
   ddb::kv_cache_write(a, stream());
 }
 
-void kv_cache_attend(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs, int64_t layer,
-                     torch::Tensor rows, torch::Tensor q, torch::Tensor o, c10::optional<torch::Tensor> lse,
-                     bool causal, int64_t unit, int64_t window, int64_t sinks, double scale,
-                     int64_t max_tokens) {
+std::vector<torch::Tensor> kv_step_attend(std::shared_ptr<KvStepHandle> hp, int64_t layer, const torch::Tensor& q0,
+                                          const std::string& causal, int64_t tokens_per_frame, int64_t window,
+                                          int64_t sinks, c10::optional<double> scale, bool return_lse) {
+  KvStepHandle& h = *hp;
+  TORCH_CHECK_VALUE(layer >= 0 && layer < h.k.size(0), "layer ", layer, " of a cache of ", h.k.size(0));
+  const c10::cuda::CUDAGuard guard(h.k.device());
+  const auto q = kv_tokens(q0, "q", h, 0);
+  const auto m = window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale ? *scale : 0.125, 0, 0);
+  TORCH_CHECK_VALUE(h.trim_sinks == -1 || (window == 0 && sinks == 0) || h.trim_sinks == m.sinks,
+                    "a trimmed sequence keeps the first tokens it was trimmed to; the call names ", m.sinks, " sinks");
   ddb::KvAttendArgs a;
-  a.pool = kv_pool(k, v, ks, vs, layer);
-  a.step = kv_step(rows, k);
-  check_tokens(q, "queries", k, a.step.B);
-  TORCH_CHECK(a.pool.heads > 0 && q.size(2) % a.pool.heads == 0, "query heads must be a multiple of the cache's ", a.pool.heads);
-  check_bf16(o, "o");
-  TORCH_CHECK(o.is_contiguous() && o.sizes() == q.sizes() && o.device() == k.device() &&
-                  reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0, "o must be contiguous and like q");
-  TORCH_CHECK(unit >= 1 && unit <= (1 << 24) && window >= 0 && window <= (1 << 24) && sinks >= 0 && sinks <= (1 << 30) &&
-                  unit * window <= (1 << 30),
-              "kv_cache_attend: unit, window or sinks out of range");
-  TORCH_CHECK(q.size(1) * (q.size(2) / a.pool.heads) <= (1 << 30), "kv_cache_attend: too many query rows");
-  const c10::cuda::CUDAGuard guard(k.device());
+  a.pool = kv_pool(h.k, h.v, h.ks, h.vs, layer);
+  a.step = kv_step(h.rows, h.k);
+  TORCH_CHECK_VALUE(q.size(1) * (q.size(2) / a.pool.heads) <= (1 << 30), "too many query rows");
+  auto o = torch::empty(q.sizes(), q.options());
   a.q = q.data_ptr();
   a.q_sb = q.stride(0); a.q_st = q.stride(1); a.q_sh = q.stride(2);
   a.o = o.data_ptr();
-  if (lse) {
-    TORCH_CHECK(lse->scalar_type() == torch::kFloat32 && lse->is_contiguous() && lse->device() == k.device() &&
-                    lse->numel() == q.size(0) * q.size(1) * q.size(2), "lse must be contiguous fp32 [B, H, T]");
-    a.lse = lse->data_ptr<float>();
+  torch::Tensor lse;
+  if (return_lse) {
+    lse = torch::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(torch::kFloat32));
+    a.lse = lse.data_ptr<float>();
   }
   a.T = q.size(1);
   a.H = q.size(2);
-  a.causal = causal;
-  a.unit = unit;
-  a.window = window;
-  a.sinks = sinks;
-  a.scale = static_cast<float>(scale);
-  a.max_tokens = max_tokens;
+  a.causal = m.causal != ddb::kCausalNone;
+  a.unit = m.unit;
+  a.window = m.window;
+  a.sinks = m.sinks;
+  a.scale = static_cast<float>(m.scale);
+  a.max_tokens = h.max_tokens;
+  kv_step_wait(h);
   ddb::kv_cache_attend(a, stream());
+  if (return_lse) return {o, lse};
+  return {o};
 }
 
-void kv_cache_copy_pages(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
-                         std::vector<int64_t> src, std::vector<int64_t> dst) {
-  TORCH_CHECK(k.dim() == 5, "cache codes must be [layers, pages, heads, 64, 64]");
-  if (k.size(0) == 0) return;
+// src, dst: int32 in host memory
+void kv_cache_copy_pages(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs, torch::Tensor src,
+                         torch::Tensor dst) {
   const auto p = kv_pool(k, v, ks, vs, 0);
   TORCH_CHECK(k.size(0) <= 65535, "cache too large");
-  TORCH_CHECK(src.size() == dst.size(), "as many pages to copy from as to");
-  std::vector<int> s(src.size()), d(dst.size());
+  for (const auto* t : {&src, &dst})
+    TORCH_CHECK(t->device().is_cpu() && t->scalar_type() == torch::kInt32 && t->is_contiguous() && t->numel() == src.numel(),
+                "pages must be int32 in host memory, as many to copy from as to");
+  const int64_t n = src.numel();
+  const int *s = src.data_ptr<int>(), *d = dst.data_ptr<int>();
   std::vector<char> is_dst(p.pages, 0);
-  for (size_t i = 0; i < src.size(); ++i) {
-    TORCH_CHECK(src[i] >= 0 && src[i] < p.pages && dst[i] >= 0 && dst[i] < p.pages, "page id out of range");
-    TORCH_CHECK(!is_dst[dst[i]], "page ", dst[i], " is written twice");
-    is_dst[dst[i]] = 1;
-    s[i] = src[i];
-    d[i] = dst[i];
+  for (int64_t i = 0; i < n; ++i) {
+    TORCH_CHECK(s[i] >= 0 && s[i] < p.pages && d[i] >= 0 && d[i] < p.pages, "page id out of range");
+    TORCH_CHECK(!is_dst[d[i]], "page ", d[i], " is written twice");
+    is_dst[d[i]] = 1;
   }
-  for (const int x : s) TORCH_CHECK(!is_dst[x], "page ", x, " is read and written by one copy");
+  for (int64_t i = 0; i < n; ++i) TORCH_CHECK(!is_dst[s[i]], "page ", s[i], " is read and written by one copy");
   const c10::cuda::CUDAGuard guard(k.device());
-  ddb::kv_cache_copy_pages(p.k, p.v, p.k_scale, p.v_scale, k.size(0), p.pages, p.heads, s.data(), d.data(), s.size(), stream());
+  ddb::kv_cache_copy_pages(p.k, p.v, p.k_scale, p.v_scale, k.size(0), p.pages, p.heads, s, d, n, stream());
 }
 
 }  // namespace
@@ -1793,8 +1844,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("window_attention", &window_attention, "differentiable attention over a window and the first tokens");
   m.def("attn_window_fwd", &attn_window_fwd_py, "its forward, for callers with a backward of their own");
   m.def("attn_window_bwd", &attn_window_bwd_py, "its backward, into given gradients");
-  m.def("kv_cache_write", &kv_cache_write, "tokens into the pages of an 8-bit key/value cache");
-  m.def("kv_cache_attend", &kv_cache_attend, "attention over an 8-bit paged key/value cache");
+  py::class_<KvStepHandle, std::shared_ptr<KvStepHandle>>(m, "KvStepHandle").def_readonly("rows", &KvStepHandle::rows);
+  m.def("kv_step_begin", &kv_step_begin, "a step's table on the device");
+  m.def("kv_step_write", &kv_step_write, "tokens into the pages of an 8-bit key/value cache");
+  m.def("kv_step_attend", &kv_step_attend, "attention over an 8-bit paged key/value cache");
   m.def("kv_cache_copy_pages", &kv_cache_copy_pages, "copy cache pages in every layer");
   m.def("attn_delta", &attn_delta, "rowsum(dO * O) per head");
   m.def("ipc_alloc", &ipc_alloc, "cudaMalloc + IPC handle -> (ptr, handle)");

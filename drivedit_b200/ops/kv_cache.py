@@ -30,28 +30,37 @@ any tensor. Bookkeeping is on the host: calls on one cache come from one thread.
 """
 from __future__ import annotations
 
-import heapq
 import math
 from typing import List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 
 from ._ext import ext
+from .window_attention import _check_mask
 
 PAGE = 64       # tokens of a page
 _INFO = 4       # words of a step's row before its page ids
 _MAX_TOKENS = 1 << 30
 
 
+def _pages(tokens: int) -> int:
+    return (tokens + PAGE - 1) // PAGE
+
+
 class _Seq:
     __slots__ = ("pages", "length", "first", "sinks", "version")
 
-    def __init__(self):
-        self.pages: List[int] = []  # ids by page of the sequence; -1: given back
-        self.length = 0             # committed tokens
-        self.first = 0              # tokens in [sinks, first) are gone
-        self.sinks = 0
+    def __init__(self, pages, length=0, first=0, sinks=0):
+        self.pages = pages          # int32 ids by page of the sequence; -1: given back
+        self.length = length        # committed tokens
+        self.first = first          # tokens in [sinks, first) are gone
+        self.sinks = sinks
         self.version = 0            # a step begun at another version is stale
+
+    @property
+    def trimmed(self):
+        return self.first > self.sinks
 
 
 def _two_to(e: torch.Tensor) -> torch.Tensor:
@@ -76,65 +85,51 @@ class CacheStep:
     Once a sequence of the step has changed otherwise (commit, trim, fork, free, a later
     ``begin``, compaction) the step is stale and its calls raise."""
 
-    def __init__(self, cache: "PagedKVCache", seqs, n_new, rows, max_tokens):
+    def __init__(self, cache: "PagedKVCache", seqs, n_new, max_tokens, table, handle):
         self.cache = cache
         self.seqs, self.n_new = seqs, n_new
         self.max_tokens = max_tokens  # launches are shaped for sequences up to this length
-        self.rows = rows              # int32 [B, 4 + max_pages_per_seq]
         self._states = [cache._seqs[i] for i in seqs]
         self._versions = [s.version for s in self._states]
-        self._ready = None            # (event, stream) of the rows' upload
+        self._epoch = cache._epoch
+        self._rows, self._h = table, handle
 
     @property
     def table(self) -> torch.Tensor:
         """Page ids by sequence, int32 ``[B, max_pages_per_seq]`` (-1: none)."""
-        return self.rows[:, _INFO:]
+        return (self._rows if self._h is None else self._h.rows)[:, _INFO:]
 
     def _check(self):
-        if any(s.version != v for s, v in zip(self._states, self._versions)):
-            raise RuntimeError("stale step: a sequence has changed since it was begun; begin a new one")
-        if self._ready is not None and not torch.cuda.is_current_stream_capturing():
-            event, stream = self._ready
-            now = torch.cuda.current_stream(self.rows.device)
-            if now != stream:
-                now.wait_event(event)
-                self.rows.record_stream(now)
+        if self._epoch != self.cache._epoch:  # something of the cache has changed
+            if any(s.version != v for s, v in zip(self._states, self._versions)):
+                raise RuntimeError("stale step: a sequence has changed since it was begun; begin a new one")
+            self._epoch = self.cache._epoch
 
     def _tokens(self, x: torch.Tensor, name: str, heads: Optional[int]):
+        """The extension's checks, for the PyTorch form."""
         c = self.cache
         if x.dim() != 4 or x.shape[0] != len(self.seqs) or x.shape[3] != 64:
             raise ValueError(f"{name} must be [{len(self.seqs)}, T, heads, 64], got {tuple(x.shape)}")
-        if heads is not None and x.shape[2] != heads:
-            raise ValueError(f"{name} has {x.shape[2]} heads, the cache {heads}")
-        if x.shape[2] == 0 or x.shape[2] % c.n_heads:
-            raise ValueError(f"{name}'s {x.shape[2]} heads are no multiple of the cache's {c.n_heads}")
+        if heads is not None and x.shape[2] != heads or x.shape[2] == 0 or x.shape[2] % c.n_heads:
+            raise ValueError(f"{name} has {x.shape[2]} heads, the cache {c.n_heads}")
         if x.shape[1] < max(self.n_new, default=0):
             raise ValueError(f"{name} holds {x.shape[1]} tokens, the step {max(self.n_new)}")
         if x.device != c.device:
             raise ValueError(f"{name} is on {x.device}, the cache on {c.device}")
-        if c.device.type == "cuda":
-            if x.dtype != torch.bfloat16:
-                raise ValueError(f"{name} must be bfloat16 on CUDA, got {x.dtype}")
-            # the kernels read 16 bytes at a time from rows of contiguous channels
-            if x.numel() and (x.stride(3) != 1 or any(s % 8 for s in x.stride()[:3]) or x.data_ptr() % 16):
-                x = x.contiguous()
-                if x.data_ptr() % 16:
-                    x = x.clone()
-        return x
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Cache the new tokens' ``k``, ``v`` ``[B, T, n_heads, 64]`` (any strides; sequence
         ``i`` has the first ``n_new[i]`` rows, the others are not read)."""
-        c = self.cache
         self._check()
+        if self._h is not None:
+            ext().kv_step_write(self._h, layer, k, v)
+            return
+        c = self.cache
         c._layer(layer)
-        k, v = self._tokens(k, "k", c.n_heads), self._tokens(v, "v", c.n_heads)
+        self._tokens(k, "k", c.n_heads), self._tokens(v, "v", c.n_heads)
         if k.shape != v.shape:
             raise ValueError("k and v differ in shape")
-        if c.device.type == "cuda":
-            ext().kv_cache_write(c.k, c.v, c.k_scale, c.v_scale, layer, self.rows, k, v)
-        else:
-            self._write_torch(layer, k, v)
+        self._write_torch(layer, k, v)
 
     def attend(self, layer: int, q: torch.Tensor, causal: str = "frame", tokens_per_frame: int = 1,
                window: int = 0, sinks: int = 0, scale: Optional[float] = None, return_lse: bool = False):
@@ -148,39 +143,25 @@ class CacheStep:
         them. Of a trimmed sequence what :meth:`PagedKVCache.trim` kept is visible at most.
         Returns ``o [B, T, heads, 64]`` (and ``lse [B, heads, T]``, log2 domain); rows
         behind a sequence's ``n_new`` and rows that see no key are zero (-inf)."""
-        c = self.cache
         self._check()
+        if self._h is not None:
+            out = ext().kv_step_attend(self._h, layer, q, causal, tokens_per_frame, window, sinks, scale, return_lse)
+            return tuple(out) if return_lse else out[0]
+        c = self.cache
         c._layer(layer)
-        q = self._tokens(q, "q", None)
-        if causal not in ("frame", "token", "none"):
-            raise ValueError(f"causal must be frame, token or none, got {causal!r}")
-        unit = tokens_per_frame if causal == "frame" else 1
-        if unit < 1 or window < 0 or sinks < 0:
-            raise ValueError("tokens_per_frame must be positive, window and sinks not negative")
-        if causal == "none" and (window or sinks):
-            raise ValueError("a window needs causal frame or token")
-        if unit > 1 << 24:
-            raise ValueError("at most 2^24 tokens per frame")
-        # a window or sinks past every token mean all of them
-        window = window if window * unit <= _MAX_TOKENS and window <= 1 << 24 else 0
-        n_sink = min(sinks * unit, _MAX_TOKENS)
+        self._tokens(q, "q", None)
         scale = 1.0 / math.sqrt(64) if scale is None else float(scale)
-        if not (scale > 0 and math.isfinite(scale)):
-            raise ValueError("scale must be positive and finite")
-        for s in self._states:
-            if s.first > s.sinks and s.sinks != n_sink and (window or sinks):
-                raise ValueError(f"a sequence was trimmed to its first {s.sinks} tokens, the call names {n_sink} sinks")
-        if c.device.type != "cuda":
-            return self._attend_torch(layer, q, causal, unit, window, n_sink, scale, return_lse)
-        o = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
-        lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device) if return_lse else None
-        ext().kv_cache_attend(c.k, c.v, c.k_scale, c.v_scale, layer, self.rows, q, o, lse, causal != "none",
-                              unit, window, n_sink, scale, self.max_tokens)
-        return (o, lse) if return_lse else o
+        _check_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, 0, 0)
+        unit = tokens_per_frame if causal == "frame" else 1
+        n_sink = min(sinks * unit, _MAX_TOKENS)
+        if (window or sinks) and any(s.trimmed and s.sinks != n_sink for s in self._states):
+            raise ValueError(f"a trimmed sequence keeps the first tokens it was trimmed to; the call names {n_sink} sinks")
+        return self._attend_torch(layer, q, causal, unit, window, n_sink, scale, return_lse)
 
     def commit(self) -> None:
         """Keep the step's tokens: its sequences grow by ``n_new``."""
         self._check()
+        self.cache._epoch += 1
         for s, n in zip(self._states, self.n_new):
             s.length += n
             s.version += 1
@@ -189,7 +170,7 @@ class CacheStep:
     def _write_torch(self, layer, k, v):
         c = self.cache
         for i, (s, n) in enumerate(zip(self._states, self.n_new)):
-            for j in range(s.length // PAGE, -(-(s.length + n) // PAGE)) if n else ():
+            for j in range(s.length // PAGE, _pages(s.length + n)) if n else ():
                 lo, hi = max(s.length, j * PAGE), min(s.length + n, (j + 1) * PAGE)
                 kept = max(0, s.length - j * PAGE)
                 for codes, scales, new, last in ((c.k, c.k_scale, k, False), (c.v, c.v_scale, v, True)):
@@ -219,7 +200,7 @@ class CacheStep:
             seen = kf <= qf if causal != "none" else torch.ones(n, total, dtype=torch.bool, device=q.device)
             if window:
                 seen = seen & ((kf > qf - window) | (pos < n_sink))
-            if s.first > s.sinks:
+            if s.trimmed:
                 seen = seen & ((pos >= s.first) | (pos < s.sinks))
             sc = sc.masked_fill(~seen, -math.inf)
             ls = torch.logsumexp(sc, -1)
@@ -254,10 +235,11 @@ class PagedKVCache:
         if not 1 <= self.max_pages_per_seq <= _MAX_TOKENS // PAGE:
             raise ValueError("max_pages_per_seq out of range")
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
-        self._free: List[int] = list(range(n_pages))
-        self._refs = [0] * n_pages
+        self._refs = np.zeros(n_pages, np.int32)  # sequences that hold a page
+        self._n_free, self._low = n_pages, 0      # no page below _low is free
         self._seqs: dict = {}
         self._next = 0
+        self._epoch = 0                           # counts changes of any sequence
 
     def _pool(self, n):
         shape = (self.n_layers, n, self.n_heads)
@@ -278,26 +260,36 @@ class PagedKVCache:
         return [self._seqs[i] for i in seqs]
 
     def _need(self, n):
-        if n > len(self._free):
-            raise RuntimeError(f"out of cache pages: {n} needed, {len(self._free)} of {self.n_pages} free")
+        if n > self._n_free:
+            raise RuntimeError(f"out of cache pages: {n} needed, {self._n_free} of {self.n_pages} free")
 
-    def _take(self) -> int:
-        page = heapq.heappop(self._free)
-        self._refs[page] = 1
-        return page
+    def _take(self, n: int) -> np.ndarray:
+        """The ``n`` lowest free pages (there are as many)."""
+        ids = np.flatnonzero(self._refs[self._low:self._low + 4 * n + 256] == 0)
+        if len(ids) < n:
+            ids = np.flatnonzero(self._refs[self._low:] == 0)
+        ids = (ids[:n] + self._low).astype(np.int32)
+        if n:
+            self._refs[ids] = 1
+            self._n_free -= n
+            self._low = int(ids[-1]) + 1
+        return ids
 
-    def _give(self, page: int):
-        if page < 0:
-            return
-        self._refs[page] -= 1
-        if not self._refs[page]:
-            heapq.heappush(self._free, page)
+    def _give(self, pages: np.ndarray) -> None:
+        """One sequence's hold of these pages ends."""
+        pages = pages[pages >= 0]
+        self._refs[pages] -= 1
+        freed = pages[self._refs[pages] == 0]
+        if len(freed):
+            self._n_free += len(freed)
+            self._low = min(self._low, int(freed.min()))
 
-    def _copy(self, src: Sequence[int], dst: Sequence[int]):
-        if not src:
+    def _copy(self, src, dst):
+        if not len(src):
             return
         if self.device.type == "cuda":
-            ext().kv_cache_copy_pages(self.k, self.v, self.k_scale, self.v_scale, list(src), list(dst))
+            ids = [torch.from_numpy(np.ascontiguousarray(x, np.int32)) for x in (src, dst)]
+            ext().kv_cache_copy_pages(self.k, self.v, self.k_scale, self.v_scale, *ids)
         else:
             for t in (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale):
                 t[:, list(dst)] = t[:, list(src)]
@@ -308,7 +300,7 @@ class PagedKVCache:
 
     @property
     def free_pages(self) -> int:
-        return len(self._free)
+        return self._n_free
 
     @property
     def sequences(self) -> List[int]:
@@ -323,18 +315,11 @@ class PagedKVCache:
 
     def table(self, seqs: Sequence[int]) -> torch.Tensor:
         """Page ids of the sequences, int32 ``[n, max_pages_per_seq]`` (-1: none)."""
-        return self._upload([s.pages for s in self._get(seqs)], self.max_pages_per_seq)
-
-    def _upload(self, rows, width, out=None):
-        # pinned memory from the caching host allocator: kept until the copy has run
-        t = torch.empty(len(rows), width, dtype=torch.int32, pin_memory=self.device.type == "cuda")
-        a = t.numpy()
-        a.fill(-1)
-        for i, r in enumerate(rows):
-            a[i, :len(r)] = r
-        if out is not None:
-            return out.copy_(t, non_blocking=True)
-        return t.to(self.device, non_blocking=True) if self.device.type == "cuda" else t
+        rows = np.full((len(seqs), self.max_pages_per_seq), -1, np.int32)
+        for i, s in enumerate(self._get(seqs)):
+            rows[i, :len(s.pages)] = s.pages
+        rows = torch.from_numpy(rows)
+        return rows.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else rows
 
     # ------------------------------------------------------------------ sequences
     def add(self, n: int = 1) -> List[int]:
@@ -344,7 +329,7 @@ class PagedKVCache:
         ids = list(range(self._next, self._next + n))
         self._next += n
         for i in ids:
-            self._seqs[i] = _Seq()
+            self._seqs[i] = _Seq(np.empty(0, np.int32))
         return ids
 
     def begin(self, seqs: Sequence[int], n_new: Union[int, Sequence[int]], max_tokens: Optional[int] = None,
@@ -373,52 +358,62 @@ class PagedKVCache:
         max_tokens = longest if max_tokens is None else int(max_tokens)
         if max_tokens < longest:
             raise ValueError(f"sequences of {longest} tokens in a step for {max_tokens}")
-        # pages to take: behind the present ones, and for a shared page that gets new tokens.
-        # Of pages shared within this call the last one to write keeps the page.
-        need, left = 0, {}
+        # Pages to take: behind the present ones, and for shared pages that get new tokens (of
+        # a page shared within this call the last one to write keeps it). Pages behind the
+        # new tokens are the room of an abandoned step.
+        need, spare, shared = 0, 0, {}
         for s, n in zip(states, n_new):
-            have = -(-s.length // PAGE)
-            need += max(0, -(-(s.length + n) // PAGE) - len(s.pages))
-            for j in range(s.length // PAGE, min(-(-(s.length + n) // PAGE), len(s.pages))) if n else ():
-                p = s.pages[j]
-                left[p] = left.get(p, self._refs[p]) - 1
-                need += left[p] > 0
-            need -= max(0, len(s.pages) - max(have, -(-(s.length + n) // PAGE)))
-        self._need(need)
-        moves = []
+            have, upto = len(s.pages), _pages(s.length + n)
+            need += max(0, upto - have)
+            spare += max(0, have - upto)
+            for j in range(s.length // PAGE, min(upto, have)) if n else ():
+                p = int(s.pages[j])
+                if self._refs[p] > 1:
+                    shared[p] = shared.get(p, int(self._refs[p])) - 1
+                    need += shared[p] > 0
+        self._need(need - spare)
+        self._epoch += 1
+        if spare:
+            for s, n in zip(states, n_new):
+                upto = _pages(s.length + n)
+                if len(s.pages) > upto:
+                    self._give(s.pages[upto:])
+                    s.pages = s.pages[:upto]
+        fresh = iter(self._take(need).tolist())
+        src, dst = [], []
         for s, n in zip(states, n_new):
-            upto = -(-(s.length + n) // PAGE)
-            while len(s.pages) > upto:  # room of an abandoned step
-                self._give(s.pages.pop())
-        for s, n in zip(states, n_new):
-            upto = -(-(s.length + n) // PAGE)
-            for j in range(s.length // PAGE, upto) if n else ():
-                if j < len(s.pages):
-                    p = s.pages[j]
-                    if self._refs[p] > 1:
-                        s.pages[j] = self._take()
-                        if j * PAGE < s.length:
-                            moves.append((p, s.pages[j]))
-                        self._give(p)
-                else:
-                    s.pages.append(self._take())
             s.version += 1
-        self._copy([a for a, _ in moves], [b for _, b in moves])
-        W = self.max_pages_per_seq
-        rows = [[s.length + n, n, *((s.first, s.sinks) if s.first > s.sinks else (0, -1))] + s.pages
-                for s, n in zip(states, n_new)]
-        rows = self._upload(rows, _INFO + W, None if out is None else out.rows)
-        if out is None:
-            step = CacheStep(self, list(seqs), n_new, rows, max_tokens)
-        else:
-            step = out
-            out.__init__(self, list(seqs), n_new, rows, max_tokens)
+            have, upto = len(s.pages), _pages(s.length + n)
+            if shared and n:
+                for j in range(s.length // PAGE, min(upto, have)):
+                    p = int(s.pages[j])
+                    if self._refs[p] > 1:
+                        s.pages = s.pages.copy()
+                        s.pages[j] = next(fresh)
+                        if j * PAGE < s.length:
+                            src.append(p)
+                            dst.append(s.pages[j])
+                        self._refs[p] -= 1
+            if upto > have:
+                s.pages = np.concatenate([s.pages, np.array([next(fresh) for _ in range(upto - have)], np.int32)])
+        self._copy(src, dst)
+        rows = np.full((len(states), _INFO + self.max_pages_per_seq), -1, np.int32)
+        trim = -1
+        for i, (s, n) in enumerate(zip(states, n_new)):
+            if s.trimmed:
+                rows[i, :_INFO] = s.length + n, n, s.first, s.sinks
+                trim = s.sinks if trim in (-1, s.sinks) else -2
+            else:
+                rows[i, :3] = s.length + n, n, 0
+            rows[i, _INFO:_INFO + len(s.pages)] = s.pages
+        rows, handle = torch.from_numpy(rows), None
         if self.device.type == "cuda":
-            stream = torch.cuda.current_stream(self.device)
-            event = torch.cuda.Event()
-            event.record(stream)
-            step._ready = (event, stream)
-        return step
+            handle = ext().kv_step_begin(self.k, self.v, self.k_scale, self.v_scale, rows, max_tokens, max(n_new, default=0),
+                                         trim, None if out is None else out._h)
+        if out is None:
+            return CacheStep(self, list(seqs), n_new, max_tokens, rows, handle)
+        out.__init__(self, list(seqs), n_new, max_tokens, rows, handle)
+        return out
 
     def fork(self, seqs: Sequence[int], copies: int = 1) -> List[int]:
         """``copies`` new sequences from each of ``seqs`` (all copies of the first, then of the
@@ -426,39 +421,38 @@ class PagedKVCache:
         states = self._get(seqs)
         if copies < 0:
             raise ValueError("copies must not be negative")
-        out = []
-        for s in states:
+        self._epoch += 1
+        out = self.add(copies * len(states))
+        for i, s in enumerate(states):
             s.version += 1
-            n = -(-s.length // PAGE)
-            for i in self.add(copies):
-                t = self._seqs[i]
-                t.pages, t.length, t.first, t.sinks = s.pages[:n], s.length, s.first, s.sinks
-                for p in t.pages:
-                    if p >= 0:
-                        self._refs[p] += 1
-                out.append(i)
+            pages = s.pages[:_pages(s.length)]
+            self._refs[pages[pages >= 0]] += copies
+            for k in out[i * copies:(i + 1) * copies]:
+                self._seqs[k] = _Seq(pages.copy(), s.length, s.first, s.sinks)
         return out
 
     def copy(self, seqs: Sequence[int]) -> List[int]:
         """New sequences with the committed tokens of ``seqs`` in pages of their own."""
         self._not_capturing("copy")
         states = self._get(seqs)
-        kept = [s.pages[:-(-s.length // PAGE)] for s in states]
-        self._need(sum(p >= 0 for ps in kept for p in ps))
-        out, moves = self.add(len(states)), []
-        for i, s, ps in zip(out, states, kept):
-            t = self._seqs[i]
-            t.length, t.first, t.sinks = s.length, s.first, s.sinks
-            t.pages = [self._take() if p >= 0 else -1 for p in ps]
-            moves += [(a, b) for a, b in zip(ps, t.pages) if a >= 0]
-        self._copy([a for a, _ in moves], [b for _, b in moves])
+        kept = [s.pages[:_pages(s.length)] for s in states]
+        src = np.concatenate([p[p >= 0] for p in kept]) if kept else np.empty(0, np.int32)
+        self._need(len(src))
+        dst = self._take(len(src))
+        out, at = self.add(len(states)), 0
+        for i, s, p in zip(out, states, kept):
+            pages, n = p.copy(), int((p >= 0).sum())
+            pages[p >= 0] = dst[at:at + n]
+            at += n
+            self._seqs[i] = _Seq(pages, s.length, s.first, s.sinks)
+        self._copy(src, dst)
         return out
 
     def free(self, seqs: Sequence[int]) -> None:
         """Drop sequences; pages that no other sequence shares become free."""
+        self._epoch += 1
         for i, s in zip(list(seqs), self._get(seqs)):
-            for p in s.pages:
-                self._give(p)
+            self._give(s.pages)
             s.version += 1
             del self._seqs[i]
 
@@ -468,64 +462,69 @@ class PagedKVCache:
         states = self._get(seqs)
         if keep < 0 or sinks < 0:
             raise ValueError("keep and sinks must not be negative")
-        if any(s.first > s.sinks and s.sinks != sinks for s in states):
+        if any(s.trimmed and s.sinks != sinks for s in states):
             raise ValueError("a sequence that was trimmed keeps its number of sinks")
+        self._epoch += 1
         for s in states:
             first = max(s.first, s.length - keep)
             if first <= sinks:
                 continue
             s.first, s.sinks = first, sinks
-            for j in range(-(-sinks // PAGE), min(first // PAGE, len(s.pages))):
-                self._give(s.pages[j])
-                s.pages[j] = -1
+            lo, hi = _pages(sinks), min(first // PAGE, len(s.pages))
+            if hi > lo:
+                self._give(s.pages[lo:hi])
+                s.pages = s.pages.copy()
+                s.pages[lo:hi] = -1
             s.version += 1
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool; returns how many there are."""
         self._not_capturing("compact")
-        used = [p for p in range(self.n_pages) if self._refs[p]]
-        n = len(used)
-        src = [p for p in used if p >= n]
-        dst = [p for p in range(n) if not self._refs[p]]
-        if src:
+        used = self._refs > 0
+        n = self.n_pages - self._n_free
+        src, dst = np.flatnonzero(used[n:]) + n, np.flatnonzero(~used[:n])
+        if len(src):
+            self._epoch += 1
             self._copy(src, dst)
-            to = dict(zip(src, dst))
+            to = np.arange(self.n_pages, dtype=np.int32)
+            to[src] = dst
             for s in self._seqs.values():
-                if any(p in to for p in s.pages):
-                    s.pages = [to.get(p, p) for p in s.pages]
+                moved = np.where(s.pages >= 0, to[s.pages], -1).astype(np.int32)
+                if not np.array_equal(moved, s.pages):
+                    s.pages = moved
                     s.version += 1
-            for a, b in to.items():
-                self._refs[b], self._refs[a] = self._refs[a], 0
-            self._free = list(range(n, self.n_pages))
+            self._refs[dst] = self._refs[src]
+            self._refs[src] = 0
+            self._low = n
         return n
 
     def resize(self, n_pages: int) -> None:
         """Change the pool to ``n_pages`` pages (compacted first when it shrinks below a page
         in use); the pages in use keep their contents."""
         self._not_capturing("resize")
-        used = sum(r > 0 for r in self._refs)
+        used = self.n_pages - self._n_free
         if n_pages < max(used, 1):
             raise ValueError(f"{used} pages are in use, {n_pages} asked for")
-        if any(self._refs[n_pages:]):
+        if self._refs[n_pages:].any():
             self.compact()
         old, n = (self.k, self.v, self.k_scale, self.v_scale), min(n_pages, self.n_pages)
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
         for a, b in zip((self.k, self.v, self.k_scale, self.v_scale), old):
             a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
             a[:, :n].copy_(b[:, :n])
-        self._refs = self._refs[:n] + [0] * (n_pages - n)
-        self._free = [p for p in range(n_pages) if not self._refs[p]]
-        self.n_pages = n_pages
+        self._refs = np.concatenate([self._refs[:n], np.zeros(n_pages - n, np.int32)])
+        self._n_free, self._low, self.n_pages = n_pages - used, 0, n_pages
+        self._epoch += 1
         for s in self._seqs.values():
             s.version += 1
 
     def _values(self, layer, s: _Seq, n: int):
-        ids = torch.tensor([max(p, 0) for p in s.pages[:-(-n // PAGE)]], dtype=torch.long, device=self.device)
+        ids = torch.from_numpy(np.maximum(s.pages[:_pages(n)], 0)).long().to(self.device)
         out = []
         for codes, scales, last in ((self.k, self.k_scale, False), (self.v, self.v_scale, True)):
             x = codes[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float() * scales[layer, ids][..., None, None]
             x = (x.mT if last else x).transpose(1, 2).reshape(-1, self.n_heads, 64)[:n]
-            if s.first > s.sinks:
+            if s.trimmed:
                 x = x.clone()
                 x[s.sinks:s.first] = 0
             out.append(x)

@@ -30,6 +30,12 @@ nvcc_flags = [
     "-DNDEBUG",
 ]
 
+# The C++ library is shared with torch's: linked statically (what g++ does where only the archive
+# is installed beside it), its streams are initialised apart from torch's, and an error
+# message that prints a number ends the process.
+libstdcxx = [f"-L{d}" for d in ("/usr/lib/x86_64-linux-gnu",) if os.path.exists(os.path.join(d, "libstdc++.so.6"))]
+libstdcxx = libstdcxx + ["-l:libstdc++.so.6"] if libstdcxx else []
+
 data_sources = sorted(glob.glob(os.path.join(CSRC, "data", "*.cpp")))
 ext_modules = [
         CUDAExtension(
@@ -37,6 +43,7 @@ ext_modules = [
             sources=[os.path.relpath(s, ROOT) for s in sources],
             include_dirs=[CSRC],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": nvcc_flags},
+            extra_link_args=libstdcxx,
         ),
 ]
 if data_sources:
@@ -49,7 +56,7 @@ if data_sources:
             include_dirs=[CSRC],
             extra_compile_args=["-O3", "-std=c++17", "-pthread"],
             libraries=["z"],
-            extra_link_args=["-pthread"],
+            extra_link_args=["-pthread"] + libstdcxx,
         )
     )
 

@@ -185,7 +185,7 @@ def test_cache_refusals_change_nothing():
     c = PagedKVCache(1, 2, 4, device="cpu", max_pages_per_seq=3)
     a, b = c.add(2)
     step, k, v = _write(c, [a], 100)
-    state = lambda: (c.free_pages, [(s.pages[:], s.length, s.version) for s in c._seqs.values()], c._refs[:])  # noqa: E731
+    state = lambda: (c.free_pages, [(s.pages.tolist(), s.length, s.version) for s in c._seqs.values()], c._refs.tolist())  # noqa: E731
     was = state()
     q = torch.randn(1, 100, 2, 64)
     for error, call in (
