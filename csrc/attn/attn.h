@@ -61,8 +61,8 @@ struct AttnArgs {
   long v_sb = 0, v_st = 0, v_sh = 0;
 };
 
-void attn_window_fwd(const AttnArgs& a, cudaStream_t s);
-int attn_window_kv_splits(const AttnArgs& a);  // as attn_fwd_kv_splits, for attn_window_fwd
+// splits: CTAs that share a query tile's keys, at most 8 (0: chosen for the launch)
+void attn_window_fwd(const AttnArgs& a, int splits, cudaStream_t s);
 
 void attn_fwd(const AttnArgs& a, cudaStream_t s);
 // key-range splits attn_fwd would use for `a` on this device (1: no scratch needed) and

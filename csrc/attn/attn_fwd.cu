@@ -25,13 +25,15 @@
 //
 // Windowed mode (attn_window_fwd): the keys of the newest frames and the first ones; a
 // query tile walks only tiles with a visible key. Any number of queries and keys, any
-// strides of the heads' rows.
+// strides of the heads' rows. Its split-KV CTAs are a cluster and merge through
+// distributed shared memory: no scratch memory, no second launch.
 // Semantics oracle: layers/attention.py attention_reference (reference layers/mha.py:88-116
 // with fp32 softmax), layers/sla.py sla_sparse_reference.
 #include <cuda.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <stdexcept>
 
 #include "../common/ptx.cuh"
@@ -55,6 +57,8 @@ constexpr int OFF_BAR = OFF_V + NS * TILE_BYTES;
 // reserved)) would not fit the SM's 228 KB and only one would be resident.
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 static_assert(2 * (SMEM_BYTES + 1024) <= 233472, "two CTAs per SM");
+constexpr int OFF_ML = OFF_K + 128 * 256;  // windowed split-KV: (maximum, sum) per row behind O
+static_assert(OFF_ML + 128 * 8 <= OFF_V, "the split's result fits the K ring");
 constexpr uint32_t TMEM_COLS = 256;
 constexpr uint32_t S_COL = 0;
 constexpr uint32_t O_COL = 128;
@@ -525,7 +529,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
-    if (row_ok && splits > 1) {
+    if (WIN && splits > 1) {
+      // this CTA's unnormalised O, maximum and sum, over the K ring (every product is done)
+      const uint32_t dst = smem_u32(smem + OFF_K) + r * 256;
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        st_shared_v4(dst + ((c ^ (r & 15)) << 4), __float_as_uint(ov[4 * c]), __float_as_uint(ov[4 * c + 1]),
+                     __float_as_uint(ov[4 * c + 2]), __float_as_uint(ov[4 * c + 3]));
+      *reinterpret_cast<float2*>(smem + OFF_ML + r * 8) = make_float2(m, l);
+    } else if (row_ok && splits > 1) {
       // this split's normalised O (fp32) and lse; attn_split_merge_kernel combines them
       const float inv = l > 0.f ? 1.f / l : 0.f;
       const long prow = static_cast<long>(split) * a.B * a.Tq + static_cast<long>(b) * a.Tq + q_local;
@@ -555,6 +567,36 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
+  }
+  if (WIN && splits > 1) {
+    // The CTAs that share the query tile form a cluster; each adds up its share of the rows
+    // through distributed shared memory, in rank order: 16 threads a row, 4 channels each.
+    cluster_sync_all();
+    const uint32_t res = smem_u32(smem + OFF_K), ml = smem_u32(smem + OFF_ML);
+    for (int i = threadIdx.x + split * kThreads; i < 128 * 16; i += splits * kThreads) {
+      const int r = i >> 4, c = i & 15, q = q0 + r;
+      if (q >= a.Tq) break;
+      float top = -INFINITY, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < splits; ++k) top = fmaxf(top, ld_cluster_v2(mapa_shared(ml + r * 8, k)).x);
+      if (top != -INFINITY)
+        for (int k = 0; k < splits; ++k) {
+          const float2 x = ld_cluster_v2(mapa_shared(ml + r * 8, k));
+          const float4 y = ld_cluster_v4(mapa_shared(res + r * 256 + ((c ^ (r & 15)) << 4), k));
+          const float w = exp2f(x.x - top);
+          sum += w * x.y;
+          v.x += w * y.x;
+          v.y += w * y.y;
+          v.z += w * y.z;
+          v.w += w * y.w;
+        }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) + (b * a.q_rows_per_b + q) * a.ldo + h * 64 + c * 4;
+      *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+      if (a.lse && c == 0)
+        a.lse[static_cast<long>(bh) * a.lse_ld + q] = sum > 0.f ? top + __log2f(sum) : -INFINITY;
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its results
   }
 }
 
@@ -591,7 +633,7 @@ __global__ void __launch_bounds__(256) attn_split_merge_kernel(const AttnArgs a)
   __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) +
                         (b * a.q_rows_per_b + q) * a.ldo + a.o_col + h * 64;
   *reinterpret_cast<uint32_t*>(orow + 2 * lane) = pack_bf16(o0 * inv, o1 * inv);
-  if (a.lse && lane == 0) a.lse[bh * (a.lse_ld ? a.lse_ld : a.Tq) + q] = wsum > 0.f ? mx + __log2f(wsum) : -INFINITY;
+  if (a.lse && lane == 0) a.lse[bh * a.Tq + q] = wsum > 0.f ? mx + __log2f(wsum) : -INFINITY;
 }
 
 }  // namespace
@@ -672,51 +714,62 @@ int window_tile_count(const AttnArgs& a, long q0) {
 }
 }  // namespace
 
-int attn_window_kv_splits(const AttnArgs& a) {
-  if (a.B <= 0 || a.H <= 0 || a.Tq <= 0) return 1;
-  int dev = 0;
-  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  const long slots = 2L * num_sms(dev);  // two CTAs per SM
-  const long ctas = static_cast<long>(a.B) * a.H * ((a.Tq + 127) / 128);
-  if (ctas >= slots) return 1;
-  const int tiles = window_tile_count(a, (a.Tq - 1) / 128 * 128);
-  // time ~ waves x key tiles of a split: the fewest splits with the smallest estimate
-  int best = 1;
-  double best_t = 1.0;
-  for (int s = 2; s <= 8 && tiles / s >= 4; ++s) {
-    const double t = static_cast<double>((ctas * s + slots - 1) / slots) / s;
-    if (t < best_t - 1e-9) {
-      best_t = t;
-      best = s;
-    }
-  }
-  return best;
-}
-
-void attn_window_fwd(const AttnArgs& a, cudaStream_t stream) {
+void attn_window_fwd(const AttnArgs& a, int splits, cudaStream_t stream) {
   if (a.B <= 0 || a.H <= 0 || a.Tq <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   raise_smem_limit<attn_fwd_kernel<true>>(SMEM_BYTES, dev);
+  const int n_qtiles = (a.Tq + 127) / 128;
+  const long ctas = static_cast<long>(a.B) * a.H * n_qtiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  if (splits <= 0) {
+    // time ~ waves x key tiles of one CTA: the fewest splits of the last (longest) query
+    // tile's keys with the smallest estimate, 4 key tiles or more each. How many clusters of
+    // a size run at once is the device's to say; it counts one CTA per SM of the two that
+    // run. Measured at 192 query tiles of 69 key tiles: 1 split 137 us, 2 127, 3 136,
+    // 4 (chosen) 121, 8 145; 32 tiles of 25: 1 split 77 us, 4 28, 6 (chosen) 25, 8 23.
+    static std::atomic<int> fits[64][9];
+    const int tiles = window_tile_count(a, (a.Tq - 1) / 128 * 128);
+    double best = 0.;
+    splits = 1;
+    for (int s = 1; s <= 8 && (s == 1 || tiles / s >= 4); ++s) {
+      int slots = s == 1 ? 2 * num_sms(dev) : fits[dev & 63][s].load();
+      if (slots == 0) {
+        cfg.gridDim = dim3(s);
+        attr[0].val.clusterDim.x = s;
+        cfg.numAttrs = 1;
+        check_cuda(cudaOccupancyMaxActiveClusters(&slots, attn_fwd_kernel<true>, &cfg), "cudaOccupancyMaxActiveClusters");
+        slots = 2 * std::max(slots, 1);
+        fits[dev & 63][s].store(slots);
+      }
+      const double t = static_cast<double>((ctas + slots - 1) / slots) / s;
+      if (s == 1 || t < best - 1e-9) {
+        best = t;
+        splits = s;
+      }
+      if (s == 1 && ctas >= slots) break;  // every SM has work: no split
+    }
+  }
+  splits = std::min(splits, 8);
+  if (ctas * splits > 0x7fffffffL) throw std::runtime_error("attn_window_fwd: too many query tiles for one launch");
+  AttnArgs w = a;
+  w.kv_splits = splits;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * splits));
+  attr[0].val.clusterDim.x = splits;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
   const CUtensorMap tQ = window_tmap(a.q, a.B, a.Tq, a.H, a.q_sb, a.q_st, a.q_sh);
   const CUtensorMap tK = window_tmap(a.k, a.B, a.S, a.H, a.k_sb, a.k_st, a.k_sh);
   const CUtensorMap tV = window_tmap(a.v, a.B, a.S, a.H, a.v_sb, a.v_st, a.v_sh);
-  const int n_qtiles = (a.Tq + 127) / 128;
-  const int splits = a.kv_splits > 1 ? a.kv_splits : 1;
-  if (splits > 1 && (a.o_part == nullptr || a.lse_part == nullptr))
-    throw std::runtime_error("attn_window_fwd: split-KV needs both scratch buffers");
-  const long grid = static_cast<long>(a.B) * a.H * n_qtiles * splits;
-  if (grid > 0x7fffffffL) throw std::runtime_error("attn_window_fwd: too many query tiles for one launch");
-  attn_fwd_kernel<true><<<static_cast<int>(grid), kThreads, SMEM_BYTES, stream>>>(
-      tQ, tK, tV, a, n_qtiles, device_status(dev), FwdTrace{nullptr, 0});
+  check_cuda(cudaLaunchKernelEx(&cfg, attn_fwd_kernel<true>, tQ, tK, tV, w, n_qtiles, device_status(dev), FwdTrace{nullptr, 0}),
+             "attn_fwd_kernel (windowed) launch");
   count_launch();
-  check_cuda(cudaGetLastError(), "attn_fwd_kernel (windowed) launch");
-  if (splits > 1) {
-    const long items = static_cast<long>(a.B) * a.Tq * a.H;
-    attn_split_merge_kernel<<<static_cast<int>((items + 7) / 8), 256, 0, stream>>>(a);
-    count_launch();
-    check_cuda(cudaGetLastError(), "attn_split_merge_kernel launch");
-  }
 }
 
 }  // namespace ddb

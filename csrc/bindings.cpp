@@ -4,6 +4,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <cstring>
 #include <map>
 #include <utility>
 #include <ATen/cuda/CUDAContext.h>
@@ -1468,7 +1469,11 @@ bool tma_rows(const torch::Tensor& t) {
   return true;
 }
 // `t` as the kernels read it (a copy if its strides or alignment do not fit)
-torch::Tensor tma_ready(const torch::Tensor& t) { return tma_rows(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+torch::Tensor tma_ready(const torch::Tensor& t) {
+  if (tma_rows(t)) return t;
+  const c10::cuda::CUDAGuard guard(t.device());
+  return t.clone(at::MemoryFormat::Contiguous);
+}
 
 // o [B, T, H, 64], and lse [B, H, T rounded up to 128] (log2 domain)
 std::vector<torch::Tensor> attn_window_fwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
@@ -1479,18 +1484,7 @@ std::vector<torch::Tensor> attn_window_fwd(const torch::Tensor& q, const torch::
   auto lse = torch::empty({a.B, a.H, (a.Tq + 127) / 128 * 128}, q.options().dtype(torch::kFloat32));
   a.o = o.data_ptr(); a.ldo = a.H * 64;
   a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
-  const int splits = g_attn_kv_splits > 0 ? static_cast<int>(g_attn_kv_splits) : ddb::attn_window_kv_splits(a);
-  torch::Tensor scratch;  // of this call: streams and captured graphs share none
-  if (splits > 1) {
-    long oe = 0, le = 0;
-    ddb::attn_fwd_split_scratch(a, splits, &oe, &le);
-    oe = (oe + 63) / 64 * 64;
-    scratch = torch::empty({oe + le}, q.options().dtype(torch::kFloat32));
-    a.kv_splits = splits;
-    a.o_part = scratch.data_ptr<float>();
-    a.lse_part = a.o_part + oe;
-  }
-  ddb::attn_window_fwd(a, stream());
+  ddb::attn_window_fwd(a, static_cast<int>(g_attn_kv_splits), stream());
   return {o, lse};
 }
 
@@ -1584,10 +1578,20 @@ void refuse_eager_leaf(const torch::Tensor& t) {
 std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                                             const std::string& causal, int64_t tokens_per_frame, int64_t window,
                                             int64_t sinks, int64_t q_pos, int64_t kv_pos, c10::optional<double> scale) {
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(3) == 64 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
+                        q.size(2) == k.size(2) && q.size(3) == k.size(3),
+                    "q must be [B, T, H, 64], k and v [B, S, H, 64]: got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                        v.device() == q.device(), "q, k and v must be of one type and on one device");
   TORCH_CHECK_VALUE(q.scalar_type() == torch::kBFloat16, "window_attention takes bfloat16 on CUDA, got ", q.scalar_type());
   const auto m = window_mask(causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale ? *scale : 0.125, q.size(1), k.size(1));
   TORCH_CHECK_VALUE(q.size(1) <= 65536 * 64, "at most ", 65536 * 64, " queries per sample");
-  if (at::GradMode::is_enabled()) {
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+    auto out = attn_window_fwd(tma_ready(q), tma_ready(k), tma_ready(v), m);
+    out[1] = out[1].narrow(2, 0, q.size(1));
+    return out;
+  }
+  {
     const c10::cuda::CUDAGuard guard(q.device());
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
       for (const auto* t : {&q, &k, &v}) refuse_eager_leaf(*t);
@@ -1672,12 +1676,14 @@ std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, to
   const c10::cuda::CUDAGuard guard(k.device());
   auto h = out ? out : std::make_shared<KvStepHandle>();
   // pinned memory of the caching host allocator: kept until the copy has run
-  const auto staged = rows.pin_memory();
+  const auto staged = torch::empty(rows.sizes(), torch::TensorOptions().dtype(torch::kInt32).pinned_memory(true));
+  std::memcpy(staged.data_ptr(), rows.data_ptr(), rows.numel() * sizeof(int));
   if (out) {
     TORCH_CHECK(h->rows.sizes() == rows.sizes() && h->rows.device() == k.device(), "the refilled step has another shape");
     h->rows.copy_(staged, true);
   } else {
-    h->rows = staged.to(k.device(), torch::kInt32, true);
+    h->rows = torch::empty(rows.sizes(), k.options().dtype(torch::kInt32));
+    h->rows.copy_(staged, true);
   }
   h->k = k; h->v = v; h->ks = ks; h->vs = vs;
   h->max_tokens = max_tokens;

@@ -75,17 +75,6 @@ __device__ __forceinline__ float inverse_power(float p) {  // 1 / 2^e, e in [-12
 }
 // every warp has its role's registers
 __device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 
 __global__ void __launch_bounds__(kThreads, 1)
     kv_attend_tiles(const KvAttendArgs a, int row_tiles, int* status) {

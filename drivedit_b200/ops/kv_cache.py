@@ -276,13 +276,14 @@ class PagedKVCache:
         return ids
 
     def _give(self, pages: np.ndarray) -> None:
-        """One sequence's hold of these pages ends."""
-        pages = pages[pages >= 0]
-        self._refs[pages] -= 1
-        freed = pages[self._refs[pages] == 0]
+        """A hold of each of these pages ends (a page named twice has two)."""
+        held = np.bincount(pages[pages >= 0])
+        refs = self._refs[:len(held)]
+        refs -= held.astype(np.int32)
+        freed = np.flatnonzero((refs == 0) & (held > 0))
         if len(freed):
             self._n_free += len(freed)
-            self._low = min(self._low, int(freed.min()))
+            self._low = min(self._low, int(freed[0]))
 
     def _copy(self, src, dst):
         if not len(src):
@@ -361,16 +362,22 @@ class PagedKVCache:
         # Pages to take: behind the present ones, and for shared pages that get new tokens (of
         # a page shared within this call the last one to write keeps it). Pages behind the
         # new tokens are the room of an abandoned step.
-        need, spare, shared = 0, 0, {}
-        for s, n in zip(states, n_new):
-            have, upto = len(s.pages), _pages(s.length + n)
-            need += max(0, upto - have)
-            spare += max(0, have - upto)
+        refs = self._refs
+        need, spare, shared, todo = 0, 0, {}, []
+        for i, (s, n) in enumerate(zip(states, n_new)):
+            have, upto = len(s.pages), (s.length + n + PAGE - 1) // PAGE
+            if upto > have:
+                need += upto - have
+                todo.append(i)
+            elif upto < have:
+                spare += have - upto
             for j in range(s.length // PAGE, min(upto, have)) if n else ():
                 p = int(s.pages[j])
-                if self._refs[p] > 1:
-                    shared[p] = shared.get(p, int(self._refs[p])) - 1
-                    need += shared[p] > 0
+                if refs[p] > 1:
+                    shared[p] = shared.get(p, int(refs[p])) - 1
+                    if shared[p] > 0:
+                        need += 1
+                        todo.append(i)
         self._need(need - spare)
         self._epoch += 1
         if spare:
@@ -379,33 +386,36 @@ class PagedKVCache:
                 if len(s.pages) > upto:
                     self._give(s.pages[upto:])
                     s.pages = s.pages[:upto]
-        fresh = iter(self._take(need).tolist())
-        src, dst = [], []
-        for s, n in zip(states, n_new):
-            s.version += 1
-            have, upto = len(s.pages), _pages(s.length + n)
-            if shared and n:
-                for j in range(s.length // PAGE, min(upto, have)):
+        if todo:
+            fresh = iter(self._take(need).tolist())
+            src, dst = [], []
+            for i in dict.fromkeys(todo):
+                s = states[i]
+                have, upto = len(s.pages), _pages(s.length + n_new[i])
+                for j in range(s.length // PAGE, min(upto, have)) if shared and n_new[i] else ():
                     p = int(s.pages[j])
-                    if self._refs[p] > 1:
+                    if refs[p] > 1:
                         s.pages = s.pages.copy()
-                        s.pages[j] = next(fresh)
+                        s.pages[j] = to = next(fresh)
                         if j * PAGE < s.length:
                             src.append(p)
-                            dst.append(s.pages[j])
-                        self._refs[p] -= 1
-            if upto > have:
-                s.pages = np.concatenate([s.pages, np.array([next(fresh) for _ in range(upto - have)], np.int32)])
-        self._copy(src, dst)
+                            dst.append(to)
+                        refs[p] -= 1
+                if upto > have:
+                    s.pages = np.append(s.pages, np.fromiter(fresh, np.int32, upto - have))
+            self._copy(src, dst)
         rows = np.full((len(states), _INFO + self.max_pages_per_seq), -1, np.int32)
-        trim = -1
+        trim, heads = -1, []
         for i, (s, n) in enumerate(zip(states, n_new)):
-            if s.trimmed:
-                rows[i, :_INFO] = s.length + n, n, s.first, s.sinks
+            s.version += 1
+            if s.first > s.sinks:
+                heads.append((s.length + n, n, s.first, s.sinks))
                 trim = s.sinks if trim in (-1, s.sinks) else -2
             else:
-                rows[i, :3] = s.length + n, n, 0
+                heads.append((s.length + n, n, 0, -1))
             rows[i, _INFO:_INFO + len(s.pages)] = s.pages
+        if heads:
+            rows[:, :_INFO] = heads
         rows, handle = torch.from_numpy(rows), None
         if self.device.type == "cuda":
             handle = ext().kv_step_begin(self.k, self.v, self.k_scale, self.v_scale, rows, max_tokens, max(n_new, default=0),
@@ -425,10 +435,11 @@ class PagedKVCache:
         out = self.add(copies * len(states))
         for i, s in enumerate(states):
             s.version += 1
-            pages = s.pages[:_pages(s.length)]
-            self._refs[pages[pages >= 0]] += copies
+            pages = s.pages[:_pages(s.length)].copy()
+            self._refs[pages[pages >= 0] if s.trimmed else pages] += copies
             for k in out[i * copies:(i + 1) * copies]:
-                self._seqs[k] = _Seq(pages.copy(), s.length, s.first, s.sinks)
+                # a sequence's page list is replaced, never written in place
+                self._seqs[k] = _Seq(pages, s.length, s.first, s.sinks)
         return out
 
     def copy(self, seqs: Sequence[int]) -> List[int]:
@@ -450,9 +461,12 @@ class PagedKVCache:
 
     def free(self, seqs: Sequence[int]) -> None:
         """Drop sequences; pages that no other sequence shares become free."""
+        states = self._get(seqs)
+        if not states:
+            return
         self._epoch += 1
-        for i, s in zip(list(seqs), self._get(seqs)):
-            self._give(s.pages)
+        self._give(np.concatenate([s.pages for s in states]))
+        for i, s in zip(seqs, states):
             s.version += 1
             del self._seqs[i]
 

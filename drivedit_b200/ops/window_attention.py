@@ -54,6 +54,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     summed in fp32 in no fixed order: equal backward passes may differ in dq by a rounding
     of bf16. A backward pass is captured into a graph only when no autograd graph of the same
     leaves made on the default stream is alive (refused otherwise)."""
+    if q.is_cuda and q.numel() and k.numel():
+        o, lse = ext().window_attention(q, k, v, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, scale)
+        return (o, lse) if return_lse else o
     if q.dim() != 4 or k.dim() != 4 or q.shape[3] != 64 or k.shape != v.shape or \
             (q.shape[0], *q.shape[2:]) != (k.shape[0], *k.shape[2:]):
         raise ValueError(f"q must be [B, T, H, 64], k and v [B, S, H, 64]: got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -61,9 +64,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
         raise ValueError("q, k and v must be of one type and on one device")
     B, T, H, _ = q.shape
     S = k.shape[1]
-    if q.is_cuda and q.numel() and S:
-        o, lse = ext().window_attention(q, k, v, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, scale)
-        return (o, lse) if return_lse else o
     scale = 1.0 / math.sqrt(64) if scale is None else float(scale)
     _check_mask(causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, scale, T, S)
     if q.numel() == 0 or S == 0:  # no key or no query: zeros that depend on nothing

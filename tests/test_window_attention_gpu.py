@@ -104,7 +104,7 @@ def test_matches_formula(case, packed):
         assert (lse.double() - rlse)[fin].abs().max() <= 1.45 * (mag * 2.0 ** -18 + 2.0 ** -19)
 
 
-@pytest.mark.parametrize("splits", [2, 3, 5])
+@pytest.mark.parametrize("splits", [2, 3, 5, 8])
 def test_split_keys(splits):
     from drivedit_b200.ops._ext import ext
     from drivedit_b200.ops.window_attention import window_attention
