@@ -107,10 +107,10 @@ void attn_bwd_with_status(const AttnBwdArgs& a, int* status, cudaStream_t s);
 void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long lddo,
                     int do_col, float* delta, int B, int H, int Tq, long rows_per_b,
                     cudaStream_t s);
-// the same with delta rows delta_ld floats apart, clearing the contiguous dQ accumulator
-// [B * Tq][H * 64] on the way
+// -scale * delta in rows delta_ld floats apart, what the windowed backward reads, clearing the
+// contiguous dQ accumulator [B * Tq][H * 64] on the way
 void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
-                         int B, int H, int Tq, cudaStream_t s);
+                         int B, int H, int Tq, float scale, cudaStream_t s);
 // dq (bf16, optionally rotated back by a rotary table) from the fp32 accumulator
 void attn_dq_finalize(const float* dq_acc, long ld_acc, void* dq, long lddq, int dq_col,
                       int rows, int H, const float2* rope_tab, int rows_per_seq,

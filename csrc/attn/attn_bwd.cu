@@ -114,8 +114,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = warp_id();
   const int lane = lane_id();
-  const int kt = blockIdx.x % n_kvtiles;
-  const int bh = blockIdx.x / n_kvtiles;
+  // windowed mode: the first key tiles of every head first, the sinks' (and without a window
+  // the most seen) among them, so that the longest CTAs do not start last
+  const int kt = WIN ? blockIdx.x / (a.B * a.H) : blockIdx.x % n_kvtiles;
+  const int bh = WIN ? blockIdx.x % (a.B * a.H) : blockIdx.x / n_kvtiles;
   const int b = bh / a.H;
   const int h = bh % a.H;
   const int k0 = kt * 128;
@@ -491,7 +493,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float4 l4 = *reinterpret_cast<const float4*>(s_lse + c0 + c4);
             const float4 d4 = *reinterpret_cast<const float4*>(s_delta + c0 + c4);
             const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-            const float nsd[4] = {-a.scale * d4.x, -a.scale * d4.y, -a.scale * d4.z, -a.scale * d4.w};
+            // windowed mode: attn_window_prepare has stored -scale * delta
+            const float nsd[4] = {WIN ? d4.x : -a.scale * d4.x, WIN ? d4.y : -a.scale * d4.y,
+                                  WIN ? d4.z : -a.scale * d4.z, WIN ? d4.w : -a.scale * d4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int c = c4 + e;
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const bool vis = half_on && (q0 + c0 + c >= qmin) && (!WIN || q0 + c0 + c < qmax);
               const float pv = vis ? exp2f(__uint_as_float(rs[c]) * sl2 - lv[e]) : 0.f;
               p[c] = pv;
-              ds[c] = pv * (__uint_as_float(rp[c]) - dv[e]) * a.scale;
+              ds[c] = WIN ? pv * fmaf(a.scale, __uint_as_float(rp[c]), dv[e]) : pv * (__uint_as_float(rp[c]) - dv[e]) * a.scale;
               if (WIN && !vis) ds[c] = 0.f;  // a masked key's dP may be anything
             }
           }
@@ -682,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int o_col,
                              const __nv_bfloat16* __restrict__ dout, long lddo, int do_col,
                              float* __restrict__ delta, int B, int H, int Tq, long rows_per_b,
-                             long delta_ld, float* __restrict__ clear) {
+                             long delta_ld, float* __restrict__ clear, float factor) {
   const int lane = threadIdx.x & 31;
   const long row = blockIdx.x * 8L + (threadIdx.x >> 5);
   if (row >= static_cast<long>(B) * Tq) return;
@@ -715,7 +719,7 @@ __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int 
     s += __shfl_xor_sync(0xffffffffu, s, 4);
     if ((lane & 7) == 0 && c < chunks) {
       const int hh = c / 8;
-      delta[(static_cast<long>(b) * H + hh) * delta_ld + t] = s;
+      delta[(static_cast<long>(b) * H + hh) * delta_ld + t] = s * factor;
     }
   }
 }
@@ -830,16 +834,16 @@ void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long l
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(o), ldo, o_col,
       reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b, Tq,
-      nullptr);
+      nullptr, 1.f);
   count_launch();
 }
 
 void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
-                         int B, int H, int Tq, cudaStream_t s) {
+                         int B, int H, int Tq, float scale, cudaStream_t s) {
   const long rows = static_cast<long>(B) * Tq;
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
       reinterpret_cast<const __nv_bfloat16*>(o), H * 64L, 0, reinterpret_cast<const __nv_bfloat16*>(dout),
-      H * 64L, 0, delta, B, H, Tq, Tq, delta_ld, dq_acc);
+      H * 64L, 0, delta, B, H, Tq, Tq, delta_ld, dq_acc, -scale);
   count_launch();
   check_cuda(cudaGetLastError(), "delta_kernel launch");
 }

@@ -124,8 +124,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int splits = a.kv_splits > 1 ? a.kv_splits : 1;
   const int split = blockIdx.x % splits;
   const int item = blockIdx.x / splits;
-  const int qt = n_qtiles - 1 - (item % n_qtiles);  // heavy (late) tiles first
-  const int bh = item / n_qtiles;
+  // heavy (late) tiles first: of each head, in the windowed mode of all heads
+  const int qt = n_qtiles - 1 - (WIN ? item / (a.B * a.H) : item % n_qtiles);
+  const int bh = WIN ? item % (a.B * a.H) : item / n_qtiles;
   const int b = bh / a.H;
   const int h = bh % a.H;
   const int q0 = qt * 128;

@@ -1531,7 +1531,7 @@ void attn_window_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch
   g.dk = dk.data_ptr();
   g.dv = dv.data_ptr();
   ddb::attn_window_prepare(o.data_ptr(), dout.data_ptr(), delta.data_ptr<float>(), lse.size(2), acc.data_ptr<float>(), a.B,
-                           a.H, a.Tq, stream());
+                           a.H, a.Tq, a.scale, stream());
   ddb::attn_window_bwd(g, stream());
   ddb::attn_dq_finalize(acc.data_ptr<float>(), a.H * 64L, dq.data_ptr(), ld_dq, 0, a.B * a.Tq, a.H, nullptr, a.Tq, 0, stream());
 }
