@@ -56,6 +56,7 @@ struct AttnArgs {
   int window = 0;
   int sink_tokens = 0;
   long lse_ld = 0;
+  void* o_rest = nullptr;     // what o's rounding left, bf16 like o; null: not kept
   long q_sb = 0, q_st = 0, q_sh = 0;
   long k_sb = 0, k_st = 0, k_sh = 0;
   long v_sb = 0, v_st = 0, v_sh = 0;
@@ -108,8 +109,10 @@ void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long l
                     int do_col, float* delta, int B, int H, int Tq, long rows_per_b,
                     cudaStream_t s);
 // -scale * delta in rows delta_ld floats apart, what the windowed backward reads, clearing the
-// contiguous dQ accumulator [B * Tq][H * 64] on the way
-void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
+// contiguous dQ accumulator [B * Tq][H * 64] on the way. o + o_rest is the forward's output
+// before its rounding: dS = P (dP - delta) cancels where a query sees few keys, and there
+// the rounding of O would be a third of dq's and dk's error.
+void attn_window_prepare(const void* o, const void* o_rest, const void* dout, float* delta, long delta_ld, float* dq_acc,
                          int B, int H, int Tq, float scale, cudaStream_t s);
 // dq (bf16, optionally rotated back by a rotary table) from the fp32 accumulator
 void attn_dq_finalize(const float* dq_acc, long ld_acc, void* dq, long lddq, int dq_col,

@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // delta[b,h,t] = sum over the head's 64 columns of dO * O (one warp per row)
-__global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int o_col,
+__global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_rest, long ldo, int o_col,
                              const __nv_bfloat16* __restrict__ dout, long lddo, int do_col,
                              float* __restrict__ delta, int B, int H, int Tq, long rows_per_b,
                              long delta_ld, float* __restrict__ clear, float factor) {
@@ -707,10 +707,15 @@ __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, long ldo, int 
       uint4 dv = ld_global_v4(dout + grow * lddo + do_col + c * 8);
       uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w};
       uint32_t dw[4] = {dv.x, dv.y, dv.z, dv.w};
+      const uint4 rv = o_rest ? ld_global_v4(o_rest + grow * ldo + o_col + c * 8) : make_uint4(0, 0, 0, 0);
+      const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float2 a = unpack_bf16(ow[j]);
         float2 d = unpack_bf16(dw[j]);
+        const float2 r = unpack_bf16(rw[j]);
+        a.x += r.x;
+        a.y += r.y;
         s += a.x * d.x + a.y * d.y;
       }
     }
@@ -832,17 +837,17 @@ void attn_bwd_delta(const void* o, long ldo, int o_col, const void* dout, long l
                     float* delta, int B, int H, int Tq, long rows_per_b, cudaStream_t s) {
   const long rows = static_cast<long>(B) * Tq;
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
-      reinterpret_cast<const __nv_bfloat16*>(o), ldo, o_col,
+      reinterpret_cast<const __nv_bfloat16*>(o), nullptr, ldo, o_col,
       reinterpret_cast<const __nv_bfloat16*>(dout), lddo, do_col, delta, B, H, Tq, rows_per_b, Tq,
       nullptr, 1.f);
   count_launch();
 }
 
-void attn_window_prepare(const void* o, const void* dout, float* delta, long delta_ld, float* dq_acc,
+void attn_window_prepare(const void* o, const void* o_rest, const void* dout, float* delta, long delta_ld, float* dq_acc,
                          int B, int H, int Tq, float scale, cudaStream_t s) {
   const long rows = static_cast<long>(B) * Tq;
   delta_kernel<<<static_cast<int>((rows + 7) / 8), 256, 0, s>>>(
-      reinterpret_cast<const __nv_bfloat16*>(o), H * 64L, 0, reinterpret_cast<const __nv_bfloat16*>(dout),
+      reinterpret_cast<const __nv_bfloat16*>(o), reinterpret_cast<const __nv_bfloat16*>(o_rest), H * 64L, 0, reinterpret_cast<const __nv_bfloat16*>(dout),
       H * 64L, 0, delta, B, H, Tq, Tq, delta_ld, dq_acc, -scale);
   count_launch();
   check_cuda(cudaGetLastError(), "delta_kernel launch");

@@ -77,6 +77,12 @@ __device__ __forceinline__ void fwd_trace(const FwdTrace& t, int role, int ev, i
   if (t.buf && blockIdx.x == t.cta && j < 64) t.buf[(role * 8 + ev) * 64 + j] = clock64();
 }
 
+// what two values lose when they are rounded to bf16
+__device__ __forceinline__ uint32_t pack_rest(float lo, float hi) {
+  const float2 r = unpack_bf16(pack_bf16(lo, hi));
+  return pack_bf16(lo - r.x, hi - r.y);
+}
+
 __device__ __forceinline__ int row_limit(const AttnArgs& a, int q_local) {
   int lim = a.S;
   const int qa = a.q_pos_offset + q_local;
@@ -559,6 +565,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                      pack_bf16(ov[c + 2] * inv, ov[c + 3] * inv),
                      pack_bf16(ov[c + 4] * inv, ov[c + 5] * inv),
                      pack_bf16(ov[c + 6] * inv, ov[c + 7] * inv));
+      if (WIN && a.o_rest) {
+        __nv_bfloat16* rest = reinterpret_cast<__nv_bfloat16*>(a.o_rest) + (b * a.q_rows_per_b + q_local) * a.ldo + h * 64;
+#pragma unroll
+        for (int c = 0; c < 64; c += 8)
+          st_global_v4(rest + c, pack_rest(ov[c] * inv, ov[c + 1] * inv), pack_rest(ov[c + 2] * inv, ov[c + 3] * inv),
+                       pack_rest(ov[c + 4] * inv, ov[c + 5] * inv), pack_rest(ov[c + 6] * inv, ov[c + 7] * inv));
+      }
       if (a.lse) a.lse[static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + q_local] = l > 0.f ? m + __log2f(l) : -INFINITY;
     }
   }
@@ -594,6 +607,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
       __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) + (b * a.q_rows_per_b + q) * a.ldo + h * 64 + c * 4;
       *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+      if (a.o_rest)
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o_rest) + (b * a.q_rows_per_b + q) * a.ldo + h * 64 + c * 4) =
+            make_uint2(pack_rest(v.x * inv, v.y * inv), pack_rest(v.z * inv, v.w * inv));
       if (a.lse && c == 0)
         a.lse[static_cast<long>(bh) * a.lse_ld + q] = sum > 0.f ? top + __log2f(sum) : -INFINITY;
     }

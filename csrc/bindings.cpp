@@ -1475,17 +1475,23 @@ torch::Tensor tma_ready(const torch::Tensor& t) {
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
-// o [B, T, H, 64], and lse [B, H, T rounded up to 128] (log2 domain)
+// o [B, T, H, 64], lse [B, H, T rounded up to 128] (log2 domain), and for the backward what o's
+// rounding left
 std::vector<torch::Tensor> attn_window_fwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                                           const WindowMask& m) {
+                                           const WindowMask& m, bool for_backward) {
   auto a = window_args(q, k, v, m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos, m.scale);
   const c10::cuda::CUDAGuard guard(q.device());
   auto o = torch::empty({a.B, a.Tq, a.H, 64}, q.options());
   auto lse = torch::empty({a.B, a.H, (a.Tq + 127) / 128 * 128}, q.options().dtype(torch::kFloat32));
   a.o = o.data_ptr(); a.ldo = a.H * 64;
   a.lse = lse.data_ptr<float>(); a.lse_ld = lse.size(2);
+  torch::Tensor rest;
+  if (for_backward) {
+    rest = torch::empty_like(o);
+    a.o_rest = rest.data_ptr();
+  }
   ddb::attn_window_fwd(a, static_cast<int>(g_attn_kv_splits), stream());
-  return {o, lse};
+  return {o, lse, rest};
 }
 
 // [B, rows, H, 64] views of a gradient whose rows lie at one stride over the samples, heads 64 apart
@@ -1502,7 +1508,7 @@ void window_grad_rows(const torch::Tensor& t, const char* name, const torch::Ten
 // Gradients into dq, dk, dv. dQ is summed over the key tiles in fp32 in no fixed order: equal
 // calls may differ in its last fp32 bits before the rounding to bf16.
 void attn_window_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
-                     const torch::Tensor& lse, const torch::Tensor& grad, const WindowMask& m, const torch::Tensor& dq,
+                     const torch::Tensor& rest, const torch::Tensor& lse, const torch::Tensor& grad, const WindowMask& m, const torch::Tensor& dq,
                      const torch::Tensor& dk, const torch::Tensor& dv) {
   ddb::AttnBwdArgs g;
   g.f = window_args(q, k, v, m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos, m.scale);
@@ -1511,10 +1517,10 @@ void attn_window_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch
                   lse.size(0) == a.B && lse.size(1) == a.H && lse.size(2) == (a.Tq + 127) / 128 * 128 && lse.device() == q.device(),
               "lse must be the forward's [B, H, T rounded up to 128]");
   const auto dout = grad.is_contiguous() && reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0 ? grad : grad.clone(at::MemoryFormat::Contiguous);
-  for (const auto* t : {&o, &dout})
+  for (const auto* t : {&o, &rest, &dout})
     TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kBFloat16 && t->is_contiguous() && t->sizes() == q.sizes() &&
                     t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "o and its gradient must be contiguous bf16 and like q");
+                "o, its rest and its gradient must be contiguous bf16 and like q");
   const c10::cuda::CUDAGuard guard(q.device());
   long ld_dq = 0;
   window_grad_rows(dq, "dq", q, ld_dq);
@@ -1530,7 +1536,7 @@ void attn_window_bwd(const torch::Tensor& q, const torch::Tensor& k, const torch
   g.dq_acc = acc.data_ptr<float>(); g.ld_dqacc = a.H * 64;
   g.dk = dk.data_ptr();
   g.dv = dv.data_ptr();
-  ddb::attn_window_prepare(o.data_ptr(), dout.data_ptr(), delta.data_ptr<float>(), lse.size(2), acc.data_ptr<float>(), a.B,
+  ddb::attn_window_prepare(o.data_ptr(), rest.data_ptr(), dout.data_ptr(), delta.data_ptr<float>(), lse.size(2), acc.data_ptr<float>(), a.B,
                            a.H, a.Tq, a.scale, stream());
   ddb::attn_window_bwd(g, stream());
   ddb::attn_dq_finalize(acc.data_ptr<float>(), a.H * 64L, dq.data_ptr(), ld_dq, 0, a.B * a.Tq, a.H, nullptr, a.Tq, 0, stream());
@@ -1541,8 +1547,8 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& q0,
                                                 const torch::Tensor& k0, const torch::Tensor& v0, const WindowMask& m) {
     const auto q = tma_ready(q0), k = tma_ready(k0), v = tma_ready(v0);
-    auto out = attn_window_fwd(q, k, v, m);
-    ctx->save_for_backward({q, k, v, out[0], out[1]});
+    auto out = attn_window_fwd(q, k, v, m, true);
+    ctx->save_for_backward({q, k, v, out[0], out[2], out[1]});
     ctx->saved_data["mask"] = std::vector<int64_t>{m.causal, m.unit, m.window, m.sinks, m.q_pos, m.kv_pos};
     ctx->saved_data["scale"] = m.scale;
     ctx->set_materialize_grads(false);
@@ -1558,7 +1564,7 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
     const c10::cuda::CUDAGuard guard(s[0].device());
     auto dq = torch::empty(s[0].sizes(), s[0].options()), dk = torch::empty(s[1].sizes(), s[1].options()),
          dv = torch::empty(s[2].sizes(), s[2].options());
-    attn_window_bwd(s[0], s[1], s[2], s[3], s[4], grads[0].to(torch::kBFloat16), m, dq, dk, dv);
+    attn_window_bwd(s[0], s[1], s[2], s[3], s[4], s[5], grads[0].to(torch::kBFloat16), m, dq, dk, dv);
     return {dq, dk, dv, torch::Tensor()};
   }
 };
@@ -1587,9 +1593,8 @@ std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch:
   const auto m = window_mask(causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale ? *scale : 0.125, q.size(1), k.size(1));
   TORCH_CHECK_VALUE(q.size(1) <= 65536 * 64, "at most ", 65536 * 64, " queries per sample");
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
-    auto out = attn_window_fwd(tma_ready(q), tma_ready(k), tma_ready(v), m);
-    out[1] = out[1].narrow(2, 0, q.size(1));
-    return out;
+    const auto out = attn_window_fwd(tma_ready(q), tma_ready(k), tma_ready(v), m, false);
+    return {out[0], out[1].narrow(2, 0, q.size(1))};
   }
   {
     const c10::cuda::CUDAGuard guard(q.device());
@@ -1602,13 +1607,13 @@ std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch:
 std::vector<torch::Tensor> attn_window_fwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                                               const std::string& causal, int64_t tokens_per_frame, int64_t window,
                                               int64_t sinks, double scale) {
-  return attn_window_fwd(q, k, v, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)));
+  return attn_window_fwd(q, k, v, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)), true);
 }
 void attn_window_bwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
-                        const torch::Tensor& lse, const torch::Tensor& grad, const std::string& causal,
+                        const torch::Tensor& rest, const torch::Tensor& lse, const torch::Tensor& grad, const std::string& causal,
                         int64_t tokens_per_frame, int64_t window, int64_t sinks, double scale, const torch::Tensor& dq,
                         const torch::Tensor& dk, const torch::Tensor& dv) {
-  attn_window_bwd(q, k, v, o, lse, grad, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)),
+  attn_window_bwd(q, k, v, o, rest, lse, grad, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)),
                   dq, dk, dv);
 }
 

@@ -196,8 +196,8 @@ def attention_fwd_kernel(qkv: torch.Tensor, bc):
     o_lin = None
     lists = (None, None, None)
     if bc.window_frames and bc.attn_mode == "dense":
-        o4, lse = ext().attn_window_fwd(*_heads(qkv, bc), *_window_args(bc))
-        return o4.view(M, d), None, lse, None
+        o4, lse, rest = ext().attn_window_fwd(*_heads(qkv, bc), *_window_args(bc))
+        return o4.view(M, d), None, lse, rest
     if bc.attn_mode == "sla":
         plan = sla_plan_kernel(qkv, B, T, H, bc.sla_cfg, bc.tpf, bc.causal)
         lists = (plan.pair_blocks, plan.pair_mask, plan.pair_count)
@@ -214,7 +214,7 @@ def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc):
     dev = qkv.device
     if bc.window_frames and bc.attn_mode == "dense":
         dqkv = torch.empty(M, 3 * d, device=dev, dtype=torch.bfloat16)
-        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), lse, do.view(B, T, H, 64), *_window_args(bc),
+        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), plan, lse, do.view(B, T, H, 64), *_window_args(bc),
                               *_heads(dqkv, bc))
         return dqkv
     delta = torch.empty(B * H * T, device=dev, dtype=torch.float32)
