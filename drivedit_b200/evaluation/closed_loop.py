@@ -94,6 +94,8 @@ class EvaluationConfig:
     flow_steps: int = 4
     window_frames: int = 32
     dt: float = 0.1
+    kv_cache: str = "bf16"  # "fp8": the window in 8-bit pages
+    sink_frames: int = 0    # first frames that stay visible (kv_cache "fp8")
 
 
 @dataclass
@@ -176,12 +178,14 @@ class ClosedLoopEvaluator:
 
     # ------------------------------------------------------------------ model io
     def _initialize_context(self, initial_observation: torch.Tensor) -> None:
-        from ..models.world_dit import KVCacheSet, forward_cached
+        from ..models.world_dit import forward_cached, make_kv_cache
 
         obs = initial_observation.to(self.device, self.dtype)
         if obs.dim() == 3:
             obs = obs[None]
-        self.cache = KVCacheSet(self.world_model, 1, self.config.window_frames, 1, self.device, self.dtype)
+        self.cache = make_kv_cache(self.world_model, 1, self.config.window_frames, obs.shape[0], self.device, self.dtype,
+                                   self.config.kv_cache, self.config.sink_frames,
+                                   obs.shape[0] + self.config.max_episode_steps)
         a = torch.zeros(1, obs.shape[0], self.A, device=self.device)
         with torch.no_grad():
             forward_cached(self.world_model, obs[None], torch.ones(1, device=self.device), a, self.cache, commit=True)

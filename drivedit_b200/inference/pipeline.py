@@ -54,6 +54,8 @@ class PipelineConfig:
     flow_steps: int = 4
     window_frames: int = 32
     seed: int = 0
+    kv_cache: str = "bf16"                # "fp8": the window in 8-bit pages
+    sink_frames: int = 0                  # first frames that stay visible (kv_cache "fp8")
 
 
 class InferencePipeline:
@@ -66,7 +68,8 @@ class InferencePipeline:
         self.model = self._load_student_model(config.model_path)
         self.vae = self._load_vae_model(config.vae_path) if config.use_vae else None
         rc = RolloutConfig(total_frames=0, chunk_frames=config.chunk_frames, flow_steps=config.flow_steps,
-                           window_frames=config.window_frames, context_frames=1, batch=config.batch_size)
+                           window_frames=config.window_frames, context_frames=1, batch=config.batch_size,
+                           kv_cache=config.kv_cache, sink_frames=config.sink_frames)
         self.rollout = StreamingRollout(self.model, rc, self.dtype)
         self.gen = torch.Generator(device=self.device).manual_seed(config.seed)
 

@@ -24,7 +24,7 @@ import torch
 import torch.nn.functional as F
 
 from ..config import RolloutConfig
-from ..models.world_dit import KVCacheSet, PagedKVCacheSet, WorldDiT
+from ..models.world_dit import WorldDiT, make_kv_cache
 from ..models.world_dit import forward_cached as _forward_cached
 
 
@@ -205,18 +205,12 @@ class StreamingRollout:
     def _make_cache(self, B: int, total: int, branches: int):
         cfg, m = self.cfg, self.model
         make_cache = getattr(m, "make_kv_cache", None)     # e.g. a tensor-parallel model
-        if cfg.kv_cache not in ("bf16", "fp8"):
-            raise ValueError(f'kv_cache must be "bf16" or "fp8", got {cfg.kv_cache!r}')
-        if cfg.kv_cache == "fp8":
-            if make_cache is not None:
-                raise ValueError("tensor-parallel rollouts hold their window in bf16")
-            return PagedKVCacheSet(m, B, cfg.window_frames, cfg.chunk_frames, self.device,
-                                   cfg.sink_frames or m.cfg.sink_frames, total, branches)
-        if cfg.sink_frames:
-            raise ValueError('sink_frames needs kv_cache="fp8"')
         if make_cache is not None:
+            if cfg.kv_cache != "bf16" or cfg.sink_frames:
+                raise ValueError("tensor-parallel rollouts hold their window in bf16, without sinks")
             return make_cache(B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype)
-        return KVCacheSet(m, B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype)
+        return make_kv_cache(m, B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype, cfg.kv_cache,
+                             cfg.sink_frames, total, branches)
 
     def _run(self, context, actions, total_frames, generator, extra_cond, replace, branches) -> RolloutResult:
         cfg = self.cfg

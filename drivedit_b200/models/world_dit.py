@@ -433,6 +433,21 @@ class PagedKVCacheSet:
         self._step = None
 
 
+def make_kv_cache(model: "WorldDiT", B: int, window_frames: int, chunk_frames: int, device, dtype,
+                  kv_cache: str = "bf16", sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1):
+    """The rolling key/value window of a stream: contiguous buffers in ``dtype``
+    (``kv_cache`` "bf16") or 8-bit pages ("fp8"), which also keep the first ``sink_frames``
+    frames (0: the model's own)."""
+    if kv_cache == "fp8":
+        return PagedKVCacheSet(model, B, window_frames, chunk_frames, device, sink_frames or model.cfg.sink_frames,
+                               max_frames, branches)
+    if kv_cache != "bf16":
+        raise ValueError(f'kv_cache must be "bf16" or "fp8", got {kv_cache!r}')
+    if sink_frames:
+        raise ValueError('sink_frames needs kv_cache="fp8"')
+    return KVCacheSet(model, B, window_frames, chunk_frames, device, dtype)
+
+
 def _block_cached_torch(blk: WorldDiTBlock, x, mod, tab_q, cache: LayerKVCache, row, frames, step=None,
                         layer=0):
     """One block over a chunk ``x [B, T, d]`` attending to the cache window + itself;

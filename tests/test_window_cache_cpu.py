@@ -302,3 +302,21 @@ def test_model_refusals():
         KVCacheSet(m, 1, 4, 2, "cpu", torch.float32)
     with pytest.raises(ValueError):
         PagedKVCacheSet(m, 1, 4, 2, "cpu", sink_frames=2)
+
+
+def test_closed_loop_and_pipeline_over_the_paged_cache():
+    from drivedit_b200.evaluation.closed_loop import ClosedLoopEvaluator, EvaluationConfig
+    from drivedit_b200.inference.pipeline import InferencePipeline, PipelineConfig
+    _, m = _model("model.window_frames=3", "model.sink_frames=1")
+    ev = ClosedLoopEvaluator(m, EvaluationConfig(flow_steps=1, window_frames=4, kv_cache="fp8", max_episode_steps=8), device="cpu")
+    ev._initialize_context(torch.randn(2, 16, 16, 16))
+    for _ in range(7):
+        frame = ev._predict_next(torch.zeros(2))
+        assert torch.isfinite(frame).all()
+    assert ev.cache.frames >= 2 and ev.cache.cache.length(ev.cache.seqs[0]) == 9 * 64
+    with pytest.raises(ValueError):
+        ClosedLoopEvaluator(m, EvaluationConfig(), device="cpu")._initialize_context(torch.randn(16, 16, 16))
+    pipe = InferencePipeline(PipelineConfig(device="cpu", model_preset="tiny", model_overrides=["model.n_layers=1"], use_vae=False,
+                                            chunk_frames=2, flow_steps=1, window_frames=2, kv_cache="fp8", sink_frames=1))
+    res = pipe.rollout.run(torch.randn(1, 1, 16, 16, 16), torch.zeros(1, 7, 2), total_frames=7)
+    assert res.frames.shape[1] == 7 and torch.isfinite(res.frames).all()
