@@ -1665,7 +1665,9 @@ ddb::KvStep kv_step(const torch::Tensor& rows, const torch::Tensor& k) {
 // upload ran on. Calls on another stream wait for the upload.
 struct KvStepHandle {
   torch::Tensor k, v, ks, vs, rows;
-  int64_t max_tokens = 0, most_new = 0;
+  ddb::KvPool base;  // of layer 0, checked when the step was begun
+  ddb::KvStep step;
+  int64_t layers = 0, max_tokens = 0, most_new = 0;
   int64_t trim_sinks = -1;  // sinks of the trimmed sequences; -1: none is, -2: they differ
   c10::optional<c10::cuda::CUDAStream> begun;
   at::cuda::CUDAEvent ready;
@@ -1675,7 +1677,7 @@ struct KvStepHandle {
 std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
                                             torch::Tensor rows, int64_t max_tokens, int64_t most_new, int64_t trim_sinks,
                                             std::shared_ptr<KvStepHandle> out) {
-  kv_pool(k, v, ks, vs, 0);
+  const auto base = kv_pool(k, v, ks, vs, 0);
   TORCH_CHECK(rows.device().is_cpu() && rows.scalar_type() == torch::kInt32 && rows.is_contiguous() && rows.dim() == 2 &&
                   rows.size(1) > ddb::kKvInfo && rows.size(0) <= 65535, "a step's table must be int32 [<= 65535, 4 + pages]");
   const c10::cuda::CUDAGuard guard(k.device());
@@ -1691,12 +1693,26 @@ std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, to
     h->rows.copy_(staged, true);
   }
   h->k = k; h->v = v; h->ks = ks; h->vs = vs;
+  h->base = base;
+  h->step = kv_step(h->rows, k);
+  h->layers = k.size(0);
   h->max_tokens = max_tokens;
   h->most_new = most_new;
   h->trim_sinks = trim_sinks;
   h->begun = at::cuda::getCurrentCUDAStream();
   h->ready.record(*h->begun);
   return h;
+}
+
+ddb::KvPool kv_layer(const KvStepHandle& h, int64_t layer) {
+  TORCH_CHECK_VALUE(layer >= 0 && layer < h.layers, "layer ", layer, " of a cache of ", h.layers);
+  const long blocks = static_cast<long>(layer) * h.base.pages * h.base.heads;
+  ddb::KvPool p = h.base;
+  p.k += blocks * 4096;
+  p.v += blocks * 4096;
+  p.k_scale += blocks;
+  p.v_scale += blocks;
+  return p;
 }
 
 void kv_step_wait(KvStepHandle& h) {
@@ -1723,13 +1739,12 @@ torch::Tensor kv_tokens(const torch::Tensor& t, const char* name, const KvStepHa
 
 void kv_step_write(std::shared_ptr<KvStepHandle> hp, int64_t layer, const torch::Tensor& k, const torch::Tensor& v) {
   KvStepHandle& h = *hp;
-  TORCH_CHECK_VALUE(layer >= 0 && layer < h.k.size(0), "layer ", layer, " of a cache of ", h.k.size(0));
   TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "k and v differ in shape");
   const c10::cuda::CUDAGuard guard(h.k.device());
   const auto kk = kv_tokens(k, "k", h, h.k.size(2)), vv = kv_tokens(v, "v", h, h.k.size(2));
   ddb::KvWriteArgs a;
-  a.pool = kv_pool(h.k, h.v, h.ks, h.vs, layer);
-  a.step = kv_step(h.rows, h.k);
+  a.pool = kv_layer(h, layer);
+  a.step = h.step;
   a.k = kk.data_ptr();
   a.k_sb = kk.stride(0); a.k_st = kk.stride(1); a.k_sh = kk.stride(2);
   a.v = vv.data_ptr();
@@ -1743,15 +1758,14 @@ std::vector<torch::Tensor> kv_step_attend(std::shared_ptr<KvStepHandle> hp, int6
                                           const std::string& causal, int64_t tokens_per_frame, int64_t window,
                                           int64_t sinks, c10::optional<double> scale, bool return_lse) {
   KvStepHandle& h = *hp;
-  TORCH_CHECK_VALUE(layer >= 0 && layer < h.k.size(0), "layer ", layer, " of a cache of ", h.k.size(0));
   const c10::cuda::CUDAGuard guard(h.k.device());
   const auto q = kv_tokens(q0, "q", h, 0);
   const auto m = window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale ? *scale : 0.125, 0, 0);
   TORCH_CHECK_VALUE(h.trim_sinks == -1 || (window == 0 && sinks == 0) || h.trim_sinks == m.sinks,
                     "a trimmed sequence keeps the first tokens it was trimmed to; the call names ", m.sinks, " sinks");
   ddb::KvAttendArgs a;
-  a.pool = kv_pool(h.k, h.v, h.ks, h.vs, layer);
-  a.step = kv_step(h.rows, h.k);
+  a.pool = kv_layer(h, layer);
+  a.step = h.step;
   TORCH_CHECK_VALUE(q.size(1) * (q.size(2) / a.pool.heads) <= (1 << 30), "too many query rows");
   auto o = torch::empty(q.sizes(), q.options());
   a.q = q.data_ptr();

@@ -81,7 +81,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 
 template <int NT>
 __global__ void __launch_bounds__(kGroups * NT * 32)
-    kv_attend_rows(const KvAttendArgs a, int row_tiles, int stages, int* status) {
+    kv_attend_rows(const KvAttendArgs a, int row_tiles, int stages, uint32_t group_inv, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int R = 8 * NT, kThreads = kGroups * NT * 32;
   const int warp = warp_id(), lane = lane_id();
@@ -97,6 +97,8 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
   const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
   const int r0 = tile * R, rows = own * G;           // rows behind `rows` are padding
+  // token of a row: rows are few, so a multiplication by 2^32 / G rounded up is exact
+  auto token = [&](int r) -> int { return G == 1 ? r : __umulhi(r, group_inv); };
 
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + off_bar(NT)) + pg * 2 * kMaxStages;
   uint64_t* empty = full + kMaxStages;
@@ -117,13 +119,22 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   KvPages pages{0, 0, 0};
   int lo_max = 0, hi_min = 0, lo_min = 0, hi_max = 0;
   if (r0 < rows) {
-    const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
-    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + R) - 1) / G, len, first);
+    const KvSpan s0 = kv_span(a, old + token(r0), len, first);
+    const KvSpan s1 = kv_span(a, old + token(min(rows, r0 + R) - 1), len, first);
     lo_min = s0.lo, hi_min = s0.hi, lo_max = s1.lo, hi_max = s1.hi;
     pages = kv_pages(lo_min, hi_max, sinks, a.step.width);
   }
   const int part = rank * kGroups + pg, parts = ranks * kGroups;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
+
+  // Q's loads go out first: row g of the warp's 8, channels 16c..16c+15
+  uint4 qraw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (r0 + rg * 8 + g < rows) {
+    const int r = r0 + rg * 8 + g, t = token(r);
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + t * a.q_st + (kh * G + r - t * G) * a.q_sh + 16 * c;
+    qraw[0] = ld_global_v4(q);
+    qraw[1] = ld_global_v4(q + 8);
+  }
 
   // the group's next 32 pages, one a lane: block of codes (-1: not in the pool) and scales
   long block = -1;
@@ -146,15 +157,17 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     }
     if (NT > 1 && !__all_sync(0xffffffffu, mbar_wait(&empty[put_stage], put_phase, abort_flag))) return false;
     const long at = __shfl_sync(0xffffffffu, block, put & 31);
-    const float kf = __shfl_sync(0xffffffffu, ks, put & 31), vf = __shfl_sync(0xffffffffu, vs, put & 31);
-    if (lane == 0) {
+    if (lane == 0) {  // the copies first: the scales may still be on their way
       const long from = max(at, 0L) * 4096;
       uint64_t* bar = &full[put_stage];
       uint8_t* dst = ring + put_stage * kPageBytes;
-      scales[put_stage] = make_float4(kf, vf, at >= 0 ? 1.f : 0.f, 0.f);
-      mbar_arrive_expect_tx(bar, kPageBytes);
       bulk_load(dst, a.pool.k + from, 4096, bar);
       bulk_load(dst + 4096, a.pool.v + from, 4096, bar);
+    }
+    const float kf = __shfl_sync(0xffffffffu, ks, put & 31), vf = __shfl_sync(0xffffffffu, vs, put & 31);
+    if (lane == 0) {
+      scales[put_stage] = make_float4(kf, vf, at >= 0 ? 1.f : 0.f, 0.f);
+      mbar_arrive_expect_tx(&full[put_stage], kPageBytes);
     }
     ++put;
     if (++put_stage == stages) {
@@ -167,28 +180,19 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   if (rg == 0)
     for (int i = 0; i < min(mine, stages); ++i) issue();  // no wait: the stages are empty
 
-  // Q: row g of the warp's 8, channels 16c..16c+15
   uint32_t qf[4][2];
   float sl2[2];   // score factors of rows 2c and 2c + 1, which this lane's scores belong to
   KvSpan span[2];
   {
-    const int r = r0 + rg * 8 + g;
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    if (r < rows) {
-      const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + (r / G) * a.q_st +
-                               (kh * G + r % G) * a.q_sh + 16 * c;
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t ws[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 w = ld_global_v4(q + i * 8);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = unpack_bf16(ws[k]);
-          x[i * 8 + 2 * k] = f.x;
-          x[i * 8 + 2 * k + 1] = f.y;
-        }
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack_bf16(ws[k]);
+        x[i * 8 + 2 * k] = f.x;
+        x[i * 8 + 2 * k + 1] = f.y;
       }
     }
     float amax = 0.f;
@@ -208,7 +212,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     for (int u = 0; u < 2; ++u) {
       sl2[u] = __shfl_sync(0xffffffffu, up, (2 * c + u) * 4);
       // a padding row keeps zeros and the span of the last row: its result is not used
-      span[u] = kv_span(a, old + (min(max(rows, 1), r0 + rg * 8 + 2 * c + u + 1) - 1) / G, len, first);
+      span[u] = kv_span(a, old + token(min(max(rows, 1), r0 + rg * 8 + 2 * c + u + 1) - 1), len, first);
     }
   }
 
@@ -249,11 +253,12 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     for (int u = 0; u < 2; ++u) {
       const float fu = sl2[u] * f.x;
       if (!whole) {
+        const uint32_t see = there ? static_cast<uint32_t>(kv_bits(span[u], sinks, key0) >> krow) : 0u;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            if (!there || !kv_visible(span[u], sinks, key0 + krow + 4 * t + 2 * k)) s[t][2 * k + u] = -INFINITY;
+            if (!(see >> (4 * t + 2 * k) & 1)) s[t][2 * k + u] = -INFINITY;
       }
       float mx = fmaxf(fmaxf(s[0][u], s[0][2 + u]), fmaxf(s[1][u], s[1][2 + u]));
       mx = fmaxf(mx, fmaxf(fmaxf(s[2][u], s[2][2 + u]), fmaxf(s[3][u], s[3][2 + u])));
@@ -286,10 +291,9 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     // tokens that no row of the tile sees are left out of P V whatever they hold
     uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
     if (!(there && key0 + kKvPage <= hi_max && (key0 >= lo_min || key0 + kKvPage <= sinks))) {
-      const KvSpan all{lo_min, hi_max};
+      const uint32_t see = there ? static_cast<uint32_t>(kv_bits(KvSpan{lo_min, hi_max}, sinks, key0) >> (16 * c)) : 0u;
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (!there || !kv_visible(all, sinks, key0 + 16 * c + k)) keep[k >> 2] &= ~(0xffu << (8 * (k & 3)));
+      for (int k = 0; k < 4; ++k) keep[k] = kv_bytes(see >> (4 * k));
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -397,7 +401,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
         v.z += w * y.z;
         v.w += w * y.w;
       }
-    const int t = row_id / G, h = kh * G + row_id % G;
+    const int t = token(row_id), h = kh * G + row_id - t * G;
     if (t >= own) {  // behind the sequence's own tokens
       sum = 0.f;
       v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -447,7 +451,8 @@ void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, stages, device_status(dev)), "kv_attend_rows launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, stages, 0xffffffffu / G + 1, device_status(dev)),
+             "kv_attend_rows launch");
   count_launch();
 }
 

@@ -355,8 +355,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int i = 2 * (j0 + j) + p;
         const int key = pages.at(i) * kKvPage;
         if (keep[p][0] && !(key + kKvPage <= all.hi && (key >= all.lo || key + kKvPage <= sinks))) {
-          for (int k = 0; k < 16; ++k)
-            if (!kv_visible(all, sinks, key + 16 * c + k)) keep[p][k >> 2] &= ~(0xffu << (8 * (k & 3)));
+          const uint32_t see = static_cast<uint32_t>(kv_bits(all, sinks, key) >> (16 * c));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) keep[p][k] = kv_bytes(see >> (4 * k));
         }
       }
       ok = mbar_wait(&v_empty[s], ((j / NS) & 1) ^ 1, abort_flag);
@@ -463,9 +464,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int i = 2 * (j0 + j) + p;
           const int key = i < pages.n ? pages.at(i) * kKvPage : 0x40000000;  // no page: no key
           if (!(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= sinks))) {
+            const uint64_t see = kv_bits(span, sinks, key);
+            const uint32_t word[2] = {static_cast<uint32_t>(see), static_cast<uint32_t>(see >> 32)};
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (!kv_visible(span, sinks, key + c)) sf[p * 64 + c] = -INFINITY;
+              if (!(word[c >> 5] >> (c & 31) & 1)) sf[p * 64 + c] = -INFINITY;
           }
         }
         float mp[8];

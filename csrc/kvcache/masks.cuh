@@ -17,9 +17,14 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttendArgs& a, int pos, int le
   s.lo = a.window > 0 ? max(first, (frame - a.window + 1) * a.unit) : first;
   return s;
 }
-__device__ __forceinline__ bool kv_visible(const KvSpan& s, int sinks, int key) {
-  return key < s.hi && (key >= s.lo || key < sinks);
+
+// The visible keys of the page at `key0`, a bit each.
+__device__ __forceinline__ uint64_t kv_bits(const KvSpan& s, int sinks, int key0) {
+  auto below = [](int n) -> uint64_t { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+  return below(s.hi - key0) & (~below(s.lo - key0) | below(sinks - key0));
 }
+// bytes of a word for four of those bits
+__device__ __forceinline__ uint32_t kv_bytes(uint32_t bits) { return ((bits & 15u) * 0x00204081u & 0x01010101u) * 255u; }
 
 // The pages that some query of a tile sees: the first `n_sink`, then from `page0` on. `lo`
 // and `hi` are the tile's smallest and largest (both grow with the position).
