@@ -12,7 +12,22 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return amax > 0.f && k < 128 ? max(k - 14, -120) : 0;
 }
 
+// Pages that a query sees at most: all, or the sinks', the window's and the call's own.
+inline int kv_seen_pages(const KvAttendArgs& a) {
+  const long all = a.max_tokens;
+  const long near = a.sinks + (a.window + 1L) * a.unit + a.T + 2 * kKvPage;
+  return static_cast<int>(((a.window > 0 && near < all ? near : all) + kKvPage - 1) / kKvPage);
+}
+
+// How a launch shares a row tile's pages, and how long it should take: measured times of a CTA's
+// start, merge and steps, times the waves of CTAs.
+struct KvPlan {
+  int ranks = 1;   // CTAs of a cluster
+  double us = 0.;
+};
+
 // attend_tiles.cu: blocks of 256 rows on the tensor cores' 128-row products
-void kv_attend_tiles_launch(KvAttendArgs a, int dev, cudaStream_t stream);
+KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev);
+void kv_attend_tiles_launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream);
 
 }  // namespace ddb

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
   const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
   const int r0 = tile * R, rows = own * G;           // rows behind `rows` are padding
-  // token of a row: rows are few, so a multiplication by 2^32 / G rounded up is exact
+  // token of a row: at most 256 rows, so the product with 2^32 / G rounded up is exact
   auto token = [&](int r) -> int { return G == 1 ? r : __umulhi(r, group_inv); };
 
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + off_bar(NT)) + pg * 2 * kMaxStages;
@@ -416,32 +416,40 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   if (ranks > 1) cluster_sync_all();  // no CTA leaves while another reads its results
 }
 
+// Share the pages of an item over the CTAs of a cluster while SMs stand idle (with few rows,
+// three CTAs fit one) and every group keeps a page or more. A CTA's start and merge
+// measured 5 us, a group's page 2.1 us with 32 rows (512 CTAs of 12 pages a group,
+// 4 waves: 118 us; 96 of 10, one wave: 28 us).
+KvPlan rows_plan(const KvAttendArgs& a, int NT, int dev) {
+  const long slots = static_cast<long>(num_sms(dev)) * (NT == 1 ? 3 : NT == 2 ? 2 : 1);
+  const int tiles = (a.T * (a.H / a.pool.heads) + 8 * NT - 1) / (8 * NT);
+  const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
+  const int pages = kv_seen_pages(a);
+  KvPlan p;
+  while (p.ranks < 8 && items * p.ranks * 2 <= slots && pages >= p.ranks * 2 * kGroups) p.ranks *= 2;
+  const int each = (pages + p.ranks * kGroups - 1) / (p.ranks * kGroups);
+  p.us = static_cast<double>((items * p.ranks + slots - 1) / slots) * (5. + 2.1 * each);
+  return p;
+}
+
 template <int NT>
-void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
+void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (dev & 63) & 1)) {
     check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
                "cudaFuncSetAttribute(kv_attend_rows)");
     set.fetch_or(1ull << (dev & 63));
   }
-  const int G = a.H / a.pool.heads, sms = num_sms(dev);
+  const int G = a.H / a.pool.heads;
   const int tiles = (a.T * G + 8 * NT - 1) / (8 * NT);
-  const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
-  // The pages that a tile sees at most: all, or the sinks', the window's and its own rows'.
-  const long seen = std::min<long>(a.max_tokens, a.window > 0 ? a.sinks + (a.window + 1L) * a.unit + a.T + 2 * kKvPage : a.max_tokens);
-  const int pages = static_cast<int>((seen + kKvPage - 1) / kKvPage);
-  // Share the pages of an item over the CTAs of a cluster while SMs stand idle (with few
-  // rows, three CTAs fit one) and every group keeps a page or more.
-  const long slots = static_cast<long>(sms) * (NT == 1 ? 3 : NT == 2 ? 2 : 1);
-  int ranks = 1;
-  while (ranks < 8 && items * ranks * 2 <= slots && pages >= ranks * 2 * kGroups) ranks *= 2;
-  if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  const long ctas = static_cast<long>(a.step.B) * a.pool.heads * tiles * ranks;
+  if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
   a.cluster = ranks;
   // Stages: all that fit where an SM holds one CTA anyway (few rows of few sequences wait for
   // the copies' latency), fewer where more CTAs share it.
-  const int stages = NT > 2 || items * ranks <= sms ? kMaxStages : NT == 2 ? 3 : 2;
+  const int stages = NT > 2 || ctas <= num_sms(dev) ? kMaxStages : NT == 2 ? 3 : 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kGroups * NT * 32);
   cfg.dynamicSmemBytes = smem_bytes(NT, stages);
   cfg.stream = stream;
@@ -456,23 +464,38 @@ void launch(KvAttendArgs a, int dev, cudaStream_t stream) {
   count_launch();
 }
 
+// Rows beyond which only the 256-row blocks are tried: there each page is read by 8 row
+// tiles of the other kernel. (Its rows' division by multiplication is exact far beyond.)
+constexpr long kMaxRows = 256;
+
 }  // namespace
 
+// Up to 32 rows one row tile of kv_attend_rows takes them, the narrowest that does (32 rows:
+// 28 us against the blocks' 42 at 12 heads of 20,000 tokens, 118 against 195 at 512 of
+// 3,000). Beyond, its pages are read once for every 32 rows, and the smaller estimate
+// decides: 64 rows take 15 us against 17 at 48 heads of 1,000 visible tokens, 205 against
+// 196 at 512 of 3,000; 128 rows 28 against 18, 412 against 216; few and short sequences stay
+// with it longer.
 void kv_cache_attend(const KvAttendArgs& a, cudaStream_t stream) {
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
-  if (rows > 64)
-    kv_attend_tiles_launch(a, dev, stream);
-  else if (rows <= 8)
-    launch<1>(a, dev, stream);
-  else if (rows <= 16)
-    launch<2>(a, dev, stream);
-  else if (rows <= 24)
-    launch<3>(a, dev, stream);
-  else
-    launch<4>(a, dev, stream);
+  const int NT = rows <= 24 ? static_cast<int>(rows + 7) / 8 : 4;
+  const KvPlan few = rows <= kMaxRows ? rows_plan(a, NT, dev) : KvPlan{};
+  if (rows > 32) {
+    const KvPlan many = kv_attend_tiles_plan(a, dev);
+    if (rows > kMaxRows || many.us < few.us) {
+      kv_attend_tiles_launch(a, many.ranks, dev, stream);
+      return;
+    }
+  }
+  switch (NT) {
+    case 1: launch<1>(a, few.ranks, dev, stream); break;
+    case 2: launch<2>(a, few.ranks, dev, stream); break;
+    case 3: launch<3>(a, few.ranks, dev, stream); break;
+    default: launch<4>(a, few.ranks, dev, stream); break;
+  }
 }
 
 }  // namespace ddb

@@ -628,55 +628,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
-void kv_attend_tiles_launch(KvAttendArgs a, int dev, cudaStream_t stream) {
+namespace {
+void raise_limit(int dev) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
-  if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
-               "cudaFuncSetAttribute(kv_attend_tiles)");
-    set.fetch_or(1ull << (dev & 63));
-  }
-  const int G = a.H / a.pool.heads;
-  const int tiles = (a.T * G + kRows - 1) / kRows;
-  const long items = static_cast<long>(a.step.B) * a.pool.heads * tiles;
+  if (set.load() >> (dev & 63) & 1) return;
+  check_cuda(cudaFuncSetAttribute(kv_attend_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+             "cudaFuncSetAttribute(kv_attend_tiles)");
+  set.fetch_or(1ull << (dev & 63));
+}
+int row_blocks(const KvAttendArgs& a) { return static_cast<int>((a.T * static_cast<long>(a.H / a.pool.heads) + kRows - 1) / kRows); }
+long row_items(const KvAttendArgs& a) { return static_cast<long>(a.step.B) * a.pool.heads * row_blocks(a); }
+cudaLaunchConfig_t config(int ranks, cudaLaunchAttribute* attr) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = ranks;
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = SMEM_BYTES;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  // Share an item's key tiles over the CTAs of a cluster: time ~ waves of clusters x key
-  // tiles of one CTA, the fewest CTAs with the smallest estimate; a CTA keeps 8 key tiles
-  // or more, some times the cost of its start and of the merge. How many clusters of a
-  // size run at once is the device's to say: of 3 CTAs only 45 do on 148 SMs (the GPCs'
-  // SMs are no multiple), so 96 of them take three waves, not two.
-  const int pairs = (a.max_tokens + 2 * kKvPage - 1) / (2 * kKvPage);
+  cfg.numAttrs = 1;
+  return cfg;
+}
+}  // namespace
+
+// The cluster size with the smallest estimate. How many clusters of a size run at once is the
+// device's to say: of 3 CTAs only 45 do on 148 SMs (the GPCs' SMs are no multiple), so 96 of
+// them take three waves, not two. A CTA's start and merge measured 7 us, a step (128 keys)
+// 1.7 us with one row tile and 2.4 us with two: 512 CTAs of 24 steps (4 waves) take
+// 190 / 254 us, 96 of 20 steps (one wave) 40 / 51 us.
+KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev) {
+  raise_limit(dev);
   static std::atomic<int> fits[64][9];
-  int ranks = 1;
-  double best = 0.;
-  for (int s = 1; s <= 8 && (s == 1 || pairs / s >= 8); ++s) {
+  const int pairs = (kv_seen_pages(a) + 1) / 2;
+  const double step = a.T * static_cast<long>(a.H / a.pool.heads) > 128 ? 2.4 : 1.7;
+  KvPlan best;
+  for (int s = 1; s <= 8 && (s == 1 || pairs >= 2 * s); ++s) {
     int slots = s == 1 ? num_sms(dev) : fits[dev & 63][s].load();
     if (slots == 0) {
-      cfg.gridDim = dim3(s);
-      attr[0].val.clusterDim.x = s;
-      cfg.numAttrs = 1;
+      cudaLaunchAttribute attr[1];
+      const cudaLaunchConfig_t cfg = config(s, attr);
       check_cuda(cudaOccupancyMaxActiveClusters(&slots, kv_attend_tiles, &cfg), "cudaOccupancyMaxActiveClusters");
       slots = std::max(slots, 1);
       fits[dev & 63][s].store(slots);
     }
-    const double t = static_cast<double>((items + slots - 1) / slots) / s;
-    if (s == 1 || t < best - 1e-9) {
-      best = t;
-      ranks = s;
-    }
+    const double us = static_cast<double>((row_items(a) + slots - 1) / slots) * (7. + step * ((pairs + s - 1) / s));
+    if (s == 1 || us < best.us) best = KvPlan{s, us};
   }
-  if (items * ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  return best;
+}
+
+void kv_attend_tiles_launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
+  raise_limit(dev);
+  const long ctas = row_items(a) * ranks;
+  if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
   a.cluster = ranks;
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  attr[0].val.clusterDim.x = ranks;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = config(ranks, attr);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.stream = stream;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, tiles, device_status(dev)), "kv_attend_tiles launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, row_blocks(a), device_status(dev)), "kv_attend_tiles launch");
   count_launch();
 }
 
