@@ -1432,6 +1432,7 @@ ddb::AttnArgs window_args(const torch::Tensor& q, const torch::Tensor& k, const 
                   unit >= 1 && unit <= (1 << 24) && window >= 0 && window * unit <= limit && sinks >= 0 && sinks <= limit,
               "windowed attention: positions, unit, window or sinks out of range");
   TORCH_CHECK(causal == ddb::kCausalNone || causal == ddb::kCausalFrame, "windowed attention: causal is 0 or 1");
+  TORCH_CHECK(B * q.size(1) <= 0x7fffffff && B * k.size(1) <= 0x7fffffff, "windowed attention: too many rows");
   a.B = B; a.H = H; a.Tq = q.size(1); a.S = k.size(1);
   a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
   a.q_rows_per_b = a.Tq; a.kv_rows_per_b = a.S;

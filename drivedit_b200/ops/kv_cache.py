@@ -20,13 +20,18 @@ Use::
 What a cached block stands for: ``code * scale``, ``scale = 2^e`` with the smallest ``e``
 for which the block's largest finite magnitude is at most ``448 * 2^e`` (``e`` in
 [-100, 119]), codes rounded to nearest even, infinities saturated, NaN kept. Writing into an
-unfinished page re-codes the tokens it already holds when its scale changes.
+unfinished page re-codes the tokens it already holds when its scale changes: exactly, but
+for codes that become subnormal, so tokens of far larger magnitude in the same page (also
+ones that are never committed) leave small values coarser.
 
 CUDA caches run the sm_100a kernels (``csrc/kvcache``); CPU caches the PyTorch statements
 below, which are also the kernels' oracle. Calls run on the current stream. A step may
 be used on another stream than the one it was begun on (its table is waited for); the
 order of writes and reads of the cache itself between streams is the caller's, as for
-any tensor. Bookkeeping is on the host: calls on one cache come from one thread.
+any tensor. Bookkeeping is on the host: calls on one cache come from one thread, and none
+that changes it can be captured into a graph. ``write`` and ``attend`` can; a graph that
+holds them is replayed after its step was refilled (``begin(..., out=step)``) for the
+sequences as they are then, and not after :meth:`PagedKVCache.resize`.
 """
 from __future__ import annotations
 
@@ -340,8 +345,9 @@ class PagedKVCache:
 
         ``max_tokens``: the longest sequence (its new tokens counted) that the step's launches
         are shaped for, for steps whose calls are captured into a graph; default: the
-        longest of now. ``out``: a step of as many sequences to refill in place, so that
-        a graph captured with it runs on the new tables; its ``max_tokens`` must suffice."""
+        longest of now. ``out``: a step of as many sequences to refill in place (on the current
+        stream, behind the calls that still read it), so that a graph captured with it runs
+        on the new tables; its ``max_tokens`` must suffice."""
         self._not_capturing("begin")
         states = self._get(seqs)
         n_new = [int(n_new)] * len(states) if not isinstance(n_new, (list, tuple)) else [int(n) for n in n_new]
@@ -514,7 +520,7 @@ class PagedKVCache:
 
     def resize(self, n_pages: int) -> None:
         """Change the pool to ``n_pages`` pages (compacted first when it shrinks below a page
-        in use); the pages in use keep their contents."""
+        in use); the pages in use keep their contents. The pool's tensors are new ones."""
         self._not_capturing("resize")
         used = self.n_pages - self._n_free
         if n_pages < max(used, 1):

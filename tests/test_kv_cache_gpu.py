@@ -355,6 +355,67 @@ def test_pool_past_32_bit_offsets():
     _check(o[0], lse[0], ref, mean, rlse, mag)
 
 
+def test_refusals():
+    c = _cache(2, 2, 8, max_pages_per_seq=4)
+    a, b = c.add(2)
+    step = c.begin([a, b], [3, 1])
+    k = _randn(2, 3, 2, 64)
+    for call in (lambda: step.write(2, k, k), lambda: step.write(-1, k, k), lambda: step.write(0, k[:1], k[:1]),
+                 lambda: step.write(0, k[:, :2], k[:, :2]), lambda: step.write(0, k[:, :, :1], k[:, :, :1]),
+                 lambda: step.write(0, k, k[:, :, :, :32]), lambda: step.write(0, k.float(), k.float()),
+                 lambda: step.write(0, k.cpu(), k.cpu()), lambda: step.attend(0, _randn(2, 3, 3, 64)),
+                 lambda: step.attend(5, k), lambda: step.attend(0, k.half()), lambda: step.attend(0, k, causal="x"),
+                 lambda: step.attend(0, k, causal="none", window=3), lambda: step.attend(0, k, tokens_per_frame=0),
+                 lambda: step.attend(0, k, window=-1), lambda: step.attend(0, k, scale=0.0), lambda: c.begin([a], 1, out=step),
+                 lambda: c.begin([a, b], [9, 9], max_tokens=500, out=step), lambda: c.begin([a], 1000)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError):
+        c.begin([a, b], 256) and c.begin(c.add(1), 64)
+    with pytest.raises(RuntimeError):  # stale by then
+        step.write(0, k, k)
+    for bad in ([0, 0], [0, 99], [1, 0]):  # a page twice, outside, read and written
+        with pytest.raises(RuntimeError):
+            from drivedit_b200.ops._ext import ext
+            ext().kv_cache_copy_pages(c.k, c.v, c.k_scale, c.v_scale, torch.tensor([1, 2], dtype=torch.int32),
+                                      torch.tensor(bad, dtype=torch.int32))
+    torch.cuda.synchronize()
+
+
+def test_empty_calls():
+    c = _cache(1, 2, 8)
+    step = c.begin([], 0)
+    assert step.attend(0, _randn(0, 3, 4, 64)).shape == (0, 3, 4, 64)
+    seqs = c.add(2)
+    step = c.begin(seqs, 0)
+    step.write(0, _randn(2, 0, 2, 64), _randn(2, 0, 2, 64))
+    assert step.attend(0, _randn(2, 0, 2, 64)).shape == (2, 0, 2, 64)
+    o, lse = step.attend(0, _randn(2, 5, 2, 64), return_lse=True)
+    assert not o.any() and (lse == -math.inf).all()
+    c.free([])
+    assert c.fork([], 3) == [] and c.copy([]) == [] and c.compact() == 0
+
+
+@pytest.mark.parametrize("T", [1, 40, 300])
+def test_two_streams_at_once(T):
+    """The same call on two streams at a time, many times: no shared workspace."""
+    c = _cache(1, 2, 200)
+    seqs = _fill(c, [5000, 3000])
+    step = c.begin(seqs, T)
+    step.write(0, _randn(2, T, 2, 64), _randn(2, T, 2, 64))
+    qs = [_randn(2, T, 4, 64) for _ in range(2)]
+    want = [step.attend(0, q, causal="token", window=4000, sinks=9) for q in qs]
+    torch.cuda.synchronize()
+    outs, streams = [[], []], [torch.cuda.Stream() for _ in qs]
+    for _ in range(10):
+        for q, s, o in zip(qs, streams, outs):
+            with torch.cuda.stream(s):
+                o.append(step.attend(0, q, causal="token", window=4000, sinks=9))
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, x) for x in o)
+
+
 def test_status_clean():
     from drivedit_b200.ops._ext import device_status
     torch.cuda.synchronize()

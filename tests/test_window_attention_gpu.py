@@ -326,3 +326,38 @@ def test_rollout_branches_on_the_kernels():
     assert res.frames.shape == (6, 10, 16, 16, 16) and torch.isfinite(res.frames).all()
     # the same pages' contents and the same kernels: equal but for the context's batch shape
     assert (res.frames - one.frames).norm() / one.frames.norm() < 2.0 ** -6
+
+
+def test_refusals():
+    from drivedit_b200.ops.window_attention import window_attention
+    q, k = _bits(1, 4, 2, 64), _bits(1, 6, 2, 64)
+    for bad in (lambda: window_attention(q[..., :32], k[..., :32], k[..., :32]),
+                lambda: window_attention(q, k[:, :, :1], k[:, :, :1]),
+                lambda: window_attention(q, k, k[:, :5]),
+                lambda: window_attention(q.float(), k.float(), k.float()),
+                lambda: window_attention(q, k.float(), k.float()),
+                lambda: window_attention(q, k.cpu(), k.cpu()),
+                lambda: window_attention(q, k, k, "block"),
+                lambda: window_attention(q, k, k, "none", window=2),
+                lambda: window_attention(q, k, k, "frame", 0),
+                lambda: window_attention(q, k, k, "frame", (1 << 24) + 1),
+                lambda: window_attention(q, k, k, "token", window=-1),
+                lambda: window_attention(q, k, k, "token", sinks=-1),
+                lambda: window_attention(q, k, k, q_pos_offset=1 << 30),
+                lambda: window_attention(q, k, k, scale=0.0),
+                lambda: window_attention(q, k, k, scale=math.inf)):
+        with pytest.raises(ValueError):
+            bad()
+    # a window and sinks past every position are all of them
+    want = window_attention(q, k, k, "token", q_pos_offset=2)
+    assert torch.equal(window_attention(q, k, k, "token", window=1 << 40, sinks=1 << 40, q_pos_offset=2), want)
+    assert torch.equal(window_attention(q, k, k, "frame", 1 << 24), window_attention(q, k, k, "none"))
+    torch.cuda.synchronize()
+
+
+def test_no_second_derivative():
+    from drivedit_b200.ops.window_attention import window_attention
+    q = _bits(1, 8, 1, 64).requires_grad_(True)
+    (g,) = torch.autograd.grad(window_attention(q, q, q, "token").sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), q)

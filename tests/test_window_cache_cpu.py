@@ -59,6 +59,21 @@ def test_window_attention_refusals():
             bad()
 
 
+def test_extension_errors_name_numbers():
+    """Errors of the extension that print numbers reach Python (its C++ library is the one that
+    torch uses)."""
+    from drivedit_b200.ops import _ext
+    if not _ext.available():
+        pytest.skip("extension not built")
+    q = torch.randn(1, 4, 1, 64).bfloat16()
+    for args, text in ((("token", 1, 0, 0, 1 << 30, 0, None), "1073741824"), (("token", 1, 0, 0, 0, 0, math.inf), "finite"),
+                       (("frame", 1 << 25, 0, 0, 0, 0, None), "2\\^24"), (("block", 1, 0, 0, 0, 0, None), "block")):
+        with pytest.raises(ValueError, match=text):
+            _ext.ext().window_attention(q, q, q, *args)
+    with pytest.raises(ValueError, match=r"\[1, 4, 1, 32\]"):
+        _ext.ext().window_attention(q[..., :32], q, q, "token", 1, 0, 0, 0, 0, None)
+
+
 def test_quantize_block_definition():
     torch.manual_seed(0)
     x = torch.randn(7, 64, 64) * torch.logspace(-12, 12, 7)[:, None, None]
