@@ -96,6 +96,7 @@ struct AttnBwdArgs {
   int max_q = 0;
   int debug_flags = 0;        // bit 0: skip the dQ reductions (timing experiments only)
   long do_sb = 0, do_st = 0, do_sh = 0;  // windowed mode: strides of dout
+  int q_front = 0;            // windowed mode, set by the launch: first queries that see no key
   long long* trace = nullptr; // optional per-role clock64 trace of CTA `trace_cta`
   int trace_cta = 0;
 };

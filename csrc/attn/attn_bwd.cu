@@ -228,10 +228,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long vb = static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + qb * 64;
         mbar_arrive_expect_tx(&qd_full[s], 2 * TILE + 1024);
         if constexpr (WIN) {
-          tma_load_4d(sq, &tmQ, &qd_full[s], 0, h, qa * 64, b);
-          tma_load_4d(sq + 8192, &tmQ, &qd_full[s], 0, h, qb * 64, b);
-          tma_load_4d(sd, &tmDO, &qd_full[s], 0, h, qa * 64, b);
-          tma_load_4d(sd + 8192, &tmDO, &qd_full[s], 0, h, qb * 64, b);
+          // from the maps' first row; rows before it read as zeros
+          const int ra = qa * 64 - g.q_front, rb = qb * 64 - g.q_front;
+          tma_load_4d(sq, &tmQ, &qd_full[s], 0, h, ra, b);
+          tma_load_4d(sq + 8192, &tmQ, &qd_full[s], 0, h, rb, b);
+          tma_load_4d(sd, &tmDO, &qd_full[s], 0, h, ra, b);
+          tma_load_4d(sd + 8192, &tmDO, &qd_full[s], 0, h, rb, b);
         } else {
           tma_load_2d(sq, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qa * 64);
           tma_load_2d(sq + 8192, &tmQ, &qd_full[s], a.q_col + h * 64, rowb + qb * 64);
@@ -803,7 +805,8 @@ void attn_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
   launch_bwd(g, device_status(dev), stream);
 }
 
-void attn_window_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
+void attn_window_bwd(const AttnBwdArgs& args, cudaStream_t stream) {
+  AttnBwdArgs g = args;
   const AttnArgs& a = g.f;
   if (a.B <= 0 || a.H <= 0 || a.S <= 0 || a.Tq <= 0) return;
   const int n_kvtiles = (a.S + 127) / 128;
@@ -817,10 +820,16 @@ void attn_window_bwd(const AttnBwdArgs& g, cudaStream_t stream) {
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   raise_smem_limit<attn_bwd_kernel<true>>(SMEM_BYTES, dev);
-  const CUtensorMap tQ = window_tmap(a.q, a.B, a.Tq, a.H, a.q_sb, a.q_st, a.q_sh);
+  // Queries that see no key stand at the front or at the end. The maps of q and dout leave them
+  // out, so that what they hold stays out of dV = P^T dO and dK = dS^T Q (0 * NaN).
+  const WindowQueries first = window_queries(a, 0), last = window_queries(a, a.S - 1);
+  g.q_front = std::min(first.lo, a.Tq - 1);
+  const int rows = std::max(std::max(first.hi, last.hi) - g.q_front, 1);
+  const auto from = [&](const void* x, long st) { return static_cast<const __nv_bfloat16*>(x) + g.q_front * st; };
+  const CUtensorMap tQ = window_tmap(from(a.q, a.q_st), a.B, rows, a.H, a.q_sb, a.q_st, a.q_sh);
   const CUtensorMap tK = window_tmap(a.k, a.B, a.S, a.H, a.k_sb, a.k_st, a.k_sh);
   const CUtensorMap tV = window_tmap(a.v, a.B, a.S, a.H, a.v_sb, a.v_st, a.v_sh);
-  const CUtensorMap tDO = window_tmap(g.dout, a.B, a.Tq, a.H, g.do_sb, g.do_st, g.do_sh);
+  const CUtensorMap tDO = window_tmap(from(g.dout, g.do_st), a.B, rows, a.H, g.do_sb, g.do_st, g.do_sh);
   // dQ accumulator [B, Tq, H, 64] fp32, boxes of 32 columns x 64 queries of one head
   const uint64_t dims[4] = {64, static_cast<uint64_t>(a.H), static_cast<uint64_t>(a.Tq), static_cast<uint64_t>(a.B)};
   const uint64_t strides[3] = {256, 256ull * a.H, 256ull * a.H * a.Tq};

@@ -48,8 +48,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     frame ``p // tokens_per_frame`` and sees that whole frame and earlier ones, of those
     the newest ``window`` (its own counted; 0: all) and the first ``sinks``; "token" counts
     tokens instead of frames; "none" sees every key. Keys sit at their index plus
-    ``kv_pos_offset``. Rows that see no key are zero and get no gradient; keys that no
-    query sees get zero gradients, and their values have no effect. Returns ``o`` (and, if
+    ``kv_pos_offset``. Rows that see no key are zero and keys that no query sees are
+    left out; both get zero gradients, and what they hold has no effect on the others. Returns ``o`` (and, if
     asked, ``lse [B, H, T]``, log2 domain of the scaled scores, without gradient). dQ is
     summed in fp32 in no fixed order: equal backward passes may differ in dq by a rounding
     of bf16. A backward pass is captured into a graph only when no autograd graph of the same
@@ -73,10 +73,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     else:
         seen = window_mask(T, S, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, q.device)
         f = torch.promote_types(q.dtype, torch.float32)
-        s = torch.einsum("bthd,bshd->bhts", q.to(f), k.to(f)) * scale
-        s = torch.where(seen, s, -math.inf)
-        some = seen.any(1)[:, None]
-        p = torch.softmax(torch.where(some, s, 0.0), -1) * some
-        o = torch.einsum("bhts,bshd->bthd", p, torch.where(seen.any(0)[:, None, None], v.to(f), 0.0)).to(q.dtype)
+        some, used = seen.any(1)[:, None, None], seen.any(0)[:, None, None]  # by query, by key
+        # what hidden rows hold stays out of the products, and of the gradients' (0 * NaN)
+        qf, kf, vf = torch.where(some, q.to(f), 0.0), torch.where(used, k.to(f), 0.0), torch.where(used, v.to(f), 0.0)
+        s = torch.where(seen, torch.einsum("bthd,bshd->bhts", qf, kf) * scale, -math.inf)
+        p = torch.softmax(torch.where(some[..., 0], s, 0.0), -1)
+        o = torch.where(some, torch.einsum("bhts,bshd->bthd", p, vf), 0.0).to(q.dtype)
         lse = torch.logsumexp(s, -1).float().detach() / math.log(2)
     return (o, lse) if return_lse else o

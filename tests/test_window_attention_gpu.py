@@ -145,6 +145,30 @@ def test_hidden_keys_do_not_matter():
     assert not got[2][:, hidden].any() and not got[3][:, hidden].any()
 
 
+@pytest.mark.parametrize("q_off,kv_off,unit", [(0, 50, 1), (0, 130, 1), (250, 0, 1), (40, 100, 20), (1000, 0, 1), (0, 400, 1)])
+def test_hidden_queries_do_not_matter(q_off, kv_off, unit):
+    """NaN in queries that see no key (before the first key, behind the window of the last),
+    in the same tiles as others, and in the gradients of their outputs."""
+    from drivedit_b200.ops.window_attention import window_attention
+    B, T, S, H = 2, 200, 300, 2
+    q, k, v = (x.requires_grad_(True) for x in (_bits(B, T, H, 64), _bits(B, S, H, 64), _bits(B, S, H, 64)))
+    do = _bits(B, T, H, 64)
+    args = ("frame", unit, 60 // unit, 0, q_off, kv_off)
+    hidden = ~_seen(T, S, "frame", unit, 60 // unit, 0, q_off, kv_off).any(1)
+    assert hidden.any()
+    o = window_attention(q, k, v, *args)
+    want = (o, *torch.autograd.grad(o, (q, k, v), do))
+    do[:, hidden] = math.nan
+    with torch.no_grad():
+        q[:, hidden] = math.nan
+    o = window_attention(q, k, v, *args)
+    got = (o, *torch.autograd.grad(o, (q, k, v), do))
+    assert torch.equal(got[0], want[0]) and not got[0][:, hidden].any() and not got[1][:, hidden].any()
+    for a, b in zip(got[1:], want[1:]):
+        # dq is summed in another order: one rounding of bf16 apart at most
+        assert torch.isfinite(a).all() and ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-5).all()
+
+
 def test_gradient_against_differences():
     """Directional differences of the forward kernel's own output, in a direction along which
     it is smooth: bf16 inputs moved by whole steps."""

@@ -6,6 +6,7 @@ import torch
 
 from drivedit_b200.config import get_config
 from drivedit_b200.inference.rollout import StreamingRollout
+from drivedit_b200.layers.attention import window_mask
 from drivedit_b200.models.world_dit import KVCacheSet, PagedKVCacheSet, WorldDiT, forward_cached
 from drivedit_b200.ops.kv_cache import PagedKVCache, quantize_block
 from drivedit_b200.ops.window_attention import window_attention
@@ -38,6 +39,25 @@ def test_window_attention_definition_and_gradients(T, S, causal, unit, window, s
     assert lse.shape == (2, 2, T)
     small = [x[:1, :, :1].detach().clone().requires_grad_(True) for x in (q, k, v)]
     assert torch.autograd.gradcheck(lambda *x: window_attention(*x, *args), small, fast_mode=True)
+
+
+@pytest.mark.parametrize("q_off,kv_off", [(250, 0), (0, 50), (0, 400)])
+def test_window_attention_hidden_rows(q_off, kv_off):
+    """What queries without a key and keys without a query hold reaches nothing else."""
+    args = ("token", 1, 60, 0, q_off, kv_off)
+    q, k, v = (torch.randn(1, n, 2, 64, requires_grad=True) for n in (200, 300, 300))
+    do = torch.randn(1, 200, 2, 64)
+    seen = window_mask(200, 300, *args)
+    rows, keys = ~seen.any(1), ~seen.any(0)
+    o = window_attention(q, k, v, *args)
+    want = (o, *torch.autograd.grad(o, (q, k, v), do))
+    do[:, rows] = math.nan
+    with torch.no_grad():
+        q[:, rows] = math.nan
+        k[:, keys] = math.nan
+        v[:, keys] = math.nan
+    o = window_attention(q, k, v, *args)
+    assert all(torch.equal(a, b) for a, b in zip((o, *torch.autograd.grad(o, (q, k, v), do)), want))
 
 
 def test_window_attention_refusals():
