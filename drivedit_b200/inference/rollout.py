@@ -219,7 +219,7 @@ class StreamingRollout:
         total = total_frames or cfg.total_frames
         chunk = cfg.chunk_frames
         fwd_chunk = getattr(m, "forward_cached_chunk", None)
-        cache = self._make_cache(B, total, branches)
+        cache = self._make_cache(B, max(total, Fc), branches)
 
         def forward_cached(m_, x_, t_, a_, cache_, commit=False, extra_cond=None):
             if fwd_chunk is not None:

@@ -306,6 +306,14 @@ def test_paged_stream_near_full_forward(over):
         assert torch.equal(again, got)
 
 
+def test_rollout_of_a_context_longer_than_asked():
+    cfg, m = _model()
+    r = cfg.rollout
+    r.total_frames, r.chunk_frames, r.flow_steps, r.window_frames, r.kv_cache = 2, 2, 1, 3, "fp8"
+    ctx = torch.randn(1, 14, 16, 16, 16)
+    assert torch.equal(StreamingRollout(m, r).run(ctx, torch.rand(1, 14, 2)).frames, ctx)
+
+
 def test_rollout_over_the_paged_cache_and_branches():
     cfg, m = _model()
     r = cfg.rollout
