@@ -28,8 +28,8 @@ CUDA caches run the sm_100a kernels (``csrc/kvcache``); CPU caches the PyTorch s
 below, which are also the kernels' oracle. Calls run on the current stream. A step may
 be used on another stream than the one it was begun on (its table is waited for); the
 order of writes and reads of the cache itself between streams is the caller's, as for
-any tensor. Bookkeeping is on the host: calls on one cache come from one thread, and none
-that changes it can be captured into a graph. ``write`` and ``attend`` can; a graph that
+any tensor. Bookkeeping (``csrc/kvcache/book.cpp``) is on the host: calls on one cache come
+from one thread, and none that changes it can be captured into a graph. ``write`` and ``attend`` can; a graph that
 holds them is replayed after its step was refilled (``begin(..., out=step)``) for the
 sequences as they are then, and not after :meth:`PagedKVCache.resize`.
 """
@@ -51,21 +51,6 @@ _MAX_TOKENS = 1 << 30
 
 def _pages(tokens: int) -> int:
     return (tokens + PAGE - 1) // PAGE
-
-
-class _Seq:
-    __slots__ = ("pages", "length", "first", "sinks", "version")
-
-    def __init__(self, pages, length=0, first=0, sinks=0):
-        self.pages = pages          # int32 ids by page of the sequence; -1: given back
-        self.length = length        # committed tokens
-        self.first = first          # tokens in [sinks, first) are gone
-        self.sinks = sinks
-        self.version = 0            # a step begun at another version is stale
-
-    @property
-    def trimmed(self):
-        return self.first > self.sinks
 
 
 def _two_to(e: torch.Tensor) -> torch.Tensor:
@@ -90,13 +75,11 @@ class CacheStep:
     Once a sequence of the step has changed otherwise (commit, trim, fork, free, a later
     ``begin``, compaction) the step is stale and its calls raise."""
 
-    def __init__(self, cache: "PagedKVCache", seqs, n_new, max_tokens, table, handle):
+    def __init__(self, cache: "PagedKVCache", seqs, n_new, versions, max_tokens, table, handle):
         self.cache = cache
         self.seqs, self.n_new = seqs, n_new
         self.max_tokens = max_tokens  # launches are shaped for sequences up to this length
-        self._states = [cache._seqs[i] for i in seqs]
-        self._versions = [s.version for s in self._states]
-        self._epoch = cache._epoch
+        self._versions, self._epoch = versions, cache._book.epoch
         self._rows, self._h = table, handle
 
     @property
@@ -105,10 +88,15 @@ class CacheStep:
         return (self._rows if self._h is None else self._h.rows)[:, _INFO:]
 
     def _check(self):
-        if self._epoch != self.cache._epoch:  # something of the cache has changed
-            if any(s.version != v for s, v in zip(self._states, self._versions)):
+        book = self.cache._book
+        if self._epoch != book.epoch:  # something of the cache has changed
+            if not book.fresh(self.seqs, self._versions):
                 raise RuntimeError("stale step: a sequence has changed since it was begun; begin a new one")
-            self._epoch = self.cache._epoch
+            self._epoch = book.epoch
+
+    @property
+    def _states(self):
+        return [self.cache._book.seq(i) for i in self.seqs]
 
     def _tokens(self, x: torch.Tensor, name: str, heads: Optional[int]):
         """The extension's checks, for the PyTorch form."""
@@ -166,10 +154,7 @@ class CacheStep:
     def commit(self) -> None:
         """Keep the step's tokens: its sequences grow by ``n_new``."""
         self._check()
-        self.cache._epoch += 1
-        for s, n in zip(self._states, self.n_new):
-            s.length += n
-            s.version += 1
+        self.cache._book.commit(self.seqs, self.n_new)
 
     # ------------------------------------------------------------------ PyTorch form
     def _write_torch(self, layer, k, v):
@@ -240,11 +225,7 @@ class PagedKVCache:
         if not 1 <= self.max_pages_per_seq <= _MAX_TOKENS // PAGE:
             raise ValueError("max_pages_per_seq out of range")
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
-        self._refs = np.zeros(n_pages, np.int32)  # sequences that hold a page
-        self._n_free, self._low = n_pages, 0      # no page below _low is free
-        self._seqs: dict = {}
-        self._next = 0
-        self._epoch = 0                           # counts changes of any sequence
+        self._book = ext().KvBook(n_pages, self.max_pages_per_seq)
 
     def _pool(self, n):
         shape = (self.n_layers, n, self.n_heads)
@@ -256,49 +237,23 @@ class PagedKVCache:
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of a cache of {self.n_layers}")
 
-    def _get(self, seqs) -> List[_Seq]:
-        if len(set(seqs)) != len(seqs):
-            raise ValueError("a sequence is named twice")
-        missing = [i for i in seqs if i not in self._seqs]
-        if missing:
-            raise ValueError(f"no sequence {missing[0]} in this cache")
-        return [self._seqs[i] for i in seqs]
+    @property
+    def _seqs(self) -> dict:
+        return self._book.seqs()
 
-    def _need(self, n):
-        if n > self._n_free:
-            raise RuntimeError(f"out of cache pages: {n} needed, {self._n_free} of {self.n_pages} free")
+    @property
+    def _refs(self) -> np.ndarray:
+        """Sequences that hold each page."""
+        return self._book.refs()
 
-    def _take(self, n: int) -> np.ndarray:
-        """The ``n`` lowest free pages (there are as many)."""
-        ids = np.flatnonzero(self._refs[self._low:self._low + 4 * n + 256] == 0)
-        if len(ids) < n:
-            ids = np.flatnonzero(self._refs[self._low:] == 0)
-        ids = (ids[:n] + self._low).astype(np.int32)
-        if n:
-            self._refs[ids] = 1
-            self._n_free -= n
-            self._low = int(ids[-1]) + 1
-        return ids
-
-    def _give(self, pages: np.ndarray) -> None:
-        """A hold of each of these pages ends (a page named twice has two)."""
-        held = np.bincount(pages[pages >= 0])
-        refs = self._refs[:len(held)]
-        refs -= held.astype(np.int32)
-        freed = np.flatnonzero((refs == 0) & (held > 0))
-        if len(freed):
-            self._n_free += len(freed)
-            self._low = min(self._low, int(freed[0]))
-
-    def _copy(self, src, dst):
-        if not len(src):
+    def _copy(self, src: torch.Tensor, dst: torch.Tensor):
+        if not src.numel():
             return
         if self.device.type == "cuda":
-            ids = [torch.from_numpy(np.ascontiguousarray(x, np.int32)) for x in (src, dst)]
-            ext().kv_cache_copy_pages(self.k, self.v, self.k_scale, self.v_scale, *ids)
+            ext().kv_cache_copy_pages(self.k, self.v, self.k_scale, self.v_scale, src, dst)
         else:
             for t in (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale):
-                t[:, list(dst)] = t[:, list(src)]
+                t[:, dst.long()] = t[:, src.long()]
 
     def _not_capturing(self, what):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
@@ -306,37 +261,28 @@ class PagedKVCache:
 
     @property
     def free_pages(self) -> int:
-        return self._n_free
+        return self._book.free_pages
 
     @property
     def sequences(self) -> List[int]:
-        return list(self._seqs)
+        return list(self._book.seqs())
 
     def length(self, seq: int) -> int:
         """Committed tokens of a sequence (its next position), dropped ones counted."""
-        return self._get([seq])[0].length
+        return self._book.seq(seq).length
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
     def table(self, seqs: Sequence[int]) -> torch.Tensor:
         """Page ids of the sequences, int32 ``[n, max_pages_per_seq]`` (-1: none)."""
-        rows = np.full((len(seqs), self.max_pages_per_seq), -1, np.int32)
-        for i, s in enumerate(self._get(seqs)):
-            rows[i, :len(s.pages)] = s.pages
-        rows = torch.from_numpy(rows)
+        rows = self._book.table(list(seqs))
         return rows.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else rows
 
     # ------------------------------------------------------------------ sequences
     def add(self, n: int = 1) -> List[int]:
         """``n`` new empty sequences; returns their ids."""
-        if n < 0:
-            raise ValueError("n must not be negative")
-        ids = list(range(self._next, self._next + n))
-        self._next += n
-        for i in ids:
-            self._seqs[i] = _Seq(np.empty(0, np.int32))
-        return ids
+        return self._book.add(n)
 
     def begin(self, seqs: Sequence[int], n_new: Union[int, Sequence[int]], max_tokens: Optional[int] = None,
               out: Optional[CacheStep] = None) -> CacheStep:
@@ -349,196 +295,73 @@ class PagedKVCache:
         stream, behind the calls that still read it), so that a graph captured with it runs
         on the new tables; its ``max_tokens`` must suffice."""
         self._not_capturing("begin")
-        states = self._get(seqs)
-        n_new = [int(n_new)] * len(states) if not isinstance(n_new, (list, tuple)) else [int(n) for n in n_new]
-        if len(n_new) != len(states) or any(n < 0 for n in n_new):
-            raise ValueError("n_new must be one number, or one for each sequence, none negative")
-        longest = max((s.length + n for s, n in zip(states, n_new)), default=0)
-        if longest > self.max_pages_per_seq * PAGE:
-            raise ValueError(f"{longest} tokens do not fit a sequence's {self.max_pages_per_seq} pages")
+        seqs = list(seqs)
+        n_new = [int(n) for n in n_new] if isinstance(n_new, (list, tuple)) else [int(n_new)] * len(seqs)
         if out is not None:
-            if out.cache is not self or len(out.seqs) != len(states):
+            if out.cache is not self or len(out.seqs) != len(seqs):
                 raise ValueError("out is a step of another cache or number of sequences")
             max_tokens = out.max_tokens if max_tokens is None else max_tokens
             if max_tokens != out.max_tokens:
                 raise ValueError("out keeps its max_tokens")
+        if max_tokens is not None and max_tokens < 0:
+            raise ValueError("max_tokens must not be negative")
+        rows, src, dst, longest, trim, versions = self._book.begin(seqs, n_new, -1 if max_tokens is None else int(max_tokens))
         max_tokens = longest if max_tokens is None else int(max_tokens)
-        if max_tokens < longest:
-            raise ValueError(f"sequences of {longest} tokens in a step for {max_tokens}")
-        # Pages to take: behind the present ones, and for shared pages that get new tokens (of
-        # a page shared within this call the last one to write keeps it). Pages behind the
-        # new tokens are the room of an abandoned step.
-        refs = self._refs
-        need, spare, shared, todo = 0, 0, {}, []
-        for i, (s, n) in enumerate(zip(states, n_new)):
-            have, upto = len(s.pages), (s.length + n + PAGE - 1) // PAGE
-            if upto > have:
-                need += upto - have
-                todo.append(i)
-            elif upto < have:
-                spare += have - upto
-            for j in range(s.length // PAGE, min(upto, have)) if n else ():
-                p = int(s.pages[j])
-                if refs[p] > 1:
-                    shared[p] = shared.get(p, int(refs[p])) - 1
-                    if shared[p] > 0:
-                        need += 1
-                        todo.append(i)
-        self._need(need - spare)
-        self._epoch += 1
-        if spare:
-            for s, n in zip(states, n_new):
-                upto = _pages(s.length + n)
-                if len(s.pages) > upto:
-                    self._give(s.pages[upto:])
-                    s.pages = s.pages[:upto]
-        if todo:
-            fresh = iter(self._take(need).tolist())
-            src, dst = [], []
-            for i in dict.fromkeys(todo):
-                s = states[i]
-                have, upto = len(s.pages), _pages(s.length + n_new[i])
-                for j in range(s.length // PAGE, min(upto, have)) if shared and n_new[i] else ():
-                    p = int(s.pages[j])
-                    if refs[p] > 1:
-                        s.pages = s.pages.copy()
-                        s.pages[j] = to = next(fresh)
-                        if j * PAGE < s.length:
-                            src.append(p)
-                            dst.append(to)
-                        refs[p] -= 1
-                if upto > have:
-                    s.pages = np.append(s.pages, np.fromiter(fresh, np.int32, upto - have))
-            self._copy(src, dst)
-        rows = np.full((len(states), _INFO + self.max_pages_per_seq), -1, np.int32)
-        trim, heads = -1, []
-        for i, (s, n) in enumerate(zip(states, n_new)):
-            s.version += 1
-            if s.first > s.sinks:
-                heads.append((s.length + n, n, s.first, s.sinks))
-                trim = s.sinks if trim in (-1, s.sinks) else -2
-            else:
-                heads.append((s.length + n, n, 0, -1))
-            rows[i, _INFO:_INFO + len(s.pages)] = s.pages
-        if heads:
-            rows[:, :_INFO] = heads
-        rows, handle = torch.from_numpy(rows), None
+        self._copy(src, dst)
+        handle = None
         if self.device.type == "cuda":
             handle = ext().kv_step_begin(self.k, self.v, self.k_scale, self.v_scale, rows, max_tokens, max(n_new, default=0),
                                          trim, None if out is None else out._h)
         if out is None:
-            return CacheStep(self, list(seqs), n_new, max_tokens, rows, handle)
-        out.__init__(self, list(seqs), n_new, max_tokens, rows, handle)
+            return CacheStep(self, seqs, n_new, versions, max_tokens, rows, handle)
+        out.__init__(self, seqs, n_new, versions, max_tokens, rows, handle)
         return out
 
     def fork(self, seqs: Sequence[int], copies: int = 1) -> List[int]:
         """``copies`` new sequences from each of ``seqs`` (all copies of the first, then of the
         next), sharing its pages; an unfinished page is copied when one of them is written."""
-        states = self._get(seqs)
-        if copies < 0:
-            raise ValueError("copies must not be negative")
-        self._epoch += 1
-        out = self.add(copies * len(states))
-        for i, s in enumerate(states):
-            s.version += 1
-            pages = s.pages[:_pages(s.length)].copy()
-            self._refs[pages[pages >= 0] if s.trimmed else pages] += copies
-            for k in out[i * copies:(i + 1) * copies]:
-                # a sequence's page list is replaced, never written in place
-                self._seqs[k] = _Seq(pages, s.length, s.first, s.sinks)
-        return out
+        return self._book.fork(list(seqs), copies)
 
     def copy(self, seqs: Sequence[int]) -> List[int]:
         """New sequences with the committed tokens of ``seqs`` in pages of their own."""
         self._not_capturing("copy")
-        states = self._get(seqs)
-        kept = [s.pages[:_pages(s.length)] for s in states]
-        src = np.concatenate([p[p >= 0] for p in kept]) if kept else np.empty(0, np.int32)
-        self._need(len(src))
-        dst = self._take(len(src))
-        out, at = self.add(len(states)), 0
-        for i, s, p in zip(out, states, kept):
-            pages, n = p.copy(), int((p >= 0).sum())
-            pages[p >= 0] = dst[at:at + n]
-            at += n
-            self._seqs[i] = _Seq(pages, s.length, s.first, s.sinks)
+        out, src, dst = self._book.copy(list(seqs))
         self._copy(src, dst)
         return out
 
     def free(self, seqs: Sequence[int]) -> None:
         """Drop sequences; pages that no other sequence shares become free."""
-        states = self._get(seqs)
-        if not states:
-            return
-        self._epoch += 1
-        self._give(np.concatenate([s.pages for s in states]))
-        for i, s in zip(seqs, states):
-            s.version += 1
-            del self._seqs[i]
+        self._book.free(list(seqs))
 
     def trim(self, seqs: Sequence[int], keep: int, sinks: int = 0) -> None:
         """Drop each sequence's tokens but its first ``sinks`` and its newest ``keep`` ones:
         no query sees them any more, and pages that held nothing else become free."""
-        states = self._get(seqs)
-        if keep < 0 or sinks < 0:
-            raise ValueError("keep and sinks must not be negative")
-        if any(s.trimmed and s.sinks != sinks for s in states):
-            raise ValueError("a sequence that was trimmed keeps its number of sinks")
-        self._epoch += 1
-        for s in states:
-            first = max(s.first, s.length - keep)
-            if first <= sinks:
-                continue
-            s.first, s.sinks = first, sinks
-            lo, hi = _pages(sinks), min(first // PAGE, len(s.pages))
-            if hi > lo:
-                self._give(s.pages[lo:hi])
-                s.pages = s.pages.copy()
-                s.pages[lo:hi] = -1
-            s.version += 1
+        self._book.trim(list(seqs), keep, sinks)
 
     def compact(self) -> int:
         """Move the pages in use to the front of the pool; returns how many there are."""
         self._not_capturing("compact")
-        used = self._refs > 0
-        n = self.n_pages - self._n_free
-        src, dst = np.flatnonzero(used[n:]) + n, np.flatnonzero(~used[:n])
-        if len(src):
-            self._epoch += 1
-            self._copy(src, dst)
-            to = np.arange(self.n_pages, dtype=np.int32)
-            to[src] = dst
-            for s in self._seqs.values():
-                moved = np.where(s.pages >= 0, to[s.pages], -1).astype(np.int32)
-                if not np.array_equal(moved, s.pages):
-                    s.pages = moved
-                    s.version += 1
-            self._refs[dst] = self._refs[src]
-            self._refs[src] = 0
-            self._low = n
-        return n
+        self._copy(*self._book.compact())
+        return self.n_pages - self.free_pages
 
     def resize(self, n_pages: int) -> None:
         """Change the pool to ``n_pages`` pages (compacted first when it shrinks below a page
         in use); the pages in use keep their contents. The pool's tensors are new ones."""
         self._not_capturing("resize")
-        used = self.n_pages - self._n_free
+        used = self.n_pages - self.free_pages
         if n_pages < max(used, 1):
             raise ValueError(f"{used} pages are in use, {n_pages} asked for")
-        if self._refs[n_pages:].any():
+        if self._book.used_end() > n_pages:
             self.compact()
         old, n = (self.k, self.v, self.k_scale, self.v_scale), min(n_pages, self.n_pages)
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
         for a, b in zip((self.k, self.v, self.k_scale, self.v_scale), old):
             a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
             a[:, :n].copy_(b[:, :n])
-        self._refs = np.concatenate([self._refs[:n], np.zeros(n_pages - n, np.int32)])
-        self._n_free, self._low, self.n_pages = n_pages - used, 0, n_pages
-        self._epoch += 1
-        for s in self._seqs.values():
-            s.version += 1
+        self._book.resize(n_pages)
+        self.n_pages = n_pages
 
-    def _values(self, layer, s: _Seq, n: int):
+    def _values(self, layer, s, n: int):
         ids = torch.from_numpy(np.maximum(s.pages[:_pages(n)], 0)).long().to(self.device)
         out = []
         for codes, scales, last in ((self.k, self.k_scale, False), (self.v, self.v_scale, True)):
@@ -554,5 +377,5 @@ class PagedKVCache:
         """The committed keys and values of a sequence as they are held, fp32
         ``[length, n_heads, 64]`` each (dropped tokens zero)."""
         self._layer(layer)
-        s = self._get([seq])[0]
+        s = self._book.seq(seq)
         return tuple(self._values(layer, s, s.length))

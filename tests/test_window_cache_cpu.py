@@ -1,5 +1,6 @@
 """Windowed attention, the 8-bit paged cache and rollouts over it, in their PyTorch form."""
 import math
+import random
 
 import pytest
 import torch
@@ -214,6 +215,67 @@ def test_trim_frees_pages_and_hides_tokens():
     for call in (lambda: c.trim([s], 50, 11), lambda: step.attend(0, q, causal="token", window=20, sinks=4)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_bookkeeping_keeps_every_sequence(seed):
+    """Random calls against plain lists of tokens (whole numbers up to 15, exact in 8 bits);
+    every page is held by as many sequences as the count says, a free one by none."""
+    rng = random.Random(seed)
+    c = PagedKVCache(1, 1, 60, device="cpu", max_pages_per_seq=12)
+    held = {}  # sequence: (tokens, first, sinks)
+
+    def check():
+        counts = [0] * c.n_pages
+        for i, (tokens, first, sinks) in held.items():
+            assert c.length(i) == len(tokens)
+            k, v = c.read(0, i)
+            want = torch.tensor(tokens, dtype=torch.float32)
+            if first > sinks:
+                want[sinks:first] = 0
+            assert torch.equal(k[:, 0, 0], want) and torch.equal(v[:, 0, 63], -want)
+            s = c._seqs[i]
+            for p in s.pages:
+                if p >= 0:
+                    counts[p] += 1
+        assert c._refs.tolist() == counts and c.free_pages == counts.count(0) and c.sequences == sorted(held)
+
+    for _ in range(150):
+        some = rng.sample(sorted(held), rng.randint(0, min(3, len(held))))
+        what = rng.choice(["add", "step", "step", "step", "step", "fork", "copy", "free", "trim", "compact", "resize"])
+        try:
+            if what == "add" and len(held) < 6:
+                held.update((i, ([], 0, 0)) for i in c.add(rng.randint(1, 2)))
+            elif what == "step":
+                new = [rng.choice([0, 1, 1, 5, 64, 130]) for _ in some]
+                step = c.begin(some, new)
+                x = torch.zeros(len(some), max(new, default=0), 1, 64)
+                for r, n in enumerate(new):
+                    x[r, :n] = torch.randint(1, 16, (n, 1, 1)).float()
+                step.write(0, x, -x)
+                if rng.random() < 0.7:
+                    step.commit()
+                    held.update((i, (held[i][0] + x[r, :n, 0, 0].int().tolist(), *held[i][1:])) for r, (i, n) in enumerate(zip(some, new)))
+            elif what == "fork" and len(held) < 8:
+                held.update(zip(c.fork(some, 2), [held[i] for i in some for _ in "12"]))
+            elif what == "copy" and len(held) < 8:
+                held.update(zip(c.copy(some), [held[i] for i in some]))
+            elif what == "free":
+                c.free(some)
+                for i in some:
+                    del held[i]
+            elif what == "trim":
+                c.trim(some, keep := rng.choice([0, 30, 100, 200]), sinks := rng.choice([0, 10]))
+                held.update((i, (t, f, sinks) if (f := max(first, len(t) - keep)) > sinks else (t, first, old))
+                            for i, (t, first, old) in [(i, held[i]) for i in some])
+            elif what == "compact":
+                assert c.compact() == c.n_pages - c.free_pages
+                assert not c._refs[c.n_pages - c.free_pages:].any()
+            elif what == "resize":
+                c.resize(rng.choice([50, 60, 70]))
+        except (RuntimeError, ValueError):  # no room, or other sinks than before: nothing has changed
+            pass
+        check()
 
 
 def test_cache_refusals_change_nothing():
