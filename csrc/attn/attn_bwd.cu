@@ -30,6 +30,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <stdexcept>
 
 #include "../common/ptx.cuh"
@@ -79,7 +80,11 @@ __device__ __forceinline__ int first_query_seeing(const AttnArgs& a, int k) {
   } while (0)
 
 // WIN: the windowed mode (any number of queries and keys, strided heads), instantiated
-// apart so that the other masks' code is unchanged.
+// apart so that the other masks' code is unchanged. 2 x 12 heads of 16 frames of 512 tokens,
+// window of 4 frames and 1 sink frame: 441 us (639 TFLOP/s). Bound by the passes over S and dP
+// between the products (TMEM loads, exponentials, dS, its stores). The longest CTAs first
+// (the sinks' key tiles are seen by every query) took 520 us to 441, with delta already
+// scaled by attn_window_prepare; the MMA warp's converged walk 571 to 520.
 template <bool WIN>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -684,7 +689,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// delta[b,h,t] = sum over the head's 64 columns of dO * O (one warp per row)
+// delta[b,h,t] = sum over the head's 64 columns of dO * O (one warp per row), times `factor`.
+// o_rest: what O's rounding to bf16 left (the windowed mode keeps it: with O rounded, dq's error
+// was 1.50 times that of fp32 arithmetic rounded once, with its rest 1.44). `clear`: the
+// row's dQ accumulator becomes zero in the same pass (a fill of its own would cost another
+// launch and the row's index arithmetic). Bound by memory: 2 x 8192 rows of 12 heads, 20 us.
 __global__ void delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_rest, long ldo, int o_col,
                              const __nv_bfloat16* __restrict__ dout, long lddo, int do_col,
                              float* __restrict__ delta, int B, int H, int Tq, long rows_per_b,

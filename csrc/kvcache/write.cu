@@ -31,9 +31,12 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b) {
 
 constexpr int kVPitch = 80;  // bytes between channel rows of the value tile in shared memory
 
-// One CTA = one page of one (sequence, head); threads 0-127 keys, 128-255 values; two
-// threads a token, 32 channels each. The page's tokens (kept ones decoded, new ones read)
-// stay in registers between the maximum and the coding, so each byte moves once.
+// One CTA = one page of one (sequence, head): a block's scale needs its maximum before its
+// first code. Threads 0-127 keys, 128-255 values; two threads a token, 32 channels each. The
+// page's tokens (kept ones decoded, new ones read) stay in registers between the maximum and
+// the coding, so each byte moves once. Bound by latency: the loads of the table, of the page
+// and of the tokens depend on one another. One token of 64 streams of 12 heads takes
+// 6.6 us (its bytes 1.5 us at the copy rate), 2048 tokens of 4 streams 9.7 us (38 MB, 3.9 TB/s).
 __global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteArgs a, int* status) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int* row = a.step.rows + static_cast<long>(b) * a.step.ld;
@@ -152,7 +155,9 @@ struct PagePairs {
 };
 
 // blockIdx.x: the pair, y: the layer, z: keys or values. A page of one layer is heads * 4 KB
-// in one piece. The pairs travel as launch arguments: no copy to the device comes first.
+// in one piece. The pairs travel as launch arguments: no copy to the device comes first, and
+// no call waits for an earlier one's upload. Four loads in flight a thread. Bound by memory:
+// 256 pages of 12 heads and 12 layers (302 MB read, as much written) take 93 us, 6.5 TB/s.
 __global__ void __launch_bounds__(256)
     kv_copy_kernel(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int pages, int heads,
                    const __grid_constant__ PagePairs pairs) {

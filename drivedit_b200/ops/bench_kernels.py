@@ -356,6 +356,65 @@ def bench_kv_attn(iters: int = 20, small: bool = False):
                           "kv_gbs": round(kv_bytes / ms / 1e6, 1)}), flush=True)
 
 
+def bench_window_attn(iters: int = 20, small: bool = False):
+    """Windowed attention forward and backward at the DiT-B training shape (16 frames of 512
+    tokens, 12 heads; window of 4 frames and 1 sink frame), the floor of each from the visible
+    (query, key) pairs: 4 and 10 multiply-adds of 64 channels, 2 operations each."""
+    import math
+
+    from ._ext import ext
+
+    H, tpf, frames, window, sinks = 12, 512, 16, 4, 1
+    T = frames * tpf
+    pairs = tpf * tpf * sum(min(f + 1, window) + min(sinks, max(0, f + 1 - window)) for f in range(frames))
+    for B in ((1,) if small else (2, 8)):
+        qkv = (torch.randn(B, T, 3, H, 64, device="cuda") * 0.5).bfloat16()
+        do, dqkv = torch.randn(B, T, H, 64, device="cuda").bfloat16(), torch.empty_like(qkv)
+        mask = ("frame", tpf, window, sinks, 1.0 / math.sqrt(64))
+        o, lse, rest = ext().attn_window_fwd(*qkv.unbind(2), *mask)
+        fwd = _timeit(lambda: ext().attn_window_fwd(*qkv.unbind(2), *mask), iters)
+        bwd = _timeit(lambda: ext().attn_window_bwd(*qkv.unbind(2), o, rest, lse, do, *mask, *dqkv.unbind(2)), iters)
+        for name, ms, n in (("window_attn_fwd", fwd, 4), ("window_attn_bwd", bwd, 10)):
+            print(json.dumps({"kernel": name, "B": B, "T": T, "window": window, "sinks": sinks, "ms": round(ms, 4),
+                              "tflops": round(n * 64 * pairs * B * H / ms / 1e9, 1)}), flush=True)
+
+
+def bench_kv_cache(iters: int = 20, small: bool = False):
+    """The 8-bit paged cache, 12 heads: writing tokens, attention of one token of 32 streams
+    (the cached bytes are the work), attention of a 4-frame chunk over 36 frames and 4 sink
+    frames (the visible pairs are), copying pages."""
+    from .kv_cache import PagedKVCache
+
+    H, tpf = 12, 512
+
+    def case(name, B, length, n, **mask):
+        cache = PagedKVCache(1, H, B * (length + n + 63) // 64 + B, device="cuda")
+        step = cache.begin(cache.add(B), length)
+        kv = (torch.randn(B, length, H, 64, device="cuda") * 0.5).bfloat16()
+        step.write(0, kv, kv)
+        step.commit()
+        step = cache.begin(step.seqs, n)
+        new = (torch.randn(B, n, H, 64, device="cuda") * 0.5).bfloat16()
+        w = _timeit(lambda: step.write(0, new, new), iters)
+        a = _timeit(lambda: step.attend(0, new, **mask), iters)
+        seen, pairs = length + n, n * (length + n)
+        if mask.get("window"):
+            frame = lambda p: p // tpf  # noqa: E731
+            see = [min(frame(p) + 1, mask["window"]) + min(mask["sinks"], max(0, frame(p) + 1 - mask["window"])) for p in range(length, length + n)]
+            pairs = sum(see) * tpf
+        print(json.dumps({"kernel": "kv_cache_write", "case": name, "B": B, "tokens": n, "ms": round(w, 4)}), flush=True)
+        print(json.dumps({"kernel": "kv_cache_attend", "case": name, "B": B, "tokens": n, "cached": length, "ms": round(a, 4),
+                          "cache_gbs": round(B * H * seen * 128 / a / 1e6, 1), "tflops": round(4 * 64 * pairs * B * H / a / 1e9, 1)}), flush=True)
+
+    case("token", 8 if small else 32, 16384, 1, causal="token")
+    case("chunk", 1, 40 * tpf, 4 * tpf, causal="frame", tokens_per_frame=tpf, window=36, sinks=4)
+    cache = PagedKVCache(12, H, 512, device="cuda")
+    src, dst = torch.arange(256, dtype=torch.int32), torch.arange(256, 512, dtype=torch.int32)
+    ms = _timeit(lambda: cache._copy(src, dst), iters)
+    print(json.dumps({"kernel": "kv_cache_copy_pages", "pages": 256, "layers": 12, "ms": round(ms, 4),
+                      "gbs": round(2 * 256 * 12 * H * 8200 / ms / 1e6, 1)}), flush=True)
+
+
 def bench_moe_gemm(iters: int = 10, N: int = 32768, d: int = 1024, E: int = 64, k: int = 6,
                    F: int = 512, ns: int = 2, small: bool = False):
     """Grouped (MoE) SwiGLU and down GEMMs of one MoE-DiT-L layer on one GPU (random
@@ -558,7 +617,7 @@ def bench_optim(iters: int = 10, numel: int = 130_000_000, transport: str = "fus
 
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("what", nargs="*", default=["gemm"], help="gemm attn sla_attn sla norm conv3d ep optim")
+    p.add_argument("what", nargs="*", default=["gemm"], help="gemm attn window_attn kv_attn kv_cache sla_attn sla norm conv3d groupnorm moe_gemm ep optim")
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--small", action="store_true", help="small attention case (for ncu)")
     p.add_argument("--B", type=int, default=8, help="attention batch")
@@ -581,7 +640,7 @@ def main():
             bench_ep(args.iters, transport=args.transport)
         elif w == "optim":
             bench_optim(args.iters, transport=args.transport)
-        elif w in ("groupnorm", "kv_attn", "moe_gemm", "sla_attn"):
+        elif w in ("groupnorm", "kv_attn", "kv_cache", "moe_gemm", "sla_attn", "window_attn"):
             globals()[f"bench_{w}"](args.iters, small=args.small)
         else:
             globals()[f"bench_{w}"](args.iters)
