@@ -53,7 +53,9 @@ constexpr int OFF_VEC = OFF_DST + 4 * TILE;    // per stage: lse[128], delta[128
 constexpr int OFF_BAR = OFF_VEC + NS * 1024;
 // no alignment slack: the dynamic shared window of a CTA without static shared memory
 // starts 1024-byte aligned; the kernel checks this and reports a status code otherwise.
+constexpr int N_BARS = 1 + 2 * NS + 13;  // then the TMEM address and the abort flag
 constexpr int SMEM_BYTES = OFF_BAR + 256;
+static_assert(N_BARS * 8 + 8 <= 256, "barriers, TMEM address and abort flag");
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t C_S = 0, C_DP = 128, C_DV = 256, C_DK = 320, C_DQ = 384, C_PT = 448;
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* ds_free = s_full + 9;   // 2 buffers: dS^T buffer free again (dQ staging read)
   uint64_t* dq_staged = s_full + 11;  // the 4 dQ warps' rows are in shared memory
   uint64_t* pt_tfree = s_full + 12;   // P^T in TMEM consumed by the dV MMAs
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_staged + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + N_BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   if ((smem_u32(smem_raw) & 1023) != 0) {
     if (threadIdx.x == 0 && status) atomicCAS(status, 0, kStatusBadArgument);

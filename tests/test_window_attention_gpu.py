@@ -169,6 +169,22 @@ def test_hidden_queries_do_not_matter(q_off, kv_off, unit):
         assert torch.isfinite(a).all() and ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-5).all()
 
 
+@pytest.mark.parametrize("window", [0, 300])
+def test_equal_backward_passes_agree(window):
+    """Many launches over many CTAs: dK and dV are summed in a fixed order, so each pass gives
+    the same bits (a race for a barrier or for TMEM would not), and the status stays clean."""
+    from drivedit_b200.ops._ext import check_device_status
+    from drivedit_b200.ops.window_attention import window_attention
+    q, k, v = (_bits(2, 2048, 12, 64).requires_grad_(True) for _ in "qkv")
+    do = _bits(2, 2048, 12, 64)
+    o = window_attention(q, k, v, "token", window=window, sinks=64 if window else 0)
+    _, dk, dv = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+    for _ in range(300):
+        _, dk2, dv2 = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+        assert torch.equal(dk, dk2) and torch.equal(dv, dv2)
+    check_device_status()
+
+
 def test_gradient_against_differences():
     """Directional differences of the forward kernel's own output, in a direction along which
     it is smooth: bf16 inputs moved by whole steps."""
