@@ -1787,8 +1787,14 @@ std::vector<torch::Tensor> kv_step_attend(std::shared_ptr<KvStepHandle> hp, int6
   a.sinks = m.sinks;
   a.scale = static_cast<float>(m.scale);
   a.max_tokens = h.max_tokens;
+  const auto plan = ddb::kv_cache_attend_plan(a);
+  torch::Tensor part;  // the call's own: calls on other streams and captured graphs have theirs
+  if (plan.scratch) {
+    part = torch::empty({plan.scratch}, q.options().dtype(torch::kFloat32));
+    a.part = part.data_ptr<float>();
+  }
   kv_step_wait(h);
-  ddb::kv_cache_attend(a, stream());
+  ddb::kv_cache_attend(a, plan, stream());
   if (return_lse) return {o, lse};
   return {o};
 }

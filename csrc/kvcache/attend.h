@@ -19,15 +19,8 @@ inline int kv_seen_pages(const KvAttendArgs& a) {
   return static_cast<int>(((a.window > 0 && near < all ? near : all) + kKvPage - 1) / kKvPage);
 }
 
-// How a launch shares a row tile's pages, and how long it should take: measured times of a CTA's
-// start, merge and steps, times the waves of CTAs.
-struct KvPlan {
-  int ranks = 1;   // CTAs of a cluster
-  double us = 0.;
-};
-
 // attend_tiles.cu: blocks of 256 rows on the tensor cores' 128-row products
 KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev);
-void kv_attend_tiles_launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream);
+void kv_attend_tiles_launch(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream);
 
 }  // namespace ddb

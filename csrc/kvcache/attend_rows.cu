@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   const int warp = warp_id(), lane = lane_id();
   const int rg = warp % NT, pg = warp / NT;  // the warp's 8 rows, and its group
   const int g = lane >> 2, c = lane & 3;
-  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  const int ranks = a.ranks, rank = blockIdx.x % ranks;
   int item = blockIdx.x / ranks;
   const int tile = item % row_tiles;
   item /= row_tiles;
@@ -449,7 +449,7 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   const int tiles = (a.T * G + 8 * NT - 1) / (8 * NT);
   const long ctas = static_cast<long>(a.step.B) * a.pool.heads * tiles * ranks;
   if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
-  a.cluster = ranks;
+  a.ranks = ranks;
   // Stages: all that fit where an SM holds one CTA anyway (few rows of few sequences wait for
   // the copies' latency), fewer where more CTAs share it.
   const int stages = NT > 2 || ctas <= num_sms(dev) ? kMaxStages : NT == 2 ? 3 : 2;
@@ -472,6 +472,8 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
 // Rows beyond which only the 256-row blocks are tried: there each page is read by 8 row
 // tiles of the other kernel. (Its rows' division by multiplication is exact far beyond.)
 constexpr long kMaxRows = 256;
+// 8-row warps of a row tile
+int row_warps(long rows) { return rows <= 24 ? static_cast<int>(rows + 7) / 8 : 4; }
 
 }  // namespace
 
@@ -481,25 +483,30 @@ constexpr long kMaxRows = 256;
 // decides: 64 rows take 15 us against 17 at 48 heads of 1,000 visible tokens, 205 against
 // 196 at 512 of 3,000; 128 rows 28 against 18, 412 against 216; few and short sequences stay
 // with it longer.
-void kv_cache_attend(const KvAttendArgs& a, cudaStream_t stream) {
-  if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
+KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
+  if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return KvPlan{};
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
-  const int NT = rows <= 24 ? static_cast<int>(rows + 7) / 8 : 4;
-  const KvPlan few = rows <= kMaxRows ? rows_plan(a, NT, dev) : KvPlan{};
-  if (rows > 32) {
-    const KvPlan many = kv_attend_tiles_plan(a, dev);
-    if (rows > kMaxRows || many.us < few.us) {
-      kv_attend_tiles_launch(a, many.ranks, dev, stream);
-      return;
-    }
+  const KvPlan few = rows <= kMaxRows ? rows_plan(a, row_warps(rows), dev) : KvPlan{};
+  if (rows <= 32) return few;
+  const KvPlan many = kv_attend_tiles_plan(a, dev);
+  return rows > kMaxRows || many.us < few.us ? many : few;
+}
+
+void kv_cache_attend(const KvAttendArgs& a, const KvPlan& plan, cudaStream_t stream) {
+  if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (plan.blocks) {
+    kv_attend_tiles_launch(a, plan, dev, stream);
+    return;
   }
-  switch (NT) {
-    case 1: launch<1>(a, few.ranks, dev, stream); break;
-    case 2: launch<2>(a, few.ranks, dev, stream); break;
-    case 3: launch<3>(a, few.ranks, dev, stream); break;
-    default: launch<4>(a, few.ranks, dev, stream); break;
+  switch (row_warps(a.T * static_cast<long>(a.H / a.pool.heads))) {
+    case 1: launch<1>(a, plan.ranks, dev, stream); break;
+    case 2: launch<2>(a, plan.ranks, dev, stream); break;
+    case 3: launch<3>(a, plan.ranks, dev, stream); break;
+    default: launch<4>(a, plan.ranks, dev, stream); break;
   }
 }
 

@@ -14,13 +14,14 @@
 //   warps 8-15   softmax: one thread per row and tile, as in the bf16 kernel; it also
 //                brings Q to fp16, scaled by a power of two per row
 // P is rounded to fp16 (2^-11), finer than the bf16 kernel's P.
-// The CTAs that share a row block form a cluster and meet through distributed shared
-// memory: no scratch memory, no second launch.
+// The CTAs that share a row block form a cluster and meet through distributed shared memory,
+// in one launch; or, where the clusters' sizes would leave SMs idle, meet in scratch memory
+// that a second launch adds up (kv_attend_tiles_plan).
 // Bound by the softmax: 256 x 128 exponentials a step at 16 a clock and SM are 2048 clocks,
-// its matrix products 1072, and a step takes 2.4 us. While one row tile is in its exponentials
+// its matrix products 1072, and a step takes 1.75 us (3300 clocks). While one row tile is in its exponentials
 // the other loads scores, takes its maximum and stores weights (they take turns); the exponential
 // unit is busy half of the time. 2048 rows over 20,480 visible tokens of 12 heads (129 GFLOP):
-// 247 us, 0.52 PFLOP/s. Tried, and slower: the next scores loaded under the exponentials
+// 222 us, 0.58 PFLOP/s (248 us in one launch of clusters). Tried, and slower than 248: the next scores loaded under the exponentials
 // (266-320 us), two threads a row (304), four streams by row tile and page, one MMA warp (306)
 // or one each (300), waits that spin instead of suspending (258).
 #include <cuda_bf16.h>
@@ -58,6 +59,7 @@ constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
 static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
 constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
 constexpr float kRescaleLog2 = 8.f;
+constexpr long kPartFloats = kRows * 66;  // a CTA's result in scratch
 constexpr int kHandOver = 3;  // quarters of a row's exponentials after which the other tile may begin
 
 // kind::f16 with fp16 A and B, fp32 D, both K-major
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* ref_bits = reinterpret_cast<int*>(smem + OFF_MISC + 8);  // largest key, value scale
 
   const int warp = warp_id(), lane = lane_id();
-  const int ranks = a.cluster, rank = blockIdx.x % ranks;
+  const int ranks = a.ranks, rank = blockIdx.x % ranks;
   int item = blockIdx.x / ranks;
   const int tile = row_tiles - 1 - item % row_tiles;  // long (late) tiles first
   item /= row_tiles;
@@ -570,7 +572,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
     if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores
-    if (ranks > 1) {
+    if (a.part) {
+      // 256 rows of 64 channels, then their (maximum, sum), for kv_tiles_merge
+      float* part = a.part + blockIdx.x * kPartFloats;
+      if (r < a.T * G) {
+        float* o = part + (t * 128 + lr) * 64;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          *reinterpret_cast<float4*>(o + 4 * c) = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
+        *reinterpret_cast<float2*>(part + kRows * 64 + (t * 128 + lr) * 2) = make_float2(r < rows ? m : -INFINITY, l);
+      }
+    } else if (ranks > 1) {
       if (done) {  // not while something may still read the operand tiles
         const uint32_t dst = smem_u32(smem + OFF_RES) + (t * 128 + lr) * 256;
 #pragma unroll
@@ -599,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (ranks > 1) {
+  if (ranks > 1 && !a.part) {
     // ---- each CTA of the cluster adds up its share of the rows, in rank order; 16 threads a
     // row, 4 channels each
     cluster_sync_all();
@@ -633,6 +645,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Adds up the CTAs' results of each row, in rank order; 16 threads a row, 4 channels each.
+__global__ void __launch_bounds__(256) kv_tiles_merge(const KvAttendArgs a, int row_tiles) {
+  const int G = a.H / a.pool.heads;
+  const int lr = (blockIdx.x % (kRows / 16)) * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  int item = blockIdx.x / (kRows / 16);
+  const float* part = a.part + static_cast<long>(item) * a.ranks * kPartFloats;
+  const int r = (item % row_tiles) * kRows + lr;
+  item /= row_tiles;
+  const int kh = item % a.pool.heads, b = item / a.pool.heads;
+  if (r >= a.T * G) return;
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < a.ranks; ++k) top = fmaxf(top, part[k * kPartFloats + kRows * 64 + lr * 2]);
+  if (top != -INFINITY)
+    for (int k = 0; k < a.ranks; ++k) {
+      const float2 x = *reinterpret_cast<const float2*>(part + k * kPartFloats + kRows * 64 + lr * 2);
+      const float4 y = *reinterpret_cast<const float4*>(part + k * kPartFloats + lr * 64 + c * 4);
+      const float w = exp2f(x.x - top);
+      sum += w * x.y;
+      v.x += w * y.x;
+      v.y += w * y.y;
+      v.z += w * y.z;
+      v.w += w * y.w;
+    }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int tok = r / G, h = kh * G + r % G;
+  const long at = (static_cast<long>(b) * a.T + tok) * a.H + h;
+  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64 + c * 4) =
+      make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+  if (a.lse && c == 0)
+    a.lse[(static_cast<long>(b) * a.H + h) * a.T + tok] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+}
+
 }  // namespace
 
 namespace {
@@ -659,17 +704,21 @@ cudaLaunchConfig_t config(int ranks, cudaLaunchAttribute* attr) {
 }
 }  // namespace
 
-// The cluster size with the smallest estimate. How many clusters of a size run at once is the
-// device's to say: of 3 CTAs only 45 do on 148 SMs (the GPCs' SMs are no multiple), so 96 of
-// them take three waves, not two. A CTA's start and merge measured 7 us, a step (128 keys)
-// 1.7 us with one row tile and 2.4 us with two: 512 CTAs of 24 steps (4 waves) take
-// 190 / 254 us, 96 of 20 steps (one wave) 40 / 51 us.
+// The way with the smallest estimate. How many clusters of a size run at once is the device's to
+// say: of 3 CTAs only 45 do on 148 SMs (the GPCs' SMs are no multiple), so 96 of them take
+// three waves; apart, meeting in scratch, two. Measured, as clusters and apart: 96 blocks of
+// 160 steps 248 and 222 us, 48 of 40 61 and 50, 49 of 33 54 and 42. A CTA's start and merge
+// take about 15 us, a step (128 keys) 1.3 us with one row tile and 1.75 us with two (512 CTAs
+// of 24 steps, 4 waves: 190 / 254 us; 96 of 20 steps, one wave: 40 / 51 us); the second
+// launch 4 us and 0.015 us a CTA (288 CTAs: 7 us).
 KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev) {
   raise_limit(dev);
   static std::atomic<int> fits[64][9];
   const int pairs = (kv_seen_pages(a) + 1) / 2;
-  const double step = a.T * static_cast<long>(a.H / a.pool.heads) > 128 ? 2.4 : 1.7;
+  const double step = a.T * static_cast<long>(a.H / a.pool.heads) > 128 ? 1.75 : 1.3;
+  const long items = row_items(a);
   KvPlan best;
+  best.blocks = true;
   for (int s = 1; s <= 8 && (s == 1 || pairs >= 2 * s); ++s) {
     int slots = s == 1 ? num_sms(dev) : fits[dev & 63][s].load();
     if (slots == 0) {
@@ -679,24 +728,35 @@ KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev) {
       slots = std::max(slots, 1);
       fits[dev & 63][s].store(slots);
     }
-    const double us = static_cast<double>((row_items(a) + slots - 1) / slots) * (7. + step * ((pairs + s - 1) / s));
-    if (s == 1 || us < best.us) best = KvPlan{s, us};
+    const double each = 15. + step * ((pairs + s - 1) / s);
+    const double us = static_cast<double>((items + slots - 1) / slots) * each;
+    if (s == 1 || us < best.us) best.ranks = s, best.scratch = 0, best.us = us;
+    if (s == 1 || items * s > 4L * num_sms(dev)) continue;  // more waves even out by themselves
+    const double apart = static_cast<double>((items * s + num_sms(dev) - 1) / num_sms(dev)) * each + 4. + items * s * 0.015;
+    if (apart < best.us) best.ranks = s, best.scratch = items * s * kPartFloats, best.us = apart;
   }
   return best;
 }
 
-void kv_attend_tiles_launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
+void kv_attend_tiles_launch(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream) {
   raise_limit(dev);
-  const long ctas = row_items(a) * ranks;
-  if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
-  a.cluster = ranks;
+  const long ctas = row_items(a) * plan.ranks;
+  if (ctas > 0x7fffffffL / (kRows / 16)) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  if (plan.scratch && !a.part) throw std::runtime_error("kv_cache_attend: no scratch");
+  a.ranks = plan.ranks;
+  if (!plan.scratch) a.part = nullptr;
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = config(ranks, attr);
+  cudaLaunchConfig_t cfg = config(plan.ranks, attr);
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.stream = stream;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  cfg.numAttrs = plan.ranks > 1 && !a.part ? 1 : 0;
   check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, row_blocks(a), device_status(dev)), "kv_attend_tiles launch");
   count_launch();
+  if (a.part) {
+    kv_tiles_merge<<<static_cast<unsigned>(row_items(a) * (kRows / 16)), 256, 0, stream>>>(a, row_blocks(a));
+    check_cuda(cudaGetLastError(), "kv_tiles_merge launch");
+    count_launch();
+  }
 }
 
 }  // namespace ddb

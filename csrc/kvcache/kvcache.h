@@ -70,12 +70,23 @@ struct KvAttendArgs {
   int sinks = 0;         // first tokens that stay visible beside the window
   float scale = 0.125f;
   int max_tokens = 0;    // no sequence is longer (sets the launch's shape only)
-  int cluster = 1;       // CTAs that share a row tile (set by the launch)
+  int ranks = 1;         // CTAs that share a row tile (set by the launch)
+  float* part = nullptr; // the plan's scratch, 16-byte aligned
 };
+
+// How a call is launched: the kernel, how many CTAs share a row tile's pages, and the scratch
+// that they meet in (0: distributed shared memory); with an estimate of its time.
+struct KvPlan {
+  bool blocks = false;   // 256-row blocks (attend_tiles.cu), not few rows (attend_rows.cu)
+  int ranks = 1;
+  long scratch = 0;      // floats
+  double us = 0.;
+};
+KvPlan kv_cache_attend_plan(const KvAttendArgs& a);
 
 // Attention of each sequence's own tokens (its newest) over its cached ones. Rows with no
 // visible key, and rows behind a sequence's own tokens, get zeros and lse = -inf.
-void kv_cache_attend(const KvAttendArgs& a, cudaStream_t s);
+void kv_cache_attend(const KvAttendArgs& a, const KvPlan& plan, cudaStream_t s);
 
 // Copies pages src[i] -> dst[i] in every layer (codes and scales). The dst are distinct and
 // none is a src.

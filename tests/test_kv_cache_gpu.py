@@ -189,6 +189,40 @@ def test_attend_matches_definition(case):
         assert not o[i, n:].any() and (lse[i, :, n:] == -math.inf).all()
 
 
+@pytest.mark.parametrize("lens,own,KH,G,window,sinks", [
+    ([4200, 4100, 3900, 64, 0, 4000, 4150], [130, 100, 1, 130, 77, 0, 64], 7, 1, 0, 0),
+    ([6000, 5000, 70, 6100, 5900, 0, 300], [120, 128, 128, 50, 3, 100, 0], 7, 2, 4000, 100),
+])
+def test_row_blocks_that_meet_in_scratch(lens, own, KH, G, window, sinks):
+    """Numbers of row blocks at which clusters would leave SMs idle: the CTAs' results are added
+    up by a second launch, alone and replayed from a graph on another stream."""
+    from drivedit_b200.ops._ext import ext
+    c = _cache(1, KH, sum(-(-(a + b) // 64) for a, b in zip(lens, own)) + 3)
+    seqs = _fill(c, lens)
+    T = max(own)
+    step = c.begin(seqs, own)
+    step.write(0, *(_randn(len(lens), T, KH, 64) for _ in "kv"))
+    q = _randn(len(lens), T, KH * G, 64, scale=2.0)
+    call = lambda: step.attend(0, q, causal="token", window=window, sinks=sinks, return_lse=True)  # noqa: E731
+    before = ext().launch_count()
+    o, lse = call()
+    assert ext().launch_count() - before == 2
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o2, lse2 = call()
+    for _ in range(2):
+        o2.zero_(), lse2.zero_()
+        graph.replay()
+        call()
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    step.commit()
+    for i, (s, n) in enumerate(zip(seqs, own)):
+        kk, vv = c.read(0, s)
+        ref, mean, rlse, mag = _oracle(kk, vv, q[i, :n], n, "token", 1, window, sinks)
+        _check(o[i, :n], lse[i, :, :n], ref, mean, rlse, mag)
+        assert not o[i, n:].any() and (lse[i, :, n:] == -math.inf).all()
+
+
 @pytest.mark.parametrize("T", [1, 20, 300])
 def test_hidden_tokens_do_not_matter(T):
     """NaN, infinities' codes and huge values at tokens that no query sees, inside visible
