@@ -18,12 +18,12 @@
 // in one launch; or, where the clusters' sizes would leave SMs idle, meet in scratch memory
 // that a second launch adds up (kv_attend_tiles_plan).
 // Bound by the softmax: 256 x 128 exponentials a step at 16 a clock and SM are 2048 clocks,
-// its matrix products 1072, and a step takes 1.75 us (3300 clocks). While one row tile is in its exponentials
-// the other loads scores, takes its maximum and stores weights (they take turns); the exponential
-// unit is busy half of the time. 2048 rows over 20,480 visible tokens of 12 heads (129 GFLOP):
-// 222 us, 0.58 PFLOP/s (248 us in one launch of clusters). Tried, and slower than 248: the next scores loaded under the exponentials
-// (266-320 us), two threads a row (304), four streams by row tile and page, one MMA warp (306)
-// or one each (300), waits that spin instead of suspending (258).
+// its matrix products 1072, and a step takes 3300 (1.75 us). While one row tile is in its
+// exponentials the other loads scores, takes its maximum and stores weights (they take
+// turns). 2048 rows over 20,480 visible tokens of 12 heads (129 GFLOP): 222 us, 0.58 PFLOP/s
+// (248 us in one launch of clusters). Tried against those 248, and slower: the next scores
+// loaded under the exponentials (266-320 us), two threads a row (304), four streams by row tile
+// and page with one MMA warp (306) or one each (300), waits that spin (258).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
