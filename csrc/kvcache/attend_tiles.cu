@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(256) kv_tiles_merge(const KvAttendArgs a, int 
   const int lr = (blockIdx.x % (kRows / 16)) * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
   int item = blockIdx.x / (kRows / 16);
   const float* part = a.part + static_cast<long>(item) * a.ranks * kPartFloats;
-  const int r = (item % row_tiles) * kRows + lr;
+  const int r = (row_tiles - 1 - item % row_tiles) * kRows + lr;  // the other kernel's order
   item /= row_tiles;
   const int kh = item % a.pool.heads, b = item / a.pool.heads;
   if (r >= a.T * G) return;

@@ -192,6 +192,7 @@ def test_attend_matches_definition(case):
 @pytest.mark.parametrize("lens,own,KH,G,window,sinks", [
     ([4200, 4100, 3900, 64, 0, 4000, 4150], [130, 100, 1, 130, 77, 0, 64], 7, 1, 0, 0),
     ([6000, 5000, 70, 6100, 5900, 0, 300], [120, 128, 128, 50, 3, 100, 0], 7, 2, 4000, 100),
+    ([5000], [2048], 6, 1, 0, 0),  # several row blocks of a sequence
 ])
 def test_row_blocks_that_meet_in_scratch(lens, own, KH, G, window, sinks):
     """Numbers of row blocks at which clusters would leave SMs idle: the CTAs' results are added
