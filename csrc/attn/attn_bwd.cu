@@ -83,8 +83,11 @@ __device__ __forceinline__ int first_query_seeing(const AttnArgs& a, int k) {
 
 // WIN: the windowed mode (any number of queries and keys, strided heads), instantiated
 // apart so that the other masks' code is unchanged. 2 x 12 heads of 16 frames of 512 tokens,
-// window of 4 frames and 1 sink frame: 441 us (639 TFLOP/s). Bound by the passes over S and dP
-// between the products (TMEM loads, exponentials, dS, its stores). The longest CTAs first
+// window of 4 frames and 1 sink frame: 441 us (639 TFLOP/s). Bound by shared memory: a unit
+// moves 176 KB of MMA operands, 33 KB of Q, dO and their vectors, 32 KB of dS, 64 KB of dQ on its
+// way out and 32 KB of broadcast vectors, 2,700 clocks at 128 bytes, and takes about 3,300;
+// twice the softmax warps (467 us) and dQ's wait behind the other products (439) gain nothing.
+// A CTA's start and end cost some 6 us more, which nothing overlaps. The longest CTAs first
 // (the sinks' key tiles are seen by every query) took 520 us to 441, with delta already
 // scaled by attn_window_prepare; the MMA warp's converged walk 571 to 520.
 template <bool WIN>
