@@ -540,6 +540,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
+    // windowed mode: a row without a key has l == 0; a NaN among its scores stays one, in the
+    // merge too (a maximum of -inf there means no key)
+    if (WIN && m == -INFINITY && l != 0.f) m = 0.f;
     if (WIN && splits > 1) {
       // this CTA's unnormalised O, maximum and sum, over the K ring (every product is done)
       const uint32_t dst = smem_u32(smem + OFF_K) + r * 256;
@@ -560,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       a.lse_part[(static_cast<long>(split) * a.B * a.H + bh) * a.Tq + q_local] =
           l > 0.f ? m + __log2f(l) : -INFINITY;
     } else if (row_ok) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const bool none = WIN ? l == 0.f : !(l > 0.f);
+      const float inv = none ? 0.f : 1.f / l;
       __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) +
                             (b * a.q_rows_per_b + q_local) * a.ldo + a.o_col + h * 64;
 #pragma unroll
@@ -576,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           st_global_v4(rest + c, pack_rest(ov[c] * inv, ov[c + 1] * inv), pack_rest(ov[c + 2] * inv, ov[c + 3] * inv),
                        pack_rest(ov[c + 4] * inv, ov[c + 5] * inv), pack_rest(ov[c + 6] * inv, ov[c + 7] * inv));
       }
-      if (a.lse) a.lse[static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + q_local] = l > 0.f ? m + __log2f(l) : -INFINITY;
+      if (a.lse) a.lse[static_cast<long>(bh) * (WIN ? a.lse_ld : a.Tq) + q_local] = none ? -INFINITY : m + __log2f(l);
     }
   }
 
@@ -608,14 +612,14 @@ __global__ void __launch_bounds__(kThreads, 2)
           v.z += w * y.z;
           v.w += w * y.w;
         }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       __nv_bfloat16* orow = reinterpret_cast<__nv_bfloat16*>(a.o) + (b * a.q_rows_per_b + q) * a.ldo + h * 64 + c * 4;
       *reinterpret_cast<uint2*>(orow) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
       if (a.o_rest)
         *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o_rest) + (b * a.q_rows_per_b + q) * a.ldo + h * 64 + c * 4) =
             make_uint2(pack_rest(v.x * inv, v.y * inv), pack_rest(v.z * inv, v.w * inv));
       if (a.lse && c == 0)
-        a.lse[static_cast<long>(bh) * a.lse_ld + q] = sum > 0.f ? top + __log2f(sum) : -INFINITY;
+        a.lse[static_cast<long>(bh) * a.lse_ld + q] = sum == 0.f ? -INFINITY : top + __log2f(sum);
     }
     cluster_sync_all();  // no CTA leaves while another reads its results
   }
