@@ -11,8 +11,10 @@
 //   16-row operand, the 8-column one holds 8 query rows, so one generated token wastes
 //   little. e4m3 -> fp16 is exact, one instruction for two codes. Q is scaled by a power of
 //   two per row (largest element near 2^14), exact but for elements 2^-28 of the row's
-//   largest. P <= 1 in fp16 is rounded by at most 2^-11 of itself. A page's key scale
-//   multiplies its scores, its value scale its P V product, both in fp32.
+//   largest. P <= 1 is held as 2^15 P in fp16: rounded by at most 2^-11 of itself down to
+//   2^-29, by at most 2^-40 below, so that a long tail of small weights is in the product as
+//   it is in the sum. A page's key scale multiplies its scores, its value scale (and
+//   2^-15) its P V product, both in fp32.
 //   Reduced indexes are permuted so that a lane's operand bytes are contiguous: of a key
 //   row, lane c of a quad holds channels 16c..16c+15 (a word of 4 codes is one k-step of
 //   16), of a value channel tokens 16c..16c+15. Row r < 8 of key tile i is token
@@ -44,6 +46,7 @@ namespace {
 constexpr int kGroups = 4;
 constexpr int kMaxStages = 6;
 constexpr int kPageBytes = 8192;  // keys, then values
+constexpr float kHeadroom = 15.f;  // log2 of what a weight of 1 is in fp16 (largest: 2^16 less a step)
 constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
 // the CTA's result and its rows' (m, l) | barriers | page scales | flag | rings, later the
@@ -274,13 +277,14 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
       const float use = top == -INFINITY ? 0.f : top;
       alpha[u] = exp2f(m[u] - use);
       m[u] = top;
+      const float down = use - kHeadroom;
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float x = s[t][2 * k + u];
-          float w = exp2f(x * fu - use);
+          float w = exp2f(x * fu - down);
           if (!whole && x == -INFINITY) w = 0.f;  // a masked score, whatever the factor is
           p[t][2 * k + u] = w;
           sum += w;
@@ -300,6 +304,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
 #pragma unroll
       for (int k = 0; k < 4; ++k) keep[k] = kv_bytes(see >> (4 * k));
     }
+    const float vf = f.y * exp2f(-kHeadroom);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
         mma_f16(d, av, pf[k][0], pf[k][1]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[t][k] = o[t][k] * alpha[k & 1] + d[k] * f.y;
+      for (int k = 0; k < 4; ++k) o[t][k] = o[t][k] * alpha[k & 1] + d[k] * vf;
     }
     __syncwarp();  // every lane has read the stage
     if (NT > 1 && lane == 0) mbar_arrive(&empty[st]);
@@ -342,6 +347,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
   for (int u = 0; u < 2; ++u) {
 #pragma unroll
     for (int x = 4; x < 32; x *= 2) l[u] += __shfl_xor_sync(0xffffffffu, l[u], x);
+    l[u] *= exp2f(-kHeadroom);
     if (m[u] == -INFINITY && l[u] != 0.f) m[u] = 0.f;  // only NaN scores so far
   }
   __syncthreads();

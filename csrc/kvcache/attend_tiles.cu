@@ -13,7 +13,8 @@
 //                2^-33 of the largest); tokens that no row sees become zeros
 //   warps 8-15   softmax: one thread per row and tile, as in the bf16 kernel; it also
 //                brings Q to fp16, scaled by a power of two per row
-// P is rounded to fp16 (2^-11), finer than the bf16 kernel's P.
+// P <= 2^8 (the running maximum may lag by that) is held as 2^7 P in fp16: rounded by at most
+// 2^-11 of itself, finer than the bf16 kernel's P, or by 2^-32 where it is below 2^-21.
 // The CTAs that share a row block form a cluster and meet through distributed shared memory,
 // in one launch; or, where the clusters' sizes would leave SMs idle, meet in scratch memory
 // that a second launch adds up (kv_attend_tiles_plan).
@@ -59,6 +60,7 @@ constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
 static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
 constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
 constexpr float kRescaleLog2 = 8.f;
+constexpr float kHeadroom = 7.f;  // log2 of what a weight of 1 is in fp16; with the lag 2^15 at most
 constexpr long kPartFloats = kRows * 66;  // a CTA's result in scratch
 constexpr int kHandOver = 3;  // quarters of a row's exponentials after which the other tile may begin
 
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           alpha = exp2f(m - mx2);
           m = mx2;
         }
-        const float use = m == -INFINITY ? 0.f : m;
+        const float down = (m == -INFINITY ? 0.f : m) - kHeadroom;
         // P V of the last key tile is done: O may be rescaled and P overwritten
         if (j > 0) {
           if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) {
@@ -529,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pk[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float p0 = exp2f(sf[ch * 32 + c] * sl2 - use);
-            const float p1 = exp2f(sf[ch * 32 + c + 1] * sl2 - use);
+            const float p0 = exp2f(sf[ch * 32 + c] * sl2 - down);
+            const float p1 = exp2f(sf[ch * 32 + c + 1] * sl2 - down);
             sp[c & 7] += p0;
             sp[(c + 1) & 7] += p1;
             pk[c >> 1] = pack_half(p0, p1);
@@ -550,6 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // every MMA is done: O may be read, and the operand tiles overwritten
     float ov[64];
+    l *= exp2f(-kHeadroom);
+    const float up = v_ref * exp2f(-kHeadroom);
     const bool done = __all_sync(0xffffffffu, mbar_wait(drain, 0, abort_flag) && ok);
     if (done && active && n > 0) {
       tc_fence_after();
@@ -559,8 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_wait_ld();
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
-        ov[c] = __uint_as_float(x0[c]) * v_ref;
-        ov[32 + c] = __uint_as_float(x1[c]) * v_ref;
+        ov[c] = __uint_as_float(x0[c]) * up;
+        ov[32 + c] = __uint_as_float(x1[c]) * up;
       }
     } else {
 #pragma unroll

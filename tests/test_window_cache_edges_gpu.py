@@ -38,6 +38,70 @@ def test_rows_that_meet_nan_are_nan_however_the_keys_are_split(splits):
     assert torch.equal(o[0][~bad], want[0][~bad]) and torch.equal(lse[0].T[~bad], wl[0].T[~bad])
 
 
+# ------------------------------------------------------------------ paged cache
+def _cache(L=1, H=2, P=64, **kw):
+    from drivedit_b200.ops.kv_cache import PagedKVCache
+    return PagedKVCache(L, H, P, device="cuda", **kw)
+
+
+def _check_rows(c, seq, o, lse, q, window=0, sinks=0):
+    """Each row against 64 bits, its bound from the keys that it sees alone.
+
+    bf16 output: half a step, 2^-8 of the value. Weights in fp16: half a step, 2^-11 of each,
+    or half the smallest number, 2^-25, where 2^7 stands for a weight as large as the largest
+    (or for one whose product with its page's scale is); a weight that becomes zero is off by
+    itself. fp32 scores of 64 products, exponentials and sums: 2^-12 in all at score
+    magnitudes up to 2^6, in proportion above."""
+    n, G, st = q.shape[0], q.shape[1] // c.n_heads, c._seqs[seq]
+    S = st.length + n
+    k, v = (x.double().repeat_interleave(G, 1) for x in c._values(0, st, S))
+    vs = c.v_scale[0, torch.from_numpy(st.pages).long().cuda()].double().repeat_interleave(64, 0)[:S].repeat_interleave(G, 1)
+    q = q.double()
+    pos = torch.arange(S, device="cuda")
+    qp = torch.arange(S - n, S, device="cuda")[:, None]
+    seen = pos[None] <= qp
+    if window:
+        seen = seen & ((qp - pos < window) | (pos < sinks))
+    s = (torch.einsum("thd,shd->hts", q, k) * 0.125).masked_fill(~seen, -math.inf)
+    mag = (torch.einsum("thd,shd->hts", q.abs(), k.abs()) * 0.125).masked_fill(~seen, 0.0).amax(-1)   # [H, T]
+    rl = torch.logsumexp(s, -1)
+    p = torch.where(seen, torch.exp(s - rl[..., None]), 0.0)
+    ref = torch.einsum("hts,shd->thd", p, v)
+    mean = torch.einsum("hts,shd->thd", p, v.abs())
+    # least step of a weight, in units of its own: by the largest weight, or by weight times scale
+    step = torch.maximum(p.amax(-1, keepdim=True), (p * vs.T[:, None]).amax(-1, keepdim=True) / vs.T[:, None])
+    lost = torch.einsum("hts,shd->thd", torch.minimum(p, 2.0 ** -32 * step), v.abs())
+    rel = (2.0 ** -11 + 2.0 ** -12 * (mag.T * 2.0 ** -6).clamp(min=1.0))[..., None]
+    bound = 2.0 ** -8 * ref.abs() + rel * mean + lost + 1e-37
+    err = (o.double() - ref).abs()
+    assert torch.isfinite(o).all() and (err <= bound).all(), (float((err / bound).max()), (err / bound).amax((1, 2)).argmax().item())
+    lerr = (lse.double() - rl / math.log(2)).abs()
+    assert (lerr <= 1.45 * (mag * 2.0 ** -18 + 2.0 ** -19)).all(), float(lerr.max())
+
+
+@pytest.mark.parametrize("T", [1, 5, 200])
+@pytest.mark.parametrize("gap", [18.7, 12.0])
+def test_a_long_tail_of_small_weights_counts(T, gap):
+    """One key takes the weight, its value zero; what is left is 20,000 weights of 2^-27 (or
+    2^-17) each."""
+    c = _cache(1, 1, 330)
+    (s,) = c.add(1)
+    n = 20000
+    k, v = _randn(1, n, 1, 64, scale=0.01), _randn(1, n, 1, 64) + 2
+    k[..., 0] = 0
+    k[:, 0, :, 0] = gap
+    v[:, 0] = 0
+    step = c.begin([s], n)
+    step.write(0, k, v)
+    step.commit()
+    step = c.begin([s], T)
+    step.write(0, k[:, 1:T + 1], v[:, 1:T + 1])
+    q = _randn(1, T, 1, 64)
+    q[..., 0] = 8
+    o, lse = step.attend(0, q, causal="token", return_lse=True)
+    _check_rows(c, s, o[0], lse[0], q[0])
+
+
 def test_status_clean():
     from drivedit_b200.ops._ext import check_device_status
     torch.cuda.synchronize()
