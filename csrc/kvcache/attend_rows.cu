@@ -47,6 +47,9 @@ constexpr int kGroups = 4;
 constexpr int kMaxStages = 6;
 constexpr int kPageBytes = 8192;  // keys, then values
 constexpr float kHeadroom = 15.f;  // log2 of what a weight of 1 is in fp16 (largest: 2^16 less a step)
+// Scores (log2) from which the rounding of a maximum, 2^-24 of it, would move a weight by 2^(1/16)
+// and more: far beyond, a fused multiply-add against it would overflow.
+constexpr float kFar = 1048576.f;
 constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
 // the CTA's result and its rows' (m, l) | barriers | page scales | flag | rings, later the
@@ -273,18 +276,26 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float top = mx == -INFINITY ? m[u] : fmaxf(m[u], mx * fu);
+      const float top = mx == -INFINITY ? m[u] : fmaxf(m[u], __fmul_rn(mx, fu));
       const float use = top == -INFINITY ? 0.f : top;
       alpha[u] = exp2f(m[u] - use);
       m[u] = top;
-      const float down = use - kHeadroom;
+      float down = use - kHeadroom, by = fu;
+      if (fabsf(use) >= kFar) {  // products rounded as the maximum's was: none passes it
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) s[t][2 * k + u] = __fadd_rn(__fmul_rn(s[t][2 * k + u], fu), -use);
+        down = -kHeadroom;
+        by = 1.f;
+      }
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float x = s[t][2 * k + u];
-          float w = exp2f(x * fu - down);
+          float w = exp2f(x * by - down);
           if (!whole && x == -INFINITY) w = 0.f;  // a masked score, whatever the factor is
           p[t][2 * k + u] = w;
           sum += w;

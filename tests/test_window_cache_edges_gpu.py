@@ -79,6 +79,34 @@ def _check_rows(c, seq, o, lse, q, window=0, sinks=0):
     assert (lerr <= 1.45 * (mag * 2.0 ** -18 + 2.0 ** -19)).all(), float(lerr.max())
 
 
+def _prompt(c, T, change):
+    """A sequence of 100 tokens and ``T`` more, whose keys and values ``change`` has altered."""
+    (s,) = c.add(1)
+    k, v = _randn(1, 100 + T, c.n_heads, 64), _randn(1, 100 + T, c.n_heads, 64)
+    change(k, v)
+    step = c.begin([s], 100)
+    step.write(0, k[:, :100], v[:, :100])
+    step.commit()
+    step = c.begin([s], T)
+    step.write(0, k[:, 100:], v[:, 100:])
+    return s, step
+
+
+@pytest.mark.parametrize("T,G", [(3, 1), (28, 1), (7, 3)])
+@pytest.mark.parametrize("far", [2.0 ** e for e in (12, 20, 24, 30, 60)])
+def test_large_scores_few_rows(T, G, far):
+    """Scores past what fp32 tells apart: the largest one takes the weight, nothing overflows."""
+    c = _cache(1, 2, 32)
+
+    def change(k, v):
+        k[:, 64:] *= far
+    s, step = _prompt(c, T, change)
+    q = _randn(1, T, 2 * G, 64)
+    for window in (0, 50):
+        o, lse = step.attend(0, q, causal="token", window=window, return_lse=True)
+        _check_rows(c, s, o[0], lse[0], q[0], window)
+
+
 @pytest.mark.parametrize("T", [1, 5, 200])
 @pytest.mark.parametrize("gap", [18.7, 12.0])
 def test_a_long_tail_of_small_weights_counts(T, gap):
