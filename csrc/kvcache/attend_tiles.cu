@@ -7,12 +7,16 @@
 //   warp 0       bulk copies of the pages' codes (keys 4 KB, values 4 KB each), 3 stages
 //   warp 1       TMEM owner and MMA issuer: S = Q K^T (M 128, N 128, K 64) and
 //                O += P V (M 128, N 64, K 128; P from TMEM), per row tile
-//   warps 4-7    e4m3 -> fp16 into the swizzled operand tiles (3 stages of 16 KB each):
-//                exact but for the page's scale relative to the largest of the CTA's
-//                pages, a power of two (below 2^-14 of it fp16 is subnormal: an error of
-//                2^-33 of the largest); tokens that no row sees become zeros
+//   warps 4-7    e4m3 -> fp16 into the swizzled operand tiles (3 stages of 16 KB each),
+//                exactly; tokens that no row sees become zeros
 //   warps 8-15   softmax: one thread per row and tile, as in the bf16 kernel; it also
 //                brings Q to fp16, scaled by a power of two per row
+// Scales: a page's key scale multiplies its half of the scores, in fp32. Its value scale goes
+// into its weights, whose reference is the largest product of weight and scale that the row
+// itself has met: a page that a row does not see, or hardly weighs, takes nothing from the others.
+// (Scales in the converted codes, relative to the CTA's largest, took 222 us at the shape below
+// where this takes 225, but lost pages 2^25 below it; the exponents' constants made only after
+// the scores, 231.)
 // P <= 2^8 (the running maximum may lag by that) is held as 2^7 P in fp16: rounded by at most
 // 2^-11 of itself, finer than the bf16 kernel's P, or by 2^-32 where it is below 2^-21.
 // The CTAs that share a row block form a cluster and meet through distributed shared memory,
@@ -50,10 +54,14 @@ constexpr int OFF_K = OFF_Q + 2 * TILE;
 constexpr int OFF_V = OFF_K + NS * TILE;
 constexpr int OFF_RAW = OFF_V + NS * TILE;   // per stage: keys of both pages, values of both
 constexpr int OFF_BAR = OFF_RAW + NR * TILE;
-constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 10 + 1;
-constexpr int OFF_META = OFF_BAR + N_BARS * 8;
-constexpr int OFF_MISC = OFF_META + NR * 16;
-constexpr int SMEM_BYTES = OFF_MISC + 32;
+constexpr int NF = 8;  // stages of page factors: more than the softmax can lie behind (NR + NS)
+constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 10 + 1 + NF;
+constexpr int OFF_FACTOR = OFF_BAR + (N_BARS + 1) / 2 * 16;
+constexpr int OFF_META = OFF_FACTOR + NF * 16;
+constexpr int OFF_MISC = OFF_META + (NR + 1) / 2 * 8;
+static_assert(NF > NR + NS && (NF & (NF - 1)) == 0, "stages of page factors");
+constexpr int SMEM_BYTES = OFF_MISC + 8;
+static_assert(OFF_FACTOR % 16 == 0 && OFF_MISC % 8 == 0, "alignment");
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 constexpr int OFF_RES = OFF_K;                    // results, once K and V are no longer read
 constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
@@ -75,15 +83,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// two codes times a power of two
-__device__ __forceinline__ uint32_t half2_scaled(uint32_t two, __half2 mul) {
+__device__ __forceinline__ uint32_t half2_of(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&h), mul);
-  return *reinterpret_cast<const uint32_t*>(&r);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float inverse_power(float p) {  // 1 / 2^e, e in [-126, 126]
-  return __int_as_float((254 << 23) - __float_as_int(p));
-}
+__device__ __forceinline__ float log2_of_power(float p) { return static_cast<float>((__float_as_int(p) >> 23) - 127); }
 // every warp has its role's registers
 __device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
@@ -108,10 +112,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_done = s_full + 6;
   uint64_t* turn = s_full + 8;
   uint64_t* drain = s_full + 10;
-  float4* meta = reinterpret_cast<float4*>(smem + OFF_META);  // per stage: key, value factors of both pages
+  uint64_t* f_full = drain + 1;  // [NF]
+  int* meta = reinterpret_cast<int*>(smem + OFF_META);  // per stage: which of both pages are there
+  // key scales and log2 of the value scales of a pair, for the softmax
+  float4* factor = reinterpret_cast<float4*>(smem + OFF_FACTOR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
-  int* ref_bits = reinterpret_cast<int*>(smem + OFF_MISC + 8);  // largest key, value scale
 
   const int warp = warp_id(), lane = lane_id();
   const int ranks = a.ranks, rank = blockIdx.x % ranks;
@@ -158,8 +164,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&turn[t], 4);
     }
     mbar_init(drain, 1);
+    for (int s = 0; s < NF; ++s) mbar_init(&f_full[s], 1);
     *abort_flag = 0;
-    ref_bits[0] = ref_bits[1] = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -170,28 +176,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // the largest scales of this CTA's pages (positive floats order like their bits)
-  {
-    int mk = 0, mv = 0;
-    for (int i = 2 * j0 + threadIdx.x; i < min(pages.n, 2 * (j0 + n)); i += kThreads) {
-      const int id = row[kKvInfo + pages.at(i)];
-      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages)) {
-        const long block = static_cast<long>(id) * a.pool.heads + kh;
-        mk = max(mk, __float_as_int(a.pool.k_scale[block]));
-        mv = max(mv, __float_as_int(a.pool.v_scale[block]));
-      }
-    }
-    mk = __reduce_max_sync(0xffffffffu, mk);
-    mv = __reduce_max_sync(0xffffffffu, mv);
-    if (lane == 0 && mk) {
-      atomicMax(&ref_bits[0], mk);
-      atomicMax(&ref_bits[1], mv);
-    }
-  }
-  __syncthreads();
-  const float k_ref = ref_bits[0] ? __int_as_float(ref_bits[0]) : 1.f;
-  const float v_ref = ref_bits[1] ? __int_as_float(ref_bits[1]) : 1.f;
-
   // Registers by role: 56 + 72 + 2 * 192 = 512 = 4 * 128, the launch's own. All go back to 128
   // before the common end; none may before every role has its share (registers_split),
   // or a role with nothing to do would take back what the softmax warps still wait for.
@@ -214,9 +198,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ks = vs = 0.f;
           if (ids >= 0) {
             const long block = static_cast<long>(ids) * a.pool.heads + kh;
-            // zero stands for an absent page; below 2^-30 the product is zero in fp16 anyway
-            ks = fmaxf(a.pool.k_scale[block] * inverse_power(k_ref), 9.3132257e-10f);
-            vs = fmaxf(a.pool.v_scale[block] * inverse_power(v_ref), 9.3132257e-10f);
+            ks = a.pool.k_scale[block];
+            vs = a.pool.v_scale[block];
           }
         }
         const int l0 = 2 * (j & 15), s = j % NR;
@@ -227,7 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if (lane == 0) {
           uint8_t* dst = smem + OFF_RAW + s * TILE;
-          meta[s] = f;
+          // The softmax has read the factors NF pairs back: codes 3 pairs back have been converted,
+          // so the scores of the pair 6 back are made, and those before it read.
+          factor[j % NF] = make_float4(f.x, f.y, log2_of_power(f.z), log2_of_power(f.w));
+          mbar_arrive(&f_full[j % NF]);
+          meta[s] = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
           mbar_arrive_expect_tx(&raw_full[s], (id0 >= 0 ? 8192 : 0) + (id1 >= 0 ? 8192 : 0));
           const int id[2] = {id0, id1};
 #pragma unroll
@@ -323,17 +310,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x - 128;
     const int r = t >> 2, c = t & 3;  // row of 32, 16-byte piece of it; then rows r + 32 i
     bool ok = true;
-    auto convert = [&](const uint8_t* raw, uint32_t dst, float f0, float f1, const uint32_t (&keep)[2][4]) {
+    auto convert = [&](const uint8_t* raw, uint32_t dst, const uint32_t (&keep)[2][4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const __half2 mul = __float2half2_rn(i < 2 ? f0 : f1);
         uint4 w = *reinterpret_cast<const uint4*>(raw + t * 16 + i * 2048);
         const uint32_t ws[4] = {w.x & keep[i >> 1][0], w.y & keep[i >> 1][1], w.z & keep[i >> 1][2], w.w & keep[i >> 1][3]};
         uint32_t o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          o[2 * k] = half2_scaled(ws[k] & 0xffff, mul);
-          o[2 * k + 1] = half2_scaled(ws[k] >> 16, mul);
+          o[2 * k] = half2_of(ws[k] & 0xffff);
+          o[2 * k + 1] = half2_of(ws[k] >> 16);
         }
         const int R = r + 32 * i;
         const uint32_t d = dst + R * 128;
@@ -349,14 +335,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
         break;
       }
-      const float4 f = meta[sr];
+      const int there = meta[sr];
       const uint8_t* raw = smem + OFF_RAW + sr * TILE;
       uint32_t keep[2][4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p)  // an absent page (factor 0) holds whatever the stage held
+      for (int p = 0; p < 2; ++p)  // an absent page holds whatever the stage held
 #pragma unroll
-        for (int k = 0; k < 4; ++k) keep[p][k] = (p ? f.y : f.x) != 0.f ? ~0u : 0u;
-      convert(raw, smem_u32(smem + OFF_K + s * TILE), f.x, f.y, keep);
+        for (int k = 0; k < 4; ++k) keep[p][k] = there >> p & 1 ? ~0u : 0u;
+      convert(raw, smem_u32(smem + OFF_K + s * TILE), keep);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[s]);
@@ -376,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
         break;
       }
-      convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), f.z, f.w, keep);
+      convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -436,16 +422,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         st_shared_v4(dst + ((i ^ (lr & 7)) << 4), h[0], h[1], h[2], h[3]);
       }
-      // not zero: a masked score is -inf times it
-      sl2 = fmaxf(a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23) * k_ref, 1e-37f);
+      sl2 = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    float m = -INFINITY, l = 0.f;
+    // The weights of the sum are relative to 2^m; those of the product, times their page's value
+    // scale, to 2^(m + d).
+    float m = -INFINITY, d = 0.f, l = 0.f;
     bool ok = true;
     if (active) {
       for (int j = 0; j < n; ++j) {
+        if (!mbar_wait(&f_full[j % NF], (j / NF) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const float4 f = factor[j % NF];
+        // of the scores; not zero: a masked score is -inf times it
+        const float f0 = fmaxf(sl2 * f.x, 1e-37f), f1 = fmaxf(sl2 * f.y, 1e-37f);
+        // The page's exponents hold its value scale; its sum is brought back. A scale far below the
+        // reference counts as 2^-64 of it, so that no weight that counts in the sum underflows.
+        float e0, e1, down0, down1;
+        auto shifts = [&] {
+          const float use = (m == -INFINITY ? 0.f : m) - kHeadroom;
+          e0 = fmaxf(f.z - d, -64.f), e1 = fmaxf(f.w - d, -64.f);
+          down0 = use - e0, down1 = use - e1;
+        };
+        shifts();
         if (!mbar_wait(&s_full[t], j & 1, abort_flag)) {
           ok = false;
           break;
@@ -482,20 +485,35 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!(word[c >> 5] >> (c & 31) & 1)) sf[p * 64 + c] = -INFINITY;
           }
         }
-        float mp[8];
+        float mp[8];  // of the first page, of the second
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mp[i] = sf[i];
+        for (int i = 0; i < 8; ++i) mp[i] = sf[(i >> 2) * 64 + (i & 3)];
 #pragma unroll
-        for (int c = 8; c < 128; ++c) mp[c & 7] = fmaxf(mp[c & 7], sf[c]);
-        const float mx2 = sl2 * fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
-                                      fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
-        // the maximum moves only when a score passes it by 2^8: P <= 256, few rescales of O
-        float alpha = 1.f;
-        if (mx2 > m + kRescaleLog2) {
-          alpha = exp2f(m - mx2);
-          m = mx2;
+        for (int c = 4; c < 64; ++c) {
+          mp[c & 3] = fmaxf(mp[c & 3], sf[c]);
+          mp[4 + (c & 3)] = fmaxf(mp[4 + (c & 3)], sf[64 + c]);
         }
-        const float down = (m == -INFINITY ? 0.f : m) - kHeadroom;
+        const float m0 = f0 * fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), m1 = f1 * fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]));
+        // A reference moves only when something passes it by 2^8: P <= 256, few rescales of O,
+        // and what the exponentials need is known before the scores are.
+        float alpha = 1.f, alpha_o = 1.f;
+        const bool moves = __any_sync(0xffffffffu, fmaxf(fmaxf(m0, m1), fmaxf(m0 + e0, m1 + e1)) > m + kRescaleLog2);
+        if (moves) {
+          const float mx2 = fmaxf(m0, m1);
+          if (mx2 > m + kRescaleLog2) {
+            alpha = exp2f(m - mx2);
+            d += m - mx2;
+            m = mx2;
+          }
+          if (m != -INFINITY) {
+            const float top = fmaxf(m0 - m + f.z, m1 - m + f.w);
+            if (top > d + kRescaleLog2) {
+              alpha_o = exp2f(d - top);
+              d = top;
+            }
+          }
+          shifts();
+        }
         // P V of the last key tile is done: O may be rescaled and P overwritten
         if (j > 0) {
           if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) {
@@ -503,14 +521,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          if (moves && __any_sync(0xffffffffu, alpha_o != 1.f)) {
 #pragma unroll
             for (int c = 0; c < 64; c += 16) {
               uint32_t ov[16];
               tmem_ld16(trow + C_O + t * 64 + c, ov);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+              for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha_o);
               tmem_st16(trow + C_O + t * 64 + c, ov);
             }
           }
@@ -528,18 +546,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&turn[t]);
           }
+          const float by = ch < 2 ? f0 : f1, down = ch < 2 ? down0 : down1;
           uint32_t pk[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const float p0 = exp2f(sf[ch * 32 + c] * sl2 - down);
-            const float p1 = exp2f(sf[ch * 32 + c + 1] * sl2 - down);
+            const float p0 = exp2f(sf[ch * 32 + c] * by - down);
+            const float p1 = exp2f(sf[ch * 32 + c + 1] * by - down);
             sp[c & 7] += p0;
             sp[(c + 1) & 7] += p1;
             pk[c >> 1] = pack_half(p0, p1);
           }
           tmem_st16(trow + C_P + t * 64 + ch * 16, pk);
+          if (ch & 1) {
+            l = (ch == 1 ? l * alpha : l) +
+                (((sp[0] + sp[1]) + (sp[2] + sp[3])) + ((sp[4] + sp[5]) + (sp[6] + sp[7]))) * exp2f(ch == 1 ? -e0 : -e1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sp[i] = 0.f;
+          }
         }
-        l = l * alpha + (((sp[0] + sp[1]) + (sp[2] + sp[3])) + ((sp[4] + sp[5]) + (sp[6] + sp[7])));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -553,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // every MMA is done: O may be read, and the operand tiles overwritten
     float ov[64];
     l *= exp2f(-kHeadroom);
-    const float up = v_ref * exp2f(-kHeadroom);
+    const float up = exp2f(d - kHeadroom);
     const bool done = __all_sync(0xffffffffu, mbar_wait(drain, 0, abort_flag) && ok);
     if (done && active && n > 0) {
       tc_fence_after();

@@ -107,6 +107,42 @@ def test_large_scores_few_rows(T, G, far):
         _check_rows(c, s, o[0], lse[0], q[0], window)
 
 
+@pytest.mark.parametrize("what,far", [("k", 2.0 ** e) for e in (12, 17, -30)] + [("v", 2.0 ** e) for e in (12, 17, 26, 60, -30)])
+@pytest.mark.parametrize("T,G", [(28, 1), (200, 1), (300, 2), (700, 1)])
+def test_pages_that_a_row_does_not_see_do_not_touch_it(T, G, what, far):
+    """Pages of far larger (or smaller) keys or values, behind the causal edge of the earlier
+    rows and out of the window of the later ones: each row is as exact as its own keys allow."""
+    c = _cache(1, 2, 32)
+
+    def change(k, v):
+        x = k if what == "k" else v
+        for lo in (64, 192, 512):  # whole pages, of the first part and of the second
+            x[:, lo:lo + 64] *= far
+    s, step = _prompt(c, T, change)
+    q = _randn(1, T, 2 * G, 64)
+    for window, sinks in ((0, 0), (50, 3)):
+        o, lse = step.attend(0, q, causal="token", window=window, sinks=sinks, return_lse=True)
+        _check_rows(c, s, o[0], lse[0], q[0], window, sinks)
+
+
+@pytest.mark.parametrize("T,G", [(3, 1), (28, 1), (200, 1), (300, 2), (2000, 1)])
+@pytest.mark.parametrize("far,gap", [(2.0 ** 26, -40.0), (2.0 ** 40, -60.0), (0.0, 8.0), (2.0 ** -40, 9.0)])
+def test_weights_and_page_scales_far_apart(T, G, far, gap):
+    """A visible page whose values are far larger but hardly weigh, and one that takes most of
+    the weight but holds zeros (or next to nothing): the other pages' part is as exact."""
+    c = _cache(1, 2, 40)
+
+    def change(k, v):
+        k[..., 0] = 0
+        k[:, :64, :, 0] = gap   # times 8 * 0.125: the scores' distance in nats
+        v[:, :64] *= far
+    s, step = _prompt(c, T, change)
+    q = _randn(1, T, 2 * G, 64, scale=0.5)
+    q[..., 0] = 8
+    o, lse = step.attend(0, q, causal="token", return_lse=True)
+    _check_rows(c, s, o[0], lse[0], q[0])
+
+
 @pytest.mark.parametrize("T", [1, 5, 200])
 @pytest.mark.parametrize("gap", [18.7, 12.0])
 def test_a_long_tail_of_small_weights_counts(T, gap):
