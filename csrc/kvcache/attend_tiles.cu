@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "../common/ptx.cuh"
 #include "../common/tma.h"
@@ -60,7 +61,7 @@ constexpr int OFF_FACTOR = OFF_BAR + (N_BARS + 1) / 2 * 16;
 constexpr int OFF_META = OFF_FACTOR + NF * 16;
 constexpr int OFF_MISC = OFF_META + (NR + 1) / 2 * 8;
 static_assert(NF > NR + NS && (NF & (NF - 1)) == 0, "stages of page factors");
-constexpr int SMEM_BYTES = OFF_MISC + 8;
+constexpr int SMEM_BYTES = OFF_MISC + 16;
 static_assert(OFF_FACTOR % 16 == 0 && OFF_MISC % 8 == 0, "alignment");
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 constexpr int OFF_RES = OFF_K;                    // results, once K and V are no longer read
@@ -68,6 +69,9 @@ constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
 static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
 constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
 constexpr float kRescaleLog2 = 8.f;
+// Scores (log2) from which the rounding of a maximum, 2^-24 of it, would move a weight by 2^(1/16)
+// and more: far beyond, a fused multiply-add against it would overflow.
+constexpr float kFar = 1048576.f;
 constexpr float kHeadroom = 7.f;  // log2 of what a weight of 1 is in fp16; with the lag 2^15 at most
 constexpr long kPartFloats = kRows * 66;  // a CTA's result in scratch
 constexpr int kHandOver = 3;  // quarters of a row's exponentials after which the other tile may begin
@@ -118,6 +122,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   float4* factor = reinterpret_cast<float4*>(smem + OFF_FACTOR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+  // largest key scale of the CTA's pages (positive floats order like their bits)
+  int* k_most = reinterpret_cast<int*>(smem + OFF_MISC + 8);
 
   const int warp = warp_id(), lane = lane_id();
   const int ranks = a.ranks, rank = blockIdx.x % ranks;
@@ -166,6 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(drain, 1);
     for (int s = 0; s < NF; ++s) mbar_init(&f_full[s], 1);
     *abort_flag = 0;
+    *k_most = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -176,6 +183,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  {
+    int most = 0;
+    for (int i = 2 * j0 + threadIdx.x; i < min(pages.n, 2 * (j0 + n)); i += kThreads) {
+      const int id = row[kKvInfo + pages.at(i)];
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages))
+        most = max(most, __float_as_int(a.pool.k_scale[static_cast<long>(id) * a.pool.heads + kh]));
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && most) atomicMax(k_most, most);
+  }
+  __syncthreads();
+
   // Registers by role: 56 + 72 + 2 * 192 = 512 = 4 * 128, the launch's own. All go back to 128
   // before the common end; none may before every role has its share (registers_split),
   // or a role with nothing to do would take back what the softmax warps still wait for.
@@ -430,13 +449,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The weights of the sum are relative to 2^m; those of the product, times their page's value
     // scale, to 2^(m + d).
     float m = -INFINITY, d = 0.f, l = 0.f;
-    bool ok = true;
-    if (active) {
+    auto steps = [&](auto far_scores) -> bool {
+      constexpr bool kFarScores = decltype(far_scores)::value;
       for (int j = 0; j < n; ++j) {
-        if (!mbar_wait(&f_full[j % NF], (j / NF) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+        if (!mbar_wait(&f_full[j % NF], (j / NF) & 1, abort_flag)) return false;
         const float4 f = factor[j % NF];
         // of the scores; not zero: a masked score is -inf times it
         const float f0 = fmaxf(sl2 * f.x, 1e-37f), f1 = fmaxf(sl2 * f.y, 1e-37f);
@@ -449,10 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           down0 = use - e0, down1 = use - e1;
         };
         shifts();
-        if (!mbar_wait(&s_full[t], j & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+        if (!mbar_wait(&s_full[t], j & 1, abort_flag)) return false;
         tc_fence_after();
         float sf[128];
         {
@@ -493,14 +506,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           mp[c & 3] = fmaxf(mp[c & 3], sf[c]);
           mp[4 + (c & 3)] = fmaxf(mp[4 + (c & 3)], sf[64 + c]);
         }
-        const float m0 = f0 * fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])), m1 = f1 * fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7]));
+        const float m0 = __fmul_rn(f0, fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])));
+        const float m1 = __fmul_rn(f1, fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
         // A reference moves only when something passes it by 2^8: P <= 256, few rescales of O,
         // and what the exponentials need is known before the scores are.
         float alpha = 1.f, alpha_o = 1.f;
-        const bool moves = __any_sync(0xffffffffu, fmaxf(fmaxf(m0, m1), fmaxf(m0 + e0, m1 + e1)) > m + kRescaleLog2);
+        const float lag = kFarScores ? 0.f : kRescaleLog2;
+        const bool moves = __any_sync(0xffffffffu, fmaxf(fmaxf(m0, m1), fmaxf(m0 + e0, m1 + e1)) > m + lag);
         if (moves) {
           const float mx2 = fmaxf(m0, m1);
-          if (mx2 > m + kRescaleLog2) {
+          if (mx2 > m + lag) {
             alpha = exp2f(m - mx2);
             d += m - mx2;
             m = mx2;
@@ -514,12 +529,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           shifts();
         }
+        if (kFarScores) {  // products rounded as the maximum's was: none passes it
+          const float use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            sf[c] = __fadd_rn(__fmul_rn(sf[c], f0), -use);
+            sf[64 + c] = __fadd_rn(__fmul_rn(sf[64 + c], f1), -use);
+          }
+          down0 = -e0 - kHeadroom, down1 = -e1 - kHeadroom;
+        }
         // P V of the last key tile is done: O may be rescaled and P overwritten
         if (j > 0) {
-          if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
+          if (!mbar_wait(&o_done[t], (j - 1) & 1, abort_flag)) return false;
           tc_fence_after();
           if (moves && __any_sync(0xffffffffu, alpha_o != 1.f)) {
 #pragma unroll
@@ -535,10 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // The tiles take turns at their exponentials, which one tile alone issues near the
         // unit's full rate: in step, both would leave it idle during their loads and maxima.
-        if (n_t == 2 && (t == 1 || j > 0) && !mbar_wait(&turn[1 - t], (j - 1 + t) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+        if (n_t == 2 && (t == 1 || j > 0) && !mbar_wait(&turn[1 - t], (j - 1 + t) & 1, abort_flag)) return false;
         float sp[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {  // stored 32 columns at a time, to hold few registers
@@ -546,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&turn[t]);
           }
-          const float by = ch < 2 ? f0 : f1, down = ch < 2 ? down0 : down1;
+          const float by = kFarScores ? 1.f : ch < 2 ? f0 : f1, down = ch < 2 ? down0 : down1;
           uint32_t pk[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
@@ -569,7 +587,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
-    }
+      return true;
+    };
+    // Scores that may be far from zero go through a loop of their own (in the other one the test
+    // and the code for them took 229-235 us where this takes 227). |S| < 2^30: 64 products of
+    // numbers up to 2^15 and 448.
+    const bool far = __any_sync(0xffffffffu, sl2 * __int_as_float(*k_most) >= kFar * 0x1p-30f);
+    const bool ok = !active || (far ? steps(std::true_type{}) : steps(std::false_type{}));
     if (!ok) {
       if (lane == 0 && status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
       *abort_flag = 1;
