@@ -6,6 +6,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <limits>
 #include <map>
 #include <utility>
 #include <ATen/cuda/CUDAContext.h>
@@ -1672,9 +1673,22 @@ struct KvStepHandle {
   ddb::KvStep step;
   int64_t layers = 0, max_tokens = 0, most_new = 0;
   int64_t trim_sinks = -1;  // sinks of the trimmed sequences; -1: none is, -2: they differ
+  // what captured calls hold fast: the fewest rows of one, and the sinks that windowed ones name
+  // (-1: none, -2: they differ)
+  int64_t captured_rows = std::numeric_limits<int64_t>::max(), captured_sinks = -1;
   c10::optional<c10::cuda::CUDAStream> begun;
   at::cuda::CUDAEvent ready;
 };
+
+bool kv_capturing() { return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None; }
+
+// Whether a step may be refilled, asked before the cache's book changes: what its calls check
+// holds for those that are captured too.
+void kv_step_check_refill(const KvStepHandle& h, int64_t most_new, int64_t trim_sinks) {
+  TORCH_CHECK_VALUE(most_new <= h.captured_rows, "the step's captured calls hold ", h.captured_rows, " tokens, the refill ", most_new);
+  TORCH_CHECK_VALUE(trim_sinks == -1 || h.captured_sinks == -1 || (trim_sinks >= 0 && trim_sinks == h.captured_sinks),
+                    "a trimmed sequence keeps the first tokens it was trimmed to; the step's captured calls name others");
+}
 
 // rows: int32 [B, 4 + pages] in host memory; `out`: a step to refill in place
 std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
@@ -1720,7 +1734,7 @@ ddb::KvPool kv_layer(const KvStepHandle& h, int64_t layer) {
 
 void kv_step_wait(KvStepHandle& h) {
   const auto now = at::cuda::getCurrentCUDAStream();
-  if (now == *h.begun || at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return;
+  if (now == *h.begun || kv_capturing()) return;
   h.ready.block(now);
   h.rows.record_stream(now);
 }
@@ -1753,6 +1767,7 @@ void kv_step_write(std::shared_ptr<KvStepHandle> hp, int64_t layer, const torch:
   a.v = vv.data_ptr();
   a.v_sb = vv.stride(0); a.v_st = vv.stride(1); a.v_sh = vv.stride(2);
   a.T = kk.size(1);
+  if (kv_capturing()) h.captured_rows = std::min<int64_t>(h.captured_rows, a.T);
   kv_step_wait(h);
   ddb::kv_cache_write(a, stream());
 }
@@ -1793,6 +1808,10 @@ std::vector<torch::Tensor> kv_step_attend(std::shared_ptr<KvStepHandle> hp, int6
     part = torch::empty({plan.scratch}, q.options().dtype(torch::kFloat32));
     a.part = part.data_ptr<float>();
   }
+  if (kv_capturing()) {
+    h.captured_rows = std::min<int64_t>(h.captured_rows, a.T);
+    if (window > 0 || sinks > 0) h.captured_sinks = h.captured_sinks == -1 || h.captured_sinks == m.sinks ? m.sinks : -2;
+  }
   kv_step_wait(h);
   ddb::kv_cache_attend(a, plan, stream());
   if (return_lse) return {o, lse};
@@ -1809,8 +1828,9 @@ torch::Tensor host_ints(const std::vector<int32_t>& v) {
 py::tuple kv_book_begin(ddb::KvBook& book, const ddb::KvBook::Ids& seqs, const ddb::KvBook::Ids& n_new, int64_t max_tokens) {
   const auto copies = book.begin(seqs, n_new, max_tokens);
   auto rows = torch::empty({static_cast<int64_t>(seqs.size()), ddb::kKvInfo + book.max_pages()}, torch::kInt32);
-  const int64_t trim = book.rows(seqs, n_new, ddb::kKvInfo, rows.data_ptr<int>());
-  return py::make_tuple(rows, host_ints(copies.src), host_ints(copies.dst), book.longest(seqs, n_new), trim, book.versions(seqs));
+  book.rows(seqs, n_new, ddb::kKvInfo, rows.data_ptr<int>());
+  return py::make_tuple(rows, host_ints(copies.src), host_ints(copies.dst), book.longest(seqs, n_new), book.trim_sinks(seqs),
+                        book.versions(seqs));
 }
 torch::Tensor kv_book_table(const ddb::KvBook& book, const ddb::KvBook::Ids& seqs) {
   auto rows = torch::empty({static_cast<int64_t>(seqs.size()), book.max_pages()}, torch::kInt32);
@@ -1924,6 +1944,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("resize", &ddb::KvBook::resize)
       .def("table", &kv_book_table)
       .def("fresh", &ddb::KvBook::fresh)
+      .def("trim_sinks", &ddb::KvBook::trim_sinks)
       .def("seq", &ddb::KvBook::seq, py::return_value_policy::copy)
       .def("seqs", &ddb::KvBook::seqs, py::return_value_policy::copy)
       .def("refs", [](const ddb::KvBook& b) { return py::array_t<int32_t>(b.refs().size(), b.refs().data()); })
@@ -1931,6 +1952,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def_property_readonly("free_pages", &ddb::KvBook::free_pages)
       .def_readonly("epoch", &ddb::KvBook::epoch);
   m.def("kv_step_begin", &kv_step_begin, "a step's table on the device");
+  m.def("kv_step_check_refill", &kv_step_check_refill, "raises where a step's captured calls do not fit a refill");
   m.def("kv_step_write", &kv_step_write, "tokens into the pages of an 8-bit key/value cache");
   m.def("kv_step_attend", &kv_step_attend, "attention over an 8-bit paged key/value cache");
   m.def("kv_cache_copy_pages", &kv_cache_copy_pages, "copy cache pages in every layer");

@@ -252,8 +252,16 @@ void KvBook::resize(int64_t pages) {
   for (auto& [id, s] : seqs_) ++s.version;
 }
 
-int64_t KvBook::rows(const Ids& ids, const Ids& n_new, int front, int32_t* out) const {
+int64_t KvBook::trim_sinks(const Ids& ids) const {
   int64_t trim = -1;
+  for (const int64_t id : ids) {
+    const Seq& s = seq(id);
+    if (s.trimmed()) trim = trim == -1 || trim == s.sinks ? s.sinks : -2;
+  }
+  return trim;
+}
+
+void KvBook::rows(const Ids& ids, const Ids& n_new, int front, int32_t* out) const {
   for (size_t i = 0; i < ids.size(); ++i) {
     const Seq& s = seq(ids[i]);
     if (front == 4) {
@@ -261,12 +269,10 @@ int64_t KvBook::rows(const Ids& ids, const Ids& n_new, int front, int32_t* out) 
       out[1] = static_cast<int32_t>(n_new[i]);
       out[2] = s.trimmed() ? static_cast<int32_t>(s.first) : 0;
       out[3] = s.trimmed() ? static_cast<int32_t>(s.sinks) : -1;
-      if (s.trimmed()) trim = trim == -1 || trim == s.sinks ? s.sinks : -2;
     }
     out = std::copy(s.pages.begin(), s.pages.end(), out + front);
     out = std::fill_n(out, max_pages_ - static_cast<int64_t>(s.pages.size()), -1);
   }
-  return trim;
 }
 
 KvBook::Ids KvBook::versions(const Ids& ids) const {

@@ -42,9 +42,10 @@ class KvBook {
   void resize(int64_t pages);
 
   // A step's table, [sequences][front + max_pages]: front 4 writes the words that precede the
-  // page ids too, 0 the ids alone. Returns the sinks of the trimmed sequences (-1: none is,
-  // -2: they differ).
-  int64_t rows(const Ids& seqs, const Ids& n_new, int front, int32_t* out) const;
+  // page ids too, 0 the ids alone.
+  void rows(const Ids& seqs, const Ids& n_new, int front, int32_t* out) const;
+  // the sinks of the trimmed sequences (-1: none is, -2: they differ)
+  int64_t trim_sinks(const Ids& seqs) const;
   int64_t longest(const Ids& seqs, const Ids& n_new) const;
   Ids versions(const Ids& seqs) const;
   bool fresh(const Ids& seqs, const Ids& versions) const;

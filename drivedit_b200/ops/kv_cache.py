@@ -293,7 +293,8 @@ class PagedKVCache:
         are shaped for, for steps whose calls are captured into a graph; default: the
         longest of now. ``out``: a step of as many sequences to refill in place (on the current
         stream, behind the calls that still read it), so that a graph captured with it runs
-        on the new tables; its ``max_tokens`` must suffice."""
+        on the new tables; its ``max_tokens`` must suffice, ``n_new`` fit the rows of its captured
+        calls, and the sinks of windowed ones be those that the sequences were trimmed to."""
         self._not_capturing("begin")
         seqs = list(seqs)
         n_new = [int(n) for n in n_new] if isinstance(n_new, (list, tuple)) else [int(n_new)] * len(seqs)
@@ -303,6 +304,8 @@ class PagedKVCache:
             max_tokens = out.max_tokens if max_tokens is None else max_tokens
             if max_tokens != out.max_tokens:
                 raise ValueError("out keeps its max_tokens")
+            if out._h is not None:
+                ext().kv_step_check_refill(out._h, max(n_new, default=0), self._book.trim_sinks(seqs))
         if max_tokens is not None and max_tokens < 0:
             raise ValueError("max_tokens must not be negative")
         rows, src, dst, longest, trim, versions = self._book.begin(seqs, n_new, -1 if max_tokens is None else int(max_tokens))

@@ -166,6 +166,57 @@ def test_a_long_tail_of_small_weights_counts(T, gap):
     _check_rows(c, s, o[0], lse[0], q[0])
 
 
+def test_refill_beyond_the_captured_rows_is_refused():
+    """A step whose calls were captured with T rows takes no refill for more, and the refused
+    refill changes nothing."""
+    c = _cache(1, 2, 16)
+    seqs = c.add(2)
+    k, v, q = (_randn(2, 3, 2, 64) for _ in "kvq")
+    step = c.begin(seqs, 3, max_tokens=600)
+    step.write(0, k, v)
+    step.attend(0, q, causal="token")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.write(0, k, v)
+        o = step.attend(0, q[:, :3], causal="token")
+    step.commit()
+    free, lengths = c.free_pages, [c.length(s) for s in seqs]
+    for n in (4, [1, 200]):
+        with pytest.raises(ValueError):
+            c.begin(seqs, n, out=step)
+    assert c.free_pages == free and [c.length(s) for s in seqs] == lengths
+    c.begin(seqs, [3, 2], out=step)
+    graph.replay()
+    assert torch.equal(o, step.attend(0, q, causal="token"))
+
+
+def test_refill_with_other_sinks_than_captured_is_refused():
+    """A captured windowed call names its sinks; sequences trimmed to others are refused at the
+    refill, as the call itself would refuse them."""
+    c = _cache(1, 2, 32)
+    seqs = c.add(1)
+    k, v, q = (_randn(1, 300, 2, 64) for _ in "kvq")
+    step = c.begin(seqs, 300)
+    step.write(0, k, v)
+    step.commit()
+    step = c.begin(seqs, 1, max_tokens=600)
+    step.attend(0, q[:, :1], causal="token", window=90, sinks=2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.attend(0, q[:, :1], causal="token", window=90, sinks=2)
+    c.trim(seqs, keep=150, sinks=70)
+    length, free = c.length(seqs[0]), c.free_pages
+    with pytest.raises(ValueError):
+        c.begin(seqs, 1, out=step)
+    assert c.length(seqs[0]) == length and c.free_pages == free
+    other = c.add(1)
+    c.begin(other, 1, out=step)  # not trimmed: as captured
+    graph.replay()
+    torch.cuda.synchronize()
+
+
 def test_status_clean():
     from drivedit_b200.ops._ext import check_device_status
     torch.cuda.synchronize()
