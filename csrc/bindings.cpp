@@ -1734,7 +1734,14 @@ ddb::KvPool kv_layer(const KvStepHandle& h, int64_t layer) {
 
 void kv_step_wait(KvStepHandle& h) {
   const auto now = at::cuda::getCurrentCUDAStream();
-  if (now == *h.begun || kv_capturing()) return;
+  if (now == *h.begun) return;
+  if (kv_capturing()) {
+    // an event from outside cannot be waited for inside a graph: the upload is done before the
+    // graph can be replayed
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    h.ready.synchronize();
+    return;
+  }
   h.ready.block(now);
   h.rows.record_stream(now);
 }

@@ -29,9 +29,10 @@ below, which are also the kernels' oracle. Calls run on the current stream. A st
 be used on another stream than the one it was begun on (its table is waited for); the
 order of writes and reads of the cache itself between streams is the caller's, as for
 any tensor. Bookkeeping (``csrc/kvcache/book.cpp``) is on the host: calls on one cache come
-from one thread, and none that changes it can be captured into a graph. ``write`` and ``attend`` can; a graph that
-holds them is replayed after its step was refilled (``begin(..., out=step)``) for the
-sequences as they are then, and not after :meth:`PagedKVCache.resize`.
+from one thread, and none that changes it can be captured into a graph. ``write`` and ``attend`` can (on another
+stream than the step's, the host waits for its table); a graph that holds them is replayed
+behind the refill of its step (``begin(..., out=step)``) for the sequences as they are then,
+as long as the step lives, and not after :meth:`PagedKVCache.resize`.
 """
 from __future__ import annotations
 

@@ -217,6 +217,32 @@ def test_refill_with_other_sinks_than_captured_is_refused():
     torch.cuda.synchronize()
 
 
+def test_step_begun_on_another_stream_than_it_is_captured_on():
+    """The table is on the device before a captured call can be replayed."""
+    c = _cache(1, 2, 64)
+    seqs = c.add(2)
+    k, v, q = (_randn(2, 200, 2, 64) for _ in "kvq")
+    warm = c.begin(seqs, 200)
+    warm.write(0, k, v)
+    warm.attend(0, q, causal="token")
+    side = torch.cuda.Stream()
+    busy = torch.randn(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+        step = c.begin(seqs, 200)  # its upload waits behind the products
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(other):  # not torch.cuda.graph, which waits for the device first
+        graph.capture_begin()
+        step.write(0, k, v)
+        o = step.attend(0, q, causal="token")
+        graph.capture_end()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, step.attend(0, q, causal="token"))
+
+
 def test_status_clean():
     from drivedit_b200.ops._ext import check_device_status
     torch.cuda.synchronize()
