@@ -13,6 +13,7 @@
 #include <ATen/cuda/CUDAEvent.h>
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "common/tma.h"
 #include "gemm/gemm.h"
@@ -1569,6 +1570,12 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
     auto dq = torch::empty(s[0].sizes(), s[0].options()), dk = torch::empty(s[1].sizes(), s[1].options()),
          dv = torch::empty(s[2].sizes(), s[2].options());
     attn_window_bwd(s[0], s[1], s[2], s[3], s[4], s[5], grads[0].to(torch::kBFloat16), m, dq, dk, dv);
+    if (!at::GradMode::is_enabled()) return {dq, dk, dv, torch::Tensor()};
+    // create_graph: the kernels leave no graph, so a second derivative through these raises, on
+    // the way to whatever the first one went to, instead of missing terms
+    const auto error = std::make_shared<torch::autograd::Error>("window_attention has no second derivative on CUDA",
+                                                                torch::autograd::edge_list(torch::autograd::get_current_node()->next_edges()));
+    for (auto* t : {&dq, &dk, &dv}) torch::autograd::create_gradient_edge(*t, error);
     return {dq, dk, dv, torch::Tensor()};
   }
 };

@@ -49,11 +49,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     the newest ``window`` (its own counted; 0: all) and the first ``sinks``; "token" counts
     tokens instead of frames; "none" sees every key. Keys sit at their index plus
     ``kv_pos_offset``. Rows that see no key are zero and keys that no query sees are
-    left out; both get zero gradients, and what they hold has no effect on the others. Returns ``o`` (and, if
-    asked, ``lse [B, H, T]``, log2 domain of the scaled scores, without gradient). dQ is
-    summed in fp32 in no fixed order: equal backward passes may differ in dq by a rounding
-    of bf16. A backward pass is captured into a graph only when no autograd graph of the same
-    leaves made on the default stream is alive (refused otherwise)."""
+    left out; both get zero gradients, and what they hold has no effect on the others.
+    Returns ``o`` (and, if asked, ``lse [B, H, T]``, log2 domain of the scaled scores, without
+    gradient). dQ is summed in fp32 in no fixed order: equal backward passes may differ in dq
+    by a rounding of bf16. A second derivative raises on CUDA. A backward pass is captured
+    into a graph only when no autograd graph of the same leaves made on the default stream is
+    alive (refused otherwise)."""
     if q.is_cuda and q.numel() and k.numel():
         o, lse = ext().window_attention(q, k, v, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, scale)
         return (o, lse) if return_lse else o

@@ -38,6 +38,16 @@ def test_rows_that_meet_nan_are_nan_however_the_keys_are_split(splits):
     assert torch.equal(o[0][~bad], want[0][~bad]) and torch.equal(lse[0].T[~bad], wl[0].T[~bad])
 
 
+def test_second_derivative_in_a_sum_is_refused():
+    """A second derivative through the operator raises, also where other terms have one."""
+    from drivedit_b200.ops.window_attention import window_attention
+    q = _randn(1, 8, 1, 64).requires_grad_(True)
+    loss = window_attention(q, q, q, "token").float().sum() + q.float().pow(3).sum()
+    (g,) = torch.autograd.grad(loss, q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), q)
+
+
 # ------------------------------------------------------------------ paged cache
 def _cache(L=1, H=2, P=64, **kw):
     from drivedit_b200.ops.kv_cache import PagedKVCache
