@@ -1592,9 +1592,9 @@ void refuse_eager_leaf(const torch::Tensor& t) {
               "pass, or warm up on another stream");
 }
 
-std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
-                                            const std::string& causal, int64_t tokens_per_frame, int64_t window,
-                                            int64_t sinks, int64_t q_pos, int64_t kv_pos, c10::optional<double> scale) {
+WindowMask window_check(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const std::string& causal,
+                        int64_t tokens_per_frame, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
+                        c10::optional<double> scale) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(3) == 64 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
                         q.size(2) == k.size(2) && q.size(3) == k.size(3),
                     "q must be [B, T, H, 64], k and v [B, S, H, 64]: got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
@@ -1603,6 +1603,13 @@ std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch:
   TORCH_CHECK_VALUE(q.scalar_type() == torch::kBFloat16, "window_attention takes bfloat16 on CUDA, got ", q.scalar_type());
   const auto m = window_mask(causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale ? *scale : 0.125, q.size(1), k.size(1));
   TORCH_CHECK_VALUE(q.size(1) <= 65536 * 64, "at most ", 65536 * 64, " queries per sample");
+  return m;
+}
+
+std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                                            const std::string& causal, int64_t tokens_per_frame, int64_t window,
+                                            int64_t sinks, int64_t q_pos, int64_t kv_pos, c10::optional<double> scale) {
+  const auto m = window_check(q, k, v, causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale);
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad())) {
     const auto out = attn_window_fwd(tma_ready(q), tma_ready(k), tma_ready(v), m, false);
     return {out[0], out[1].narrow(2, 0, q.size(1))};
@@ -1617,15 +1624,16 @@ std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch:
 
 std::vector<torch::Tensor> attn_window_fwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
                                               const std::string& causal, int64_t tokens_per_frame, int64_t window,
-                                              int64_t sinks, double scale) {
-  return attn_window_fwd(q, k, v, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)), true);
+                                              int64_t sinks, c10::optional<double> scale, int64_t q_pos, int64_t kv_pos) {
+  const auto m = window_check(q, k, v, causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale);
+  return attn_window_fwd(tma_ready(q), tma_ready(k), tma_ready(v), m, true);
 }
 void attn_window_bwd_py(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
                         const torch::Tensor& rest, const torch::Tensor& lse, const torch::Tensor& grad, const std::string& causal,
-                        int64_t tokens_per_frame, int64_t window, int64_t sinks, double scale, const torch::Tensor& dq,
-                        const torch::Tensor& dk, const torch::Tensor& dv) {
-  attn_window_bwd(q, k, v, o, rest, lse, grad, window_mask(causal, tokens_per_frame, window, sinks, 0, 0, scale, q.size(1), k.size(1)),
-                  dq, dk, dv);
+                        int64_t tokens_per_frame, int64_t window, int64_t sinks, c10::optional<double> scale, const torch::Tensor& dq,
+                        const torch::Tensor& dk, const torch::Tensor& dv, int64_t q_pos, int64_t kv_pos) {
+  const auto m = window_check(q, k, v, causal, tokens_per_frame, window, sinks, q_pos, kv_pos, scale);
+  attn_window_bwd(tma_ready(q), tma_ready(k), tma_ready(v), o, rest, lse, grad, m, dq, dk, dv);
 }
 
 // ---------------------------------------------------------------- 8-bit paged key/value cache
@@ -1929,8 +1937,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_qmask"), py::arg("kv_count"), py::arg("debug_flags") = 0,
         py::arg("trace") = py::none(), py::arg("trace_cta") = 0);
   m.def("window_attention", &window_attention, "differentiable attention over a window and the first tokens");
-  m.def("attn_window_fwd", &attn_window_fwd_py, "its forward, for callers with a backward of their own");
-  m.def("attn_window_bwd", &attn_window_bwd_py, "its backward, into given gradients");
+  m.def("attn_window_fwd", &attn_window_fwd_py, "its forward, for callers with a backward of their own", py::arg("q"),
+        py::arg("k"), py::arg("v"), py::arg("causal"), py::arg("tokens_per_frame"), py::arg("window"), py::arg("sinks"),
+        py::arg("scale"), py::arg("q_pos_offset") = 0, py::arg("kv_pos_offset") = 0);
+  m.def("attn_window_bwd", &attn_window_bwd_py, "its backward, into given gradients", py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("o"), py::arg("rest"), py::arg("lse"), py::arg("grad"), py::arg("causal"),
+        py::arg("tokens_per_frame"), py::arg("window"), py::arg("sinks"), py::arg("scale"), py::arg("dq"), py::arg("dk"),
+        py::arg("dv"), py::arg("q_pos_offset") = 0, py::arg("kv_pos_offset") = 0);
   py::class_<KvStepHandle, std::shared_ptr<KvStepHandle>>(m, "KvStepHandle").def_readonly("rows", &KvStepHandle::rows);
   py::class_<ddb::KvBook::Seq>(m, "KvSeq")
       .def_property_readonly("pages", [](const ddb::KvBook::Seq& s) { return py::array_t<int32_t>(s.pages.size(), s.pages.data()); })

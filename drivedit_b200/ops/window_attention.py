@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from ..layers.attention import window_mask
-from ._ext import ext
+from ._ext import ext, sync_check
 
 _LIMIT = 1 << 30  # positions stay below
 
@@ -38,6 +38,31 @@ def _check_mask(causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_of
         raise ValueError("at most 2^24 tokens per frame")
 
 
+class _SyncChecked(torch.autograd.Function):
+    """The operator for the sync-check mode, which brackets entry points called from Python: the
+    extension's own autograd node calls its backward behind it."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, *args):
+        o, lse, rest = ext().attn_window_fwd(q, k, v, *args)
+        ctx.save_for_backward(q, k, v, o, rest, lse)
+        ctx.args = args
+        ctx.set_materialize_grads(False)
+        lse = lse[..., :q.shape[1]]
+        ctx.mark_non_differentiable(lse)
+        return o, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * (3 + len(ctx.args))
+        q, k, v, o, rest, lse = ctx.saved_tensors
+        out = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v)]
+        ext().attn_window_bwd(q, k, v, o, rest, lse, grad, *ctx.args[:5], *out, *ctx.args[5:])
+        return (*out, *(None for _ in ctx.args))
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: str = "frame",
                      tokens_per_frame: int = 1, window: int = 0, sinks: int = 0, q_pos_offset: int = 0,
                      kv_pos_offset: int = 0, scale: Optional[float] = None, return_lse: bool = False):
@@ -56,6 +81,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     into a graph only when no autograd graph of the same leaves made on the default stream is
     alive (refused otherwise)."""
     if q.is_cuda and q.numel() and k.numel():
+        if sync_check() and torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v)):
+            o, lse = _SyncChecked.apply(q, k, v, causal, tokens_per_frame, window, sinks, scale, q_pos_offset, kv_pos_offset)
+            return (o, lse) if return_lse else o
         o, lse = ext().window_attention(q, k, v, causal, tokens_per_frame, window, sinks, q_pos_offset, kv_pos_offset, scale)
         return (o, lse) if return_lse else o
     if q.dim() != 4 or k.dim() != 4 or q.shape[3] != 64 or k.shape != v.shape or \

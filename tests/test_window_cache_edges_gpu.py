@@ -48,6 +48,30 @@ def test_second_derivative_in_a_sum_is_refused():
         torch.autograd.grad(g.float().sum(), q)
 
 
+def test_sync_check_names_both_passes():
+    from drivedit_b200.ops import debug
+    from drivedit_b200.ops._ext import ext
+    from drivedit_b200.ops.window_attention import window_attention
+    q, k, v = (_randn(2, 70, 2, 64).requires_grad_(True) for _ in "qkv")
+    do = _randn(2, 70, 2, 64)
+    args = ("token", 1, 30, 2, 5, 5)
+    want = window_attention(q, k, v, *args, return_lse=True)
+    wg = torch.autograd.grad(want[0], (q, k, v), do)
+    debug.set_sync_check(True)
+    try:
+        got = window_attention(q, k, v, *args, return_lse=True)
+        gg = torch.autograd.grad(got[0], (q, k, v), do)
+        with torch.no_grad():
+            plain = window_attention(q, k, v, *args)
+        names = [d.split()[1].split("(")[0] for d in ext().recent]
+    finally:
+        debug.set_sync_check(False)
+    assert names.count("attn_window_bwd") == 1 and any(n in ("attn_window_fwd", "window_attention") for n in names), names
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(plain, want[0])
+    assert torch.equal(gg[1], wg[1]) and torch.equal(gg[2], wg[2])
+    assert (gg[0].float() - wg[0].float()).abs().max() <= 2.0 ** -7 * wg[0].float().abs().max()  # dq: no fixed order
+
+
 # ------------------------------------------------------------------ paged cache
 def _cache(L=1, H=2, P=64, **kw):
     from drivedit_b200.ops.kv_cache import PagedKVCache
