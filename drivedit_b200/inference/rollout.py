@@ -202,7 +202,7 @@ class StreamingRollout:
             raise ValueError(f"actions must be [B, K, F, A], got {tuple(actions.shape)}")
         return self._run(context, actions.flatten(0, 1), total_frames, generator, None, None, actions.shape[1])
 
-    def _make_cache(self, B: int, total: int, branches: int):
+    def _make_cache(self, B: int, total: int, branches: int, context: int):
         cfg, m = self.cfg, self.model
         make_cache = getattr(m, "make_kv_cache", None)     # e.g. a tensor-parallel model
         if make_cache is not None:
@@ -210,7 +210,7 @@ class StreamingRollout:
                 raise ValueError("tensor-parallel rollouts hold their window in bf16, without sinks")
             return make_cache(B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype)
         return make_kv_cache(m, B, cfg.window_frames, cfg.chunk_frames, self.device, self.dtype, cfg.kv_cache,
-                             cfg.sink_frames, total, branches)
+                             cfg.sink_frames, total, branches, context)
 
     def _run(self, context, actions, total_frames, generator, extra_cond, replace, branches) -> RolloutResult:
         cfg = self.cfg
@@ -219,7 +219,7 @@ class StreamingRollout:
         total = total_frames or cfg.total_frames
         chunk = cfg.chunk_frames
         fwd_chunk = getattr(m, "forward_cached_chunk", None)
-        cache = self._make_cache(B, max(total, Fc), branches)
+        cache = self._make_cache(B, max(total, Fc), branches, Fc)
 
         def forward_cached(m_, x_, t_, a_, cache_, commit=False, extra_cond=None):
             if fwd_chunk is not None:

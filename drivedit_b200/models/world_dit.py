@@ -387,10 +387,11 @@ class PagedKVCacheSet:
     (:class:`~drivedit_b200.ops.kv_cache.PagedKVCache`): of ``B`` streams the newest
     ``window_frames`` committed frames and the first ``sink_frames`` stay, older ones give
     their pages back. ``max_frames`` bounds a stream's length. :meth:`branch` turns the
-    streams into several that share their past."""
+    streams into several that share their past; the pool holds ``branches`` of each if they
+    branch behind ``context_frames`` frames or more."""
 
     def __init__(self, model: "WorldDiT", B: int, window_frames: int, chunk_frames: int, device,
-                 sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1):
+                 sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1, context_frames: int = 0):
         from ..ops.kv_cache import PAGE, PagedKVCache
 
         cfg = model.cfg
@@ -406,7 +407,9 @@ class PagedKVCacheSet:
         # a chunk joins the window before the oldest frames leave it; two unfinished pages
         own = pages(window_frames + 2 * chunk_frames) + 2
         total = pages(max_frames or cfg.max_frames) + 1
-        n = B * (pages(sink_frames) + own) + (B * branches * own if branches > 1 else 0)
+        n = B * (pages(sink_frames) + own)
+        if branches > 1:  # sinks behind the context are each branch's own, from the page where it ends
+            n += B * branches * (own + (pages(sink_frames - context_frames) + 1 if sink_frames > context_frames else 0))
         self.cache = PagedKVCache(len(model.blocks), cfg.n_heads, n, device, max_pages_per_seq=max(total, own))
         self.layers = [None] * len(model.blocks)
         self.seqs = self.cache.add(B)
@@ -434,13 +437,14 @@ class PagedKVCacheSet:
 
 
 def make_kv_cache(model: "WorldDiT", B: int, window_frames: int, chunk_frames: int, device, dtype,
-                  kv_cache: str = "bf16", sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1):
+                  kv_cache: str = "bf16", sink_frames: int = 0, max_frames: Optional[int] = None, branches: int = 1,
+                  context_frames: int = 0):
     """The rolling key/value window of a stream: contiguous buffers in ``dtype``
     (``kv_cache`` "bf16") or 8-bit pages ("fp8"), which also keep the first ``sink_frames``
     frames (0: the model's own)."""
     if kv_cache == "fp8":
         return PagedKVCacheSet(model, B, window_frames, chunk_frames, device, sink_frames or model.cfg.sink_frames,
-                               max_frames, branches)
+                               max_frames, branches, context_frames)
     if kv_cache != "bf16":
         raise ValueError(f'kv_cache must be "bf16" or "fp8", got {kv_cache!r}')
     if sink_frames:

@@ -1,0 +1,42 @@
+"""The paged cache and rollouts over it at their edges, on the CPU."""
+import pytest
+import torch
+
+from drivedit_b200.config import get_config
+from drivedit_b200.inference.rollout import StreamingRollout
+from drivedit_b200.models.world_dit import WorldDiT, make_kv_cache
+
+
+def _model(*over):
+    torch.manual_seed(0)
+    cfg = get_config("tiny", ["model.n_layers=1", *over])
+    return cfg, WorldDiT(cfg.model).eval()
+
+
+@pytest.mark.parametrize("context,sinks,window,chunk,branches", [
+    (1, 8, 4, 1, 16), (1, 16, 8, 4, 8), (2, 5, 1, 2, 9), (3, 3, 2, 1, 7), (4, 2, 2, 3, 5), (1, 3, 1, 1, 2),
+])
+def test_branched_streams_fit_their_pool(context, sinks, window, chunk, branches):
+    """Streams that branch before, at and after the end of their sinks, past sinks + window."""
+    _, m = _model()
+    total = context + sinks + 2 * window + 4 * chunk
+    cache = make_kv_cache(m, 2, window, chunk, "cpu", torch.float32, "fp8", sinks, total, branches, context)
+    for f0 in range(0, context, chunk):
+        cache.step(min(chunk, context - f0) * cache.tpf)
+        cache.commit(min(chunk, context - f0))
+    cache.branch(branches)
+    while cache.frames < total:
+        n = min(chunk, total - cache.frames)
+        cache.step(n * cache.tpf)
+        cache.commit(n)
+    assert len(cache.seqs) == 2 * branches
+    assert all(cache.cache.length(s) == total * cache.tpf for s in cache.seqs)
+
+
+def test_branched_rollout_with_sinks_behind_the_context():
+    cfg, m = _model()
+    r = cfg.rollout
+    r.chunk_frames, r.flow_steps, r.window_frames, r.kv_cache, r.sink_frames = 1, 1, 2, "fp8", 8
+    roll = StreamingRollout(m, r)
+    res = roll.run_branches(torch.randn(1, 1, 16, 16, 16), torch.zeros(1, 16, 14, 2), total_frames=14)
+    assert res.frames.shape[:2] == (16, 14) and torch.isfinite(res.frames).all()
