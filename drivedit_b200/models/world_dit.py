@@ -443,6 +443,9 @@ def make_kv_cache(model: "WorldDiT", B: int, window_frames: int, chunk_frames: i
     (``kv_cache`` "bf16") or 8-bit pages ("fp8"), which also keep the first ``sink_frames``
     frames (0: the model's own)."""
     if kv_cache == "fp8":
+        # the fused path's keys and values are bf16 whatever the frames are
+        if torch.device(device).type == "cuda" and dtype != torch.bfloat16 and model.fused is None:
+            raise ValueError(f"the 8-bit cache takes bfloat16 keys and values on CUDA, the model streams {dtype}")
         return PagedKVCacheSet(model, B, window_frames, chunk_frames, device, sink_frames or model.cfg.sink_frames,
                                max_frames, branches, context_frames)
     if kv_cache != "bf16":

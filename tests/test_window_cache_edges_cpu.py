@@ -4,7 +4,7 @@ import torch
 
 from drivedit_b200.config import get_config
 from drivedit_b200.inference.rollout import StreamingRollout
-from drivedit_b200.models.world_dit import WorldDiT, make_kv_cache
+from drivedit_b200.models.world_dit import PagedKVCacheSet, WorldDiT, make_kv_cache
 
 
 def _model(*over):
@@ -40,3 +40,11 @@ def test_branched_rollout_with_sinks_behind_the_context():
     roll = StreamingRollout(m, r)
     res = roll.run_branches(torch.randn(1, 1, 16, 16, 16), torch.zeros(1, 16, 14, 2), total_frames=14)
     assert res.frames.shape[:2] == (16, 14) and torch.isfinite(res.frames).all()
+
+
+def test_types_the_cuda_cache_does_not_hold_are_refused_when_it_is_made():
+    _, m = _model()
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(ValueError, match="bfloat16"):
+            make_kv_cache(m, 1, 2, 1, torch.device("cuda"), dtype, "fp8")
+    assert isinstance(make_kv_cache(m, 1, 2, 1, "cpu", torch.float32, "fp8"), PagedKVCacheSet)
