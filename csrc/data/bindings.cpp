@@ -1,5 +1,6 @@
-// Python bindings of the native data runtime (module drivedit_b200._data): ENFCAP
-// reader/writer, telemetry CSV parsing + control normalisation, PNG frame loading.
+// Python bindings of the host-only runtime (module drivedit_b200._data): ENFCAP
+// reader/writer, telemetry CSV parsing + control normalisation, PNG frame loading, and the
+// paged key/value cache's bookkeeping.
 // Heavy calls release the GIL; results are returned as torch tensors.
 #include <torch/extension.h>
 
@@ -12,6 +13,10 @@
 #include "telemetry.h"
 
 namespace py = pybind11;
+
+namespace ddb {
+void bind_kv_book(py::module_& m);  // kvcache/book_py.cpp
+}
 
 namespace {
 
@@ -99,7 +104,8 @@ ddd::TelemetryTable table_from(const py::dict& d) {
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "native data runtime: ENFCAP, telemetry, frames";
+  m.doc() = "native data runtime: ENFCAP, telemetry, frames; bookkeeping of the paged key/value cache";
+  ddb::bind_kv_book(m);
   py::class_<ddd::EnfcapReader, std::shared_ptr<ddd::EnfcapReader>>(m, "ENFCAPReader")
       .def(py::init<const std::string&>())
       .def_property_readonly("frame_count", &ddd::EnfcapReader::frame_count)

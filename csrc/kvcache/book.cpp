@@ -264,7 +264,7 @@ int64_t KvBook::trim_sinks(const Ids& ids) const {
 void KvBook::rows(const Ids& ids, const Ids& n_new, int front, int32_t* out) const {
   for (size_t i = 0; i < ids.size(); ++i) {
     const Seq& s = seq(ids[i]);
-    if (front == 4) {
+    if (front == kFront) {
       out[0] = static_cast<int32_t>(s.length + n_new[i]);
       out[1] = static_cast<int32_t>(n_new[i]);
       out[2] = s.trimmed() ? static_cast<int32_t>(s.first) : 0;

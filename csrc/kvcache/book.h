@@ -14,6 +14,7 @@ class KvBook {
  public:
   using Ids = std::vector<int64_t>;
   using Pages = std::vector<int32_t>;
+  static constexpr int kFront = 4;  // words of a step's row before its page ids (kvcache.h)
 
   struct Seq {
     Pages pages;          // by page of the sequence; -1: given back
@@ -41,8 +42,8 @@ class KvBook {
   Copies compact();
   void resize(int64_t pages);
 
-  // A step's table, [sequences][front + max_pages]: front 4 writes the words that precede the
-  // page ids too, 0 the ids alone.
+  // A step's table, [sequences][front + max_pages]: front kFront writes the words that precede
+  // the page ids too, 0 the ids alone.
   void rows(const Ids& seqs, const Ids& n_new, int front, int32_t* out) const;
   // the sinks of the trimmed sequences (-1: none is, -2: they differ)
   int64_t trim_sinks(const Ids& seqs) const;

@@ -42,6 +42,7 @@ from typing import List, Optional, Sequence, Union
 import numpy as np
 import torch
 
+from ..data.native import native
 from ._ext import ext
 from .window_attention import _check_mask
 
@@ -226,7 +227,7 @@ class PagedKVCache:
         if not 1 <= self.max_pages_per_seq <= _MAX_TOKENS // PAGE:
             raise ValueError("max_pages_per_seq out of range")
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
-        self._book = ext().KvBook(n_pages, self.max_pages_per_seq)
+        self._book = native().KvBook(n_pages, self.max_pages_per_seq)
 
     def _pool(self, n):
         shape = (self.n_layers, n, self.n_heads)

@@ -16,8 +16,9 @@ sources = sorted(
     glob.glob(os.path.join(CSRC, "**", "*.cu"), recursive=True)
     + glob.glob(os.path.join(CSRC, "**", "*.cpp"), recursive=True)
 )
-# host-only C++ data runtime is a separate extension
-sources = [s for s in sources if os.sep + "data" + os.sep not in s]
+# the host-only C++ runtime (data, the paged cache's bookkeeping) is a separate extension
+book_sources = [os.path.join(CSRC, "kvcache", f) for f in ("book.cpp", "book_py.cpp")]
+sources = [s for s in sources if os.sep + "data" + os.sep not in s and s not in book_sources]
 
 nvcc_flags = [
     "-O3",
@@ -36,7 +37,7 @@ nvcc_flags = [
 libstdcxx = [f"-L{d}" for d in ("/usr/lib/x86_64-linux-gnu",) if os.path.exists(os.path.join(d, "libstdc++.so.6"))]
 libstdcxx = libstdcxx + ["-l:libstdc++.so.6"] if libstdcxx else []
 
-data_sources = sorted(glob.glob(os.path.join(CSRC, "data", "*.cpp")))
+data_sources = sorted(glob.glob(os.path.join(CSRC, "data", "*.cpp"))) + book_sources
 ext_modules = [
         CUDAExtension(
             name="drivedit_b200._C",

@@ -1,4 +1,7 @@
 """The paged cache and rollouts over it at their edges, on the CPU."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -48,3 +51,25 @@ def test_types_the_cuda_cache_does_not_hold_are_refused_when_it_is_made():
         with pytest.raises(ValueError, match="bfloat16"):
             make_kv_cache(m, 1, 2, 1, torch.device("cuda"), dtype, "fp8")
     assert isinstance(make_kv_cache(m, 1, 2, 1, "cpu", torch.float32, "fp8"), PagedKVCacheSet)
+
+
+def test_cpu_cache_needs_no_cuda_extension():
+    code = """
+import sys
+sys.modules["drivedit_b200._C"] = None  # its import fails
+import torch
+from drivedit_b200.ops.kv_cache import PagedKVCache
+c = PagedKVCache(1, 1, 8, device="cpu")
+s = c.add(2)
+step = c.begin(s, [70, 3])
+x = torch.randn(2, 70, 1, 64)
+step.write(0, x, x)
+assert torch.isfinite(step.attend(0, x, causal="token")).all()
+step.commit()
+kids = c.fork(s, 2)
+c.trim(kids, keep=4)
+c.free(s), c.compact(), c.resize(16), c.copy(kids)
+print(c.table(kids).tolist(), c.length(kids[0]))
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip().endswith("70"), run.stderr[-2000:]
