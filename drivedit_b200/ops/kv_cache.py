@@ -136,8 +136,8 @@ class CacheStep:
         "none". ``window`` (frames, for "token" tokens; 0: no limit) keeps the newest ones
         visible, the query's own counted, and ``sinks`` the sequence's first ones beside
         them. Of a trimmed sequence what :meth:`PagedKVCache.trim` kept is visible at most.
-        Returns ``o [B, T, heads, 64]`` (and ``lse [B, heads, T]``, log2 domain); rows
-        behind a sequence's ``n_new`` and rows that see no key are zero (-inf)."""
+        Returns ``o [B, T, heads, 64]`` (and ``lse [B, heads, T]``, log2 domain), without
+        gradient; rows behind a sequence's ``n_new`` and rows that see no key are zero (-inf)."""
         self._check()
         if self._h is not None:
             out = ext().kv_step_attend(self._h, layer, q, causal, tokens_per_frame, window, sinks, scale, return_lse)
@@ -159,6 +159,7 @@ class CacheStep:
         self.cache._book.commit(self.seqs, self.n_new)
 
     # ------------------------------------------------------------------ PyTorch form
+    @torch.no_grad()
     def _write_torch(self, layer, k, v):
         c = self.cache
         for i, (s, n) in enumerate(zip(self._states, self.n_new)):
@@ -174,6 +175,7 @@ class CacheStep:
                     codes[layer, s.pages[j]] = y.mT if last else y
                     scales[layer, s.pages[j]] = sc
 
+    @torch.no_grad()
     def _attend_torch(self, layer, q, causal, unit, window, n_sink, scale, return_lse):
         c = self.cache
         o = torch.zeros(q.shape, dtype=q.dtype, device=q.device)

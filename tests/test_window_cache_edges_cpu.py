@@ -8,6 +8,7 @@ import torch
 from drivedit_b200.config import get_config
 from drivedit_b200.inference.rollout import StreamingRollout
 from drivedit_b200.models.world_dit import PagedKVCacheSet, WorldDiT, make_kv_cache
+from drivedit_b200.ops.kv_cache import PagedKVCache
 
 
 def _model(*over):
@@ -73,3 +74,14 @@ print(c.table(kids).tolist(), c.length(kids[0]))
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip().endswith("70"), run.stderr[-2000:]
+
+
+def test_cache_calls_take_no_gradients():
+    """The cache holds codes: what is read from it has no gradient, on either device."""
+    c = PagedKVCache(1, 1, 4, device="cpu")
+    step = c.begin(c.add(1), 5)
+    x = torch.randn(1, 5, 1, 64, requires_grad=True)
+    step.write(0, x, x)
+    o, lse = step.attend(0, x, causal="token", return_lse=True)
+    assert not o.requires_grad and not lse.requires_grad
+    assert not any(t.requires_grad for t in (c.k_scale, c.v_scale, *c.read(0, step.seqs[0])))
