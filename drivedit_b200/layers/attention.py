@@ -58,6 +58,13 @@ def frame_causal_mask(T: int, tokens_per_frame: int, S: Optional[int] = None,
     return (kf <= qf)[None, None]
 
 
+def frames_span(causal: str, tokens_per_frame: int, window_frames: int, sink_frames: int) -> Dict:
+    """A window and sinks of whole frames as the windowed operators' arguments, which count them in
+    frames for ``causal`` "frame" and in tokens otherwise."""
+    per = 1 if causal == "frame" else tokens_per_frame
+    return dict(causal=causal, tokens_per_frame=tokens_per_frame, window=window_frames * per, sinks=sink_frames * per)
+
+
 def window_mask(T: int, S: int, causal: str = "frame", tokens_per_frame: int = 1, window: int = 0,
                 sinks: int = 0, q_pos_offset: int = 0, kv_pos_offset: int = 0, device=None) -> torch.Tensor:
     """``[T, S]`` bool, True = attend: a query of frame f sees the frames f - window + 1 .. f

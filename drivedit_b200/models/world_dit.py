@@ -34,7 +34,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..config import ModelConfig
-from ..layers.attention import attention_reference, frame_causal_mask, window_mask
+from ..layers.attention import attention_reference, frame_causal_mask, frames_span, window_mask
 from ..layers.mlp import split_gu
 from ..layers.moe import MoEFFN
 from ..layers.rope import RoPE3D, apply_rope
@@ -42,10 +42,8 @@ from ..layers.sla import SLAConfig, sla_topk_reference
 
 
 def attention_span(cfg: ModelConfig, tpf: int) -> Dict:
-    """The model's causal mask as the windowed operators' arguments (``causal``,
-    ``tokens_per_frame``, ``window``, ``sinks``; frames for "frame", tokens for "token")."""
-    per = 1 if cfg.causal == "frame" else tpf
-    return dict(causal=cfg.causal, tokens_per_frame=tpf, window=cfg.window_frames * per, sinks=cfg.sink_frames * per)
+    """The model's causal mask as the windowed operators' arguments."""
+    return frames_span(cfg.causal, tpf, cfg.window_frames, cfg.sink_frames)
 
 
 def patchify(x: torch.Tensor, p: int) -> torch.Tensor:

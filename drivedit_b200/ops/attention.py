@@ -35,12 +35,11 @@ def _split(qkv, bc):
 
 
 def _torch_dense(q, k, v, bc):
-    from ..layers.attention import frame_causal_mask, window_mask
+    from ..layers.attention import frame_causal_mask, frames_span, window_mask
 
     T = q.shape[1]
     if getattr(bc, "window_frames", 0):
-        per = 1 if bc.causal == "frame" else bc.tpf
-        mask = window_mask(T, T, bc.causal, bc.tpf, bc.window_frames * per, bc.sink_frames * per, device=q.device)
+        mask = window_mask(T, T, device=q.device, **frames_span(bc.causal, bc.tpf, bc.window_frames, bc.sink_frames))
     elif bc.causal == "frame":
         mask = frame_causal_mask(T, bc.tpf, device=q.device)
     elif bc.causal == "token":

@@ -21,6 +21,7 @@ from typing import Optional
 
 import torch
 
+from ..layers.attention import frames_span
 from ..layers.sla import SLAConfig, block_valid_mask, n_selected, sla_linear_reference
 from ._ext import ext
 
@@ -180,14 +181,16 @@ def _heads(qkv, bc):
 
 
 def _window_args(bc):
-    per = 1 if bc.causal == "frame" else bc.tpf
-    return bc.causal, bc.tpf, bc.window_frames * per, bc.sink_frames * per, 1.0 / math.sqrt(bc.Dh)
+    return dict(frames_span(bc.causal, bc.tpf, bc.window_frames, bc.sink_frames), scale=1.0 / math.sqrt(bc.Dh))
 
 
 def attention_fwd_kernel(qkv: torch.Tensor, bc):
     B, T, H, d = bc.B, bc.T, bc.H, bc.d
     assert bc.Dh == 64, "the attention kernels are written for d_head = 64"
     M = qkv.shape[0]
+    if bc.window_frames and bc.attn_mode == "dense":
+        o4, lse, rest = ext().attn_window_fwd(*_heads(qkv, bc), **_window_args(bc))
+        return o4.view(M, d), None, lse, rest
     o = torch.empty(M, d, device=qkv.device, dtype=torch.bfloat16)
     lse = torch.empty(B * H * T, device=qkv.device, dtype=torch.float32)
     scale = 1.0 / math.sqrt(bc.Dh)
@@ -195,9 +198,6 @@ def attention_fwd_kernel(qkv: torch.Tensor, bc):
     plan = None
     o_lin = None
     lists = (None, None, None)
-    if bc.window_frames and bc.attn_mode == "dense":
-        o4, lse, rest = ext().attn_window_fwd(*_heads(qkv, bc), *_window_args(bc))
-        return o4.view(M, d), None, lse, rest
     if bc.attn_mode == "sla":
         plan = sla_plan_kernel(qkv, B, T, H, bc.sla_cfg, bc.tpf, bc.causal)
         lists = (plan.pair_blocks, plan.pair_mask, plan.pair_count)
@@ -214,8 +214,9 @@ def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc):
     dev = qkv.device
     if bc.window_frames and bc.attn_mode == "dense":
         dqkv = torch.empty(M, 3 * d, device=dev, dtype=torch.bfloat16)
-        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), plan, lse, do.view(B, T, H, 64), *_window_args(bc),
-                              *_heads(dqkv, bc))
+        dq, dk, dv = _heads(dqkv, bc)
+        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), plan, lse, do.view(B, T, H, 64), dq=dq, dk=dk, dv=dv,
+                              **_window_args(bc))
         return dqkv
     delta = torch.empty(B * H * T, device=dev, dtype=torch.float32)
     ext().attn_delta(o, do, delta, 0, 0, B, H, T, T)
