@@ -47,9 +47,9 @@ constexpr int kGroups = 4;
 constexpr int kMaxStages = 6;
 constexpr int kPageBytes = 8192;  // keys, then values
 constexpr float kHeadroom = 15.f;  // log2 of what a weight of 1 is in fp16 (largest: 2^16 less a step)
-// Scores (log2) from which the rounding of a maximum, 2^-24 of it, would move a weight by 2^(1/16)
-// and more: far beyond, a fused multiply-add against it would overflow.
-constexpr float kFar = 1048576.f;
+// Scores (log2) from which the rounding of a maximum, 2^-24 of it, moves the weights against it by
+// more than 2^(1/2), all alike; from 2^24 on they would overflow.
+constexpr float kFar = 8388608.f;
 constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
 // the CTA's result and its rows' (m, l) | barriers | page scales | flag | rings, later the

@@ -69,9 +69,9 @@ constexpr int OFF_RES_ML = OFF_RES + kRows * 256; // (max, sum) per row
 static_assert(OFF_RES_ML + kRows * 8 <= OFF_RAW, "results fit the operand tiles");
 constexpr uint32_t C_S = 0, C_O = 256, C_P = 384;  // + 128 / 64 / 64 per row tile
 constexpr float kRescaleLog2 = 8.f;
-// Scores (log2) from which the rounding of a maximum, 2^-24 of it, would move a weight by 2^(1/16)
-// and more: far beyond, a fused multiply-add against it would overflow.
-constexpr float kFar = 1048576.f;
+// Scores (log2) from which the rounding of a maximum, 2^-24 of it, moves the weights against it by
+// more than 2^(1/2), all alike; from 2^24 on they would overflow.
+constexpr float kFar = 8388608.f;
 constexpr float kHeadroom = 7.f;  // log2 of what a weight of 1 is in fp16; with the lag 2^15 at most
 constexpr long kPartFloats = kRows * 66;  // a CTA's result in scratch
 constexpr int kHandOver = 3;  // quarters of a row's exponentials after which the other tile may begin
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     // a padding row keeps zeros and the span of the last row: its result is not used
     const KvSpan span = kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
-    float sl2;
+    float sl2, bound;
     {
       uint4 w[8];
 #pragma unroll
@@ -442,6 +442,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_shared_v4(dst + ((i ^ (lr & 7)) << 4), h[0], h[1], h[2], h[3]);
       }
       sl2 = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
+      // |S| < 2^30, 64 products of numbers up to 2^15 and 448; zero for a row of zeros (padding)
+      bound = amax > 0.f ? sl2 * 0x1p30f * __int_as_float(*k_most) : 0.f;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
@@ -590,9 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     // Scores that may be far from zero go through a loop of their own (in the other one the test
-    // and the code for them took 229-235 us where this takes 227). |S| < 2^30: 64 products of
-    // numbers up to 2^15 and 448.
-    const bool far = __any_sync(0xffffffffu, sl2 * __int_as_float(*k_most) >= kFar * 0x1p-30f);
+    // and the code for them took 229-235 us where this takes 227).
+    const bool far = __any_sync(0xffffffffu, bound >= kFar);
     const bool ok = !active || (far ? steps(std::true_type{}) : steps(std::false_type{}));
     if (!ok) {
       if (lane == 0 && status) atomicCAS(status, 0, kStatusTimeoutEpilogue);

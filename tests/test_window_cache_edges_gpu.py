@@ -141,7 +141,7 @@ def test_large_scores_few_rows(T, G, far):
         _check_rows(c, s, o[0], lse[0], q[0], window)
 
 
-@pytest.mark.parametrize("what,far", [("k", 2.0 ** e) for e in (12, 17, 26, 60, -30)] + [("v", 2.0 ** e) for e in (12, 17, 26, 60, -30)])
+@pytest.mark.parametrize("what,far", [("k", 2.0 ** e) for e in (12, 17, 20, 23, 26, 60, -30)] + [("v", 2.0 ** e) for e in (12, 17, 26, 60, -30)])
 @pytest.mark.parametrize("T,G", [(28, 1), (200, 1), (300, 2), (700, 1)])
 def test_pages_that_a_row_does_not_see_do_not_touch_it(T, G, what, far):
     """Pages of far larger (or smaller) keys or values, behind the causal edge of the earlier
