@@ -243,8 +243,9 @@ int64_t KvBook::used_end() const {
   return p;
 }
 
-void KvBook::resize(int64_t pages) {
+void KvBook::resize(int64_t pages, int64_t max_pages) {
   if (pages < used_end()) refuse("pages behind the new size are in use");
+  max_pages_ = std::max(max_pages_, max_pages);
   free_ += pages - static_cast<int64_t>(refs_.size());
   refs_.resize(pages, 0);
   low_ = 0;

@@ -40,7 +40,7 @@ class KvBook {
   void free(const Ids& seqs);
   void trim(const Ids& seqs, int64_t keep, int64_t sinks);
   Copies compact();
-  void resize(int64_t pages);
+  void resize(int64_t pages, int64_t max_pages);  // max_pages does not shrink
 
   // A step's table, [sequences][front + max_pages]: front kFront writes the words that precede
   // the page ids too, 0 the ids alone.

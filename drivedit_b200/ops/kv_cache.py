@@ -210,7 +210,8 @@ class PagedKVCache:
 
     ``k`` / ``v``: float8_e4m3fn ``[layers, pages, heads, 64, 64]``, keys by (token, channel),
     values by (channel, token); ``k_scale`` / ``v_scale``: float32 ``[layers, pages, heads]``.
-    ``max_pages_per_seq`` bounds a sequence (default: the pool). Free pages are taken in
+    ``max_pages_per_seq`` bounds a sequence (default: the pool, at the largest that it has
+    been). Free pages are taken in
     the order of their ids. Every call that does not fit raises before it changes anything."""
 
     def __init__(self, n_layers: int, n_heads: int, n_pages: int, device=None,
@@ -226,6 +227,7 @@ class PagedKVCache:
         self.device = device
         self.n_layers, self.n_heads, self.n_pages = n_layers, n_heads, n_pages
         self.max_pages_per_seq = n_pages if max_pages_per_seq is None else max_pages_per_seq
+        self._bound_by_pool = max_pages_per_seq is None
         if not 1 <= self.max_pages_per_seq <= _MAX_TOKENS // PAGE:
             raise ValueError("max_pages_per_seq out of range")
         self.k, self.v, self.k_scale, self.v_scale = self._pool(n_pages)
@@ -305,6 +307,8 @@ class PagedKVCache:
         if out is not None:
             if out.cache is not self or len(out.seqs) != len(seqs):
                 raise ValueError("out is a step of another cache or number of sequences")
+            if out._rows.shape[1] != _INFO + self.max_pages_per_seq:
+                raise ValueError("out was begun before the cache grew")
             max_tokens = out.max_tokens if max_tokens is None else max_tokens
             if max_tokens != out.max_tokens:
                 raise ValueError("out keeps its max_tokens")
@@ -358,6 +362,8 @@ class PagedKVCache:
         used = self.n_pages - self.free_pages
         if n_pages < max(used, 1):
             raise ValueError(f"{used} pages are in use, {n_pages} asked for")
+        if self._bound_by_pool and n_pages > _MAX_TOKENS // PAGE:
+            raise ValueError("max_pages_per_seq out of range")
         if self._book.used_end() > n_pages:
             self.compact()
         old, n = (self.k, self.v, self.k_scale, self.v_scale), min(n_pages, self.n_pages)
@@ -365,7 +371,9 @@ class PagedKVCache:
         for a, b in zip((self.k, self.v, self.k_scale, self.v_scale), old):
             a, b = (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in (a, b))
             a[:, :n].copy_(b[:, :n])
-        self._book.resize(n_pages)
+        if self._bound_by_pool:
+            self.max_pages_per_seq = max(self.max_pages_per_seq, n_pages)
+        self._book.resize(n_pages, self.max_pages_per_seq)
         self.n_pages = n_pages
 
     def _values(self, layer, s, n: int):

@@ -85,3 +85,30 @@ def test_cache_calls_take_no_gradients():
     o, lse = step.attend(0, x, causal="token", return_lse=True)
     assert not o.requires_grad and not lse.requires_grad
     assert not any(t.requires_grad for t in (c.k_scale, c.v_scale, *c.read(0, step.seqs[0])))
+
+
+def test_sequences_grow_with_the_pool():
+    """Without a bound of its own a sequence may take the pages that the pool has gained."""
+    c = PagedKVCache(1, 1, 4, device="cpu")
+    (s,) = c.add(1)
+    old = c.begin([s], 256)
+    old.commit()
+    with pytest.raises(ValueError):
+        c.begin([s], 1)
+    c.resize(7)
+    free = c.free_pages
+    with pytest.raises(ValueError):
+        c.begin([s], 1, max_tokens=old.max_tokens, out=old)  # its table is of the old size
+    assert c.free_pages == free and c.length(s) == 256
+    step = c.begin([s], 192)
+    assert step.table.shape == (1, 7) and (step.table >= 0).all()
+    step.commit()
+    c.trim([s], keep=64)
+    c.resize(4)
+    assert c.table([s]).shape == (1, 7) and c.length(s) == 448
+    with pytest.raises(ValueError):
+        c.begin([s], 1)
+    fixed = PagedKVCache(1, 1, 4, device="cpu", max_pages_per_seq=2)
+    fixed.resize(8)
+    with pytest.raises(ValueError):
+        fixed.begin(fixed.add(1), 129)
