@@ -26,11 +26,16 @@
 // Windowed mode (attn_window_fwd): the keys of the newest frames and the first ones; a
 // query tile walks only tiles with a visible key. Any number of queries and keys, any
 // strides of the heads' rows. Its split-KV CTAs are a cluster and merge through
-// distributed shared memory: no scratch memory, no second launch. Bound by the softmax
-// (16 exponentials a clock and SM): 2 x 12 heads of 16 frames of 512 tokens, window of 4 frames
-// and 1 sink frame, 199 us (566 TFLOP/s; the exponentials alone 98 us), 10 us of it for what
+// distributed shared memory: no scratch memory, no second launch. 2 x 12 heads of 16 frames of
+// 512 tokens, window of 4 frames and 1 sink frame: 199 us (566 TFLOP/s), 10 us of it for what
 // rounding o to bf16 leaves, kept for the backward; 1024 queries over 9,216 of 12,288 keys,
-// 2 x 12 heads, 119 us.
+// 2 x 12 heads: 120 us. Bound by a row's chain of softmax steps (load, maximum, exponentials,
+// store): the exponentials alone (16 a clock and SM) are 98 and 50 us, their unit is busy 54 %
+// of the time, and nothing keeps the SM's two CTAs out of step.
+// P is held in bf16 (half a step is 2^-8 of a weight), since both operands of a product are
+// of one type and V is bf16, and O is rounded once more: together 1.4 times the error of fp32
+// arithmetic rounded once. The sum l takes the weights before their rounding: lse is exact to
+// fp32.
 // Semantics oracle: layers/attention.py attention_reference (reference layers/mha.py:88-116
 // with fp32 softmax), layers/sla.py sla_sparse_reference.
 #include <cuda.h>

@@ -24,10 +24,11 @@
 // form a cluster and meet through distributed shared memory. No scratch memory, no second
 // launch, and a fixed order of sums.
 // Measured: 64 streams of 16 heads and up to 16,384 cached tokens, one new token each,
-// 255 us: 1.62 GB of codes at 0.97 of the rate of a plain copy, bound by memory. One token
+// 255-285 us by GPU: 1.62 GB of codes at 0.97-0.87 of the rate of a plain copy, bound by memory. One token
 // of one stream of 1,500 tokens, 12 heads: 6.5 us, a chain of latencies (launch, table, page,
-// scores, merge). 5 tokens of 16 streams, 16 heads over 4 cached ones, window 2,048: 13.3 us,
-// 2.6 us of bytes: 3 row tiles' warps wait for the next page of their group.
+// scores, merge). 5 tokens of 16 streams, 16 heads over 4 cached ones, window 2,048: 14.7 us a
+// call, 2.6 us of bytes: the 3 warps of a group each convert the page's codes, for 8 rows each, and only
+// 4 pages of a CTA are in work at once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -15,18 +15,21 @@
 // into its weights, whose reference is the largest product of weight and scale that the row
 // itself has met: a page that a row does not see, or hardly weighs, takes nothing from the others.
 // (Scales in the converted codes, relative to the CTA's largest, took 222 us at the shape below
-// where this takes 225, but lost pages 2^25 below it; the exponents' constants made only after
-// the scores, 231.)
+// where this takes 227, but lost pages 2^25 below it. With a loop of its own for scales that lie
+// too far apart for that: 226, and 436 where they do. The exponents' constants made only after
+// the scores: 231.)
 // P <= 2^8 (the running maximum may lag by that) is held as 2^7 P in fp16: rounded by at most
 // 2^-11 of itself, finer than the bf16 kernel's P, or by 2^-32 where it is below 2^-21.
 // The CTAs that share a row block form a cluster and meet through distributed shared memory,
 // in one launch; or, where the clusters' sizes would leave SMs idle, meet in scratch memory
 // that a second launch adds up (kv_attend_tiles_plan).
-// Bound by the softmax: 256 x 128 exponentials a step at 16 a clock and SM are 2048 clocks,
-// its matrix products 1072, and a step takes 3300 (1.75 us). While one row tile is in its
-// exponentials the other loads scores, takes its maximum and stores weights (they take
-// turns). 2048 rows over 20,480 visible tokens of 12 heads (129 GFLOP): 222 us, 0.58 PFLOP/s
-// (248 us in one launch of clusters). Tried against those 248, and slower: the next scores
+// Bound by a row's chain of softmax steps: of the 3300 clocks (1.75 us) that a step of 256 x 128
+// takes, the exponentials (16 a clock and SM) are 2048, and the matrix products that run beside
+// them 1072. While one row tile is in its exponentials the other loads scores, takes its
+// maximum and stores weights (they take turns); where that takes longer than the exponentials
+// their unit waits (busy 57 % of the time). 2048 rows over 20,480 visible tokens of 12 heads (129
+// GFLOP): 227 us, 0.57 PFLOP/s (in one launch of clusters 248 us, with 222 for this one then).
+// Tried against those 248, and slower: the next scores
 // loaded under the exponentials (266-320 us), two threads a row (304), four streams by row tile
 // and page with one MMA warp (306) or one each (300), waits that spin (258).
 #include <cuda_bf16.h>
@@ -591,8 +594,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return true;
     };
-    // Scores that may be far from zero go through a loop of their own (in the other one the test
-    // and the code for them took 229-235 us where this takes 227).
+    // Scores that may be far from zero go through a loop of their own, twice as slow (in the other
+    // one the test and the code for them took 229-235 us where this takes 227).
     const bool far = __any_sync(0xffffffffu, bound >= kFar);
     const bool ok = !active || (far ? steps(std::true_type{}) : steps(std::false_type{}));
     if (!ok) {
