@@ -76,7 +76,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     ``kv_pos_offset``. Rows that see no key are zero and keys that no query sees are
     left out; both get zero gradients, and what they hold has no effect on the others.
     Returns ``o`` (and, if asked, ``lse [B, H, T]``, log2 domain of the scaled scores, without
-    gradient). dQ is summed in fp32 in no fixed order: equal backward passes may differ in dq
+    gradient). Scaled scores are fp32 and stay below 2^30 in magnitude; what that leaves of a
+    score's difference from the row's ``lse``, 2^-24 of it, is a gradient's error too. dQ is summed in fp32 in no fixed order: equal backward passes may differ in dq
     by a rounding of bf16. A second derivative raises on CUDA. A backward pass is captured
     into a graph only when no autograd graph of the same leaves made on the default stream is
     alive (refused otherwise)."""

@@ -38,6 +38,23 @@ def test_rows_that_meet_nan_are_nan_however_the_keys_are_split(splits):
     assert torch.equal(o[0][~bad], want[0][~bad]) and torch.equal(lse[0].T[~bad], wl[0].T[~bad])
 
 
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("far", [2.0 ** 12, 2.0 ** 20, 2.0 ** 24])
+def test_large_scores_give_finite_rows(far, splits):
+    """Scores up to 2^28, past what fp32 tells apart: rows are means of values."""
+    from drivedit_b200.ops._ext import ext
+    from drivedit_b200.ops.window_attention import window_attention
+    q, k, v = _randn(1, 150, 2, 64).clamp(-1, 1), _randn(1, 1100, 2, 64).clamp(-1, 1) * far, _randn(1, 1100, 2, 64)
+    prev = ext().attn_fwd_set_kv_splits(splits)
+    try:
+        o, lse = window_attention(q, k, v, "token", 1, 700, 3, 950, return_lse=True)
+    finally:
+        ext().attn_fwd_set_kv_splits(prev)
+    assert torch.isfinite(lse).all() and torch.isfinite(o).all()
+    # weights and output in bf16 (half a step, 2^-8, each), fp32 sums under 2^-12
+    assert (o.abs().amax((0, 1)) <= v.abs().amax((0, 1)).float() * (1 + 2.0 ** -8) ** 2 * (1 + 2.0 ** -12)).all()
+
+
 def test_second_derivative_in_a_sum_is_refused():
     """A second derivative through the operator raises, also where other terms have one."""
     from drivedit_b200.ops.window_attention import window_attention
@@ -81,11 +98,11 @@ def _cache(L=1, H=2, P=64, **kw):
 def _check_rows(c, seq, o, lse, q, window=0, sinks=0):
     """Each row against 64 bits, its bound from the keys that it sees alone.
 
-    bf16 output: half a step, 2^-8 of the value. Weights in fp16: half a step, 2^-11 of each,
-    or half the smallest number, 2^-25, where 2^7 stands for a weight as large as the largest
-    (or for one whose product with its page's scale is); a weight that becomes zero is off by
-    itself. fp32 scores of 64 products, exponentials and sums: 2^-12 in all at score
-    magnitudes up to 2^6, in proportion above."""
+    bf16 output: half a step, 2^-8 of the computed value, which is off itself. Weights in fp16:
+    half a step, 2^-11 of each, or half the smallest number, 2^-25, where 2^7 stands for a
+    weight as large as the largest (or for one whose product with its page's scale is); a
+    weight that becomes zero is off by itself. fp32 scores of 64 products, exponentials and
+    sums: 2^-12 in all at score magnitudes up to 2^6, in proportion above."""
     n, G, st = q.shape[0], q.shape[1] // c.n_heads, c._seqs[seq]
     S = st.length + n
     k, v = (x.double().repeat_interleave(G, 1) for x in c._values(0, st, S))
@@ -106,7 +123,8 @@ def _check_rows(c, seq, o, lse, q, window=0, sinks=0):
     step = torch.maximum(p.amax(-1, keepdim=True), (p * vs.T[:, None]).amax(-1, keepdim=True) / vs.T[:, None])
     lost = torch.einsum("hts,shd->thd", torch.minimum(p, 2.0 ** -32 * step), v.abs())
     rel = (2.0 ** -11 + 2.0 ** -12 * (mag.T * 2.0 ** -6).clamp(min=1.0))[..., None]
-    bound = 2.0 ** -8 * ref.abs() + rel * mean + lost + 1e-37
+    off = rel * mean + lost
+    bound = 2.0 ** -8 * (ref.abs() + off) + off + 1e-37
     err = (o.double() - ref).abs()
     assert torch.isfinite(o).all() and (err <= bound).all(), (float((err / bound).max()), (err / bound).amax((1, 2)).argmax().item())
     lerr = (lse.double() - rl / math.log(2)).abs()
