@@ -150,7 +150,7 @@ class RolloutConfig:
     batch: int = 1
     tp: int = 1
     # "bf16": contiguous rolling buffers; "fp8": 8-bit pages (drivedit_b200.ops.kv_cache),
-    # half the memory (at the same speed), which also keep the first sink_frames frames visible
+    # half the memory (not more speed), which also keep the first sink_frames frames visible
     kv_cache: str = "bf16"
     sink_frames: int = 0
 

@@ -76,11 +76,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: 
     ``kv_pos_offset``. Rows that see no key are zero and keys that no query sees are
     left out; both get zero gradients, and what they hold has no effect on the others.
     Returns ``o`` (and, if asked, ``lse [B, H, T]``, log2 domain of the scaled scores, without
-    gradient). Scaled scores are fp32 and stay below 2^30 in magnitude; what that leaves of a
-    score's difference from the row's ``lse``, 2^-24 of it, is a gradient's error too. dQ is summed in fp32 in no fixed order: equal backward passes may differ in dq
-    by a rounding of bf16. A second derivative raises on CUDA. A backward pass is captured
-    into a graph only when no autograd graph of the same leaves made on the default stream is
-    alive (refused otherwise)."""
+    gradient). On CUDA scaled scores are fp32 and have to stay below 2^30 in magnitude, or
+    rows become NaN; the backward pass makes each weight from its score and ``lse``, so that
+    scores of magnitude M leave it a relative error of M * 2^-24. dQ is summed in fp32 in no
+    fixed order: equal backward passes may differ in dq by a rounding of bf16. A second
+    derivative raises on CUDA. A backward pass is captured into a graph only when no autograd
+    graph of the same leaves made on the default stream is alive (refused otherwise)."""
     if q.is_cuda and q.numel() and k.numel():
         if sync_check() and torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v)):
             o, lse = _SyncChecked.apply(q, k, v, causal, tokens_per_frame, window, sinks, scale, q_pos_offset, kv_pos_offset)
