@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include "common/capture.h"
 #include "common/tma.h"
 #include "gemm/gemm.h"
 #include "fused/fused.h"
@@ -25,6 +26,8 @@
 #include "kvcache/kvcache.h"
 #include "vae/conv3d.h"
 #include "vae/groupnorm.h"
+
+void bind_rotary(pybind11::module_& m);  // rotary/rotary_py.cpp
 
 namespace {
 
@@ -1579,18 +1582,6 @@ class WindowAttention : public torch::autograd::Function<WindowAttention> {
   }
 };
 
-// A backward pass that is captured while an eager graph of the same leaf is alive ends the
-// process inside autograd: the leaf's accumulation node belongs to the default stream.
-void refuse_eager_leaf(const torch::Tensor& t) {
-  if (!t.requires_grad() || !t.is_leaf()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!node) return;
-  const auto s = node->stream();
-  TORCH_CHECK(!s || c10::cuda::CUDAStream(*s).stream() != nullptr,
-              "an autograd graph made on the default stream still uses this leaf: drop it before capturing a backward "
-              "pass, or warm up on another stream");
-}
-
 WindowMask window_check(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const std::string& causal,
                         int64_t tokens_per_frame, int64_t window, int64_t sinks, int64_t q_pos, int64_t kv_pos,
                         c10::optional<double> scale) {
@@ -1616,7 +1607,7 @@ std::vector<torch::Tensor> window_attention(const torch::Tensor& q, const torch:
   {
     const c10::cuda::CUDAGuard guard(q.device());
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None)
-      for (const auto* t : {&q, &k, &v}) refuse_eager_leaf(*t);
+      for (const auto* t : {&q, &k, &v}) ddb::refuse_eager_leaf(*t);
   }
   return WindowAttention::apply(q, k, v, m);
 }
@@ -1903,6 +1894,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_flat", &adamw_flat, "flat AdamW + bf16 copy");
   m.def("cast_bf16", &cast_bf16, "fp32 -> bf16 cast");
   m.def("sq_norm", &sq_norm, "sum of squares (fp32)");
+  bind_rotary(m);
   m.def("rope_rotate", &rope_rotate, "in-place rotary rotation of leading columns");
   m.def("attn_fwd", &attn_fwd, "tcgen05 flash attention forward (dense / frame-causal / sparse)");
   m.def("attn_fwd_set_trace", &attn_fwd_set_trace, "clock64 trace of one forward CTA (None: off)");

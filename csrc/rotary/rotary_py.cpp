@@ -1,0 +1,368 @@
+// Python bindings of the rotary kernels: checks, allocations and the autograd nodes.
+#include <torch/extension.h>
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include "../common/capture.h"
+#include "../common/tma.h"
+#include "rotary.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+// How a call rotates: the table, the tokens' positions, and the layout by name.
+struct Rotation {
+  OptTensor table, positions;
+  int64_t offset = 0;
+  std::string layout = "interleaved";
+  bool inverse = false;
+};
+
+ddb::RotLayout layout_of(const Rotation& r) {
+  ddb::RotLayout l;
+  l.in_halves = r.layout == "half" || (r.layout == "split" && r.inverse);
+  l.out_halves = r.layout == "half" || (r.layout == "split" && !r.inverse);
+  return l;
+}
+
+// x is [B, T, H, D], or [T, H, D]
+Tensor four(const Tensor& x) { return x.dim() == 3 ? x.unsqueeze(0) : x; }
+
+void check_heads(const Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_VALUE(x.dim() == 4 || x.dim() == 3, name, " must be [B, T, H, D] or [T, H, D], got ", x.sizes());
+  TORCH_CHECK_VALUE(x.scalar_type() == torch::kBFloat16 || x.scalar_type() == torch::kHalf || x.scalar_type() == torch::kFloat, name,
+                    " must be bfloat16, float16 or float32 on CUDA, got ", x.scalar_type());
+  const auto D = x.size(-1);
+  TORCH_CHECK_VALUE(D >= 2 && D <= 256 && D % 2 == 0, "heads must have an even number of channels up to 256, got ", D);
+  const auto y = four(x);
+  TORCH_CHECK_VALUE(y.size(0) * y.size(1) * y.size(2) < (1L << 30), "at most 2^30 heads of tokens in a call");
+}
+
+void check_rotation(const Rotation& r, const Tensor& x0) {
+  const auto x = four(x0);
+  TORCH_CHECK_VALUE(r.layout == "interleaved" || r.layout == "half" || r.layout == "split", "layout must be interleaved, half or split, got '",
+                    r.layout, "'");
+  if (!r.table) {
+    TORCH_CHECK_VALUE(!r.positions && r.offset == 0, "positions need a table");
+    return;
+  }
+  const auto& tab = *r.table;
+  TORCH_CHECK_VALUE(tab.dim() == 3 && tab.size(2) == 2 && tab.scalar_type() == torch::kFloat && tab.is_contiguous() &&
+                        2 * tab.size(1) <= x.size(3),
+                    "table must be contiguous float32 [positions, rotated channels / 2, 2] for heads of ", x.size(3), ", got ", tab.sizes());
+  TORCH_CHECK_VALUE(tab.device() == x.device(), "table is on ", tab.device(), ", the heads on ", x.device());
+  TORCH_CHECK_VALUE(!tab.requires_grad(), "the table has no gradient");
+  if (r.positions) {
+    const auto& p = *r.positions;
+    TORCH_CHECK_VALUE(r.offset == 0, "positions and offset exclude each other");
+    TORCH_CHECK_VALUE(p.scalar_type() == torch::kInt || p.scalar_type() == torch::kLong, "positions must be int32 or int64, got ", p.scalar_type());
+    TORCH_CHECK_VALUE(p.device() == x.device(), "positions are on ", p.device(), ", the heads on ", x.device());
+    TORCH_CHECK_VALUE((p.dim() == 1 && p.size(0) == x.size(1)) ||
+                          (p.dim() == 2 && x0.dim() == 4 && (p.size(0) == x.size(0) || p.size(0) == 1) && p.size(1) == x.size(1)),
+                      "positions must be [T] or [B, T], got ", p.sizes(), " for heads ", x0.sizes());
+  } else {
+    TORCH_CHECK_VALUE(r.offset >= 0 && r.offset <= tab.size(0) && x.size(1) <= tab.size(0) - r.offset, "the table has ", tab.size(0),
+                      " positions, the call needs ", x.size(1), " from ", r.offset);
+  }
+}
+
+ddb::RotType type_of(const Tensor& x) {
+  return x.scalar_type() == torch::kBFloat16 ? ddb::RotType::kBf16 : x.scalar_type() == torch::kHalf ? ddb::RotType::kF16 : ddb::RotType::kF32;
+}
+
+// Contiguous channels (a copy where they are not)
+Tensor channels(const Tensor& x) {
+  return x.stride(-1) == 1 || x.numel() == 0 ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+struct Strides {
+  long sb, st, sh;
+};
+Strides strides(const Tensor& x) {  // of axes of one entry the stride does not matter
+  return {x.size(0) > 1 ? x.stride(0) : 0, x.size(1) > 1 ? x.stride(1) : 0, x.size(2) > 1 ? x.stride(2) : 0};
+}
+
+ddb::RotArgs args_of(const Rotation& r, const Tensor& x) {
+  ddb::RotArgs a;
+  a.type = type_of(x);
+  a.layout = layout_of(r);
+  a.inverse = r.inverse;
+  a.B = x.size(0);
+  a.T = x.size(1);
+  a.D = x.size(3);
+  if (r.table) {
+    a.R = 2 * r.table->size(1);
+    a.table = reinterpret_cast<const float2*>(r.table->data_ptr<float>());
+    a.places = r.table->size(0);
+  }
+  a.offset = r.offset;
+  if (r.positions) {
+    const auto& p = *r.positions;
+    a.pos = p.data_ptr();
+    a.pos64 = p.scalar_type() == torch::kLong;
+    a.pos_sb = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+    a.pos_st = p.stride(-1);
+  }
+  return a;
+}
+
+void put_x(ddb::RotTensor& t, const Tensor& x) {
+  const auto s = strides(x);
+  t.x = x.data_ptr();
+  t.x_sb = s.sb, t.x_st = s.st, t.x_sh = s.sh;
+  t.H = x.size(2);
+}
+void put_y(ddb::RotTensor& t, const Tensor& y) {
+  const auto s = strides(y);
+  t.y = y.data_ptr();
+  t.y_sb = s.sb, t.y_st = s.st, t.y_sh = s.sh;
+}
+void put_g(ddb::RotTensor& t, const Tensor& g) {
+  const auto s = strides(g);
+  t.g = g.data_ptr();
+  t.g_sb = s.sb, t.g_st = s.st, t.g_sh = s.sh;
+}
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+void check_inplace(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.numel() == 0 || x.stride(-1) == 1, name, " must have contiguous channels to be written in place");
+  // of an expanded axis several tokens or heads would be one place
+  for (int i = 0; i < x.dim() - 1; ++i) TORCH_CHECK_VALUE(x.size(i) <= 1 || x.stride(i) != 0, name, " has entries that share memory");
+}
+
+// What was overwritten no longer is what an autograd graph may have kept of it
+void overwritten(const Tensor& x) {
+  if (!x.is_inference()) torch::autograd::impl::bump_version(x);
+}
+
+// ---------------------------------------------------------------- rotary
+Tensor rotate(const Tensor& x0, const Rotation& r, bool inplace) {
+  const c10::cuda::CUDAGuard guard(x0.device());
+  if (inplace) check_inplace(x0, "x");
+  const auto x = channels(x0);
+  auto y = inplace ? x0 : torch::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return y;
+  const auto x4 = four(x), y4 = four(y);
+  auto a = args_of(r, x4);
+  put_x(a.t[0], x4);
+  put_y(a.t[0], y4);
+  ddb::rot_forward(a, stream());
+  if (inplace) overwritten(x0);
+  return y;
+}
+
+class Rotary : public torch::autograd::Function<Rotary> {
+ public:
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Rotation& r) {
+    ctx->save_for_backward({r.table ? *r.table : Tensor(), r.positions ? *r.positions : Tensor()});
+    ctx->saved_data["offset"] = r.offset;
+    ctx->saved_data["layout"] = r.layout;
+    ctx->saved_data["inverse"] = r.inverse;
+    ctx->set_materialize_grads(false);
+    return rotate(x, r, false);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    const auto s = ctx->get_saved_variables();
+    Rotation r;
+    if (s[0].defined()) r.table = s[0];
+    if (s[1].defined()) r.positions = s[1];
+    r.offset = ctx->saved_data["offset"].toInt();
+    r.layout = ctx->saved_data["layout"].toStringRef();
+    r.inverse = !ctx->saved_data["inverse"].toBool();
+    // linear in the gradient: a second derivative is one more rotation
+    if (at::GradMode::is_enabled() && grads[0].requires_grad()) return {Rotary::apply(grads[0], r), Tensor()};
+    return {rotate(grads[0], r, false), Tensor()};
+  }
+};
+
+Tensor rotary(const Tensor& x, const Tensor& table, const OptTensor& positions, int64_t offset, const std::string& layout, bool inverse,
+              bool inplace) {
+  check_heads(x, "x");
+  const Rotation r{table, positions, offset, layout, inverse};
+  check_rotation(r, x);
+  if (!at::GradMode::is_enabled() || !x.requires_grad()) return rotate(x, r, inplace);
+  TORCH_CHECK_VALUE(!inplace, "x requires a gradient: it cannot be rotated in place");
+  {
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (ddb::capturing()) ddb::refuse_eager_leaf(x);
+  }
+  return Rotary::apply(x, r);
+}
+
+// ---------------------------------------------------------------- norms of queries and keys, rotated
+OptTensor weight32(const OptTensor& w) {
+  if (!w) return w;
+  return w->detach().to(torch::kFloat).contiguous();
+}
+
+void check_qk(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const Rotation& r, double eps) {
+  check_heads(q, "q");
+  check_heads(k, "k");
+  TORCH_CHECK_VALUE(q.dim() == k.dim() && q.size(0) == k.size(0) && (q.dim() == 3 || q.size(1) == k.size(1)) && q.size(-1) == k.size(-1),
+                    "q and k must agree in batch, tokens and channels, got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.device() == k.device(), "q and k must be of one type and on one device");
+  TORCH_CHECK_VALUE(eps >= 1e-30 && std::isfinite(eps), "eps must be positive (at least 1e-30)");
+  for (const auto* w : {&wq, &wk})
+    if (*w)
+      TORCH_CHECK_VALUE((*w)->dim() == 1 && (*w)->size(0) == q.size(-1) && (*w)->is_floating_point() && (*w)->device() == q.device(),
+                        "a norm's weight must be floating-point [", q.size(-1), "] on the heads' device");
+  check_rotation(r, q);
+}
+
+std::vector<Tensor> qk_forward(const Tensor& q0, const Tensor& k0, const OptTensor& wq, const OptTensor& wk, const Rotation& r, double eps,
+                               bool inplace) {
+  const c10::cuda::CUDAGuard guard(q0.device());
+  if (inplace) check_inplace(q0, "q"), check_inplace(k0, "k");
+  const auto q = channels(q0), k = channels(k0);
+  std::vector<Tensor> out = {inplace ? q0 : torch::empty(q.sizes(), q.options()), inplace ? k0 : torch::empty(k.sizes(), k.options())};
+  if (q.numel() == 0 && k.numel() == 0) return out;
+  const auto w0 = weight32(wq), w1 = weight32(wk);
+  const auto q4 = four(q), k4 = four(k);
+  auto a = args_of(r, q4);
+  a.n = 2;
+  a.norm = true;
+  a.eps = static_cast<float>(eps);
+  put_x(a.t[0], q4), put_x(a.t[1], k4);
+  put_y(a.t[0], four(out[0])), put_y(a.t[1], four(out[1]));
+  if (w0) a.t[0].w = w0->data_ptr<float>();
+  if (w1) a.t[1].w = w1->data_ptr<float>();
+  ddb::rot_forward(a, stream());
+  if (inplace) overwritten(q0), overwritten(k0);
+  return out;
+}
+
+// dq, dk into the given tensors (which may be the gradients' own), the weights' gradients into
+// given fp32 ones (or none), added to what they hold if `add`. An undefined gradient leaves its tensor
+// out.
+void qk_backward(const Tensor& q0, const Tensor& k0, const OptTensor& wq, const OptTensor& wk, const Rotation& r, double eps, const Tensor& gq0,
+                 const Tensor& gk0, const Tensor& dq, const Tensor& dk, const OptTensor& dwq, const OptTensor& dwk, bool add) {
+  const c10::cuda::CUDAGuard guard(q0.device());
+  const auto q = channels(four(q0)), k = channels(four(k0));
+  const auto w0 = weight32(wq), w1 = weight32(wk);
+  auto a = args_of(r, q);
+  a.n = 0;
+  a.norm = true;
+  a.eps = static_cast<float>(eps);
+  Tensor keep[2];
+  auto tensor = [&](const Tensor& x, const OptTensor& w, const Tensor& g0, const Tensor& dx, const OptTensor& dw) {
+    if (!g0.defined()) return;
+    TORCH_CHECK_VALUE(four(g0).sizes() == x.sizes() && g0.scalar_type() == x.scalar_type() && four(dx).sizes() == x.sizes() &&
+                          dx.scalar_type() == x.scalar_type() && g0.device() == x.device() && dx.device() == x.device(),
+                      "gradients must be like their tensors");
+    check_inplace(dx, "a gradient");
+    if (dw)
+      TORCH_CHECK_VALUE(dw->scalar_type() == torch::kFloat && dw->is_contiguous() && dw->dim() == 1 && dw->size(0) == x.size(3) &&
+                            dw->device() == x.device(), "a weight's gradient must be contiguous float32 [", x.size(3), "]");
+    auto& t = a.t[a.n];
+    keep[a.n] = channels(four(g0));
+    put_x(t, x);
+    put_g(t, keep[a.n]);
+    put_y(t, four(dx));
+    if (w) t.w = w->data_ptr<float>();
+    if (dw) t.dw = dw->data_ptr<float>();
+    t.dw_add = add;
+    ++a.n;
+  };
+  tensor(q, w0, gq0, dq, dwq);
+  tensor(k, w1, gk0, dk, dwk);
+  if (a.n == 0) return;
+  const auto part = torch::empty({ddb::rot_parts(a)}, q.options().dtype(torch::kFloat));
+  a.part = part.data_ptr<float>();
+  ddb::rot_backward(a, stream());
+}
+
+class QkNormRotary : public torch::autograd::Function<QkNormRotary> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& wq,
+                                                const OptTensor& wk, const Rotation& r, double eps) {
+    ctx->save_for_backward({q, k, wq ? *wq : Tensor(), wk ? *wk : Tensor(), r.table ? *r.table : Tensor(), r.positions ? *r.positions : Tensor()});
+    ctx->saved_data["offset"] = r.offset;
+    ctx->saved_data["layout"] = r.layout;
+    ctx->saved_data["eps"] = eps;
+    ctx->set_materialize_grads(false);
+    auto out = qk_forward(q, k, wq, wk, r, eps, false);
+    return {out[0], out[1]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    Rotation r;
+    if (s[4].defined()) r.table = s[4];
+    if (s[5].defined()) r.positions = s[5];
+    r.offset = ctx->saved_data["offset"].toInt();
+    r.layout = ctx->saved_data["layout"].toStringRef();
+    const c10::cuda::CUDAGuard guard(s[0].device());
+    OptTensor w[2], dw[2];
+    for (int i = 0; i < 2; ++i) {
+      if (grads[i].defined()) out[i] = torch::empty(s[i].sizes(), s[i].options());
+      if (!s[2 + i].defined()) continue;
+      w[i] = s[2 + i];
+      if (grads[i].defined() && w[i]->requires_grad()) dw[i] = torch::empty(w[i]->sizes(), w[i]->options().dtype(torch::kFloat));
+    }
+    qk_backward(s[0], s[1], w[0], w[1], r, ctx->saved_data["eps"].toDouble(), grads[0], grads[1], out[0], out[1], dw[0], dw[1], false);
+    for (int i = 0; i < 2; ++i)
+      if (dw[i]) out[2 + i] = dw[i]->to(w[i]->scalar_type());
+    if (!at::GradMode::is_enabled()) return out;
+    // create_graph: the kernels leave no graph, so a second derivative through these raises, on
+    // the way to whatever the first one went to, instead of missing terms
+    const auto error = std::make_shared<torch::autograd::Error>("qk_norm_rotary has no second derivative on CUDA",
+                                                                torch::autograd::edge_list(torch::autograd::get_current_node()->next_edges()));
+    for (auto& t : out)
+      if (t.defined()) torch::autograd::create_gradient_edge(t, error);
+    return out;
+  }
+};
+
+std::vector<Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table,
+                                   const OptTensor& positions, int64_t offset, const std::string& layout, double eps, bool inplace) {
+  const Rotation r{table, positions, offset, layout, false};
+  check_qk(q, k, wq, wk, r, eps);
+  bool grad = q.requires_grad() || k.requires_grad();
+  for (const auto* w : {&wq, &wk}) grad = grad || (*w && (*w)->requires_grad());
+  if (!at::GradMode::is_enabled() || !grad) return qk_forward(q, k, wq, wk, r, eps, inplace);
+  TORCH_CHECK_VALUE(!inplace, "something requires a gradient: q and k cannot be overwritten");
+  {
+    const c10::cuda::CUDAGuard guard(q.device());
+    if (ddb::capturing()) {
+      for (const auto* t : {&q, &k}) ddb::refuse_eager_leaf(*t);
+      for (const auto* w : {&wq, &wk})
+        if (*w) ddb::refuse_eager_leaf(**w);
+    }
+  }
+  const auto out = QkNormRotary::apply(q, k, wq, wk, r, eps);
+  return {out[0], out[1]};
+}
+
+std::vector<Tensor> qk_fwd_py(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table,
+                              const OptTensor& positions, int64_t offset, const std::string& layout, double eps) {
+  const Rotation r{table, positions, offset, layout, false};
+  check_qk(q, k, wq, wk, r, eps);
+  return qk_forward(q, k, wq, wk, r, eps, false);
+}
+
+void qk_bwd_py(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table, const OptTensor& positions,
+               int64_t offset, const std::string& layout, double eps, const OptTensor& gq, const OptTensor& gk, const OptTensor& dq,
+               const OptTensor& dk, const OptTensor& dwq, const OptTensor& dwk, bool add) {
+  const Rotation r{table, positions, offset, layout, false};
+  check_qk(q, k, wq, wk, r, eps);
+  auto or_none = [](const OptTensor& t) { return t ? *t : Tensor(); };
+  TORCH_CHECK_VALUE((!gq || dq) && (!gk || dk), "a gradient needs a place");
+  qk_backward(q, k, wq, wk, r, eps, or_none(gq), or_none(gk), or_none(dq), or_none(dk), dwq, dwk, add);
+}
+
+}  // namespace
+
+void bind_rotary(pybind11::module_& m) {
+  m.def("rotary", &rotary, "differentiable rotation of heads by their tokens' positions");
+  m.def("qk_norm_rotary", &qk_norm_rotary, "differentiable norms of queries and keys, rotated");
+  m.def("qk_norm_rotary_fwd", &qk_fwd_py, "its forward, for callers with a backward of their own");
+  m.def("qk_norm_rotary_bwd", &qk_bwd_py, "its backward, into given gradients");
+}

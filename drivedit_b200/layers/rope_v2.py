@@ -278,6 +278,14 @@ class RoPELayerV2(nn.Module):
         """Multiplier of the attention logits under YaRN (1.0 otherwise)."""
         return self._yarn_attention_scale
 
+    def table(self, seq_len: int, device=None) -> torch.Tensor:
+        """(cos, sin) of the first ``seq_len`` positions ``[seq_len, dim/2, 2]`` in float32, as
+        :func:`drivedit_b200.ops.rotary.rotary` takes them (its layout "split" writes what
+        ``forward`` does)."""
+        n = max(seq_len, self.config.original_max_seq_len if self.config.dynamic_ntk else self.config.max_seq_len)
+        s, c, _ = _freqs_for(self.config, n, device)
+        return torch.stack([c[:seq_len], s[:seq_len]], -1).contiguous()
+
     def _tables(self, end: int, seq_len: Optional[int], device, dtype) -> SinCos:
         n = seq_len or end
         if self.config.dynamic_ntk and n > self.config.original_max_seq_len:

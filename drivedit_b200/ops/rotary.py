@@ -1,0 +1,190 @@
+"""Rotary positions of heads, and norms of queries and keys for each head with the rotation in
+the same pass; forward and backward.
+
+A table ``[positions, R/2, 2]`` (float32, contiguous) holds (cos, sin) of each pair's angle at each
+position: :func:`drivedit_b200.layers.rope.rope_table` of any angles (plain, NTK, YaRN,
+interpolated, 3-D), :meth:`RoPE3D.table` or :meth:`RoPELayerV2.table`. The first ``R`` channels
+of a head are rotated, the others pass. A pair (a, b) becomes (a cos - b sin, a sin + b cos);
+its channels lie, by ``layout``,
+
+* "interleaved": side by side, ``(2i, 2i + 1)`` (this framework's models);
+* "half": in two halves, ``(i, i + R/2)``;
+* "split": read side by side and written as halves (:func:`layers.rope.rope_apply`).
+
+CUDA tensors (bfloat16, float16, float32; heads of an even size up to 256; any strides) run the
+sm_100a kernels (``csrc/rotary``), fp32 inside and rounded once; CPU tensors the PyTorch
+statements below. Token t is at row ``offset + t`` of the table, or at ``positions``
+(int32 or int64, ``[T]`` or ``[B, T]``). A position outside the table raises on the CPU; on CUDA
+it is recorded in the device's status word (:func:`ops._ext.check_device_status` raises) and the
+token's rotated channels become NaN. With ``inplace`` (only where nothing requires a gradient)
+the results are written over the inputs. A backward pass is captured into a graph only when no
+autograd graph of the same leaves made on the default stream is alive (refused otherwise).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from ._ext import ext, sync_check
+
+LAYOUTS = ("interleaved", "half", "split")
+
+
+class _SyncChecked(torch.autograd.Function):
+    """The norms for the sync-check mode, which brackets entry points called from Python: the
+    extension's own autograd node calls its backward behind it."""
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, table, positions, *args):
+        ctx.save_for_backward(q, k, wq, wk, table, positions)
+        ctx.args = args
+        ctx.set_materialize_grads(False)
+        return tuple(ext().qk_norm_rotary_fwd(q, k, wq, wk, table, positions, *args))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, table, positions = ctx.saved_tensors
+        heads = [None if g is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x, g in ((q, gq), (k, gk))]
+        weights = [None if g is None or w is None else torch.empty(w.shape, device=w.device) for w, g in ((wq, gq), (wk, gk))]
+        ext().qk_norm_rotary_bwd(q, k, wq, wk, table, positions, *ctx.args, gq, gk, *heads, *weights, False)
+        weights = [d if d is None else d.to(w.dtype) for d, w in zip(weights, (wq, wk))]
+        return (*heads, *weights, None, None, *(None for _ in ctx.args))
+
+
+class _SyncCheckedRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, positions, offset, layout, inverse):
+        ctx.save_for_backward(table, positions)
+        ctx.args = offset, layout, inverse
+        return ext().rotary(x, table, positions, offset, layout, inverse, False)
+
+    @staticmethod
+    def backward(ctx, g):
+        table, positions = ctx.saved_tensors
+        offset, layout, inverse = ctx.args
+        return (_SyncCheckedRotary.apply(g, table, positions, offset, layout, not inverse), *(None,) * 5)
+
+
+def _check(x, name):
+    """The extension's checks, for the PyTorch statements."""
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [B, T, H, D] or [T, H, D], got {tuple(x.shape)}")
+    if not x.is_floating_point():
+        raise ValueError(f"{name} must be floating-point, got {x.dtype}")
+    D = x.shape[-1]
+    if not (2 <= D <= 256 and D % 2 == 0):
+        raise ValueError(f"heads must have an even number of channels up to 256, got {D}")
+
+
+def _rows(x, table, positions, offset, layout):
+    """(cos, sin) of each token of ``x``, ``[.., T, 1, R/2, 2]``."""
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be interleaved, half or split, got {layout!r}")
+    if table is None:
+        if positions is not None or offset:
+            raise ValueError("positions need a table")
+        return None
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous() \
+            or 2 * table.shape[1] > x.shape[-1]:
+        raise ValueError(f"table must be contiguous float32 [positions, rotated channels / 2, 2] for heads of {x.shape[-1]}, "
+                         f"got {tuple(table.shape)}")
+    if table.device != x.device:
+        raise ValueError(f"table is on {table.device}, the heads on {x.device}")
+    if table.requires_grad:
+        raise ValueError("the table has no gradient")
+    T = x.shape[-3]
+    if positions is None:
+        if offset < 0 or T > table.shape[0] - offset:
+            raise ValueError(f"the table has {table.shape[0]} positions, the call needs {T} from {offset}")
+        return table[offset:offset + T, None]
+    if offset:
+        raise ValueError("positions and offset exclude each other")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if positions.device != x.device:
+        raise ValueError(f"positions are on {positions.device}, the heads on {x.device}")
+    if not (positions.shape == (T,) or (x.dim() == 4 and positions.dim() == 2 and positions.shape[0] in (1, x.shape[0])
+                                        and positions.shape[1] == T)):
+        raise ValueError(f"positions must be [T] or [B, T], got {tuple(positions.shape)} for heads {tuple(x.shape)}")
+    p = positions.long()
+    if p.numel() and not (0 <= int(p.min()) and int(p.max()) < table.shape[0]):
+        raise IndexError(f"a position lies outside the table's {table.shape[0]}")
+    return table[p].unsqueeze(-3)
+
+
+def _rotate(x, cs, layout, inverse):
+    R = 2 * cs.shape[-2]
+    c, s = cs[..., 0], cs[..., 1]
+    s = -s if inverse else s
+    halves = layout == "half" or (layout == "split" and inverse)
+    a, b = (x[..., :R // 2], x[..., R // 2:R]) if halves else (x[..., 0:R:2], x[..., 1:R:2])
+    y, z = a * c - b * s, a * s + b * c
+    halves = layout == "half" or (layout == "split" and not inverse)
+    y = torch.cat([y, z], -1) if halves else torch.stack([y, z], -1).flatten(-2)
+    return torch.cat([y, x[..., R:]], -1) if R < x.shape[-1] else y
+
+
+def _wide(x):
+    return x.to(torch.promote_types(x.dtype, torch.float32))
+
+
+def _result(y, x, inplace):
+    return x.copy_(y) if inplace else y.to(x.dtype)
+
+
+def _writable(inplace, *inputs):
+    """Whether nothing requires a gradient that an overwritten input would lose."""
+    if inplace and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        raise ValueError("something requires a gradient: the inputs cannot be overwritten")
+
+
+def rotary(x: torch.Tensor, table: torch.Tensor, positions: Optional[torch.Tensor] = None, offset: int = 0,
+           layout: str = "interleaved", inverse: bool = False, inplace: bool = False) -> torch.Tensor:
+    """``x [B, T, H, D]`` (or packed ``[T, H, D]``) with its heads rotated; differentiable in ``x``, twice
+    and more. ``inverse`` rotates by the negative angle (and "split" back from halves to side
+    by side): the backward pass of the call without it."""
+    if x.is_cuda:
+        if sync_check() and torch.is_grad_enabled() and x.requires_grad and not inplace:
+            return _SyncCheckedRotary.apply(x, table, positions, offset, layout, inverse)
+        return ext().rotary(x, table, positions, offset, layout, inverse, inplace)
+    _check(x, "x")
+    cs = _rows(x, table, positions, offset, layout)
+    _writable(inplace, x)
+    return _result(_rotate(_wide(x), cs, layout, inverse), x, inplace)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None, offset: int = 0, layout: str = "interleaved",
+                   eps: float = 1e-6, inplace: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Every head of ``q [B, T, H, D]`` and ``k [B, T, KH, D]`` (or packed ``[T, H, D]``) divided by the root
+    of its mean square plus ``eps``, times ``q_weight`` / ``k_weight`` ``[D]`` (None: ones), then rotated
+    (``table`` None: not at all). One launch for both, differentiable in the heads and weights; the
+    weights' gradients are summed in a fixed order. A second derivative raises on CUDA."""
+    if q.is_cuda:
+        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+        if sync_check() and grad and not inplace:
+            return _SyncChecked.apply(q, k, q_weight, k_weight, table, positions, offset, layout, eps)
+        return tuple(ext().qk_norm_rotary(q, k, q_weight, k_weight, table, positions, offset, layout, eps, inplace))
+    _check(q, "q"), _check(k, "k")
+    if (q.dim(), q.shape[:-2], q.shape[-1]) != (k.dim(), k.shape[:-2], k.shape[-1]):
+        raise ValueError(f"q and k must agree in batch, tokens and channels, got {tuple(q.shape)} and {tuple(k.shape)}")
+    if q.dtype != k.dtype or q.device != k.device:
+        raise ValueError("q and k must be of one type and on one device")
+    if not (eps >= 1e-30 and math.isfinite(eps)):
+        raise ValueError("eps must be positive (at least 1e-30)")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (q.shape[-1],) or not w.is_floating_point() or w.device != q.device):
+            raise ValueError(f"a norm's weight must be floating-point [{q.shape[-1]}] on the heads' device")
+    cs = _rows(q, table, positions, offset, layout)
+    _writable(inplace, q, k, q_weight, k_weight)
+    out = []
+    for x, w in ((q, q_weight), (k, k_weight)):
+        h = _wide(x)
+        h = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
+        h = h if w is None else h * w.to(h.dtype)
+        out.append(_result(h if cs is None else _rotate(h, cs, layout, False), x, inplace))
+    return tuple(out)

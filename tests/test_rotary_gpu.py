@@ -1,0 +1,436 @@
+"""Rotary positions and norms of queries and keys on the GPU, forward and backward, against the
+formula in 64 bits and against differences."""
+import math
+
+import pytest
+import torch
+
+from test_rotary_cpu import refusals
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+TINY = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -126}  # below: absolute
+
+
+def _table(n, pairs):
+    a = torch.rand(n, pairs, dtype=torch.float64, device="cuda") * 6.28
+    return torch.stack([a.cos(), a.sin()], -1).float().contiguous()
+
+
+def _heads(B, T, H, D, dtype, how):
+    """Heads with the strides that callers have: columns of a projection, heads before tokens, an
+    odd base, channels apart, one sample for all."""
+    if how == "packed":
+        return torch.randn(B, T, H + 3, D, device="cuda").to(dtype)[:, :, 2:2 + H]
+    if how == "heads first":
+        return torch.randn(B, H, T, D, device="cuda").to(dtype).transpose(1, 2)
+    if how == "odd base":
+        return torch.randn(B * T * H * D + 1, device="cuda").to(dtype)[1:].view(B, T, H, D)
+    if how == "channels apart":
+        return torch.randn(B, T, D, H, device="cuda").to(dtype).transpose(2, 3)
+    if how == "expanded":
+        return torch.randn(1, T, H, D, device="cuda").to(dtype).expand(B, T, H, D)
+    return torch.randn(B, T, H, D, device="cuda").to(dtype)
+
+
+def _pairs(layout, R, D):
+    """Channels of each pair as they are read and written, the passing ones paired as they lie."""
+    i = torch.arange(R // 2, device="cuda")
+    side, halves = torch.stack([2 * i, 2 * i + 1]), torch.stack([i, i + R // 2])
+    rest = torch.arange(R, D, device="cuda").view(-1, 2).T
+    read = halves if layout == "half" else side
+    write = side if layout == "interleaved" else halves
+    return torch.cat([read, rest], 1), torch.cat([write, rest], 1)
+
+
+def _turn(x, cs, layout, R, back=False, size=False):
+    """The rotation in 64 bits (``back``: transposed; ``size``: of magnitudes, a bound on its terms)."""
+    D = x.shape[-1]
+    read, write = _pairs(layout, R, D)
+    if back:
+        read, write = write, read
+    c = torch.cat([cs[..., 0], torch.ones(*cs.shape[:-2], (D - R) // 2, device="cuda", dtype=torch.float64)], -1)
+    s = torch.cat([cs[..., 1], torch.zeros(*cs.shape[:-2], (D - R) // 2, device="cuda", dtype=torch.float64)], -1)
+    s = -s if back else s
+    a, b = x[..., read[0]], x[..., read[1]]
+    y = torch.empty_like(x)
+    if size:
+        c, s, a, b = c.abs(), s.abs(), a.abs(), b.abs()
+        y[..., write[0]] = a * c + b * s
+    else:
+        y[..., write[0]] = a * c - b * s
+    y[..., write[1]] = a * s + b * c
+    return y
+
+
+def _rounded(x, dtype):
+    return torch.finfo(dtype).eps / 2 * x.abs() + TINY[dtype]
+
+
+def _rows(tab, pos, B, T, offset):
+    p = torch.arange(offset, offset + T, device="cuda") if pos is None else pos.long()
+    return tab.double()[p.expand(B, T)][:, :, None]
+
+
+SHAPES = [
+    # B, T, H, KH, D, R: heads of whole 16s, then others
+    (2, 33, 3, 1, 64, 64), (1, 1, 1, 1, 64, 64), (3, 50, 12, 4, 128, 64), (2, 17, 5, 5, 96, 48), (2, 9, 2, 1, 256, 256), (1, 300, 7, 7, 32, 16),
+    (5, 1, 4, 2, 48, 32), (2, 40, 3, 3, 64, 0), (2, 65, 3, 1, 72, 40), (1, 31, 2, 2, 2, 2), (2, 20, 3, 1, 66, 64), (1, 70, 5, 1, 250, 100),
+    (3, 11, 2, 2, 80, 18), (1, 23, 2, 1, 130, 130), (4, 1003, 2, 1, 64, 32),
+]
+HOW = ["plain", "packed", "heads first", "odd base", "channels apart", "expanded"]
+
+
+def _positions(kind, B, T, n):
+    if kind == "none":
+        return None, 0
+    if kind == "offset":
+        return None, n - T
+    if kind == "tokens":
+        return torch.randint(0, n, (T,), device="cuda"), 0
+    if kind == "strided":
+        return torch.randint(0, n, (T, B, 2), device="cuda", dtype=torch.int32)[..., 1].T, 0
+    return torch.randint(0, n, (B, T), device="cuda"), 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["interleaved", "half", "split"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rotary(shape, layout, dtype):
+    from drivedit_b200.ops.rotary import rotary
+    B, T, H, _, D, R = shape
+    tab = _table(T + 40, R // 2)
+    for how, kind in zip(HOW, ["none", "offset", "tokens", "each", "strided", "each"]):
+        x = _heads(B, T, H, D, dtype, how).detach().requires_grad_()
+        pos, offset = _positions(kind, B, T, T + 40)
+        dy = _heads(B, T, H, D, dtype, how)
+        y = rotary(x, tab, pos, offset, layout)
+        dx, = torch.autograd.grad(y, x, dy)
+        cs = _rows(tab, pos, B, T, offset)
+        for got, src, back in ((y, x, False), (dx, dy, True)):
+            src = src.detach().double()
+            want = _turn(src, cs, layout, R, back)
+            # two products and their sum, each rounded to 32 bits, then one rounding
+            bound = 2.0 ** -23 * _turn(src, cs, layout, R, back, size=True) + _rounded(want, dtype) * (1 + 2.0 ** -20)
+            assert got.dtype == dtype and got.shape == want.shape
+            assert ((got.detach().double() - want).abs() <= bound).all(), (how, kind, back)
+        assert torch.equal(rotary(dy, tab, pos, offset, layout, inverse=True), dx)
+        # the PyTorch statement, bit for bit
+        p = None if pos is None else pos.cpu()
+        assert torch.equal(rotary(x.detach().cpu(), tab.cpu(), p, offset, layout), y.detach().cpu())
+
+
+def _formula(x, w, dy, cs, layout, R, eps, dtype):
+    """y, dx, dw of one tensor in 64 bits, and a bound on each one's error.
+
+    In 32 bits a sum of D <= 256 squares is 16 in a row and a tree of 4, so r, behind a division,
+    a sum, a root and a reciprocal, is off by less than 16 * 2^-24 of itself, x r w by 18, and
+    what is rotated by 20 of its terms' magnitudes: E = 2^-19 covers each of them.
+      y:  E |.| + its rounding.  With g the rotated-back dy, u = g w, h = x r:
+      dw: E sum |g h|, and sums of N numbers, at most 64 in a row: 2^-18 sum |g h| more
+      dx: r (u - h m), m = mean(u h): 2 E r (|u| + |h| mean |u h|) + its rounding"""
+    E = 2.0 ** -19
+    x, dy = x.double(), dy.double()
+    w = torch.ones(x.shape[-1], device="cuda", dtype=torch.float64) if w is None else w.double()
+    r = 1 / torch.sqrt(x.square().mean(-1, keepdim=True) + eps)
+    h = x * r
+    y = _turn(h * w, cs, layout, R)
+    g, ga = _turn(dy, cs, layout, R, back=True), _turn(dy, cs, layout, R, back=True, size=True)
+    u, ua = g * w, ga * w.abs()
+    dx = r * (u - h * (u * h).mean(-1, keepdim=True))
+    dw = (g * h).sum((0, 1, 2))
+    return {
+        "y": (y, E * _turn(h * w, cs, layout, R, size=True) + _rounded(y, dtype) * (1 + 2.0 ** -18)),
+        "dx": (dx, 2 * E * r * (ua + h.abs() * (ua * h.abs()).mean(-1, keepdim=True)) + _rounded(dx, dtype) * (1 + 2.0 ** -18)),
+        "dw": (dw, (E + 2.0 ** -18) * (ga * h.abs()).sum((0, 1, 2)) + 2.0 ** -24 * dw.abs() + 1e-37),
+    }
+
+
+def _check(got, want):
+    for n, (x, bound) in want.items():
+        err = (got[n].detach().double() - x).abs()
+        assert got[n].shape == x.shape and (err <= bound).all(), (n, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["interleaved", "half", "split"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_norms(shape, layout, dtype):
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    B, T, H, KH, D, R = shape
+    tab = _table(T + 40, R // 2) if R else None
+    for i, (how, kind) in enumerate(zip(HOW, ["none", "offset", "tokens", "each", "strided", "each"])):
+        q, k = (_heads(B, T, n, D, dtype, how) * (4.0 ** (i - 2)) for n in (H, KH))
+        if i == 1:
+            q[0, 0, 0] = 0
+        q, k = (x.detach().requires_grad_() for x in (q, k))
+        wq = (1 + 0.3 * torch.randn(D, device="cuda")).requires_grad_()
+        wk = None if i == 2 else (1 + 0.3 * torch.randn(D, device="cuda")).bfloat16().requires_grad_()
+        pos, offset = _positions(kind, B, T, T + 40) if R else (None, 0)
+        gq, gk = (_heads(B, T, n, D, dtype, how) for n in (H, KH))
+        a, b = qk_norm_rotary(q, k, wq, wk, tab, pos, offset, layout, eps=1e-5)
+        leaves = [q, k, wq] + [wk] * (wk is not None)
+        got = torch.autograd.grad((a, b), leaves, (gq, gk))
+        cs = _rows(tab, pos, B, T, offset) if R else torch.zeros(B, T, 1, 0, 2, device="cuda", dtype=torch.float64)
+        _check({"y": a, "dx": got[0], "dw": got[2]}, _formula(q.detach(), wq.detach(), gq, cs, layout, R, 1e-5, dtype))
+        want = _formula(k.detach(), None if wk is None else wk.detach(), gk, cs, layout, R, 1e-5, dtype)
+        mine = {"y": b, "dx": got[1]}
+        if wk is None:
+            del want["dw"]
+        else:  # a bf16 weight's gradient is rounded to bf16
+            mine["dw"] = got[3]
+            want["dw"] = (want["dw"][0], want["dw"][1] * (1 + 2.0 ** -8) + _rounded(want["dw"][0], torch.bfloat16))
+            assert got[3].dtype == torch.bfloat16
+        _check(mine, want)
+
+
+def test_gradient_against_differences():
+    """The change along a direction, by differences of the formula in 64 bits."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    for layout, R in (("interleaved", 64), ("half", 32), ("split", 48)):
+        q, k = (torch.randn(2, 19, n, 64, device="cuda").requires_grad_() for n in (4, 2))
+        wq, wk = (torch.rand(64, device="cuda").requires_grad_() for _ in "qk")
+        tab = _table(19, R // 2)
+        cs = _rows(tab, None, 2, 19, 0)
+        gs = [torch.randn_like(x) for x in (q, k)]
+        leaves = (q, k, wq, wk)
+        got = torch.autograd.grad(qk_norm_rotary(*leaves, tab, layout=layout), leaves, gs)
+        to = [torch.randn_like(x).double() for x in leaves]
+
+        def value(t):
+            x = [v.detach().double() + t * d for v, d in zip(leaves, to)]
+            return sum((_formula(a, w, g, cs, layout, R, 1e-6, torch.float32)["y"][0] * g.double()).sum() for a, w, g in zip(x[:2], x[2:], gs))
+
+        h = 1e-4
+        # central differences of five points: the step's fourth power, and 64-bit rounding over the step
+        want = (8 * (value(h) - value(-h)) - (value(2 * h) - value(-2 * h))) / (12 * h)
+        mine = sum((g.double() * d).sum() for g, d in zip(got, to))
+        size = sum((g.double() * d).abs().sum() for g, d in zip(got, to))
+        assert abs(mine - want) <= 2.0 ** -17 * size + 1e-7 * size
+
+
+def test_extreme_rows():
+    """Rows whose squares pass 32 bits, infinities and NaN stay in their own rows."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    tab = _table(8, 32)
+    for dtype in (torch.float32, torch.bfloat16):
+        for D in (64, 68):
+            x = torch.randn(1, 8, 4, D, device="cuda")
+            x[0, 1] *= 1e25
+            x[0, 2] *= 1e-25
+            x = x.to(dtype)
+            x[0, 3, 1, 5], x[0, 4, 2, 7] = math.inf, math.nan
+            w = torch.rand(D, device="cuda")
+            y, _ = qk_norm_rotary(x, x[:, :, :1], w, None, tab)
+            cs = _rows(tab, None, 1, 8, 0)
+            want = _formula(x, w, torch.zeros_like(x), cs, "interleaved", 64, 1e-6, dtype)["y"]
+            bad = torch.zeros(1, 8, 4, dtype=torch.bool, device="cuda")
+            bad[0, 3, 1] = bad[0, 4, 2] = True
+            err = (y.double() - want[0]).abs()
+            # magnitudes near 1e-25 lose nothing: what is flushed is below 2^-126
+            assert (err <= want[1] + 1e-30)[~bad].all() and torch.isfinite(y)[~bad].all()
+            assert torch.isnan(y[0, 4, 2]).all() and torch.isnan(y[0, 3, 1]).any()
+            z = rotary(x, tab)
+            assert torch.isfinite(z)[~bad].all() and torch.isnan(z[0, 4, 2, 6:8]).all() and not torch.isnan(z[0, 4, 2, :6]).any()
+
+
+def test_positions_outside_the_table_are_recorded():
+    from drivedit_b200.ops._ext import check_device_status, device_status, reset_device_status
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    reset_device_status()
+    for D in (64, 70):
+        x, tab = torch.randn(1, 4, 2, D, device="cuda"), _table(8, 16)
+        want = rotary(x, tab, torch.tensor([0, 1, 0, 2], device="cuda"))
+        for bad in (-1, 8, 1 << 40):
+            y = rotary(x, tab, torch.tensor([0, 1, bad, 2], device="cuda"))
+            assert torch.isnan(y[0, 2, :, :32]).all() and torch.equal(y[0, 2, :, 32:], x[0, 2, :, 32:])
+            assert torch.equal(y[:, [0, 1, 3]], want[:, [0, 1, 3]])
+            assert device_status() != 0
+            with pytest.raises(RuntimeError):
+                check_device_status()
+            assert device_status() == 0
+        q, _ = qk_norm_rotary(x, x, table=tab, positions=torch.tensor([0, 1, -5, 2], device="cuda"))
+        assert torch.isnan(q[0, 2, :, :32]).all() and torch.isfinite(q[0, [0, 1, 3]]).all()
+        reset_device_status()
+
+
+def test_inplace():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    for D, layout in ((64, "split"), (64, "half"), (96, "interleaved"), (70, "split"), (256, "split")):
+        packed = torch.randn(3, 200, 9, D, device="cuda").bfloat16()
+        before = packed.clone()
+        q, k, v = packed[:, :, :4], packed[:, :, 4:6], packed[:, :, 6:]
+        tab = _table(200, D // 4)
+        want = qk_norm_rotary(q, k, table=tab, layout=layout)
+        version = packed._version
+        got = qk_norm_rotary(q, k, table=tab, layout=layout, inplace=True)
+        assert got[0].data_ptr() == q.data_ptr() and torch.equal(q, want[0]) and torch.equal(k, want[1])
+        assert torch.equal(v, before[:, :, 6:]) and packed._version > version
+        want = rotary(v, tab, layout=layout)
+        assert torch.equal(rotary(v, tab, layout=layout, inplace=True), want) and torch.equal(v, want)
+    with pytest.raises(ValueError):
+        rotary(torch.zeros(1, 4, 2, 8, device="cuda").expand(3, 4, 2, 8), _table(4, 4), inplace=True)
+    with pytest.raises(ValueError):
+        rotary(torch.zeros(1, 4, 8, 2, device="cuda").transpose(2, 3), _table(4, 4), inplace=True)
+
+
+def test_empty():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    x, tab = torch.randn(2, 4, 3, 16, device="cuda"), _table(8, 8)
+    for z in (x[:0], x[:, :0], x[:, :, :0]):
+        z = z.detach().requires_grad_()
+        y = rotary(z, tab)
+        assert y.shape == z.shape and torch.autograd.grad(y.sum(), z)[0].shape == z.shape
+        w = torch.ones(16, device="cuda", requires_grad=True)
+        q, k = qk_norm_rotary(z, z, w, w, tab)
+        assert q.shape == z.shape
+        assert not torch.autograd.grad(q.sum() + k.sum(), w)[0].any()
+    w = torch.ones(16, device="cuda", requires_grad=True)  # no query heads, and keys
+    q, k = qk_norm_rotary(x[:, :, :0], x, w, w, tab)
+    assert torch.isfinite(torch.autograd.grad(k.sum(), w)[0]).all()
+    assert torch.equal(rotary(x, tab[:, :0].contiguous()), x)
+
+
+def test_one_of_both_and_shared_weights():
+    """A gradient of one output only, one weight for both, and the same tensor as q and k."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    q, k = (torch.randn(2, 30, n, 64, device="cuda").bfloat16().requires_grad_() for n in (4, 4))
+    w = torch.rand(64, device="cuda").requires_grad_()
+    tab = _table(30, 32)
+    g = torch.randn_like(q)
+    a, b = qk_norm_rotary(q, k, w, w, tab)
+    both = torch.autograd.grad((a, b), (q, k, w), (g, g))
+    a, b = qk_norm_rotary(q, k, w, w, tab)
+    one = torch.autograd.grad(a, (q, w), g)
+    a, b = qk_norm_rotary(q, k, w, w, tab)
+    other = torch.autograd.grad(b, (k, w), g)
+    assert torch.equal(one[0], both[0]) and torch.equal(other[0], both[1])
+    # a sum of two sums, each rounded to 32 bits
+    assert torch.allclose(one[1] + other[1], both[2], rtol=2 ** -22, atol=0)
+    a, b = qk_norm_rotary(q, q, w, w, tab)
+    assert torch.equal(a, b)
+    got = torch.autograd.grad((a, b), q, (g, g))[0]
+    assert torch.allclose(got.float(), 2 * both[0].float(), rtol=2 ** -7, atol=0)
+
+
+def test_second_derivatives():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    x = torch.randn(1, 5, 2, 64, device="cuda", requires_grad=True)
+    tab = _table(5, 32)
+    y = rotary(x, tab)
+    g, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+    gg, = torch.autograd.grad((g * g).sum(), x)
+    # g = 2 x (a rotation keeps lengths, its float32 cosines to 2^-23), so gg = 8 x
+    assert torch.allclose(gg, 8 * x.detach(), rtol=1e-5, atol=1e-5)
+    q, k = qk_norm_rotary(x, x, table=tab)
+    g, = torch.autograd.grad((q * q).sum() + k.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_strides_past_32_bits():
+    """Tokens and positions whose offsets in elements do not fit 31 or 32 bits."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    far = torch.empty((1 << 32) + 4096, dtype=torch.bfloat16, device="cuda")
+    q = far.as_strided((1, 3, 2, 64), (0, 1 << 31, 64, 1))
+    q.copy_(torch.randn(1, 3, 2, 64, device="cuda"))
+    tab = _table(3, 32)
+    want = qk_norm_rotary(q.clone(), q.clone(), table=tab)
+    got = qk_norm_rotary(q, q.clone(), table=tab)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_streams_and_graphs():
+    """On a stream of its own, and captured, forward and backward, replayed on new inputs."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    tab = _table(64, 32)
+    pos = torch.randint(0, 64, (2, 40), device="cuda")
+    q, k = (torch.randn(2, 40, n, 64, device="cuda").bfloat16() for n in (4, 2))
+    w = torch.rand(64, device="cuda")
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+    side = torch.cuda.Stream()
+
+    def both(q, k, w, pos):
+        a, b = qk_norm_rotary(q, k, w, None, tab, pos)
+        return (a, b, *torch.autograd.grad((a, b), (q, k, w), (gq, gk)))
+
+    leaves = [x.clone().requires_grad_() for x in (q, k, w)]
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            both(*leaves, pos)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = both(*leaves, pos)
+    for _ in range(3):
+        with torch.no_grad():
+            for x in leaves:
+                x.copy_(torch.randn_like(x))
+            pos.copy_(torch.randint(0, 64, (2, 40), device="cuda"))
+        graph.replay()
+        want = both(*(x.detach().clone().requires_grad_() for x in leaves), pos)
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_capture_refuses_a_living_eager_graph():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    x, tab = torch.randn(1, 4, 2, 64, device="cuda", requires_grad=True), _table(4, 32)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for call in (lambda: rotary(x, tab), lambda: qk_norm_rotary(x.detach(), x.detach(), w, None, tab)[0]):
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        refused = False
+        with torch.cuda.graph(graph):
+            try:
+                call()
+            except RuntimeError as e:
+                refused = "eager" in str(e) or "default stream" in str(e)
+        assert refused and alive is not None
+
+
+def test_sync_check_mode():
+    from drivedit_b200.ops import _ext
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    q, k = (torch.randn(2, 9, n, 64, device="cuda").bfloat16().requires_grad_() for n in (4, 2))
+    w = torch.rand(64, device="cuda").requires_grad_()
+    tab = _table(9, 32)
+
+    def all_of():
+        a, b = qk_norm_rotary(q, k, w, None, tab)
+        y = rotary(q, tab, layout="split")
+        return (a, b, y, *torch.autograd.grad((a, b, y), (q, k, w), (torch.ones_like(a), torch.ones_like(b), torch.ones_like(y))))
+
+    want = all_of()
+    _ext.set_sync_check(True)
+    try:
+        got = all_of()
+        calls = [c.split("(")[0].split()[1] for c in _ext.ext().recent]
+    finally:
+        _ext.set_sync_check(False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert {"qk_norm_rotary_fwd", "qk_norm_rotary_bwd", "rotary"} <= set(calls)
+
+
+def test_refusals():
+    for what, call in refusals("cuda"):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+            pytest.fail(what)
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    x, tab = torch.randn(1, 4, 2, 64, device="cuda"), _table(4, 32)
+    for call in (lambda: rotary(x.double(), tab), lambda: rotary(x, tab.cpu()), lambda: rotary(x, tab, torch.arange(4)),
+                 lambda: qk_norm_rotary(x, x.cpu()), lambda: qk_norm_rotary(x, x, torch.ones(64))):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+
+
+def test_counts_launches():
+    from drivedit_b200.ops._ext import ext
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    x, tab = torch.randn(1, 4, 2, 64, device="cuda"), _table(4, 32)
+    n = ext().launch_count()
+    qk_norm_rotary(x, x, table=tab)
+    assert ext().launch_count() == n + 1
