@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <stdexcept>
 
 #include "../common/ptx.cuh"
@@ -45,10 +46,13 @@ struct Div {
 struct Launch {
   RotArgs a;
   Div by_T, by_H[2];
+  uint32_t heads[2] = {0, 0};  // items of a token: heads, or blocks of them (by_H divides by it)
   int ctas0 = 0;       // CTAs of the first tensor
   int ctas1 = 0;
   int log_lanes = 0;   // lanes of a head
+  int unroll = 1;      // heads of a lane at once
   int* status = nullptr;
+  int dev = 0;
 };
 
 template <typename T>
@@ -57,11 +61,10 @@ template <>
 struct Io<__nv_bfloat16> {
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ void get8(const __nv_bfloat16* p, float* v) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
+    const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       v[2 * i] = __uint_as_float(w[i] << 16);
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
@@ -74,11 +77,10 @@ template <>
 struct Io<__half> {
   static __device__ __forceinline__ float get(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-  static __device__ __forceinline__ void get8(const __half* p, float* v) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
+    const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       v[2 * i] = f.x;
       v[2 * i + 1] = f.y;
@@ -98,9 +100,12 @@ template <>
 struct Io<float> {
   static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
-  static __device__ __forceinline__ void get8(const float* p, float* v) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  static __device__ __forceinline__ void unpack(const uint4 (&u)[4], float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[4 * i] = __uint_as_float(u[i].x), v[4 * i + 1] = __uint_as_float(u[i].y);
+      v[4 * i + 2] = __uint_as_float(u[i].z), v[4 * i + 3] = __uint_as_float(u[i].w);
+    }
   }
   static __device__ __forceinline__ void put8(float* p, const float* v) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -110,8 +115,7 @@ struct Io<float> {
 
 // One (token, head): where its channels lie, and its row of the table (-1: no such row)
 struct Item {
-  long b, t, h;
-  long row;
+  int b, t, h, row;
   bool there;
 };
 
@@ -120,7 +124,7 @@ __device__ __forceinline__ Item item_of(const Launch& L, int which, uint32_t i, 
   Item it;
   it.there = i < n;
   const uint32_t token = L.by_H[which](it.there ? i : 0);
-  it.h = (it.there ? i : 0) - token * a.t[which].H;
+  it.h = (it.there ? i : 0) - token * L.heads[which];
   const uint32_t b = L.by_T(token);
   it.b = b;
   it.t = token - b * a.T;
@@ -128,13 +132,14 @@ __device__ __forceinline__ Item item_of(const Launch& L, int which, uint32_t i, 
   if (a.R > 0 && it.there) {
     if (a.pos) {
       const long at = it.b * a.pos_sb + it.t * a.pos_st;
-      it.row = a.pos64 ? reinterpret_cast<const long long*>(a.pos)[at] : reinterpret_cast<const int*>(a.pos)[at];
-      if (it.row < 0 || it.row >= a.places) {  // recorded; the token's rotated channels become NaN
-        record_bad_index(L.status, it.row);
+      const long row = a.pos64 ? reinterpret_cast<const long long*>(a.pos)[at] : reinterpret_cast<const int*>(a.pos)[at];
+      it.row = static_cast<int>(row);
+      if (row < 0 || row >= a.places) {  // recorded; the token's rotated channels become NaN
+        record_bad_index(L.status, row);
         it.row = -1;
       }
     } else {
-      it.row = a.offset + it.t;
+      it.row = static_cast<int>(a.offset) + it.t;
     }
   }
   return it;
@@ -151,150 +156,345 @@ __device__ __forceinline__ float rms_inv(float sum, float D, float eps, float do
 }
 constexpr float kDown = 0x1p-70f;  // its square times a sum of 256 squares of the largest fp32 is finite
 
-template <typename T, bool IN_H, bool OUT_H, bool NORM, bool BWD, int U>
+// Two numbers to an instruction
+__device__ __forceinline__ unsigned long long& bits(float2& x) { return reinterpret_cast<unsigned long long&>(x); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
+
+// Where a lane's two runs of 8 channels begin on one side. Pairs in halves: a run in each. Side by
+// side: 4 pairs in each run, which lie R / 2 apart as well, so that the lanes of an access are
+// contiguous; but where the other side has halves ("split") the lane's 8 pairs have to be in a
+// row, and the runs are.
+struct Runs {
+  int c0, c1;
+};
+template <bool HALVES, bool MIXED>
+__device__ __forceinline__ Runs runs_of(int l, int R, bool rot) {
+  if (!rot) return {16 * l, 16 * l + 8};
+  if (MIXED && !HALVES) return {16 * l, 16 * l + 8};
+  return {8 * l, R / 2 + 8 * l};
+}
+
+// 16 bytes into the thread's own place of shared memory, zeros where `there` is false
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A lane's 8 pairs, their first and their second channels, two pairs to an entry
+struct Pairs {
+  float2 a[4], b[4];
+  // from and to channels in memory order (runs one after the other)
+  template <bool HALVES>
+  __device__ __forceinline__ void from(const float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = HALVES ? make_float2(v[2 * i], v[2 * i + 1]) : make_float2(v[4 * i], v[4 * i + 2]);
+      b[i] = HALVES ? make_float2(v[8 + 2 * i], v[9 + 2 * i]) : make_float2(v[4 * i + 1], v[4 * i + 3]);
+    }
+  }
+  template <bool HALVES>
+  __device__ __forceinline__ void to(float (&v)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[HALVES ? 2 * i : 4 * i] = a[i].x, v[HALVES ? 2 * i + 1 : 4 * i + 2] = a[i].y;
+      v[HALVES ? 8 + 2 * i : 4 * i + 1] = b[i].x, v[HALVES ? 9 + 2 * i : 4 * i + 3] = b[i].y;
+    }
+  }
+  __device__ __forceinline__ void times(float2 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = mul2(a[i], x), b[i] = mul2(b[i], x);
+  }
+  __device__ __forceinline__ void times(const Pairs& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = mul2(a[i], x.a[i]), b[i] = mul2(b[i], x.b[i]);
+  }
+};
+// sum of the products of two heads' channels, over the head's lanes
+__device__ __forceinline__ float dot(const Pairs& x, const Pairs& y, int lg) {
+  float2 s = mul2(x.a[0], y.a[0]), t = mul2(x.b[0], y.b[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = fma2(x.a[i], y.a[i], s), t = fma2(x.b[i], y.b[i], t);
+  s = add2(s, t);
+  float r = s.x + s.y;
+  for (int o = 1; o < 1 << lg; o *= 2) r += __shfl_xor_sync(0xffffffffu, r, o);
+  return r;
+}
+
+// (mean + eps)^-1/2: the unit's estimate and one step of Newton's method
+__device__ __forceinline__ float rms_inv_fast(float sum, float inv_D, float eps) {
+  const float m = fmaf(sum, inv_D, eps);
+  const float r = rsqrtf(m);
+  return m > 3e38f ? 0.f : r * fmaf(-0.5f * m * r, r, 1.5f);
+}
+
+template <typename T>
+constexpr int kChunks = sizeof(T) == 4 ? 4 : 2;  // of 16 bytes, of a lane's 16 channels
+// Places of a thread for a turn (x, then its row of the table) and turns on their way, the one in
+// work counted
+template <typename T, int U>
+constexpr int kPlaces = U * kChunks<T> + 4;
+template <typename T, int U>
+constexpr int kStages = kPlaces<T, U> > 8 ? 2 : 3;
+
+// The row's angles, of the lane's 8 pairs: cosines, and sines times `flip`. NaN off the table.
+struct Angles {
+  float2 c[4], s[4];
+  __device__ __forceinline__ void put(int i, float4 f, int row, float flip) {
+    const float nan = row < 0 ? NAN : 0.f;
+    c[i] = make_float2(f.x + nan, f.z + nan);
+    s[i] = make_float2(f.y * flip, f.w * flip);
+  }
+};
+
+// The weights of the lane's channels
+template <bool HALVES>
+__device__ __forceinline__ Pairs weights(const float* w, const Runs& r, bool active) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+    if (w && active) f = __ldg(reinterpret_cast<const float4*>(w + (i < 2 ? r.c0 : r.c1) + 4 * (i & 1)));
+    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+  }
+  Pairs p;
+  p.from<HALVES>(v);
+  return p;
+}
+
+// 1 / rms of a head (its channels brought down by a power of two where their squares are too large)
+__device__ __forceinline__ float rms_inv_of(Pairs& v, int lg, float inv_D, float eps, float& down) {
+  float s = dot(v, v, lg);
+  down = 1.f;
+  if (__any_sync(0xffffffffu, !(s < 1e38f))) {  // squares too large for fp32, infinities, NaN
+    if (!(s < 1e38f)) down = kDown;
+    v.times(both(down));
+    s = dot(v, v, lg);
+  }
+  return rms_inv_fast(s, inv_D, eps * down * down);
+}
+
+// A group of lanes takes U heads of one token: they share its row of the table and the weights.
+// Heads u of the groups of a warp lie side by side. CTAs stay; each thread's copies run kStages - 1
+// turns ahead of it into places of its own.
+template <typename T, bool IN_H, bool OUT_H, bool NORM, int U>
 __global__ void __launch_bounds__(kThreads, 2) rot_wide(const Launch L) {
+  extern __shared__ __align__(16) uint4 ring[];  // [stage][place][thread]
+  constexpr bool kMixed = IN_H != OUT_H;
+  constexpr int C = kChunks<T>, S = kStages<T, U>, kStage = kPlaces<T, U> * kThreads;
   const RotArgs& a = L.a;
   const int which = blockIdx.x >= L.ctas0;
   const RotTensor& t = a.t[which];
   const int lg = L.log_lanes, l = threadIdx.x & ((1 << lg) - 1);
   const bool active = l < a.D >> 4, rot = l < a.R >> 4;
-  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * t.H;
+  const int blocks = L.heads[which];
+  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * blocks;
   const uint32_t per = kThreads >> lg;
-  const int in0 = rot && IN_H ? 8 * l : 16 * l, in1 = rot && IN_H ? a.R / 2 + 8 * l : 16 * l + 8;
-  const int out0 = rot && OUT_H ? 8 * l : 16 * l, out1 = rot && OUT_H ? a.R / 2 + 8 * l : 16 * l + 8;
-  float w[16], dw[16];
-  if (NORM) {
+  const Runs in = runs_of<IN_H, kMixed>(l, a.R, rot), out = runs_of<OUT_H, kMixed>(l, a.R, rot);
+  // the lane's pairs: a row of 8, or 4 and 4
+  const int p0 = kMixed || IN_H ? 8 * l : 4 * l, p1 = kMixed || IN_H ? 8 * l + 4 : a.R / 4 + 4 * l;
+  const float inv_D = 1.f / static_cast<float>(a.D);
+  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), step = (which ? L.ctas1 : L.ctas0) * per;
+  const uint32_t mine = smem_u32(ring + threadIdx.x);
+  auto fetch = [&](uint32_t i0, int stage) {
+    if (i0 < n) {
+      const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
+      const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
+      uint32_t dst = mine + stage * (kStage * 16);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      w[i] = t.w && active ? t.w[(i < 8 ? in0 : in1) + (i & 7)] : 1.f;
-      dw[i] = 0.f;
-    }
-  }
-  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), ctas = which ? L.ctas1 : L.ctas0;
-  for (uint32_t i0 = cta * per * U; i0 < n; i0 += ctas * per * U) {  // one turn in the forward
-    float v[U][16], g[U][16];
-    Item it[U];
+      for (int u = 0; u < U; ++u) {
+        const int h = it.h + u * blocks;
+        const bool have = it.there && active && h < t.H;
+        const T* p = px + h * t.x_sh;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      it[u] = item_of(L, which, i0 + u * per + (threadIdx.x >> lg), n);
-      if (it[u].there && active) {
-        const T* x = reinterpret_cast<const T*>(t.x) + it[u].b * t.x_sb + it[u].t * t.x_st + it[u].h * t.x_sh;
-        Io<T>::get8(x + in0, v[u]);
-        Io<T>::get8(x + in1, v[u] + 8);
-        if (BWD) {
-          const T* y = reinterpret_cast<const T*>(t.g) + it[u].b * t.g_sb + it[u].t * t.g_st + it[u].h * t.g_sh;
-          Io<T>::get8(y + out0, g[u]);
-          Io<T>::get8(y + out1, g[u] + 8);
-        }
-      } else {
+        for (int i = 0; i < C; ++i, dst += kThreads * 16)
+          copy16(dst, have ? p + (i < C / 2 ? in.c0 : in.c1) + (i % (C / 2)) * (16 / sizeof(T)) : t.x, have);
+      }
+      if (rot && it.there) {
+        const float2* tab = a.table + static_cast<long>(max(it.row, 0)) * (a.R / 2);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[u][i] = g[u][i] = 0.f;
+        for (int i = 0; i < 4; ++i, dst += kThreads * 16) copy16(dst, tab + (i < 2 ? p0 : p1) + 2 * (i & 1), true);
       }
     }
+    copies_end();
+  };
+  uint32_t i0 = cta * per;
+#pragma unroll
+  for (int k = 0; k < S - 1; ++k) fetch(i0 + k * step, k);
+  for (int stage = 0; i0 < n; i0 += step, stage = stage == S - 1 ? 0 : stage + 1) {
+    const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
+    Pairs w;
+    if (NORM) w = weights<IN_H>(t.w, in, active);
+    copies_wait<S - 2>();
+    __syncwarp();  // every lane has read what another one may write (a result in the place of its input)
+    fetch(i0 + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    const uint4* got = ring + stage * kStage + threadIdx.x;
+    Angles ang;
+    if (rot && it.there) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        ang.put(i, reinterpret_cast<const float4*>(got)[(U * C + i) * kThreads], it.row, a.inverse ? -1.f : 1.f);
+    }
+    T* py = reinterpret_cast<T*>(t.y) + it.b * t.y_sb + it.t * t.y_st;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const int h = it.h + u * blocks;
+      float buf[16];
+      uint4 raw[C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) raw[i] = got[(u * C + i) * kThreads];
+      Io<T>::unpack(raw, buf);
+      Pairs z;
+      z.from<IN_H>(buf);
       float r = 1.f;
       if (NORM) {
-        float down = 1.f;
-        auto sum = [&]() {
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s = fmaf(v[u][i], v[u][i], s);
-          for (int o = 1; o < 1 << lg; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-          return s;
-        };
-        float s = sum();
-        if (__any_sync(0xffffffffu, !(s < 1e38f))) {  // squares too large for fp32, infinities, NaN
-          if (!(s < 1e38f)) down = kDown;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[u][i] *= down;
-          s = sum();
-        }
-        r = rms_inv(s, static_cast<float>(a.D), a.eps, down);
-        if (BWD) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[u][i] *= r;
-          r *= down;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[u][i] = v[u][i] * r * w[i];
-        }
+        float down;
+        r = rms_inv_of(z, lg, inv_D, a.eps, down);
+        z.times(w);
       }
-      float z[16];  // the rotated, or rotated back
-      const float* from = BWD ? g[u] : v[u];
-      if (a.R > 0) {
-        float2 cs[8];
-        if (rot && it[u].there && it[u].row >= 0) {
-          const float4* tab = reinterpret_cast<const float4*>(a.table + it[u].row * (a.R / 2) + 8 * l);
+      if (rot && it.there) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 f = __ldg(tab + i);
-            cs[2 * i] = make_float2(f.x, f.y);
-            cs[2 * i + 1] = make_float2(f.z, f.w);
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = z.a[i], q = z.b[i];
+          if (NORM) {
+            z.a[i] = fma2(p, ang.c[i], mul2(q, neg(ang.s[i])));
+            z.b[i] = fma2(p, ang.s[i], mul2(q, ang.c[i]));
+          } else {  // as the PyTorch statement rounds it (the paired instructions are contracted)
+            const float2 y0 = turn(p.x, q.x, ang.c[i].x, ang.s[i].x), y1 = turn(p.y, q.y, ang.c[i].y, ang.s[i].y);
+            z.a[i] = make_float2(y0.x, y1.x);
+            z.b[i] = make_float2(y0.y, y1.y);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) cs[i] = make_float2(NAN, NAN);
         }
-        const bool back = a.inverse;  // the backward of a rotation is its inverse
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          // forward: pairs as they are read, to where they are written; backward: the other way
-          constexpr bool kFrom = BWD ? OUT_H : IN_H, kTo = BWD ? IN_H : OUT_H;
-          const int f0 = kFrom ? j : 2 * j, f1 = kFrom ? j + 8 : 2 * j + 1;
-          const int t0 = kTo ? j : 2 * j, t1 = kTo ? j + 8 : 2 * j + 1;
-          const float2 q = turn(from[f0], from[f1], cs[j].x, back != BWD ? -cs[j].y : cs[j].y);
-          z[t0] = q.x;
-          z[t1] = q.y;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = rot ? z[i] : from[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) z[i] = from[i];
       }
-      if (BWD) {
-        float m = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (it[u].there) dw[i] = fmaf(z[i], v[u][i], dw[i]);
-          z[i] *= w[i];
-          m = fmaf(z[i], v[u][i], m);
-        }
-        for (int o = 1; o < 1 << lg; o *= 2) m += __shfl_xor_sync(0xffffffffu, m, o);
-        m = __fdiv_rn(m, static_cast<float>(a.D));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[u][i] = r * (z[i] - v[u][i] * m);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[u][i] = z[i];
+      if (NORM) z.times(both(r));
+      z.to<OUT_H>(buf);
+      if (kMixed && !rot) z.to<IN_H>(buf);
+      if (it.there && active && h < t.H) {
+        T* y = py + h * t.y_sh;
+        Io<T>::put8(y + out.c0, buf);
+        Io<T>::put8(y + out.c1, buf + 8);
       }
     }
-    __syncwarp();  // every lane has read what another one may write (a result in the place of its input)
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (it[u].there && active) {
-        T* y = reinterpret_cast<T*>(t.y) + it[u].b * t.y_sb + it[u].t * t.y_st + it[u].h * t.y_sh;
-        Io<T>::put8(y + (BWD ? in0 : out0), v[u]);
-        Io<T>::put8(y + (BWD ? in1 : out1), v[u] + 8);
-      }
-    if (!BWD) break;
   }
-  if (BWD) {
-    // the CTA's sums of each channel: lanes of a warp, then warps, in a fixed order
-    __shared__ float red[kThreads / 32][256];
+}
+
+// The backward. Loads go straight to registers: copies ahead of the work, as above, need the
+// shared memory of x and g and were slower here (52 and 46 us of a dit_b step's 16,384 tokens of 12 and 12 heads).
+template <typename T, bool IN_H, bool OUT_H, int U>
+__global__ void __launch_bounds__(kThreads, 2) rot_wide_back(const Launch L) {
+  constexpr bool kMixed = IN_H != OUT_H;
+  constexpr int C = kChunks<T>;
+  const RotArgs& a = L.a;
+  const int which = blockIdx.x >= L.ctas0;
+  const RotTensor& t = a.t[which];
+  const int lg = L.log_lanes, l = threadIdx.x & ((1 << lg) - 1);
+  const bool active = l < a.D >> 4, rot = l < a.R >> 4;
+  const int blocks = L.heads[which];
+  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * blocks;
+  const uint32_t per = kThreads >> lg;
+  const Runs in = runs_of<IN_H, kMixed>(l, a.R, rot), out = runs_of<OUT_H, kMixed>(l, a.R, rot);
+  const int p0 = kMixed || IN_H ? 8 * l : 4 * l, p1 = kMixed || IN_H ? 8 * l + 4 : a.R / 4 + 4 * l;
+  const float inv_D = 1.f / static_cast<float>(a.D);
+  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), step = (which ? L.ctas1 : L.ctas0) * per;
+  Pairs dw;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      for (int o = 1 << lg; o < 32; o *= 2) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-      if ((threadIdx.x & 31) == l && active) red[threadIdx.x >> 5][(i < 8 ? in0 : in1) + (i & 7)] = dw[i];
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.D; c += kThreads) {
-      float s = 0.f;
+  for (int i = 0; i < 4; ++i) dw.a[i] = dw.b[i] = both(0.f);
+  for (uint32_t i0 = cta * per; i0 < n; i0 += step) {
+    const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
+    uint4 x[U][C], g[U][C];
+    const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
+    const T* pg = reinterpret_cast<const T*>(t.g) + it.b * t.g_sb + it.t * t.g_st;
 #pragma unroll
-      for (int k = 0; k < kThreads / 32; ++k) s += red[k][c];
-      a.part[static_cast<long>(blockIdx.x) * a.D + c] = s;
+    for (int u = 0; u < U; ++u) {
+      const int h = it.h + u * blocks;
+      const bool have = it.there && active && h < t.H;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int at = (i % (C / 2)) * (16 / sizeof(T));
+        x[u][i] = g[u][i] = make_uint4(0, 0, 0, 0);
+        if (have) {
+          x[u][i] = *reinterpret_cast<const uint4*>(px + h * t.x_sh + (i < C / 2 ? in.c0 : in.c1) + at);
+          g[u][i] = *reinterpret_cast<const uint4*>(pg + h * t.g_sh + (i < C / 2 ? out.c0 : out.c1) + at);
+        }
+      }
     }
+    Angles ang;
+    if (rot && it.there) {
+      const float2* tab = a.table + static_cast<long>(max(it.row, 0)) * (a.R / 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        ang.put(i, __ldg(reinterpret_cast<const float4*>(tab + (i < 2 ? p0 : p1) + 2 * (i & 1))), it.row, 1.f);
+    }
+    __syncwarp();  // every lane has read what another one may write (a gradient in the place of the result's)
+    T* py = reinterpret_cast<T*>(t.y) + it.b * t.y_sb + it.t * t.y_st;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = it.h + u * blocks;
+      float buf[16], down;
+      Pairs v, z;
+      Io<T>::unpack(x[u], buf);
+      v.from<IN_H>(buf);
+      const float r = rms_inv_of(v, lg, inv_D, a.eps, down);
+      Io<T>::unpack(g[u], buf);
+      z.from<OUT_H>(buf);
+      if (kMixed && !rot) z.from<IN_H>(buf);
+      if (rot && it.there) {  // by the negative angle
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 p = z.a[i], q = z.b[i];
+          z.a[i] = fma2(p, ang.c[i], mul2(q, ang.s[i]));
+          z.b[i] = fma2(q, ang.c[i], mul2(p, neg(ang.s[i])));
+        }
+      }
+      // gr = g r; dw += gr x; dx = gr w - x r^2 mean(gr w x)
+      z.times(both(r));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dw.a[i] = fma2(z.a[i], v.a[i], dw.a[i]), dw.b[i] = fma2(z.b[i], v.b[i], dw.b[i]);
+      z.times(weights<IN_H>(t.w, in, active));
+      const float2 k = both(-dot(z, v, lg) * inv_D * r * r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z.a[i] = fma2(v.a[i], k, z.a[i]), z.b[i] = fma2(v.b[i], k, z.b[i]);
+      if (down != 1.f) z.times(both(down));
+      z.to<IN_H>(buf);
+      if (it.there && active && h < t.H) {
+        T* y = py + h * t.y_sh;
+        Io<T>::put8(y + in.c0, buf);
+        Io<T>::put8(y + in.c1, buf + 8);
+      }
+    }
+  }
+  // the CTA's sums of each channel: lanes of a warp, then warps, in a fixed order
+  __shared__ float red[kThreads / 32][256];
+  float v[16];
+  dw.to<IN_H>(v);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    for (int o = 1 << lg; o < 32; o *= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if ((threadIdx.x & 31) == l && active) red[threadIdx.x >> 5][(i < 8 ? in.c0 : in.c1) + (i & 7)] = v[i];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.D; c += kThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kThreads / 32; ++k) s += red[k][c];
+    a.part[static_cast<long>(blockIdx.x) * a.D + c] = s;
   }
 }
 
@@ -310,6 +510,7 @@ __global__ void __launch_bounds__(kThreads) rot_any(const Launch L) {
   // channels of a lane's pair i as one side has them
   auto chan = [&](int i, bool halves, int& c0, int& c1) {
     const int p = l + (i << lg);
+    if (i << lg >= pairs) return false;  // for all lanes
     if (p < turned && halves) c0 = p, c1 = p + turned;
     else c0 = 2 * p, c1 = 2 * p + 1;
     return p < pairs;
@@ -363,7 +564,7 @@ __global__ void __launch_bounds__(kThreads) rot_any(const Launch L) {
       const int p = l + (i << lg);
       if (p < turned) {
         float2 cs = make_float2(NAN, NAN);
-        if (it.there && it.row >= 0) cs = __ldg(a.table + it.row * turned + p);
+        if (it.there && it.row >= 0) cs = __ldg(a.table + static_cast<long>(it.row) * turned + p);
         const float2 q = turn(z[2 * i], z[2 * i + 1], cs.x, a.inverse != BWD ? -cs.y : cs.y);
         z[2 * i] = q.x;
         z[2 * i + 1] = q.y;
@@ -446,12 +647,10 @@ bool wide(const RotArgs& a, bool bwd) {
   for (int i = 0; i < a.n; ++i) {
     const RotTensor& t = a.t[i];
     if (!ok(t.x, t.x_sb, t.x_st, t.x_sh) || !ok(t.y, t.y_sb, t.y_st, t.y_sh)) return false;
-    if (bwd && !ok(t.g, t.g_sb, t.g_st, t.g_sh)) return false;
+    if ((bwd && !ok(t.g, t.g_sb, t.g_st, t.g_sh)) || reinterpret_cast<uintptr_t>(t.w) % 16) return false;
   }
   return true;
 }
-
-constexpr int unroll(bool bwd) { return bwd ? 1 : 2; }  // heads of a lane at once
 
 int log2_up(int n) {
   int lg = 0;
@@ -465,14 +664,30 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
   L.log_lanes = is_wide ? log2_up(a.D / 16) : a.D <= 128 ? 3 : 4;
   L.by_T = Div(a.T);
   L.status = device_status(dev);
-  const long per = (kThreads >> L.log_lanes) * (is_wide ? unroll(bwd) : 1);
+  L.dev = dev;
+  const long per = kThreads >> L.log_lanes;
   long need[2] = {0, 0};
-  for (int i = 0; i < a.n; ++i) {
-    L.by_H[i] = Div(a.t[i].H);
-    need[i] = (static_cast<long>(a.B) * a.T * a.t[i].H + per - 1) / per;
+  auto count = [&](int unroll) {
+    L.unroll = unroll;
+    for (int i = 0; i < a.n; ++i) {
+      L.heads[i] = (a.t[i].H + unroll - 1) / unroll;
+      L.by_H[i] = Div(L.heads[i]);
+      need[i] = (static_cast<long>(a.B) * a.T * L.heads[i] + per - 1) / per;
+    }
+  };
+  if (!is_wide) {
+    count(1);
+  } else if (bwd) {
+    count(a.type == RotType::kF32 ? 1 : 2);  // (more spill registers)
+  } else {
+    // 4 heads of a token at once where few of the places stay empty and the CTAs fill the device
+    count(a.type == RotType::kF32 ? 2 : 4);
+    long slots = 0, heads = 0;
+    for (int i = 0; i < a.n; ++i) slots += 4 * L.heads[i], heads += a.t[i].H;
+    if (a.type != RotType::kF32 && (slots * 5 > heads * 6 || need[0] + need[1] < 4 * num_sms(dev))) count(2);
   }
-  if (bwd || !is_wide) {  // CTAs that stay: their sums of the weights' gradients are added up behind them
-    const long room = static_cast<long>(num_sms(dev)) * (bwd ? 2 : 8);
+  {  // CTAs that stay
+    const long room = static_cast<long>(num_sms(dev)) * (is_wide || bwd ? 2 : 8);
     const long all = need[0] + need[1];
     if (all > room)
       for (int i = 0; i < a.n; ++i) need[i] = std::max(1L, need[i] * room / all);
@@ -482,16 +697,44 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
   return L;
 }
 
+template <auto kernel, int BYTES>
+void launch_ring(const Launch& L, cudaStream_t s) {
+  static_assert(2 * (BYTES + 1024) <= 233472, "two CTAs an SM");
+  static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+  if (!(set.load() >> (L.dev & 63) & 1)) {
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES), "cudaFuncSetAttribute(rot_wide)");
+    set.fetch_or(1ull << (L.dev & 63));
+  }
+  kernel<<<L.ctas0 + L.ctas1, kThreads, BYTES, s>>>(L);
+}
+
+template <typename T, bool NORM, int U>
+void launch_wide(const Launch& L, cudaStream_t s) {
+  const bool ih = L.a.layout.in_halves, oh = L.a.layout.out_halves;
+  constexpr int kBytes = kStages<T, U> * kPlaces<T, U> * kThreads * 16;
+  if (!ih && !oh) launch_ring<rot_wide<T, false, false, NORM, U>, kBytes>(L, s);
+  else if (ih && oh) launch_ring<rot_wide<T, true, true, NORM, U>, kBytes>(L, s);
+  else if (oh) launch_ring<rot_wide<T, false, true, NORM, U>, kBytes>(L, s);
+  else if constexpr (!NORM) launch_ring<rot_wide<T, true, false, NORM, U>, kBytes>(L, s);
+  else throw std::runtime_error("rotary: a norm is not behind an inverse rotation");
+}
+
+template <typename T, int U>
+void launch_back(const Launch& L, cudaStream_t s) {
+  const bool ih = L.a.layout.in_halves, oh = L.a.layout.out_halves;
+  const int grid = L.ctas0 + L.ctas1;
+  if (!ih && !oh) rot_wide_back<T, false, false, U><<<grid, kThreads, 0, s>>>(L);
+  else if (ih && oh) rot_wide_back<T, true, true, U><<<grid, kThreads, 0, s>>>(L);
+  else rot_wide_back<T, false, true, U><<<grid, kThreads, 0, s>>>(L);
+}
+
 template <typename T, bool NORM, bool BWD>
 void launch(const Launch& L, bool is_wide, cudaStream_t s) {
-  const int grid = L.ctas0 + L.ctas1;
-  const bool ih = L.a.layout.in_halves, oh = L.a.layout.out_halves;
-  if (!is_wide) rot_any<T, NORM, BWD><<<grid, kThreads, 0, s>>>(L);
-  else if (!ih && !oh) rot_wide<T, false, false, NORM, BWD, unroll(BWD)><<<grid, kThreads, 0, s>>>(L);
-  else if (ih && oh) rot_wide<T, true, true, NORM, BWD, unroll(BWD)><<<grid, kThreads, 0, s>>>(L);
-  else if (oh) rot_wide<T, false, true, NORM, BWD, unroll(BWD)><<<grid, kThreads, 0, s>>>(L);
-  else if constexpr (!NORM) rot_wide<T, true, false, NORM, BWD, unroll(BWD)><<<grid, kThreads, 0, s>>>(L);
-  else throw std::runtime_error("rotary: a norm is not behind an inverse rotation");
+  if (!is_wide) rot_any<T, NORM, BWD><<<L.ctas0 + L.ctas1, kThreads, 0, s>>>(L);
+  else if constexpr (BWD) launch_back<T, sizeof(T) == 4 ? 1 : 2>(L, s);
+  else if constexpr (sizeof(T) == 4) launch_wide<T, NORM, 2>(L, s);
+  else if (L.unroll == 2) launch_wide<T, NORM, 2>(L, s);
+  else launch_wide<T, NORM, 4>(L, s);
   check_cuda(cudaGetLastError(), "rotary launch");
   count_launch();
 }
@@ -508,7 +751,7 @@ void launch(const Launch& L, bool is_wide, cudaStream_t s) {
 void check(const RotArgs& a) {
   long items = 0;
   for (int i = 0; i < a.n; ++i) items = std::max(items, static_cast<long>(a.B) * a.T * a.t[i].H);
-  if (a.n < 1 || a.n > 2 || a.D < 2 || a.D > 256 || a.D % 2 || a.R < 0 || a.R > a.D || a.R % 2 || items >= 1L << 30)
+  if (a.n < 1 || a.n > 2 || a.D < 2 || a.D > 256 || a.D % 2 || a.R < 0 || a.R > a.D || a.R % 2 || items >= 1L << 30 || a.places > 0x7fffffffL)
     throw std::runtime_error("rotary: sizes out of range");
 }
 

@@ -55,6 +55,7 @@ void check_rotation(const Rotation& r, const Tensor& x0) {
   TORCH_CHECK_VALUE(tab.dim() == 3 && tab.size(2) == 2 && tab.scalar_type() == torch::kFloat && tab.is_contiguous() &&
                         2 * tab.size(1) <= x.size(3),
                     "table must be contiguous float32 [positions, rotated channels / 2, 2] for heads of ", x.size(3), ", got ", tab.sizes());
+  TORCH_CHECK_VALUE(tab.size(0) <= 0x7fffffff, "at most 2^31 - 1 positions in a table");
   TORCH_CHECK_VALUE(tab.device() == x.device(), "table is on ", tab.device(), ", the heads on ", x.device());
   TORCH_CHECK_VALUE(!tab.requires_grad(), "the table has no gradient");
   if (r.positions) {
