@@ -1659,16 +1659,20 @@ ddb::KvPool kv_pool(const torch::Tensor& k, const torch::Tensor& v, const torch:
 
 static_assert(ddb::kKvInfo == ddb::KvBook::kFront, "words before a row's page ids");
 
-ddb::KvStep kv_step(const torch::Tensor& rows, const torch::Tensor& k) {
+// rows: of B sequences, then of the groups of `branches` (none where that is 1)
+ddb::KvStep kv_step(const torch::Tensor& rows, const torch::Tensor& k, int64_t branches) {
   TORCH_CHECK(rows.scalar_type() == torch::kInt32 && rows.is_contiguous() && rows.dim() == 2 &&
                   rows.size(1) > ddb::kKvInfo && rows.device() == k.device(),
               "a step's table must be contiguous int32 [sequences, 4 + pages] on the cache's device");
-  TORCH_CHECK(rows.size(0) <= 65535, "at most 65535 sequences in a step");
+  TORCH_CHECK(branches >= 1 && (branches == 1 || rows.size(0) % (branches + 1) == 0), "a step's table and its groups differ");
+  const int64_t B = branches == 1 ? rows.size(0) : rows.size(0) / (branches + 1) * branches;
+  TORCH_CHECK(B <= 65535, "at most 65535 sequences in a step");
   ddb::KvStep s;
   s.rows = rows.data_ptr<int>();
   s.ld = rows.size(1);
   s.width = rows.size(1) - ddb::kKvInfo;
-  s.B = rows.size(0);
+  s.B = B;
+  s.branches = branches;
   return s;
 }
 
@@ -1679,6 +1683,7 @@ struct KvStepHandle {
   ddb::KvPool base;  // of layer 0, checked when the step was begun
   ddb::KvStep step;
   int64_t layers = 0, max_tokens = 0, most_new = 0;
+  int64_t shared_pages = 0, own_tokens = 0;  // most pages that a group shares, most tokens behind them
   int64_t trim_sinks = -1;  // sinks of the trimmed sequences; -1: none is, -2: they differ
   // what captured calls hold fast: the fewest rows of one, and the sinks that windowed ones name
   // (-1: none, -2: they differ)
@@ -1697,13 +1702,14 @@ void kv_step_check_refill(const KvStepHandle& h, int64_t most_new, int64_t trim_
                     "a trimmed sequence keeps the first tokens it was trimmed to; the step's captured calls name others");
 }
 
-// rows: int32 [B, 4 + pages] in host memory; `out`: a step to refill in place
+// rows: int32 [B (+ groups), 4 + pages] in host memory; `out`: a step to refill in place
 std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, torch::Tensor ks, torch::Tensor vs,
                                             torch::Tensor rows, int64_t max_tokens, int64_t most_new, int64_t trim_sinks,
+                                            int64_t branches, int64_t shared_pages, int64_t own_tokens,
                                             std::shared_ptr<KvStepHandle> out) {
   const auto base = kv_pool(k, v, ks, vs, 0);
   TORCH_CHECK(rows.device().is_cpu() && rows.scalar_type() == torch::kInt32 && rows.is_contiguous() && rows.dim() == 2 &&
-                  rows.size(1) > ddb::kKvInfo && rows.size(0) <= 65535, "a step's table must be int32 [<= 65535, 4 + pages]");
+                  rows.size(1) > ddb::kKvInfo && rows.size(0) <= 2 * 65535, "a step's table must be int32 [sequences, 4 + pages]");
   const c10::cuda::CUDAGuard guard(k.device());
   auto h = out ? out : std::make_shared<KvStepHandle>();
   // pinned memory of the caching host allocator: kept until the copy has run
@@ -1718,11 +1724,13 @@ std::shared_ptr<KvStepHandle> kv_step_begin(torch::Tensor k, torch::Tensor v, to
   }
   h->k = k; h->v = v; h->ks = ks; h->vs = vs;
   h->base = base;
-  h->step = kv_step(h->rows, k);
+  h->step = kv_step(h->rows, k, branches);
   h->layers = k.size(0);
   h->max_tokens = max_tokens;
   h->most_new = most_new;
   h->trim_sinks = trim_sinks;
+  h->shared_pages = shared_pages;
+  h->own_tokens = own_tokens;
   h->begun = at::cuda::getCurrentCUDAStream();
   h->ready.record(*h->begun);
   return h;
@@ -1755,7 +1763,7 @@ void kv_step_wait(KvStepHandle& h) {
 
 // tokens [B, T, H, 64] bf16 as the kernels read them: contiguous channels, rows on 16 bytes
 torch::Tensor kv_tokens(const torch::Tensor& t, const char* name, const KvStepHandle& h, int64_t heads) {
-  TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == h.rows.size(0) && t.size(3) == 64, name, " must be [", h.rows.size(0),
+  TORCH_CHECK_VALUE(t.dim() == 4 && t.size(0) == h.step.B && t.size(3) == 64, name, " must be [", h.step.B,
                     ", T, heads, 64], got ", t.sizes());
   TORCH_CHECK_VALUE(heads ? t.size(2) == heads : t.size(2) > 0 && t.size(2) % h.k.size(2) == 0, name, " has ", t.size(2),
                     " heads, the cache ", h.k.size(2));
@@ -1816,6 +1824,8 @@ std::vector<torch::Tensor> kv_step_attend(std::shared_ptr<KvStepHandle> hp, int6
   a.sinks = m.sinks;
   a.scale = static_cast<float>(m.scale);
   a.max_tokens = h.max_tokens;
+  a.shared_pages = h.shared_pages;
+  a.own_tokens = h.own_tokens;
   const auto plan = ddb::kv_cache_attend_plan(a);
   torch::Tensor part;  // the call's own: calls on other streams and captured graphs have theirs
   if (plan.scratch) {

@@ -29,10 +29,6 @@
 // scores, merge). 5 tokens of 16 streams, 16 heads over 4 cached ones, window 2,048: 14.7 us a
 // call, 2.6 us of bytes: the 3 warps of a group each convert the page's codes, for 8 rows each, and only
 // 4 pages of a CTA are in work at once.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <atomic>
 
@@ -40,18 +36,13 @@
 #include "../common/tma.h"
 #include "attend.h"
 #include "masks.cuh"
+#include "rows.cuh"
 
 namespace ddb {
 namespace {
 
 constexpr int kGroups = 4;
 constexpr int kMaxStages = 6;
-constexpr int kPageBytes = 8192;  // keys, then values
-constexpr float kHeadroom = 15.f;  // log2 of what a weight of 1 is in fp16 (largest: 2^16 less a step)
-// Scores (log2) from which the rounding of a maximum, 2^-24 of it, moves the weights against it by
-// more than 2^(1/2), all alike; from 2^24 on they would overflow.
-constexpr float kFar = 8388608.f;
-constexpr int kPitch = 68;        // floats between result rows (their writes then hit distinct banks)
 
 // the CTA's result and its rows' (m, l) | barriers | page scales | flag | rings, later the
 // groups' results
@@ -65,33 +56,9 @@ constexpr int smem_bytes(int NT, int stages) { return off_ring(NT) + kGroups * s
 static_assert(kGroups * (out_floats(4) * 4 + 64 * 4) <= kGroups * 2 * kPageBytes, "results fit the rings");
 static_assert(smem_bytes(4, kMaxStages) <= 232448, "shared memory per CTA");
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t half2_of(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-// transposes an 8x8 matrix of 16-bit values held two to a lane (row lane / 4)
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
-template <int NT>
+// OWN: only the pages behind those that the sequence's group shares; kv_attend_past has the others'
+// part of each row.
+template <int NT, bool OWN>
 __global__ void __launch_bounds__(kGroups * NT * 32)
     kv_attend_rows(const KvAttendArgs a, int row_tiles, int stages, uint32_t group_inv, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -135,6 +102,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     const KvSpan s1 = kv_span(a, old + token(min(rows, r0 + R) - 1), len, first);
     lo_min = s0.lo, hi_min = s0.hi, lo_max = s1.lo, hi_max = s1.hi;
     pages = kv_pages(lo_min, hi_max, sinks, a.step.width);
+    if (OWN) pages = kv_pages_from(pages, min(max(a.step.rows[static_cast<long>(a.step.B + b / a.step.branches) * a.step.ld], 0), a.step.width));
   }
   const int part = rank * kGroups + pg, parts = ranks * kGroups;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
@@ -401,6 +369,7 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     *reinterpret_cast<float4*>(co + r * kPitch + d) = v;
     if (d == 0) cml[r] = make_float2(top, sum);
   }
+  if (OWN) asm volatile("griddepcontrol.wait;" ::: "memory");  // the other launch's part is written
   if (ranks > 1) cluster_sync_all(); else __syncthreads();
   // ---- the cluster's CTAs share the rows; each adds the others' parts in rank order
   const uint32_t so = smem_u32(co), sml = smem_u32(cml);
@@ -411,6 +380,27 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < ranks; ++k) top = fmaxf(top, ld_cluster_v2(ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8).x);
+    const float* past = nullptr;  // of the row's tile of its group
+    int past_row = 0;
+    if (OWN) {
+      const int n = a.step.branches, all = b % n * a.T * G + row_id, tiles = (n * a.T * G + a.past_rows - 1) / a.past_rows;
+      past_row = all % a.past_rows;
+      past = a.part + (static_cast<long>(b / n * a.pool.heads + kh) * tiles + all / a.past_rows) * a.past_ranks * kv_past_floats(a.past_rows);
+      for (int k = 0; k < a.past_ranks; ++k)
+        top = fmaxf(top, past[k * kv_past_floats(a.past_rows) + a.past_rows * 64 + past_row * 2]);
+    }
+    if (OWN && top != -INFINITY)
+      for (int k = 0; k < a.past_ranks; ++k) {
+        const float* p = past + k * kv_past_floats(a.past_rows);
+        const float2 x = *reinterpret_cast<const float2*>(p + a.past_rows * 64 + past_row * 2);
+        const float4 y = *reinterpret_cast<const float4*>(p + past_row * 64 + d);
+        const float w = exp2f(x.x - top);
+        sum += w * x.y;
+        v.x += w * y.x;
+        v.y += w * y.y;
+        v.z += w * y.z;
+        v.w += w * y.w;
+      }
     if (top != -INFINITY)
       for (int k = 0; k < ranks; ++k) {
         const uint32_t ml = ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8;
@@ -455,11 +445,11 @@ KvPlan rows_plan(const KvAttendArgs& a, int NT, int dev) {
   return p;
 }
 
-template <int NT>
+template <int NT, bool OWN>
 void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
+    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
                "cudaFuncSetAttribute(kv_attend_rows)");
     set.fetch_or(1ull << (dev & 63));
   }
@@ -476,13 +466,21 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   cfg.blockDim = dim3(kGroups * NT * 32);
   cfg.dynamicSmemBytes = smem_bytes(NT, stages);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = ranks > 1 ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, stages, 0xffffffffu / G + 1, device_status(dev)),
+  cfg.numAttrs = 0;
+  if (ranks > 1) {
+    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeClusterDimension;
+    x.val.clusterDim.x = ranks;
+    x.val.clusterDim.y = x.val.clusterDim.z = 1;
+  }
+  if (OWN) {  // beside the launch before it
+    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
+    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    x.val.programmaticStreamSerializationAllowed = 1;
+  }
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT, OWN>, a, tiles, stages, 0xffffffffu / G + 1, device_status(dev)),
              "kv_attend_rows launch");
   count_launch();
 }
@@ -506,13 +504,21 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
+  if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows) {
+    KvPlan split = kv_attend_past_plan(a, dev);
+    KvAttendArgs own = a;
+    own.max_tokens = a.own_tokens;
+    split.ranks = rows_plan(own, row_warps(rows), dev).ranks;
+    return split;
+  }
   const KvPlan few = rows <= kMaxRows ? rows_plan(a, row_warps(rows), dev) : KvPlan{};
   if (rows <= 32) return few;
   const KvPlan many = kv_attend_tiles_plan(a, dev);
   return rows > kMaxRows || many.us < few.us ? many : few;
 }
 
-void kv_cache_attend(const KvAttendArgs& a, const KvPlan& plan, cudaStream_t stream) {
+void kv_cache_attend(const KvAttendArgs& args, const KvPlan& plan, cudaStream_t stream) {
+  KvAttendArgs a = args;
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
@@ -520,11 +526,24 @@ void kv_cache_attend(const KvAttendArgs& a, const KvPlan& plan, cudaStream_t str
     kv_attend_tiles_launch(a, plan, dev, stream);
     return;
   }
-  switch (row_warps(a.T * static_cast<long>(a.H / a.pool.heads))) {
-    case 1: launch<1>(a, plan.ranks, dev, stream); break;
-    case 2: launch<2>(a, plan.ranks, dev, stream); break;
-    case 3: launch<3>(a, plan.ranks, dev, stream); break;
-    default: launch<4>(a, plan.ranks, dev, stream); break;
+  const int warps = row_warps(a.T * static_cast<long>(a.H / a.pool.heads));
+  if (plan.split) {
+    a.past_ranks = plan.past_ranks;
+    a.past_rows = plan.past_rows;
+    kv_attend_past_launch(a, dev, stream);
+    switch (warps) {
+      case 1: launch<1, true>(a, plan.ranks, dev, stream); break;
+      case 2: launch<2, true>(a, plan.ranks, dev, stream); break;
+      case 3: launch<3, true>(a, plan.ranks, dev, stream); break;
+      default: launch<4, true>(a, plan.ranks, dev, stream); break;
+    }
+    return;
+  }
+  switch (warps) {
+    case 1: launch<1, false>(a, plan.ranks, dev, stream); break;
+    case 2: launch<2, false>(a, plan.ranks, dev, stream); break;
+    case 3: launch<3, false>(a, plan.ranks, dev, stream); break;
+    default: launch<4, false>(a, plan.ranks, dev, stream); break;
   }
 }
 

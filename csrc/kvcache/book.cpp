@@ -276,6 +276,35 @@ void KvBook::rows(const Ids& ids, const Ids& n_new, int front, int32_t* out) con
   }
 }
 
+std::pair<int64_t, int64_t> KvBook::shared_rows(const Ids& ids, const Ids& n_new, int64_t branches, int32_t* out) const {
+  int64_t most = 0, own = 0;
+  for (size_t i = 0; i < ids.size(); i += branches) {
+    std::vector<const Seq*> group;
+    int64_t n = max_pages_;
+    for (int64_t k = 0; k < branches; ++k) {
+      group.push_back(&seq(ids[i + k]));
+      n = std::min(n, group[k]->length / kPage);
+    }
+    int32_t* pages = out + kFront;
+    std::copy_n(group[0]->pages.begin(), n, pages);
+    for (const Seq* s : group) {
+      if (std::equal(pages, pages + n, s->pages.begin())) continue;
+      for (int64_t j = 0; j < n; ++j) {  // a page that one sequence gave back is hidden from it alone
+        const int32_t p = s->pages[j];
+        if (pages[j] < 0) pages[j] = p;
+        else if (p >= 0 && p != pages[j]) n = j;
+      }
+    }
+    std::fill_n(out, kFront, 0);
+    out[0] = static_cast<int32_t>(n);
+    std::fill_n(pages + n, max_pages_ - n, -1);
+    out += kFront + max_pages_;
+    most = std::max(most, n);
+    for (int64_t k = 0; k < branches; ++k) own = std::max(own, group[k]->length + n_new[i + k] - n * kPage);
+  }
+  return {most, own};
+}
+
 KvBook::Ids KvBook::versions(const Ids& ids) const {
   Ids out;
   out.reserve(ids.size());

@@ -45,6 +45,11 @@ class KvBook {
   // A step's table, [sequences][front + max_pages]: front kFront writes the words that precede
   // the page ids too, 0 the ids alone.
   void rows(const Ids& seqs, const Ids& n_new, int front, int32_t* out) const;
+  // The pages that groups of `branches` consecutive sequences share, [groups][kFront + max_pages]: how
+  // many leading pages lie behind no sequence's new tokens and are the same for all that still have
+  // them, then their ids (-1: none has it). Returns the most such pages of a group, and the most
+  // tokens of a sequence behind its group's.
+  std::pair<int64_t, int64_t> shared_rows(const Ids& seqs, const Ids& n_new, int64_t branches, int32_t* out) const;
   // the sinks of the trimmed sequences (-1: none is, -2: they differ)
   int64_t trim_sinks(const Ids& seqs) const;
   int64_t longest(const Ids& seqs, const Ids& n_new) const;

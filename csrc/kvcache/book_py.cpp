@@ -15,13 +15,19 @@ torch::Tensor host_ints(const std::vector<int32_t>& v) {
   return t;
 }
 
-// (step rows, pages to copy from, to, longest sequence, sinks of the trimmed ones, versions)
-py::tuple kv_book_begin(ddb::KvBook& book, const ddb::KvBook::Ids& seqs, const ddb::KvBook::Ids& n_new, int64_t max_tokens) {
+// (step rows, behind them those of the groups' shared pages; pages to copy from, to, longest sequence,
+// sinks of the trimmed ones, versions, most shared pages, most tokens behind them)
+py::tuple kv_book_begin(ddb::KvBook& book, const ddb::KvBook::Ids& seqs, const ddb::KvBook::Ids& n_new, int64_t max_tokens,
+                        int64_t branches) {
+  const int64_t n = seqs.size();
+  if (branches < 1 || n % branches) throw std::invalid_argument("the sequences are no whole groups of branches");
   const auto copies = book.begin(seqs, n_new, max_tokens);
-  auto rows = torch::empty({static_cast<int64_t>(seqs.size()), ddb::KvBook::kFront + book.max_pages()}, torch::kInt32);
+  const int64_t groups = branches > 1 ? n / branches : 0, ld = ddb::KvBook::kFront + book.max_pages();
+  auto rows = torch::empty({n + groups, ld}, torch::kInt32);
   book.rows(seqs, n_new, ddb::KvBook::kFront, rows.data_ptr<int>());
+  const auto shared = groups ? book.shared_rows(seqs, n_new, branches, rows.data_ptr<int>() + n * ld) : std::pair<int64_t, int64_t>{0, 0};
   return py::make_tuple(rows, host_ints(copies.src), host_ints(copies.dst), book.longest(seqs, n_new), book.trim_sinks(seqs),
-                        book.versions(seqs));
+                        book.versions(seqs), shared.first, shared.second);
 }
 torch::Tensor kv_book_table(const ddb::KvBook& book, const ddb::KvBook::Ids& seqs) {
   auto rows = torch::empty({static_cast<int64_t>(seqs.size()), book.max_pages()}, torch::kInt32);

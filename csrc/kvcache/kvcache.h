@@ -15,6 +15,9 @@
 //   tokens in the cache with the call's own | the call's own tokens | first token kept
 //   behind the sinks (0: all) | sinks of a trimmed sequence, or -1 | page ids of the
 //   sequence, 64 tokens each (-1: none)
+// and, for groups of sequences that branched from one, behind them [group][4 + width]:
+//   whole pages behind which all the group's new tokens lie and that are the same for all
+//   sequences that still have them | three zeros | their ids (-1: no sequence has it)
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -38,6 +41,7 @@ struct KvStep {
   int ld = 0;     // words between rows
   int width = 0;  // page ids of a row
   int B = 0;
+  int branches = 1;  // groups of so many sequences; their rows follow the sequences' (1: none do)
 };
 
 struct KvWriteArgs {
@@ -72,12 +76,21 @@ struct KvAttendArgs {
   int max_tokens = 0;    // no sequence is longer (sets the launch's shape only)
   int ranks = 1;         // CTAs that share a row tile (set by the launch)
   float* part = nullptr; // the plan's scratch, 16-byte aligned
+  // of a step in groups of branches: the most pages that a group shares, and the most tokens of a
+  // sequence behind them (set the launch's shape only)
+  int shared_pages = 0;
+  int own_tokens = 0;
+  bool split = false;    // shared pages apart from the sequences' own (the plan's)
+  int past_ranks = 1;    // CTAs that share a row tile's shared pages
+  int past_rows = 32;    // rows of such a tile
 };
 
 // How a call is launched: the kernel, how many CTAs share a row tile's pages, and the scratch
 // that they meet in (0: distributed shared memory); with an estimate of its time.
 struct KvPlan {
   bool blocks = false;   // 256-row blocks (attend_tiles.cu), not few rows (attend_rows.cu)
+  bool split = false;    // a group's shared pages once for all its rows (attend_past.cu)
+  int past_ranks = 1, past_rows = 32;
   int ranks = 1;
   long scratch = 0;      // floats
   double us = 0.;

@@ -30,7 +30,8 @@ __device__ __forceinline__ uint32_t kv_bytes(uint32_t bits) { return ((bits & 15
 // and `hi` are the tile's smallest and largest (both grow with the position).
 struct KvPages {
   int n_sink, page0, n;
-  __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : page0 + i - n_sink; }
+  int skip = 0;  // sink pages left out
+  __device__ __forceinline__ int at(int i) const { return i < n_sink ? skip + i : page0 + i - n_sink; }
 };
 __device__ __forceinline__ KvPages kv_pages(int lo, int hi, int sinks, int width) {
   KvPages p;
@@ -39,6 +40,22 @@ __device__ __forceinline__ KvPages kv_pages(int lo, int hi, int sinks, int width
   p.n_sink = lo > 0 ? min((min(sinks, hi) + kKvPage - 1) / kKvPage, min(near, end)) : 0;
   p.page0 = near;
   p.n = p.n_sink + max(0, end - near);
+  return p;
+}
+
+// Of those the ones from page `from` on, or before it.
+__device__ __forceinline__ KvPages kv_pages_from(KvPages p, int from) {
+  const int near = p.page0 + p.n - p.n_sink;  // behind the last
+  p.skip = min(from, p.n_sink);
+  p.n_sink -= p.skip;
+  p.page0 = max(p.page0, from);
+  p.n = p.n_sink + max(0, near - p.page0);
+  return p;
+}
+__device__ __forceinline__ KvPages kv_pages_before(KvPages p, int to) {
+  const int near = min(p.page0 + p.n - p.n_sink, to);
+  p.n_sink = min(p.n_sink, to);
+  p.n = p.n_sink + max(0, near - p.page0);
   return p;
 }
 

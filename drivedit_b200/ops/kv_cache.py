@@ -77,9 +77,9 @@ class CacheStep:
     Once a sequence of the step has changed otherwise (commit, trim, fork, free, a later
     ``begin``, compaction) the step is stale and its calls raise."""
 
-    def __init__(self, cache: "PagedKVCache", seqs, n_new, versions, max_tokens, table, handle):
+    def __init__(self, cache: "PagedKVCache", seqs, n_new, versions, max_tokens, table, handle, branches=1):
         self.cache = cache
-        self.seqs, self.n_new = seqs, n_new
+        self.seqs, self.n_new, self.branches = seqs, n_new, branches
         self.max_tokens = max_tokens  # launches are shaped for sequences up to this length
         self._versions, self._epoch = versions, cache._book.epoch
         self._rows, self._h = table, handle
@@ -87,7 +87,7 @@ class CacheStep:
     @property
     def table(self) -> torch.Tensor:
         """Page ids by sequence, int32 ``[B, max_pages_per_seq]`` (-1: none)."""
-        return (self._rows if self._h is None else self._h.rows)[:, _INFO:]
+        return (self._rows if self._h is None else self._h.rows)[:len(self.seqs), _INFO:]
 
     def _check(self):
         book = self.cache._book
@@ -291,7 +291,7 @@ class PagedKVCache:
         return self._book.add(n)
 
     def begin(self, seqs: Sequence[int], n_new: Union[int, Sequence[int]], max_tokens: Optional[int] = None,
-              out: Optional[CacheStep] = None) -> CacheStep:
+              out: Optional[CacheStep] = None, branches: int = 1) -> CacheStep:
         """Make room for ``n_new`` tokens (one number, or one for each sequence) behind each
         sequence's committed ones. A shared unfinished page that they go into is copied first.
 
@@ -300,15 +300,24 @@ class PagedKVCache:
         longest of now. ``out``: a step of as many sequences to refill in place (on the current
         stream, behind the calls that still read it), so that a graph captured with it runs
         on the new tables; its ``max_tokens`` must suffice, ``n_new`` fit the rows of its captured
-        calls, and the sinks of windowed ones be those that the sequences were trimmed to."""
+        calls, and the sinks of windowed ones be those that the sequences were trimmed to.
+
+        ``branches``: the sequences are consecutive groups of that many which branched from one
+        (in the order of :meth:`fork`). ``attend`` then reads the whole pages that a group still
+        shares once for all its queries, where that is faster (few query rows a sequence); what
+        it computes is the same. It may differ from step to step, not between a step and its refill."""
         self._not_capturing("begin")
         seqs = list(seqs)
+        if branches < 1 or len(seqs) % branches:
+            raise ValueError(f"{len(seqs)} sequences are no whole groups of {branches} branches")
         n_new = [int(n) for n in n_new] if isinstance(n_new, (list, tuple)) else [int(n_new)] * len(seqs)
         if out is not None:
             if out.cache is not self or len(out.seqs) != len(seqs):
                 raise ValueError("out is a step of another cache or number of sequences")
             if out._rows.shape[1] != _INFO + self.max_pages_per_seq:
                 raise ValueError("out was begun before the cache grew")
+            if out.branches != branches:
+                raise ValueError(f"out keeps its groups of {out.branches} branches")
             max_tokens = out.max_tokens if max_tokens is None else max_tokens
             if max_tokens != out.max_tokens:
                 raise ValueError("out keeps its max_tokens")
@@ -316,16 +325,17 @@ class PagedKVCache:
                 ext().kv_step_check_refill(out._h, max(n_new, default=0), self._book.trim_sinks(seqs))
         if max_tokens is not None and max_tokens < 0:
             raise ValueError("max_tokens must not be negative")
-        rows, src, dst, longest, trim, versions = self._book.begin(seqs, n_new, -1 if max_tokens is None else int(max_tokens))
+        rows, src, dst, longest, trim, versions, shared, own = self._book.begin(
+            seqs, n_new, -1 if max_tokens is None else int(max_tokens), int(branches))
         max_tokens = longest if max_tokens is None else int(max_tokens)
         self._copy(src, dst)
         handle = None
         if self.device.type == "cuda":
             handle = ext().kv_step_begin(self.k, self.v, self.k_scale, self.v_scale, rows, max_tokens, max(n_new, default=0),
-                                         trim, None if out is None else out._h)
+                                         trim, branches, shared, own, None if out is None else out._h)
         if out is None:
-            return CacheStep(self, seqs, n_new, versions, max_tokens, rows, handle)
-        out.__init__(self, seqs, n_new, versions, max_tokens, rows, handle)
+            return CacheStep(self, seqs, n_new, versions, max_tokens, rows, handle, branches)
+        out.__init__(self, seqs, n_new, versions, max_tokens, rows, handle, branches)
         return out
 
     def fork(self, seqs: Sequence[int], copies: int = 1) -> List[int]:

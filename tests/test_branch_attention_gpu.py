@@ -1,0 +1,310 @@
+"""Attention of sequences that branched from one over the pages that they share, against the
+definition in 64 bits and the same call without the groups."""
+import math
+
+import pytest
+import torch
+
+from test_kv_cache_gpu import _cache, _check, _fill, _oracle, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _branches(c, ctx, n, more, scale=1.0):
+    """``n`` branches of each of the contexts, the i-th with ``more[i % len(more)]`` tokens of its own."""
+    roots = _fill(c, ctx, scale=scale)
+    kids = c.fork(roots, n)
+    c.free(roots)
+    more = [more[i % len(more)] for i in range(len(kids))]
+    T = max(max(more), 1)
+    step = c.begin(kids, more)
+    step.write(0, *(_randn(len(kids), T, c.n_heads, 64, scale=scale) for _ in "kv"))
+    step.commit()
+    return kids
+
+
+def _launches(call):
+    from drivedit_b200.ops._ext import ext
+    n = ext().launch_count()
+    out = call()
+    return out, ext().launch_count() - n
+
+
+CASES = [
+    # contexts, branches, tokens of their own (in turn), new tokens (in turn), cached heads, group, causal, unit, window, sinks
+    ([64], 2, [0], [1], 1, 1, "token", 1, 0, 0),
+    ([1500], 8, [0, 40, 3], [1], 3, 1, "token", 1, 0, 0),
+    ([200, 64, 700], 3, [5, 0, 64, 130], [1, 2, 1], 2, 1, "token", 1, 0, 0),
+    ([1000], 33, [1], [1], 1, 1, "token", 1, 0, 0),
+    ([4100], 5, [70, 0], [3], 2, 4, "token", 1, 0, 0),
+    ([2000, 300], 4, [10, 200], [5, 1, 0, 3], 2, 4, "token", 1, 600, 4),
+    ([3000], 6, [100], [2], 2, 2, "token", 1, 64, 130),     # the window lies behind the shared pages, the sinks in them
+    ([900], 4, [300, 100], [1], 1, 1, "token", 1, 50, 0),   # the window leaves nothing shared to see
+    ([1280], 4, [64], [64], 2, 1, "frame", 64, 0, 0),
+    ([980], 3, [0, 49], [49], 2, 2, "frame", 49, 7, 2),
+    ([700], 2, [0], [200], 1, 1, "token", 1, 0, 0),
+    ([500], 3, [9], [7], 2, 3, "none", 1, 0, 0),
+    ([640], 40, [0], [2], 1, 8, "token", 1, 0, 0),          # many rows to a head
+    ([20], 3, [5], [1], 2, 1, "token", 1, 0, 0),            # nothing whole to share
+    ([8000], 3, [0], [1], 12, 1, "token", 1, 0, 0),
+]
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_matches_definition(case):
+    ctx, n, more, own, KH, G, causal, unit, window, sinks = case
+    B = len(ctx) * n
+    own = [own[i % len(own)] for i in range(B)]
+    c = _cache(1, KH, sum(x // 64 + 1 for x in ctx) + B * ((max(more) + max(own)) // 64 + 3) + 2)
+    junk = c.add(1)
+    c.begin(junk, 65)
+    c.k.view(torch.uint8).fill_(0x7f)  # NaN wherever nothing is written
+    c.v.view(torch.uint8).fill_(0x7f)
+    seqs = _branches(c, ctx, n, more)
+    T = max(own) + 2
+    step = c.begin(seqs, own, branches=n)
+    step.write(0, *(_randn(B, T, KH, 64) for _ in "kv"))
+    q = _randn(B, T, 2, KH * G, 64, scale=2.0)[:, :, 1]
+    args = dict(causal=causal, tokens_per_frame=unit, window=window, sinks=sinks)
+    (o, lse), launches = _launches(lambda: step.attend(0, q, return_lse=True, **args))
+    if min(ctx) >= 64 and T * G <= 32:
+        assert launches == 2  # the shared pages, then the sequences' own
+    assert torch.equal(o, step.attend(0, q, **args))
+    step.commit()
+    for i, (s, m) in enumerate(zip(seqs, own)):
+        kk, vv = c.read(0, s)
+        ref, mean, rlse, mag = _oracle(kk, vv, q[i, :m], m, causal, unit, window, sinks)
+        _check(o[i, :m], lse[i, :, :m], ref, mean, rlse, mag)
+        assert not o[i, m:].any() and (lse[i, :, m:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("sinks", [0, 70])
+def test_trimmed_branches(sinks):
+    """Branches trimmed at different places, one not at all: pages that some gave back, some share."""
+    c = _cache(1, 2, 80)
+    seqs = _branches(c, [1200], 4, [0, 100, 30, 60])
+    full = [c.read(0, s) for s in seqs]
+    for s, keep in zip(seqs[:3], (400, 700, 300)):
+        c.trim([s], keep, sinks)
+    for branches, T in ((4, 2), (2, 1)):
+        step = c.begin(seqs, T, branches=branches)
+        step.write(0, *(_randn(4, T, 2, 64) for _ in "kv"))
+        q = _randn(4, T, 4, 64)
+        for window in (0, 350, 2000):
+            args = dict(causal="token", window=window, sinks=sinks if window else 0)
+            (o, lse), launches = _launches(lambda: step.attend(0, q, return_lse=True, **args))
+            assert launches == 2
+            for i, s in enumerate(seqs):
+                n = full[i][0].shape[0]
+                kk, vv = c._values(0, c._seqs[s], n + T)
+                first = n - (400, 700, 300, n)[i]
+                _check(o[i], lse[i], *_oracle(kk, vv, q[i], T, "token", 1, args["window"], args["sinks"], first, sinks))
+
+
+def test_groups_that_share_nothing():
+    """Sequences of one group that never had a page in common, and one that shares with another."""
+    c = _cache(1, 2, 60)
+    a = _branches(c, [300], 2, [10])
+    seqs = [a[0], *_fill(c, [500, 130]), a[1]]
+    for order in (seqs, [a[0], a[1], *seqs[1:3]]):
+        for n in (2, 4):
+            step = c.begin(order, 1, branches=n)
+            step.write(0, *(_randn(4, 1, 2, 64) for _ in "kv"))
+            q = _randn(4, 1, 2, 64)
+            o, lse = step.attend(0, q, causal="token", return_lse=True)
+            for i, s in enumerate(order):
+                kk, vv = c._values(0, c._seqs[s], c.length(s) + 1)
+                _check(o[i], lse[i], *_oracle(kk, vv, q[i], 1, "token", 1, 0, 0))
+
+
+def test_hidden_shared_tokens_do_not_matter():
+    """NaN at shared tokens that no branch sees, in pages that they see too."""
+    c = _cache(1, 2, 60)
+    seqs = _branches(c, [1500], 3, [0, 20])
+    step = c.begin(seqs, 1, branches=3)
+    step.write(0, *(_randn(3, 1, 2, 64) for _ in "kv"))
+    q = _randn(3, 1, 4, 64)
+    args = dict(causal="token", window=300, sinks=10)
+    want = step.attend(0, q, **args)
+    assert torch.isfinite(want).all()
+    for pos in range(10, 1201):
+        page = int(step.table[0, pos // 64])
+        c.k.view(torch.uint8)[0, page, :, pos % 64] = 0x7f
+        c.v.view(torch.uint8)[0, page, :, :, pos % 64] = 0x7f
+    assert torch.equal(step.attend(0, q, **args), want)
+
+
+@pytest.mark.parametrize("far", [2.0 ** e for e in (12, 20, 24, 30, 60)])
+def test_large_scores(far):
+    """Scores far from zero: rows stay finite, with the weights of their definition."""
+    c = _cache(1, 1, 40)
+    seqs = _branches(c, [900], 4, [10])
+    page = c.begin(seqs, 1).table[0, 3].long()
+    for at in (3, 9):
+        c.k_scale[0, c.begin(seqs, 1).table[0, at].long()] *= far
+    step = c.begin(seqs, 1, branches=4)
+    step.write(0, *(_randn(4, 1, 1, 64) for _ in "kv"))
+    q = _randn(4, 1, 2, 64)
+    o = step.attend(0, q, causal="token")
+    assert torch.isfinite(o).all() and page >= 0
+    for i, s in enumerate(seqs):
+        kk, vv = c._values(0, c._seqs[s], c.length(s) + 1)
+        ref, mean, _, mag = _oracle(kk, vv, q[i], 1, "token", 1, 0, 0)
+        # a score is a sum of 64 fp32 products (2^-18 of the magnitudes), so weights near the largest move
+        # by that much; where it passes 1 the row is one key's value, and which of two is not decided
+        if mag * 2.0 ** -18 < 2.0 ** -6:
+            err = (o[i].double() - ref).abs()
+            assert (err <= 2.0 ** -8 * ref.abs() + (2.0 ** -10 + 4 * mag * 2.0 ** -18) * mean).all()
+        else:
+            assert (o[i].double().abs() <= vv.double().abs().amax() * (1 + 2.0 ** -7)).all()
+
+
+@pytest.mark.parametrize("magnitude", [2.0 ** -60, 2.0 ** 40])
+def test_scales_exactly(magnitude):
+    outs = []
+    for f in (1.0, magnitude):
+        torch.manual_seed(3)
+        c = _cache(1, 1, 20)
+        seqs = _branches(c, [300], 3, [7], scale=f)
+        step = c.begin(seqs, 2, branches=3)
+        step.write(0, *(_randn(3, 2, 1, 64, scale=f) for _ in "kv"))
+        outs.append(step.attend(0, _randn(3, 2, 2, 64, scale=1 / f), causal="token"))
+    assert torch.equal(outs[0].float() * magnitude, outs[1].float())
+
+
+def test_nan_stays_in_its_rows():
+    c = _cache(1, 2, 40)
+    seqs = _branches(c, [500], 4, [10])
+    step = c.begin(seqs, 1, branches=4)
+    step.write(0, *(_randn(4, 1, 2, 64) for _ in "kv"))
+    q = _randn(4, 1, 4, 64)
+    want = step.attend(0, q, causal="token")
+    q[2, 0, 1, 5] = math.nan
+    o, lse = step.attend(0, q, causal="token", return_lse=True)
+    assert torch.isnan(o[2, 0, 1]).all() and torch.isnan(lse[2, 1, 0])
+    o[2, 0, 1] = want[2, 0, 1]
+    assert torch.equal(o, want)
+
+
+def test_run_of_branches():
+    """A run as a user makes it, over two layers, with query and key norms and positions: the
+    same with the groups named as without."""
+    from drivedit_b200.ops.rotary import qk_norm_rotary
+    a = torch.arange(400, dtype=torch.float64, device="cuda")[:, None] * 10000.0 ** (-torch.arange(0, 64, 2, device="cuda") / 64)
+    tab = torch.stack([a.cos(), a.sin()], -1).float().contiguous()
+    w = torch.rand(64, device="cuda")
+    outs = []
+    for branches in (1, 5):
+        torch.manual_seed(2)
+        c, got = _cache(2, 2, 60), []
+
+        def run(seqs, T, branches=1):
+            step = c.begin(seqs, T, branches=branches)
+            at = torch.tensor([c.length(s) for s in seqs], device="cuda")[:, None] + torch.arange(T, device="cuda")
+            for layer in range(2):
+                qkv = _randn(len(seqs), T, 8, 64)
+                q, k = qk_norm_rotary(qkv[:, :, :4], qkv[:, :, 4:6], w, w, tab, at, inplace=True)
+                step.write(layer, k, qkv[:, :, 6:])
+                got.append(step.attend(layer, q, causal="token", window=250, sinks=3))
+            step.commit()
+
+        roots = c.add(2)
+        run(roots, 200)
+        kids = c.fork(roots, 5)
+        c.free(roots)
+        for i in range(70):
+            run(kids, 1, branches)
+            c.trim(kids, 250, 3)
+        c.free(kids[5:])
+        run(kids[:5], 2, branches)
+        outs.append(got)
+    for x, y in zip(*outs):
+        # P in fp16 and the order of fp32 sums, then a bf16 rounding each
+        assert ((x.float() - y.float()).abs() <= 2.0 ** -7 * y.float().abs() + 2.0 ** -10 * y.float().abs().max()).all()
+
+
+def test_capture_and_refill():
+    """A captured step of branches, replayed while what they share shrinks and the sequences grow."""
+    c = _cache(1, 2, 120)
+    seqs = _branches(c, [700, 300], 3, [0, 10])
+    k, v, q = (_randn(6, 1, 2, 64) for _ in "kvq")
+    step = c.begin(seqs, 1, max_tokens=1200, branches=3)
+    step.write(0, k, v)
+    step.attend(0, q, causal="token", window=400, sinks=2)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=other):
+        step.write(0, k, v)
+        o, lse = step.attend(0, q, causal="token", window=400, sinks=2, return_lse=True)
+    for i in range(150):
+        for t in (k, v, q):
+            t.copy_(_randn(6, 1, 2, 64))
+        c.begin(seqs, 1, out=step, branches=3)
+        graph.replay()
+        if i % 30 == 0 or i > 145:
+            for j, s in enumerate(seqs):
+                kk, vv = c._values(0, c._seqs[s], c.length(s) + 1)
+                _check(o[j], lse[j], *_oracle(kk, vv, q[j], 1, "token", 1, 400, 2, c._seqs[s].first, c._seqs[s].sinks))
+        step.commit()
+        if i % 10 == 9:
+            c.trim(seqs, 400, 2)
+        if i == 140:  # nothing in common any more
+            new = c.copy(seqs)
+            c.free(seqs)
+            seqs = new
+    with pytest.raises(ValueError):
+        c.begin(seqs, 1, out=step)
+
+
+def test_two_streams_and_graphs_at_once():
+    """Calls of two steps on two streams, and two captured ones replayed together, keep to themselves."""
+    c = _cache(1, 2, 200)
+    calls, want = [], []
+    for i in range(2):
+        seqs = _branches(c, [3000 - 700 * i], 6, [10 + i])
+        step = c.begin(seqs, 1, branches=6)
+        step.write(0, *(_randn(6, 1, 2, 64) for _ in "kv"))
+        q = _randn(6, 1, 8, 64)
+        calls.append(lambda step=step, q=q: step.attend(0, q, causal="token"))
+        want.append(calls[i]())
+    streams = [torch.cuda.Stream() for _ in "ab"]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s, call in zip(streams, calls):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            outs.append(call())
+    for _ in range(20):
+        got = []
+        for s, call, graph in zip(streams, calls, graphs):
+            with torch.cuda.stream(s):
+                got.append(call())
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got + outs, want + want))
+
+
+def test_refusals_and_empty_calls():
+    c = _cache(1, 2, 20)
+    seqs = _branches(c, [200], 4, [3])
+    for n in (3, 0, -1, 8):
+        with pytest.raises(ValueError):
+            c.begin(seqs, 1, branches=n)
+    step = c.begin(seqs, 1, branches=4)
+    assert step.table.shape[0] == 4
+    with pytest.raises(ValueError):
+        step.attend(0, _randn(5, 1, 2, 64))
+    with pytest.raises(ValueError):
+        c.begin(seqs, 1, out=step, branches=2)
+    c.begin(seqs, 1, out=step, branches=4)
+    with pytest.raises(ValueError):
+        step.attend(0, _randn(4, 0, 2, 64))
+    none = c.begin(seqs, 0, branches=4)
+    o, lse = none.attend(0, _randn(4, 3, 2, 64), causal="token", return_lse=True)
+    assert not o.any() and (lse == -math.inf).all()
+    assert none.attend(0, _randn(4, 0, 2, 64)).shape == (4, 0, 2, 64)
+    empty = c.begin([], 1, branches=4)
+    assert empty.attend(0, _randn(0, 1, 2, 64)).shape == (0, 1, 2, 64)
+    from drivedit_b200.ops._ext import device_status
+    assert device_status() == 0
