@@ -29,6 +29,10 @@ inline long kv_past_tiles(const KvAttendArgs& a, int rows) { return (kv_group_ro
 KvPlan kv_attend_past_plan(const KvAttendArgs& a, int dev);  // split, past_ranks, past_rows, scratch, us
 void kv_attend_past_launch(const KvAttendArgs& a, int dev, cudaStream_t stream);
 
+// the same by blocks of 256 rows (attend_tiles.cu)
+KvPlan kv_past_tiles_plan(const KvAttendArgs& a, int dev);
+void kv_past_tiles_launch(const KvAttendArgs& a, int dev, cudaStream_t stream);
+
 // attend_tiles.cu: blocks of 256 rows on the tensor cores' 128-row products
 KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev);
 void kv_attend_tiles_launch(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream);

@@ -506,6 +506,7 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
   const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
   if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows) {
     KvPlan split = kv_attend_past_plan(a, dev);
+    if (kv_group_rows(a) > 128) split = kv_past_tiles_plan(a, dev);
     KvAttendArgs own = a;
     own.max_tokens = a.own_tokens;
     split.ranks = rows_plan(own, row_warps(rows), dev).ranks;
@@ -522,7 +523,7 @@ void kv_cache_attend(const KvAttendArgs& args, const KvPlan& plan, cudaStream_t 
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  if (plan.blocks) {
+  if (plan.blocks && !plan.split) {
     kv_attend_tiles_launch(a, plan, dev, stream);
     return;
   }
@@ -530,7 +531,7 @@ void kv_cache_attend(const KvAttendArgs& args, const KvPlan& plan, cudaStream_t 
   if (plan.split) {
     a.past_ranks = plan.past_ranks;
     a.past_rows = plan.past_rows;
-    kv_attend_past_launch(a, dev, stream);
+    (plan.blocks ? kv_past_tiles_launch : kv_attend_past_launch)(a, dev, stream);
     switch (warps) {
       case 1: launch<1, true>(a, plan.ranks, dev, stream); break;
       case 2: launch<2, true>(a, plan.ranks, dev, stream); break;

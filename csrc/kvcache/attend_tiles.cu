@@ -98,6 +98,8 @@ __device__ __forceinline__ float log2_of_power(float p) { return static_cast<flo
 // every warp has its role's registers
 __device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
+// PAST: rows of all sequences of a group over the pages that it shares (attend.h).
+template <bool PAST>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_attend_tiles(const KvAttendArgs a, int row_tiles, int* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -128,23 +130,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   // largest key scale of the CTA's pages (positive floats order like their bits)
   int* k_most = reinterpret_cast<int*>(smem + OFF_MISC + 8);
 
+  if (PAST) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = warp_id(), lane = lane_id();
-  const int ranks = a.ranks, rank = blockIdx.x % ranks;
+  const int ranks = PAST ? a.past_ranks : a.ranks, rank = blockIdx.x % ranks;
   int item = blockIdx.x / ranks;
   const int tile = row_tiles - 1 - item % row_tiles;  // long (late) tiles first
   item /= row_tiles;
-  const int kh = item % a.pool.heads, b = item / a.pool.heads;
-  const int G = a.H / a.pool.heads;
-  const int* row = a.step.rows + static_cast<long>(b) * a.step.ld;
+  const int kh = item % a.pool.heads, b = item / a.pool.heads;  // PAST: b is a group
+  const int G = a.H / a.pool.heads, TG = a.T * G;
+  const int* row = a.step.rows + static_cast<long>(PAST ? a.step.B + b : b) * a.step.ld;
   const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
-  const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
-  const int r0 = tile * kRows, rows = own * G;       // rows behind `rows` are padding
+  int sinks = row[3] >= 0 ? row[3] : a.sinks;        // a trimmed sequence has its own
+  // rows behind `rows` are padding
+  const int r0 = tile * kRows, rows = PAST ? a.step.branches * TG : own * G;
   const int n_t = rows - r0 > 128 ? 2 : 1;
 
   // the block's pages, and this CTA's run of key tiles (page pairs)
   KvPages pages{0, 0, 0};
   KvSpan all{0, 0};
-  if (r0 < rows) {
+  // PAST: a row's sequence and token, the shared keys that it sees and its sinks; it sees none if it is padding
+  const int* seq = nullptr;
+  int seq_token = 0, seq_sinks = 0;
+  const int P = PAST ? min(max(row[0], 0), a.step.width) : 0;
+  KvSpan seq_span{0x7fffffff, P * kKvPage};
+  auto past_row = [&](int r) {
+    if (r >= rows) return;
+    const int i = r / TG;
+    seq = a.step.rows + (static_cast<long>(b) * a.step.branches + i) * a.step.ld;
+    seq_token = (r - i * TG) / G;
+    if (seq_token >= min(seq[1], a.T)) return;
+    seq_span.lo = kv_span(a, seq[0] - seq[1] + seq_token, seq[0], seq[2]).lo;
+    seq_sinks = seq[3] >= 0 ? seq[3] : a.sinks;
+  };
+  if (PAST) {
+    // the smallest and largest of the block's rows; every key of a shared page is before all of them
+    int* low = reinterpret_cast<int*>(smem + OFF_RAW);  // not yet in use
+    past_row(r0 + (threadIdx.x & 255));
+    if (threadIdx.x < 256) {
+      const int lo = __reduce_min_sync(0xffffffffu, seq_span.lo), most = __reduce_max_sync(0xffffffffu, seq_sinks);
+      if (lane == 0) low[warp] = lo, low[8 + warp] = most;
+    }
+    __syncthreads();
+    all.lo = low[0], sinks = low[8];
+    for (int w = 1; w < 8; ++w) all.lo = min(all.lo, low[w]), sinks = max(sinks, low[8 + w]);
+    all.hi = P * kKvPage;
+    if (all.lo != 0x7fffffff) pages = kv_pages_before(kv_pages(all.lo, P * kKvPage, sinks, a.step.width), P);
+    __syncthreads();  // before copies land there
+  } else if (r0 < rows) {
     const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
     const KvSpan s1 = kv_span(a, old + (min(rows, r0 + kRows) - 1) / G, len, first);
     all = KvSpan{s0.lo, s1.hi};
@@ -214,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int i = 2 * (j0 + j) + lane;
           ids = i < min(pages.n, 2 * (j0 + n)) ? row[kKvInfo + pages.at(i)] : -2;
           if (ids != -2 && static_cast<unsigned>(ids) >= static_cast<unsigned>(a.pool.pages)) {
-            record_bad_index(status, ids);  // recorded, read as zeros
+            // recorded, read as zeros (but for a page that no sequence of a group has any more)
+            if (!PAST || ids != -1) record_bad_index(status, ids);
             ids = -2;
           }
           ks = vs = 0.f;
@@ -408,14 +441,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool active = t < n_t;  // of a second tile that is all padding nothing is computed
     const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     // a padding row keeps zeros and the span of the last row: its result is not used
-    const KvSpan span = kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
+    const KvSpan span = PAST ? seq_span : kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
+    const int row_sinks = PAST ? seq_sinks : sinks;
     float sl2, bound;
     {
       uint4 w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + (r / G) * a.q_st +
+      if (PAST ? seq_span.lo != 0x7fffffff : r < rows) {
+        const int s = PAST ? b * a.step.branches + r / TG : b, tok = PAST ? seq_token : r / G;
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + s * a.q_sb + tok * a.q_st +
                                  (kh * G + r % G) * a.q_sh;
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = ld_global_v4(q + i * 8);
@@ -495,8 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int p = 0; p < 2; ++p) {
           const int i = 2 * (j0 + j) + p;
           const int key = i < pages.n ? pages.at(i) * kKvPage : 0x40000000;  // no page: no key
-          if (!(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= sinks))) {
-            const uint64_t see = kv_bits(span, sinks, key);
+          if (!(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= row_sinks))) {
+            const uint64_t see = kv_bits(span, row_sinks, key);
             const uint32_t word[2] = {static_cast<uint32_t>(see), static_cast<uint32_t>(see >> 32)};
 #pragma unroll
             for (int c = 0; c < 64; ++c)
@@ -628,10 +663,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
     if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores
-    if (a.part) {
+    if (PAST || a.part) {
       // 256 rows of 64 channels, then their (maximum, sum), for kv_tiles_merge
-      float* part = a.part + blockIdx.x * kPartFloats;
-      if (r < a.T * G) {
+      const long at = PAST ? ((static_cast<long>(b) * a.pool.heads + kh) * row_tiles + tile) * ranks + rank : blockIdx.x;
+      float* part = a.part + at * kPartFloats;
+      if (r < (PAST ? rows : TG)) {
         float* o = part + (t * 128 + lr) * 64;
 #pragma unroll
         for (int c = 0; c < 16; ++c)
@@ -667,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (ranks > 1 && !a.part) {
+  if (!PAST && ranks > 1 && !a.part) {
     // ---- each CTA of the cluster adds up its share of the rows, in rank order; 16 threads a
     // row, 4 channels each
     cluster_sync_all();
@@ -740,7 +776,9 @@ namespace {
 void raise_limit(int dev) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (set.load() >> (dev & 63) & 1) return;
-  check_cuda(cudaFuncSetAttribute(kv_attend_tiles, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+  check_cuda(cudaFuncSetAttribute(kv_attend_tiles<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+             "cudaFuncSetAttribute(kv_attend_tiles)");
+  check_cuda(cudaFuncSetAttribute(kv_attend_tiles<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
              "cudaFuncSetAttribute(kv_attend_tiles)");
   set.fetch_or(1ull << (dev & 63));
 }
@@ -780,7 +818,7 @@ KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev) {
     if (slots == 0) {
       cudaLaunchAttribute attr[1];
       const cudaLaunchConfig_t cfg = config(s, attr);
-      check_cuda(cudaOccupancyMaxActiveClusters(&slots, kv_attend_tiles, &cfg), "cudaOccupancyMaxActiveClusters");
+      check_cuda(cudaOccupancyMaxActiveClusters(&slots, kv_attend_tiles<false>, &cfg), "cudaOccupancyMaxActiveClusters");
       slots = std::max(slots, 1);
       fits[dev & 63][s].store(slots);
     }
@@ -806,13 +844,37 @@ void kv_attend_tiles_launch(KvAttendArgs a, const KvPlan& plan, int dev, cudaStr
   cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.stream = stream;
   cfg.numAttrs = plan.ranks > 1 && !a.part ? 1 : 0;
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles, a, row_blocks(a), device_status(dev)), "kv_attend_tiles launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_tiles<false>, a, row_blocks(a), device_status(dev)), "kv_attend_tiles launch");
   count_launch();
   if (a.part) {
     kv_tiles_merge<<<static_cast<unsigned>(row_items(a) * (kRows / 16)), 256, 0, stream>>>(a, row_blocks(a));
     check_cuda(cudaGetLastError(), "kv_tiles_merge launch");
     count_launch();
   }
+}
+
+KvPlan kv_past_tiles_plan(const KvAttendArgs& a, int dev) {
+  const long rows = kv_group_rows(a), items = a.step.B / a.step.branches * static_cast<long>(a.pool.heads) * kv_past_tiles(a, kRows);
+  const int pairs = static_cast<int>((std::min<long>(a.shared_pages, kv_seen_pages(a)) + 1) / 2);
+  const double step = rows > 128 ? 1.75 : 1.3;
+  KvPlan best;
+  best.split = best.blocks = true;
+  best.past_rows = kRows;
+  for (int s = 1; s == 1 || (s <= 16 && pairs >= 2 * s && items * s <= 4L * num_sms(dev)); ++s) {
+    const double us = static_cast<double>((items * s + num_sms(dev) - 1) / num_sms(dev)) * (15. + step * ((pairs + s - 1) / s)) + items * s * 0.015;
+    if (s == 1 || us < best.us) best.past_ranks = s, best.us = us;
+  }
+  best.scratch = items * best.past_ranks * kPartFloats;
+  return best;
+}
+
+void kv_past_tiles_launch(const KvAttendArgs& a, int dev, cudaStream_t stream) {
+  raise_limit(dev);
+  const long tiles = kv_past_tiles(a, kRows), ctas = a.step.B / a.step.branches * static_cast<long>(a.pool.heads) * tiles * a.past_ranks;
+  if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  kv_attend_tiles<true><<<static_cast<unsigned>(ctas), kThreads, SMEM_BYTES, stream>>>(a, static_cast<int>(tiles), device_status(dev));
+  check_cuda(cudaGetLastError(), "kv_attend_tiles launch");
+  count_launch();
 }
 
 }  // namespace ddb
