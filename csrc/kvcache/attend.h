@@ -19,19 +19,20 @@ inline int kv_seen_pages(const KvAttendArgs& a) {
   return static_cast<int>(((a.window > 0 && near < all ? near : all) + kKvPage - 1) / kKvPage);
 }
 
-// attend_past.cu: the pages that groups of branches share, for the rows of all their sequences at
-// once. What it finds of a row goes into a.part, for kv_attend_rows to add: of tile i (of
-// a.past_rows rows; heads before groups) and CTA k of a.past_ranks, [i][k]: unnormalised outputs
-// [row][64], then (maximum, sum) [row].
-__host__ __device__ constexpr long kv_past_floats(int rows) { return rows * 66L; }
+// attend_branches.cu: groups of branches. A block of rows (of all the group's sequences) walks the
+// pages that the group shares, then each of its sequences' own. What a CTA finds goes into a.part:
+// of block i (heads before groups) and CTA k of a.ranks, [i][k]: unnormalised outputs [row][64],
+// then (maximum, sum) [row]; a second launch adds it up.
+constexpr long kv_part_floats(int rows) { return rows * 66L; }
 inline long kv_group_rows(const KvAttendArgs& a) { return a.step.branches * static_cast<long>(a.T) * (a.H / a.pool.heads); }
-inline long kv_past_tiles(const KvAttendArgs& a, int rows) { return (kv_group_rows(a) + rows - 1) / rows; }
-KvPlan kv_attend_past_plan(const KvAttendArgs& a, int dev);  // split, past_ranks, past_rows, scratch, us
-void kv_attend_past_launch(const KvAttendArgs& a, int dev, cudaStream_t stream);
-
-// the same by blocks of 256 rows (attend_tiles.cu)
-KvPlan kv_past_tiles_plan(const KvAttendArgs& a, int dev);
-void kv_past_tiles_launch(const KvAttendArgs& a, int dev, cudaStream_t stream);
+// row blocks of all groups and heads
+inline long kv_group_blocks(const KvAttendArgs& a, int rows) {
+  return a.step.B / a.step.branches * static_cast<long>(a.pool.heads) * ((kv_group_rows(a) + rows - 1) / rows);
+}
+KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev);  // (kv_set_branch_mode)
+void kv_attend_branches(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream);
+// the first launch by blocks of 256 rows (attend_tiles.cu)
+void kv_attend_group_tiles(const KvAttendArgs& a, int dev, cudaStream_t stream);
 
 // attend_tiles.cu: blocks of 256 rows on the tensor cores' 128-row products
 KvPlan kv_attend_tiles_plan(const KvAttendArgs& a, int dev);

@@ -1,0 +1,496 @@
+// Attention of branches over the cache: what a group of sequences shares is read once for the queries
+// of all.
+//
+// Rows are (sequence of the group, token, query head of the group of heads). A block of rows walks
+// a list of pages: the shared ones that some row sees, then its sequences' own, each of which
+// the others' rows do not see. Blocks of 8 or 16 rows (here) where there are few, of 256
+// (attend_tiles.cu) where there are many; CTAs that share a block's pages leave their part of
+// each row in scratch, and a second launch adds the parts up, in a fixed order.
+//
+// One CTA here = 8 * NJ rows and a share of the block's pages, as 16 warps with pages of their
+// own, each with all the rows: a code is brought to fp16 once for NJ 8-row products, and no
+// warp waits for another until the end. Formats, permutations and the softmax are those of
+// attend_rows.cu (S^T = K Q^T, O^T = V^T P^T with the codes as the 16-row operand of the
+// 16x8x16 instruction), two numbers to an fp32 instruction. The keys of the warp's next two
+// pages and the values of its next one are on their way while it works: 16 warps with
+// two whole pages each do not fit the shared memory.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "../common/tma.h"
+#include "attend.h"
+#include "masks.cuh"
+#include "rows.cuh"
+
+namespace ddb {
+namespace {
+
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+
+// Of each warp: two places for a page's keys, one for its values, their barriers, and what is known
+// of the page in work and the three behind it. Of the block: its rows, sequences and pages.
+constexpr int kRing = 3 * 4096;
+constexpr int OFF_PAGES = kWarps * 3 * 8;
+constexpr int OFF_BRANCH = OFF_PAGES + kWarps * 4 * 16;
+constexpr int OFF_ROWS = OFF_BRANCH + kWarps * 4 * 4;
+constexpr int OFF_TABLE = OFF_ROWS + 16 * 16;
+constexpr int OFF_LOW = OFF_TABLE + 16 * 16;
+constexpr int OFF_FLAG = OFF_LOW + 16;
+constexpr int OFF_RING = (OFF_FLAG + 16 + 127) / 128 * 128;
+constexpr int SMEM_BYTES = OFF_RING + kWarps * kRing;
+static_assert(OFF_PAGES % 16 == 0 && OFF_BRANCH % 16 == 0 && OFF_ROWS % 16 == 0 && OFF_FLAG % 16 == 0, "alignment");
+static_assert(16 * (kPitch * 4 + 8) <= kRing, "a warp's results fit its ring");
+static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+
+template <int NJ>
+__global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArgs a, int row_tiles, int* status) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int R = 8 * NJ;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = warp_id(), lane = lane_id();
+  const int g = lane >> 2, c = lane & 3;
+  const int ranks = a.ranks, rank = blockIdx.x % ranks;
+  int item = blockIdx.x / ranks;
+  const int r0 = item % row_tiles * R;
+  item /= row_tiles;
+  const int kh = item % a.pool.heads;
+  const KvGroup grp(a, item / a.pool.heads);
+
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem) + warp * 3;  // [2], then the values'
+  uint64_t* v_full = k_full + 2;
+  float4* known = reinterpret_cast<float4*>(smem + OFF_PAGES) + warp * 4;  // scales, id, first key
+  int* branch_of = reinterpret_cast<int*>(smem + OFF_BRANCH) + warp * 4;
+  int4* spans = reinterpret_cast<int4*>(smem + OFF_ROWS);  // lo, hi, sinks, sequence in the block
+  KvBranch* table = reinterpret_cast<KvBranch*>(smem + OFF_TABLE);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_FLAG);
+  uint8_t* ring = smem + OFF_RING + warp * kRing;
+  if (lane == 0) {
+    for (int s = 0; s < 3; ++s) mbar_init(&k_full[s], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  // Q: row g of each 8, channels 16c..16c+15
+  uint4 qraw[NJ][2];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    qraw[j][0] = qraw[j][1] = make_uint4(0, 0, 0, 0);
+    const KvGroupRow x = grp.row(r0 + j * 8 + g);
+    if (x.span.lo != kNoKey) {
+      const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + grp.seq(x.i) * a.q_sb + x.t * a.q_st + (kh * grp.G + x.g) * a.q_sh + 16 * c;
+      qraw[j][0] = ld_global_v4(q);
+      qraw[j][1] = ld_global_v4(q + 8);
+    }
+  }
+  if (threadIdx.x < R) {
+    const KvGroupRow x = grp.row(r0 + threadIdx.x);
+    spans[threadIdx.x] = make_int4(x.span.lo, x.span.hi, x.sinks, x.i - r0 / grp.TG);
+  }
+  const KvGroupPages pages = kv_group_pages<R>(grp, r0, table, reinterpret_cast<int*>(smem + OFF_LOW));
+  const int part = rank * kWarps + warp, parts = ranks * kWarps;
+  const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
+
+  // the warp's next 32 pages, one a lane: id (-1: not in the pool), index, sequence and scales
+  int ids = -1, index = 0, branch = -1;
+  float ks = 0.f, vs = 0.f;
+  auto issue_keys = [&](int i) {  // of the warp's page i, and what is known of it
+    if ((i & 31) == 0) {
+      const int k = part + (i + lane) * parts;
+      ids = -1;
+      if (k < pages.n) {
+        int id;
+        pages.at(grp, table, k, index, branch, id);
+        if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages)) {
+          ids = id;
+          ks = a.pool.k_scale[static_cast<long>(id) * a.pool.heads + kh];
+          vs = a.pool.v_scale[static_cast<long>(id) * a.pool.heads + kh];
+        } else if (id != -1 || branch >= 0) {  // recorded, hidden (no sequence sees a shared page that none has)
+          record_bad_index(status, id);
+        }
+      }
+    }
+    // the copies first: the scales may still be on their way
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    if (lane == 0) {
+      bulk_load(ring + (i & 1) * 4096, a.pool.k + (static_cast<long>(max(id, 0)) * a.pool.heads + kh) * 4096, 4096, &k_full[i & 1]);
+      if (i == 0) bulk_load(ring + 8192, a.pool.v + (static_cast<long>(max(id, 0)) * a.pool.heads + kh) * 4096, 4096, v_full);
+    }
+    const int at = __shfl_sync(0xffffffffu, index, i & 31), br = __shfl_sync(0xffffffffu, branch, i & 31);
+    const float kf = __shfl_sync(0xffffffffu, ks, i & 31), vf = __shfl_sync(0xffffffffu, vs, i & 31);
+    if (lane == 0) {
+      known[i & 3] = make_float4(kf, vf, __int_as_float(id), __int_as_float(at * kKvPage));
+      branch_of[i & 3] = br;
+      mbar_arrive_expect_tx(&k_full[i & 1], 4096);
+      if (i == 0) mbar_arrive_expect_tx(v_full, 4096);
+    }
+  };
+  auto issue_values = [&](int i) {  // of a page whose keys have been issued
+    if (lane == 0) {
+      const int id = __float_as_int(known[i & 3].z);
+      bulk_load(ring + 8192, a.pool.v + (static_cast<long>(max(id, 0)) * a.pool.heads + kh) * 4096, 4096, v_full);
+      mbar_arrive_expect_tx(v_full, 4096);
+    }
+  };
+  if (mine > 0) issue_keys(0);  // and its values
+  if (mine > 1) issue_keys(1);
+
+  uint32_t qf[NJ][4][2];
+  float sl2[NJ][2];  // score factors of rows 8j + 2c and 8j + 2c + 1, which this lane's scores belong to
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t ws[4] = {qraw[j][i].x, qraw[j][i].y, qraw[j][i].z, qraw[j][i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack_bf16(ws[k]);
+        x[i * 8 + 2 * k] = f.x;
+        x[i * 8 + 2 * k + 1] = f.y;
+      }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int e = row_exponent(amax);
+    const float down = __int_as_float((127 - e) << 23);
+    const float up = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      qf[j][s][0] = pack_half(x[4 * s] * down, x[4 * s + 1] * down);
+      qf[j][s][1] = pack_half(x[4 * s + 2] * down, x[4 * s + 3] * down);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) sl2[j][u] = __shfl_sync(0xffffffffu, up, (2 * c + u) * 4);
+  }
+
+  float m[NJ][2], l[NJ][2];
+  float o[NJ][4][4];  // channels 16 i + g, + 8 of rows 8j + 2c, 2c + 1
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    m[j][0] = m[j][1] = -INFINITY;
+    l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[j][i][k] = 0.f;
+  }
+
+  const int krow = 16 * (g >> 1) + (g & 1);
+  bool ok = true;
+  for (int i = 0; i < mine; ++i) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&k_full[i & 1], i >> 1 & 1, abort_flag));
+    if (!ok) break;
+    const uint32_t sk = smem_u32(ring + (i & 1) * 4096), sv = smem_u32(ring + 8192);
+    const float4 f = known[i & 3];
+    const int br = branch_of[i & 3];
+    const bool there = __float_as_int(f.z) >= 0;
+    const int key0 = __float_as_int(f.w);
+
+    float s[NJ][4][4];  // keys krow + 4 t (and 2 behind it) of rows 8j + 2c, 2c + 1
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint4 w0 = lds128(sk + (krow + 4 * t) * 64 + c * 16), w1 = lds128(sk + (krow + 4 * t + 2) * 64 + c * 16);
+      const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (k == 0) mma_f16_zero(s[j][t], av, qf[j][k][0], qf[j][k][1]);
+          else mma_f16(s[j][t], av, qf[j][k][0], qf[j][k][1]);
+      }
+    }
+    __syncwarp();  // every lane has read the keys
+    if (i + 2 < mine) issue_keys(i + 2);
+    // a page that every row of the block sees whole needs no mask
+    const bool whole = there && br < 0 && (key0 >= pages.lo_max || key0 + kKvPage <= pages.sinks_min);
+    auto rest = [&](auto masked) -> bool {  // of the page: its softmax and P V
+      constexpr bool kMasked = decltype(masked)::value;
+    uint32_t pf[NJ][4][2];
+    float2 alpha[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float fu[2], use[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        fu[u] = sl2[j][u] * f.x;
+        if constexpr (kMasked) {
+          const int4 span = spans[j * 8 + 2 * c + u];
+          const uint32_t see = there && (br < 0 || br == span.w) ? static_cast<uint32_t>(kv_bits(KvSpan{span.x, span.y}, span.z, key0) >> krow) : 0u;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (!(see >> (4 * t + 2 * k) & 1)) s[j][t][2 * k + u] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(s[j][0][u], s[j][0][2 + u]), fmaxf(s[j][1][u], s[j][1][2 + u]));
+        mx = fmaxf(mx, fmaxf(fmaxf(s[j][2][u], s[j][2][2 + u]), fmaxf(s[j][3][u], s[j][3][2 + u])));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float top = mx == -INFINITY ? m[j][u] : fmaxf(m[j][u], __fmul_rn(mx, fu[u]));
+        use[u] = top == -INFINITY ? 0.f : top;
+        (u ? alpha[j].y : alpha[j].x) = exp2f(m[j][u] - use[u]);
+        m[j][u] = top;
+      }
+      float2 up = make_float2(kHeadroom - use[0], kHeadroom - use[1]), by = make_float2(fu[0], fu[1]);
+      if (__any_sync(0xffffffffu, fmaxf(fabsf(use[0]), fabsf(use[1])) >= kFar)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (fabsf(use[u]) >= kFar) {  // products rounded as the maximum's was: none passes it
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) s[j][t][2 * k + u] = __fadd_rn(__fmul_rn(s[j][t][2 * k + u], fu[u]), -use[u]);
+            (u ? up.y : up.x) = kHeadroom;
+            (u ? by.y : by.x) = 1.f;
+          }
+      }
+      float2 sum = both(0.f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        float2 w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 x = make_float2(s[j][t][2 * k], s[j][t][2 * k + 1]), e = fma2(x, by, up);
+          w[k] = make_float2(exp2f(e.x), exp2f(e.y));
+          if constexpr (kMasked) {  // a masked score, whatever the factor is
+            if (x.x == -INFINITY) w[k].x = 0.f;
+            if (x.y == -INFINITY) w[k].y = 0.f;
+          }
+          sum = add2(sum, w[k]);
+          pf[j][t][k] = transpose8x8(pack_half(w[k].x, w[k].y));
+        }
+      }
+      const float2 ll = fma2(make_float2(l[j][0], l[j][1]), alpha[j], sum);
+      l[j][0] = ll.x;
+      l[j][1] = ll.y;
+    }
+    // tokens that no row of the block sees are left out of P V whatever they hold
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    if constexpr (kMasked) {
+      KvSpan seen{pages.lo_min, grp.P * kKvPage};
+      int sinks = pages.sinks_max;
+      if (br >= 0) seen = KvSpan{table[br].lo, table[br].hi}, sinks = table[br].sinks;
+      const uint32_t see = there ? static_cast<uint32_t>(kv_bits(seen, sinks, key0) >> (16 * c)) : 0u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) keep[k] = kv_bytes(see >> (4 * k));
+    }
+    const float vf = f.y * exp2f(-kHeadroom);
+    if (!__all_sync(0xffffffffu, mbar_wait(v_full, i & 1, abort_flag))) return false;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
+      const uint32_t x0[4] = {w0.x & keep[0], w0.y & keep[1], w0.z & keep[2], w0.w & keep[3]};
+      const uint32_t x1[4] = {w1.x & keep[0], w1.y & keep[1], w1.z & keep[2], w1.w & keep[3]};
+      float d[NJ][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t av[4] = {half2_of(x0[k] & 0xffff), half2_of(x1[k] & 0xffff), half2_of(x0[k] >> 16), half2_of(x1[k] >> 16)};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          if (k == 0) mma_f16_zero(d[j], av, pf[j][k][0], pf[j][k][1]);
+          else mma_f16(d[j], av, pf[j][k][0], pf[j][k][1]);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const float2 x = fma2(make_float2(d[j][k], d[j][k + 1]), both(vf), mul2(make_float2(o[j][t][k], o[j][t][k + 1]), alpha[j]));
+          o[j][t][k] = x.x;
+          o[j][t][k + 1] = x.y;
+        }
+    }
+    return true;
+    };
+    ok = whole ? rest(std::false_type{}) : rest(std::true_type{});
+    if (!ok) break;
+    __syncwarp();  // every lane has read the values
+    if (i + 1 < mine) issue_values(i + 1);
+  }
+  if (!ok) {
+    if (lane == 0) {
+      if (status) atomicCAS(status, 0, kStatusTimeoutEpilogue);
+      *abort_flag = 1;
+      const long long t0 = clock64();  // copies in flight land before the ring is reused
+      for (int s = 0; s < 3; ++s)
+        for (int ph = 0; ph < 2; ++ph)
+          while (!mbar_try_wait(&k_full[s], ph) && clock64() - t0 < kSpinLimitCycles / 8) {
+          }
+    }
+    __syncwarp();
+  }
+  // ---- the warps' results: unnormalised O, m and l (whole sums), over the rings
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) l[j][u] += __shfl_xor_sync(0xffffffffu, l[j][u], x);
+      l[j][u] *= exp2f(-kHeadroom);
+      if (m[j][u] == -INFINITY && l[j][u] != 0.f) m[j][u] = 0.f;  // only NaN scores so far
+    }
+  __syncthreads();
+  float* wo = reinterpret_cast<float*>(smem + OFF_RING);  // [warp][row][kPitch], then [warp][row] (m, l)
+  float2* wml = reinterpret_cast<float2*>(wo + kWarps * R * kPitch);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = j * 8 + 2 * c + u;
+      float* w = wo + (warp * R + r) * kPitch + g;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        w[t * 16] = o[j][t][u];
+        w[t * 16 + 8] = o[j][t][2 + u];
+      }
+      if (g == 0) wml[warp * R + r] = make_float2(m[j][u], l[j][u]);
+    }
+  __syncthreads();
+  float* out = a.part + blockIdx.x * kv_part_floats(R);
+  for (int i = threadIdx.x; i < R * 16; i += kThreads) {
+    const int r = i >> 4, d = (i & 15) * 4;
+    float top = -INFINITY, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wml[w * R + r].x);
+    if (top != -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = wml[w * R + r];
+        const float k = exp2f(ml.x - top);
+        const float4 x = *reinterpret_cast<const float4*>(wo + (w * R + r) * kPitch + d);
+        v.x += k * x.x;
+        v.y += k * x.y;
+        v.z += k * x.z;
+        v.w += k * x.w;
+        sum += k * ml.y;
+      }
+    }
+    *reinterpret_cast<float4*>(out + r * 64 + d) = v;
+    if (d == 0) *reinterpret_cast<float2*>(out + R * 64 + r * 2) = make_float2(top, sum);
+  }
+}
+
+// Adds up the parts of each row, in the order of the CTAs; 16 threads a row, 4 channels each.
+template <int R>
+__global__ void __launch_bounds__(256) kv_group_merge(const KvAttendArgs a, int row_tiles) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
+  constexpr int kOnce = R < 16 ? R : 16;  // rows of a CTA
+  const int lr = blockIdx.x % (R / kOnce) * kOnce + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+  int item = blockIdx.x / (R / kOnce);
+  const float* part = a.part + static_cast<long>(item) * a.ranks * kv_part_floats(R);
+  const int r = item % row_tiles * R + lr;
+  item /= row_tiles;
+  const int kh = item % a.pool.heads;
+  const KvGroup grp(a, item / a.pool.heads);
+  if (r >= grp.rows) return;
+  const KvGroupRow x = grp.row(r);
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (x.span.lo != kNoKey)
+#pragma unroll 8
+    for (int k = 0; k < a.ranks; ++k) top = fmaxf(top, part[k * kv_part_floats(R) + R * 64 + lr * 2]);
+  if (top != -INFINITY)
+#pragma unroll 4
+    for (int k = 0; k < a.ranks; ++k) {
+      const float* p = part + k * kv_part_floats(R);
+      const float2 ml = *reinterpret_cast<const float2*>(p + R * 64 + lr * 2);
+      const float4 y = *reinterpret_cast<const float4*>(p + lr * 64 + d);
+      const float w = exp2f(ml.x - top);
+      sum += w * ml.y;
+      v.x += w * y.x;
+      v.y += w * y.y;
+      v.z += w * y.z;
+      v.w += w * y.w;
+    }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int h = kh * grp.G + x.g;
+  const long b = grp.seq(x.i), at = (b * a.T + x.t) * a.H + h;
+  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64 + d) =
+      make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+  if (a.lse && d == 0) a.lse[(b * a.H + h) * a.T + x.t] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+}
+
+template <int NJ>
+void launch(const KvAttendArgs& a, int dev, cudaStream_t stream) {
+  static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+  if (!(set.load() >> (dev & 63) & 1)) {
+    check_cuda(cudaFuncSetAttribute(kv_attend_group<NJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+               "cudaFuncSetAttribute(kv_attend_group)");
+    set.fetch_or(1ull << (dev & 63));
+  }
+  const long blocks = kv_group_blocks(a, 8 * NJ), tiles = (kv_group_rows(a) + 8 * NJ - 1) / (8 * NJ);
+  if (blocks * a.ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  kv_attend_group<NJ><<<static_cast<unsigned>(blocks * a.ranks), kThreads, SMEM_BYTES, stream>>>(a, static_cast<int>(tiles), device_status(dev));
+  check_cuda(cudaGetLastError(), "kv_attend_group launch");
+  count_launch();
+}
+
+template <int R>
+void merge(const KvAttendArgs& a, cudaStream_t stream) {
+  constexpr int kOnce = R < 16 ? R : 16;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(kv_group_blocks(a, R) * (R / kOnce)));
+  cfg.blockDim = dim3(kOnce * 16);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];  // its launch beside the end of the one before it
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_group_merge<R>, a, static_cast<int>((kv_group_rows(a) + R - 1) / R)), "kv_group_merge launch");
+  count_launch();
+}
+
+constexpr int kBlockRows = 256;  // of attend_tiles.cu
+
+}  // namespace
+
+// Estimates from measured calls (cold caches): few rows 8 us and 2.6 or 3.3 us for a page of each warp
+// (8 rows: 15,000 pages on 144 CTAs 26 us; 16: 22,700 on 128 48 us), blocks of 256 as in
+// kv_attend_tiles_plan, the second launch 4 us and 0.2 us a part of a row.
+KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
+  const long rows = kv_group_rows(a), TG = a.T * static_cast<long>(a.H / a.pool.heads), sms = num_sms(dev);
+  const long shared = std::min<long>(a.shared_pages, kv_seen_pages(a)), own = (a.own_tokens + kKvPage - 1) / kKvPage;
+  KvPlan best;
+  for (const int R : {rows <= 8 ? 8 : 16, kBlockRows}) {
+    if (mode ? (R == kBlockRows) != (mode == 3) : R == kBlockRows && rows <= 64) continue;  // (mostly padding)
+    const long blocks = kv_group_blocks(a, R), seqs = std::min<long>(a.step.branches, (R + TG - 2) / TG + 1);
+    const long pages = shared + seqs * own, units = R == kBlockRows ? (pages + 1) / 2 : (pages + kWarps - 1) / kWarps;
+    for (long s = 1; s <= 32 && (s == 1 || (blocks * s <= 4 * sms && units >= s)); ++s) {
+      const long each = (units + s - 1) / s;
+      const double one = R == kBlockRows ? 15. + (rows > 128 ? 1.75 : 1.3) * each : 8. + (R == 8 ? 2.6 : 3.3) * each;
+      const double us = static_cast<double>((blocks * s + sms - 1) / sms) * one + 4. + 0.2 * s;
+      if (best.rows && us >= best.us) continue;
+      best.branches = true;
+      best.blocks = R == kBlockRows;
+      best.rows = R;
+      best.ranks = static_cast<int>(s);
+      best.scratch = blocks * s * kv_part_floats(R);
+      best.us = us;
+    }
+  }
+  return best;
+}
+
+void kv_attend_branches(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream) {
+  if (!a.part) throw std::runtime_error("kv_cache_attend: no scratch");
+  a.ranks = plan.ranks;
+  if (plan.blocks) {
+    kv_attend_group_tiles(a, dev, stream);
+    merge<kBlockRows>(a, stream);
+  } else if (plan.rows == 8) {
+    launch<1>(a, dev, stream);
+    merge<8>(a, stream);
+  } else {
+    launch<2>(a, dev, stream);
+    merge<16>(a, stream);
+  }
+}
+
+}  // namespace ddb

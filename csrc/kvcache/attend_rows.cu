@@ -56,9 +56,7 @@ constexpr int smem_bytes(int NT, int stages) { return off_ring(NT) + kGroups * s
 static_assert(kGroups * (out_floats(4) * 4 + 64 * 4) <= kGroups * 2 * kPageBytes, "results fit the rings");
 static_assert(smem_bytes(4, kMaxStages) <= 232448, "shared memory per CTA");
 
-// OWN: only the pages behind those that the sequence's group shares; kv_attend_past has the others'
-// part of each row.
-template <int NT, bool OWN>
+template <int NT>
 __global__ void __launch_bounds__(kGroups * NT * 32)
     kv_attend_rows(const KvAttendArgs a, int row_tiles, int stages, uint32_t group_inv, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -102,7 +100,6 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     const KvSpan s1 = kv_span(a, old + token(min(rows, r0 + R) - 1), len, first);
     lo_min = s0.lo, hi_min = s0.hi, lo_max = s1.lo, hi_max = s1.hi;
     pages = kv_pages(lo_min, hi_max, sinks, a.step.width);
-    if (OWN) pages = kv_pages_from(pages, min(max(a.step.rows[static_cast<long>(a.step.B + b / a.step.branches) * a.step.ld], 0), a.step.width));
   }
   const int part = rank * kGroups + pg, parts = ranks * kGroups;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
@@ -369,7 +366,6 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     *reinterpret_cast<float4*>(co + r * kPitch + d) = v;
     if (d == 0) cml[r] = make_float2(top, sum);
   }
-  if (OWN) asm volatile("griddepcontrol.wait;" ::: "memory");  // the other launch's part is written
   if (ranks > 1) cluster_sync_all(); else __syncthreads();
   // ---- the cluster's CTAs share the rows; each adds the others' parts in rank order
   const uint32_t so = smem_u32(co), sml = smem_u32(cml);
@@ -380,27 +376,6 @@ __global__ void __launch_bounds__(kGroups * NT * 32)
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < ranks; ++k) top = fmaxf(top, ld_cluster_v2(ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8).x);
-    const float* past = nullptr;  // of the row's tile of its group
-    int past_row = 0;
-    if (OWN) {
-      const int n = a.step.branches, all = b % n * a.T * G + row_id, tiles = (n * a.T * G + a.past_rows - 1) / a.past_rows;
-      past_row = all % a.past_rows;
-      past = a.part + (static_cast<long>(b / n * a.pool.heads + kh) * tiles + all / a.past_rows) * a.past_ranks * kv_past_floats(a.past_rows);
-      for (int k = 0; k < a.past_ranks; ++k)
-        top = fmaxf(top, past[k * kv_past_floats(a.past_rows) + a.past_rows * 64 + past_row * 2]);
-    }
-    if (OWN && top != -INFINITY)
-      for (int k = 0; k < a.past_ranks; ++k) {
-        const float* p = past + k * kv_past_floats(a.past_rows);
-        const float2 x = *reinterpret_cast<const float2*>(p + a.past_rows * 64 + past_row * 2);
-        const float4 y = *reinterpret_cast<const float4*>(p + past_row * 64 + d);
-        const float w = exp2f(x.x - top);
-        sum += w * x.y;
-        v.x += w * y.x;
-        v.y += w * y.y;
-        v.z += w * y.z;
-        v.w += w * y.w;
-      }
     if (top != -INFINITY)
       for (int k = 0; k < ranks; ++k) {
         const uint32_t ml = ranks > 1 ? mapa_shared(sml + r * 8, k) : sml + r * 8;
@@ -445,11 +420,11 @@ KvPlan rows_plan(const KvAttendArgs& a, int NT, int dev) {
   return p;
 }
 
-template <int NT, bool OWN>
+template <int NT>
 void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
+    check_cuda(cudaFuncSetAttribute(kv_attend_rows<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NT, kMaxStages)),
                "cudaFuncSetAttribute(kv_attend_rows)");
     set.fetch_or(1ull << (dev & 63));
   }
@@ -466,21 +441,13 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   cfg.blockDim = dim3(kGroups * NT * 32);
   cfg.dynamicSmemBytes = smem_bytes(NT, stages);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 0;
-  if (ranks > 1) {
-    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
-    x.id = cudaLaunchAttributeClusterDimension;
-    x.val.clusterDim.x = ranks;
-    x.val.clusterDim.y = x.val.clusterDim.z = 1;
-  }
-  if (OWN) {  // beside the launch before it
-    cudaLaunchAttribute& x = attr[cfg.numAttrs++];
-    x.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    x.val.programmaticStreamSerializationAllowed = 1;
-  }
-  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT, OWN>, a, tiles, stages, 0xffffffffu / G + 1, device_status(dev)),
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_rows<NT>, a, tiles, stages, 0xffffffffu / G + 1, device_status(dev)),
              "kv_attend_rows launch");
   count_launch();
 }
@@ -488,10 +455,13 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
 // Rows beyond which only the 256-row blocks are tried: there each page is read by 8 row
 // tiles of the other kernel. (Its rows' division by multiplication is exact far beyond.)
 constexpr long kMaxRows = 256;
+std::atomic<int> g_branch_mode{0};
 // 8-row warps of a row tile
 int row_warps(long rows) { return rows <= 24 ? static_cast<int>(rows + 7) / 8 : 4; }
 
 }  // namespace
+
+int kv_set_branch_mode(int mode) { return g_branch_mode.exchange(mode); }
 
 // Up to 32 rows one row tile of kv_attend_rows takes them, the narrowest that does (32 rows:
 // 28 us against the blocks' 42 at 12 heads of 20,000 tokens, 118 against 195 at 512 of
@@ -504,47 +474,40 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
   const long rows = a.T * static_cast<long>(a.H / a.pool.heads);
-  if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows) {
-    KvPlan split = kv_attend_past_plan(a, dev);
-    if (kv_group_rows(a) > 128) split = kv_past_tiles_plan(a, dev);
-    KvAttendArgs own = a;
-    own.max_tokens = a.own_tokens;
-    split.ranks = rows_plan(own, row_warps(rows), dev).ranks;
-    return split;
-  }
   const KvPlan few = rows <= kMaxRows ? rows_plan(a, row_warps(rows), dev) : KvPlan{};
-  if (rows <= 32) return few;
-  const KvPlan many = kv_attend_tiles_plan(a, dev);
-  return rows > kMaxRows || many.us < few.us ? many : few;
+  KvPlan alone = few;  // every sequence for itself
+  if (rows > 32) {
+    const KvPlan many = kv_attend_tiles_plan(a, dev);
+    if (rows > kMaxRows || many.us < few.us) alone = many;
+  }
+  // Groups that share pages: together where that is estimated faster. (8-row tiles take 0.65 of their
+  // estimate where pages are many: 128 on 60,000 tokens 155 us, 192 on 8,000 32 us. Eight branches of 1,500
+  // tokens 7.5 us alone and 10 together, 64 of 16,384 275 and 50; of 64 rows over 12,800 tokens 136 and 57.)
+  const int mode = g_branch_mode.load(std::memory_order_relaxed);
+  if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows && mode != 1) {
+    const KvPlan group = kv_attend_branches_plan(a, mode, dev);
+    if (mode || group.us < alone.us * (!alone.blocks && rows <= 8 ? 0.65 : 1.)) return group;
+  }
+  return alone;
 }
 
-void kv_cache_attend(const KvAttendArgs& args, const KvPlan& plan, cudaStream_t stream) {
-  KvAttendArgs a = args;
+void kv_cache_attend(const KvAttendArgs& a, const KvPlan& plan, cudaStream_t stream) {
   if (a.step.B <= 0 || a.T <= 0 || a.H <= 0) return;
   int dev = 0;
   check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  if (plan.blocks && !plan.split) {
+  if (plan.branches) {
+    kv_attend_branches(a, plan, dev, stream);
+    return;
+  }
+  if (plan.blocks) {
     kv_attend_tiles_launch(a, plan, dev, stream);
     return;
   }
-  const int warps = row_warps(a.T * static_cast<long>(a.H / a.pool.heads));
-  if (plan.split) {
-    a.past_ranks = plan.past_ranks;
-    a.past_rows = plan.past_rows;
-    (plan.blocks ? kv_past_tiles_launch : kv_attend_past_launch)(a, dev, stream);
-    switch (warps) {
-      case 1: launch<1, true>(a, plan.ranks, dev, stream); break;
-      case 2: launch<2, true>(a, plan.ranks, dev, stream); break;
-      case 3: launch<3, true>(a, plan.ranks, dev, stream); break;
-      default: launch<4, true>(a, plan.ranks, dev, stream); break;
-    }
-    return;
-  }
-  switch (warps) {
-    case 1: launch<1, false>(a, plan.ranks, dev, stream); break;
-    case 2: launch<2, false>(a, plan.ranks, dev, stream); break;
-    case 3: launch<3, false>(a, plan.ranks, dev, stream); break;
-    default: launch<4, false>(a, plan.ranks, dev, stream); break;
+  switch (row_warps(a.T * static_cast<long>(a.H / a.pool.heads))) {
+    case 1: launch<1>(a, plan.ranks, dev, stream); break;
+    case 2: launch<2>(a, plan.ranks, dev, stream); break;
+    case 3: launch<3>(a, plan.ranks, dev, stream); break;
+    default: launch<4>(a, plan.ranks, dev, stream); break;
   }
 }
 

@@ -63,6 +63,11 @@ constexpr int N_BARS = 1 + 2 * NR + 4 * NS + 10 + 1 + NF;
 constexpr int OFF_FACTOR = OFF_BAR + (N_BARS + 1) / 2 * 16;
 constexpr int OFF_META = OFF_FACTOR + NF * 16;
 constexpr int OFF_MISC = OFF_META + (NR + 1) / 2 * 8;
+// GROUP: first key and sequence of both pages, per stage of factors and of codes; the sequences
+constexpr int OFF_WHERE = (OFF_MISC + 16 + 15) / 16 * 16;
+constexpr int OFF_TABLE = OFF_WHERE + (NF + NR) * 16;
+constexpr int GROUP_BYTES = OFF_TABLE + kRows * 16;
+static_assert(GROUP_BYTES <= 232448, "shared memory per CTA");
 static_assert(NF > NR + NS && (NF & (NF - 1)) == 0, "stages of page factors");
 constexpr int SMEM_BYTES = OFF_MISC + 16;
 static_assert(OFF_FACTOR % 16 == 0 && OFF_MISC % 8 == 0, "alignment");
@@ -98,8 +103,9 @@ __device__ __forceinline__ float log2_of_power(float p) { return static_cast<flo
 // every warp has its role's registers
 __device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
-// PAST: rows of all sequences of a group over the pages that it shares (attend.h).
-template <bool PAST>
+// GROUP: rows of all sequences of a group, over the pages that it shares and then their own (attend.h);
+// every CTA leaves its part in scratch.
+template <bool GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
     kv_attend_tiles(const KvAttendArgs a, int row_tiles, int* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -130,52 +136,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   // largest key scale of the CTA's pages (positive floats order like their bits)
   int* k_most = reinterpret_cast<int*>(smem + OFF_MISC + 8);
 
-  if (PAST) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (GROUP) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = warp_id(), lane = lane_id();
-  const int ranks = PAST ? a.past_ranks : a.ranks, rank = blockIdx.x % ranks;
+  const int ranks = a.ranks, rank = blockIdx.x % ranks;
   int item = blockIdx.x / ranks;
-  const int tile = row_tiles - 1 - item % row_tiles;  // long (late) tiles first
+  const int tile = GROUP ? item % row_tiles : row_tiles - 1 - item % row_tiles;  // long (late) tiles first
   item /= row_tiles;
-  const int kh = item % a.pool.heads, b = item / a.pool.heads;  // PAST: b is a group
-  const int G = a.H / a.pool.heads, TG = a.T * G;
-  const int* row = a.step.rows + static_cast<long>(PAST ? a.step.B + b : b) * a.step.ld;
+  const int kh = item % a.pool.heads, b = item / a.pool.heads;  // GROUP: a group
+  const int G = a.H / a.pool.heads;
+  const KvGroup grp(a, GROUP ? b : -1);
+  const int* row = a.step.rows + static_cast<long>(GROUP ? 0 : b) * a.step.ld;
   const int len = row[0], own = min(row[1], a.T), first = row[2], old = len - row[1];
-  int sinks = row[3] >= 0 ? row[3] : a.sinks;        // a trimmed sequence has its own
-  // rows behind `rows` are padding
-  const int r0 = tile * kRows, rows = PAST ? a.step.branches * TG : own * G;
+  const int sinks = row[3] >= 0 ? row[3] : a.sinks;  // a trimmed sequence has its own
+  const int r0 = tile * kRows, rows = GROUP ? grp.rows : own * G;  // rows behind `rows` are padding
   const int n_t = rows - r0 > 128 ? 2 : 1;
+  int4* where = reinterpret_cast<int4*>(smem + OFF_WHERE);  // [NF], then [NR]
+  KvBranch* table = reinterpret_cast<KvBranch*>(smem + OFF_TABLE);
 
   // the block's pages, and this CTA's run of key tiles (page pairs)
   KvPages pages{0, 0, 0};
   KvSpan all{0, 0};
-  // PAST: a row's sequence and token, the shared keys that it sees and its sinks; it sees none if it is padding
-  const int* seq = nullptr;
-  int seq_token = 0, seq_sinks = 0;
-  const int P = PAST ? min(max(row[0], 0), a.step.width) : 0;
-  KvSpan seq_span{0x7fffffff, P * kKvPage};
-  auto past_row = [&](int r) {
-    if (r >= rows) return;
-    const int i = r / TG;
-    seq = a.step.rows + (static_cast<long>(b) * a.step.branches + i) * a.step.ld;
-    seq_token = (r - i * TG) / G;
-    if (seq_token >= min(seq[1], a.T)) return;
-    seq_span.lo = kv_span(a, seq[0] - seq[1] + seq_token, seq[0], seq[2]).lo;
-    seq_sinks = seq[3] >= 0 ? seq[3] : a.sinks;
-  };
-  if (PAST) {
-    // the smallest and largest of the block's rows; every key of a shared page is before all of them
-    int* low = reinterpret_cast<int*>(smem + OFF_RAW);  // not yet in use
-    past_row(r0 + (threadIdx.x & 255));
-    if (threadIdx.x < 256) {
-      const int lo = __reduce_min_sync(0xffffffffu, seq_span.lo), most = __reduce_max_sync(0xffffffffu, seq_sinks);
-      if (lane == 0) low[warp] = lo, low[8 + warp] = most;
-    }
-    __syncthreads();
-    all.lo = low[0], sinks = low[8];
-    for (int w = 1; w < 8; ++w) all.lo = min(all.lo, low[w]), sinks = max(sinks, low[8 + w]);
-    all.hi = P * kKvPage;
-    if (all.lo != 0x7fffffff) pages = kv_pages_before(kv_pages(all.lo, P * kKvPage, sinks, a.step.width), P);
-    __syncthreads();  // before copies land there
+  KvGroupPages list;
+  if (GROUP) {
+    list = kv_group_pages<kRows>(grp, r0, table, reinterpret_cast<int*>(smem + OFF_RAW));  // (not yet in use)
+    pages.n = list.n;
   } else if (r0 < rows) {
     const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
     const KvSpan s1 = kv_span(a, old + (min(rows, r0 + kRows) - 1) / G, len, first);
@@ -221,7 +205,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   {
     int most = 0;
     for (int i = 2 * j0 + threadIdx.x; i < min(pages.n, 2 * (j0 + n)); i += kThreads) {
-      const int id = row[kKvInfo + pages.at(i)];
+      int id, page, branch;
+      if (GROUP) list.at(grp, table, i, page, branch, id);
+      else id = row[kKvInfo + pages.at(i)];
       if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages))
         most = max(most, __float_as_int(a.pool.k_scale[static_cast<long>(id) * a.pool.heads + kh]));
     }
@@ -239,15 +225,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       // ---------------------------------------------------------- copies of the codes
       bool ok = true;
-      int ids = -1, issued = 0;
+      int ids = -1, issued = 0, key = 0, branch = -1;
       float ks = 0.f, vs = 0.f;
       for (int j = 0; j < n; ++j) {
         if ((j & 15) == 0) {  // the next 16 pairs, one page a lane
           const int i = 2 * (j0 + j) + lane;
-          ids = i < min(pages.n, 2 * (j0 + n)) ? row[kKvInfo + pages.at(i)] : -2;
+          if (GROUP) {
+            ids = -2, key = 0x40000000, branch = -1;  // no page: no key
+            if (i < min(pages.n, 2 * (j0 + n))) {
+              list.at(grp, table, i, key, branch, ids);
+              key *= kKvPage;
+            }
+          } else {
+            ids = i < min(pages.n, 2 * (j0 + n)) ? row[kKvInfo + pages.at(i)] : -2;
+          }
           if (ids != -2 && static_cast<unsigned>(ids) >= static_cast<unsigned>(a.pool.pages)) {
-            // recorded, read as zeros (but for a page that no sequence of a group has any more)
-            if (!PAST || ids != -1) record_bad_index(status, ids);
+            // recorded, read as zeros (no sequence sees a shared page that none has)
+            if (!GROUP || ids != -1 || branch >= 0) record_bad_index(status, ids);
             ids = -2;
           }
           ks = vs = 0.f;
@@ -261,9 +255,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int id0 = __shfl_sync(0xffffffffu, ids, l0), id1 = __shfl_sync(0xffffffffu, ids, l0 + 1);
         const float4 f = make_float4(__shfl_sync(0xffffffffu, ks, l0), __shfl_sync(0xffffffffu, ks, l0 + 1),
                                      __shfl_sync(0xffffffffu, vs, l0), __shfl_sync(0xffffffffu, vs, l0 + 1));
+        int4 w = make_int4(0, 0, 0, 0);
+        if (GROUP)
+          w = make_int4(__shfl_sync(0xffffffffu, key, l0), __shfl_sync(0xffffffffu, branch, l0), __shfl_sync(0xffffffffu, key, l0 + 1),
+                        __shfl_sync(0xffffffffu, branch, l0 + 1));
         ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[s], ((j / NR) & 1) ^ 1, abort_flag));
         if (!ok) break;
         if (lane == 0) {
+          if (GROUP) where[j % NF] = where[NF + s] = w;
           uint8_t* dst = smem + OFF_RAW + s * TILE;
           // The softmax has read the factors NF pairs back: codes 3 pairs back have been converted,
           // so the scores of the pair 6 back are made, and those before it read.
@@ -391,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const int there = meta[sr];
+      const int4 w = GROUP ? where[NF + sr] : make_int4(0, 0, 0, 0);
       const uint8_t* raw = smem + OFF_RAW + sr * TILE;
       uint32_t keep[2][4];
 #pragma unroll
@@ -405,9 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const int i = 2 * (j0 + j) + p;
-        const int key = pages.at(i) * kKvPage;
-        if (keep[p][0] && !(key + kKvPage <= all.hi && (key >= all.lo || key + kKvPage <= sinks))) {
-          const uint32_t see = static_cast<uint32_t>(kv_bits(all, sinks, key) >> (16 * c));
+        const int key = GROUP ? (p ? w.z : w.x) : pages.at(i) * kKvPage;
+        KvSpan seen = all;
+        int seen_sinks = sinks;
+        if (GROUP) {  // of all the block's rows, or of a sequence's
+          const int br = p ? w.w : w.y;
+          seen = br < 0 ? KvSpan{list.lo_min, grp.P * kKvPage} : KvSpan{table[br].lo, table[br].hi};
+          seen_sinks = br < 0 ? list.sinks_max : table[br].sinks;
+        }
+        if (keep[p][0] && !(key + kKvPage <= seen.hi && (key >= seen.lo || key + kKvPage <= seen_sinks))) {
+          const uint32_t see = static_cast<uint32_t>(kv_bits(seen, seen_sinks, key) >> (16 * c));
 #pragma unroll
           for (int k = 0; k < 4; ++k) keep[p][k] = kv_bytes(see >> (4 * k));
         }
@@ -441,17 +448,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool active = t < n_t;  // of a second tile that is all padding nothing is computed
     const uint32_t trow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     // a padding row keeps zeros and the span of the last row: its result is not used
-    const KvSpan span = PAST ? seq_span : kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
-    const int row_sinks = PAST ? seq_sinks : sinks;
+    const KvGroupRow mine = GROUP ? grp.row(r) : KvGroupRow{};
+    const KvSpan span = GROUP ? mine.span : kv_span(a, old + (min(max(rows, 1), r + 1) - 1) / G, len, first);
+    const int row_sinks = GROUP ? mine.sinks : sinks, row_branch = GROUP ? mine.i - list.first : -1;
     float sl2, bound;
     {
       uint4 w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = make_uint4(0, 0, 0, 0);
-      if (PAST ? seq_span.lo != 0x7fffffff : r < rows) {
-        const int s = PAST ? b * a.step.branches + r / TG : b, tok = PAST ? seq_token : r / G;
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + s * a.q_sb + tok * a.q_st +
-                                 (kh * G + r % G) * a.q_sh;
+      if (GROUP ? mine.span.lo != kNoKey : r < rows) {
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (GROUP ? grp.seq(mine.i) : b) * a.q_sb +
+                                 (GROUP ? mine.t : r / G) * a.q_st + (kh * G + (GROUP ? mine.g : r % G)) * a.q_sh;
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = ld_global_v4(q + i * 8);
       }
@@ -494,6 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < n; ++j) {
         if (!mbar_wait(&f_full[j % NF], (j / NF) & 1, abort_flag)) return false;
         const float4 f = factor[j % NF];
+        const int4 w = GROUP ? where[j % NF] : make_int4(0, 0, 0, 0);
         // of the scores; not zero: a masked score is -inf times it
         const float f0 = fmaxf(sl2 * f.x, 1e-37f), f1 = fmaxf(sl2 * f.y, 1e-37f);
         // The page's exponents hold its value scale; its sum is brought back. A scale far below the
@@ -529,9 +537,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int i = 2 * (j0 + j) + p;
-          const int key = i < pages.n ? pages.at(i) * kKvPage : 0x40000000;  // no page: no key
-          if (!(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= row_sinks))) {
-            const uint64_t see = kv_bits(span, row_sinks, key);
+          int key = i < pages.n ? pages.at(i) * kKvPage : 0x40000000;  // no page: no key
+          bool other = false;  // another sequence's own page
+          if (GROUP) {
+            const int br = p ? w.w : w.y;
+            key = p ? w.z : w.x;
+            other = br >= 0 && br != row_branch;
+          }
+          if (other || !(key + kKvPage <= span.hi && (key >= span.lo || key + kKvPage <= row_sinks))) {
+            const uint64_t see = other ? 0 : kv_bits(span, row_sinks, key);
             const uint32_t word[2] = {static_cast<uint32_t>(see), static_cast<uint32_t>(see >> 32)};
 #pragma unroll
             for (int c = 0; c < 64; ++c)
@@ -663,11 +677,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
     if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores
-    if (PAST || a.part) {
+    if (GROUP || a.part) {
       // 256 rows of 64 channels, then their (maximum, sum), for kv_tiles_merge
-      const long at = PAST ? ((static_cast<long>(b) * a.pool.heads + kh) * row_tiles + tile) * ranks + rank : blockIdx.x;
-      float* part = a.part + at * kPartFloats;
-      if (r < (PAST ? rows : TG)) {
+      float* part = a.part + blockIdx.x * kPartFloats;
+      if (r < (GROUP ? rows : a.T * G)) {
         float* o = part + (t * 128 + lr) * 64;
 #pragma unroll
         for (int c = 0; c < 16; ++c)
@@ -703,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (!PAST && ranks > 1 && !a.part) {
+  if (!GROUP && ranks > 1 && !a.part) {
     // ---- each CTA of the cluster adds up its share of the rows, in rank order; 16 threads a
     // row, 4 channels each
     cluster_sync_all();
@@ -778,7 +791,7 @@ void raise_limit(int dev) {
   if (set.load() >> (dev & 63) & 1) return;
   check_cuda(cudaFuncSetAttribute(kv_attend_tiles<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
              "cudaFuncSetAttribute(kv_attend_tiles)");
-  check_cuda(cudaFuncSetAttribute(kv_attend_tiles<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+  check_cuda(cudaFuncSetAttribute(kv_attend_tiles<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, GROUP_BYTES),
              "cudaFuncSetAttribute(kv_attend_tiles)");
   set.fetch_or(1ull << (dev & 63));
 }
@@ -853,26 +866,11 @@ void kv_attend_tiles_launch(KvAttendArgs a, const KvPlan& plan, int dev, cudaStr
   }
 }
 
-KvPlan kv_past_tiles_plan(const KvAttendArgs& a, int dev) {
-  const long rows = kv_group_rows(a), items = a.step.B / a.step.branches * static_cast<long>(a.pool.heads) * kv_past_tiles(a, kRows);
-  const int pairs = static_cast<int>((std::min<long>(a.shared_pages, kv_seen_pages(a)) + 1) / 2);
-  const double step = rows > 128 ? 1.75 : 1.3;
-  KvPlan best;
-  best.split = best.blocks = true;
-  best.past_rows = kRows;
-  for (int s = 1; s == 1 || (s <= 16 && pairs >= 2 * s && items * s <= 4L * num_sms(dev)); ++s) {
-    const double us = static_cast<double>((items * s + num_sms(dev) - 1) / num_sms(dev)) * (15. + step * ((pairs + s - 1) / s)) + items * s * 0.015;
-    if (s == 1 || us < best.us) best.past_ranks = s, best.us = us;
-  }
-  best.scratch = items * best.past_ranks * kPartFloats;
-  return best;
-}
-
-void kv_past_tiles_launch(const KvAttendArgs& a, int dev, cudaStream_t stream) {
+void kv_attend_group_tiles(const KvAttendArgs& a, int dev, cudaStream_t stream) {
   raise_limit(dev);
-  const long tiles = kv_past_tiles(a, kRows), ctas = a.step.B / a.step.branches * static_cast<long>(a.pool.heads) * tiles * a.past_ranks;
-  if (ctas > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
-  kv_attend_tiles<true><<<static_cast<unsigned>(ctas), kThreads, SMEM_BYTES, stream>>>(a, static_cast<int>(tiles), device_status(dev));
+  const long blocks = kv_group_blocks(a, kRows), tiles = (kv_group_rows(a) + kRows - 1) / kRows;
+  if (blocks * a.ranks > 0x7fffffffL / (kRows / 16)) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
+  kv_attend_tiles<true><<<static_cast<unsigned>(blocks * a.ranks), kThreads, GROUP_BYTES, stream>>>(a, static_cast<int>(tiles), device_status(dev));
   check_cuda(cudaGetLastError(), "kv_attend_tiles launch");
   count_launch();
 }

@@ -81,21 +81,22 @@ struct KvAttendArgs {
   int shared_pages = 0;
   int own_tokens = 0;
   bool split = false;    // shared pages apart from the sequences' own (the plan's)
-  int past_ranks = 1;    // CTAs that share a row tile's shared pages
-  int past_rows = 32;    // rows of such a tile
 };
 
 // How a call is launched: the kernel, how many CTAs share a row tile's pages, and the scratch
 // that they meet in (0: distributed shared memory); with an estimate of its time.
 struct KvPlan {
   bool blocks = false;   // 256-row blocks (attend_tiles.cu), not few rows (attend_rows.cu)
-  bool split = false;    // a group's shared pages once for all its rows (attend_past.cu)
-  int past_ranks = 1, past_rows = 32;
+  bool branches = false; // groups of sequences, their shared pages once for all rows (attend_branches.cu),
+  int rows = 0;          // in blocks of so many
   int ranks = 1;
   long scratch = 0;      // floats
   double us = 0.;
 };
 KvPlan kv_cache_attend_plan(const KvAttendArgs& a);
+// How groups that share pages are taken: 0 as the estimates say, 1 every sequence alone, 2 together in
+// blocks of 8 or 16 rows, 3 of 256 (for tests). Returns the setting before.
+int kv_set_branch_mode(int mode);
 
 // Attention of each sequence's own tokens (its newest) over its cached ones. Rows with no
 // visible key, and rows behind a sequence's own tokens, get zeros and lse = -inf.

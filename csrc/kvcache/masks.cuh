@@ -59,4 +59,120 @@ __device__ __forceinline__ KvPages kv_pages_before(KvPages p, int to) {
   return p;
 }
 
+constexpr int kNoKey = 0x7fffffff;  // `lo` of a row that sees nothing
+
+// One row of a block of a group's rows: (sequence, token, head of the group of heads)
+struct KvGroupRow {
+  int i, t, g;    // sequence of the group
+  KvSpan span;
+  int sinks;
+};
+// A block of `R` of a group's rows from r0 on: the pages that some row of it sees, those that the
+// group shares first, then its sequences' own in turn.
+struct KvGroup {
+  const KvAttendArgs& a;
+  int grp, G, TG, rows, P;  // P: pages that the group shares
+  const int* shared;        // the group's row of the step's table
+  __device__ __forceinline__ KvGroup(const KvAttendArgs& args, int group) : a(args), grp(group) {
+    G = a.H / a.pool.heads;
+    TG = a.T * G;
+    rows = a.step.branches * TG;
+    shared = a.step.rows + static_cast<long>(a.step.B + grp) * a.step.ld;
+    P = group >= 0 ? min(max(shared[0], 0), a.step.width) : 0;  // (-1: no group)
+  }
+  __device__ __forceinline__ int seq(int i) const { return grp * a.step.branches + i; }
+  __device__ __forceinline__ const int* seq_row(int i) const { return a.step.rows + static_cast<long>(seq(i)) * a.step.ld; }
+  // rows behind the last, and tokens behind a sequence's own, see nothing
+  __device__ __forceinline__ KvGroupRow row(int r) const {
+    KvGroupRow x{0, 0, 0, {kNoKey, 0}, 0};
+    if (r >= rows) return x;
+    x.i = r / TG;
+    x.t = (r - x.i * TG) / G;
+    x.g = r - x.i * TG - x.t * G;
+    const int* s = seq_row(x.i);
+    if (x.t >= min(s[1], a.T)) return x;
+    x.span = kv_span(a, s[0] - s[1] + x.t, s[0], s[2]);
+    x.sinks = s[3] >= 0 ? s[3] : a.sinks;
+    return x;
+  }
+};
+// What a block's rows of one sequence see, and where its own pages begin in the block's list
+struct __align__(16) KvBranch {
+  int lo, hi, sinks, start;
+};
+// The block's list: `n_shared` pages that it sees of the shared ones, `n` in all
+struct KvGroupPages {
+  KvPages shared;
+  int n, first, count;  // sequences of the group in the block
+  int lo_min, lo_max, sinks_min, sinks_max;  // of the block's rows
+  // The page at k: its index in the sequence, its sequence in the block (-1: shared), its id
+  __device__ __forceinline__ void at(const KvGroup& g, const KvBranch* table, int k, int& page, int& branch, int& id) const {
+    if (k < shared.n) {
+      page = shared.at(k);
+      branch = -1;
+      id = g.shared[kKvInfo + page];
+      return;
+    }
+    int b = 0;  // the last that begins at k or before
+    for (int step = 128; step; step >>= 1)
+      if (b + step < count && table[b + step].start <= k) b += step;
+    const KvBranch t = table[b];
+    page = kv_pages_from(kv_pages(t.lo, t.hi, t.sinks, g.a.step.width), g.P).at(k - t.start);
+    branch = b;
+    id = g.seq_row(first + b)[kKvInfo + page];
+  }
+};
+// The list of the block of R <= 256 rows from r0 on. All threads of the CTA (at least R), which meet
+// in it; `table` and `low` (4 words a warp) are shared memory.
+template <int R>
+__device__ __forceinline__ KvGroupPages kv_group_pages(const KvGroup& g, int r0, KvBranch* table, int* low) {
+  KvGroupPages p;
+  const int last = min(g.rows, r0 + R) - 1;
+  p.first = r0 / g.TG;
+  p.count = last < r0 ? 0 : last / g.TG - p.first + 1;
+  const int b = threadIdx.x, lane = threadIdx.x & 31;
+  if (b < p.count) {
+    KvBranch x{kNoKey, 0, 0, 0};
+    const int i = p.first + b;
+    const int t0 = (max(r0, i * g.TG) - i * g.TG) / g.G, t1 = min((min(last, (i + 1) * g.TG - 1) - i * g.TG) / g.G, min(g.seq_row(i)[1], g.a.T) - 1);
+    if (t0 <= t1) {
+      const KvGroupRow a = g.row(i * g.TG + t0 * g.G), z = g.row(i * g.TG + t1 * g.G);
+      x = KvBranch{a.span.lo, z.span.hi, a.sinks, kv_pages_from(kv_pages(a.span.lo, z.span.hi, a.sinks, g.a.step.width), g.P).n};
+    }
+    table[b] = x;
+  }
+  constexpr int kUsed = (R + 31) / 32;  // warps with rows
+  if (threadIdx.x < kUsed * 32) {
+    KvGroupRow x{0, 0, 0, {kNoKey, 0}, 0};
+    if (b < R) x = g.row(r0 + b);
+    const bool sees = x.span.lo != kNoKey;
+    const int v[4] = {__reduce_min_sync(0xffffffffu, x.span.lo), __reduce_max_sync(0xffffffffu, sees ? x.span.lo : 0),
+                      __reduce_min_sync(0xffffffffu, sees ? x.sinks : kNoKey), __reduce_max_sync(0xffffffffu, x.sinks)};
+    if (lane == 0)
+      for (int k = 0; k < 4; ++k) low[(threadIdx.x >> 5) * 4 + k] = v[k];
+  }
+  __syncthreads();
+  p.lo_min = low[0], p.lo_max = low[1], p.sinks_min = low[2], p.sinks_max = low[3];
+  for (int w = 1; w < kUsed; ++w) {
+    p.lo_min = min(p.lo_min, low[4 * w]);
+    p.lo_max = max(p.lo_max, low[4 * w + 1]);
+    p.sinks_min = min(p.sinks_min, low[4 * w + 2]);
+    p.sinks_max = max(p.sinks_max, low[4 * w + 3]);
+  }
+  p.shared = KvPages{0, 0, 0};
+  // every key of a shared page is before all of the block's queries
+  if (p.lo_min != kNoKey) p.shared = kv_pages_before(kv_pages(p.lo_min, g.P * kKvPage, p.sinks_max, g.a.step.width), g.P);
+  int start = p.shared.n, all = p.shared.n;
+  for (int k = 0; k < p.count; ++k) {
+    const int own = table[k].start;  // still its number of pages
+    start += k < b ? own : 0;
+    all += own;
+  }
+  p.n = all;
+  __syncthreads();
+  if (b < p.count) table[b].start = start;
+  __syncthreads();
+  return p;
+}
+
 }  // namespace ddb

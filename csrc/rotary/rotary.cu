@@ -156,26 +156,6 @@ __device__ __forceinline__ float rms_inv(float sum, float D, float eps, float do
 }
 constexpr float kDown = 0x1p-70f;  // its square times a sum of 256 squares of the largest fp32 is finite
 
-// Two numbers to an instruction
-__device__ __forceinline__ unsigned long long& bits(float2& x) { return reinterpret_cast<unsigned long long&>(x); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(bits(d)) : "l"(bits(a)), "l"(bits(b)));
-  return d;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
-
 // Where a lane's two runs of 8 channels begin on one side. Pairs in halves: a run in each. Side by
 // side: 4 pairs in each run, which lie R / 2 apart as well, so that the lanes of an access are
 // contiguous; but where the other side has halves ("split") the lane's 8 pairs have to be in a

@@ -8,6 +8,17 @@ import torch
 from test_kv_cache_gpu import _cache, _check, _fill, _oracle, _randn
 
 pytestmark = pytest.mark.gpu
+ALONE, ROWS, BLOCKS = 1, 2, 3
+
+
+@pytest.fixture(autouse=True, params=[ROWS, BLOCKS, 0], ids=["rows", "blocks", "chosen"])
+def mode(request):
+    """Groups taken together by either kernel, then as the estimates say."""
+    from drivedit_b200.ops._ext import ext
+    before = ext().kv_set_branch_mode(request.param)
+    yield request.param
+    ext().kv_set_branch_mode(before)
+
 
 
 def _branches(c, ctx, n, more, scale=1.0):
@@ -51,7 +62,7 @@ CASES = [
 
 
 @pytest.mark.parametrize("case", CASES)
-def test_matches_definition(case):
+def test_matches_definition(case, mode):
     ctx, n, more, own, KH, G, causal, unit, window, sinks = case
     B = len(ctx) * n
     own = [own[i % len(own)] for i in range(B)]
@@ -67,8 +78,8 @@ def test_matches_definition(case):
     q = _randn(B, T, 2, KH * G, 64, scale=2.0)[:, :, 1]
     args = dict(causal=causal, tokens_per_frame=unit, window=window, sinks=sinks)
     (o, lse), launches = _launches(lambda: step.attend(0, q, return_lse=True, **args))
-    if min(ctx) >= 64 and T * G <= 32:
-        assert launches == 2  # the shared pages, then the sequences' own
+    if max(ctx) >= 64 and mode:
+        assert launches == 2  # the parts, and their sum
     assert torch.equal(o, step.attend(0, q, **args))
     step.commit()
     for i, (s, m) in enumerate(zip(seqs, own)):
@@ -79,7 +90,7 @@ def test_matches_definition(case):
 
 
 @pytest.mark.parametrize("sinks", [0, 70])
-def test_trimmed_branches(sinks):
+def test_trimmed_branches(sinks, mode):
     """Branches trimmed at different places, one not at all: pages that some gave back, some share."""
     c = _cache(1, 2, 80)
     seqs = _branches(c, [1200], 4, [0, 100, 30, 60])
@@ -93,7 +104,7 @@ def test_trimmed_branches(sinks):
         for window in (0, 350, 2000):
             args = dict(causal="token", window=window, sinks=sinks if window else 0)
             (o, lse), launches = _launches(lambda: step.attend(0, q, return_lse=True, **args))
-            assert launches == 2
+            assert launches == 2 or not mode
             for i, s in enumerate(seqs):
                 n = full[i][0].shape[0]
                 kk, vv = c._values(0, c._seqs[s], n + T)
@@ -186,7 +197,7 @@ def test_nan_stays_in_its_rows():
     assert torch.equal(o, want)
 
 
-def test_run_of_branches():
+def test_run_of_branches(mode):
     """A run as a user makes it, over two layers, with query and key norms and positions: the
     same with the groups named as without."""
     from drivedit_b200.ops.rotary import qk_norm_rotary
@@ -285,6 +296,25 @@ def test_two_streams_and_graphs_at_once():
         assert all(torch.equal(a, b) for a, b in zip(got + outs, want + want))
 
 
+@pytest.mark.parametrize("B,n,T,G,ctx", [(1, 64, 1, 1, 9000), (2, 8, 64, 1, 3000), (1, 300, 1, 1, 500), (1, 3, 250, 1, 1000)])
+def test_long_and_many(B, n, T, G, ctx, mode):
+    """Many branches (more than a block has rows), frames, long pasts: the same as each alone."""
+    from drivedit_b200.ops._ext import ext
+    c = _cache(1, 2, B * (ctx // 64 + 1) + B * n * (T // 64 + 4))
+    seqs = _branches(c, [ctx] * B, n, [10, 0, 90])
+    step = c.begin(seqs, T, branches=n)
+    step.write(0, *(_randn(B * n, T, 2, 64) for _ in "kv"))
+    q = _randn(B * n, T, 2 * G, 64)
+    args = dict(causal="frame", tokens_per_frame=T, return_lse=True)
+    o, lse = step.attend(0, q, **args)
+    ext().kv_set_branch_mode(ALONE)
+    want, want_lse = step.attend(0, q, **args)
+    ext().kv_set_branch_mode(mode)
+    # P in fp16 and the order of fp32 sums, then a bf16 rounding each
+    assert ((o.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -10 * want.float().abs().max()).all()
+    assert (lse - want_lse).abs().max() <= 2.0 ** -12
+
+
 def test_refusals_and_empty_calls():
     c = _cache(1, 2, 20)
     seqs = _branches(c, [200], 4, [3])
@@ -306,5 +336,7 @@ def test_refusals_and_empty_calls():
     assert none.attend(0, _randn(4, 0, 2, 64)).shape == (4, 0, 2, 64)
     empty = c.begin([], 1, branches=4)
     assert empty.attend(0, _randn(0, 1, 2, 64)).shape == (0, 1, 2, 64)
-    from drivedit_b200.ops._ext import device_status
+    from drivedit_b200.ops._ext import device_status, ext
     assert device_status() == 0
+    with pytest.raises(ValueError):
+        ext().kv_set_branch_mode(4)
