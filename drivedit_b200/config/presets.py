@@ -81,6 +81,9 @@ class ModelConfig:
     # window_frames frames (its own counted; 0: all earlier ones) and the first sink_frames
     window_frames: int = 0
     sink_frames: int = 0
+    # queries and keys divided by their head's root mean square, times learned weights, before
+    # they are rotated (dense attention)
+    qk_norm: bool = False
     sla: SLAParams = field(default_factory=SLAParams)
     moe: Optional[MoEParams] = None
     rope_base: float = 10000.0

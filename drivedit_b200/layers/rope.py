@@ -149,6 +149,12 @@ def apply_rope(x: torch.Tensor, table: torch.Tensor, inverse: bool = False) -> t
     """Rotate channel pairs ``(2i, 2i+1)`` of ``x [..., T, H, D]`` with ``table
     [T, D/2, 2]``; ``inverse`` rotates by the negative angle (the backward pass)."""
     T, H, D = x.shape[-3:]
+    if (x.is_cuda and x.dim() in (3, 4) and D <= 256 and table.shape[0] >= T and table.shape[1:] == (D // 2, 2)
+            and x.dtype in (torch.bfloat16, torch.float16, torch.float32) and table.dtype == torch.float32
+            and table.device == x.device and table.is_contiguous() and not table.requires_grad):
+        from ..ops.rotary import rotary  # one pass, the same bits
+
+        return rotary(x, table, inverse=inverse)
     xf = x.float().reshape(*x.shape[:-1], D // 2, 2)
     c = table[:T, None, :, 0]
     s = table[:T, None, :, 1]

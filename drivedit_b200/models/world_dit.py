@@ -13,7 +13,8 @@ Built from the reference's pieces, with the semantics decisions spelled out:
     AdaLN(RMSNorm) -> attention -> residual, AdaLN -> SwiGLU -> residual; the AdaLN
     scale/shift come per frame from ``c`` (one ``ada`` projection per block), optional
     adaLN-Zero gates (blocks/flow_matching.py:131-144).
-  * attention: 3-D RoPE with an explicit (16, 24, 24) channel split for d_head = 64,
+  * attention: 3-D RoPE with an explicit (16, 24, 24) channel split for d_head = 64, behind norms
+    of each head's queries and keys where asked for (``qk_norm``, not in the reference),
     frame-causal masking (every token of frame f sees frames <= f) or token-causal /
     bidirectional, dense softmax or SLA (:mod:`drivedit_b200.layers.sla`).
   * FFN: dense SwiGLU (gate/value rows interleaved by 32 for the fused epilogue) or the
@@ -39,6 +40,7 @@ from ..layers.mlp import split_gu
 from ..layers.moe import MoEFFN
 from ..layers.rope import RoPE3D, apply_rope
 from ..layers.sla import SLAConfig, sla_topk_reference
+from ..ops.rotary import qk_norm_rotary
 
 
 def attention_span(cfg: ModelConfig, tpf: int) -> Dict:
@@ -119,6 +121,9 @@ class WorldDiTBlock(nn.Module):
         self.attn = nn.Module()
         self.attn.qkv = _Lin(3 * d, d, 0.02)
         self.attn.proj = _Lin(d, d, 0.02 / math.sqrt(2 * cfg.n_layers))
+        if cfg.qk_norm:
+            self.attn.q_norm = _Norm(cfg.d_head)
+            self.attn.k_norm = _Norm(cfg.d_head)
         if cfg.attention == "sla":
             self.attn.proj_lin = _Lin(d, d, 0.0)
         if cfg.moe is None:
@@ -136,6 +141,13 @@ class WorldDiTBlock(nn.Module):
         self.ada = nn.Linear(d, self.n_mod * d)
         nn.init.zeros_(self.ada.weight)
         nn.init.zeros_(self.ada.bias)
+
+    def position(self, q: torch.Tensor, k: torch.Tensor, tab: torch.Tensor):
+        """``q``, ``k`` ``[B, T, H, d_head]`` as the attention takes them: rotated, behind their norms
+        if the model has them."""
+        if self.cfg.qk_norm:
+            return qk_norm_rotary(q, k, self.attn.q_norm.weight, self.attn.k_norm.weight, tab, eps=self.cfg.norm_eps)
+        return apply_rope(q, tab), apply_rope(k, tab)
 
     # ---------------------------------------------------------------- torch path
     def forward_torch(self, x: torch.Tensor, mod: torch.Tensor, rope_tab: torch.Tensor,
@@ -157,7 +169,7 @@ class WorldDiTBlock(nn.Module):
         h = norm(x, self.norm1.weight) * (1 + s1) + b1
         qkv = (h @ self.attn.qkv.weight.to(dt).t()).view(B, T, 3, H, Dh)
         q, k, v = qkv.unbind(2)
-        q, k = apply_rope(q, rope_tab), apply_rope(k, rope_tab)
+        q, k = self.position(q, k, rope_tab)
         if cfg.attention == "sla":
             scfg = SLAConfig(block_size=cfg.sla.block_size, topk_frac=cfg.sla.topk_frac,
                              always_diag=cfg.sla.always_diag,
@@ -207,6 +219,8 @@ class WorldDiT(nn.Module):
             raise ValueError("window_frames and sink_frames must not be negative, and sinks need a window")
         if cfg.window_frames and (cfg.attention != "dense" or cfg.causal == "none"):
             raise ValueError("window_frames needs dense causal attention")
+        if cfg.qk_norm and cfg.attention != "dense":
+            raise ValueError("qk_norm needs dense attention")
         self.cfg = cfg
         d = cfg.d_model
         self.patch_embed = nn.Linear(cfg.patch_dim, d)
@@ -411,13 +425,14 @@ class PagedKVCacheSet:
         self.cache = PagedKVCache(len(model.blocks), cfg.n_heads, n, device, max_pages_per_seq=max(total, own))
         self.layers = [None] * len(model.blocks)
         self.seqs = self.cache.add(B)
+        self.branches = 1
         self.frames = 0
         self._step = None
 
     def step(self, n_tokens: int):
         """The open step for ``n_tokens`` more of each stream (kept until committed)."""
         if self._step is None or self._step.n_new[:1] != [n_tokens]:
-            self._step = self.cache.begin(self.seqs, n_tokens)
+            self._step = self.cache.begin(self.seqs, n_tokens, branches=self.branches)
         return self._step
 
     def commit(self, n_frames: int):
@@ -427,10 +442,12 @@ class PagedKVCacheSet:
         self.frames += n_frames
 
     def branch(self, copies: int) -> None:
-        """Every stream becomes ``copies`` streams (those of the first stream first)."""
+        """Every stream becomes ``copies`` streams (those of the first stream first). What they still
+        share of their past is read once for all where that is faster."""
         old = self.seqs
         self.seqs = self.cache.fork(old, copies)
         self.cache.free(old)
+        self.branches *= max(copies, 1)
         self._step = None
 
 
@@ -472,7 +489,7 @@ def _block_cached_torch(blk: WorldDiTBlock, x, mod, tab_q, cache: LayerKVCache, 
     h = norm(x, blk.norm1.weight) * (1 + s1) + b1
     qkv = (h @ blk.attn.qkv.weight.to(dt).t()).view(B, T, 3, H, Dh)
     q, k, v = qkv.unbind(2)
-    q, k = apply_rope(q, tab_q), apply_rope(k, tab_q)
+    q, k = blk.position(q, k, tab_q)
     if step is not None:
         step.write(layer, k, v)
         o = step.attend(layer, q, **attention_span(cfg, tpf))

@@ -2,7 +2,8 @@
 
 ``attention_fwd(qkv, bc)`` takes the ``[M, 3d]`` output of the QKV GEMM (q, k already
 rotated) and returns ``(o [M, d] bf16, o_lin or None, lse, aux)``;
-``attention_bwd`` returns ``dqkv [M, 3d]`` (q/k gradients still in the rotated frame).
+``attention_bwd`` returns ``dqkv [M, 3d]`` (q/k gradients still in the rotated frame). With
+``qk`` (rotated queries and keys ``[B, T, H, 64]``, dense modes) only v is read from ``qkv``.
 
 Modes: ``dense`` (frame-causal / token-causal / bidirectional softmax attention) and
 ``sla`` (top-k block routing, block-sparse softmax, linear branch).
@@ -28,10 +29,10 @@ def _kernels(t: torch.Tensor) -> bool:
     return True
 
 
-def _split(qkv, bc):
+def _split(qkv, bc, qk=None):
     B, T, H, Dh = bc.B, bc.T, bc.H, bc.Dh
     q, k, v = qkv.view(B, T, 3, H, Dh).unbind(2)
-    return q, k, v
+    return (q, k, v) if qk is None else (*qk, v)
 
 
 def _torch_dense(q, k, v, bc):
@@ -51,24 +52,26 @@ def _torch_dense(q, k, v, bc):
     return o.transpose(1, 2)
 
 
-def attention_fwd(qkv: torch.Tensor, bc):
+def attention_fwd(qkv: torch.Tensor, bc, qk=None):
+    if qk is not None and bc.attn_mode != "dense":
+        raise RuntimeError("queries and keys apart from qkv need dense attention")
     if _kernels(qkv):
         from .attention_kernels import attention_fwd_kernel
 
-        return attention_fwd_kernel(qkv, bc)
+        return attention_fwd_kernel(qkv, bc, qk)
     if bc.attn_mode != "dense":
         raise RuntimeError("SLA attention on the fused block path needs CUDA tensors")
-    q, k, v = _split(qkv, bc)
+    q, k, v = _split(qkv, bc, qk)
     o = _torch_dense(q, k, v, bc)
     return o.reshape(qkv.shape[0], -1).contiguous(), None, None, None
 
 
-def attention_bwd(qkv, o, lse, do, do_lin, aux, bc):
+def attention_bwd(qkv, o, lse, do, do_lin, aux, bc, qk=None):
     if _kernels(qkv):
         from .attention_kernels import attention_bwd_kernel
 
-        return attention_bwd_kernel(qkv, o, lse, do, do_lin, aux, bc)
-    q, k, v = (t.detach().requires_grad_(True) for t in _split(qkv, bc))
+        return attention_bwd_kernel(qkv, o, lse, do, do_lin, aux, bc, qk)
+    q, k, v = (t.detach().requires_grad_(True) for t in _split(qkv, bc, qk))
     with torch.enable_grad():
         out = _torch_dense(q, k, v, bc)
         gq, gk, gv = torch.autograd.grad(out, (q, k, v), do.view_as(out))

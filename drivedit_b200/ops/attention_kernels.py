@@ -174,22 +174,29 @@ def sla_linear_bwd_kernel(qkv, o_lin, do_lin, plan: SLAKernelPlan, dqkv, B, T, H
     ext().sla_lin_bwd_kv(qkv, dkvz, dqkv, B, T, H)
 
 
-def _heads(qkv, bc):
+def _heads(qkv, bc, qk=None):
     B, T, H = bc.B, bc.T, bc.H
     v = qkv.view(B, T, 3, H, 64)
-    return v[:, :, 0], v[:, :, 1], v[:, :, 2]
+    return (v[:, :, 0], v[:, :, 1], v[:, :, 2]) if qk is None else (*qk, v[:, :, 2])
+
+
+def _columns(qkv, bc, qk):
+    """(q, k, v, their first columns) for the packed kernels."""
+    if qk is None:
+        return qkv, qkv, qkv, 0, bc.d, 2 * bc.d
+    return qk[0].view(-1, bc.d), qk[1].view(-1, bc.d), qkv, 0, 0, 2 * bc.d
 
 
 def _window_args(bc):
     return dict(frames_span(bc.causal, bc.tpf, bc.window_frames, bc.sink_frames), scale=1.0 / math.sqrt(bc.Dh))
 
 
-def attention_fwd_kernel(qkv: torch.Tensor, bc):
+def attention_fwd_kernel(qkv: torch.Tensor, bc, qk=None):
     B, T, H, d = bc.B, bc.T, bc.H, bc.d
     assert bc.Dh == 64, "the attention kernels are written for d_head = 64"
     M = qkv.shape[0]
     if bc.window_frames and bc.attn_mode == "dense":
-        o4, lse, rest = ext().attn_window_fwd(*_heads(qkv, bc), **_window_args(bc))
+        o4, lse, rest = ext().attn_window_fwd(*_heads(qkv, bc, qk), **_window_args(bc))
         return o4.view(M, d), None, lse, rest
     o = torch.empty(M, d, device=qkv.device, dtype=torch.bfloat16)
     lse = torch.empty(B * H * T, device=qkv.device, dtype=torch.float32)
@@ -203,19 +210,20 @@ def attention_fwd_kernel(qkv: torch.Tensor, bc):
         lists = (plan.pair_blocks, plan.pair_mask, plan.pair_count)
         o_lin = sla_linear_fwd_kernel(qkv, plan, B, T, H)
         plan.o_lin = o_lin
-    ext().attn_fwd(qkv, qkv, qkv, o, lse, 0, d, 2 * d, 0, B, H, T, T, T, T, causal, bc.tpf,
+    q, k, v, *cols = _columns(qkv, bc, qk)
+    ext().attn_fwd(q, k, v, o, lse, *cols, 0, B, H, T, T, T, T, causal, bc.tpf,
                    0, 0, scale, *lists)
     return o, o_lin, lse, plan
 
 
-def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc):
+def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc, qk=None):
     B, T, H, d = bc.B, bc.T, bc.H, bc.d
     M = qkv.shape[0]
     dev = qkv.device
     if bc.window_frames and bc.attn_mode == "dense":
         dqkv = torch.empty(M, 3 * d, device=dev, dtype=torch.bfloat16)
         dq, dk, dv = _heads(dqkv, bc)
-        ext().attn_window_bwd(*_heads(qkv, bc), o.view(B, T, H, 64), plan, lse, do.view(B, T, H, 64), dq=dq, dk=dk, dv=dv,
+        ext().attn_window_bwd(*_heads(qkv, bc, qk), o.view(B, T, H, 64), plan, lse, do.view(B, T, H, 64), dq=dq, dk=dk, dv=dv,
                               **_window_args(bc))
         return dqkv
     delta = torch.empty(B * H * T, device=dev, dtype=torch.float32)
@@ -225,7 +233,8 @@ def attention_bwd_kernel(qkv, o, lse, do, do_lin, plan, bc):
     lists = (None, None, None)
     if plan is not None:
         lists = (plan.kv_qtiles, plan.kv_qmask, plan.kv_count)
-    ext().attn_bwd(qkv, qkv, qkv, o, do, lse, delta, dq_acc, dqkv, dqkv, 0, d, 2 * d, 0, 0, d,
+    q, k, v, *cols = _columns(qkv, bc, qk)
+    ext().attn_bwd(q, k, v, o, do, lse, delta, dq_acc, dqkv, dqkv, *cols, 0, 0, d,
                    2 * d, B, H, T, T, T, T, CAUSAL[bc.causal], bc.tpf, 0, 0,
                    1.0 / math.sqrt(bc.Dh), *lists, 0)
     ext().attn_dq_finalize(dq_acc, dqkv, 0, H, None, T, 0)

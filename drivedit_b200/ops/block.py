@@ -5,6 +5,7 @@ Per block, with ``M = B*T`` token rows, ``d`` model width, ``F`` SwiGLU width:
 forward                                           kernels
   h1, r1 = adaln_rmsnorm(x, w1, mod[s1, b1])        fused/norm.cu
   qkv    = h1 Wqkv^T  (+ 3-D RoPE on q, k)          gemm.cu, rope epilogue
+  (with qk_norm: qkv = h1 Wqkv^T, then q, k normed and rotated   gemm.cu, rotary/rotary.cu)
   o, lse = attention(qkv)  (dense or SLA)           attn/*.cu
   x1     = x + o Wo^T (+ o_lin Wlin^T)              gemm.cu, residual epilogue
   h2, r2 = adaln_rmsnorm(x1, w2, mod[s2, b2])
@@ -28,6 +29,7 @@ from typing import Optional
 import torch
 
 from ..parallel.flat import FlatParamGroup
+from ._ext import ext
 from .attention import attention_bwd, attention_fwd
 from .fused import adaln_rmsnorm, adaln_rmsnorm_bwd, rope_rotate_
 from .gemm import gemm
@@ -38,7 +40,7 @@ class BlockCtx:
     """Static per-call data shared by all blocks of one forward."""
 
     def __init__(self, B, T, frames, tpf, d, H, Dh, rope_tab, attn_mode, sla_cfg, causal,
-                 rope_pos_offset=0, window_frames=0, sink_frames=0):
+                 rope_pos_offset=0, window_frames=0, sink_frames=0, qk_eps=None):
         self.B, self.T, self.frames, self.tpf = B, T, frames, tpf
         self.d, self.H, self.Dh = d, H, Dh
         self.rope_tab = rope_tab
@@ -47,6 +49,7 @@ class BlockCtx:
         self.causal = causal
         self.rope_pos_offset = rope_pos_offset
         self.window_frames, self.sink_frames = window_frames, sink_frames
+        self.qk_eps = qk_eps  # eps of the norms of queries and keys (None: the model has none)
         self.recompute = False  # activation checkpointing: blocks rerun their forward in backward
         self.grad_ready = None  # callback(block index) once a block's backward is enqueued
 
@@ -57,19 +60,31 @@ def _gather_of(W):
     return fn if fn is not None else (lambda p: None)
 
 
+def _qk_args(qkv, blk, bc):
+    """The queries' and keys' norms and rotation, as the extension takes them: of ``qkv [M, 3d]``."""
+    q, k, _ = qkv.view(bc.B, bc.T, 3, bc.H, bc.Dh).unbind(2)
+    return (q, k, blk.attn.q_norm.weight.detach(), blk.attn.k_norm.weight.detach(), bc.rope_tab, None, bc.rope_pos_offset,
+            "interleaved", bc.qk_eps)
+
+
 def _attn_forward(x, mod, blk, W, bc):
     d = bc.d
     G = _gather_of(W)
     h1, r1 = adaln_rmsnorm(x, blk.norm1.weight, mod, 0, d, bc.tpf)
-    qkv = gemm(h1, W(blk.attn.qkv.weight), epi="rope", rope_tab=bc.rope_tab, rope_cols=2 * d,
-               rope_rows_per_seq=bc.T, rope_pos_offset=bc.rope_pos_offset, rope_head_dim=bc.Dh,
-               gather=G(blk.attn.qkv.weight))
-    o, o_lin, lse, aux = attention_fwd(qkv, bc)
+    if bc.qk_eps is None:
+        qk = None
+        qkv = gemm(h1, W(blk.attn.qkv.weight), epi="rope", rope_tab=bc.rope_tab, rope_cols=2 * d,
+                   rope_rows_per_seq=bc.T, rope_pos_offset=bc.rope_pos_offset, rope_head_dim=bc.Dh,
+                   gather=G(blk.attn.qkv.weight))
+    else:
+        qkv = gemm(h1, W(blk.attn.qkv.weight), gather=G(blk.attn.qkv.weight))
+        qk = ext().qk_norm_rotary_fwd(*_qk_args(qkv, blk, bc))
+    o, o_lin, lse, aux = attention_fwd(qkv, bc, qk)
     x1 = gemm(o, W(blk.attn.proj.weight), residual=x, gather=G(blk.attn.proj.weight))
     if o_lin is not None:
         gemm(o_lin, W(blk.attn.proj_lin.weight), x1, residual=x1,
              gather=G(blk.attn.proj_lin.weight))
-    return x1, dict(x=x, h1=h1, r1=r1, qkv=qkv, o=o, o_lin=o_lin, lse=lse, aux=aux)
+    return x1, dict(x=x, h1=h1, r1=r1, qkv=qkv, qk=qk, o=o, o_lin=o_lin, lse=lse, aux=aux)
 
 
 def _attn_backward(dx1, sa, blk, W, bc, mod, dmod):
@@ -81,9 +96,14 @@ def _attn_backward(dx1, sa, blk, W, bc, mod, dmod):
     if sa["o_lin"] is not None:
         do_lin = gemm(dx1, W(blk.attn.proj_lin.weight), b_t=True)
         gemm(dx1, sa["o_lin"], blk.attn.proj_lin.weight.grad, epi="f32_acc", a_t=True, b_t=True)
-    dqkv = attention_bwd(sa["qkv"], sa["o"], sa["lse"], do, do_lin, sa["aux"], bc)
-    # q, k gradients back through the rotation
-    rope_rotate_(dqkv, 2 * d, bc.rope_tab, bc.Dh, bc.T, bc.rope_pos_offset, inverse=True)
+    dqkv = attention_bwd(sa["qkv"], sa["o"], sa["lse"], do, do_lin, sa["aux"], bc, sa["qk"])
+    # q, k gradients back through the rotation (and the norms), in place
+    if bc.qk_eps is None:
+        rope_rotate_(dqkv, 2 * d, bc.rope_tab, bc.Dh, bc.T, bc.rope_pos_offset, inverse=True)
+    else:
+        dq, dk, _ = dqkv.view(bc.B, bc.T, 3, bc.H, bc.Dh).unbind(2)
+        ext().qk_norm_rotary_bwd(*_qk_args(sa["qkv"], blk, bc), dq, dk, dq, dk, blk.attn.q_norm.weight.grad,
+                                 blk.attn.k_norm.weight.grad, True)
     dh1 = gemm(dqkv, W(blk.attn.qkv.weight), b_t=True)
     gemm(dqkv, sa["h1"], blk.attn.qkv.weight.grad, epi="f32_acc", a_t=True, b_t=True)
     return adaln_rmsnorm_bwd(dh1, sa["x"], sa["r1"], blk.norm1.weight, mod, 0, d, bc.tpf, dmod,
@@ -306,7 +326,7 @@ class FusedWorldDiT:
         tab = model.rope.table(Fr, frame_offset).to(x.device)
         bc = BlockCtx(B, T, Fr, T // Fr, d, cfg.n_heads, cfg.d_head, tab, cfg.attention,
                       cfg.sla, cfg.causal, window_frames=cfg.window_frames,
-                      sink_frames=cfg.sink_frames)
+                      sink_frames=cfg.sink_frames, qk_eps=cfg.norm_eps if cfg.qk_norm else None)
         bc.recompute = self.recompute and torch.is_grad_enabled()
         bc.grad_ready = self.grad_ready
         feats = None
@@ -387,7 +407,7 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
     cache window -> flash attention with absolute query/key offsets -> output GEMM with
     residual -> AdaLN-RMSNorm -> SwiGLU GEMM -> down GEMM with residual."""
     from ..models.world_dit import PagedKVCacheSet, attention_span, patchify, unpatchify
-    from ._ext import ext
+    from .rotary import qk_norm_rotary
 
     cfg = model.cfg
     g = self.group
@@ -419,8 +439,13 @@ def _forward_cached_fused(self, model, x_t, t, actions, cache, commit, extra_con
         else:
             mod = blk.ada(c2)
         h1, _ = adaln_rmsnorm(x, blk.norm1.weight, mod, 0, d, tpf)
-        qkv = gemm(h1, W(blk.attn.qkv.weight), epi="rope", rope_tab=tab, rope_cols=2 * d,
-                   rope_rows_per_seq=T, rope_head_dim=cfg.d_head)
+        if cfg.qk_norm:
+            qkv = gemm(h1, W(blk.attn.qkv.weight))
+            q_, k_, _ = qkv.view(B, T, 3, Hh, cfg.d_head).unbind(2)
+            qk_norm_rotary(q_, k_, blk.attn.q_norm.weight, blk.attn.k_norm.weight, tab, eps=cfg.norm_eps, inplace=True)
+        else:
+            qkv = gemm(h1, W(blk.attn.qkv.weight), epi="rope", rope_tab=tab, rope_cols=2 * d,
+                       rope_rows_per_seq=T, rope_head_dim=cfg.d_head)
         q3 = qkv.view(B, T, 3 * d)
         if paged:
             qh, kh, vh = qkv.view(B, T, 3, Hh, cfg.d_head).unbind(2)

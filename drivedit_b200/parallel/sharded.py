@@ -214,7 +214,7 @@ class ShardedDataParallel:
         spans: Dict[int, list] = {}
         for name in self.flat.names:
             mm = re.match(r"^blocks\.(\d+)\.", name)
-            if mm is None or ".ada." in name or name.endswith("norm1.weight") or name.endswith("norm2.weight"):
+            if mm is None or ".ada." in name or name.endswith(("norm1.weight", "norm2.weight", "_norm.weight")):
                 continue
             o, k = self.flat.offsets[name]
             spans.setdefault(int(mm.group(1)), []).append((o, o + k))

@@ -123,6 +123,8 @@ class TensorParallelWorldDiT:
         residual stream replicated on every rank and all-reduces (see the module notes)."""
         if model.cfg.window_frames:
             raise ValueError("windowed models (window_frames) have no tensor-parallel rollout")
+        if model.cfg.qk_norm:
+            raise ValueError("models with qk_norm have no tensor-parallel rollout")
         self.model = model
         self.cfg = model.cfg
         self.group = group if group is not None else dist.group.WORLD

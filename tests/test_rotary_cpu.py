@@ -143,3 +143,133 @@ def test_position_outside_the_table():
     for bad in (-1, 8):
         with pytest.raises(IndexError):
             rotary(x, tab, torch.tensor([0, 1, bad, 2]))
+
+
+def _model(*over):
+    from drivedit_b200.config import get_config
+    from drivedit_b200.models.world_dit import WorldDiT
+    torch.manual_seed(0)
+    cfg = get_config("tiny", ["model.n_layers=2", "model.qk_norm=true", *over])
+    m = WorldDiT(cfg.model)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if p.abs().sum() == 0:
+                p.normal_(0, 0.02)
+            elif "_norm" in n:
+                p.uniform_(0.5, 1.5)
+    return cfg, m
+
+
+def test_model_with_norms():
+    """Its streams, through the rolling buffers and the 8-bit pages, against its full forward; its norms
+    are learned, keep out of weight decay, and scaling queries before them changes nothing."""
+    from drivedit_b200.models.world_dit import KVCacheSet, PagedKVCacheSet, forward_cached
+    _, m = _model()
+    x, t, a = torch.randn(2, 4, 16, 16, 16), torch.rand(2), torch.rand(2, 4, 2)
+    full = m(x, t, a)
+    for cache, bound in ((KVCacheSet(m, 2, 4, 2, "cpu", torch.float32), 1e-5), (PagedKVCacheSet(m, 2, 4, 2, "cpu", max_frames=4), 2.0 ** -4)):
+        got = torch.cat([forward_cached(m, x[:, f:f + 2], t, a[:, f:f + 2], cache, commit=True) for f in (0, 2)], 1)
+        # the pages' keys and values are rounded to 2^-4 of themselves, averaged over a head
+        assert (got - full).norm() / full.norm() < bound
+    full.square().sum().backward()
+    names = [n for n, _ in m.named_parameters() if "q_norm" in n or "k_norm" in n]
+    assert len(names) == 4 and set(names) <= set(m.no_decay_names())
+    assert all(m.get_parameter(n).grad.abs().sum() > 0 for n in names)
+    with torch.no_grad():
+        d = m.cfg.d_model
+        for b in m.blocks:
+            b.attn.qkv.weight[:2 * d] *= 4
+    # eps is 1e-6 of a mean square near 0.1
+    assert torch.allclose(m(x, t, a), full, atol=1e-3)
+    with pytest.raises(ValueError):
+        _model("model.attention=sla")
+
+
+def test_branches_of_a_model_with_norms():
+    from drivedit_b200.inference.rollout import StreamingRollout
+    cfg, m = _model()
+    r = cfg.rollout
+    r.total_frames, r.chunk_frames, r.flow_steps, r.window_frames, r.kv_cache, r.sink_frames = 8, 2, 2, 3, "fp8", 1
+    ctx, act = torch.randn(2, 2, 16, 16, 16), torch.rand(2, 3, 8, 2)
+    act[:, :, :2] = act[:, :1, :2]
+    roll = StreamingRollout(m, r)
+    res = roll.run_branches(ctx, act, generator=torch.Generator().manual_seed(1))
+    one = roll.run(ctx.repeat_interleave(3, 0), act.flatten(0, 1), generator=torch.Generator().manual_seed(1))
+    assert torch.allclose(one.frames, res.frames, atol=1e-4)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_shared_pages_of_random_runs(seed):
+    """The rows of a step's groups: the leading pages that all sequences of a group share, or have given
+    back, and that hold committed tokens only; the CPU form does not depend on the groups."""
+    import random
+    from drivedit_b200.ops.kv_cache import _INFO, PAGE, PagedKVCache
+    rng = random.Random(seed)
+    c = PagedKVCache(1, 1, 400, device="cpu", max_pages_per_seq=30)
+    roots = c.add(3)
+    c.begin(roots, [rng.randint(0, 700) for _ in roots]).commit()
+    seqs = c.fork(roots, 4)
+    for _ in range(25):
+        n = [rng.choice([0, 1, 1, 5, 70]) for _ in seqs]
+        branches = rng.choice([2, 3, 4, 6, 12])
+        step = c.begin(seqs, n, branches=branches)
+        assert step.table.shape == (12, 30) and step._rows.shape[0] == 12 + 12 // branches
+        for g in range(12 // branches):
+            own = [c._seqs[s] for s in seqs[g * branches:(g + 1) * branches]]
+            row = step._rows[12 + g].tolist()
+            most = min(s.length // PAGE for s in own)
+            want = []
+            for j in range(most):
+                ids = {int(s.pages[j]) for s in own} - {-1}
+                if len(ids) > 1:
+                    break
+                want.append(ids.pop() if ids else -1)
+            assert row[0] == len(want) and row[_INFO:_INFO + len(want)] == want and set(row[_INFO + len(want):]) <= {-1}
+        if rng.random() < 0.7:
+            step.commit()
+        if rng.random() < 0.3:
+            c.trim(rng.sample(seqs, 5), rng.choice([100, 200, 400]), 70)
+        if rng.random() < 0.15:
+            c.compact()
+        if rng.random() < 0.2:  # a sequence starts anew from another
+            i, j = rng.sample(range(12), 2)
+            c.free([seqs[i]])
+            seqs[i] = c.fork([seqs[j]])[0]
+        if max(c.length(s) for s in seqs) > 1700:
+            break
+
+
+def test_groups_do_not_change_what_is_computed():
+    from drivedit_b200.ops.kv_cache import PagedKVCache
+    c = PagedKVCache(1, 2, 40, device="cpu")
+    roots = c.add(1)
+    step = c.begin(roots, 150)
+    step.write(0, torch.randn(1, 150, 2, 64), torch.randn(1, 150, 2, 64))
+    step.commit()
+    kids = c.fork(roots, 3)
+    q = torch.randn(3, 2, 4, 64)
+    outs = []
+    for branches in (1, 3):
+        step = c.begin(kids, 2, branches=branches)
+        step.write(0, *(torch.ones(3, 2, 2, 64) * x for x in (1, 2)))
+        outs.append(step.attend(0, q, causal="token"))
+    assert torch.equal(*outs)
+    for n in (0, 2, -3):
+        with pytest.raises(ValueError):
+            c.begin(kids, 1, branches=n)
+    with pytest.raises(ValueError):
+        c.begin(kids, 1, out=step)
+    free = c.free_pages
+    c.begin(kids, 2, out=step, branches=3)
+    assert c.free_pages == free
+
+
+def test_norms_keep_the_gradient_buckets_whole():
+    """The overlapped reduce-scatter's buckets of a model with norms: a run for every block."""
+    from drivedit_b200.parallel.flat import FlatParamGroup
+    from drivedit_b200.parallel.sharded import ShardedDataParallel
+    cfg, m = _model()
+    eng = ShardedDataParallel.__new__(ShardedDataParallel)
+    eng.world, eng.rank = 2, 0
+    eng.flat = FlatParamGroup(m.flat_layout(m.named_parameters()), "cpu", no_decay=m.no_decay_names(), pad_to=8)
+    assert eng._plan_pieces() is not None and eng.bucket_ids == set(range(cfg.model.n_layers))

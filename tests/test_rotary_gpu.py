@@ -434,3 +434,86 @@ def test_counts_launches():
     n = ext().launch_count()
     qk_norm_rotary(x, x, table=tab)
     assert ext().launch_count() == n + 1
+
+
+def _world(*over, frames=4):
+    from drivedit_b200.config import get_config
+    from drivedit_b200.models.world_dit import WorldDiT
+    torch.manual_seed(0)
+    cfg = get_config("tiny", ["model.n_layers=2", "model.qk_norm=true", f"train.frames={frames}", *over])
+    m = WorldDiT(cfg.model)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if p.abs().sum() == 0:
+                p.normal_(0, 0.02)
+            elif "_norm" in n:
+                p.uniform_(0.5, 1.5)
+    return cfg, m
+
+
+@pytest.mark.parametrize("recompute", [False, True])
+@pytest.mark.parametrize("over", [(), ("model.window_frames=2", "model.sink_frames=1"), ("model.causal=token",)])
+def test_model_trains_on_the_kernels(over, recompute):
+    """The flagship's fused forward and backward with norms of queries and keys against its PyTorch
+    path; gradients add up over two passes."""
+    cfg, m = _world(*over)
+    m = m.cuda()
+    x, t, a = torch.randn(2, 4, 16, 16, 16, device="cuda"), torch.rand(2, device="cuda"), torch.rand(2, 4, 2, device="cuda")
+    w = torch.randn(2, 4, 16, 16, 16, device="cuda")
+    ref = m(x, t, a)
+    (ref * w).sum().backward()
+    names = ["blocks.0.attn.qkv.weight", "blocks.0.attn.q_norm.weight", "blocks.1.attn.k_norm.weight", "blocks.1.attn.proj.weight"]
+    want = {n: p.grad.clone() for n, p in m.named_parameters() if n in names}
+    m.zero_grad(set_to_none=True)
+    m.enable_fused()
+    m.fused.recompute = recompute
+    m.fused.group.grad.zero_()
+    for _ in range(2):
+        got = m(x, t, a)
+        # bf16 activations (2^-8 a rounding, about 20 in a row in two blocks) against fp32
+        assert (got.float() - ref).norm() / ref.norm() < 20 * 2.0 ** -9
+        (got.float() * w).sum().backward()
+    for n, p in m.named_parameters():
+        if n in names:
+            assert (p.grad - 2 * want[n]).norm() / (2 * want[n]).norm() < 40 * 2.0 ** -9, n
+
+
+def test_streams_on_the_kernels_match_the_pytorch_form():
+    from drivedit_b200.inference.rollout import StreamingRollout
+    from drivedit_b200.models.world_dit import KVCacheSet, PagedKVCacheSet, forward_cached
+    x, t, a = torch.randn(2, 6, 16, 16, 16), torch.rand(2), torch.rand(2, 6, 2)
+    outs = []
+    for dev, dt in (("cpu", torch.float32), ("cuda", torch.bfloat16)):
+        cfg, m = _world()
+        m = m.to(dev)
+        if dev == "cuda":
+            m.enable_fused()
+        caches = [PagedKVCacheSet(m, 2, 2, 2, torch.device(dev), 1, 6), KVCacheSet(m, 2, 4, 2, dev, dt)]
+        outs.append([torch.cat([forward_cached(m, x[:, f:f + 2].to(dev, dt), t.to(dev), a[:, f:f + 2].to(dev), c, commit=True)
+                                .float().cpu() for f in (0, 2, 4)], 1) for c in caches])
+    for got, want in zip(outs[1], outs[0]):
+        # bf16 activations, and codes that fall to the other side of an e4m3 step for it
+        assert (got - want).norm() / want.norm() < 20 * 2.0 ** -9 + 2.0 ** -5
+    r = cfg.rollout
+    r.chunk_frames, r.flow_steps, r.window_frames, r.kv_cache, r.sink_frames = 1, 2, 6, "fp8", 1
+    ctx, act = torch.randn(1, 6, 16, 16, 16, device="cuda"), torch.rand(1, 4, 12, 2, device="cuda")
+    act[:, :, :6] = act[:, :1, :6]
+    roll = StreamingRollout(m, r)
+    g = lambda: torch.Generator(device="cuda").manual_seed(4)  # noqa: E731
+    res = roll.run_branches(ctx, act, total_frames=12, generator=g())
+    one = roll.run(ctx.repeat_interleave(4, 0), act.flatten(0, 1), total_frames=12, generator=g())
+    # the same pages' contents; read by other kernels
+    assert (res.frames - one.frames).norm() / one.frames.norm() < 2.0 ** -6
+
+
+def test_apply_rope_on_cuda_is_the_kernel():
+    from drivedit_b200.layers.rope import RoPE3D, apply_rope
+    from drivedit_b200.ops._ext import ext
+    rope = RoPE3D(64, 2, 3, 8).cuda()
+    for dtype in TYPES:
+        x = torch.randn(2, 24, 3, 64, device="cuda").to(dtype)
+        n = ext().launch_count()
+        y = apply_rope(x, rope.table(4, 2))
+        assert ext().launch_count() == n + 1
+        assert torch.equal(y.cpu(), apply_rope(x.cpu(), rope.table(4, 2).cpu()))
+        assert torch.equal(apply_rope(x[None], rope.table(4, 2))[0], y)  # more leading axes: the PyTorch form
