@@ -143,8 +143,14 @@ int* device_status(int device) {
   check_cuda(cudaGetDevice(&prev), "cudaGetDevice");
   check_cuda(cudaSetDevice(device), "cudaSetDevice");
   int* p = nullptr;
-  check_cuda(cudaMalloc(&p, sizeof(int) * 8), "cudaMalloc(status)");
-  check_cuda(cudaMemset(p, 0, sizeof(int) * 8), "cudaMemset(status)");
+  // the first call of a process may be a captured one
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+  const cudaError_t made = cudaMalloc(&p, sizeof(int) * 8);
+  const cudaError_t cleared = made == cudaSuccess ? cudaMemset(p, 0, sizeof(int) * 8) : made;
+  check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+  check_cuda(made, "cudaMalloc(status)");
+  check_cuda(cleared, "cudaMemset(status)");
   check_cuda(cudaSetDevice(prev), "cudaSetDevice");
   words[device] = p;
   return p;

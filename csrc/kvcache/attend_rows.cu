@@ -456,6 +456,7 @@ void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
 // tiles of the other kernel. (Its rows' division by multiplication is exact far beyond.)
 constexpr long kMaxRows = 256;
 std::atomic<int> g_branch_mode{0};
+constexpr long kMaxScratch = 1L << 28;  // floats that groups taken together may need
 // 8-row warps of a row tile
 int row_warps(long rows) { return rows <= 24 ? static_cast<int>(rows + 7) / 8 : 4; }
 
@@ -486,7 +487,8 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
   const int mode = g_branch_mode.load(std::memory_order_relaxed);
   if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows && mode != 1) {
     const KvPlan group = kv_attend_branches_plan(a, mode, dev);
-    if (mode || group.us < alone.us * (!alone.blocks && rows <= 8 ? 0.65 : 1.)) return group;
+    const bool faster = group.us < alone.us * (!alone.blocks && rows <= 8 ? 0.65 : 1.);
+    if (mode || (faster && group.scratch <= kMaxScratch)) return group;
   }
   return alone;
 }

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
 #include "../common/ptx.cuh"
 #include "../common/tma.h"
@@ -61,6 +62,12 @@ template <>
 struct Io<__nv_bfloat16> {
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ void get2(const __nv_bfloat16* p, float& x, float& y) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    x = __uint_as_float(w << 16);
+    y = __uint_as_float(w & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void put2(__nv_bfloat16* p, float x, float y) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
     const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
@@ -77,6 +84,12 @@ template <>
 struct Io<__half> {
   static __device__ __forceinline__ float get(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+  static __device__ __forceinline__ void get2(const __half* p, float& x, float& y) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+    x = f.x;
+    y = f.y;
+  }
+  static __device__ __forceinline__ void put2(__half* p, float x, float y) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
     const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
@@ -100,6 +113,12 @@ template <>
 struct Io<float> {
   static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void get2(const float* p, float& x, float& y) {
+    const float2 f = *reinterpret_cast<const float2*>(p);
+    x = f.x;
+    y = f.y;
+  }
+  static __device__ __forceinline__ void put2(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[4], float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -149,12 +168,8 @@ __device__ __forceinline__ float2 turn(float x, float y, float c, float s) {
   return make_float2(__fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)), __fadd_rn(__fmul_rn(x, s), __fmul_rn(y, c)));
 }
 
-// (mean + eps)^-1/2 of a sum of squares. `down`: a power of two by which the squares' roots were
-// brought down so that the sum stays finite.
-__device__ __forceinline__ float rms_inv(float sum, float D, float eps, float down) {
-  return __frcp_rn(__fsqrt_rn(__fdiv_rn(sum, D) + eps * down * down));
-}
-constexpr float kDown = 0x1p-70f;  // its square times a sum of 256 squares of the largest fp32 is finite
+// Rows whose squares pass fp32 are brought down by it: 256 squares of the largest number then stay finite
+constexpr float kDown = 0x1p-70f;
 
 // Where a lane's two runs of 8 channels begin on one side. Pairs in halves: a run in each. Side by
 // side: 4 pairs in each run, which lie R / 2 apart as well, so that the lanes of an access are
@@ -478,112 +493,142 @@ __global__ void __launch_bounds__(kThreads, 2) rot_wide_back(const Launch L) {
   }
 }
 
-// Heads of any even size up to 256, any strides: 8 lanes (16 above 128 channels) a head, 8 pairs a lane.
-template <typename T, bool NORM, bool BWD>
-__global__ void __launch_bounds__(kThreads) rot_any(const Launch L) {
+// Heads of any even size up to 256, any strides: 8 lanes (16 above 128 channels) a head, up to 8
+// pairs a lane, U heads of one token. IN2, OUT2: on that side pairs lie side by side and a pair's two
+// channels are one access.
+template <typename T, bool NORM, bool BWD, bool IN2, bool OUT2>
+__global__ void __launch_bounds__(kThreads, 2) rot_any(const Launch L) {
+  constexpr int U = BWD ? 1 : 2, NP = 8;
   const RotArgs& a = L.a;
   const int which = blockIdx.x >= L.ctas0;
   const RotTensor& t = a.t[which];
   const int lg = L.log_lanes, l = threadIdx.x & ((1 << lg) - 1);
-  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * t.H, per = kThreads >> lg;
+  const int blocks = L.heads[which];
+  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * blocks, per = kThreads >> lg;
   const int pairs = a.D / 2, turned = a.R / 2;
-  // channels of a lane's pair i as one side has them
+  // Channels of a lane's pair as one side has them. The lanes that have a pair i, if any:
+  auto have = [&](int i) { return l + (i << lg) < pairs; };
   auto chan = [&](int i, bool halves, int& c0, int& c1) {
     const int p = l + (i << lg);
-    if (i << lg >= pairs) return false;  // for all lanes
     if (p < turned && halves) c0 = p, c1 = p + turned;
     else c0 = 2 * p, c1 = 2 * p + 1;
-    return p < pairs;
   };
-  float dw[16];
+  auto load = [&](const T* p, int i, bool halves, auto two, float& x, float& y) {
+    int c0, c1;
+    if constexpr (decltype(two)::value) {
+      Io<T>::get2(p + 2 * (l + (i << lg)), x, y);
+    } else {
+      chan(i, halves, c0, c1);
+      x = Io<T>::get(p + c0), y = Io<T>::get(p + c1);
+    }
+  };
+  const float inv_D = 1.f / static_cast<float>(a.D);
+  float2 dw[NP];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
-  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), ctas = which ? L.ctas1 : L.ctas0;
-  for (uint32_t i0 = cta * per; i0 < n; i0 += ctas * per) {
+  for (int i = 0; i < NP; ++i) dw[i] = both(0.f);
+  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), step = (which ? L.ctas1 : L.ctas0) * per;
+  for (uint32_t i0 = cta * per; i0 < n; i0 += step) {
     const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
-    const T* x = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st + it.h * t.x_sh;
-    const T* dy = reinterpret_cast<const T*>(t.g) + it.b * t.g_sb + it.t * t.g_st + it.h * t.g_sh;
-    T* y = reinterpret_cast<T*>(t.y) + it.b * t.y_sb + it.t * t.y_st + it.h * t.y_sh;
-    float v[16], g[16];
+    const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
+    const T* pg = reinterpret_cast<const T*>(t.g) + it.b * t.g_sb + it.t * t.g_st;
+    T* py = reinterpret_cast<T*>(t.y) + it.b * t.y_sb + it.t * t.y_st;
+    float2 v[U][NP], g[BWD ? U : 1][NP], cs[NP];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      int c0, c1;
-      v[2 * i] = v[2 * i + 1] = g[2 * i] = g[2 * i + 1] = 0.f;
-      if (chan(i, a.layout.in_halves, c0, c1) && it.there) v[2 * i] = Io<T>::get(x + c0), v[2 * i + 1] = Io<T>::get(x + c1);
-      if (BWD && chan(i, a.layout.out_halves, c0, c1) && it.there) g[2 * i] = Io<T>::get(dy + c0), g[2 * i + 1] = Io<T>::get(dy + c1);
-    }
-    float r = 1.f;
-    if (NORM) {
-      float down = 1.f;
-      auto sum = [&]() {
-        float s = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int h = it.h + u * blocks;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s = fmaf(v[i], v[i], s);
-        for (int o = 1; o < 1 << lg; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-        return s;
-      };
-      float s = sum();
-      if (__any_sync(0xffffffffu, !(s < 1e38f))) {
-        if (!(s < 1e38f)) down = kDown;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= down;
-        s = sum();
+      for (int i = 0; i < NP; ++i) {
+        v[u][i] = both(0.f);
+        if (BWD) g[u][i] = both(0.f);
+        if (i << lg >= pairs) continue;  // for all lanes
+        if (!have(i) || !it.there || h >= t.H) continue;
+        load(px + h * t.x_sh, i, a.layout.in_halves, std::bool_constant<IN2>{}, v[u][i].x, v[u][i].y);
+        if (BWD) load(pg + h * t.g_sh, i, a.layout.out_halves, std::bool_constant<OUT2>{}, g[u][i].x, g[u][i].y);
       }
-      r = rms_inv(s, static_cast<float>(a.D), a.eps, down);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int c0, c1;
-        v[2 * i] *= r, v[2 * i + 1] *= r;
-        if (!BWD && chan(i, a.layout.in_halves, c0, c1) && t.w) v[2 * i] *= t.w[c0], v[2 * i + 1] *= t.w[c1];
-      }
-      r *= down;
     }
-    float* z = BWD ? g : v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NP; ++i) {
+      cs[i] = make_float2(1.f, 0.f);
       const int p = l + (i << lg);
-      if (p < turned) {
-        float2 cs = make_float2(NAN, NAN);
-        if (it.there && it.row >= 0) cs = __ldg(a.table + static_cast<long>(it.row) * turned + p);
-        const float2 q = turn(z[2 * i], z[2 * i + 1], cs.x, a.inverse != BWD ? -cs.y : cs.y);
-        z[2 * i] = q.x;
-        z[2 * i + 1] = q.y;
+      if (p < turned && it.there) {
+        const float2 f = __ldg(a.table + static_cast<long>(max(it.row, 0)) * turned + p);
+        cs[i] = make_float2(it.row < 0 ? NAN : f.x, a.inverse != BWD ? -f.y : f.y);
       }
     }
-    if (BWD) {
-      float m = 0.f;
+    __syncwarp();  // every lane has read what another one may write (a result in the place of its input)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int c0, c1;
-        const bool have = chan(i, a.layout.in_halves, c0, c1);
-        if (have && it.there) dw[2 * i] = fmaf(g[2 * i], v[2 * i], dw[2 * i]), dw[2 * i + 1] = fmaf(g[2 * i + 1], v[2 * i + 1], dw[2 * i + 1]);
-        if (have && t.w) g[2 * i] *= t.w[c0], g[2 * i + 1] *= t.w[c1];
-        m = fmaf(g[2 * i], v[2 * i], m);
-        m = fmaf(g[2 * i + 1], v[2 * i + 1], m);
+    for (int u = 0; u < U; ++u) {
+      const int h = it.h + u * blocks;
+      float r = 1.f, down = 1.f;
+      auto dot = [&](const float2 (&x)[NP], const float2 (&y)[NP]) {
+        float2 s = mul2(x[0], y[0]);
+#pragma unroll
+        for (int i = 1; i < NP; ++i) s = fma2(x[i], y[i], s);
+        float z = s.x + s.y;
+        for (int o = 1; o < 1 << lg; o *= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
+        return z;
+      };
+      if (NORM) {
+        float s = dot(v[u], v[u]);
+        if (__any_sync(0xffffffffu, !(s < 1e38f))) {
+          if (!(s < 1e38f)) down = kDown;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) v[u][i] = mul2(v[u][i], both(down));
+          s = dot(v[u], v[u]);
+        }
+        r = rms_inv_fast(s, inv_D, a.eps * down * down);
       }
-      for (int o = 1; o < 1 << lg; o *= 2) m += __shfl_xor_sync(0xffffffffu, m, o);
-      m = __fdiv_rn(m, static_cast<float>(a.D));
+      float2 z[NP];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = r * (g[i] - v[i] * m);
-    }
-    __syncwarp();
+      for (int i = 0; i < NP; ++i) {
+        z[i] = BWD ? g[u][i] : v[u][i];
+        if (i << lg >= pairs) continue;
+        float2 w = both(1.f);
+        if (NORM && t.w && have(i)) {
+          int c0, c1;
+          chan(i, a.layout.in_halves, c0, c1);
+          w = make_float2(__ldg(t.w + c0), __ldg(t.w + c1));
+        }
+        if (NORM && !BWD) z[i] = mul2(z[i], w);
+        if (l + (i << lg) < turned) z[i] = turn(z[i].x, z[i].y, cs[i].x, cs[i].y);
+        if (NORM) z[i] = mul2(z[i], both(r));
+        if (BWD) {  // gr = g r; dw += gr x; gr w
+          dw[i] = fma2(z[i], v[u][i], dw[i]);
+          z[i] = mul2(z[i], w);
+        }
+      }
+      if (BWD) {  // dx = gr w - x r^2 mean(gr w x)
+        const float2 k = both(-dot(z, v[u]) * inv_D * r * r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      int c0, c1;
-      if (chan(i, BWD ? a.layout.in_halves : a.layout.out_halves, c0, c1) && it.there) Io<T>::put(y + c0, v[2 * i]), Io<T>::put(y + c1, v[2 * i + 1]);
+        for (int i = 0; i < NP; ++i) z[i] = mul2(fma2(v[u][i], k, z[i]), both(down));
+      }
+      T* y = py + h * t.y_sh;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (i << lg >= pairs) continue;
+        if (!have(i) || !it.there || h >= t.H) continue;
+        if constexpr (BWD ? IN2 : OUT2) {
+          Io<T>::put2(y + 2 * (l + (i << lg)), z[i].x, z[i].y);
+        } else {
+          int c0, c1;
+          chan(i, BWD ? a.layout.in_halves : a.layout.out_halves, c0, c1);
+          Io<T>::put(y + c0, z[i].x);
+          Io<T>::put(y + c1, z[i].y);
+        }
+      }
     }
   }
   if (BWD) {
     __shared__ float red[kThreads / 32][256];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < NP; ++i) {
       int c0, c1;
-      const bool have = chan(i, a.layout.in_halves, c0, c1);
+      chan(i, a.layout.in_halves, c0, c1);
       for (int o = 1 << lg; o < 32; o *= 2) {
-        dw[2 * i] += __shfl_xor_sync(0xffffffffu, dw[2 * i], o);
-        dw[2 * i + 1] += __shfl_xor_sync(0xffffffffu, dw[2 * i + 1], o);
+        dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
+        dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
       }
-      if ((threadIdx.x & 31) == l && have) red[threadIdx.x >> 5][c0] = dw[2 * i], red[threadIdx.x >> 5][c1] = dw[2 * i + 1];
+      if ((threadIdx.x & 31) == l && have(i)) red[threadIdx.x >> 5][c0] = dw[i].x, red[threadIdx.x >> 5][c1] = dw[i].y;
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.D; c += kThreads) {
@@ -617,19 +662,26 @@ __global__ void __launch_bounds__(1024) rot_weight_grad(const Launch L) {
 
 int size_of(RotType t) { return t == RotType::kF32 ? 4 : 2; }
 
-// 16-byte accesses of runs of 8 channels: heads of whole 16s, rotated channels too
-bool wide(const RotArgs& a, bool bwd) {
+// Whether all bases and strides are multiples of `bytes`
+bool aligned(const RotArgs& a, bool bwd, int bytes) {
   const int size = size_of(a.type);
-  if (a.D % 16 || a.R % 16 || reinterpret_cast<uintptr_t>(a.table) % 16) return false;
   auto ok = [&](const void* p, long sb, long st, long sh) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sb * size % 16 == 0 && st * size % 16 == 0 && sh * size % 16 == 0;
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && sb * size % bytes == 0 && st * size % bytes == 0 && sh * size % bytes == 0;
   };
   for (int i = 0; i < a.n; ++i) {
     const RotTensor& t = a.t[i];
     if (!ok(t.x, t.x_sb, t.x_st, t.x_sh) || !ok(t.y, t.y_sb, t.y_st, t.y_sh)) return false;
-    if ((bwd && !ok(t.g, t.g_sb, t.g_st, t.g_sh)) || reinterpret_cast<uintptr_t>(t.w) % 16) return false;
+    if (bwd && !ok(t.g, t.g_sb, t.g_st, t.g_sh)) return false;
   }
   return true;
+}
+
+// 16-byte accesses of runs of 8 channels: heads of whole 16s, rotated channels too
+bool wide(const RotArgs& a, bool bwd) {
+  if (a.D % 16 || a.R % 16 || reinterpret_cast<uintptr_t>(a.table) % 16) return false;
+  for (int i = 0; i < a.n; ++i)
+    if (reinterpret_cast<uintptr_t>(a.t[i].w) % 16) return false;
+  return aligned(a, bwd, 16);
 }
 
 int log2_up(int n) {
@@ -656,7 +708,7 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
     }
   };
   if (!is_wide) {
-    count(1);
+    count(bwd ? 1 : 2);
   } else if (bwd) {
     count(a.type == RotType::kF32 ? 1 : 2);  // (more spill registers)
   } else {
@@ -667,7 +719,7 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
     if (a.type != RotType::kF32 && (slots * 5 > heads * 6 || need[0] + need[1] < 4 * num_sms(dev))) count(2);
   }
   {  // CTAs that stay
-    const long room = static_cast<long>(num_sms(dev)) * (is_wide || bwd ? 2 : 8);
+    const long room = static_cast<long>(num_sms(dev)) * 2;
     const long all = need[0] + need[1];
     if (all > room)
       for (int i = 0; i < a.n; ++i) need[i] = std::max(1L, need[i] * room / all);
@@ -709,8 +761,18 @@ void launch_back(const Launch& L, cudaStream_t s) {
 }
 
 template <typename T, bool NORM, bool BWD>
+void launch_any(const Launch& L, cudaStream_t s) {
+  const bool two = aligned(L.a, BWD, 2 * sizeof(T)), in2 = two && !L.a.layout.in_halves, out2 = two && !L.a.layout.out_halves;
+  const int grid = L.ctas0 + L.ctas1;
+  if (in2 && out2) rot_any<T, NORM, BWD, true, true><<<grid, kThreads, 0, s>>>(L);
+  else if (in2) rot_any<T, NORM, BWD, true, false><<<grid, kThreads, 0, s>>>(L);
+  else if (!NORM && out2) rot_any<T, NORM, BWD, false, !NORM><<<grid, kThreads, 0, s>>>(L);
+  else rot_any<T, NORM, BWD, false, false><<<grid, kThreads, 0, s>>>(L);
+}
+
+template <typename T, bool NORM, bool BWD>
 void launch(const Launch& L, bool is_wide, cudaStream_t s) {
-  if (!is_wide) rot_any<T, NORM, BWD><<<L.ctas0 + L.ctas1, kThreads, 0, s>>>(L);
+  if (!is_wide) launch_any<T, NORM, BWD>(L, s);
   else if constexpr (BWD) launch_back<T, sizeof(T) == 4 ? 1 : 2>(L, s);
   else if constexpr (sizeof(T) == 4) launch_wide<T, NORM, 2>(L, s);
   else if (L.unroll == 2) launch_wide<T, NORM, 2>(L, s);

@@ -29,6 +29,13 @@ ddb::RotLayout layout_of(const Rotation& r) {
   return l;
 }
 
+// The table where its pairs lie on 8 bytes (a copy where they do not)
+OptTensor aligned_pairs(const OptTensor& table) {
+  if (!table || reinterpret_cast<uintptr_t>(table->data_ptr()) % 8 == 0) return table;
+  const c10::cuda::OptionalCUDAGuard guard(table->is_cuda() ? c10::optional<c10::Device>(table->device()) : c10::nullopt);
+  return table->clone();
+}
+
 // x is [B, T, H, D], or [T, H, D]
 Tensor four(const Tensor& x) { return x.dim() == 3 ? x.unsqueeze(0) : x; }
 
@@ -137,6 +144,26 @@ void check_inplace(const Tensor& x, const char* name) {
   for (int i = 0; i < x.dim() - 1; ++i) TORCH_CHECK_VALUE(x.size(i) <= 1 || x.stride(i) != 0, name, " has entries that share memory");
 }
 
+// Whether some head of q and some head of k, of equal strides over samples and tokens, share memory
+bool share_heads(const Tensor& q, const Tensor& k) {
+  if (q.numel() == 0 || k.numel() == 0 || !q.is_alias_of(k)) return false;
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3), delta = k.storage_offset() - q.storage_offset();
+  const int64_t sb = B > 1 ? q.stride(0) : 0, st = T > 1 ? q.stride(1) : 0;
+  if ((B > 1 && k.stride(0) != sb) || (T > 1 && k.stride(1) != st)) return true;  // not told apart
+  auto near = [](int64_t x, int64_t step, int64_t n, auto&& hit) {  // x - i step for the i nearest to 0, |i| < n
+    if (n <= 1) return hit(x);
+    for (int64_t i = x / step - 1; i <= x / step + 1; ++i)
+      if (std::abs(i) < n && hit(x - i * step)) return true;
+    return false;
+  };
+  for (int64_t hq = 0; hq < q.size(2); ++hq)
+    for (int64_t hk = 0; hk < k.size(2); ++hk) {
+      const int64_t d = delta + hk * (k.size(2) > 1 ? k.stride(2) : 0) - hq * (q.size(2) > 1 ? q.stride(2) : 0);
+      if (near(d, sb, B, [&](int64_t x) { return near(x, st, T, [&](int64_t y) { return std::abs(y) < D; }); })) return true;
+    }
+  return false;
+}
+
 // What was overwritten no longer is what an autograd graph may have kept of it
 void overwritten(const Tensor& x) {
   if (!x.is_inference()) torch::autograd::impl::bump_version(x);
@@ -186,8 +213,9 @@ class Rotary : public torch::autograd::Function<Rotary> {
 Tensor rotary(const Tensor& x, const Tensor& table, const OptTensor& positions, int64_t offset, const std::string& layout, bool inverse,
               bool inplace) {
   check_heads(x, "x");
-  const Rotation r{table, positions, offset, layout, inverse};
+  Rotation r{table, positions, offset, layout, inverse};
   check_rotation(r, x);
+  r.table = aligned_pairs(r.table);
   if (!at::GradMode::is_enabled() || !x.requires_grad()) return rotate(x, r, inplace);
   TORCH_CHECK_VALUE(!inplace, "x requires a gradient: it cannot be rotated in place");
   {
@@ -220,7 +248,10 @@ void check_qk(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTe
 std::vector<Tensor> qk_forward(const Tensor& q0, const Tensor& k0, const OptTensor& wq, const OptTensor& wk, const Rotation& r, double eps,
                                bool inplace) {
   const c10::cuda::CUDAGuard guard(q0.device());
-  if (inplace) check_inplace(q0, "q"), check_inplace(k0, "k");
+  if (inplace) {
+    check_inplace(q0, "q"), check_inplace(k0, "k");
+    TORCH_CHECK_VALUE(!share_heads(four(q0), four(k0)), "q and k share heads: they cannot be overwritten both");
+  }
   const auto q = channels(q0), k = channels(k0);
   std::vector<Tensor> out = {inplace ? q0 : torch::empty(q.sizes(), q.options()), inplace ? k0 : torch::empty(k.sizes(), k.options())};
   if (q.numel() == 0 && k.numel() == 0) return out;
@@ -324,8 +355,9 @@ class QkNormRotary : public torch::autograd::Function<QkNormRotary> {
 
 std::vector<Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table,
                                    const OptTensor& positions, int64_t offset, const std::string& layout, double eps, bool inplace) {
-  const Rotation r{table, positions, offset, layout, false};
+  Rotation r{table, positions, offset, layout, false};
   check_qk(q, k, wq, wk, r, eps);
+  r.table = aligned_pairs(r.table);
   bool grad = q.requires_grad() || k.requires_grad();
   for (const auto* w : {&wq, &wk}) grad = grad || (*w && (*w)->requires_grad());
   if (!at::GradMode::is_enabled() || !grad) return qk_forward(q, k, wq, wk, r, eps, inplace);
@@ -344,16 +376,18 @@ std::vector<Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTe
 
 std::vector<Tensor> qk_fwd_py(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table,
                               const OptTensor& positions, int64_t offset, const std::string& layout, double eps) {
-  const Rotation r{table, positions, offset, layout, false};
+  Rotation r{table, positions, offset, layout, false};
   check_qk(q, k, wq, wk, r, eps);
+  r.table = aligned_pairs(r.table);
   return qk_forward(q, k, wq, wk, r, eps, false);
 }
 
 void qk_bwd_py(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const OptTensor& table, const OptTensor& positions,
                int64_t offset, const std::string& layout, double eps, const OptTensor& gq, const OptTensor& gk, const OptTensor& dq,
                const OptTensor& dk, const OptTensor& dwq, const OptTensor& dwk, bool add) {
-  const Rotation r{table, positions, offset, layout, false};
+  Rotation r{table, positions, offset, layout, false};
   check_qk(q, k, wq, wk, r, eps);
+  r.table = aligned_pairs(r.table);
   auto or_none = [](const OptTensor& t) { return t ? *t : Tensor(); };
   TORCH_CHECK_VALUE((!gq || dq) && (!gk || dk), "a gradient needs a place");
   qk_backward(q, k, wq, wk, r, eps, or_none(gq), or_none(gk), or_none(dq), or_none(dk), dwq, dwk, add);

@@ -415,6 +415,57 @@ def bench_kv_cache(iters: int = 20, small: bool = False):
                       "gbs": round(2 * 256 * 12 * H * 8200 / ms / 1e6, 1)}), flush=True)
 
 
+def bench_branches(iters: int = 20, small: bool = False):
+    """Attention of branches over the pages that they share (``csrc/kvcache/attend_branches.cu``),
+    together and each alone; bytes of the shared and own codes, products of the visible pairs."""
+    from ._ext import ext
+    from .kv_cache import PagedKVCache
+
+    H = 12
+
+    def case(name, n, ctx, T, **mask):
+        cache = PagedKVCache(1, H, ctx // 64 + 1 + n * (T // 64 + 2), device="cuda")
+        root = cache.add(1)
+        kv, new = ((torch.randn(*shape, H, 64, device="cuda") * 0.5).bfloat16() for shape in ((1, ctx), (n, T)))
+        step = cache.begin(root, ctx)
+        step.write(0, kv, kv)
+        step.commit()
+        kids = cache.fork(root, n)
+        step = cache.begin(kids, T, branches=n)
+        step.write(0, new, new)
+        out = {"kernel": "kv_cache_branches", "case": name, "branches": n, "cached": ctx, "tokens": T}
+        for mode, label in ((0, "ms"), (1, "alone_ms")):
+            before = ext().kv_set_branch_mode(mode)
+            out[label] = round(_timeit(lambda: step.attend(0, new, **mask), iters), 4)
+            ext().kv_set_branch_mode(before)
+        out["cache_gbs"] = round((ctx + n * T) * H * 128 / out["ms"] / 1e6, 1)
+        out["tflops"] = round(4 * 64 * n * T * (ctx + T) * H / out["ms"] / 1e9, 1)
+        print(json.dumps(out), flush=True)
+
+    case("token", 8 if small else 64, 16384, 1, causal="token")
+    case("frame", 8, 12800, 64, causal="frame", tokens_per_frame=64)
+
+
+def bench_rotary(iters: int = 20, small: bool = False):
+    """Rotation, and norms of queries and keys with it, of a DiT-B step's tokens (2 x 8,192, 12 heads
+    of 64; queries, keys and values packed) against the bytes that are read and written."""
+    from ._ext import ext
+    from .rotary import rotary
+
+    B, T, H = (1 if small else 2), 8192, 12
+    a = torch.rand(T, 32, device="cuda") * 6
+    tab = torch.stack([a.cos(), a.sin()], -1).contiguous()
+    q, k, v = torch.randn(B, T, 3, H, 64, device="cuda").bfloat16().unbind(2)
+    w = torch.rand(64, device="cuda")
+    g, out, dw = (torch.randn(B, T, H, 64, device="cuda").bfloat16() for _ in "qk"), [torch.empty(B, T, H, 64, device="cuda", dtype=torch.bfloat16) for _ in "qk"], [torch.empty_like(w) for _ in "qk"]
+    args, g = (q, k, w, w, tab, None, 0, "interleaved", 1e-6), list(g)
+    one = q.numel() * 2
+    for name, ms, moved in (("rotary", _timeit(lambda: rotary(q, tab), iters), 2 * one),
+                            ("qk_norm_rotary_fwd", _timeit(lambda: ext().qk_norm_rotary_fwd(*args), iters), 4 * one),
+                            ("qk_norm_rotary_bwd", _timeit(lambda: ext().qk_norm_rotary_bwd(*args, *g, *out, *dw, False), iters), 6 * one)):
+        print(json.dumps({"kernel": name, "B": B, "T": T, "H": H, "ms": round(ms, 4), "gbs": round(moved / ms / 1e6, 1)}), flush=True)
+
+
 def bench_moe_gemm(iters: int = 10, N: int = 32768, d: int = 1024, E: int = 64, k: int = 6,
                    F: int = 512, ns: int = 2, small: bool = False):
     """Grouped (MoE) SwiGLU and down GEMMs of one MoE-DiT-L layer on one GPU (random
@@ -617,7 +668,7 @@ def bench_optim(iters: int = 10, numel: int = 130_000_000, transport: str = "fus
 
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("what", nargs="*", default=["gemm"], help="gemm attn window_attn kv_attn kv_cache sla_attn sla norm conv3d groupnorm moe_gemm ep optim")
+    p.add_argument("what", nargs="*", default=["gemm"], help="gemm attn window_attn kv_attn kv_cache branches rotary sla_attn sla norm conv3d groupnorm moe_gemm ep optim")
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--small", action="store_true", help="small attention case (for ncu)")
     p.add_argument("--B", type=int, default=8, help="attention batch")
@@ -640,7 +691,7 @@ def main():
             bench_ep(args.iters, transport=args.transport)
         elif w == "optim":
             bench_optim(args.iters, transport=args.transport)
-        elif w in ("groupnorm", "kv_attn", "kv_cache", "moe_gemm", "sla_attn", "window_attn"):
+        elif w in ("branches", "rotary", "groupnorm", "kv_attn", "kv_cache", "moe_gemm", "sla_attn", "window_attn"):
             globals()[f"bench_{w}"](args.iters, small=args.small)
         else:
             globals()[f"bench_{w}"](args.iters)

@@ -255,6 +255,23 @@ def test_positions_outside_the_table_are_recorded():
         reset_device_status()
 
 
+def test_tables_and_weights_off_their_alignment():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    buf, wbuf = torch.rand(1 + 30 * 64, device="cuda"), torch.rand(65, device="cuda")
+    odd, w = buf[1:].view(30, 32, 2), wbuf[1:]
+    x = torch.randn(2, 30, 3, 64, device="cuda").bfloat16().requires_grad_()
+    assert odd.data_ptr() % 8 and w.data_ptr() % 16
+    assert torch.equal(rotary(x, odd), rotary(x, odd.clone()))
+    outs = []
+    for t, v in ((odd, w), (odd.clone(), w.clone())):
+        v = v.detach().requires_grad_()
+        a, b = qk_norm_rotary(x, x, v, None, t)
+        outs.append((a, b, *torch.autograd.grad((a, b), (x, v), (x.detach(), x.detach()))))
+    # another kernel, for other alignments: fp32 sums in another order, then a rounding
+    for a, b in zip(*outs):
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -7, atol=1e-5 * float(b.abs().max()))
+
+
 def test_inplace():
     from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
     for D, layout in ((64, "split"), (64, "half"), (96, "interleaved"), (70, "split"), (256, "split")):
@@ -269,6 +286,17 @@ def test_inplace():
         assert torch.equal(v, before[:, :, 6:]) and packed._version > version
         want = rotary(v, tab, layout=layout)
         assert torch.equal(rotary(v, tab, layout=layout, inplace=True), want) and torch.equal(v, want)
+    x = torch.randn(2, 6, 8, 64, device="cuda")
+    tab = _table(6, 32)
+    for q, k in ((x, x), (x[:, :, :4], x[:, :, 3:]), (x[:, :5], x[:, 1:]), (x[:1], x[:1, :, 2:3]), (x[:, :, ::2], x[:, :, 2::4])):
+        with pytest.raises(ValueError, match="share"):
+            qk_norm_rotary(q, k, table=tab, inplace=True)
+    pair = torch.randn(2, 6, 4, 2, 64, device="cuda")
+    heads = torch.randn(2, 8, 6, 64, device="cuda").transpose(1, 2)
+    for q, k in ((x[:, :, ::2], x[:, :, 1::2]), (pair[..., 0, :], pair[..., 1, :]), (heads[:, :, :5], heads[:, :, 5:]), (x[:1], x[1:])):
+        want = qk_norm_rotary(q.clone(), k.clone(), table=tab)
+        got = qk_norm_rotary(q, k, table=tab, inplace=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     with pytest.raises(ValueError):
         rotary(torch.zeros(1, 4, 2, 8, device="cuda").expand(3, 4, 2, 8), _table(4, 4), inplace=True)
     with pytest.raises(ValueError):
@@ -373,6 +401,18 @@ def test_streams_and_graphs():
         want = both(*(x.detach().clone().requires_grad_() for x in leaves), pos)
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+def test_first_call_of_a_process_captured():
+    """The device's status word is made in the first call, wherever that is."""
+    import subprocess
+    import sys
+    code = ("import torch\nfrom drivedit_b200.ops.rotary import rotary\n"
+            "x, tab, pos = torch.randn(1, 4, 2, 64, device='cuda'), torch.rand(4, 32, 2, device='cuda'), torch.arange(4, device='cuda')\n"
+            "g = torch.cuda.CUDAGraph()\nwith torch.cuda.graph(g):\n    y = rotary(x, tab, pos)\n"
+            "g.replay()\nassert torch.equal(y, rotary(x, tab, pos))\nprint('same')")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
 
 
 def test_capture_refuses_a_living_eager_graph():
