@@ -52,6 +52,9 @@ struct Launch {
   int ctas1 = 0;
   int log_lanes = 0;   // lanes of a head
   int unroll = 1;      // heads of a lane at once
+  // rot_any: pieces of a head, bytes between heads in shared memory, stages
+  Div by_pieces;
+  int piece = 0, pitch = 0, stages = 0, bytes = 0;
   int* status = nullptr;
   int dev = 0;
 };
@@ -62,12 +65,6 @@ template <>
 struct Io<__nv_bfloat16> {
   static __device__ __forceinline__ float get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ void get2(const __nv_bfloat16* p, float& x, float& y) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-    x = __uint_as_float(w << 16);
-    y = __uint_as_float(w & 0xffff0000u);
-  }
-  static __device__ __forceinline__ void put2(__nv_bfloat16* p, float x, float y) { *reinterpret_cast<uint32_t*>(p) = pack_bf16(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
     const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
@@ -84,12 +81,6 @@ template <>
 struct Io<__half> {
   static __device__ __forceinline__ float get(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-  static __device__ __forceinline__ void get2(const __half* p, float& x, float& y) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
-    x = f.x;
-    y = f.y;
-  }
-  static __device__ __forceinline__ void put2(__half* p, float x, float y) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[2], float (&v)[16]) {
     const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
@@ -113,12 +104,6 @@ template <>
 struct Io<float> {
   static __device__ __forceinline__ float get(const float* p) { return *p; }
   static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
-  static __device__ __forceinline__ void get2(const float* p, float& x, float& y) {
-    const float2 f = *reinterpret_cast<const float2*>(p);
-    x = f.x;
-    y = f.y;
-  }
-  static __device__ __forceinline__ void put2(float* p, float x, float y) { *reinterpret_cast<float2*>(p) = make_float2(x, y); }
   static __device__ __forceinline__ void unpack(const uint4 (&u)[4], float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -493,142 +478,186 @@ __global__ void __launch_bounds__(kThreads, 2) rot_wide_back(const Launch L) {
   }
 }
 
-// Heads of any even size up to 256, any strides: 8 lanes (16 above 128 channels) a head, up to 8
-// pairs a lane, U heads of one token. IN2, OUT2: on that side pairs lie side by side and a pair's two
-// channels are one access.
-template <typename T, bool NORM, bool BWD, bool IN2, bool OUT2>
+// Heads of any even size up to 256, any strides: through shared memory, where a warp brings whole
+// heads by the widest copies that their sizes and addresses allow some turns ahead, and takes their
+// pairs apart: 8 lanes (16 above 128 channels) a head, up to 8 pairs a lane. Straight to registers, a
+// channel at a time, too few bytes were on their way (16,384 tokens of 24 heads of 72: 137 us). A
+// lane's places in a head, and the weights there, do not change; lanes without a pair have a place
+// of zeros behind the head to read and another to write.
+constexpr int kPasses = 2;  // turns of a warp's lanes over the heads of a stage
+template <typename T, bool IN_H, bool OUT_H, bool NORM, bool BWD>
 __global__ void __launch_bounds__(kThreads, 2) rot_any(const Launch L) {
-  constexpr int U = BWD ? 1 : 2, NP = 8;
+  extern __shared__ __align__(16) uint8_t heads[];  // [warp][stage][x, g][head]
+  constexpr int NP = 8;
   const RotArgs& a = L.a;
   const int which = blockIdx.x >= L.ctas0;
   const RotTensor& t = a.t[which];
-  const int lg = L.log_lanes, l = threadIdx.x & ((1 << lg) - 1);
-  const int blocks = L.heads[which];
-  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * blocks, per = kThreads >> lg;
-  const int pairs = a.D / 2, turned = a.R / 2;
-  // Channels of a lane's pair as one side has them. The lanes that have a pair i, if any:
-  auto have = [&](int i) { return l + (i << lg) < pairs; };
-  auto chan = [&](int i, bool halves, int& c0, int& c1) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = L.log_lanes, l = lane & ((1 << lg) - 1);
+  const int batch = kPasses * (32 >> lg), S = L.stages;
+  const uint32_t n = static_cast<uint32_t>(a.B) * a.T * t.H;
+  const int pairs = a.D / 2, turned = a.R / 2, slots = (pairs + (1 << lg) - 1) >> lg;
+  const int pitch = L.pitch, tensor = batch * pitch, stage_bytes = (BWD ? 2 : 1) * tensor;
+  const int bytes = a.D * static_cast<int>(sizeof(T)), piece = L.piece, pieces = bytes / piece;
+  const int spare = pitch - 16;  // zeros, then what nobody reads (4 and 4 channels, or 2 and 2)
+  uint8_t* mine = heads + warp * S * stage_bytes;
+  // A lane's pair i in a head, as one side has it: bytes to its channels
+  auto chan = [&](int i, bool halves, bool write, int& c0, int& c1) {
     const int p = l + (i << lg);
-    if (p < turned && halves) c0 = p, c1 = p + turned;
-    else c0 = 2 * p, c1 = 2 * p + 1;
-  };
-  auto load = [&](const T* p, int i, bool halves, auto two, float& x, float& y) {
-    int c0, c1;
-    if constexpr (decltype(two)::value) {
-      Io<T>::get2(p + 2 * (l + (i << lg)), x, y);
-    } else {
-      chan(i, halves, c0, c1);
-      x = Io<T>::get(p + c0), y = Io<T>::get(p + c1);
-    }
+    const bool half = halves && p < turned;
+    c0 = (half ? p : 2 * p) * static_cast<int>(sizeof(T));
+    c1 = c0 + (half ? turned : 1) * static_cast<int>(sizeof(T));
+    if (p >= pairs) c0 = spare + (write ? 8 : 0), c1 = c0 + static_cast<int>(sizeof(T));
   };
   const float inv_D = 1.f / static_cast<float>(a.D);
-  float2 dw[NP];
+  float2 w[NP], dw[NP];
 #pragma unroll
-  for (int i = 0; i < NP; ++i) dw[i] = both(0.f);
-  const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), step = (which ? L.ctas1 : L.ctas0) * per;
-  for (uint32_t i0 = cta * per; i0 < n; i0 += step) {
-    const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
-    const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
-    const T* pg = reinterpret_cast<const T*>(t.g) + it.b * t.g_sb + it.t * t.g_st;
-    T* py = reinterpret_cast<T*>(t.y) + it.b * t.y_sb + it.t * t.y_st;
-    float2 v[U][NP], g[BWD ? U : 1][NP], cs[NP];
+  for (int i = 0; i < NP; ++i) {
+    dw[i] = both(0.f);
+    w[i] = both(1.f);
+    const int p = l + (i << lg);
+    if (NORM && t.w && p < pairs) {
+      const int c0 = IN_H && p < turned ? p : 2 * p;
+      w[i] = make_float2(t.w[c0], t.w[c0 + (IN_H && p < turned ? turned : 1)]);
+    }
+  }
+  for (int i = lane; i < S * stage_bytes / pitch; i += 32) *reinterpret_cast<uint4*>(mine + i * pitch + spare) = make_uint4(0, 0, 0, 0);
+  const uint32_t first = ((blockIdx.x - (which ? L.ctas0 : 0)) * (kThreads / 32) + warp) * batch;
+  const uint32_t step = (which ? L.ctas1 : L.ctas0) * (kThreads / 32) * batch;
+  // f(bytes to the tensor's piece, and to its place in the stage) for every piece of the batch's heads, of
+  // which lane k has the offset of head k
+  auto each_piece = [&](long offset, int count, auto&& f) {
+    const int all = count * pieces;
+    for (int i = lane; i < ((all + 31) & ~31); i += 32) {
+      const int k = min(static_cast<int>(L.by_pieces(i)), count - 1), at = (i - k * pieces) * piece;
+      const long from = __shfl_sync(0xffffffffu, offset, k);
+      if (i < all) f(from + at, k * pitch + at);
+    }
+  };
+  auto count_of = [&](uint32_t i0) { return static_cast<int>(min(static_cast<uint32_t>(batch), n - i0)); };
+  auto fetch = [&](uint32_t i0, int stage) {
+    if (i0 < n) {
+      const int count = count_of(i0);
+      const Item it = item_of(L, which, i0 + min(lane, count - 1), n);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = it.h + u * blocks;
+      for (int k = 0; k < (BWD ? 2 : 1); ++k) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(k ? t.g : t.x);
+        const long offset = k ? it.b * t.g_sb + it.t * t.g_st + it.h * t.g_sh : it.b * t.x_sb + it.t * t.x_st + it.h * t.x_sh;
+        uint8_t* to = mine + stage * stage_bytes + k * tensor;
+        const uint32_t dst = smem_u32(to);
+        each_piece(offset * static_cast<long>(sizeof(T)), count, [&](long at, int place) {
+          if (piece == 16) copy16(dst + place, from + at, true);
+          else if (piece == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + place), "l"(from + at) : "memory");
+          else if (piece == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + place), "l"(from + at) : "memory");
+          else *reinterpret_cast<uint16_t*>(to + place) = *reinterpret_cast<const uint16_t*>(from + at);
+        });
+      }
+    }
+    copies_end();
+  };
+  for (int k = 0; k < S - 1; ++k) fetch(first + k * step, k);
+  int stage = 0;
+  for (uint32_t i0 = first; i0 < n; i0 += step, stage = stage == S - 1 ? 0 : stage + 1) {
+    const int count = count_of(i0);
+    const Item it = item_of(L, which, i0 + min(lane, count - 1), n);  // of head `lane`
+    if (S == 3) copies_wait<1>();
+    else copies_wait<0>();
+    __syncwarp();
+    fetch(i0 + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+    uint8_t* base = mine + stage * stage_bytes;
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int k = pass * (32 >> lg) + (lane >> lg);
+      const int row = __shfl_sync(0xffffffffu, it.row, min(k, count - 1));
+      uint8_t* px = base + k * pitch;
+      const uint8_t* pg = px + tensor;
+      const float2* tab = a.table + static_cast<long>(max(row, 0)) * turned + l;
+      float2 v[NP], z[NP], cs[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        v[u][i] = both(0.f);
-        if (BWD) g[u][i] = both(0.f);
-        if (i << lg >= pairs) continue;  // for all lanes
-        if (!have(i) || !it.there || h >= t.H) continue;
-        load(px + h * t.x_sh, i, a.layout.in_halves, std::bool_constant<IN2>{}, v[u][i].x, v[u][i].y);
-        if (BWD) load(pg + h * t.g_sh, i, a.layout.out_halves, std::bool_constant<OUT2>{}, g[u][i].x, g[u][i].y);
+        v[i] = z[i] = both(0.f);
+        cs[i] = make_float2(1.f, 0.f);
+        if (i >= slots) continue;  // for all lanes
+        int c0, c1;
+        chan(i, IN_H, false, c0, c1);
+        v[i] = make_float2(Io<T>::get(reinterpret_cast<const T*>(px + c0)), Io<T>::get(reinterpret_cast<const T*>(px + c1)));
+        if (BWD) {
+          if (IN_H != OUT_H) chan(i, OUT_H, false, c0, c1);
+          z[i] = make_float2(Io<T>::get(reinterpret_cast<const T*>(pg + c0)), Io<T>::get(reinterpret_cast<const T*>(pg + c1)));
+        }
+        if (l + (i << lg) < turned) cs[i] = __ldg(tab + (i << lg));
       }
-    }
+      if (__any_sync(0xffffffffu, row < 0) && row < 0) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      cs[i] = make_float2(1.f, 0.f);
-      const int p = l + (i << lg);
-      if (p < turned && it.there) {
-        const float2 f = __ldg(a.table + static_cast<long>(max(it.row, 0)) * turned + p);
-        cs[i] = make_float2(it.row < 0 ? NAN : f.x, a.inverse != BWD ? -f.y : f.y);
+        for (int i = 0; i < NP; ++i)
+          if (l + (i << lg) < turned) cs[i].x = NAN;
       }
-    }
-    __syncwarp();  // every lane has read what another one may write (a result in the place of its input)
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = it.h + u * blocks;
       float r = 1.f, down = 1.f;
       auto dot = [&](const float2 (&x)[NP], const float2 (&y)[NP]) {
         float2 s = mul2(x[0], y[0]);
 #pragma unroll
-        for (int i = 1; i < NP; ++i) s = fma2(x[i], y[i], s);
-        float z = s.x + s.y;
-        for (int o = 1; o < 1 << lg; o *= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
-        return z;
+        for (int i = 1; i < NP; ++i)
+          if (i < slots) s = fma2(x[i], y[i], s);
+        float q = s.x + s.y;
+        for (int o = 1; o < 1 << lg; o *= 2) q += __shfl_xor_sync(0xffffffffu, q, o);
+        return q;
       };
       if (NORM) {
-        float s = dot(v[u], v[u]);
+        float s = dot(v, v);
         if (__any_sync(0xffffffffu, !(s < 1e38f))) {
           if (!(s < 1e38f)) down = kDown;
 #pragma unroll
-          for (int i = 0; i < NP; ++i) v[u][i] = mul2(v[u][i], both(down));
-          s = dot(v[u], v[u]);
+          for (int i = 0; i < NP; ++i) v[i] = mul2(v[i], both(down));
+          s = dot(v, v);
         }
         r = rms_inv_fast(s, inv_D, a.eps * down * down);
       }
-      float2 z[NP];
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        z[i] = BWD ? g[u][i] : v[u][i];
-        if (i << lg >= pairs) continue;
-        float2 w = both(1.f);
-        if (NORM && t.w && have(i)) {
-          int c0, c1;
-          chan(i, a.layout.in_halves, c0, c1);
-          w = make_float2(__ldg(t.w + c0), __ldg(t.w + c1));
-        }
-        if (NORM && !BWD) z[i] = mul2(z[i], w);
-        if (l + (i << lg) < turned) z[i] = turn(z[i].x, z[i].y, cs[i].x, cs[i].y);
+        if (!BWD) z[i] = v[i];
+        if (i >= slots) continue;
+        if (NORM && !BWD) z[i] = mul2(z[i], w[i]);
+        const float sn = a.inverse != BWD ? -cs[i].y : cs[i].y;
+        if (l + (i << lg) < turned) z[i] = turn(z[i].x, z[i].y, cs[i].x, sn);
         if (NORM) z[i] = mul2(z[i], both(r));
         if (BWD) {  // gr = g r; dw += gr x; gr w
-          dw[i] = fma2(z[i], v[u][i], dw[i]);
-          z[i] = mul2(z[i], w);
+          if (k < count) dw[i] = fma2(z[i], v[i], dw[i]);
+          z[i] = mul2(z[i], w[i]);
         }
       }
       if (BWD) {  // dx = gr w - x r^2 mean(gr w x)
-        const float2 k = both(-dot(z, v[u]) * inv_D * r * r);
+        const float2 q = both(-dot(z, v) * inv_D * r * r);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) z[i] = mul2(fma2(v[u][i], k, z[i]), both(down));
+        for (int i = 0; i < NP; ++i) z[i] = mul2(fma2(v[i], q, z[i]), both(down));
       }
-      T* y = py + h * t.y_sh;
+      __syncwarp();  // the head's channels have been read
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        if (i << lg >= pairs) continue;
-        if (!have(i) || !it.there || h >= t.H) continue;
-        if constexpr (BWD ? IN2 : OUT2) {
-          Io<T>::put2(y + 2 * (l + (i << lg)), z[i].x, z[i].y);
-        } else {
-          int c0, c1;
-          chan(i, BWD ? a.layout.in_halves : a.layout.out_halves, c0, c1);
-          Io<T>::put(y + c0, z[i].x);
-          Io<T>::put(y + c1, z[i].y);
-        }
+        if (i >= slots) continue;
+        int c0, c1;
+        chan(i, BWD ? IN_H : OUT_H, true, c0, c1);
+        Io<T>::put(reinterpret_cast<T*>(px + c0), z[i].x);
+        Io<T>::put(reinterpret_cast<T*>(px + c1), z[i].y);
       }
     }
+    __syncwarp();
+    uint8_t* to = reinterpret_cast<uint8_t*>(t.y);
+    each_piece((it.b * t.y_sb + it.t * t.y_st + it.h * t.y_sh) * static_cast<long>(sizeof(T)), count, [&](long at, int place) {
+      if (piece == 16) *reinterpret_cast<uint4*>(to + at) = *reinterpret_cast<const uint4*>(base + place);
+      else if (piece == 8) *reinterpret_cast<uint2*>(to + at) = *reinterpret_cast<const uint2*>(base + place);
+      else if (piece == 4) *reinterpret_cast<uint32_t*>(to + at) = *reinterpret_cast<const uint32_t*>(base + place);
+      else *reinterpret_cast<uint16_t*>(to + at) = *reinterpret_cast<const uint16_t*>(base + place);
+    });
+    __syncwarp();  // before the next copies into this stage
   }
   if (BWD) {
     __shared__ float red[kThreads / 32][256];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      int c0, c1;
-      chan(i, a.layout.in_halves, c0, c1);
+      const int p = l + (i << lg), c0 = IN_H && p < turned ? p : 2 * p, c1 = c0 + (IN_H && p < turned ? turned : 1);
       for (int o = 1 << lg; o < 32; o *= 2) {
         dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
         dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
       }
-      if ((threadIdx.x & 31) == l && have(i)) red[threadIdx.x >> 5][c0] = dw[i].x, red[threadIdx.x >> 5][c1] = dw[i].y;
+      if (lane == l && p < pairs) red[warp][c0] = dw[i].x, red[warp][c1] = dw[i].y;
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.D; c += kThreads) {
@@ -684,6 +713,8 @@ bool wide(const RotArgs& a, bool bwd) {
   return aligned(a, bwd, 16);
 }
 
+constexpr int kMaxBytes = 216 * 1024;  // of shared memory beside 9 KB for the sums of a backward
+
 int log2_up(int n) {
   int lg = 0;
   while (1 << lg < n) ++lg;
@@ -708,7 +739,17 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
     }
   };
   if (!is_wide) {
-    count(bwd ? 1 : 2);
+    count(1);
+    const int bytes = a.D * size_of(a.type), batch = kPasses * (32 >> L.log_lanes);
+    L.piece = 16;
+    while (L.piece > 2 && (bytes % L.piece || !aligned(a, bwd, L.piece))) L.piece /= 2;
+    L.by_pieces = Div(bytes / L.piece);
+    L.pitch = (bytes + 15) / 16 * 16 + 16;  // a lane without a pair reads and writes behind the head
+    const long stage = static_cast<long>(kThreads / 32) * (bwd ? 2 : 1) * batch * L.pitch;
+    L.stages = 3 * stage <= 100 * 1024 ? 3 : 2;
+    L.bytes = static_cast<int>(L.stages * stage);
+    const long heads = kThreads / 32 * batch;  // of a CTA's turn
+    for (int i = 0; i < a.n; ++i) need[i] = (static_cast<long>(a.B) * a.T * a.t[i].H + heads - 1) / heads;
   } else if (bwd) {
     count(a.type == RotType::kF32 ? 1 : 2);  // (more spill registers)
   } else {
@@ -729,25 +770,25 @@ Launch plan(const RotArgs& a, bool bwd, bool is_wide, int dev) {
   return L;
 }
 
-template <auto kernel, int BYTES>
-void launch_ring(const Launch& L, cudaStream_t s) {
-  static_assert(2 * (BYTES + 1024) <= 233472, "two CTAs an SM");
+template <auto kernel>
+void launch_ring(const Launch& L, int bytes, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
   if (!(set.load() >> (L.dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES), "cudaFuncSetAttribute(rot_wide)");
+    check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBytes), "cudaFuncSetAttribute(rotary)");
     set.fetch_or(1ull << (L.dev & 63));
   }
-  kernel<<<L.ctas0 + L.ctas1, kThreads, BYTES, s>>>(L);
+  kernel<<<L.ctas0 + L.ctas1, kThreads, bytes, s>>>(L);
 }
 
 template <typename T, bool NORM, int U>
 void launch_wide(const Launch& L, cudaStream_t s) {
   const bool ih = L.a.layout.in_halves, oh = L.a.layout.out_halves;
   constexpr int kBytes = kStages<T, U> * kPlaces<T, U> * kThreads * 16;
-  if (!ih && !oh) launch_ring<rot_wide<T, false, false, NORM, U>, kBytes>(L, s);
-  else if (ih && oh) launch_ring<rot_wide<T, true, true, NORM, U>, kBytes>(L, s);
-  else if (oh) launch_ring<rot_wide<T, false, true, NORM, U>, kBytes>(L, s);
-  else if constexpr (!NORM) launch_ring<rot_wide<T, true, false, NORM, U>, kBytes>(L, s);
+  static_assert(2 * (kBytes + 1024) <= 233472, "two CTAs an SM");
+  if (!ih && !oh) launch_ring<rot_wide<T, false, false, NORM, U>>(L, kBytes, s);
+  else if (ih && oh) launch_ring<rot_wide<T, true, true, NORM, U>>(L, kBytes, s);
+  else if (oh) launch_ring<rot_wide<T, false, true, NORM, U>>(L, kBytes, s);
+  else if constexpr (!NORM) launch_ring<rot_wide<T, true, false, NORM, U>>(L, kBytes, s);
   else throw std::runtime_error("rotary: a norm is not behind an inverse rotation");
 }
 
@@ -762,12 +803,11 @@ void launch_back(const Launch& L, cudaStream_t s) {
 
 template <typename T, bool NORM, bool BWD>
 void launch_any(const Launch& L, cudaStream_t s) {
-  const bool two = aligned(L.a, BWD, 2 * sizeof(T)), in2 = two && !L.a.layout.in_halves, out2 = two && !L.a.layout.out_halves;
-  const int grid = L.ctas0 + L.ctas1;
-  if (in2 && out2) rot_any<T, NORM, BWD, true, true><<<grid, kThreads, 0, s>>>(L);
-  else if (in2) rot_any<T, NORM, BWD, true, false><<<grid, kThreads, 0, s>>>(L);
-  else if (!NORM && out2) rot_any<T, NORM, BWD, false, !NORM><<<grid, kThreads, 0, s>>>(L);
-  else rot_any<T, NORM, BWD, false, false><<<grid, kThreads, 0, s>>>(L);
+  const bool ih = L.a.layout.in_halves, oh = L.a.layout.out_halves;
+  if (!ih && !oh) launch_ring<rot_any<T, false, false, NORM, BWD>>(L, L.bytes, s);
+  else if (ih && oh) launch_ring<rot_any<T, true, true, NORM, BWD>>(L, L.bytes, s);
+  else if (oh) launch_ring<rot_any<T, false, true, NORM, BWD>>(L, L.bytes, s);
+  else if constexpr (!NORM) launch_ring<rot_any<T, true, false, NORM, BWD>>(L, L.bytes, s);
 }
 
 template <typename T, bool NORM, bool BWD>
