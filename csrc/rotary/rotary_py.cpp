@@ -227,7 +227,7 @@ Tensor rotary(const Tensor& x, const Tensor& table, const OptTensor& positions, 
 
 // ---------------------------------------------------------------- norms of queries and keys, rotated
 OptTensor weight32(const OptTensor& w) {
-  if (!w) return w;
+  if (!w || (w->scalar_type() == torch::kFloat && w->is_contiguous())) return w;
   return w->detach().to(torch::kFloat).contiguous();
 }
 

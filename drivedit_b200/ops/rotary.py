@@ -165,8 +165,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     (``table`` None: not at all). One launch for both, differentiable in the heads and weights; the
     weights' gradients are summed in a fixed order. A second derivative raises on CUDA."""
     if q.is_cuda:
-        grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
-        if sync_check() and grad and not inplace:
+        if sync_check() and not inplace and torch.is_grad_enabled() and \
+                any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
             return _SyncChecked.apply(q, k, q_weight, k_weight, table, positions, offset, layout, eps)
         return tuple(ext().qk_norm_rotary(q, k, q_weight, k_weight, table, positions, offset, layout, eps, inplace))
     _check(q, "q"), _check(k, "k")
