@@ -14,6 +14,11 @@
 // 16x8x16 instruction), two numbers to an fp32 instruction. The keys of the warp's next two
 // pages and the values of its next one are on their way while it works: 16 warps with
 // two whole pages each do not fit the shared memory.
+// Measured: 64 branches of 16,384 tokens, up to 700 of their own, 16 heads: 48 us and 6 for the sum
+// (each for itself 275), 855 instructions a page, 2 a cycle: issue and latency of 16 warps, DRAM
+// at 0.27 of a copy's rate. Eight branches of 200 frames of 64 tokens, 12 heads, in 256-row blocks: 56 us
+// and 10 (131). A launch of its own for the sequences' own pages: 54 and 63 us in all for these
+// two, where a list of both kinds takes 49 and 53.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -6,15 +6,16 @@
 //              dx = r (u - h mean(u h))
 // r is made again from x in the backward: nothing but x is kept between the two.
 //
-// Bound by memory: every value is read and written once. Wide heads (rot_wide): 16 channels
-// to a lane, as two runs of 8 that hold 8 whole pairs in either layout, so that a pair never
-// leaves its lane and both layouts take 16-byte accesses; D / 16 lanes make a head, its sum of
-// squares is a shuffle over them. A lane's pairs are 8 l .. 8 l + 7 in every layout, so its
-// 64 bytes of the table are contiguous; the heads of a token find them in L1. Heads whose
-// sizes, strides or bases do not allow that (rot_any): 8 or 16 lanes a head, a channel pair at
-// a time.
-// Everything is fp32 inside, without contraction of a c - b s (the same bits as the PyTorch
-// statement of the rotation), rounded once.
+// Every value is read and written once. Wide heads (rot_wide): 16 channels to a lane, as two runs
+// of 8 that hold 8 whole pairs in either layout, so that a pair never leaves its lane and both
+// layouts take 16-byte accesses; D / 16 lanes make a head, its sum of squares is a shuffle over
+// them. Heads whose sizes, strides or bases do not allow that (rot_any) go through shared memory.
+// Everything is fp32 inside and rounded once; the plain rotation without contraction of a c - b s
+// (the same bits as the PyTorch statement).
+// Measured (cold caches): rotation of 32,768 tokens of 8 heads of 128, half of each, 22.7 us for
+// 139 MB, 0.93 of a plain copy's rate. Norms and rotation of 16,384 tokens of 24 heads of 64 (101
+// MB) 23.5 us, 0.65 of it: instruction issue and the latency of 16 warps an SM; backward (151 MB)
+// 37.6 us, 0.61, and 5 us for the weights' gradients. 3,009 tokens of 5 heads of 72, fp32: 7.8 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -376,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 2) rot_wide(const Launch L) {
 }
 
 // The backward. Loads go straight to registers: copies ahead of the work, as above, need the
-// shared memory of x and g and were slower here (52 and 46 us of a dit_b step's 16,384 tokens of 12 and 12 heads).
+// shared memory of x and g and were slower here (52 and 46 us of a call with 16,384 tokens of 12 and 12
+// heads of 64; one head at a time 58).
 template <typename T, bool IN_H, bool OUT_H, int U>
 __global__ void __launch_bounds__(kThreads, 2) rot_wide_back(const Launch L) {
   constexpr bool kMixed = IN_H != OUT_H;
