@@ -49,6 +49,51 @@ static_assert(OFF_PAGES % 16 == 0 && OFF_BRANCH % 16 == 0 && OFF_ROWS % 16 == 0 
 static_assert(16 * (kPitch * 4 + 8) <= kRing, "a warp's results fit its ring");
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 
+// Which of a lane's sums of a page meet a value that is NaN in a token that their row sees: bit
+// 8 t + 4 j + k for the sum k of channels t and rows j. By a product of ones where a value is NaN
+// and ones where a row sees a token; the page's NaN become zeros behind it. Out of line, for it is hardly
+// ever called. `br` -2: no page.
+template <int NJ>
+__device__ __noinline__ uint32_t nan_sums(uint32_t sv, const int4* spans, int br, int key0) {
+  const int lane = lane_id(), g = lane >> 2, c = lane & 3, krow = 16 * (g >> 1) + (g & 1);
+  auto ones = [](uint32_t two) { return (two & 0xff ? 0x3c00u : 0u) | (two & 0xff00 ? 0x3c000000u : 0u); };
+  uint32_t bad = 0;
+  for (int j = 0; j < NJ; ++j) {
+    uint32_t see[2], sees[4][2];
+    for (int u = 0; u < 2; ++u) {
+      const int4 span = spans[j * 8 + 2 * c + u];
+      see[u] = br == -1 || br == span.w ? static_cast<uint32_t>(kv_bits(KvSpan{span.x, span.y}, span.z, key0) >> krow) : 0u;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        sees[t][k] = transpose8x8((see[0] >> (4 * t + 2 * k) & 1 ? 0x3c00u : 0u) | (see[1] >> (4 * t + 2 * k) & 1 ? 0x3c000000u : 0u));
+    for (int t = 0; t < 4; ++t) {
+      const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
+      const uint32_t x0[4] = {nan_bytes(w0.x), nan_bytes(w0.y), nan_bytes(w0.z), nan_bytes(w0.w)};
+      const uint32_t x1[4] = {nan_bytes(w1.x), nan_bytes(w1.y), nan_bytes(w1.z), nan_bytes(w1.w)};
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t av[4] = {ones(x0[k]), ones(x1[k]), ones(x0[k] >> 16), ones(x1[k] >> 16)};
+        mma_f16(d, av, sees[k][0], sees[k][1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (d[k] > 0.f) bad |= 1u << (8 * t + 4 * j + k);
+    }
+  }
+  __syncwarp();
+  for (int t = 0; t < 8; ++t) {
+    const uint32_t at = sv + (t * 8 + g) * 64 + c * 16;
+    const uint4 v = lds128(at);
+    st_shared_v4(at, v.x & ~nan_bytes(v.x), v.y & ~nan_bytes(v.y), v.z & ~nan_bytes(v.z), v.w & ~nan_bytes(v.w));
+  }
+  __syncwarp();
+  return bad;
+}
+
 template <int NJ>
 __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArgs a, int row_tiles, int* status) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -287,6 +332,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
     }
     const float vf = f.y * exp2f(-kHeadroom);
     if (!__all_sync(0xffffffffu, mbar_wait(v_full, i & 1, abort_flag))) return false;
+    // A value that is NaN makes NaN of the rows that see its token, and of no other (whose weight for it is
+    // zero, and zero times NaN is NaN): it is taken out of the page, and nan_sums finds those rows.
+    uint32_t bad = 0;
+    if constexpr (kMasked) {
+      uint32_t found = 0;  // a byte's top bit where it is NaN
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const uint4 v = lds128(sv + (t * 8 + g) * 64 + c * 16);
+        found |= ((v.x & 0x7f7f7f7fu) + 0x01010101u) & keep[0];
+        found |= ((v.y & 0x7f7f7f7fu) + 0x01010101u) & keep[1];
+        found |= ((v.z & 0x7f7f7f7fu) + 0x01010101u) & keep[2];
+        found |= ((v.w & 0x7f7f7f7fu) + 0x01010101u) & keep[3];
+      }
+      if (__any_sync(0xffffffffu, (found & 0x80808080u) != 0)) bad = nan_sums<NJ>(sv, spans, there ? br : -2, key0);
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint4 w0 = lds128(sv + (t * 16 + g) * 64 + c * 16), w1 = lds128(sv + (t * 16 + 8 + g) * 64 + c * 16);
@@ -309,6 +369,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
           o[j][t][k] = x.x;
           o[j][t][k + 1] = x.y;
         }
+    }
+    if constexpr (kMasked) {
+      if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll
+        for (int i = 0; i < NJ * 16; ++i)
+          if (bad >> (8 * (i & 3) + 4 * (i >> 4) + (i >> 2 & 3)) & 1) o[i >> 4][i & 3][i >> 2 & 3] = NAN;
+      }
     }
     return true;
     };

@@ -66,7 +66,12 @@ constexpr int OFF_MISC = OFF_META + (NR + 1) / 2 * 8;
 // GROUP: first key and sequence of both pages, per stage of factors and of codes; the sequences
 constexpr int OFF_WHERE = (OFF_MISC + 16 + 15) / 16 * 16;
 constexpr int OFF_TABLE = OFF_WHERE + (NF + NR) * 16;
-constexpr int GROUP_BYTES = OFF_TABLE + kRows * 16;
+// Pairs that hold a NaN value in a page that some row does not see whole, a bit each (of pair j % NN)
+constexpr int NN = 4096;
+constexpr int OFF_NAN = OFF_TABLE + kRows * 16;
+constexpr int OFF_WORK = OFF_NAN + NN / 8 + 16;
+constexpr int kWorkBytes = 64;
+constexpr int GROUP_BYTES = OFF_WORK + kWorkBytes;
 static_assert(GROUP_BYTES <= 232448, "shared memory per CTA");
 static_assert(NF > NR + NS && (NF & (NF - 1)) == 0, "stages of page factors");
 constexpr int SMEM_BYTES = OFF_MISC + 16;
@@ -99,15 +104,50 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// the NaN codes of a word of four: their bytes all ones
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 __device__ __forceinline__ float log2_of_power(float p) { return static_cast<float>((__float_as_int(p) >> 23) - 127); }
 // every warp has its role's registers
 __device__ __forceinline__ void registers_split() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+// What a CTA of a group's block walks, for nan_channels
+struct GroupWork {
+  KvGroupPages list;
+  int group, head, rank, pairs;
+};
+static_assert(sizeof(GroupWork) <= kWorkBytes, "its place");
+
+// The channels in which some token that row r sees is NaN, of the pairs noted. Out of line and from
+// shared memory, for it is hardly ever called: what it needs would cost the softmax registers.
+__device__ __noinline__ uint64_t nan_channels(const KvAttendArgs& a, uint8_t* smem, int r) {
+  const GroupWork work = *reinterpret_cast<const GroupWork*>(smem + OFF_WORK);
+  const KvBranch* table = reinterpret_cast<const KvBranch*>(smem + OFF_TABLE);
+  const uint32_t* nan_pairs = reinterpret_cast<const uint32_t*>(smem + OFF_NAN);
+  const KvGroup grp(a, work.group);
+  const KvGroupRow row = grp.row(r);
+  uint64_t channels = 0;
+  for (int j = 0; j < work.pairs; ++j) {
+    if (!(nan_pairs[j % NN / 32] >> j % 32 & 1)) continue;
+    const int i0 = 2 * (work.rank + j * a.ranks);
+    for (int i = i0; i < min(work.list.n, i0 + 2); ++i) {
+      int page, br, id;
+      work.list.at(grp, table, i, page, br, id);
+      if ((br >= 0 && br != row.i - work.list.first) || static_cast<unsigned>(id) >= static_cast<unsigned>(a.pool.pages)) continue;
+      const uint32_t* values = reinterpret_cast<const uint32_t*>(a.pool.v + (static_cast<long>(id) * a.pool.heads + work.head) * 4096);
+      const uint64_t see = kv_bits(row.span, row.sinks, page * kKvPage);
+      for (int c = 0; c < 64; ++c)
+        for (int k = 0; k < 16; ++k)
+          if (nan_bytes(values[c * 16 + k]) & kv_bytes(static_cast<uint32_t>(see >> 4 * k))) channels |= 1ull << c;
+    }
+  }
+  return channels;
+}
 
 // GROUP: rows of all sequences of a group, over the pages that it shares and then their own (attend.h);
 // every CTA leaves its part in scratch.
 template <bool GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
-    kv_attend_tiles(const KvAttendArgs a, int row_tiles, int* status) {
+    kv_attend_tiles(const __grid_constant__ KvAttendArgs a, int row_tiles, int* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023) != 0) {  // uniform over the grid
     if (threadIdx.x == 0 && status) atomicCAS(status, 0, kStatusBadArgument);
@@ -152,6 +192,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n_t = rows - r0 > 128 ? 2 : 1;
   int4* where = reinterpret_cast<int4*>(smem + OFF_WHERE);  // [NF], then [NR]
   KvBranch* table = reinterpret_cast<KvBranch*>(smem + OFF_TABLE);
+  uint32_t* nan_pairs = reinterpret_cast<uint32_t*>(smem + OFF_NAN);  // NN / 32, then whether there is any
+  if (GROUP)
+    for (int i = threadIdx.x; i <= NN / 32; i += kThreads) nan_pairs[i] = 0;
 
   // the block's pages, and this CTA's run of key tiles (page pairs)
   KvPages pages{0, 0, 0};
@@ -167,8 +210,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     pages = kv_pages(s0.lo, s1.hi, sinks, a.step.width);
   }
   const int pairs = (pages.n + 1) / 2, per = (pairs + ranks - 1) / ranks;
-  const int j0 = min(pairs, rank * per), n = min(pairs, j0 + per) - j0;
+  const int j0 = min(pairs, rank * per);
+  // GROUP: pairs in turn, since those of the sequences' own pages, at the end, take longer
+  const int n = GROUP ? max(0, (pairs - rank + ranks - 1) / ranks) : min(pairs, j0 + per) - j0;
+  auto pair_at = [&](int j) { return GROUP ? rank + j * ranks : j0 + j; };
 
+  if (GROUP && threadIdx.x == 0) *reinterpret_cast<GroupWork*>(smem + OFF_WORK) = GroupWork{list, b, kh, rank, n};
   if (threadIdx.x == 0) {
     mbar_init(q_full, 8);
     for (int s = 0; s < NR; ++s) {
@@ -204,7 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   {
     int most = 0;
-    for (int i = 2 * j0 + threadIdx.x; i < min(pages.n, 2 * (j0 + n)); i += kThreads) {
+    for (int k = threadIdx.x; k < 2 * n; k += kThreads) {
+      const int i = 2 * pair_at(k >> 1) + (k & 1);
+      if (i >= pages.n) break;
       int id, page, branch;
       if (GROUP) list.at(grp, table, i, page, branch, id);
       else id = row[kKvInfo + pages.at(i)];
@@ -229,15 +278,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       float ks = 0.f, vs = 0.f;
       for (int j = 0; j < n; ++j) {
         if ((j & 15) == 0) {  // the next 16 pairs, one page a lane
-          const int i = 2 * (j0 + j) + lane;
+          const int i = j + (lane >> 1) < n ? 2 * pair_at(j + (lane >> 1)) + (lane & 1) : pages.n;
           if (GROUP) {
             ids = -2, key = 0x40000000, branch = -1;  // no page: no key
-            if (i < min(pages.n, 2 * (j0 + n))) {
+            if (i < pages.n) {
               list.at(grp, table, i, key, branch, ids);
               key *= kKvPage;
             }
           } else {
-            ids = i < min(pages.n, 2 * (j0 + n)) ? row[kKvInfo + pages.at(i)] : -2;
+            ids = i < pages.n ? row[kKvInfo + pages.at(i)] : -2;
           }
           if (ids != -2 && static_cast<unsigned>(ids) >= static_cast<unsigned>(a.pool.pages)) {
             // recorded, read as zeros (no sequence sees a shared page that none has)
@@ -364,11 +413,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x - 128;
     const int r = t >> 2, c = t & 3;  // row of 32, 16-byte piece of it; then rows r + 32 i
     bool ok = true;
-    auto convert = [&](const uint8_t* raw, uint32_t dst, const uint32_t (&keep)[2][4]) {
+    auto convert = [&](const uint8_t* raw, uint32_t dst, const uint32_t (&keep)[2][4], auto nan_out, uint32_t no_nan) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 w = *reinterpret_cast<const uint4*>(raw + t * 16 + i * 2048);
-        const uint32_t ws[4] = {w.x & keep[i >> 1][0], w.y & keep[i >> 1][1], w.z & keep[i >> 1][2], w.w & keep[i >> 1][3]};
+        uint32_t ws[4] = {w.x & keep[i >> 1][0], w.y & keep[i >> 1][1], w.z & keep[i >> 1][2], w.w & keep[i >> 1][3]};
+        if (decltype(nan_out)::value && no_nan >> (i >> 1) & 1) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ws[k] &= ~nan_bytes(ws[k]);
+        }
         uint32_t o[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -397,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int p = 0; p < 2; ++p)  // an absent page holds whatever the stage held
 #pragma unroll
         for (int k = 0; k < 4; ++k) keep[p][k] = there >> p & 1 ? ~0u : 0u;
-      convert(raw, smem_u32(smem + OFF_K + s * TILE), keep);
+      convert(raw, smem_u32(smem + OFF_K + s * TILE), keep, std::false_type{}, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[s]);
@@ -419,12 +472,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k) keep[p][k] = kv_bytes(see >> (4 * k));
         }
       }
+      uint32_t no_nan = 0;  // bytes of ones where a page's NaN stay in the product
+      if (GROUP) {
+        // A value that is NaN makes NaN of the rows that see its token, and of no other (whose weight
+        // for it is zero, and zero times NaN is NaN): where some row does not, it is taken out
+        // of the product, and its pair noted for the end (nan_seen).
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int key = p ? w.z : w.x, br = p ? w.w : w.y;
+          if (!(there >> p & 1) || (br < 0 && (key >= list.lo_max || key + kKvPage <= list.sinks_min))) continue;
+          no_nan |= 1u << p;
+#pragma unroll
+          for (int i = 2 * p; i < 2 * p + 2; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(raw + 8192 + t * 16 + i * 2048);
+            const uint32_t bad[4] = {nan_bytes(v.x) & keep[p][0], nan_bytes(v.y) & keep[p][1], nan_bytes(v.z) & keep[p][2], nan_bytes(v.w) & keep[p][3]};
+            if (bad[0] | bad[1] | bad[2] | bad[3]) {
+              atomicOr(nan_pairs + j % NN / 32, 1u << j % 32);
+              nan_pairs[NN / 32] = 1;
+            }
+          }
+        }
+      }
       ok = mbar_wait(&v_empty[s], ((j / NS) & 1) ^ 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
-      convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep);
+      if (GROUP && no_nan) convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::bool_constant<GROUP>{}, no_nan);
+      else convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::false_type{}, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -677,6 +752,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = 0; c < 64; ++c) ov[c] = 0.f;
     }
     if (m == -INFINITY && l != 0.f) m = 0.f;  // only NaN scores
+    if (GROUP && done && active) {
+      // the converters' notes: all their pairs are in the operand tiles
+      for (int j = max(0, n - NS); j < n; ++j) mbar_wait(&v_full[j % NS], (j / NS) & 1, abort_flag);
+      if (*reinterpret_cast<volatile uint32_t*>(nan_pairs + NN / 32)) {
+        const uint64_t bad = nan_channels(a, smem, r);
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (bad >> c & 1) ov[c] = NAN;
+      }
+    }
     if (GROUP || a.part) {
       // 256 rows of 64 channels, then their (maximum, sum), for kv_tiles_merge
       float* part = a.part + blockIdx.x * kPartFloats;

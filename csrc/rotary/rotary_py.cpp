@@ -69,6 +69,7 @@ void check_rotation(const Rotation& r, const Tensor& x0) {
     const auto& p = *r.positions;
     TORCH_CHECK_VALUE(r.offset == 0, "positions and offset exclude each other");
     TORCH_CHECK_VALUE(p.scalar_type() == torch::kInt || p.scalar_type() == torch::kLong, "positions must be int32 or int64, got ", p.scalar_type());
+    TORCH_CHECK_VALUE(tab.size(0) > 0 || p.numel() == 0, "the table has no positions");
     TORCH_CHECK_VALUE(p.device() == x.device(), "positions are on ", p.device(), ", the heads on ", x.device());
     TORCH_CHECK_VALUE((p.dim() == 1 && p.size(0) == x.size(1)) ||
                           (p.dim() == 2 && x0.dim() == 4 && (p.size(0) == x.size(0) || p.size(0) == 1) && p.size(1) == x.size(1)),

@@ -104,6 +104,8 @@ def _rows(x, table, positions, offset, layout):
         raise ValueError("positions and offset exclude each other")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if table.shape[0] == 0 and positions.numel():
+        raise ValueError("the table has no positions")
     if positions.device != x.device:
         raise ValueError(f"positions are on {positions.device}, the heads on {x.device}")
     if not (positions.shape == (T,) or (x.dim() == 4 and positions.dim() == 2 and positions.shape[0] in (1, x.shape[0])

@@ -197,6 +197,46 @@ def test_nan_stays_in_its_rows():
     assert torch.equal(o, want)
 
 
+@pytest.mark.parametrize("what", ["own", "past"])
+def test_nan_values_reach_only_rows_that_see_them(what, mode):
+    """A value that is NaN, in one branch's own tokens or in shared ones that only some branches' windows
+    still hold: NaN in its channel of the rows that see it, the others as without it."""
+    for T, G, ctx, more in ((1, 1, 1400, [0, 300, 70]), (3, 2, 700, [0, 200, 64]), (40, 1, 900, [10, 400, 130])):
+        if T > 1 and not mode:  # (one sequence's rows alone share what any of them sees)
+            continue
+        c = _cache(1, 2, 80)
+        seqs = _branches(c, [ctx], 3, more)
+        step = c.begin(seqs, T, branches=3)
+        step.write(0, *(_randn(3, T, 2, 64) for _ in "kv"))
+        q = _randn(3, T, 2 * G, 64)
+        window = 500
+        args = dict(causal="token", window=window, sinks=0)
+        clean = step.attend(0, q, **args)
+        assert torch.isfinite(clean).all()
+        # (sequence, position, head, channel) of a few values
+        lens = [c.length(s) for s in seqs]
+        if what == "own":
+            at = [(1, lens[1] - 1, 0, 5), (1, lens[1] + T - 1, 1, 63), (2, lens[2], 0, 17)]
+        else:
+            at = [(0, lens[0] - window + 2, 0, 9), (0, lens[2] - window + 3, 1, 33), (0, lens[0] - 65, 1, 2)]
+            at = [(i, p, h, ch) for i, p, h, ch in at if p < ctx // 64 * 64]
+        saw = torch.zeros_like(clean, dtype=torch.bool)
+        for i, pos, h, ch in at:
+            page = int(step.table[i, pos // 64])
+            c.v.view(torch.uint8)[0, page, h, ch, pos % 64] = 0x7f
+            for j in range(3):
+                if what == "own" and j != i:
+                    continue
+                for t in range(T):
+                    if lens[j] + t - window < pos <= lens[j] + t:
+                        saw[j, t, h * G:(h + 1) * G, ch] = True
+        assert saw.any() and not saw.flatten(1).any(1).all() or what == "past"
+        got = step.attend(0, q, **args)
+        assert torch.equal(torch.isnan(got), saw)
+        assert torch.equal(got[~saw], clean[~saw])
+        assert torch.equal(torch.isnan(step.attend(0, q, **args)), saw)
+
+
 def test_run_of_branches(mode):
     """A run as a user makes it, over two layers, with query and key norms and positions: the
     same with the groups named as without."""

@@ -119,6 +119,7 @@ def refusals(dev):
         ("positions' shape", lambda: rotary(x, tab, torch.arange(5, device=dev))),
         ("positions' batch", lambda: rotary(x, tab, torch.zeros(3, 4, dtype=torch.long, device=dev))),
         ("positions of packed heads", lambda: rotary(x[0], tab, torch.zeros(1, 4, dtype=torch.long, device=dev))),
+        ("empty table", lambda: rotary(x, tab[:0], torch.zeros(4, dtype=torch.long, device=dev))),
         ("in place of a leaf", lambda: rotary(leaf, tab, inplace=True)),
         ("tokens differ", lambda: qk_norm_rotary(q, k[:, :3], table=tab)), ("heads' sizes differ", lambda: qk_norm_rotary(q, k[..., :8])),
         ("types differ", lambda: qk_norm_rotary(q, k.bfloat16())), ("eps", lambda: qk_norm_rotary(q, k, eps=0.0)),
@@ -129,10 +130,10 @@ def refusals(dev):
     ]
 
 
-@pytest.mark.parametrize("i", range(29))
+@pytest.mark.parametrize("i", range(30))
 def test_refusals(i):
     cases = refusals("cpu")
-    assert len(cases) == 29
+    assert len(cases) == 30
     what, call = cases[i]
     with pytest.raises(ValueError):
         call()
