@@ -294,42 +294,38 @@ __global__ void __launch_bounds__(kThreads, 2) rot_wide(const Launch L) {
   const float inv_D = 1.f / static_cast<float>(a.D);
   const uint32_t cta = blockIdx.x - (which ? L.ctas0 : 0), step = (which ? L.ctas1 : L.ctas0) * per;
   const uint32_t mine = smem_u32(ring + threadIdx.x);
-  auto fetch = [&](const Item& it, int stage) {
-    const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
-    uint32_t dst = mine + stage * (kStage * 16);
+  auto fetch = [&](uint32_t i0, int stage) {
+    if (i0 < n) {
+      const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
+      const T* px = reinterpret_cast<const T*>(t.x) + it.b * t.x_sb + it.t * t.x_st;
+      uint32_t dst = mine + stage * (kStage * 16);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = it.h + u * blocks;
-      const bool have = it.there && active && h < t.H;
-      const T* p = px + h * t.x_sh;
+      for (int u = 0; u < U; ++u) {
+        const int h = it.h + u * blocks;
+        const bool have = it.there && active && h < t.H;
+        const T* p = px + h * t.x_sh;
 #pragma unroll
-      for (int i = 0; i < C; ++i, dst += kThreads * 16)
-        copy16(dst, have ? p + (i < C / 2 ? in.c0 : in.c1) + (i % (C / 2)) * (16 / sizeof(T)) : t.x, have);
-    }
-    if (rot && it.there) {
-      const float2* tab = a.table + static_cast<long>(max(it.row, 0)) * (a.R / 2);
+        for (int i = 0; i < C; ++i, dst += kThreads * 16)
+          copy16(dst, have ? p + (i < C / 2 ? in.c0 : in.c1) + (i % (C / 2)) * (16 / sizeof(T)) : t.x, have);
+      }
+      if (rot && it.there) {
+        const float2* tab = a.table + static_cast<long>(max(it.row, 0)) * (a.R / 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i, dst += kThreads * 16) copy16(dst, tab + (i < 2 ? p0 : p1) + 2 * (i & 1), true);
+        for (int i = 0; i < 4; ++i, dst += kThreads * 16) copy16(dst, tab + (i < 2 ? p0 : p1) + 2 * (i & 1), true);
+      }
     }
     copies_end();
   };
-  // this turn's, those whose copies are on their way, and the one whose position is
   uint32_t i0 = cta * per;
-  Item turns[S];
 #pragma unroll
-  for (int k = 0; k < S; ++k) turns[k] = item_of(L, which, i0 + k * step + (threadIdx.x >> lg), n);
-#pragma unroll
-  for (int k = 0; k < S - 1; ++k) fetch(turns[k], k);
+  for (int k = 0; k < S - 1; ++k) fetch(i0 + k * step, k);
   for (int stage = 0; i0 < n; i0 += step, stage = stage == S - 1 ? 0 : stage + 1) {
-    const Item it = turns[0];
+    const Item it = item_of(L, which, i0 + (threadIdx.x >> lg), n);
     Pairs w;
     if (NORM) w = weights<IN_H>(t.w, in, active);
     copies_wait<S - 2>();
     __syncwarp();  // every lane has read what another one may write (a result in the place of its input)
-    fetch(turns[S - 1], stage == 0 ? S - 1 : stage - 1);
-#pragma unroll
-    for (int k = 0; k < S - 1; ++k) turns[k] = turns[k + 1];
-    turns[S - 1] = item_of(L, which, i0 + S * step + (threadIdx.x >> lg), n);
+    fetch(i0 + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
     const uint4* got = ring + stage * kStage + threadIdx.x;
     Angles ang;
     if (rot && it.there) {
