@@ -14,11 +14,11 @@
 // 16x8x16 instruction), two numbers to an fp32 instruction. The keys of the warp's next two
 // pages and the values of its next one are on their way while it works: 16 warps with
 // two whole pages each do not fit the shared memory.
-// Measured: 64 branches of 16,384 tokens, up to 700 of their own, 16 heads: 48 us and 6 for the sum
-// (each for itself 275), 855 instructions a page, 2 a cycle: issue and latency of 16 warps, DRAM
-// at 0.27 of a copy's rate. Eight branches of 200 frames of 64 tokens, 12 heads, in 256-row blocks: 56 us
-// and 10 (131). A launch of its own for the sequences' own pages: 54 and 63 us in all for these
-// two, where a list of both kinds takes 49 and 53.
+// Measured: 64 branches of 16,384 tokens, up to 700 of their own, 16 heads: 50 us and 6.6 for the sum
+// (each for itself 275), about 860 instructions a page, 2 a cycle: issue and latency of 16 warps,
+// DRAM at 0.26 of a copy's rate. Eight branches of 200 frames of 64 tokens, 12 heads, in 256-row
+// blocks: 60 us and 11 (131). A launch of its own for the sequences' own pages took 54 and 63 us in
+// all for these two, where a list of both kinds took 49 and 53 (51 and 57 since NaN are kept apart).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -524,7 +524,7 @@ constexpr int kBlockRows = 256;  // of attend_tiles.cu
 }  // namespace
 
 // Estimates from measured calls (cold caches): few rows 8 us and 2.6 or 3.3 us for a page of each warp
-// (8 rows: 15,000 pages on 144 CTAs 26 us; 16: 22,700 on 128 48 us), blocks of 256 as in
+// (8 rows: 15,000 pages on 144 CTAs 26 us; 16: 22,700 on 128 50 us), blocks of 256 as in
 // kv_attend_tiles_plan, the second launch 4 us and 0.2 us a part of a row.
 KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
   const long rows = kv_group_rows(a), TG = a.T * static_cast<long>(a.H / a.pool.heads), sms = num_sms(dev);

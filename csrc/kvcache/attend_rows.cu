@@ -483,7 +483,7 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
   }
   // Groups that share pages: together where that is estimated faster. (8-row tiles take 0.65 of their
   // estimate where pages are many: 128 on 60,000 tokens 155 us, 192 on 8,000 32 us. Eight branches of 1,500
-  // tokens 7.5 us alone and 10 together, 64 of 16,384 275 and 50; of 64 rows over 12,800 tokens 136 and 57.)
+  // tokens 7.5 us alone and 10 together, 64 of 16,384 275 and 51; of 64 rows over 12,800 tokens 131 and 57.)
   const int mode = g_branch_mode.load(std::memory_order_relaxed);
   if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows && mode != 1) {
     const KvPlan group = kv_attend_branches_plan(a, mode, dev);

@@ -12,10 +12,10 @@
 // them. Heads whose sizes, strides or bases do not allow that (rot_any) go through shared memory.
 // Everything is fp32 inside and rounded once; the plain rotation without contraction of a c - b s
 // (the same bits as the PyTorch statement).
-// Measured (cold caches): rotation of 32,768 tokens of 8 heads of 128, half of each, 22.7 us for
-// 139 MB, 0.93 of a plain copy's rate. Norms and rotation of 16,384 tokens of 24 heads of 64 (101
-// MB) 23.5 us, 0.65 of it: instruction issue and the latency of 16 warps an SM; backward (151 MB)
-// 37.6 us, 0.61, and 5 us for the weights' gradients. 3,009 tokens of 5 heads of 72, fp32: 7.8 us.
+// Measured (cold caches): rotation of 32,768 tokens of 8 heads of 128, half of each, 23 us for
+// 139 MB, 0.92 of a plain copy's rate. Norms and rotation of 16,384 tokens of 24 heads of 64 (101
+// MB) 23.7 us, 0.65 of it: instruction issue and the latency of 16 warps an SM; backward (151 MB)
+// 38 us, 0.61, and 5.4 us for the weights' gradients. 3,009 tokens of 5 heads of 72, fp32: 8.1 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
