@@ -145,13 +145,24 @@ def rope_table(angles: torch.Tensor) -> torch.Tensor:
     return torch.stack([angles.cos(), angles.sin()], -1).float().contiguous()
 
 
+def _kernel_takes(x: torch.Tensor, table: torch.Tensor, T: int, D: int) -> bool:
+    """Whether :func:`drivedit_b200.ops.rotary.rotary` takes the call: plain tensors in the types and shapes it
+    has, outside function transforms, forward-mode derivatives and compilation (which the PyTorch
+    statement goes through), and not a leaf (whose captured calls it may refuse)."""
+    return (type(x) in (torch.Tensor, nn.Parameter) and type(table) in (torch.Tensor, nn.Parameter)
+            and x.dim() in (3, 4) and D <= 256 and D % 2 == 0 and table.shape[0] >= T and table.shape[1:] == (D // 2, 2)
+            and x.dtype in (torch.bfloat16, torch.float16, torch.float32) and table.dtype == torch.float32
+            and table.device == x.device and table.is_contiguous() and not table.requires_grad
+            and not (x.requires_grad and x.is_leaf) and x.numel() // max(D, 1) < 1 << 30
+            and torch._C._functorch.peek_interpreter_stack() is None and not torch.compiler.is_compiling()
+            and torch.autograd.forward_ad._current_level < 0)
+
+
 def apply_rope(x: torch.Tensor, table: torch.Tensor, inverse: bool = False) -> torch.Tensor:
     """Rotate channel pairs ``(2i, 2i+1)`` of ``x [..., T, H, D]`` with ``table
     [T, D/2, 2]``; ``inverse`` rotates by the negative angle (the backward pass)."""
     T, H, D = x.shape[-3:]
-    if (x.is_cuda and x.dim() in (3, 4) and D <= 256 and table.shape[0] >= T and table.shape[1:] == (D // 2, 2)
-            and x.dtype in (torch.bfloat16, torch.float16, torch.float32) and table.dtype == torch.float32
-            and table.device == x.device and table.is_contiguous() and not table.requires_grad):
+    if x.is_cuda and _kernel_takes(x, table, T, D):
         from ..ops.rotary import rotary  # one pass, the same bits
 
         return rotary(x, table, inverse=inverse)

@@ -557,3 +557,17 @@ def test_apply_rope_on_cuda_is_the_kernel():
         assert ext().launch_count() == n + 1
         assert torch.equal(y.cpu(), apply_rope(x.cpu(), rope.table(4, 2).cpu()))
         assert torch.equal(apply_rope(x[None], rope.table(4, 2))[0], y)  # more leading axes: the PyTorch form
+    # transforms and forward-mode derivatives go through the PyTorch form, on the CPU as here
+    x, v = torch.randn(2, 24, 3, 64, device="cuda"), torch.randn(2, 24, 3, 64, device="cuda")
+    tab = rope.table(4, 2)
+    _, jvp = torch.func.jvp(lambda x: apply_rope(x, tab), (x,), (v,))
+    assert torch.allclose(jvp, apply_rope(v, tab), atol=1e-6)
+    assert torch.equal(torch.vmap(lambda x: apply_rope(x, tab))(x), apply_rope(x, tab))
+    with torch.autograd.forward_ad.dual_level():
+        dual = apply_rope(torch.autograd.forward_ad.make_dual(x, v), tab)
+        assert torch.allclose(torch.autograd.forward_ad.unpack_dual(dual).tangent, apply_rope(v, tab), atol=1e-6)
+    leaf = x.clone().requires_grad_()
+    g = torch.randn_like(x)
+    a, = torch.autograd.grad(apply_rope(leaf, tab), leaf, g)
+    b, = torch.autograd.grad(apply_rope(leaf * 1, tab), leaf, g)
+    assert torch.equal(a, b)
