@@ -165,6 +165,9 @@ bool share_heads(const Tensor& q, const Tensor& k) {
   return false;
 }
 
+// A tangent of forward-mode derivatives would be lost
+bool has_tangent(const Tensor& x) { return x._fw_grad(/*level=*/0).defined(); }
+
 // What was overwritten no longer is what an autograd graph may have kept of it
 void overwritten(const Tensor& x) {
   if (!x.is_inference()) torch::autograd::impl::bump_version(x);
@@ -217,6 +220,7 @@ Tensor rotary(const Tensor& x, const Tensor& table, const OptTensor& positions, 
   Rotation r{table, positions, offset, layout, inverse};
   check_rotation(r, x);
   r.table = aligned_pairs(r.table);
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(x) && !has_tangent(table), "rotary has no forward-mode derivative on CUDA");
   if (!at::GradMode::is_enabled() || !x.requires_grad()) return rotate(x, r, inplace);
   TORCH_CHECK_VALUE(!inplace, "x requires a gradient: it cannot be rotated in place");
   {
@@ -359,8 +363,10 @@ std::vector<Tensor> qk_norm_rotary(const Tensor& q, const Tensor& k, const OptTe
   Rotation r{table, positions, offset, layout, false};
   check_qk(q, k, wq, wk, r, eps);
   r.table = aligned_pairs(r.table);
-  bool grad = q.requires_grad() || k.requires_grad();
-  for (const auto* w : {&wq, &wk}) grad = grad || (*w && (*w)->requires_grad());
+  bool grad = q.requires_grad() || k.requires_grad(), tangent = has_tangent(q) || has_tangent(k) || (table && has_tangent(*table));
+  for (const auto* w : {&wq, &wk})
+    if (*w) grad = grad || (*w)->requires_grad(), tangent = tangent || has_tangent(**w);
+  TORCH_CHECK_NOT_IMPLEMENTED(!tangent, "qk_norm_rotary has no forward-mode derivative on CUDA");
   if (!at::GradMode::is_enabled() || !grad) return qk_forward(q, k, wq, wk, r, eps, inplace);
   TORCH_CHECK_VALUE(!inplace, "something requires a gradient: q and k cannot be overwritten");
   {

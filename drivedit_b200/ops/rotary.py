@@ -143,10 +143,21 @@ def _writable(inplace, *inputs):
         raise ValueError("something requires a gradient: the inputs cannot be overwritten")
 
 
+def _share(q, k):
+    """Whether some element of ``q`` is one of ``k``."""
+    if not q.numel() or not k.numel() or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
+        return False
+    n = q.untyped_storage().nbytes() // q.element_size()
+    place = torch.arange(n)
+    taken = torch.zeros(n, dtype=torch.bool)
+    taken[place.as_strided(q.shape, q.stride(), q.storage_offset())] = True
+    return bool(taken[place.as_strided(k.shape, k.stride(), k.storage_offset())].any())
+
+
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: Optional[torch.Tensor] = None, offset: int = 0,
            layout: str = "interleaved", inverse: bool = False, inplace: bool = False) -> torch.Tensor:
     """``x [B, T, H, D]`` (or packed ``[T, H, D]``) with its heads rotated; differentiable in ``x``, twice
-    and more. ``inverse`` rotates by the negative angle (and "split" back from halves to side
+    and more (forward-mode derivatives raise on CUDA). ``inverse`` rotates by the negative angle (and "split" back from halves to side
     by side): the backward pass of the call without it."""
     if x.is_cuda:
         if sync_check() and torch.is_grad_enabled() and x.requires_grad and not inplace:
@@ -165,7 +176,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     """Every head of ``q [B, T, H, D]`` and ``k [B, T, KH, D]`` (or packed ``[T, H, D]``) divided by the root
     of its mean square plus ``eps``, times ``q_weight`` / ``k_weight`` ``[D]`` (None: ones), then rotated
     (``table`` None: not at all). One launch for both, differentiable in the heads and weights; the
-    weights' gradients are summed in a fixed order. A second derivative raises on CUDA."""
+    weights' gradients are summed in a fixed order. A second derivative, and a forward-mode one, raise on
+    CUDA."""
     if q.is_cuda:
         if sync_check() and not inplace and torch.is_grad_enabled() and \
                 any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
@@ -183,6 +195,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
             raise ValueError(f"a norm's weight must be floating-point [{q.shape[-1]}] on the heads' device")
     cs = _rows(q, table, positions, offset, layout)
     _writable(inplace, q, k, q_weight, k_weight)
+    if inplace and _share(q, k):
+        raise ValueError("q and k share heads: they cannot be overwritten both")
     out = []
     for x, w in ((q, q_weight), (k, k_weight)):
         h = _wide(x)

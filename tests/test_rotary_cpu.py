@@ -274,3 +274,15 @@ def test_norms_keep_the_gradient_buckets_whole():
     eng.world, eng.rank = 2, 0
     eng.flat = FlatParamGroup(m.flat_layout(m.named_parameters()), "cpu", no_decay=m.no_decay_names(), pad_to=8)
     assert eng._plan_pieces() is not None and eng.bucket_ids == set(range(cfg.model.n_layers))
+
+
+def test_heads_of_both_are_not_overwritten():
+    x = torch.randn(2, 5, 6, 32)
+    before = x.clone()
+    for q, k in ((x, x), (x[:, :, :4], x[:, :, 3:]), (x[..., ::2], x[..., 16:])):
+        with pytest.raises(ValueError, match="share"):
+            qk_norm_rotary(q, k, inplace=True)
+    assert torch.equal(x, before)
+    want = qk_norm_rotary(x[:, :, 0::2], x[:, :, 1::2])
+    got = qk_norm_rotary(x[:, :, 0::2], x[:, :, 1::2], inplace=True)  # in turn, none of both
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

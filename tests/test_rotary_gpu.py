@@ -571,3 +571,17 @@ def test_apply_rope_on_cuda_is_the_kernel():
     a, = torch.autograd.grad(apply_rope(leaf, tab), leaf, g)
     b, = torch.autograd.grad(apply_rope(leaf * 1, tab), leaf, g)
     assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused():
+    from drivedit_b200.ops.rotary import qk_norm_rotary, rotary
+    from torch.autograd import forward_ad as fwd
+
+    tab = torch.randn(4, 8, 2, device="cuda")
+    x, w = torch.randn(1, 4, 2, 16, device="cuda"), torch.ones(16, device="cuda")
+    with fwd.dual_level():
+        dx, dw = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(w, torch.ones_like(w))
+        for call in (lambda: rotary(dx, tab), lambda: qk_norm_rotary(dx, x), lambda: qk_norm_rotary(x, dx), lambda: qk_norm_rotary(x, x, w, dw)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        rotary(x, tab)
