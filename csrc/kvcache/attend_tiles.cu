@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (GROUP) {
         // A value that is NaN makes NaN of the rows that see its token, and of no other (whose weight
         // for it is zero, and zero times NaN is NaN): where some row does not, it is taken out
-        // of the product, and its pair noted for the end (nan_seen).
+        // of the product, and its pair noted for the end (nan_channels).
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int key = p ? w.z : w.x, br = p ? w.w : w.y;

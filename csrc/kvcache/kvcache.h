@@ -80,7 +80,6 @@ struct KvAttendArgs {
   // sequence behind them (set the launch's shape only)
   int shared_pages = 0;
   int own_tokens = 0;
-  bool split = false;    // shared pages apart from the sequences' own (the plan's)
 };
 
 // How a call is launched: the kernel, how many CTAs share a row tile's pages, and the scratch
