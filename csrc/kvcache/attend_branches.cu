@@ -108,6 +108,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
   const int kh = item % a.pool.heads;
   const KvGroup grp(a, item / a.pool.heads);
 
+  grp.prefetch_ids();
+  if (threadIdx.x < R) grp.prefetch_q(r0 + threadIdx.x, kh);
+
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem) + warp * 3;  // [2], then the values'
   uint64_t* v_full = k_full + 2;
   float4* known = reinterpret_cast<float4*>(smem + OFF_PAGES) + warp * 4;  // scales, id, first key
@@ -133,11 +136,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
       qraw[j][1] = ld_global_v4(q + 8);
     }
   }
-  if (threadIdx.x < R) {
-    const KvGroupRow x = grp.row(r0 + threadIdx.x);
-    spans[threadIdx.x] = make_int4(x.span.lo, x.span.hi, x.sinks, x.i - r0 / grp.TG);
+  const int own_row = static_cast<int>(threadIdx.x) - kv_row_thread<R>(0);
+  KvGroupRow of_row{0, 0, 0, {kNoKey, 0}, 0};
+  if (own_row >= 0 && own_row < R) {
+    of_row = grp.row(r0 + own_row);
+    spans[own_row] = make_int4(of_row.span.lo, of_row.span.hi, of_row.sinks, of_row.i - r0 / grp.TG);
   }
-  const KvGroupPages pages = kv_group_pages<R>(grp, r0, table, reinterpret_cast<int*>(smem + OFF_LOW));
+  const KvGroupPages pages = kv_group_pages<R>(grp, r0, of_row, table, reinterpret_cast<int*>(smem + OFF_LOW));
   const int part = rank * kWarps + warp, parts = ranks * kWarps;
   const int mine = pages.n > part ? (pages.n - part + parts - 1) / parts : 0;
 
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
   __syncthreads();
   float* out = a.part + blockIdx.x * kv_part_floats(R);
   for (int i = threadIdx.x; i < R * 16; i += kThreads) {
-    const int r = i >> 4, d = (i & 15) * 4;
+    const int r = i % R, d = i / R * 4;
     float top = -INFINITY, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
         sum += k * ml.y;
       }
     }
-    *reinterpret_cast<float4*>(out + r * 64 + d) = v;
+    *reinterpret_cast<float4*>(out + d * R + r * 4) = v;
     if (d == 0) *reinterpret_cast<float2*>(out + R * 64 + r * 2) = make_float2(top, sum);
   }
 }
@@ -451,9 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
 // Adds up the parts of each row, in the order of the CTAs; 16 threads a row, 4 channels each.
 template <int R>
 __global__ void __launch_bounds__(256) kv_group_merge(const KvAttendArgs a, int row_tiles) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
   constexpr int kOnce = R < 16 ? R : 16;  // rows of a CTA
-  const int lr = blockIdx.x % (R / kOnce) * kOnce + (threadIdx.x >> 4), d = (threadIdx.x & 15) * 4;
+  const int lr = blockIdx.x % (R / kOnce) * kOnce + threadIdx.x % kOnce, d = threadIdx.x / kOnce * 4;
   int item = blockIdx.x / (R / kOnce);
   const float* part = a.part + static_cast<long>(item) * a.ranks * kv_part_floats(R);
   const int r = item % row_tiles * R + lr;
@@ -462,6 +466,7 @@ __global__ void __launch_bounds__(256) kv_group_merge(const KvAttendArgs a, int 
   const KvGroup grp(a, item / a.pool.heads);
   if (r >= grp.rows) return;
   const KvGroupRow x = grp.row(r);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
   float top = -INFINITY, sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (x.span.lo != kNoKey)
@@ -472,7 +477,7 @@ __global__ void __launch_bounds__(256) kv_group_merge(const KvAttendArgs a, int 
     for (int k = 0; k < a.ranks; ++k) {
       const float* p = part + k * kv_part_floats(R);
       const float2 ml = *reinterpret_cast<const float2*>(p + R * 64 + lr * 2);
-      const float4 y = *reinterpret_cast<const float4*>(p + lr * 64 + d);
+      const float4 y = *reinterpret_cast<const float4*>(p + d * R + lr * 4);
       const float w = exp2f(ml.x - top);
       sum += w * ml.y;
       v.x += w * y.x;

@@ -196,27 +196,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (GROUP)
     for (int i = threadIdx.x; i <= NN / 32; i += kThreads) nan_pairs[i] = 0;
 
-  // the block's pages, and this CTA's run of key tiles (page pairs)
-  KvPages pages{0, 0, 0};
-  KvSpan all{0, 0};
-  KvGroupPages list;
   if (GROUP) {
-    list = kv_group_pages<kRows>(grp, r0, table, reinterpret_cast<int*>(smem + OFF_RAW));  // (not yet in use)
-    pages.n = list.n;
-  } else if (r0 < rows) {
-    const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
-    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + kRows) - 1) / G, len, first);
-    all = KvSpan{s0.lo, s1.hi};
-    pages = kv_pages(s0.lo, s1.hi, sinks, a.step.width);
+    grp.prefetch_ids();
+    if (warp >= 8) grp.prefetch_q(r0 + static_cast<int>(threadIdx.x) - 256, kh);
   }
-  const int pairs = (pages.n + 1) / 2, per = (pairs + ranks - 1) / ranks;
-  const int j0 = min(pairs, rank * per);
-  // GROUP: pairs in turn, since those of the sequences' own pages, at the end, take longer
-  const int n = GROUP ? max(0, (pairs - rank + ranks - 1) / ranks) : min(pairs, j0 + per) - j0;
-  auto pair_at = [&](int j) { return GROUP ? rank + j * ranks : j0 + j; };
 
-  if (GROUP && threadIdx.x == 0) *reinterpret_cast<GroupWork*>(smem + OFF_WORK) = GroupWork{list, b, kh, rank, n};
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 64) {
     mbar_init(q_full, 8);
     for (int s = 0; s < NR; ++s) {
       mbar_init(&raw_full[s], 1);
@@ -245,25 +230,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+
+  // the block's pages, and this CTA's run of key tiles (page pairs)
+  KvPages pages{0, 0, 0};
+  KvSpan all{0, 0};
+  KvGroupPages list;
+  if (GROUP) {
+    static_assert(2 * kRows == kThreads, "the softmax threads have a row each");
+    KvGroupRow x{0, 0, 0, {kNoKey, 0}, 0};
+    if (warp >= 8) x = grp.row(r0 + static_cast<int>(threadIdx.x) - kv_row_thread<kRows>(0));
+    list = kv_group_pages<kRows>(grp, r0, x, table, reinterpret_cast<int*>(smem + OFF_RAW));  // (not yet in use)
+    pages.n = list.n;
+  } else if (r0 < rows) {
+    const KvSpan s0 = kv_span(a, old + r0 / G, len, first);
+    const KvSpan s1 = kv_span(a, old + (min(rows, r0 + kRows) - 1) / G, len, first);
+    all = KvSpan{s0.lo, s1.hi};
+    pages = kv_pages(s0.lo, s1.hi, sinks, a.step.width);
+  }
+  const int pairs = (pages.n + 1) / 2, per = (pairs + ranks - 1) / ranks;
+  const int j0 = min(pairs, rank * per);
+  // GROUP: pairs in turn, since those of the sequences' own pages, at the end, take longer
+  const int n = GROUP ? max(0, (pairs - rank + ranks - 1) / ranks) : min(pairs, j0 + per) - j0;
+  auto pair_at = [&](int j) { return GROUP ? rank + j * ranks : j0 + j; };
+
+  if (GROUP && threadIdx.x == 0) *reinterpret_cast<GroupWork*>(smem + OFF_WORK) = GroupWork{list, b, kh, rank, n};
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  {
-    int most = 0;
-    for (int k = threadIdx.x; k < 2 * n; k += kThreads) {
-      const int i = 2 * pair_at(k >> 1) + (k & 1);
-      if (i >= pages.n) break;
-      int id, page, branch;
-      if (GROUP) list.at(grp, table, i, page, branch, id);
-      else id = row[kKvInfo + pages.at(i)];
-      if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages))
-        most = max(most, __float_as_int(a.pool.k_scale[static_cast<long>(id) * a.pool.heads + kh]));
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0 && most) atomicMax(k_most, most);
-  }
-  __syncthreads();
 
   // Registers by role: 56 + 72 + 2 * 192 = 512 = 4 * 128, the launch's own. All go back to 128
   // before the common end; none may before every role has its share (registers_split),
@@ -302,8 +296,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int l0 = 2 * (j & 15), s = j % NR;
         const int id0 = __shfl_sync(0xffffffffu, ids, l0), id1 = __shfl_sync(0xffffffffu, ids, l0 + 1);
-        const float4 f = make_float4(__shfl_sync(0xffffffffu, ks, l0), __shfl_sync(0xffffffffu, ks, l0 + 1),
-                                     __shfl_sync(0xffffffffu, vs, l0), __shfl_sync(0xffffffffu, vs, l0 + 1));
         int4 w = make_int4(0, 0, 0, 0);
         if (GROUP)
           w = make_int4(__shfl_sync(0xffffffffu, key, l0), __shfl_sync(0xffffffffu, branch, l0), __shfl_sync(0xffffffffu, key, l0 + 1),
@@ -313,10 +305,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           if (GROUP) where[j % NF] = where[NF + s] = w;
           uint8_t* dst = smem + OFF_RAW + s * TILE;
-          // The softmax has read the factors NF pairs back: codes 3 pairs back have been converted,
-          // so the scores of the pair 6 back are made, and those before it read.
-          factor[j % NF] = make_float4(f.x, f.y, log2_of_power(f.z), log2_of_power(f.w));
-          mbar_arrive(&f_full[j % NF]);
           meta[s] = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
           mbar_arrive_expect_tx(&raw_full[s], (id0 >= 0 ? 8192 : 0) + (id1 >= 0 ? 8192 : 0));
           const int id[2] = {id0, id1};
@@ -329,6 +317,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         ++issued;
+        // behind the copies, which do not wait for the scales
+        const float4 f = make_float4(__shfl_sync(0xffffffffu, ks, l0), __shfl_sync(0xffffffffu, ks, l0 + 1),
+                                     __shfl_sync(0xffffffffu, vs, l0), __shfl_sync(0xffffffffu, vs, l0 + 1));
+        if (lane == 0) {
+          // The softmax has read the factors NF pairs back: codes 3 pairs back have been converted,
+          // so the scores of the pair 6 back are made, and those before it read.
+          factor[j % NF] = make_float4(f.x, f.y, log2_of_power(f.z), log2_of_power(f.w));
+          mbar_arrive(&f_full[j % NF]);
+        }
         __syncwarp();
       }
       if (lane == 0) {
@@ -562,11 +559,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_shared_v4(dst + ((i ^ (lr & 7)) << 4), h[0], h[1], h[2], h[3]);
       }
       sl2 = a.scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
-      // |S| < 2^30, 64 products of numbers up to 2^15 and 448; zero for a row of zeros (padding)
-      bound = amax > 0.f ? sl2 * 0x1p30f * __int_as_float(*k_most) : 0.f;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
+      int most = 0;
+      for (int k = threadIdx.x - 256; k < 2 * n; k += 256) {
+        const int i = 2 * pair_at(k >> 1) + (k & 1);
+        if (i >= pages.n) break;
+        int id, page, branch;
+        if (GROUP) list.at(grp, table, i, page, branch, id);
+        else id = row[kKvInfo + pages.at(i)];
+        if (static_cast<unsigned>(id) < static_cast<unsigned>(a.pool.pages))
+          most = max(most, __float_as_int(a.pool.k_scale[static_cast<long>(id) * a.pool.heads + kh]));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0 && most) atomicMax(k_most, most);
+      asm volatile("bar.sync 2, 256;" ::: "memory");  // the softmax warps
+      // |S| < 2^30, 64 products of numbers up to 2^15 and 448; zero for a row of zeros (padding)
+      bound = amax > 0.f ? sl2 * 0x1p30f * __int_as_float(*const_cast<volatile int*>(k_most)) : 0.f;
     }
     // The weights of the sum are relative to 2^m; those of the product, times their page's value
     // scale, to 2^(m + d).
@@ -766,10 +776,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // 256 rows of 64 channels, then their (maximum, sum), for kv_tiles_merge
       float* part = a.part + blockIdx.x * kPartFloats;
       if (r < (GROUP ? rows : a.T * G)) {
-        float* o = part + (t * 128 + lr) * 64;
+        float* o = part + (t * 128 + lr) * 4;  // by 4 channels, then rows: a warp's stores are in a row
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          *reinterpret_cast<float4*>(o + 4 * c) = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
+          *reinterpret_cast<float4*>(o + c * kRows * 4) = make_float4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
         *reinterpret_cast<float2*>(part + kRows * 64 + (t * 128 + lr) * 2) = make_float2(r < rows ? m : -INFINITY, l);
       }
     } else if (ranks > 1) {
@@ -838,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Adds up the CTAs' results of each row, in rank order; 16 threads a row, 4 channels each.
 __global__ void __launch_bounds__(256) kv_tiles_merge(const KvAttendArgs a, int row_tiles) {
   const int G = a.H / a.pool.heads;
-  const int lr = (blockIdx.x % (kRows / 16)) * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  const int lr = (blockIdx.x % (kRows / 16)) * 16 + (threadIdx.x & 15), c = threadIdx.x >> 4;
   int item = blockIdx.x / (kRows / 16);
   const float* part = a.part + static_cast<long>(item) * a.ranks * kPartFloats;
   const int r = (row_tiles - 1 - item % row_tiles) * kRows + lr;  // the other kernel's order
@@ -851,7 +861,7 @@ __global__ void __launch_bounds__(256) kv_tiles_merge(const KvAttendArgs a, int 
   if (top != -INFINITY)
     for (int k = 0; k < a.ranks; ++k) {
       const float2 x = *reinterpret_cast<const float2*>(part + k * kPartFloats + kRows * 64 + lr * 2);
-      const float4 y = *reinterpret_cast<const float4*>(part + k * kPartFloats + lr * 64 + c * 4);
+      const float4 y = *reinterpret_cast<const float4*>(part + k * kPartFloats + (c * kRows + lr) * 4);
       const float w = exp2f(x.x - top);
       sum += w * x.y;
       v.x += w * y.x;

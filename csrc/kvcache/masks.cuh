@@ -80,6 +80,15 @@ struct KvGroup {
     shared = a.step.rows + static_cast<long>(a.step.B + grp) * a.step.ld;
     P = group >= 0 ? min(max(shared[0], 0), a.step.width) : 0;  // (-1: no group)
   }
+  // What a launch reads first, ahead of what says which of it: the ids of the shared pages, and rows of q
+  __device__ __forceinline__ void prefetch_ids() const {
+    for (int i = threadIdx.x * 32; i < a.step.ld; i += blockDim.x * 32) prefetch_l2(shared + i);
+  }
+  __device__ __forceinline__ void prefetch_q(int r, int kh) const {
+    const int i = r / TG, t = (r - i * TG) / G;
+    if (r < rows)
+      prefetch_l2(reinterpret_cast<const __nv_bfloat16*>(a.q) + seq(i) * a.q_sb + t * a.q_st + (kh * G + r - i * TG - t * G) * a.q_sh);
+  }
   __device__ __forceinline__ int seq(int i) const { return grp * a.step.branches + i; }
   __device__ __forceinline__ const int* seq_row(int i) const { return a.step.rows + static_cast<long>(seq(i)) * a.step.ld; }
   // rows behind the last, and tokens behind a sequence's own, see nothing
@@ -122,10 +131,13 @@ struct KvGroupPages {
     id = g.seq_row(first + b)[kKvInfo + page];
   }
 };
-// The list of the block of R <= 256 rows from r0 on. All threads of the CTA (at least R), which meet
-// in it; `table` and `low` (4 words a warp) are shared memory.
+// The list of the block of R <= 256 rows from r0 on. All threads of the CTA, which meet in it; one from
+// kv_row_thread<R>(0) on for each row, with that row in `mine` (the others: a row that sees nothing),
+// beside those that see to the sequences. `table` and `low` (4 words a warp) are shared memory.
 template <int R>
-__device__ __forceinline__ KvGroupPages kv_group_pages(const KvGroup& g, int r0, KvBranch* table, int* low) {
+__device__ __forceinline__ int kv_row_thread(int row) { return (R + 31) / 32 * 32 + row; }
+template <int R>
+__device__ __forceinline__ KvGroupPages kv_group_pages(const KvGroup& g, int r0, const KvGroupRow& mine, KvBranch* table, int* low) {
   KvGroupPages p;
   const int last = min(g.rows, r0 + R) - 1;
   p.first = r0 / g.TG;
@@ -133,23 +145,23 @@ __device__ __forceinline__ KvGroupPages kv_group_pages(const KvGroup& g, int r0,
   const int b = threadIdx.x, lane = threadIdx.x & 31;
   if (b < p.count) {
     KvBranch x{kNoKey, 0, 0, 0};
-    const int i = p.first + b;
-    const int t0 = (max(r0, i * g.TG) - i * g.TG) / g.G, t1 = min((min(last, (i + 1) * g.TG - 1) - i * g.TG) / g.G, min(g.seq_row(i)[1], g.a.T) - 1);
+    const int i = p.first + b, base = i * g.TG;
+    const int* s = g.seq_row(i);
+    const int len = s[0], own = s[1], first = s[2], sinks = s[3] >= 0 ? s[3] : g.a.sinks;
+    const int t0 = (max(r0, base) - base) / g.G, t1 = min((min(last, base + g.TG - 1) - base) / g.G, min(own, g.a.T) - 1);
     if (t0 <= t1) {
-      const KvGroupRow a = g.row(i * g.TG + t0 * g.G), z = g.row(i * g.TG + t1 * g.G);
-      x = KvBranch{a.span.lo, z.span.hi, a.sinks, kv_pages_from(kv_pages(a.span.lo, z.span.hi, a.sinks, g.a.step.width), g.P).n};
+      const int lo = kv_span(g.a, len - own + t0, len, first).lo, hi = kv_span(g.a, len - own + t1, len, first).hi;
+      x = KvBranch{lo, hi, sinks, kv_pages_from(kv_pages(lo, hi, sinks, g.a.step.width), g.P).n};
     }
     table[b] = x;
   }
   constexpr int kUsed = (R + 31) / 32;  // warps with rows
-  if (threadIdx.x < kUsed * 32) {
-    KvGroupRow x{0, 0, 0, {kNoKey, 0}, 0};
-    if (b < R) x = g.row(r0 + b);
-    const bool sees = x.span.lo != kNoKey;
-    const int v[4] = {__reduce_min_sync(0xffffffffu, x.span.lo), __reduce_max_sync(0xffffffffu, sees ? x.span.lo : 0),
-                      __reduce_min_sync(0xffffffffu, sees ? x.sinks : kNoKey), __reduce_max_sync(0xffffffffu, x.sinks)};
+  if (threadIdx.x >= kUsed * 32 && threadIdx.x < 2 * kUsed * 32) {
+    const bool sees = mine.span.lo != kNoKey;
+    const int v[4] = {__reduce_min_sync(0xffffffffu, mine.span.lo), __reduce_max_sync(0xffffffffu, sees ? mine.span.lo : 0),
+                      __reduce_min_sync(0xffffffffu, sees ? mine.sinks : kNoKey), __reduce_max_sync(0xffffffffu, mine.sinks)};
     if (lane == 0)
-      for (int k = 0; k < 4; ++k) low[(threadIdx.x >> 5) * 4 + k] = v[k];
+      for (int k = 0; k < 4; ++k) low[((threadIdx.x >> 5) - kUsed) * 4 + k] = v[k];
   }
   __syncthreads();
   p.lo_min = low[0], p.lo_max = low[1], p.sinks_min = low[2], p.sinks_max = low[3];
