@@ -528,9 +528,9 @@ constexpr int kBlockRows = 256;  // of attend_tiles.cu
 
 }  // namespace
 
-// Estimates from measured calls (cold caches): few rows 8 us and 2.6 or 3.3 us for a page of each warp
-// (8 rows: 15,000 pages on 144 CTAs 26 us; 16: 22,700 on 128 50 us), blocks of 256 as in
-// kv_attend_tiles_plan, the second launch 4 us and 0.2 us a part of a row.
+// Estimates from measured calls (cold caches): 8 rows 6 us and 3.3 us for a page of each warp (those of
+// one page wait for it; seven pages 37 us with the second launch), 16 rows 8 and 2.8 us (5 pages 27, 14
+// pages 50), blocks of 256 as in kv_attend_tiles_plan, the second launch 4 us and 0.2 us a part of a row.
 KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
   const long rows = kv_group_rows(a), TG = a.T * static_cast<long>(a.H / a.pool.heads), sms = num_sms(dev);
   const long shared = std::min<long>(a.shared_pages, kv_seen_pages(a)), own = (a.own_tokens + kKvPage - 1) / kKvPage;
@@ -541,7 +541,7 @@ KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
     const long pages = shared + seqs * own, units = R == kBlockRows ? (pages + 1) / 2 : (pages + kWarps - 1) / kWarps;
     for (long s = 1; s <= 32 && (s == 1 || (blocks * s <= 4 * sms && units >= s)); ++s) {
       const long each = (units + s - 1) / s;
-      const double one = R == kBlockRows ? 15. + (rows > 128 ? 1.75 : 1.3) * each : 8. + (R == 8 ? 2.6 : 3.3) * each;
+      const double one = R == kBlockRows ? 15. + (rows > 128 ? 1.75 : 1.3) * each : R == 8 ? 6. + 3.3 * each : 8. + 2.8 * each;
       const double us = static_cast<double>((blocks * s + sms - 1) / sms) * one + 4. + 0.2 * s;
       if (best.rows && us >= best.us) continue;
       best.branches = true;

@@ -420,6 +420,14 @@ KvPlan rows_plan(const KvAttendArgs& a, int NT, int dev) {
   return p;
 }
 
+// A closer estimate for 8-row tiles, from 20 measured shapes (8 to 275 us, most within 10 %): three CTAs of
+// an SM slow one another, and waves that are not full even out.
+double narrow_us(const KvAttendArgs& a, int ranks, int dev) {
+  const long sms = num_sms(dev), ctas = static_cast<long>(a.step.B) * a.pool.heads * ranks;
+  const int each = (kv_seen_pages(a) + ranks * kGroups - 1) / (ranks * kGroups);
+  return std::max(1., ctas / (3. * sms)) * (6. + (ctas > 2 * sms ? 1.8 : 1.35) * each);
+}
+
 template <int NT>
 void launch(KvAttendArgs a, int ranks, int dev, cudaStream_t stream) {
   static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
@@ -481,13 +489,13 @@ KvPlan kv_cache_attend_plan(const KvAttendArgs& a) {
     const KvPlan many = kv_attend_tiles_plan(a, dev);
     if (rows > kMaxRows || many.us < few.us) alone = many;
   }
-  // Groups that share pages: together where that is estimated faster. (8-row tiles take 0.65 of their
-  // estimate where pages are many: 128 on 60,000 tokens 155 us, 192 on 8,000 32 us. Eight branches of 1,500
-  // tokens 7.5 us alone and 10 together, 64 of 16,384 275 and 51; of 64 rows over 12,800 tokens 131 and 57.)
+  // Groups that share pages: together where that is estimated faster. (Eight branches of 1,500 tokens
+  // 10.3 us alone and 12.6 together, 16 heads of 4,000 18.4 and 14.3, 64 of 16,384 275 and 50; 48 of 8 rows over
+  // 12,000 28.6 and 26.6; 16 of 8 rows 16.4 and 20.5; eight of 64 rows over 12,800 130 and 56.)
   const int mode = g_branch_mode.load(std::memory_order_relaxed);
   if (a.step.branches > 1 && a.shared_pages > 0 && rows <= kMaxRows && mode != 1) {
     const KvPlan group = kv_attend_branches_plan(a, mode, dev);
-    const bool faster = group.us < alone.us * (!alone.blocks && rows <= 8 ? 0.65 : 1.);
+    const bool faster = group.us < (!alone.blocks && rows <= 8 ? narrow_us(a, few.ranks, dev) : alone.us);
     if (mode || (faster && group.scratch <= kMaxScratch)) return group;
   }
   return alone;
