@@ -20,9 +20,10 @@ inline int kv_seen_pages(const KvAttendArgs& a) {
 }
 
 // attend_branches.cu: groups of branches. A block of rows (of all the group's sequences) walks the
-// pages that the group shares, then each of its sequences' own. What a CTA finds goes into a.part:
-// of block i (heads before groups) and CTA k of a.ranks, [i][k]: unnormalised outputs [16][row][4] (of 4
-// channels each), then (maximum, sum) [row]; a second launch adds it up.
+// pages that the group shares, then each of its sequences' own. What a CTA finds goes into a.part
+// (or to the CTAs of its cluster where that is null): of block i (heads before groups) and CTA k of
+// a.ranks, [i][k]: unnormalised outputs [16][row][4] (of 4 channels each), then (maximum, sum) [row];
+// a second launch adds it up.
 constexpr long kv_part_floats(int rows) { return rows * 66L; }
 inline long kv_group_rows(const KvAttendArgs& a) { return a.step.branches * static_cast<long>(a.T) * (a.H / a.pool.heads); }
 // row blocks of all groups and heads

@@ -4,8 +4,8 @@
 // Rows are (sequence of the group, token, query head of the group of heads). A block of rows walks
 // a list of pages: the shared ones that some row sees, then its sequences' own, each of which
 // the others' rows do not see. Blocks of 8 or 16 rows (here) where there are few, of 256
-// (attend_tiles.cu) where there are many; CTAs that share a block's pages leave their part of
-// each row in scratch, and a second launch adds the parts up, in a fixed order.
+// (attend_tiles.cu) where there are many; CTAs that share a block's pages meet in a cluster, or leave
+// their part of each row in scratch that a second launch adds up, in a fixed order either way.
 //
 // One CTA here = 8 * NJ rows and a share of the block's pages, as 16 warps with pages of their
 // own, each with all the rows: a code is brought to fp16 once for NJ 8-row products, and no
@@ -14,11 +14,14 @@
 // 16x8x16 instruction), two numbers to an fp32 instruction. The keys of the warp's next two
 // pages and the values of its next one are on their way while it works: 16 warps with
 // two whole pages each do not fit the shared memory.
-// Measured: 64 branches of 16,384 tokens, up to 700 of their own, 16 heads: 50 us and 6.6 for the sum
-// (each for itself 275), about 860 instructions a page, 2 a cycle: issue and latency of 16 warps,
+// Measured: 64 branches of 16,384 tokens, up to 700 of their own, 16 heads: 50 us (each for itself
+// 275), about 860 instructions a page, 2 a cycle: issue and latency of 16 warps on 128 of 148 SMs,
 // DRAM at 0.26 of a copy's rate. Eight branches of 200 frames of 64 tokens, 12 heads, in 256-row
-// blocks: 60 us and 11 (131). A launch of its own for the sequences' own pages took 54 and 63 us in
-// all for these two, where a list of both kinds took 49 and 53 (51 and 57 since NaN are kept apart).
+// blocks: 55 us (130). Of a short call 4 us go by before the first page is there (an eighth of it less
+// with the ids and queries brought near before it is known which of them count). A launch of its own for
+// the sequences' own pages took 5 and 10 us more for these two; a sequence's own pages in one half of the
+// 16 rows alone the same time, with more registers than there are; keys and values taking three
+// places in turn 38 us for eight branches of 60,000 tokens that take 36.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -32,6 +35,7 @@ namespace ddb {
 namespace {
 
 constexpr int kWarps = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kThreads = kWarps * 32;
 
 // Of each warp: two places for a page's keys, one for its values, their barriers, and what is known
@@ -47,6 +51,8 @@ constexpr int OFF_RING = (OFF_FLAG + 16 + 127) / 128 * 128;
 constexpr int SMEM_BYTES = OFF_RING + kWarps * kRing;
 static_assert(OFF_PAGES % 16 == 0 && OFF_BRANCH % 16 == 0 && OFF_ROWS % 16 == 0 && OFF_FLAG % 16 == 0, "alignment");
 static_assert(16 * (kPitch * 4 + 8) <= kRing, "a warp's results fit its ring");
+constexpr int OFF_RES = OFF_RING + kWarps * 16 * (kPitch * 4 + 8);  // the CTA's part, for those of its cluster
+static_assert(OFF_RES % 16 == 0 && OFF_RES + 16 * 66 * 4 <= SMEM_BYTES, "behind the warps' results");
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 
 // Which of a lane's sums of a page meet a value that is NaN in a token that their row sees: bit
@@ -92,6 +98,35 @@ __device__ __noinline__ uint32_t nan_sums(uint32_t sv, const int4* spans, int br
   }
   __syncwarp();
   return bad;
+}
+
+// Adds up the CTAs' parts of one row's 4 channels from d on, in the order of the CTAs: most(k) and parts(k, ..) read them
+template <class M, class P>
+__device__ __forceinline__ void join_parts(const KvAttendArgs& a, const KvGroup& grp, const KvGroupRow& x, int kh, int d, M&& most, P&& parts) {
+  float top = -INFINITY, sum = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (x.span.lo != kNoKey)
+#pragma unroll 8
+    for (int k = 0; k < a.ranks; ++k) top = fmaxf(top, most(k));
+  if (top != -INFINITY)
+#pragma unroll 4
+    for (int k = 0; k < a.ranks; ++k) {
+      float2 ml;
+      float4 y;
+      parts(k, ml, y);
+      const float w = exp2f(ml.x - top);
+      sum += w * ml.y;
+      v.x += w * y.x;
+      v.y += w * y.y;
+      v.z += w * y.z;
+      v.w += w * y.w;
+    }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int h = kh * grp.G + x.g;
+  const long b = grp.seq(x.i), at = (b * a.T + x.t) * a.H + h;
+  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64 + d) =
+      make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+  if (a.lse && d == 0) a.lse[(b * a.H + h) * a.T + x.t] = sum == 0.f ? -INFINITY : top + __log2f(sum);
 }
 
 template <int NJ>
@@ -428,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
       if (g == 0) wml[warp * R + r] = make_float2(m[j][u], l[j][u]);
     }
   __syncthreads();
-  float* out = a.part + blockIdx.x * kv_part_floats(R);
+  float* out = a.part ? a.part + blockIdx.x * kv_part_floats(R) : reinterpret_cast<float*>(smem + OFF_RES);
   for (int i = threadIdx.x; i < R * 16; i += kThreads) {
     const int r = i % R, d = i / R * 4;
     float top = -INFINITY, sum = 0.f;
@@ -451,6 +486,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attend_group(const KvAttendArg
     *reinterpret_cast<float4*>(out + d * R + r * 4) = v;
     if (d == 0) *reinterpret_cast<float2*>(out + R * 64 + r * 2) = make_float2(top, sum);
   }
+  if (a.part) return;
+  // ---- each CTA of the cluster adds up its share of the rows
+  cluster_sync_all();
+  const uint32_t res = smem_u32(smem + OFF_RES);
+  for (int i = threadIdx.x; i < R * 16; i += kThreads) {
+    const int r = i % R, d = i / R * 4;
+    if (r % ranks != rank || r0 + r >= grp.rows) continue;
+    join_parts(a, grp, grp.row(r0 + r), kh, d, [&](int k) { return ld_cluster_v2(mapa_shared(res + (R * 64 + r * 2) * 4, k)).x; },
+               [&](int k, float2& ml, float4& y) {
+                 ml = ld_cluster_v2(mapa_shared(res + (R * 64 + r * 2) * 4, k));
+                 y = ld_cluster_v4(mapa_shared(res + (d * R + r * 4) * 4, k));
+               });
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its part
 }
 
 // Adds up the parts of each row, in the order of the CTAs; 16 threads a row, 4 channels each.
@@ -467,44 +516,63 @@ __global__ void __launch_bounds__(256) kv_group_merge(const KvAttendArgs a, int 
   if (r >= grp.rows) return;
   const KvGroupRow x = grp.row(r);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
-  float top = -INFINITY, sum = 0.f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (x.span.lo != kNoKey)
-#pragma unroll 8
-    for (int k = 0; k < a.ranks; ++k) top = fmaxf(top, part[k * kv_part_floats(R) + R * 64 + lr * 2]);
-  if (top != -INFINITY)
-#pragma unroll 4
-    for (int k = 0; k < a.ranks; ++k) {
-      const float* p = part + k * kv_part_floats(R);
-      const float2 ml = *reinterpret_cast<const float2*>(p + R * 64 + lr * 2);
-      const float4 y = *reinterpret_cast<const float4*>(p + d * R + lr * 4);
-      const float w = exp2f(ml.x - top);
-      sum += w * ml.y;
-      v.x += w * y.x;
-      v.y += w * y.y;
-      v.z += w * y.z;
-      v.w += w * y.w;
-    }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int h = kh * grp.G + x.g;
-  const long b = grp.seq(x.i), at = (b * a.T + x.t) * a.H + h;
-  *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.o) + at * 64 + d) =
-      make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-  if (a.lse && d == 0) a.lse[(b * a.H + h) * a.T + x.t] = sum == 0.f ? -INFINITY : top + __log2f(sum);
+  join_parts(a, grp, x, kh, d, [&](int k) { return part[k * kv_part_floats(R) + R * 64 + lr * 2]; },
+             [&](int k, float2& ml, float4& y) {
+               const float* p = part + k * kv_part_floats(R);
+               ml = *reinterpret_cast<const float2*>(p + R * 64 + lr * 2);
+               y = *reinterpret_cast<const float4*>(p + d * R + lr * 4);
+             });
+}
+
+template <int NJ>
+void raise_limit(int dev) {
+  static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+  if (set.load() >> (dev & 63) & 1) return;
+  check_cuda(cudaFuncSetAttribute(kv_attend_group<NJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+             "cudaFuncSetAttribute(kv_attend_group)");
+  set.fetch_or(1ull << (dev & 63));
+}
+
+cudaLaunchConfig_t config(int ranks, cudaLaunchAttribute* attr) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = ranks;
+  attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// How many clusters of `ranks` CTAs run at once (as many of either kernel: one CTA fills an SM)
+int clusters_at_once(int ranks, int dev) {
+  if (ranks == 1) return num_sms(dev);
+  static std::atomic<int> fits[64][kMaxCluster + 1];
+  int n = fits[dev & 63][ranks].load();
+  if (n == 0) {
+    raise_limit<2>(dev);
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = config(ranks, attr);
+    check_cuda(cudaOccupancyMaxActiveClusters(&n, kv_attend_group<2>, &cfg), "cudaOccupancyMaxActiveClusters");
+    n = std::max(n, 1);
+    fits[dev & 63][ranks].store(n);
+  }
+  return n;
 }
 
 template <int NJ>
 void launch(const KvAttendArgs& a, int dev, cudaStream_t stream) {
-  static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
-  if (!(set.load() >> (dev & 63) & 1)) {
-    check_cuda(cudaFuncSetAttribute(kv_attend_group<NJ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
-               "cudaFuncSetAttribute(kv_attend_group)");
-    set.fetch_or(1ull << (dev & 63));
-  }
+  raise_limit<NJ>(dev);
   const long blocks = kv_group_blocks(a, 8 * NJ), tiles = (kv_group_rows(a) + 8 * NJ - 1) / (8 * NJ);
   if (blocks * a.ranks > 0x7fffffffL) throw std::runtime_error("kv_cache_attend: too many rows for one launch");
-  kv_attend_group<NJ><<<static_cast<unsigned>(blocks * a.ranks), kThreads, SMEM_BYTES, stream>>>(a, static_cast<int>(tiles), device_status(dev));
-  check_cuda(cudaGetLastError(), "kv_attend_group launch");
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = config(a.ranks, attr);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * a.ranks));
+  cfg.stream = stream;
+  cfg.numAttrs = a.ranks > 1 && !a.part ? 1 : 0;
+  check_cuda(cudaLaunchKernelEx(&cfg, kv_attend_group<NJ>, a, static_cast<int>(tiles), device_status(dev)), "kv_attend_group launch");
   count_launch();
 }
 
@@ -528,9 +596,10 @@ constexpr int kBlockRows = 256;  // of attend_tiles.cu
 
 }  // namespace
 
-// Estimates from measured calls (cold caches): 8 rows 6 us and 3.3 us for a page of each warp (those of
-// one page wait for it; seven pages 37 us with the second launch), 16 rows 8 and 2.8 us (5 pages 27, 14
-// pages 50), blocks of 256 as in kv_attend_tiles_plan, the second launch 4 us and 0.2 us a part of a row.
+// Estimates from measured calls (cold caches): 8 rows 6 us and 3.3 us for a page of each warp (seven pages
+// 36 us in all), 16 rows 8 and 2.8 us (5 pages 27, 14 pages 50), blocks of 256 as in kv_attend_tiles_plan;
+// the second launch 4 us and 0.2 us a part of a row, meeting in clusters 3 us (64 branches of 4,000
+// tokens, 16 heads, 26.1 and 24.2; 32 of 4 rows over 8,000 twice 26.5 and 24.8).
 KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
   const long rows = kv_group_rows(a), TG = a.T * static_cast<long>(a.H / a.pool.heads), sms = num_sms(dev);
   const long shared = std::min<long>(a.shared_pages, kv_seen_pages(a)), own = (a.own_tokens + kKvPage - 1) / kKvPage;
@@ -542,13 +611,17 @@ KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
     for (long s = 1; s <= 32 && (s == 1 || (blocks * s <= 4 * sms && units >= s)); ++s) {
       const long each = (units + s - 1) / s;
       const double one = R == kBlockRows ? 15. + (rows > 128 ? 1.75 : 1.3) * each : R == 8 ? 6. + 3.3 * each : 8. + 2.8 * each;
-      const double us = static_cast<double>((blocks * s + sms - 1) / sms) * one + 4. + 0.2 * s;
+      const bool cluster = R != kBlockRows && s <= kMaxCluster;
+      const long slots = cluster ? clusters_at_once(static_cast<int>(s), dev) : 0;
+      const double apart = static_cast<double>((blocks * s + sms - 1) / sms) * one + 4. + 0.2 * s;
+      const double met = cluster ? static_cast<double>((blocks + slots - 1) / slots) * one + 3. : apart;
+      const double us = std::min(met, apart);
       if (best.rows && us >= best.us) continue;
       best.branches = true;
       best.blocks = R == kBlockRows;
       best.rows = R;
       best.ranks = static_cast<int>(s);
-      best.scratch = blocks * s * kv_part_floats(R);
+      best.scratch = cluster && met <= apart ? 0 : blocks * s * kv_part_floats(R);
       best.us = us;
     }
   }
@@ -556,17 +629,18 @@ KvPlan kv_attend_branches_plan(const KvAttendArgs& a, int mode, int dev) {
 }
 
 void kv_attend_branches(KvAttendArgs a, const KvPlan& plan, int dev, cudaStream_t stream) {
-  if (!a.part) throw std::runtime_error("kv_cache_attend: no scratch");
+  if (plan.scratch && !a.part) throw std::runtime_error("kv_cache_attend: no scratch");
+  if (!plan.scratch) a.part = nullptr;
   a.ranks = plan.ranks;
   if (plan.blocks) {
     kv_attend_group_tiles(a, dev, stream);
     merge<kBlockRows>(a, stream);
   } else if (plan.rows == 8) {
     launch<1>(a, dev, stream);
-    merge<8>(a, stream);
+    if (a.part) merge<8>(a, stream);
   } else {
     launch<2>(a, dev, stream);
-    merge<16>(a, stream);
+    if (a.part) merge<16>(a, stream);
   }
 }
 
