@@ -410,14 +410,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = threadIdx.x - 128;
     const int r = t >> 2, c = t & 3;  // row of 32, 16-byte piece of it; then rows r + 32 i
     bool ok = true;
-    auto convert = [&](const uint8_t* raw, uint32_t dst, const uint32_t (&keep)[2][4], auto nan_out, uint32_t no_nan) {
+    auto convert = [&](const uint8_t* raw, uint32_t dst, const uint32_t (&keep)[2][4], auto nan_out, uint32_t no_nan) -> uint32_t {
+      uint32_t found = 0;  // NaN of the pages `no_nan`, which become zeros
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 w = *reinterpret_cast<const uint4*>(raw + t * 16 + i * 2048);
         uint32_t ws[4] = {w.x & keep[i >> 1][0], w.y & keep[i >> 1][1], w.z & keep[i >> 1][2], w.w & keep[i >> 1][3]};
         if (decltype(nan_out)::value && no_nan >> (i >> 1) & 1) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) ws[k] &= ~nan_bytes(ws[k]);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t bad = nan_bytes(ws[k]);
+            found |= bad;
+            ws[k] &= ~bad;
+          }
         }
         uint32_t o[8];
 #pragma unroll
@@ -430,6 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_shared_v4(d + (((2 * c) ^ (R & 7)) << 4), o[0], o[1], o[2], o[3]);
         st_shared_v4(d + (((2 * c + 1) ^ (R & 7)) << 4), o[4], o[5], o[6], o[7]);
       }
+      return found;
     };
     for (int j = 0; j < n; ++j) {
       const int sr = j % NR, s = j % NS;
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < 4; ++k) keep[p][k] = kv_bytes(see >> (4 * k));
         }
       }
-      uint32_t no_nan = 0;  // bytes of ones where a page's NaN stay in the product
+      uint32_t no_nan = 0;  // pages whose NaN are taken out
       if (GROUP) {
         // A value that is NaN makes NaN of the rows that see its token, and of no other (whose weight
         // for it is zero, and zero times NaN is NaN): where some row does not, it is taken out
@@ -479,15 +485,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = p ? w.z : w.x, br = p ? w.w : w.y;
           if (!(there >> p & 1) || (br < 0 && (key >= list.lo_max || key + kKvPage <= list.sinks_min))) continue;
           no_nan |= 1u << p;
-#pragma unroll
-          for (int i = 2 * p; i < 2 * p + 2; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(raw + 8192 + t * 16 + i * 2048);
-            const uint32_t bad[4] = {nan_bytes(v.x) & keep[p][0], nan_bytes(v.y) & keep[p][1], nan_bytes(v.z) & keep[p][2], nan_bytes(v.w) & keep[p][3]};
-            if (bad[0] | bad[1] | bad[2] | bad[3]) {
-              atomicOr(nan_pairs + j % NN / 32, 1u << j % 32);
-              nan_pairs[NN / 32] = 1;
-            }
-          }
         }
       }
       ok = mbar_wait(&v_empty[s], ((j / NS) & 1) ^ 1, abort_flag);
@@ -495,8 +492,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = false;
         break;
       }
-      if (GROUP && no_nan) convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::bool_constant<GROUP>{}, no_nan);
-      else convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::false_type{}, 0u);
+      if (GROUP && no_nan) {
+        if (convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::bool_constant<GROUP>{}, no_nan)) {
+          atomicOr(nan_pairs + j % NN / 32, 1u << j % 32);
+          nan_pairs[NN / 32] = 1;
+        }
+      } else convert(raw + 8192, smem_u32(smem + OFF_V + s * TILE), keep, std::false_type{}, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
